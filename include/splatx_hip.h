@@ -697,6 +697,132 @@ int32_t sxh_exec_set_isect_order(sxh_executor* e, int32_t mode);
 #define SXH_ROW_ORDER_SPATIAL 2
 int32_t sxh_exec_set_row_order(sxh_executor* e, int32_t mode);
 
+/* ------------------------------------------------------------------------------------------ */
+/* Learned heads: what trains a small network over [splats, features] rows beside the splats'  */
+/* own parameters. No counterpart in the reference. Unlike the ops above these work on DEVICE  */
+/* buffers of the backend's device, and where the caller wants on its stream:                  */
+/*   q == NULL: on the backend's stream; the caller's own work on the buffers is done before,  */
+/*              and the call returns when the operator's is.                                   */
+/*   else:      enqueued on q->stream (a hipStream_t of the backend's device; NULL: the        */
+/*              device's default stream) after what is there; the call returns at once and     */
+/*              allocates nothing, so that it can be captured into a graph.                    */
+/* Every pointer is checked to be device memory that holds what the operator reads or writes;   */
+/* outputs overlap neither inputs nor each other. Sums and statistics are in 32 bits or more,  */
+/* and a call's results are the same bits on every run.                                        */
+/* ------------------------------------------------------------------------------------------ */
+enum { SXH_TYPE_F32 = 0, SXH_TYPE_BF16 = 1, SXH_TYPE_F16 = 2 };
+
+typedef struct {
+    void* stream;
+} sxh_queue;
+
+/* Layer norm over each row of [rows, width], after the addition of a residual:
+ *   h = x + residual, rounded to `type` (without a residual, h = x), and with the statistics of h's row
+ *   mean = sum(h) / width, rstd = 1 / sqrt(sum((h - mean)^2) / width + eps):
+ *   y = (h - mean) * rstd * weight + bias.
+ * Rows are `*_stride` elements apart (at least width; for inputs also 0: every row the same one). Rows whose
+ * values are not all finite give NaN in their own y only. */
+typedef struct {
+    const void* x;         /* [rows, width] */
+    const void* residual;  /* [rows, width] or NULL */
+    const void* weight;    /* [width], or NULL: 1 */
+    const void* bias;      /* [width], or NULL: 0 */
+    int64_t rows, width;   /* rows may be 0 */
+    int64_t x_stride, residual_stride;
+    float eps;             /* > 0 */
+    uint8_t type;          /* of x, residual, h, y */
+    uint8_t weight_type;   /* of weight and bias: SXH_TYPE_F32, or `type` */
+} sxh_layer_norm_inputs;
+typedef struct {
+    void* y;               /* [rows, width] */
+    void* h;               /* [rows, width]; with a residual only, else NULL */
+    float* mean;           /* [rows], with rstd what the backward reads; both may be NULL */
+    float* rstd;           /* [rows] */
+    int64_t y_stride, h_stride;
+} sxh_layer_norm_outputs;
+int32_t sxh_layer_norm_fwd(sxh_backend* b, const sxh_layer_norm_inputs* in, const sxh_layer_norm_outputs* out,
+                           const sxh_queue* q);
+
+/* Its gradients, with xhat = (h - mean) * rstd and g = dy * weight:
+ *   dx = rstd * (g - mean_row(g) - xhat * mean_row(g * xhat)) + dh   (the gradient of x, and of the residual),
+ *   dweight = sum over rows of dy * xhat, dbias = sum over rows of dy. */
+typedef struct {
+    const void* dy;        /* [rows, width] */
+    const void* h;         /* [rows, width] what was normalised */
+    const void* dh;        /* [rows, width] the gradient that reaches h past the norm, or NULL: 0 */
+    const float* mean;     /* [rows] of the forward */
+    const float* rstd;     /* [rows] */
+    const void* weight;    /* [width], or NULL: 1 */
+    int64_t rows, width;
+    int64_t dy_stride, h_stride, dh_stride;
+    uint8_t type;          /* of dy, h, dh, dx */
+    uint8_t weight_type;   /* of weight, dweight, dbias: SXH_TYPE_F32, or `type` */
+} sxh_layer_norm_grads_in;
+typedef struct {
+    void* dx;              /* [rows, width], or NULL: not wanted (the rows are not learned; then dh is NULL) */
+    void* dweight;         /* [width] or NULL */
+    void* dbias;           /* [width] or NULL */
+    int64_t dx_stride;
+    void* workspace;       /* sxh_layer_norm_bwd_workspace(rows, width) bytes of device memory, 16-byte aligned; not
+                              needed (may be NULL) when neither dweight nor dbias is wanted */
+    int64_t workspace_bytes;
+} sxh_layer_norm_grads;
+int64_t sxh_layer_norm_bwd_workspace(int64_t rows, int64_t width);
+int32_t sxh_layer_norm_bwd(sxh_backend* b, const sxh_layer_norm_grads_in* in, const sxh_layer_norm_grads* out,
+                           const sxh_queue* q);
+
+/* The 2-norm of all tensors' elements together, sqrt(sum g^2), squares and sum in 64 bits: no element overflows
+ * or vanishes in it. Not finite exactly when an element is not (or the norm itself is beyond float). */
+typedef struct {
+    const void* grad;      /* [n] */
+    int64_t n;             /* may be 0 */
+    uint8_t type;
+} sxh_norm_tensor;
+int64_t sxh_grad_norm_workspace(int64_t n_tensors);
+int32_t sxh_grad_norm(sxh_backend* b, const sxh_norm_tensor* tensors /* host array */, int64_t n_tensors,
+                      float* norm /* [1] device */, void* workspace /* device, 16-byte aligned */,
+                      int64_t workspace_bytes, const sxh_queue* q);
+
+/* One AdamW step of every tensor, in place:
+ *   c = grad_scale; with grad_norm and max_norm > 0 and n = grad_scale * grad_norm > max_norm also times max_norm / n
+ *   g = c * grad; m = b1 m + (1 - b1) g; v = b2 v + (1 - b2) g^2
+ *   param = param (1 - lr weight_decay) - lr / (1 - b1^step) * m / (sqrt(v) / sqrt(1 - b2^step) + eps).
+ * With grad_norm the step is left out, no buffer changed, where n is not finite (an overflowed loss scale). The rates
+ * and 1 - b^step are formed in 64 bits on the host, the rest in 32.
+ * state_bits 32: exp_avg and exp_avg_sq are float[n], the scales NULL. state_bits 8: exp_avg holds m and exp_avg_sq
+ * sqrt(v) as E4M3 bytes [n] (sign, 4 exponent bits of bias 7, 3 of mantissa, 0x7f not a number), each block of 256
+ * consecutive elements in units of its float scale [ceil(n / 256)], which is the block's largest finite magnitude /
+ * 448 (0 for a block of none above 2^-100). The step itself uses m and v before they are rounded. A magnitude is
+ * rounded up to the next code with the probability of its distance from the code below, in steps of 2^-16: a running
+ * mean whose step is far below the codes' distance would stand still under rounding to nearest. The bits are a
+ * function of (seed, step, tensor's place in the call, element) alone (m takes the low half, the root the high half).
+ * A root that is not zero keeps the least code 2^-9, so that no quotient loses its denominator. Elements that are not
+ * finite are held as not a number and leave the others of their block as they are. */
+typedef struct {
+    void* param;             /* [n] param_type */
+    float* master;           /* [n] what the step works on, param being its rounded copy: with a param_type other
+                                than SXH_TYPE_F32 only, else NULL */
+    const void* grad;        /* [n] grad_type */
+    void* exp_avg;           /* [n] */
+    void* exp_avg_sq;        /* [n] */
+    float* exp_avg_scale;    /* [ceil(n / 256)] with state_bits 8, else NULL */
+    float* exp_avg_sq_scale;
+    int64_t n;               /* may be 0 */
+    double lr, weight_decay;
+    uint8_t param_type, grad_type;
+} sxh_adamw_tensor;
+typedef struct {
+    int64_t step;            /* 1 for the first */
+    uint64_t seed;           /* of the rounding, with state_bits 8 */
+    double b1, b2, eps;      /* 0 <= b < 1, eps > 0 */
+    const float* grad_norm;  /* [1] device, or NULL */
+    float max_norm;          /* 0: no clipping */
+    float grad_scale;        /* 1 / the loss scale */
+    int32_t state_bits;      /* 32 or 8 */
+} sxh_adamw_params;
+int32_t sxh_adamw(sxh_backend* b, const sxh_adamw_tensor* tensors /* host array */, int64_t n_tensors,
+                  const sxh_adamw_params* params, const sxh_queue* q);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif

@@ -1,0 +1,76 @@
+// sx_learn.h — kernel arguments and launchers of the learned heads' operators (k_norm.hip, k_adamw.hip).
+// Every pointer is a device pointer; launchers allocate nothing and wait for nothing.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace sxk {
+
+// The types of include/splatx_hip.h.
+enum ElemType : uint8_t { kF32 = 0, kBf16 = 1, kF16 = 2 };
+
+struct NormFwdArgs {
+    const void *x, *residual, *weight, *bias;
+    void *y, *h;
+    float *mean, *rstd;
+    int64_t rows, x_stride, residual_stride, y_stride, h_stride;
+    int width;
+    float eps;
+};
+void layer_norm_fwd(const NormFwdArgs& a, ElemType type, ElemType weight_type, hipStream_t s);
+
+struct NormBwdArgs {
+    const void *dy, *h, *dh, *weight;
+    const float *mean, *rstd;
+    void *dx, *dweight, *dbias;
+    float* partial;  // [norm_bwd_slabs][2][width]
+    int64_t rows, dy_stride, h_stride, dh_stride, dx_stride;
+    int width;
+};
+// Parts of the rows whose column sums are formed one by one, then joined.
+int norm_bwd_slabs(int64_t rows, int64_t width);
+void layer_norm_bwd(const NormBwdArgs& a, ElemType type, ElemType weight_type, hipStream_t s);
+
+// Tensors of one launch, passed by value: a launch's arguments hold at most 4 KiB.
+constexpr int kNormTensors = 160;
+struct NormTable {
+    const void* grad[kNormTensors];
+    int64_t n[kNormTensors];
+    uint8_t type[kNormTensors];
+    int tensors;
+};
+constexpr int kNormSlots = 1024;  // partial sums (doubles) of a launch, at most
+// Partial sums of the table's tensors into part[0, slots); returns the slots written.
+int sum_squares(const NormTable& t, double* part, hipStream_t s);
+// norm[0] = sqrt(sum of part[0, n))
+void norm_of_sums(const double* part, int64_t n, float* norm, hipStream_t s);
+
+constexpr int kAdamTensors = 36;
+constexpr int kAdamBlock = 256;  // elements that share a scale with moments in 8 bits
+struct AdamTensor {
+    void* param;
+    float* master;
+    const void* grad;
+    void *m, *v;
+    float *m_scale, *v_scale;
+    int64_t n;
+    float decay;     // 1 - lr weight_decay
+    float rate;      // lr / (1 - b1^step)
+    uint32_t key;    // of the rounding
+    uint8_t param_type, grad_type, aligned;
+};
+struct AdamTable {
+    AdamTensor t[kAdamTensors];
+    int32_t first[kAdamTensors + 1];  // tensor i has the launch's chunks [first[i], first[i + 1])
+    int tensors;
+    const float* grad_norm;
+    float max_norm, grad_scale, b1, b2, c1, c2, root_c2, eps;  // c = 1 - b; root_c2 = 1 / sqrt(1 - b2^step)
+};
+static_assert(sizeof(AdamTable) <= 4096 && sizeof(NormTable) <= 4096, "a launch's arguments hold 4 KiB");
+constexpr int kAdamChunk = 1024;  // elements of a workgroup
+// The key of the rounding of the call's tensor.
+uint32_t adam_key(uint64_t seed, int64_t step, int64_t tensor);
+void adamw(const AdamTable& t, bool eight_bits, hipStream_t s);
+
+}  // namespace sxk
