@@ -199,7 +199,10 @@ int32_t sxh_layer_norm_fwd(sxh_backend* b, const sxh_layer_norm_inputs* in, cons
 
 int64_t sxh_layer_norm_bwd_workspace(int64_t rows, int64_t width) {
     if (rows < 0 || width < 1 || width > (int64_t{1} << 24)) return 0;
-    return int64_t{sxk::norm_bwd_slabs(rows, width)} * 2 * width * 4;
+    int slabs = 0;  // the most that any type needs
+    for (const sxk::ElemType t : {sxk::kF32, sxk::kBf16}) slabs = std::max(slabs, sxk::norm_bwd_slabs(rows, width, t, false));
+    for (const sxk::ElemType t : {sxk::kF32, sxk::kBf16}) slabs = std::max(slabs, sxk::norm_bwd_slabs(rows, width, t, true));
+    return int64_t{slabs} * 2 * width * 4;
 }
 
 int32_t sxh_layer_norm_bwd(sxh_backend* b, const sxh_layer_norm_grads_in* in, const sxh_layer_norm_grads* out,

@@ -1,4 +1,5 @@
-// sx_elem.h — device loads and stores of float, bfloat16 and half elements as floats. A store rounds to nearest even.
+// sx_elem.h — device helpers of the learned heads' kernels: float, bfloat16 and half elements as floats, one at a time
+// and 16 bytes at a time, and sums over groups of lanes. A store rounds to nearest even.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -18,11 +19,92 @@ __device__ inline void store_float(void* p, int64_t i, float v, int type) {
     else static_cast<_Float16*>(p)[i] = static_cast<_Float16>(v);
 }
 
-__device__ inline float wave_sum(float v) {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
+// 16 bytes of elements. The address need only be aligned to an element: the GPU runs in unaligned access mode.
+template <class T>
+constexpr int kVec = 16 / sizeof(T);
+template <class T>
+using Vec = T __attribute__((ext_vector_type(kVec<T>)));
+template <class T>
+using Floats = float __attribute__((ext_vector_type(kVec<T>)));
+
+// The elements as they are, where the compiler would keep their floats since their last use: half the registers for a
+// conversion again.
+template <class T>
+__device__ inline Floats<T> floats_again(Vec<T>& v) {
+    if constexpr (sizeof(T) == 2) {
+        using Words = uint32_t __attribute__((ext_vector_type(4)));
+        Words w;
+        __builtin_memcpy(&w, &v, sizeof(w));
+        asm volatile("" : "+v"(w));
+        __builtin_memcpy(&v, &w, sizeof(w));
+    }
+    return __builtin_convertvector(v, Floats<T>);
+}
+template <class T>
+__device__ inline Vec<T> load_raw(const T* p) {
+    Vec<T> v;
+    __builtin_memcpy(&v, p, sizeof(v));
     return v;
 }
+// The same of what is not read again soon: it does not displace what the caches hold.
+template <class T>
+__device__ inline Vec<T> load_once(const T* p) {
+    using Words = uint32_t __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+    const uint32_t __attribute__((ext_vector_type(4))) w = __builtin_nontemporal_load(reinterpret_cast<const Words*>(p));
+    Vec<T> v;
+    __builtin_memcpy(&v, &w, sizeof(v));
+    return v;
+}
+template <class T>
+__device__ inline void store_raw(T* p, Vec<T> v) {
+    __builtin_memcpy(p, &v, sizeof(v));
+}
+template <class T>
+__device__ inline Floats<T> floats(Vec<T> v) {
+    return __builtin_convertvector(v, Floats<T>);
+}
+template <class T>
+__device__ inline Vec<T> raw(Floats<T> f) {
+    return __builtin_convertvector(f, Vec<T>);
+}
+template <class T>
+__device__ inline Floats<T> load_vec(const T* p) {
+    return floats<T>(load_raw(p));
+}
+
+// Sum over each aligned group of L lanes of a wave (a power of two), in every lane of the group; a fixed order.
+template <int CTRL>
+__device__ inline float dpp_add(float v) {
+    return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+template <int L>
+__device__ inline float group_sum(float v) {
+    if constexpr (L >= 2) v = dpp_add<0xB1>(v);   // quad_perm [1,0,3,2]
+    if constexpr (L >= 4) v = dpp_add<0x4E>(v);   // quad_perm [2,3,0,1]
+    if constexpr (L >= 8) v = dpp_add<0x141>(v);  // row_half_mirror: the other quad of 8
+    if constexpr (L >= 16) v = dpp_add<0x140>(v); // row_mirror: the other half of 16
+    if constexpr (L >= 32) {
+        const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+    }
+    if constexpr (L >= 64) {
+        const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+    }
+    return v;
+}
+// Sum over the lanes of a wave that are equal modulo L, in every one of them.
+template <int L>
+__device__ inline float across_groups(float v) {
+    if constexpr (L <= 1) v = dpp_add<0xB1>(v);
+    if constexpr (L <= 2) v = dpp_add<0x4E>(v);
+    if constexpr (L <= 4) v += __shfl_xor(v, 4);
+    if constexpr (L <= 8) v += __shfl_xor(v, 8);
+    if constexpr (L <= 16) v += __shfl_xor(v, 16);
+    if constexpr (L <= 32) v += __shfl_xor(v, 32);
+    return v;
+}
+
 __device__ inline double wave_sum(double v) {
 #pragma unroll
     for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);

@@ -27,9 +27,10 @@ struct NormBwdArgs {
     float* partial;  // [norm_bwd_slabs][2][width]
     int64_t rows, dy_stride, h_stride, dh_stride, dx_stride;
     int width;
+    bool stream;  // set by the launcher
 };
 // Parts of the rows whose column sums are formed one by one, then joined.
-int norm_bwd_slabs(int64_t rows, int64_t width);
+int norm_bwd_slabs(int64_t rows, int64_t width, ElemType type, bool dh);
 void layer_norm_bwd(const NormBwdArgs& a, ElemType type, ElemType weight_type, hipStream_t s);
 
 // Tensors of one launch, passed by value: a launch's arguments hold at most 4 KiB.
