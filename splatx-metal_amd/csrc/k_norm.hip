@@ -8,7 +8,6 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
-#include <type_traits>
 
 #include "sx_elem.h"
 #include "sx_learn.h"
@@ -179,11 +178,7 @@ __global__ void __launch_bounds__(kThreadsOf<TPR>) k_norm_bwd(NormBwdArgs a, boo
         Vec<T> dy[R][K], x[R][K], dh[R][K];
         float mean[R], rstd[R];
     };
-    const auto load_as = [&](auto once, Rows& to, int64_t first) {
-        const auto get = [](const T* from) {
-            if constexpr (decltype(once)::value) return load_once(from);
-            else return load_raw(from);
-        };
+    const auto load = [&](Rows& to, int64_t first) {
 #pragma unroll
         for (int r = 0; r < R; r++) {
             const int64_t row = min(first + group + r * kRows, a.rows - 1);
@@ -193,8 +188,8 @@ __global__ void __launch_bounds__(kThreadsOf<TPR>) k_norm_bwd(NormBwdArgs a, boo
             to.rstd[r] = a.rstd[row];
 #pragma unroll
             for (int k = 0; k < K; k++) {
-                to.dy[r][k] = get(pd + p.at[k]);
-                to.x[r][k] = get(ph + p.at[k]);
+                to.dy[r][k] = load_raw(pd + p.at[k]);
+                to.x[r][k] = load_raw(ph + p.at[k]);
             }
         }
         if (a.dh)
@@ -202,11 +197,7 @@ __global__ void __launch_bounds__(kThreadsOf<TPR>) k_norm_bwd(NormBwdArgs a, boo
             for (int r = 0; r < R; r++)
 #pragma unroll
                 for (int k = 0; k < K; k++)
-                    to.dh[r][k] = get(static_cast<const T*>(a.dh) + min(first + group + r * kRows, a.rows - 1) * a.dh_stride + p.at[k]);
-    };
-    const auto load = [&](Rows& to, int64_t first) {
-        if (a.stream) load_as(std::true_type{}, to, first);
-        else load_as(std::false_type{}, to, first);
+                    to.dh[r][k] = load_raw(static_cast<const T*>(a.dh) + min(first + group + r * kRows, a.rows - 1) * a.dh_stride + p.at[k]);
     };
     const int64_t stride = int64_t{gridDim.x} * (kRows * R);
     constexpr bool kAhead = K == 1;  // the next rows are on their way while these are worked on
@@ -538,12 +529,6 @@ void layer_norm_bwd(const NormBwdArgs& args, ElemType type, ElemType weight_type
     const int slabs = norm_bwd_slabs(a.rows, a.width, type, a.dh != nullptr);
     const bool columns = a.dweight || a.dbias, fw = weight_type == kF32;
     if (!columns) a.partial = nullptr;
-    // Rows that are read once go past the caches where they are more than those hold (256 MiB) by the time they come again:
-    // 16,383 x 2048 36 us against 40, while 50,000 x 64 takes 8.6 against 8.0. Vectors that share lines with others need
-    // the cache (1 M x 45: 101 against 96).
-    const auto whole = [&](const void* p, int64_t stride) { return (reinterpret_cast<uintptr_t>(p) | static_cast<uintptr_t>(stride * size)) % 16 == 0; };
-    a.stream = a.rows * a.width * size * (a.dh ? 4 : 3) > (int64_t{128} << 20) && whole(a.dy, a.dy_stride) && whole(a.h, a.h_stride) &&
-               whole(a.dh, a.dh_stride);
     if (sp.vectors == 0 || a.rows == 0) {
         if (a.dx && a.rows) {
             const int grid = grid_of(a.rows, block_rows(sp));

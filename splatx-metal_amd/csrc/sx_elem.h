@@ -46,15 +46,6 @@ __device__ inline Vec<T> load_raw(const T* p) {
     __builtin_memcpy(&v, p, sizeof(v));
     return v;
 }
-// The same of what is not read again soon: it does not displace what the caches hold.
-template <class T>
-__device__ inline Vec<T> load_once(const T* p) {
-    using Words = uint32_t __attribute__((ext_vector_type(4), aligned(sizeof(T))));
-    const uint32_t __attribute__((ext_vector_type(4))) w = __builtin_nontemporal_load(reinterpret_cast<const Words*>(p));
-    Vec<T> v;
-    __builtin_memcpy(&v, &w, sizeof(v));
-    return v;
-}
 template <class T>
 __device__ inline void store_raw(T* p, Vec<T> v) {
     __builtin_memcpy(p, &v, sizeof(v));

@@ -27,7 +27,6 @@ struct NormBwdArgs {
     float* partial;  // [norm_bwd_slabs][2][width]
     int64_t rows, dy_stride, h_stride, dh_stride, dx_stride;
     int width;
-    bool stream;  // set by the launcher
 };
 // Parts of the rows whose column sums are formed one by one, then joined.
 int norm_bwd_slabs(int64_t rows, int64_t width, ElemType type, bool dh);
