@@ -14,34 +14,81 @@ namespace sxk {
 using namespace sxd;
 namespace {
 
-constexpr int kBlock = 256, kWave = 64;
+constexpr int kBlock = 256, kWave = 64, kFewBlock = 1024;
+static_assert(kAdamTensors <= kWave && kNormTensors <= kWave, "a lane for each tensor of a launch");
 
+// Sum over a workgroup of THREADS, in its first wave.
+template <int THREADS>
 __device__ double block_sum(double v) {
-    __shared__ double part[kBlock / kWave];
+    __shared__ double part[THREADS / kWave];
     v = wave_sum(v);
     if (threadIdx.x % kWave == 0) part[threadIdx.x / kWave] = v;
     __syncthreads();
-    double s = 0.0;
+    return wave_sum(threadIdx.x < THREADS / kWave ? part[threadIdx.x] : 0.0);
+}
+
+// The tensor of a launch's chunk: each lane asks for one, so that 64 cost what one does.
+__device__ inline int tensor_of(const int32_t* first, int tensors, int chunk) {
+    const int lane = threadIdx.x % kWave;
+    const bool past = lane < tensors && chunk >= first[lane + 1];
+    return __builtin_amdgcn_readfirstlane(__builtin_popcountll(__builtin_amdgcn_ballot_w64(past)));
+}
+
+// Squares of a chunk's elements [begin, end) of p, all its loads on their way at once.
+template <int THREADS, class T>
+__device__ inline double chunk_squares(const T* p, int64_t begin, int64_t end) {
+    constexpr int V = kVec<T>, U = kNormChunk / (THREADS * V);
+    const int thread = threadIdx.x % THREADS;
+    double sum = 0.0;
+    if (begin + kNormChunk <= end) {
+        Vec<T> x[U];
 #pragma unroll
-    for (int i = 0; i < kBlock / kWave; i++) s += part[i];
-    return s;
+        for (int u = 0; u < U; u++) x[u] = load_raw(p + begin + (u * THREADS + thread) * V);
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int e = 0; e < V; e++) {
+                const double g = static_cast<float>(x[u][e]);
+                sum = __builtin_fma(g, g, sum);
+            }
+        return sum;
+    }
+    for (int64_t i = begin + thread; i < min(begin + kNormChunk, end); i += THREADS) {
+        const double g = static_cast<float>(p[i]);
+        sum = __builtin_fma(g, g, sum);
+    }
+    return sum;
+}
+
+// Squares of every `step`-th chunk from `first` on, THREADS of them at a chunk.
+template <int THREADS>
+__device__ inline double sum_chunks(const NormTable& t, int first, int step) {
+    double sum = 0.0;
+    for (int chunk = first; chunk < t.first[t.tensors]; chunk += step) {
+        const int k = tensor_of(t.first, t.tensors, chunk);
+        const int64_t begin = int64_t{chunk - t.first[k]} * kNormChunk;
+        if (t.type[k] == kF32) sum += chunk_squares<THREADS>(static_cast<const float*>(t.grad[k]), begin, t.n[k]);
+        else if (t.type[k] == kBf16) sum += chunk_squares<THREADS>(static_cast<const __bf16*>(t.grad[k]), begin, t.n[k]);
+        else sum += chunk_squares<THREADS>(static_cast<const _Float16*>(t.grad[k]), begin, t.n[k]);
+    }
+    return sum;
 }
 
 __global__ void __launch_bounds__(kBlock) k_sum_squares(NormTable t, double* __restrict__ part) {
-    double sum = 0.0;
-    for (int k = 0; k < t.tensors; k++)
-        for (int64_t i = blockIdx.x * int64_t{kBlock} + threadIdx.x; i < t.n[k]; i += int64_t{gridDim.x} * kBlock) {
-            const double g = load_as_float(t.grad[k], i, t.type[k]);
-            sum += g * g;
-        }
-    sum = block_sum(sum);
+    const double sum = block_sum<kBlock>(sum_chunks<kBlock>(t, blockIdx.x, gridDim.x));
     if (threadIdx.x == 0) part[blockIdx.x] = sum;
+}
+// One workgroup, a wave at each chunk.
+__global__ void __launch_bounds__(kFewBlock) k_norm_of_few(NormTable t, float* __restrict__ norm) {
+    constexpr int kWaves = kFewBlock / kWave;
+    const double sum = block_sum<kFewBlock>(sum_chunks<kWave>(t, __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), kWaves));
+    if (threadIdx.x == 0) norm[0] = static_cast<float>(__builtin_sqrt(sum));
 }
 
 __global__ void __launch_bounds__(kBlock) k_norm_of_sums(const double* __restrict__ part, int64_t n, float* __restrict__ norm) {
     double sum = 0.0;
     for (int64_t i = threadIdx.x; i < n; i += kBlock) sum += part[i];
-    sum = block_sum(sum);
+    sum = block_sum<kBlock>(sum);
     if (threadIdx.x == 0) norm[0] = static_cast<float>(__builtin_sqrt(sum));
 }
 
@@ -55,42 +102,115 @@ __device__ bool grad_factor(const AdamTable& t, float* c) {
     return true;
 }
 
-__device__ int tensor_of(const AdamTable& t, int chunk) {
-    int k = 0;
-    while (chunk >= t.first[k + 1]) k++;
-    return k;
+template <int E>
+using Few = float __attribute__((ext_vector_type(E)));
+using Four = Few<4>;
+
+// E elements at p, which need only be aligned to one: the GPU runs in unaligned access mode. ONCE: what is not read again
+// before the caches have turned over goes past them.
+template <bool ONCE, class V, class T>
+__device__ inline V load_as(const T* p) {
+    using At = V __attribute__((aligned(sizeof(T))));
+    if constexpr (ONCE) return __builtin_nontemporal_load(reinterpret_cast<const At*>(p));
+    return *reinterpret_cast<const At*>(p);
+}
+template <bool ONCE, class V, class T>
+__device__ inline void store_as(T* p, V v) {
+    using At = V __attribute__((aligned(sizeof(T))));
+    if constexpr (ONCE) __builtin_nontemporal_store(v, reinterpret_cast<At*>(p));
+    else *reinterpret_cast<At*>(p) = v;
 }
 
-// The moments after this gradient, and the parameter after its step.
-__device__ float adam_one(const AdamTable& t, const AdamTensor& a, float p, float g, float& m, float& v) {
-    m = __builtin_fmaf(t.c1, g, t.b1 * m);
-    v = __builtin_fmaf(t.c2, g * g, t.b2 * v);
-    return p * a.decay - a.rate * (m / (__builtin_sqrtf(v) * t.root_c2 + t.eps));
-}
-
-__device__ void step_param(const AdamTable& t, const AdamTensor& a, int64_t i, float g, float& m, float& v) {
-    if (a.param_type == kF32) {
-        float* p = static_cast<float*>(a.param) + i;
-        *p = adam_one(t, a, *p, g, m, v);
+// Elements i .. i + E - 1 of a tensor of n as floats, zeros from n on.
+template <int E, bool ONCE, class T>
+__device__ inline Few<E> load_few(const T* p, int64_t i, int64_t n) {
+    using V = T __attribute__((ext_vector_type(E)));
+    V v = V(0);
+    if (i + E <= n) {
+        v = load_as<ONCE, V>(p + i);
     } else {
-        const float p = adam_one(t, a, a.master[i], g, m, v);
-        a.master[i] = p;
-        store_float(a.param, i, p, a.param_type);
+#pragma unroll
+        for (int j = 0; j < E - 1; j++)
+            if (i + j < n) v[j] = p[i + j];
+    }
+    return __builtin_convertvector(v, Few<E>);
+}
+template <int E, bool ONCE, class T>
+__device__ inline void store_few(T* p, int64_t i, int64_t n, Few<E> f) {
+    using V = T __attribute__((ext_vector_type(E)));
+    const V v = __builtin_convertvector(f, V);
+    if (i + E <= n) {
+        store_as<ONCE>(p + i, v);
+    } else {
+#pragma unroll
+        for (int j = 0; j < E - 1; j++)
+            if (i + j < n) p[i + j] = v[j];
     }
 }
+template <int E, bool ONCE>
+__device__ inline Few<E> load_grad(const AdamTensor& a, int64_t i) {
+    if (a.grad_type == kF32) return load_few<E, ONCE>(static_cast<const float*>(a.grad), i, a.n);
+    if (a.grad_type == kBf16) return load_few<E, ONCE>(static_cast<const __bf16*>(a.grad), i, a.n);
+    return load_few<E, ONCE>(static_cast<const _Float16*>(a.grad), i, a.n);
+}
+// The step's parameter, and where it is a master copy its rounded one.
+template <int E, bool ONCE>
+__device__ inline void store_param(const AdamTensor& a, int64_t i, Few<E> p) {
+    if (a.param_type == kF32) {
+        store_few<E, ONCE>(static_cast<float*>(a.param), i, a.n, p);
+        return;
+    }
+    store_few<E, ONCE>(a.master, i, a.n, p);
+    if (a.param_type == kBf16) store_few<E, ONCE>(static_cast<__bf16*>(a.param), i, a.n, p);
+    else store_few<E, ONCE>(static_cast<_Float16*>(a.param), i, a.n, p);
+}
 
+// The square root to nearest for x of 2^-100 or more, by one correction of the approximate one with the remainder of its
+// square (Markstein): 8 instructions where the library's takes 15, which the 8-bit step would wait for.
+__device__ inline float root(float x) {
+    const float y = __builtin_amdgcn_rsqf(x), s = x * y;
+    const float r = __builtin_fmaf(0.5f * y, __builtin_fmaf(-s, s, x), s);
+    return x > 0.0f && x < __builtin_inff() ? r : x;  // (0, infinity and NaN are their own)
+}
+
+// The moments after this gradient, the second one's root, and the parameter after its step. The quotient is off by 2 units
+// in its last place at most (the hardware's reciprocal), which the parameter's own rounding covers.
+struct AdamStep {
+    float m, v, root, p;
+};
+__device__ inline AdamStep adam_one(const AdamTable& t, float decay, float rate, float p, float g, float m, float v) {
+    AdamStep s;
+    s.m = __builtin_fmaf(t.c1, g, t.b1 * m);
+    s.v = __builtin_fmaf(t.c2, g * g, t.b2 * v);
+    s.root = root(s.v);
+    s.p = __builtin_fmaf(-rate, s.m * __builtin_amdgcn_rcpf(__builtin_fmaf(s.root, t.root_c2, t.eps)), p * decay);
+    return s;
+}
+
+// Two elements a thread at a time, kAdamChunk a workgroup.
+template <bool ONCE>
 __global__ void __launch_bounds__(kBlock) k_adamw(AdamTable t) {
+    const int k = tensor_of(t.first, t.tensors, blockIdx.x);
+    const AdamTensor a = t.t[k];
     float c;
     if (!grad_factor(t, &c)) return;
-    const int k = tensor_of(t, blockIdx.x);
-    const AdamTensor& a = t.t[k];
-    const int64_t begin = int64_t{static_cast<int>(blockIdx.x) - t.first[k]} * kAdamChunk;
-    const int64_t end = begin + kAdamChunk < a.n ? begin + kAdamChunk : a.n;
-    for (int64_t i = begin + threadIdx.x; i < end; i += kBlock) {
-        float m = static_cast<float*>(a.m)[i], v = static_cast<float*>(a.v)[i];
-        step_param(t, a, i, load_as_float(a.grad, i, a.grad_type) * c, m, v);
-        static_cast<float*>(a.m)[i] = m;
-        static_cast<float*>(a.v)[i] = v;
+    const int64_t begin = int64_t{static_cast<int>(blockIdx.x) - t.first[k]} * kAdamChunk, end = min(begin + kAdamChunk, a.n);
+    const float* from = a.param_type == kF32 ? static_cast<const float*>(a.param) : a.master;
+    float *am = static_cast<float*>(a.m), *av = static_cast<float*>(a.v);
+#pragma unroll 1
+    for (int64_t i = begin + threadIdx.x * 2; i < end; i += kBlock * 2) {
+        Few<2> p = load_few<2, ONCE>(from, i, a.n), m = load_few<2, ONCE>(am, i, a.n), v = load_few<2, ONCE>(av, i, a.n);
+        const Few<2> g = load_grad<2, ONCE>(a, i);
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const AdamStep s = adam_one(t, a.decay, a.rate, p[j], g[j] * c, m[j], v[j]);
+            p[j] = s.p;
+            m[j] = s.m;
+            v[j] = s.v;
+        }
+        store_few<2, ONCE>(am, i, a.n, m);
+        store_few<2, ONCE>(av, i, a.n, v);
+        store_param<2, ONCE>(a, i, p);
     }
 }
 
@@ -105,76 +225,124 @@ __host__ __device__ inline uint32_t mix(uint32_t h) {
 
 constexpr float kLeastMax = 0x1p-100f;
 
-__device__ float decode(uint8_t code, float scale) {
-    return __builtin_amdgcn_cvt_f32_fp8(code, 0) * scale;
+// The bytes of elements i .. i + 3, zeros from element n on.
+template <bool ONCE>
+__device__ inline uint32_t load_codes(const void* p, int64_t i, int64_t n) {
+    const uint8_t* c = static_cast<const uint8_t*>(p) + i;
+    uint32_t w = 0;
+    if (i + 4 <= n) {
+        w = load_as<ONCE, uint32_t>(c);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 3; j++)
+            if (i + j < n) w |= uint32_t{c[j]} << (8 * j);
+    }
+    return w;
 }
-// E4M3 of x: |x| * inv (at most 448 but for rounding) rounded up with the probability of bits / 2^16.
-__device__ uint8_t encode(float x, float inv, uint32_t bits, bool least) {
-    const float size = fabsf(x);
-    if (!(size < __builtin_inff())) return 0x7f;
-    const float u = fminf(size * inv, 448.0f);
-    const bool low = u < 0x1p-6f;
-    const float at = low ? u + 0x1p-6f : u;
-    uint32_t code = ((__float_as_uint(at) + (bits << 4)) >> 20) - (low ? 968u : 960u);
-    if (least && inv > 0.0f && size > 0.0f && code == 0u) code = 1u;
-    return static_cast<uint8_t>(x < 0.0f ? code + 128u : code);
+template <bool ONCE>
+__device__ inline void store_codes(void* p, int64_t i, int64_t n, uint32_t w) {
+    uint8_t* c = static_cast<uint8_t*>(p) + i;
+    if (i + 4 <= n) {
+        store_as<ONCE>(c, w);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 3; j++)
+            if (i + j < n) c[j] = static_cast<uint8_t>(w >> (8 * j));
+    }
 }
-__device__ float finite_size(float x) {
-    const float s = fabsf(x);
-    return s < __builtin_inff() ? s : 0.0f;
+__device__ inline Four decode(uint32_t w, float scale) {
+    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
+    return Four{lo[0] * scale, lo[1] * scale, hi[0] * scale, hi[1] * scale};
+}
+__device__ inline bool finite(float x) { return fabsf(x) < __builtin_inff(); }
+
+// The codes of four values of at most 448 in magnitude: the hardware adds the high 20 of the random bits to what lies below
+// a code's last bit and cuts off.
+__device__ inline uint32_t encode(const float (&u)[4], const uint32_t (&bits)[4]) {
+    uint32_t w = __builtin_amdgcn_cvt_sr_fp8_f32(u[0], bits[0], 0, 0);
+    w = __builtin_amdgcn_cvt_sr_fp8_f32(u[1], bits[1], w, 1);
+    w = __builtin_amdgcn_cvt_sr_fp8_f32(u[2], bits[2], w, 2);
+    return __builtin_amdgcn_cvt_sr_fp8_f32(u[3], bits[3], w, 3);
 }
 
-// A wave per block of 256 elements, four a lane.
+// A wave per block of 256 elements, four side by side a lane.
+template <bool ONCE>
 __global__ void __launch_bounds__(kBlock) k_adamw8(AdamTable t) {
+    const int k = tensor_of(t.first, t.tensors, blockIdx.x);
+    const AdamTensor a = t.t[k];
     float c;
     if (!grad_factor(t, &c)) return;
-    const int k = tensor_of(t, blockIdx.x);
-    const AdamTensor& a = t.t[k];
-    const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+    const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int64_t block = int64_t{static_cast<int>(blockIdx.x) - t.first[k]} * (kAdamChunk / kAdamBlock) + wave;
+    const int64_t i = block * kAdamBlock + lane * 4;
     if (block * kAdamBlock >= a.n) return;
+    static_assert(kAdamChunk / kAdamBlock == kBlock / kWave && kAdamBlock == 4 * kWave);
+    const float* from = a.param_type == kF32 ? static_cast<const float*>(a.param) : a.master;
     const float m_scale = a.m_scale[block], v_scale = a.v_scale[block];
-    float m[4], v[4], top_m = 0.0f, top_v = 0.0f;
+    const uint32_t mc = load_codes<ONCE>(a.m, i, a.n), vc = load_codes<ONCE>(a.v, i, a.n);
+    Four p = load_few<4, ONCE>(from, i, a.n);
+    const Four g = load_grad<4, ONCE>(a, i);
+    const Four m = decode(mc, m_scale), r = decode(vc, v_scale);
+    float um[4], ur[4], top_m = 0.0f, top_r = 0.0f;
+    bool good = true;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-        const int64_t i = block * kAdamBlock + j * kWave + lane;
-        m[j] = v[j] = 0.0f;
-        if (i < a.n) {
-            m[j] = decode(static_cast<uint8_t*>(a.m)[i], m_scale);
-            const float root = decode(static_cast<uint8_t*>(a.v)[i], v_scale);
-            v[j] = root * root;
-            step_param(t, a, i, load_as_float(a.grad, i, a.grad_type) * c, m[j], v[j]);
-            v[j] = __builtin_sqrtf(v[j]);
-            top_m = fmaxf(top_m, finite_size(m[j]));
-            top_v = fmaxf(top_v, finite_size(v[j]));
+        const AdamStep s = adam_one(t, a.decay, a.rate, p[j], g[j] * c, m[j], r[j] * r[j]);
+        p[j] = s.p;
+        um[j] = s.m;
+        ur[j] = s.root;
+        good = good && finite(s.m) && finite(s.root);
+    }
+    store_param<4, ONCE>(a, i, p);
+    uint32_t bad_m = 0, bad_r = 0;  // a byte of ones for each that is not finite
+    if (!good) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            if (!finite(um[j])) bad_m |= 0xffu << (8 * j), um[j] = 0.0f;
+            if (!finite(ur[j])) bad_r |= 0xffu << (8 * j), ur[j] = 0.0f;
         }
     }
-    top_m = wave_max(top_m);
-    top_v = wave_max(top_v);
-    const float inv_m = top_m >= kLeastMax ? 448.0f * (1.0f / top_m) : 0.0f;
-    const float inv_v = top_v >= kLeastMax ? 448.0f * (1.0f / top_v) : 0.0f;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-        const int64_t i = block * kAdamBlock + j * kWave + lane;
-        if (i >= a.n) continue;
-        const uint32_t r = mix(static_cast<uint32_t>(i) * 0x9E3779B9u + a.key);
-        static_cast<uint8_t*>(a.m)[i] = encode(m[j], inv_m, r & 0xffffu, false);
-        static_cast<uint8_t*>(a.v)[i] = encode(v[j], inv_v, r >> 16, true);
+        top_m = fmaxf(top_m, fabsf(um[j]));
+        top_r = fmaxf(top_r, ur[j]);
     }
+    top_m = wave_max(top_m);
+    top_r = wave_max(top_r);
+    const float inv_m = top_m >= kLeastMax ? 448.0f * (1.0f / top_m) : 0.0f;
+    const float inv_r = top_r >= kLeastMax ? 448.0f * (1.0f / top_r) : 0.0f;
+    const float least = inv_r > 0.0f ? 0x1p-9f : 0.0f;
+    uint32_t bits_m[4], bits_r[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        um[j] = __builtin_amdgcn_fmed3f(um[j] * inv_m, -448.0f, 448.0f);
+        ur[j] = ur[j] > 0.0f ? __builtin_amdgcn_fmed3f(ur[j] * inv_r, least, 448.0f) : 0.0f;
+        bits_r[j] = mix(static_cast<uint32_t>(i + j) * 0x9E3779B9u + a.key);
+        bits_m[j] = bits_r[j] << 16;
+        bits_r[j] &= 0xffff0000u;
+    }
+    const uint32_t wm = encode(um, bits_m), wr = encode(ur, bits_r);
+    store_codes<ONCE>(a.m, i, a.n, (wm & ~bad_m) | (bad_m & 0x7f7f7f7fu));
+    store_codes<ONCE>(a.v, i, a.n, (wr & ~bad_r) | (bad_r & 0x7f7f7f7fu));
     if (lane == 0) {
         a.m_scale[block] = inv_m > 0.0f ? top_m * (1.0f / 448.0f) : 0.0f;
-        a.v_scale[block] = inv_v > 0.0f ? top_v * (1.0f / 448.0f) : 0.0f;
+        a.v_scale[block] = inv_r > 0.0f ? top_r * (1.0f / 448.0f) : 0.0f;
     }
 }
 
 }  // namespace
 
 int sum_squares(const NormTable& t, double* part, hipStream_t s) {
-    int64_t most = 1;
-    for (int k = 0; k < t.tensors; k++) most = std::max(most, t.n[k]);
-    const int grid = static_cast<int>(std::min<int64_t>((most + kBlock - 1) / kBlock, kNormSlots));
+    const int grid = std::min(t.first[t.tensors], kNormSlots);
     hipLaunchKernelGGL(k_sum_squares, dim3(grid), dim3(kBlock), 0, s, t, part);
     return grid;
+}
+bool norm_of_few(const NormTable& t, float* norm, hipStream_t s) {
+    int64_t total = 0;
+    for (int k = 0; k < t.tensors; k++) total += t.n[k];
+    if (t.first[t.tensors] > kFewBlock / kWave || total > 16384) return false;
+    hipLaunchKernelGGL(k_norm_of_few, dim3(1), dim3(kFewBlock), 0, s, t, norm);
+    return true;
 }
 void norm_of_sums(const double* part, int64_t n, float* norm, hipStream_t s) {
     hipLaunchKernelGGL(k_norm_of_sums, dim3(1), dim3(kBlock), 0, s, part, n, norm);
@@ -187,11 +355,16 @@ uint32_t adam_key(uint64_t seed, int64_t step, int64_t tensor) {
     return k;
 }
 
-void adamw(const AdamTable& t, bool eight_bits, hipStream_t s) {
+void adamw(const AdamTable& t, bool eight_bits, bool once, hipStream_t s) {
     const dim3 grid(t.first[t.tensors]);
     if (grid.x == 0) return;
-    if (eight_bits) hipLaunchKernelGGL(k_adamw8, grid, dim3(kBlock), 0, s, t);
-    else hipLaunchKernelGGL(k_adamw, grid, dim3(kBlock), 0, s, t);
+    if (eight_bits) {
+        if (once) hipLaunchKernelGGL(k_adamw8<true>, grid, dim3(kBlock), 0, s, t);
+        else hipLaunchKernelGGL(k_adamw8<false>, grid, dim3(kBlock), 0, s, t);
+    } else {
+        if (once) hipLaunchKernelGGL(k_adamw<true>, grid, dim3(kBlock), 0, s, t);
+        else hipLaunchKernelGGL(k_adamw<false>, grid, dim3(kBlock), 0, s, t);
+    }
 }
 
 }  // namespace sxk

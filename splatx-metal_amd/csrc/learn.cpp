@@ -268,7 +268,7 @@ int32_t sxh_grad_norm(sxh_backend* b, const sxh_norm_tensor* tensors, int64_t n_
         for (int64_t i = 0; i < n_tensors; i++) {
             const sxh_norm_tensor& t = tensors[i];
             need_type(what, t.type, "type");
-            if (t.n < 0 || t.n > (int64_t{1} << 48)) invalid(what, "n must be 0..2^48");
+            if (t.n < 0 || t.n > (int64_t{1} << 40)) invalid(what, "n must be 0..2^40");
             if (!t.n) continue;
             const size_t size = static_cast<size_t>(t.n) * type_size(t.type);
             mem.need(t.grad, size, type_size(t.type), "grad");
@@ -280,14 +280,26 @@ int32_t sxh_grad_norm(sxh_backend* b, const sxh_norm_tensor* tensors, int64_t n_
         auto* part = static_cast<double*>(workspace);
         int64_t slots = 0;
         for (int64_t i = 0; i < n_tensors;) {
-            sxk::NormTable t{};
+            sxk::NormTable t;
+            t.tensors = 0;
+            t.first[0] = 0;
             for (; i < n_tensors && t.tensors < sxk::kNormTensors; i++) {
-                if (!tensors[i].n) continue;
-                t.grad[t.tensors] = tensors[i].grad;
-                t.n[t.tensors] = tensors[i].n;
-                t.type[t.tensors++] = tensors[i].type;
+                const sxh_norm_tensor& x = tensors[i];
+                const int64_t chunks = (x.n + sxk::kNormChunk - 1) / sxk::kNormChunk;
+                if (!chunks) continue;
+                if (t.tensors && t.first[t.tensors] + chunks > INT32_MAX) break;
+                t.grad[t.tensors] = x.grad;
+                t.n[t.tensors] = x.n;
+                t.type[t.tensors] = x.type;
+                t.first[t.tensors + 1] = t.first[t.tensors] + static_cast<int32_t>(chunks);
+                t.tensors++;
             }
-            if (t.tensors) slots += sxk::sum_squares(t, part + slots, on.stream());
+            if (!t.tensors) break;
+            if (i == n_tensors && slots == 0 && sxk::norm_of_few(t, norm, on.stream())) {
+                on.done();
+                return;
+            }
+            slots += sxk::sum_squares(t, part + slots, on.stream());
         }
         sxk::norm_of_sums(part, slots, norm, on.stream());
         on.done();
@@ -311,12 +323,14 @@ int32_t sxh_adamw(sxh_backend* b, const sxh_adamw_tensor* tensors, int64_t n_ten
         const bool eight = p->state_bits == 8;
         DeviceMemory mem(what, b->device);
         std::vector<Rows> written, read;
+        size_t total = 0;  // bytes of all
         written.reserve(static_cast<size_t>(n_tensors) * (eight ? 6 : 4));
         read.reserve(static_cast<size_t>(n_tensors) + 1);
         auto range = [&](std::vector<Rows>& to, const void* ptr, int64_t n, size_t e, const char* name) {
             const size_t bytes = static_cast<size_t>(n) * e;
             mem.need(ptr, bytes, e, name);
             to.push_back({name, reinterpret_cast<uintptr_t>(ptr), bytes, bytes, 0});
+            total += bytes;
         };
         if (p->grad_norm) range(read, p->grad_norm, 1, 4, "grad_norm");
         for (int64_t i = 0; i < n_tensors; i++) {
@@ -361,8 +375,9 @@ int32_t sxh_adamw(sxh_backend* b, const sxh_adamw_tensor* tensors, int64_t n_ten
         const double step = static_cast<double>(p->step);
         t.root_c2 = static_cast<float>(1.0 / std::sqrt(1.0 - std::pow(p->b2, step)));
         const double by = 1.0 / (1.0 - std::pow(p->b1, step));
+        constexpr size_t kCacheBytes = size_t{256} << 20;  // of the last-level cache
         auto flush = [&] {
-            sxk::adamw(t, eight, on.stream());
+            sxk::adamw(t, eight, total > kCacheBytes, on.stream());
             t.tensors = 0;
         };
         constexpr int64_t kMostChunks = int64_t{1} << 30;  // of a launch

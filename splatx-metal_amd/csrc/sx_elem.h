@@ -63,32 +63,41 @@ __device__ inline Floats<T> load_vec(const T* p) {
     return floats<T>(load_raw(p));
 }
 
-// Sum over each aligned group of L lanes of a wave (a power of two), in every lane of the group; a fixed order.
+// A value of another lane by data-parallel primitives; every lane of the wave takes part.
 template <int CTRL>
-__device__ inline float dpp_add(float v) {
-    return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+__device__ inline float dpp(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
 }
-template <int L>
-__device__ inline float group_sum(float v) {
-    if constexpr (L >= 2) v = dpp_add<0xB1>(v);   // quad_perm [1,0,3,2]
-    if constexpr (L >= 4) v = dpp_add<0x4E>(v);   // quad_perm [2,3,0,1]
-    if constexpr (L >= 8) v = dpp_add<0x141>(v);  // row_half_mirror: the other quad of 8
-    if constexpr (L >= 16) v = dpp_add<0x140>(v); // row_mirror: the other half of 16
+// `with` (a sum or a maximum) over each aligned group of L lanes of a wave (a power of two), in every lane of the group, in
+// a fixed order.
+template <int L, class F>
+__device__ inline float over_group(float v, F with) {
+    if constexpr (L >= 2) v = with(v, dpp<0xB1>(v));    // quad_perm [1,0,3,2]
+    if constexpr (L >= 4) v = with(v, dpp<0x4E>(v));    // quad_perm [2,3,0,1]
+    if constexpr (L >= 8) v = with(v, dpp<0x141>(v));   // row_half_mirror: the other quad of 8
+    if constexpr (L >= 16) v = with(v, dpp<0x140>(v));  // row_mirror: the other half of 16
     if constexpr (L >= 32) {
         const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-        v = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+        v = with(__uint_as_float(s[0]), __uint_as_float(s[1]));
     }
     if constexpr (L >= 64) {
         const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-        v = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+        v = with(__uint_as_float(s[0]), __uint_as_float(s[1]));
     }
     return v;
+}
+template <int L>
+__device__ inline float group_sum(float v) {
+    return over_group<L>(v, [](float a, float b) { return a + b; });
+}
+__device__ inline float wave_max(float v) {
+    return over_group<64>(v, [](float a, float b) { return fmaxf(a, b); });
 }
 // Sum over the lanes of a wave that are equal modulo L, in every one of them.
 template <int L>
 __device__ inline float across_groups(float v) {
-    if constexpr (L <= 1) v = dpp_add<0xB1>(v);
-    if constexpr (L <= 2) v = dpp_add<0x4E>(v);
+    if constexpr (L <= 1) v += dpp<0xB1>(v);
+    if constexpr (L <= 2) v += dpp<0x4E>(v);
     if constexpr (L <= 4) v += __shfl_xor(v, 4);
     if constexpr (L <= 8) v += __shfl_xor(v, 8);
     if constexpr (L <= 16) v += __shfl_xor(v, 16);
@@ -101,10 +110,4 @@ __device__ inline double wave_sum(double v) {
     for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
     return v;
 }
-__device__ inline float wave_max(float v) {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
-    return v;
-}
-
 }  // namespace sxd

@@ -33,18 +33,22 @@ int norm_bwd_slabs(int64_t rows, int64_t width, ElemType type, bool dh);
 void layer_norm_bwd(const NormBwdArgs& a, ElemType type, ElemType weight_type, hipStream_t s);
 
 // Tensors of one launch, passed by value: a launch's arguments hold at most 4 KiB.
-constexpr int kNormTensors = 160;
+constexpr int kNormTensors = 64;
+constexpr int kNormChunk = 4096;  // elements that a workgroup (of few tensors a wave) takes at a time
 struct NormTable {
     const void* grad[kNormTensors];
     int64_t n[kNormTensors];
+    int32_t first[kNormTensors + 1];  // tensor i has the launch's chunks [first[i], first[i + 1])
     uint8_t type[kNormTensors];
     int tensors;
 };
-constexpr int kNormSlots = 1024;  // partial sums (doubles) of a launch, at most
+constexpr int kNormSlots = 2048;  // partial sums (doubles) of a launch, at most
 // Partial sums of the table's tensors into part[0, slots); returns the slots written.
 int sum_squares(const NormTable& t, double* part, hipStream_t s);
 // norm[0] = sqrt(sum of part[0, n))
 void norm_of_sums(const double* part, int64_t n, float* norm, hipStream_t s);
+// Both in one launch, where the tensors are few enough for one workgroup; else false.
+bool norm_of_few(const NormTable& t, float* norm, hipStream_t s);
 
 constexpr int kAdamTensors = 36;
 constexpr int kAdamBlock = 256;  // elements that share a scale with moments in 8 bits
@@ -58,7 +62,7 @@ struct AdamTensor {
     float decay;     // 1 - lr weight_decay
     float rate;      // lr / (1 - b1^step)
     uint32_t key;    // of the rounding
-    uint8_t param_type, grad_type, aligned;
+    uint8_t param_type, grad_type;
 };
 struct AdamTable {
     AdamTensor t[kAdamTensors];
@@ -71,6 +75,7 @@ static_assert(sizeof(AdamTable) <= 4096 && sizeof(NormTable) <= 4096, "a launch'
 constexpr int kAdamChunk = 1024;  // elements of a workgroup
 // The key of the rounding of the call's tensor.
 uint32_t adam_key(uint64_t seed, int64_t step, int64_t tensor);
-void adamw(const AdamTable& t, bool eight_bits, hipStream_t s);
+// `once`: the call's tensors are more than the caches hold.
+void adamw(const AdamTable& t, bool eight_bits, bool once, hipStream_t s);
 
 }  // namespace sxk

@@ -21,6 +21,7 @@ import splatx_hip as sh
 TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # SXH_TYPE_*
 ADAMW_BLOCK = 256  # elements that share a scale with 8-bit moments
 _CODE_TYPES = (torch.float8_e4m3fn, torch.uint8)
+_FLOAT = (torch.float32,)
 
 
 class Queue(C.Structure):
@@ -65,14 +66,26 @@ class AdamWParams(C.Structure):
                 ("grad_norm", C.c_void_p), ("max_norm", C.c_float), ("grad_scale", C.c_float), ("state_bits", C.c_int32)]
 
 
-# the two tables' rows as bytes: a step of many tensors fills them each time
+# The structs as bytes, which a call fills in a third of the time that it takes through ctypes: a small operator's time is
+# its call's.
+_QUEUE = struct.Struct("<Q")
+_NORM_IN = struct.Struct("<4Q4qfBB2x")
+_NORM_OUT = struct.Struct("<4Q2q")
+_GRADS_IN = struct.Struct("<6Q5qBB6x")
+_GRADS = struct.Struct("<3QqQq")
 _NORM_ROW = struct.Struct("<QqB7x")
 _ADAMW_ROW = struct.Struct("<7QqddBB6x")
-assert _NORM_ROW.size == C.sizeof(NormTensor) and _ADAMW_ROW.size == C.sizeof(AdamWTensor)
+_ADAMW = struct.Struct("<qQdddQffi4x")
+for _packed, _struct in ((_QUEUE, Queue), (_NORM_IN, LayerNormInputs), (_NORM_OUT, LayerNormOutputs), (_GRADS_IN, LayerNormGradsIn),
+                         (_GRADS, LayerNormGrads), (_NORM_ROW, NormTensor), (_ADAMW_ROW, AdamWTensor), (_ADAMW, AdamWParams)):
+    assert _packed.size == C.sizeof(_struct), _struct
 
 _is_contiguous = torch.Tensor.is_contiguous
 _numel = torch.Tensor.numel
 _ptr = torch.Tensor.data_ptr
+_empty = torch.empty
+# (the public way to the current stream's handle makes an object of it, 2 us)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
 
 
 def _one_hip_runtime():
@@ -94,27 +107,36 @@ class TorchBackend(sh.Backend):
 
     def __init__(self, device_ordinal: int = 0, lib=None):
         torch.cuda.init()
-        super().__init__(device_ordinal, lib)
+        lib = lib or sh.load_library()
         _one_hip_runtime()
+        super().__init__(device_ordinal, lib)
         self.device = torch.device("cuda", device_ordinal)
-        for name, args in (("layer_norm_fwd", 4), ("layer_norm_bwd", 4)):
-            getattr(self.lib, "sxh_" + name).argtypes = [C.c_void_p] * args
-        self.lib.sxh_grad_norm.argtypes = [C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]
-        self.lib.sxh_adamw.argtypes = [C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p]
-        for name, args in (("layer_norm_bwd_workspace", 2), ("grad_norm_workspace", 1)):
-            f = getattr(self.lib, "sxh_" + name)
-            f.argtypes, f.restype = [C.c_int64] * args, C.c_int64
+        self._index = device_ordinal
+        p, n = C.c_void_p, C.c_int64
+        self._ops = {}
+        for name, args in (("layer_norm_fwd", (p, p, p, p)), ("layer_norm_bwd", (p, p, p, p)), ("grad_norm", (p, p, n, p, p, n, p)),
+                           ("adamw", (p, p, n, p, p))):
+            f = self._ops[name] = getattr(self.lib, "sxh_" + name)
+            f.argtypes, f.restype = args, C.c_int32
+        for name, args in (("layer_norm_bwd_workspace", (n, n)), ("grad_norm_workspace", (n,))):
+            f = self._ops[name] = getattr(self.lib, "sxh_" + name)
+            f.argtypes, f.restype = args, n
 
-    def _queue(self):
-        return C.byref(Queue(torch.cuda.current_stream(self.device).cuda_stream))
+    def _enqueue(self, name, *args):
+        """The operator on torch's current stream of the device."""
+        rc = self._ops[name](self.handle, *args, _QUEUE.pack(_raw_stream(self._index)))
+        if rc != sh.SXH_OK:
+            msg = self.lib.sxh_last_error().decode(errors="replace")
+            raise (sh.SxInvalidArgument if rc == sh.SXH_ERR_INVALID_ARGUMENT else sh.SxRuntimeError)(msg)
 
     def _rows(self, t, name, like=None):
         """(tensor as [rows, width], its row stride)"""
         if not isinstance(t, torch.Tensor) or t.device != self.device:
             raise sh.SxInvalidArgument(f"{name} must be a tensor on {self.device}")
-        if t.dtype not in TYPES:
-            raise sh.SxInvalidArgument(f"{name} must be float32, bfloat16 or float16")
-        if like is not None and (t.dtype != like.dtype or t.shape != like.shape):
+        if like is None:
+            if t.dtype not in TYPES:
+                raise sh.SxInvalidArgument(f"{name} must be float32, bfloat16 or float16")
+        elif t.dtype != like.dtype or t.shape != like.shape:
             raise sh.SxInvalidArgument(f"{name} must have the rows' type and shape")
         if t.dim() != 2:
             if t.dim() == 0:
@@ -124,10 +146,10 @@ class TorchBackend(sh.Backend):
             except RuntimeError:
                 raise sh.SxInvalidArgument(f"{name}: rows of {tuple(t.shape)} with strides {t.stride()} are not evenly spaced") from None
         rows, width = t.shape
-        stride = t.stride()
-        if width > 1 and stride[1] != 1:
+        stride, inner = t.stride()
+        if inner != 1 and width > 1:
             raise sh.SxInvalidArgument(f"{name}: the elements of a row must lie side by side")
-        return t, stride[0] if rows > 1 else width
+        return t, stride if rows > 1 else width
 
     def _vector(self, t, name, n, types):
         if not isinstance(t, torch.Tensor) or t.device != self.device:
@@ -136,80 +158,96 @@ class TorchBackend(sh.Backend):
             raise sh.SxInvalidArgument(f"{name} must be {n} contiguous elements of {' or '.join(map(str, types))}")
         return t.data_ptr()
 
+    def _like(self, t):
+        """Contiguous rows like t's."""
+        return torch.empty_like(t) if t.is_contiguous() else _empty(t.shape, dtype=t.dtype, device=self.device)
+
     # -- layer norm ------------------------------------------------------------------------------------
     def layer_norm_fwd(self, x, weight=None, bias=None, eps=1e-5, residual=None, stats=True):
         """(y, h, mean, rstd): h = x + residual (x itself without one), y = (h - mean) rstd weight + bias over the last
         dimension; mean and rstd, one per row, are None without `stats`."""
         x2, x_stride = self._rows(x, "x")
         rows, width = x2.shape
-        types = (torch.float32, x.dtype)
+        t = x.dtype
         wt = weight.dtype if weight is not None else bias.dtype if bias is not None else torch.float32
-        w = self._vector(weight, "weight", width, types) if weight is not None else None
-        b = self._vector(bias, "bias", width, (wt,)) if bias is not None else None
-        y = torch.empty(x.shape, dtype=x.dtype, device=self.device)
-        h, r2, r_stride = None, None, 0
+        w = self._vector(weight, "weight", width, (torch.float32, t)) if weight is not None else 0
+        b = self._vector(bias, "bias", width, (wt,) if weight is not None else (torch.float32, t)) if bias is not None else 0
+        y = self._like(x)
+        h, r, r_stride = x, 0, 0
         if residual is not None:
-            r2, r_stride = self._rows(residual, "residual", x)
-            h = torch.empty_like(y)
+            residual, r_stride = self._rows(residual, "residual", x)
+            h, r = self._like(x), residual.data_ptr()
         mean = rstd = None
+        m = s = 0
         if stats:
-            mean, rstd = (torch.empty(x.shape[:-1], dtype=torch.float32, device=self.device) for _ in range(2))
-        self._call("layer_norm_fwd",
-                   C.byref(LayerNormInputs(x2.data_ptr(), r2.data_ptr() if r2 is not None else None, w, b, rows, width, x_stride,
-                                           r_stride, eps, TYPES[x.dtype], TYPES[wt])),
-                   C.byref(LayerNormOutputs(y.data_ptr(), h.data_ptr() if h is not None else None,
-                                            mean.data_ptr() if stats else None, rstd.data_ptr() if stats else None, width, width)),
-                   self._queue())
-        return y, x if h is None else h, mean, rstd
+            mean = _empty(x.shape[:-1], dtype=torch.float32, device=self.device)
+            rstd = torch.empty_like(mean)
+            m, s = mean.data_ptr(), rstd.data_ptr()
+        self._enqueue("layer_norm_fwd",
+                      _NORM_IN.pack(x2.data_ptr(), r, w, b, rows, width, x_stride, r_stride, eps, TYPES[t], TYPES[wt]),
+                      _NORM_OUT.pack(y.data_ptr(), h.data_ptr() if r else 0, m, s, width, width))
+        return y, h, mean, rstd
 
     def layer_norm_bwd(self, dy, h, mean, rstd, weight=None, dh=None, want_dx=True, want_dweight=True, want_dbias=True):
         """(dx, dweight, dbias) of layer_norm_fwd's h, mean and rstd; dx is the gradient of x and of the residual, with the
         gradient dh that reaches h past the norm. dweight and dbias have the weight's type (float32 without one)."""
         h2, h_stride = self._rows(h, "h")
-        dy2, dy_stride = self._rows(dy, "dy", h)
+        dy, dy_stride = self._rows(dy, "dy", h)
         rows, width = h2.shape
-        w = self._vector(weight, "weight", width, (torch.float32, h.dtype)) if weight is not None else None
-        wt = weight.dtype if weight is not None else torch.float32
-        dh2, dh_stride = self._rows(dh, "dh", h) if dh is not None else (None, 0)
+        wt, w, dh_ptr, dh_stride = torch.float32, 0, 0, 0
+        if weight is not None:
+            wt, w = weight.dtype, self._vector(weight, "weight", width, (torch.float32, h.dtype))
+        if dh is not None:
+            dh, dh_stride = self._rows(dh, "dh", h)
+            dh_ptr = dh.data_ptr()
         m = self._vector(mean, "mean", rows, (torch.float32,))
         s = self._vector(rstd, "rstd", rows, (torch.float32,))
-        dx = torch.empty(h.shape, dtype=h.dtype, device=self.device) if want_dx else None
-        dweight = torch.empty(width, dtype=wt, device=self.device) if want_dweight else None
-        dbias = torch.empty(width, dtype=wt, device=self.device) if want_dbias else None
-        work, bytes_ = None, 0
+        dx = dweight = dbias = work = None
+        dx_ptr = dweight_ptr = dbias_ptr = work_ptr = bytes_ = 0
+        if want_dx:
+            dx = self._like(h)
+            dx_ptr = dx.data_ptr()
         if want_dweight or want_dbias:
-            bytes_ = self.lib.sxh_layer_norm_bwd_workspace(rows, width)
-            work = torch.empty(bytes_, dtype=torch.uint8, device=self.device)
-        self._call("layer_norm_bwd",
-                   C.byref(LayerNormGradsIn(dy2.data_ptr(), h2.data_ptr(), dh2.data_ptr() if dh is not None else None, m, s, w,
-                                            rows, width, dy_stride, h_stride, dh_stride, TYPES[h.dtype], TYPES[wt])),
-                   C.byref(LayerNormGrads(dx.data_ptr() if want_dx else None, dweight.data_ptr() if want_dweight else None,
-                                          dbias.data_ptr() if want_dbias else None, width,
-                                          work.data_ptr() if work is not None else None, bytes_)),
-                   self._queue())
+            if want_dweight:
+                dweight = _empty(width, dtype=wt, device=self.device)
+                dweight_ptr = dweight.data_ptr()
+            if want_dbias:
+                dbias = _empty(width, dtype=wt, device=self.device)
+                dbias_ptr = dbias.data_ptr()
+            bytes_ = self._ops["layer_norm_bwd_workspace"](rows, width)
+            work = _empty(bytes_, dtype=torch.uint8, device=self.device)
+            work_ptr = work.data_ptr()
+        self._enqueue("layer_norm_bwd",
+                      _GRADS_IN.pack(dy.data_ptr(), h2.data_ptr(), dh_ptr, m, s, w, rows, width, dy_stride, h_stride, dh_stride,
+                                     TYPES[h.dtype], TYPES[wt]),
+                      _GRADS.pack(dx_ptr, dweight_ptr, dbias_ptr, width, work_ptr, bytes_))
         return dx, dweight, dbias
 
     # -- many tensors ------------------------------------------------------------------------------------
-    def _tensors(self, ts, name, types):
-        """Pointers of a list of contiguous tensors of the device."""
-        for t in ts:
-            if not isinstance(t, torch.Tensor) or t.device != self.device:
-                raise sh.SxInvalidArgument(f"{name} must be tensors on {self.device}")
-            if t.dtype not in types:
-                raise sh.SxInvalidArgument(f"{name} must be {' or '.join(map(str, types))}, not {t.dtype}")
+    @staticmethod
+    def _tensors(ts, name, types):
+        """(pointers, sizes, types) of a list of contiguous tensors; that they are on the device is checked with the pointers."""
+        try:
+            ptrs, sizes = list(map(_ptr, ts)), list(map(_numel, ts))
+        except TypeError:
+            raise sh.SxInvalidArgument(f"{name} must be tensors") from None
+        dtypes = [t.dtype for t in ts]
+        for t in set(dtypes):
+            if t not in types:
+                raise sh.SxInvalidArgument(f"{name} must be {' or '.join(map(str, types))}, not {t}")
         if not all(map(_is_contiguous, ts)):
             raise sh.SxInvalidArgument(f"{name} must be contiguous")
-        return list(map(_ptr, ts))
+        return ptrs, sizes, dtypes
 
     def grad_norm(self, grads):
         """The 2-norm of all the tensors together, as a tensor of one float32 on the device."""
         grads = list(grads)
-        ptrs = self._tensors(grads, "grads", tuple(TYPES))
-        norm = torch.empty((), dtype=torch.float32, device=self.device)
-        bytes_ = self.lib.sxh_grad_norm_workspace(len(grads))
-        work = torch.empty(bytes_, dtype=torch.uint8, device=self.device)
-        table = b"".join(_NORM_ROW.pack(p, t.numel(), TYPES[t.dtype]) for p, t in zip(ptrs, grads))
-        self._call("grad_norm", table, len(grads), norm.data_ptr(), work.data_ptr(), bytes_, self._queue())
+        ptrs, sizes, dtypes = self._tensors(grads, "grads", TYPES)
+        norm = _empty((), dtype=torch.float32, device=self.device)
+        bytes_ = self._ops["grad_norm_workspace"](len(grads))
+        work = _empty(bytes_, dtype=torch.uint8, device=self.device)
+        table = b"".join(map(_NORM_ROW.pack, ptrs, sizes, map(TYPES.__getitem__, dtypes)))
+        self._enqueue("grad_norm", table, len(grads), norm.data_ptr(), work.data_ptr(), bytes_)
         return norm
 
     def adamw_step(self, params, grads, exp_avg, exp_avg_sq, *, step, lr, weight_decay=0.0, b1=0.9, b2=0.999, eps=1e-8,
@@ -218,44 +256,41 @@ class TorchBackend(sh.Backend):
         float32 copies that the step works on, with 16-bit params. With the scales, exp_avg and exp_avg_sq are float8_e4m3fn
         (or uint8) tensors: m, and the root of v, in units of their block's scale. grad_norm: `grad_norm`'s result of these
         gradients; where it is not finite the step is left out."""
-        params, grads = list(params), list(grads)
         n = len(params)
         eight = exp_avg_scale is not None
         if eight != (exp_avg_sq_scale is not None):
             raise sh.SxInvalidArgument("exp_avg_scale and exp_avg_sq_scale are given together")
-        lists = [params, params if master is None else list(master), grads, list(exp_avg), list(exp_avg_sq)]
-        states = _CODE_TYPES if eight else (torch.float32,)
-        named = [("params", tuple(TYPES)), ("master", (torch.float32,) if master is not None else tuple(TYPES)),
-                 ("grads", tuple(TYPES)), ("exp_avg", states), ("exp_avg_sq", states)]
+        states = _CODE_TYPES if eight else _FLOAT
+        none = [0] * n
+        param_ptrs, sizes, param_types = self._tensors(params, "params", TYPES)
+        grad_ptrs, got, grad_types = self._tensors(grads, "grads", TYPES)
+        self._same(got, sizes, "grads")
+
+        def like(ts, name, types, want):
+            ptrs, got, _ = self._tensors(ts, name, types)
+            self._same(got, want, name)
+            return ptrs
+
+        master_ptrs = none if master is None else like(master, "master", _FLOAT, sizes)
+        m, v = like(exp_avg, "exp_avg", states, sizes), like(exp_avg_sq, "exp_avg_sq", states, sizes)
+        m_scale = v_scale = none
         if eight:
-            lists += [list(exp_avg_scale), list(exp_avg_sq_scale)]
-            named += [("exp_avg_scale", (torch.float32,)), ("exp_avg_sq_scale", (torch.float32,))]
-        for ts, (name, _) in zip(lists, named):
-            if len(ts) != n:
-                raise sh.SxInvalidArgument(f"{name}: {len(ts)} tensors for {n} params")
-        sizes = list(map(_numel, params))
-        for ts, (name, _) in zip(lists[1:5], named[1:5]):
-            if list(map(_numel, ts)) != sizes:
-                raise sh.SxInvalidArgument(f"{name} must have the params' sizes")
-        if eight:
-            blocks = list(map(adamw_blocks, sizes))
-            for ts, (name, _) in zip(lists[5:], named[5:]):
-                if list(map(_numel, ts)) != blocks:
-                    raise sh.SxInvalidArgument(f"{name} must have a scale for each {ADAMW_BLOCK} elements of a param")
-        ptrs = [self._tensors(ts, name, types) for ts, (name, types) in zip(lists, named)]
-        if master is None:
-            ptrs[1] = [0] * n
-        if not eight:
-            ptrs += [[0] * n, [0] * n]
+            blocks = [-(-k // ADAMW_BLOCK) for k in sizes]
+            m_scale = like(exp_avg_scale, "exp_avg_scale", _FLOAT, blocks)
+            v_scale = like(exp_avg_sq_scale, "exp_avg_sq_scale", _FLOAT, blocks)
         lrs = lr if isinstance(lr, (list, tuple)) else [lr] * n
         decays = weight_decay if isinstance(weight_decay, (list, tuple)) else [weight_decay] * n
         if len(lrs) != n or len(decays) != n:
             raise sh.SxInvalidArgument("lr and weight_decay are a number, or one for each tensor")
-        norm = self._vector(grad_norm, "grad_norm", 1, (torch.float32,)) if grad_norm is not None else None
-        table = b"".join(map(_ADAMW_ROW.pack, *ptrs, sizes, lrs, decays, [TYPES[p.dtype] for p in params],
-                             [TYPES[g.dtype] for g in grads]))
-        self._call("adamw", table, n,
-                   C.byref(AdamWParams(step, seed, b1, b2, eps, norm, max_norm, grad_scale, 8 if eight else 32)), self._queue())
+        norm = self._vector(grad_norm, "grad_norm", 1, _FLOAT) if grad_norm is not None else 0
+        table = b"".join(map(_ADAMW_ROW.pack, param_ptrs, master_ptrs, grad_ptrs, m, v, m_scale, v_scale, sizes, lrs, decays,
+                             map(TYPES.__getitem__, param_types), map(TYPES.__getitem__, grad_types)))
+        self._enqueue("adamw", table, n, _ADAMW.pack(step, seed, b1, b2, eps, norm, max_norm, grad_scale, 8 if eight else 32))
+
+    @staticmethod
+    def _same(got, want, name):
+        if got != want:
+            raise sh.SxInvalidArgument(f"{name}: {len(got)} tensors of {got[:8]}.. elements, wanted are {len(want)} of {want[:8]}..")
 
 
 class _LayerNorm(torch.autograd.Function):
