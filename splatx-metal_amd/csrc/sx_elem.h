@@ -46,6 +46,16 @@ __device__ inline Vec<T> load_raw(const T* p) {
     __builtin_memcpy(&v, p, sizeof(v));
     return v;
 }
+// ONCE: what is not read again before the caches have turned over goes past them.
+template <bool ONCE, class T>
+__device__ inline Vec<T> load_rows(const T* p) {
+    if constexpr (!ONCE) return load_raw(p);
+    using At = uint32_t __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+    const uint32_t __attribute__((ext_vector_type(4))) w = __builtin_nontemporal_load(reinterpret_cast<const At*>(p));
+    Vec<T> v;
+    __builtin_memcpy(&v, &w, sizeof(v));
+    return v;
+}
 template <class T>
 __device__ inline void store_raw(T* p, Vec<T> v) {
     __builtin_memcpy(p, &v, sizeof(v));
