@@ -37,13 +37,13 @@ __device__ inline int tensor_of(const int32_t* first, int tensors, int chunk) {
 // Squares of a chunk's elements [begin, end) of p, all its loads on their way at once.
 template <int THREADS, class T>
 __device__ inline double chunk_squares(const T* p, int64_t begin, int64_t end) {
-    constexpr int V = kVec<T>, U = kNormChunk / (THREADS * V);
+    constexpr int V = 16 / sizeof(T), U = kNormChunk / (THREADS * V);
     const int thread = threadIdx.x % THREADS;
     double sum = 0.0;
     if (begin + kNormChunk <= end) {
-        Vec<T> x[U];
+        Vec<T, V> x[U];
 #pragma unroll
-        for (int u = 0; u < U; u++) x[u] = load_raw(p + begin + (u * THREADS + thread) * V);
+        for (int u = 0; u < U; u++) x[u] = load_raw<V>(p + begin + (u * THREADS + thread) * V);
 #pragma unroll
         for (int u = 0; u < U; u++)
 #pragma unroll
@@ -102,45 +102,24 @@ __device__ bool grad_factor(const AdamTable& t, float* c) {
     return true;
 }
 
-template <int E>
-using Few = float __attribute__((ext_vector_type(E)));
-using Four = Few<4>;
-
-// E elements at p, which need only be aligned to one: the GPU runs in unaligned access mode. ONCE: what is not read again
-// before the caches have turned over goes past them.
-template <bool ONCE, class V, class T>
-__device__ inline V load_as(const T* p) {
-    using At = V __attribute__((aligned(sizeof(T))));
-    if constexpr (ONCE) return __builtin_nontemporal_load(reinterpret_cast<const At*>(p));
-    return *reinterpret_cast<const At*>(p);
-}
-template <bool ONCE, class V, class T>
-__device__ inline void store_as(T* p, V v) {
-    using At = V __attribute__((aligned(sizeof(T))));
-    if constexpr (ONCE) __builtin_nontemporal_store(v, reinterpret_cast<At*>(p));
-    else *reinterpret_cast<At*>(p) = v;
-}
-
 // Elements i .. i + E - 1 of a tensor of n as floats, zeros from n on.
 template <int E, bool ONCE, class T>
-__device__ inline Few<E> load_few(const T* p, int64_t i, int64_t n) {
-    using V = T __attribute__((ext_vector_type(E)));
-    V v = V(0);
+__device__ inline Floats<E> load_few(const T* p, int64_t i, int64_t n) {
+    Vec<T, E> v = Vec<T, E>(0);
     if (i + E <= n) {
-        v = load_as<ONCE, V>(p + i);
+        v = load_raw<E, ONCE>(p + i);
     } else {
 #pragma unroll
         for (int j = 0; j < E - 1; j++)
             if (i + j < n) v[j] = p[i + j];
     }
-    return __builtin_convertvector(v, Few<E>);
+    return floats<T, E>(v);
 }
 template <int E, bool ONCE, class T>
-__device__ inline void store_few(T* p, int64_t i, int64_t n, Few<E> f) {
-    using V = T __attribute__((ext_vector_type(E)));
-    const V v = __builtin_convertvector(f, V);
+__device__ inline void store_few(T* p, int64_t i, int64_t n, Floats<E> f) {
+    const Vec<T, E> v = raw<T, E>(f);
     if (i + E <= n) {
-        store_as<ONCE>(p + i, v);
+        store_raw<E, ONCE>(p + i, v);
     } else {
 #pragma unroll
         for (int j = 0; j < E - 1; j++)
@@ -148,14 +127,14 @@ __device__ inline void store_few(T* p, int64_t i, int64_t n, Few<E> f) {
     }
 }
 template <int E, bool ONCE>
-__device__ inline Few<E> load_grad(const AdamTensor& a, int64_t i) {
+__device__ inline Floats<E> load_grad(const AdamTensor& a, int64_t i) {
     if (a.grad_type == kF32) return load_few<E, ONCE>(static_cast<const float*>(a.grad), i, a.n);
     if (a.grad_type == kBf16) return load_few<E, ONCE>(static_cast<const __bf16*>(a.grad), i, a.n);
     return load_few<E, ONCE>(static_cast<const _Float16*>(a.grad), i, a.n);
 }
 // The step's parameter, and where it is a master copy its rounded one.
 template <int E, bool ONCE>
-__device__ inline void store_param(const AdamTensor& a, int64_t i, Few<E> p) {
+__device__ inline void store_param(const AdamTensor& a, int64_t i, Floats<E> p) {
     if (a.param_type == kF32) {
         store_few<E, ONCE>(static_cast<float*>(a.param), i, a.n, p);
         return;
@@ -199,8 +178,8 @@ __global__ void __launch_bounds__(kBlock) k_adamw(AdamTable t) {
     float *am = static_cast<float*>(a.m), *av = static_cast<float*>(a.v);
 #pragma unroll 1
     for (int64_t i = begin + threadIdx.x * 2; i < end; i += kBlock * 2) {
-        Few<2> p = load_few<2, ONCE>(from, i, a.n), m = load_few<2, ONCE>(am, i, a.n), v = load_few<2, ONCE>(av, i, a.n);
-        const Few<2> g = load_grad<2, ONCE>(a, i);
+        Floats<2> p = load_few<2, ONCE>(from, i, a.n), m = load_few<2, ONCE>(am, i, a.n), v = load_few<2, ONCE>(av, i, a.n);
+        const Floats<2> g = load_grad<2, ONCE>(a, i);
 #pragma unroll
         for (int j = 0; j < 2; j++) {
             const AdamStep s = adam_one(t, a.decay, a.rate, p[j], g[j] * c, m[j], v[j]);
@@ -231,7 +210,8 @@ __device__ inline uint32_t load_codes(const void* p, int64_t i, int64_t n) {
     const uint8_t* c = static_cast<const uint8_t*>(p) + i;
     uint32_t w = 0;
     if (i + 4 <= n) {
-        w = load_as<ONCE, uint32_t>(c);
+        const Vec<uint8_t, 4> b = load_raw<4, ONCE>(c);
+        __builtin_memcpy(&w, &b, 4);
     } else {
 #pragma unroll
         for (int j = 0; j < 3; j++)
@@ -243,16 +223,18 @@ template <bool ONCE>
 __device__ inline void store_codes(void* p, int64_t i, int64_t n, uint32_t w) {
     uint8_t* c = static_cast<uint8_t*>(p) + i;
     if (i + 4 <= n) {
-        store_as<ONCE>(c, w);
+        Vec<uint8_t, 4> b;
+        __builtin_memcpy(&b, &w, 4);
+        store_raw<4, ONCE>(c, b);
     } else {
 #pragma unroll
         for (int j = 0; j < 3; j++)
             if (i + j < n) c[j] = static_cast<uint8_t>(w >> (8 * j));
     }
 }
-__device__ inline Four decode(uint32_t w, float scale) {
+__device__ inline Floats<4> decode(uint32_t w, float scale) {
     const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
-    return Four{lo[0] * scale, lo[1] * scale, hi[0] * scale, hi[1] * scale};
+    return Floats<4>{lo[0] * scale, lo[1] * scale, hi[0] * scale, hi[1] * scale};
 }
 __device__ inline bool finite(float x) { return fabsf(x) < __builtin_inff(); }
 
@@ -280,9 +262,9 @@ __global__ void __launch_bounds__(kBlock) k_adamw8(AdamTable t) {
     const float* from = a.param_type == kF32 ? static_cast<const float*>(a.param) : a.master;
     const float m_scale = a.m_scale[block], v_scale = a.v_scale[block];
     const uint32_t mc = load_codes<ONCE>(a.m, i, a.n), vc = load_codes<ONCE>(a.v, i, a.n);
-    Four p = load_few<4, ONCE>(from, i, a.n);
-    const Four g = load_grad<4, ONCE>(a, i);
-    const Four m = decode(mc, m_scale), r = decode(vc, v_scale);
+    Floats<4> p = load_few<4, ONCE>(from, i, a.n);
+    const Floats<4> g = load_grad<4, ONCE>(a, i);
+    const Floats<4> m = decode(mc, m_scale), r = decode(vc, v_scale);
     float um[4], ur[4], top_m = 0.0f, top_r = 0.0f;
     bool good = true;
 #pragma unroll

@@ -8,6 +8,8 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <stdexcept>
+#include <type_traits>
 
 #include "sx_elem.h"
 #include "sx_learn.h"
@@ -16,28 +18,34 @@ namespace sxk {
 using namespace sxd;
 namespace {
 
-constexpr int kBlock = 256, kWave = 64;
+constexpr int kBlock = 256, kWave = 64, kUnits = 256;
+// TPR threads share a row: a power of two up to a wave, of which a workgroup has several rows, or a workgroup of up to TPR
+// threads, whole waves.
 template <int TPR>
-constexpr int kThreadsOf = TPR > kWave ? TPR : kBlock;  // of a workgroup: rows of up to a wave share one
+constexpr int kThreadsOf = TPR > kWave ? TPR : kBlock;  // of a workgroup, at most
+template <int TPR>
+constexpr int kRowsOf = TPR > kWave ? 1 : kBlock / TPR;  // of a workgroup
+template <int TPR>
+__device__ inline int threads_of_row() { return TPR > kWave ? static_cast<int>(blockDim.x) : TPR; }
 
-// The thread's place in its row: where its vectors begin, and what of the last one is its own.
-template <class T, int TPR, int K>
+// The thread's place in its row: where its vectors of V begin, and what of the last one is its own.
+template <int V, int TPR, int K>
 struct Place {
     int at[K];
     bool mine[K];
-    Floats<T> mask;  // of vector K - 1
+    Floats<V> mask;  // of vector K - 1
     int shift;       // its first elements that are another thread's
     __device__ Place(int width) {
-        const int t = threadIdx.x % TPR;
+        const int n = threads_of_row<TPR>(), t = TPR > kWave ? threadIdx.x : threadIdx.x % TPR;
 #pragma unroll
         for (int k = 0; k < K; k++) {
-            const int c = (k * TPR + t) * kVec<T>;
+            const int c = (k * n + t) * V;
             mine[k] = c < width;
-            at[k] = min(c, width - kVec<T>);
-            if (k == K - 1) shift = mine[k] ? c - at[k] : kVec<T>;
+            at[k] = min(c, width - V);
+            if (k == K - 1) shift = mine[k] ? c - at[k] : V;
         }
 #pragma unroll
-        for (int e = 0; e < kVec<T>; e++) mask[e] = e >= shift ? 1.0f : 0.0f;
+        for (int e = 0; e < V; e++) mask[e] = e >= shift ? 1.0f : 0.0f;
     }
 };
 
@@ -49,6 +57,7 @@ __device__ inline void row_sums(float (&v)[N]) {
     if constexpr (TPR > kWave) {
         constexpr int W = TPR / kWave;
         __shared__ float part[N][W];
+        const int waves = blockDim.x / kWave;
         __syncthreads();  // the sums before these have been read
         if (threadIdx.x % kWave == 0)
 #pragma unroll
@@ -58,45 +67,41 @@ __device__ inline void row_sums(float (&v)[N]) {
         for (int i = 0; i < N; i++) {
             float s = 0.0f;
 #pragma unroll
-            for (int w = 0; w < W; w++) s += part[i][w];
+            for (int w = 0; w < W; w++) s += w < waves ? part[i][w] : 0.0f;
             v[i] = s;
         }
     }
 }
 
-template <class T>
-__device__ inline Floats<T> load_weights(const void* w, int at, bool is_float, float none) {
-    if (!w) return Floats<T>(none);
-    if (is_float) {
-        Floats<T> v;
-        __builtin_memcpy(&v, static_cast<const float*>(w) + at, sizeof(v));
-        return v;
-    }
-    return load_vec(static_cast<const T*>(w) + at);
+template <class T, int V>
+__device__ inline Floats<V> load_weights(const void* w, int at, bool is_float, float none) {
+    if (!w) return Floats<V>(none);
+    if (is_float) return load_raw<V>(static_cast<const float*>(w) + at);
+    return floats<T, V>(load_raw<V>(static_cast<const T*>(w) + at));
 }
 
 // R rows of each group of threads at a time. The weights of a thread's only vector stay in its registers; those of more are
 // read again for each row (they lie in the L1 cache), which leaves the registers to the rows.
-template <class T, int TPR, int K, int R>
+template <class T, int V, int TPR, int K, int R>
 __global__ void __launch_bounds__(kThreadsOf<TPR>) k_norm_fwd(NormFwdArgs a, bool float_weights) {
-    constexpr int V = kVec<T>, kRows = kThreadsOf<TPR> / TPR;
-    const Place<T, TPR, K> p(a.width);
-    Floats<T> w, b;
+    constexpr int kRows = kRowsOf<TPR>;
+    const Place<V, TPR, K> p(a.width);
+    Floats<V> w, b;
     if constexpr (K == 1) {
-        w = load_weights<T>(a.weight, p.at[0], float_weights, 1.0f);
-        b = load_weights<T>(a.bias, p.at[0], float_weights, 0.0f);
+        w = load_weights<T, V>(a.weight, p.at[0], float_weights, 1.0f);
+        b = load_weights<T, V>(a.bias, p.at[0], float_weights, 0.0f);
     }
     const float inv_width = 1.0f / static_cast<float>(a.width);
-    const int group = threadIdx.x / TPR;
+    const int group = TPR > kWave ? 0 : threadIdx.x / TPR;
     for (int64_t first = blockIdx.x * int64_t{kRows * R}; first < a.rows; first += int64_t{gridDim.x} * (kRows * R)) {
         const int64_t row0 = first + group;  // and every kRows-th after it: a load of the workgroup's covers rows side by side
-        Vec<T> x[R][K];
+        Vec<T, V> x[R][K];
         float sum[R], sq[R];
 #pragma unroll
         for (int r = 0; r < R; r++) {
             const T* px = static_cast<const T*>(a.x) + min(row0 + r * kRows, a.rows - 1) * a.x_stride;
 #pragma unroll
-            for (int k = 0; k < K; k++) x[r][k] = load_raw(px + p.at[k]);
+            for (int k = 0; k < K; k++) x[r][k] = load_raw<V>(px + p.at[k]);
         }
         if (a.residual) {
 #pragma unroll
@@ -106,8 +111,8 @@ __global__ void __launch_bounds__(kThreadsOf<TPR>) k_norm_fwd(NormFwdArgs a, boo
                 T* ph = static_cast<T*>(a.h) + row * a.h_stride;
 #pragma unroll
                 for (int k = 0; k < K; k++) {
-                    x[r][k] = raw<T>(floats<T>(x[r][k]) + load_vec(pr + p.at[k]));
-                    if (p.mine[k] && row0 + r * kRows < a.rows) store_raw(ph + p.at[k], x[r][k]);
+                    x[r][k] = raw<T, V>(floats<T, V>(x[r][k]) + floats<T, V>(load_raw<V>(pr + p.at[k])));
+                    if (p.mine[k] && row0 + r * kRows < a.rows) store_raw<V>(ph + p.at[k], x[r][k]);
                 }
             }
         }
@@ -116,7 +121,7 @@ __global__ void __launch_bounds__(kThreadsOf<TPR>) k_norm_fwd(NormFwdArgs a, boo
             sum[r] = 0.0f;
 #pragma unroll
             for (int k = 0; k < K; k++) {
-                const Floats<T> v = floats<T>(x[r][k]);
+                const Floats<V> v = floats<T, V>(x[r][k]);
 #pragma unroll
                 for (int e = 0; e < V; e++) sum[r] = k == K - 1 ? __builtin_fmaf(v[e], p.mask[e], sum[r]) : sum[r] + v[e];
             }
@@ -128,7 +133,7 @@ __global__ void __launch_bounds__(kThreadsOf<TPR>) k_norm_fwd(NormFwdArgs a, boo
             sq[r] = 0.0f;
 #pragma unroll
             for (int k = 0; k < K; k++) {
-                const Floats<T> v = floats_again<T>(x[r][k]);
+                const Floats<V> v = floats_again<T, V>(x[r][k]);
 #pragma unroll
                 for (int e = 0; e < V; e++) {
                     const float d = v[e] - sum[r];
@@ -141,20 +146,20 @@ __global__ void __launch_bounds__(kThreadsOf<TPR>) k_norm_fwd(NormFwdArgs a, boo
         for (int r = 0; r < R; r++) {
             if (row0 + r * kRows >= a.rows) break;
             const int64_t row = row0 + r * kRows;
-            const float rstd = 1.0f / __builtin_sqrtf(sq[r] * inv_width + a.eps);
+            const float rstd = 1.0f / __builtin_sqrtf(sq[r] * inv_width + a.eps), at_zero = -sum[r] * rstd;
             T* py = static_cast<T*>(a.y) + row * a.y_stride;
 #pragma unroll
             for (int k = 0; k < K; k++) {
                 if constexpr (K > 1) {
-                    w = load_weights<T>(a.weight, p.at[k], float_weights, 1.0f);
-                    b = load_weights<T>(a.bias, p.at[k], float_weights, 0.0f);
+                    w = load_weights<T, V>(a.weight, p.at[k], float_weights, 1.0f);
+                    b = load_weights<T, V>(a.bias, p.at[k], float_weights, 0.0f);
                 }
-                Floats<T> y = floats_again<T>(x[r][k]);
+                Floats<V> y = floats_again<T, V>(x[r][k]);
 #pragma unroll
-                for (int e = 0; e < V; e++) y[e] = __builtin_fmaf((y[e] - sum[r]) * rstd, w[e], b[e]);
-                if (p.mine[k]) store_raw(py + p.at[k], raw<T>(y));
+                for (int e = 0; e < V; e++) y[e] = __builtin_fmaf(__builtin_fmaf(y[e], rstd, at_zero), w[e], b[e]);
+                if (p.mine[k]) store_raw<V>(py + p.at[k], raw<T, V>(y));
             }
-            if (a.mean && threadIdx.x % TPR == 0) {
+            if (a.mean && (TPR > kWave ? threadIdx.x : threadIdx.x % TPR) == 0) {
                 a.mean[row] = sum[r];
                 a.rstd[row] = rstd;
             }
@@ -164,18 +169,18 @@ __global__ void __launch_bounds__(kThreadsOf<TPR>) k_norm_fwd(NormFwdArgs a, boo
 
 // The backward of R rows of each group of threads at a time; the columns' sums stay in registers over the rows, are added
 // over the workgroup's groups at the end and written as its part of the partial sums.
-template <class T, int TPR, int K, int R, bool ONCE>
+template <class T, int V, int TPR, int K, int R, bool ONCE>
 __global__ void __launch_bounds__(kThreadsOf<TPR>) k_norm_bwd(NormBwdArgs a, bool float_weights) {
-    constexpr int V = kVec<T>, kThreads = kThreadsOf<TPR>, kRows = kThreads / TPR;
-    const Place<T, TPR, K> p(a.width);
-    Floats<T> w, dw[K], db[K];
-    if constexpr (K == 1) w = load_weights<T>(a.weight, p.at[0], float_weights, 1.0f);
+    constexpr int kRows = kRowsOf<TPR>;
+    const Place<V, TPR, K> p(a.width);
+    Floats<V> w, dw[K], db[K];
+    if constexpr (K == 1) w = load_weights<T, V>(a.weight, p.at[0], float_weights, 1.0f);
 #pragma unroll
-    for (int k = 0; k < K; k++) dw[k] = db[k] = Floats<T>(0.0f);
+    for (int k = 0; k < K; k++) dw[k] = db[k] = Floats<V>(0.0f);
     const float inv_width = 1.0f / static_cast<float>(a.width);
-    const int group = threadIdx.x / TPR;
+    const int group = TPR > kWave ? 0 : threadIdx.x / TPR;
     struct Rows {
-        Vec<T> dy[R][K], x[R][K], dh[R][K];
+        Vec<T, V> dy[R][K], x[R][K], dh[R][K];
         float mean[R], rstd[R];
     };
     const auto load = [&](Rows& to, int64_t first) {
@@ -188,8 +193,8 @@ __global__ void __launch_bounds__(kThreadsOf<TPR>) k_norm_bwd(NormBwdArgs a, boo
             to.rstd[r] = a.rstd[row];
 #pragma unroll
             for (int k = 0; k < K; k++) {
-                to.dy[r][k] = load_rows<ONCE>(pd + p.at[k]);
-                to.x[r][k] = load_rows<ONCE>(ph + p.at[k]);
+                to.dy[r][k] = load_raw<V, ONCE>(pd + p.at[k]);
+                to.x[r][k] = load_raw<V, ONCE>(ph + p.at[k]);
             }
         }
         if (a.dh)
@@ -197,12 +202,12 @@ __global__ void __launch_bounds__(kThreadsOf<TPR>) k_norm_bwd(NormBwdArgs a, boo
             for (int r = 0; r < R; r++)
 #pragma unroll
                 for (int k = 0; k < K; k++)
-                    to.dh[r][k] = load_rows<ONCE>(static_cast<const T*>(a.dh) + min(first + group + r * kRows, a.rows - 1) * a.dh_stride + p.at[k]);
+                    to.dh[r][k] = load_raw<V, ONCE>(static_cast<const T*>(a.dh) + min(first + group + r * kRows, a.rows - 1) * a.dh_stride + p.at[k]);
     };
     const int64_t stride = int64_t{gridDim.x} * (kRows * R);
     constexpr bool kAhead = K == 1;  // the next rows are on their way while these are worked on
     Rows next;
-    if constexpr (kAhead) load(next, blockIdx.x * int64_t{kRows * R});
+    if (kAhead && a.rows) load(next, blockIdx.x * int64_t{kRows * R});
     for (int64_t first = blockIdx.x * int64_t{kRows * R}; first < a.rows; first += stride) {
         const int64_t row0 = first + group;  // and every kRows-th after it: a load of the workgroup's covers rows side by side
         Rows now;
@@ -219,12 +224,12 @@ __global__ void __launch_bounds__(kThreadsOf<TPR>) k_norm_bwd(NormBwdArgs a, boo
         for (int r = 0; r < R; r++) {
             if (row0 + r * kRows >= a.rows)  // read in place of a row there is not
 #pragma unroll
-                for (int k = 0; k < K; k++) dy[r][k] = Vec<T>(0);
+                for (int k = 0; k < K; k++) dy[r][k] = Vec<T, V>(0);
             sums[2 * r] = sums[2 * r + 1] = 0.0f;
 #pragma unroll
             for (int k = 0; k < K; k++) {
-                const Floats<T> d = floats<T>(dy[r][k]), h = floats<T>(x[r][k]);
-                if constexpr (K > 1) w = load_weights<T>(a.weight, p.at[k], float_weights, 1.0f);
+                const Floats<V> d = floats<T, V>(dy[r][k]), h = floats<T, V>(x[r][k]);
+                if constexpr (K > 1) w = load_weights<T, V>(a.weight, p.at[k], float_weights, 1.0f);
 #pragma unroll
                 for (int e = 0; e < V; e++) {
                     const float xhat = (h[e] - mean[r]) * rstd[r], g = d[e] * w[e], gm = k == K - 1 ? g * p.mask[e] : g;
@@ -245,16 +250,16 @@ __global__ void __launch_bounds__(kThreadsOf<TPR>) k_norm_bwd(NormBwdArgs a, boo
             T* px = static_cast<T*>(a.dx) + row * a.dx_stride;
 #pragma unroll
             for (int k = 0; k < K; k++) {
-                Floats<T> d = floats_again<T>(dy[r][k]);
-                const Floats<T> h = floats_again<T>(x[r][k]);
-                if constexpr (K > 1) w = load_weights<T>(a.weight, p.at[k], float_weights, 1.0f);
+                Floats<V> d = floats_again<T, V>(dy[r][k]);
+                const Floats<V> h = floats_again<T, V>(x[r][k]);
+                if constexpr (K > 1) w = load_weights<T, V>(a.weight, p.at[k], float_weights, 1.0f);
 #pragma unroll
                 for (int e = 0; e < V; e++) {
                     const float xhat = (h[e] - mean[r]) * rstd[r];
                     d[e] = rstd[r] * __builtin_fmaf(-xhat, mgx, d[e] * w[e] - mg);
                 }
-                if (a.dh) d += floats<T>(now.dh[r][k]);
-                if (p.mine[k]) store_raw(px + p.at[k], raw<T>(d));
+                if (a.dh) d += floats<T, V>(now.dh[r][k]);
+                if (p.mine[k]) store_raw<V>(px + p.at[k], raw<T, V>(d));
             }
         }
     }
@@ -279,7 +284,7 @@ __global__ void __launch_bounds__(kThreadsOf<TPR>) k_norm_bwd(NormBwdArgs a, boo
                 dw[k][e] = across_groups<TPR>(dw[k][e]);
                 db[k][e] = across_groups<TPR>(db[k][e]);
             }
-        for (int turn = 0; turn < kThreads / kWave; turn++) {
+        for (int turn = 0; turn < kBlock / kWave; turn++) {
             if (wave == turn && t < TPR)
 #pragma unroll
                 for (int k = 0; k < K; k++)
@@ -326,141 +331,158 @@ __global__ void __launch_bounds__(kBlock) k_norm_join(NormBwdArgs a, int slabs, 
     }
 }
 
-// ---- rows that do not fit: narrower than a vector (a thread each), wider than a workgroup's registers (a workgroup each) --
+// ---- rows wider than a workgroup's registers: it goes over its row several times ------------------------------------------
 
-__device__ inline float block_sum(float v) {
-    __shared__ float part[kBlock / kWave];
-    v = group_sum<kWave>(v);
-    __syncthreads();
-    if (threadIdx.x % kWave == 0) part[threadIdx.x / kWave] = v;
-    __syncthreads();
-    float s = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kBlock / kWave; i++) s += part[i];
-    return s;
-}
-template <int TPR>
-__device__ inline float loop_sum(float v) {
-    if constexpr (TPR > 1) return block_sum(v);
-    return v;
+constexpr int kWideBlock = 1024;
+
+// f(where its vector begins, how many of its first elements are another's) for each of the thread's vectors.
+template <int V, class F>
+__device__ inline void each_vector(int width, F f) {
+    for (int c = threadIdx.x * V; c < width; c += kWideBlock * V) {
+        const int at = min(c, width - V);
+        f(at, c - at);
+    }
 }
 
-template <int TPR>
-__global__ void __launch_bounds__(kBlock) k_norm_fwd_loop(NormFwdArgs a, int type, int weight_type) {
-    const int lane = threadIdx.x % TPR;
-    for (int64_t row = blockIdx.x * int64_t{kBlock / TPR} + threadIdx.x / TPR; row < a.rows; row += int64_t{gridDim.x} * (kBlock / TPR)) {
-        const int64_t x0 = row * a.x_stride, r0 = row * a.residual_stride, h0 = row * a.h_stride, y0 = row * a.y_stride;
-        const void* from = a.residual ? a.h : a.x;
-        const int64_t f0 = a.residual ? h0 : x0;
-        float sum = 0.0f;
-        for (int c = lane; c < a.width; c += TPR) {
-            float v = load_as_float(a.x, x0 + c, type);
+template <class T>
+__global__ void __launch_bounds__(kWideBlock) k_norm_fwd_wide(NormFwdArgs a, bool float_weights) {
+    constexpr int V = 16 / sizeof(T);
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const T* px = static_cast<const T*>(a.x) + row * a.x_stride;
+        const T* from = a.residual ? static_cast<const T*>(a.h) + row * a.h_stride : px;
+        T* py = static_cast<T*>(a.y) + row * a.y_stride;
+        float sum[1] = {0.0f}, sq[1] = {0.0f};
+        each_vector<V>(a.width, [&](int at, int shift) {
+            Vec<T, V> x = load_raw<V>(px + at);
             if (a.residual) {
-                store_float(a.h, h0 + c, v + load_as_float(a.residual, r0 + c, type), type);
-                v = load_as_float(a.h, h0 + c, type);
+                x = raw<T, V>(floats<T, V>(x) + floats<T, V>(load_raw<V>(static_cast<const T*>(a.residual) + row * a.residual_stride + at)));
+                store_raw<V>(static_cast<T*>(a.h) + row * a.h_stride + at, x);
             }
-            sum += v;
-        }
-        const float mean = loop_sum<TPR>(sum) / static_cast<float>(a.width);
-        float sq = 0.0f;
-        for (int c = lane; c < a.width; c += TPR) {
-            const float d = load_as_float(from, f0 + c, type) - mean;
-            sq += d * d;
-        }
-        const float rstd = 1.0f / __builtin_sqrtf(loop_sum<TPR>(sq) / static_cast<float>(a.width) + a.eps);
-        for (int c = lane; c < a.width; c += TPR) {
-            float v = (load_as_float(from, f0 + c, type) - mean) * rstd;
-            if (a.weight) v *= load_as_float(a.weight, c, weight_type);
-            if (a.bias) v += load_as_float(a.bias, c, weight_type);
-            store_float(a.y, y0 + c, v, type);
-        }
-        if (a.mean && lane == 0) {
+            const Floats<V> v = floats<T, V>(x);
+#pragma unroll
+            for (int e = 0; e < V; e++) sum[0] += e >= shift ? v[e] : 0.0f;
+        });
+        row_sums<kWideBlock>(sum);  // (its barriers also let the sums' vectors be read by other threads)
+        const float mean = sum[0] / static_cast<float>(a.width);
+        each_vector<V>(a.width, [&](int at, int shift) {
+            const Floats<V> v = floats<T, V>(load_raw<V>(from + at));
+#pragma unroll
+            for (int e = 0; e < V; e++) {
+                const float d = e >= shift ? v[e] - mean : 0.0f;
+                sq[0] = __builtin_fmaf(d, d, sq[0]);
+            }
+        });
+        row_sums<kWideBlock>(sq);
+        const float rstd = 1.0f / __builtin_sqrtf(sq[0] / static_cast<float>(a.width) + a.eps), at_zero = -mean * rstd;
+        each_vector<V>(a.width, [&](int at, int) {
+            Floats<V> y = floats<T, V>(load_raw<V>(from + at));
+            const Floats<V> w = load_weights<T, V>(a.weight, at, float_weights, 1.0f), b = load_weights<T, V>(a.bias, at, float_weights, 0.0f);
+#pragma unroll
+            for (int e = 0; e < V; e++) y[e] = __builtin_fmaf(__builtin_fmaf(y[e], rstd, at_zero), w[e], b[e]);
+            store_raw<V>(py + at, raw<T, V>(y));
+        });
+        if (a.mean && threadIdx.x == 0) {
             a.mean[row] = mean;
             a.rstd[row] = rstd;
         }
     }
 }
 
-template <int TPR>
-__global__ void __launch_bounds__(kBlock) k_norm_dx_loop(NormBwdArgs a, int type, int weight_type) {
-    const int lane = threadIdx.x % TPR;
-    for (int64_t row = blockIdx.x * int64_t{kBlock / TPR} + threadIdx.x / TPR; row < a.rows; row += int64_t{gridDim.x} * (kBlock / TPR)) {
-        const int64_t y0 = row * a.dy_stride, h0 = row * a.h_stride;
+template <class T>
+__global__ void __launch_bounds__(kWideBlock) k_norm_dx_wide(NormBwdArgs a, bool float_weights) {
+    constexpr int V = 16 / sizeof(T);
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const T* pd = static_cast<const T*>(a.dy) + row * a.dy_stride;
+        const T* ph = static_cast<const T*>(a.h) + row * a.h_stride;
         const float mean = a.mean[row], rstd = a.rstd[row];
-        float sg = 0.0f, sgx = 0.0f;
-        for (int c = lane; c < a.width; c += TPR) {
-            const float g = load_as_float(a.dy, y0 + c, type) * (a.weight ? load_as_float(a.weight, c, weight_type) : 1.0f);
-            sg += g;
-            sgx += g * ((load_as_float(a.h, h0 + c, type) - mean) * rstd);
-        }
-        const float mg = loop_sum<TPR>(sg) / static_cast<float>(a.width), mgx = loop_sum<TPR>(sgx) / static_cast<float>(a.width);
-        for (int c = lane; c < a.width; c += TPR) {
-            const float g = load_as_float(a.dy, y0 + c, type) * (a.weight ? load_as_float(a.weight, c, weight_type) : 1.0f);
-            const float xhat = (load_as_float(a.h, h0 + c, type) - mean) * rstd;
-            float d = rstd * (g - mg - xhat * mgx);
-            if (a.dh) d += load_as_float(a.dh, row * a.dh_stride + c, type);
-            store_float(a.dx, row * a.dx_stride + c, d, type);
-        }
+        float sums[2] = {0.0f, 0.0f};
+        each_vector<V>(a.width, [&](int at, int shift) {
+            const Floats<V> d = floats<T, V>(load_raw<V>(pd + at)), h = floats<T, V>(load_raw<V>(ph + at));
+            const Floats<V> w = load_weights<T, V>(a.weight, at, float_weights, 1.0f);
+#pragma unroll
+            for (int e = 0; e < V; e++) {
+                const float g = e >= shift ? d[e] * w[e] : 0.0f;
+                sums[0] += g;
+                if (e >= shift) sums[1] = __builtin_fmaf(g, (h[e] - mean) * rstd, sums[1]);
+            }
+        });
+        row_sums<kWideBlock>(sums);
+        const float mg = sums[0] / static_cast<float>(a.width), mgx = sums[1] / static_cast<float>(a.width);
+        each_vector<V>(a.width, [&](int at, int) {
+            Floats<V> d = floats<T, V>(load_raw<V>(pd + at));
+            const Floats<V> h = floats<T, V>(load_raw<V>(ph + at)), w = load_weights<T, V>(a.weight, at, float_weights, 1.0f);
+#pragma unroll
+            for (int e = 0; e < V; e++) d[e] = rstd * __builtin_fmaf(-(h[e] - mean) * rstd, mgx, d[e] * w[e] - mg);
+            if (a.dh) d += floats<T, V>(load_raw<V>(static_cast<const T*>(a.dh) + row * a.dh_stride + at));
+            store_raw<V>(static_cast<T*>(a.dx) + row * a.dx_stride + at, raw<T, V>(d));
+        });
     }
 }
 
-// Column sums of a slab of rows (blockIdx.y): a thread per column, or with few columns `share` threads for each.
-__global__ void __launch_bounds__(kBlock) k_norm_columns(NormBwdArgs a, int slabs, int share, int type) {
-    __shared__ float part[2][kBlock];
-    const int per = kBlock / share, lane = threadIdx.x % per, group = threadIdx.x / per;
-    const int64_t c = blockIdx.x * int64_t{per} + lane;
+// Column sums of a slab of rows (blockIdx.y), a thread per vector of columns.
+template <class T>
+__global__ void __launch_bounds__(kBlock) k_norm_columns(NormBwdArgs a, int slabs) {
+    constexpr int V = 16 / sizeof(T);
+    const int c = (blockIdx.x * kBlock + threadIdx.x) * V, at = min(c, a.width - V);
+    if (c >= a.width) return;
     const int64_t r0 = a.rows * blockIdx.y / slabs, r1 = a.rows * (blockIdx.y + 1) / slabs;
-    float dw = 0.0f, db = 0.0f;
-    if (c < a.width)
-        for (int64_t r = r0 + group; r < r1; r += share) {
-            const float d = load_as_float(a.dy, r * a.dy_stride + c, type);
-            dw += d * ((load_as_float(a.h, r * a.h_stride + c, type) - a.mean[r]) * a.rstd[r]);
-            db += d;
+    Floats<V> dw = Floats<V>(0.0f), db = Floats<V>(0.0f);
+#pragma unroll 4
+    for (int64_t r = r0; r < r1; r++) {
+        const Floats<V> d = floats<T, V>(load_raw<V>(static_cast<const T*>(a.dy) + r * a.dy_stride + at));
+        const Floats<V> h = floats<T, V>(load_raw<V>(static_cast<const T*>(a.h) + r * a.h_stride + at));
+        const float mean = a.mean[r], rstd = a.rstd[r];
+#pragma unroll
+        for (int e = 0; e < V; e++) {
+            dw[e] = __builtin_fmaf(d[e], (h[e] - mean) * rstd, dw[e]);
+            db[e] += d[e];
         }
-    part[0][threadIdx.x] = dw;
-    part[1][threadIdx.x] = db;
-    __syncthreads();
-    if (group || c >= a.width) return;
-    for (int g = 1; g < share; g++) {
-        dw += part[0][g * per + lane];
-        db += part[1][g * per + lane];
     }
-    a.partial[int64_t{blockIdx.y} * 2 * a.width + c] = dw;
-    a.partial[(int64_t{blockIdx.y} * 2 + 1) * a.width + c] = db;
+    // (columns that two vectors hold have the same sums in both)
+    store_raw<V>(a.partial + int64_t{blockIdx.y} * 2 * a.width + at, dw);
+    store_raw<V>(a.partial + (int64_t{blockIdx.y} * 2 + 1) * a.width + at, db);
 }
 
 // ---- which kernel --------------------------------------------------------------------------------------------
 
 struct Split {
-    int threads, vectors;  // of a row, and of a thread; 0 vectors: a loop over the row
-    int rows;              // that a thread works on at a time
+    int vec;      // elements of a vector; 0: a loop over the row
+    int most;     // threads of a row as the kernel is compiled: a power of two up to a wave, or the most of a workgroup
+    int threads;  // of a row
+    int vectors;  // of a thread
+    int rows;     // that a thread works on at a time
+    int block_rows() const { return most <= kWave ? kBlock / most : 1; }
+    int block() const { return most <= kWave ? kBlock : threads; }
 };
-// A vector a thread up to 1024 threads: of the splits that hold a row this one was the fastest or within 3 % throughout
-// (16,383 x 2048 half, backward: a workgroup of 256 40 us, 128 threads of two vectors 44, a wave of four 57; 1 M x 48
-// bfloat16, forward: 8 threads 36 us, 2 of three vectors 37). Two rows at a time where they fit the registers: the loads of
-// one alone do not cover the memory's latency (2 M x 96, forward: 133 us against 161; four rows 131). Wider rows take 512
-// threads of up to four vectors, as many as the backward's sums leave registers for (4000 x 16,000 half, backward: 144 us,
-// 1024 threads of two 198).
-Split split_of(int64_t width, int vec) {
-    if (width < vec) return {1, 0, 1};
+// A vector of 16 bytes a thread up to a workgroup: of the splits that hold a row this one was the fastest or within 3 %
+// throughout (16,383 x 2048 half, backward: a workgroup of 256 40 us, 128 threads of two vectors 44, a wave of four 57;
+// 1 M x 48 bfloat16, forward: 8 threads 36 us, 2 of three vectors 37). Rows of over a wave take as many whole waves as they
+// need (31,128 x 2056, forward: 5 waves 56 us, 8 would leave a third of them idle). Two rows at a time where they fit the
+// registers: the loads of one alone do not cover the memory's latency (2 M x 96, forward: 133 us against 161, four rows
+// 131; 31,128 x 2056: 56 against 76). From 513 vectors on the forward takes three or four a thread (15,621 x 4100: 56 us, two
+// 70, one 72), the backward, whose sums take the registers, only from 1025 on (10,666 x 6000: one 85 us, two 114, three 92).
+Split split_of(int64_t width, int size, bool backward) {
+    const int full = 16 / size, vec = width >= full ? full : width >= 4 ? 4 : 1;
     const int64_t n = (width + vec - 1) / vec;
-    int t = 1;
-    while (t < 1024 && t < n) t *= 2;
-    if (n <= t) return {t, 1, t <= 256 ? 2 : 1};
+    const auto waves = [](int64_t threads) { return static_cast<int>((threads + kWave - 1) / kWave * kWave); };
+    if (n <= (backward ? 1024 : 512)) {
+        int t = 1;
+        while (t < n) t *= 2;
+        return {vec, t, t <= kWave ? t : waves(n), 1, !backward || t <= 256 ? 2 : 1};
+    }
     for (int k : {3, 4})
-        if (n <= 512 * k) return {512, k, 1};
-    return {kBlock, 0, 1};
+        if (n <= 512 * k) return {vec, 512, waves((n + k - 1) / k), k, 1};
+    if (n <= 4096 && !backward) return {vec, 1024, waves((n + 3) / 4), 4, 1};
+    return {0, 0, kWideBlock, 0, 1};
 }
-// Rows side by side in a workgroup.
-int block_rows(const Split& s) { return s.threads <= kWave ? kBlock / s.threads : 1; }
 
-template <class T, int TPR, int K>
-void fwd(const NormFwdArgs& a, bool fw, int grid, hipStream_t s) {
-    constexpr int R = K == 1 && TPR <= 256 ? 2 : 1;
-    hipLaunchKernelGGL((k_norm_fwd<T, TPR, K, R>), dim3(grid), dim3(kThreadsOf<TPR>), 0, s, a, fw);
+template <class T, int V, int TPR, int K>
+void launch(const Split& sp, const NormFwdArgs& a, bool fw, int grid, hipStream_t s) {
+    constexpr int R = K == 1 ? 2 : 1;
+    hipLaunchKernelGGL((k_norm_fwd<T, V, TPR, K, R>), dim3(grid), dim3(sp.block()), 0, s, a, fw);
 }
-template <class T, int TPR, int K>
-void bwd(const NormBwdArgs& a, bool fw, int grid, hipStream_t s) {
+template <class T, int V, int TPR, int K>
+void launch(const Split& sp, const NormBwdArgs& a, bool fw, int grid, hipStream_t s) {
     constexpr int R = K == 1 && TPR <= 256 ? 2 : 1;
     // Rows of 256 threads or more, 16-byte aligned, go past the caches where a call moves more than half of what the last
     // one holds (256 MiB): 16,383 x 2048 36.5 us against 40.0. Within it they do not (33 against 36), nor where rows share
@@ -469,96 +491,102 @@ void bwd(const NormBwdArgs& a, bool fw, int grid, hipStream_t s) {
         const auto whole = [](const void* p, int64_t stride) { return (reinterpret_cast<uintptr_t>(p) | static_cast<uintptr_t>(stride) * sizeof(T)) % 16 == 0; };
         if (a.rows * a.width * static_cast<int64_t>(sizeof(T)) * (a.dh ? 4 : 3) > (int64_t{128} << 20) && whole(a.dy, a.dy_stride) &&
             whole(a.h, a.h_stride) && whole(a.dh, a.dh_stride)) {
-            hipLaunchKernelGGL((k_norm_bwd<T, TPR, K, R, true>), dim3(grid), dim3(kThreadsOf<TPR>), 0, s, a, fw);
+            hipLaunchKernelGGL((k_norm_bwd<T, V, TPR, K, R, true>), dim3(grid), dim3(sp.block()), 0, s, a, fw);
             return;
         }
     }
-    hipLaunchKernelGGL((k_norm_bwd<T, TPR, K, R, false>), dim3(grid), dim3(kThreadsOf<TPR>), 0, s, a, fw);
+    hipLaunchKernelGGL((k_norm_bwd<T, V, TPR, K, R, false>), dim3(grid), dim3(sp.block()), 0, s, a, fw);
 }
 
-#define SX_SPLIT(T, P, V)                                            \
-    if (sp.threads == P && sp.vectors == V) return DO(T, P, V)
-#define SX_SPLITS(T)                                                                                                  \
-    SX_SPLIT(T, 1, 1); SX_SPLIT(T, 2, 1); SX_SPLIT(T, 4, 1); SX_SPLIT(T, 8, 1); SX_SPLIT(T, 16, 1); SX_SPLIT(T, 32, 1);  \
-    SX_SPLIT(T, 64, 1); SX_SPLIT(T, 128, 1); SX_SPLIT(T, 256, 1); SX_SPLIT(T, 512, 1); SX_SPLIT(T, 1024, 1);              \
-    SX_SPLIT(T, 512, 3); SX_SPLIT(T, 512, 4)
-
-template <class T>
-void fwd_of(const Split& sp, const NormFwdArgs& a, bool fw, int grid, hipStream_t s) {
-#define DO(T, P, V) fwd<T, P, V>(a, fw, grid, s)
-    SX_SPLITS(T);
-#undef DO
-}
-template <class T>
-void bwd_of(const Split& sp, const NormBwdArgs& a, bool fw, int grid, hipStream_t s) {
-#define DO(T, P, V) bwd<T, P, V>(a, fw, grid, s)
-    SX_SPLITS(T);
-#undef DO
+template <class T, class Args>
+void launch_split(const Split& sp, const Args& a, bool fw, int grid, hipStream_t s) {
+    constexpr int F = 16 / sizeof(T);
+#define SX_SPLIT(V, P, K) \
+    if (sp.vec == V && sp.most == P && sp.vectors == K) return launch<T, V, P, K>(sp, a, fw, grid, s)
+    SX_SPLIT(F, 1, 1);
+    SX_SPLIT(F, 2, 1);
+    SX_SPLIT(F, 4, 1);
+    SX_SPLIT(F, 8, 1);
+    SX_SPLIT(F, 16, 1);
+    SX_SPLIT(F, 32, 1);
+    SX_SPLIT(F, 64, 1);
+    SX_SPLIT(F, 128, 1);
+    SX_SPLIT(F, 256, 1);
+    SX_SPLIT(F, 512, 1);
+    SX_SPLIT(F, 512, 3);
+    SX_SPLIT(F, 512, 4);
+    if constexpr (std::is_same_v<Args, NormBwdArgs>) {
+        SX_SPLIT(F, 1024, 1);
+    } else {
+        SX_SPLIT(F, 1024, 4);
+    }
+    SX_SPLIT(1, 1, 1);
+    SX_SPLIT(1, 2, 1);
+    SX_SPLIT(1, 4, 1);
+    if constexpr (F == 8) {
+        SX_SPLIT(4, 1, 1);
+        SX_SPLIT(4, 2, 1);
+    }
+#undef SX_SPLIT
+    throw std::logic_error("layer norm: a split without a kernel");
 }
 
 int grid_of(int64_t rows, int64_t per) {
     return static_cast<int>(std::max<int64_t>(std::min<int64_t>((rows + per - 1) / per, 1 << 20), 1));
 }
+int size_of(ElemType type) { return type == kF32 ? 4 : 2; }
 
 }  // namespace
 
+// f of the rows' type, by a value of it.
+template <class F>
+void with_type(ElemType type, F f) {
+    if (type == kF32) f(float{});
+    else if (type == kBf16) f(__bf16{});
+    else f(_Float16{});
+}
+
 void layer_norm_fwd(const NormFwdArgs& a, ElemType type, ElemType weight_type, hipStream_t s) {
     if (a.rows == 0) return;
-    const Split sp = split_of(a.width, type == kF32 ? 4 : 8);
+    const Split sp = split_of(a.width, size_of(type), false);
     const bool fw = weight_type == kF32;
-    const int grid = grid_of(a.rows, int64_t{block_rows(sp)} * sp.rows);
-    if (sp.vectors == 0) {
-        if (sp.threads == 1) hipLaunchKernelGGL(k_norm_fwd_loop<1>, dim3(grid), dim3(kBlock), 0, s, a, int{type}, int{weight_type});
-        else hipLaunchKernelGGL(k_norm_fwd_loop<kBlock>, dim3(grid), dim3(kBlock), 0, s, a, int{type}, int{weight_type});
-    } else if (type == kF32) {
-        fwd_of<float>(sp, a, fw, grid, s);
-    } else if (type == kBf16) {
-        fwd_of<__bf16>(sp, a, fw, grid, s);
-    } else {
-        fwd_of<_Float16>(sp, a, fw, grid, s);
-    }
+    with_type(type, [&](auto t) {
+        using T = decltype(t);
+        if (sp.vec) launch_split<T>(sp, a, fw, grid_of(a.rows, int64_t{sp.block_rows()} * sp.rows), s);
+        else hipLaunchKernelGGL(k_norm_fwd_wide<T>, dim3(grid_of(a.rows, 1)), dim3(kWideBlock), 0, s, a, fw);
+    });
 }
 
 // A workgroup's rows are as many as keep its partial sums (16 bytes a column, written and read) to a fraction of what it
-// reads, and as few as keep the memory busy: about 2^17 threads, half of them where three tensors are read, twice where a
-// row takes over 256 (1 M x 64 with dh: 256 workgroups 90 us, 512 98, 1024 107; 1 M x 45: 512 96, 1024 109; 4000 x 8000:
-// 256 of 1024 threads 51, 512 56, 1024 67). 32 MiB of partial sums at most.
+// reads, and as few as keep the memory busy: 512 threads on each of the 256 compute units, half of them where three tensors
+// are read, 1024 where a row takes over 256 (1 M x 64 with dh: 256 workgroups 90 us, 512 98, 1024 107; 1 M x 45: 512 96, 1024
+// 109; 4000 x 8000: 256 of 1024 threads 51, 512 56, 1024 67). As many on each unit: 341 workgroups of 768 threads, of which
+// a unit holds one, take as long as 512 would (10,666 x 6000: 126 us, 256 of them 85). 32 MiB of partial sums at most.
 int norm_bwd_slabs(int64_t rows, int64_t width, ElemType type, bool dh) {
-    const int size = type == kF32 ? 4 : 2;
-    const Split sp = split_of(width, 16 / size);
-    const int64_t per = sp.vectors ? int64_t{block_rows(sp)} * sp.rows : 64;
-    const int64_t threads = sp.threads > 256 ? 1 << 18 : sp.threads <= kWave && dh ? 1 << 16 : 1 << 17;
-    int64_t most = sp.vectors ? threads / (sp.threads <= kWave ? kBlock : sp.threads) : 1024;
-    most = std::min({most, std::max<int64_t>(rows * size * 3 / 128, 256), (int64_t{32} << 20) / (8 * width)});
-    return static_cast<int>(std::max<int64_t>(std::min((rows + per - 1) / per, most), 1));
+    const int size = size_of(type);
+    const Split sp = split_of(width, size, true);
+    const int64_t per = sp.vec ? int64_t{sp.block_rows()} * sp.rows : 16;
+    const int64_t threads = sp.most > 256 && sp.vectors == 1 ? 1024 : sp.most <= kWave && dh ? 256 : 512;  // of a unit
+    const int64_t most = kUnits * std::max<int64_t>(sp.vec ? std::min(threads / sp.block(), rows * size * 3 / 128 / kUnits) : 4, 1);
+    return static_cast<int>(std::max<int64_t>(std::min({(rows + per - 1) / per, most, (int64_t{32} << 20) / (8 * width)}), 1));
 }
 
 void layer_norm_bwd(const NormBwdArgs& args, ElemType type, ElemType weight_type, hipStream_t s) {
     NormBwdArgs a = args;
-    const int size = type == kF32 ? 4 : 2;
-    const Split sp = split_of(a.width, 16 / size);
+    const Split sp = split_of(a.width, size_of(type), true);
     const int slabs = norm_bwd_slabs(a.rows, a.width, type, a.dh != nullptr);
     const bool columns = a.dweight || a.dbias, fw = weight_type == kF32;
     if (!columns) a.partial = nullptr;
-    if (sp.vectors == 0 || a.rows == 0) {
-        if (a.dx && a.rows) {
-            const int grid = grid_of(a.rows, block_rows(sp));
-            if (sp.threads == 1) hipLaunchKernelGGL(k_norm_dx_loop<1>, dim3(grid), dim3(kBlock), 0, s, a, int{type}, int{weight_type});
-            else hipLaunchKernelGGL(k_norm_dx_loop<kBlock>, dim3(grid), dim3(kBlock), 0, s, a, int{type}, int{weight_type});
+    with_type(type, [&](auto t) {
+        using T = decltype(t);
+        if (sp.vec) {  // (without rows: sums of nothing)
+            launch_split<T>(sp, a, fw, slabs, s);
+            return;
         }
-        if (columns) {
-            int share = 1;
-            while (share < 32 && a.width * share * 2 <= kBlock) share *= 2;
-            const int per = kBlock / share;
-            hipLaunchKernelGGL(k_norm_columns, dim3((a.width + per - 1) / per, slabs), dim3(kBlock), 0, s, a, slabs, share, int{type});
-        }
-    } else if (type == kF32) {
-        bwd_of<float>(sp, a, fw, slabs, s);
-    } else if (type == kBf16) {
-        bwd_of<__bf16>(sp, a, fw, slabs, s);
-    } else {
-        bwd_of<_Float16>(sp, a, fw, slabs, s);
-    }
+        if (a.dx && a.rows) hipLaunchKernelGGL(k_norm_dx_wide<T>, dim3(grid_of(a.rows, 1)), dim3(kWideBlock), 0, s, a, fw);
+        const int per = kBlock * (16 / size_of(type));
+        if (columns) hipLaunchKernelGGL(k_norm_columns<T>, dim3((a.width + per - 1) / per, slabs), dim3(kBlock), 0, s, a, slabs);
+    });
     if (columns)
         hipLaunchKernelGGL(k_norm_join, dim3((2 * a.width + 15) / 16), dim3(kBlock), 0, s, a, slabs, int{weight_type});
 }

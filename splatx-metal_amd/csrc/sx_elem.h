@@ -19,58 +19,45 @@ __device__ inline void store_float(void* p, int64_t i, float v, int type) {
     else static_cast<_Float16*>(p)[i] = static_cast<_Float16>(v);
 }
 
-// 16 bytes of elements. The address need only be aligned to an element: the GPU runs in unaligned access mode.
-template <class T>
-constexpr int kVec = 16 / sizeof(T);
-template <class T>
-using Vec = T __attribute__((ext_vector_type(kVec<T>)));
-template <class T>
-using Floats = float __attribute__((ext_vector_type(kVec<T>)));
+// V elements side by side. The address need only be aligned to one of them: the GPU runs in unaligned access mode.
+template <class T, int V>
+using Vec = T __attribute__((ext_vector_type(V)));
+template <int V>
+using Floats = float __attribute__((ext_vector_type(V)));
 
+// ONCE: what is not read again before the caches have turned over goes past them.
+template <int V, bool ONCE = false, class T>
+__device__ inline Vec<T, V> load_raw(const T* p) {
+    using At = Vec<T, V> __attribute__((aligned(sizeof(T))));
+    if constexpr (ONCE) return __builtin_nontemporal_load(reinterpret_cast<const At*>(p));
+    return *reinterpret_cast<const At*>(p);
+}
+template <int V, bool ONCE = false, class T>
+__device__ inline void store_raw(T* p, Vec<T, V> v) {
+    using At = Vec<T, V> __attribute__((aligned(sizeof(T))));
+    if constexpr (ONCE) __builtin_nontemporal_store(v, reinterpret_cast<At*>(p));
+    else *reinterpret_cast<At*>(p) = v;
+}
+template <class T, int V>
+__device__ inline Floats<V> floats(Vec<T, V> v) {
+    return __builtin_convertvector(v, Floats<V>);
+}
+template <class T, int V>
+__device__ inline Vec<T, V> raw(Floats<V> f) {
+    return __builtin_convertvector(f, Vec<T, V>);
+}
 // The elements as they are, where the compiler would keep their floats since their last use: half the registers for a
 // conversion again.
-template <class T>
-__device__ inline Floats<T> floats_again(Vec<T>& v) {
-    if constexpr (sizeof(T) == 2) {
+template <class T, int V>
+__device__ inline Floats<V> floats_again(Vec<T, V>& v) {
+    if constexpr (sizeof(v) == 16 && sizeof(T) == 2) {
         using Words = uint32_t __attribute__((ext_vector_type(4)));
         Words w;
         __builtin_memcpy(&w, &v, sizeof(w));
         asm volatile("" : "+v"(w));
         __builtin_memcpy(&v, &w, sizeof(w));
     }
-    return __builtin_convertvector(v, Floats<T>);
-}
-template <class T>
-__device__ inline Vec<T> load_raw(const T* p) {
-    Vec<T> v;
-    __builtin_memcpy(&v, p, sizeof(v));
-    return v;
-}
-// ONCE: what is not read again before the caches have turned over goes past them.
-template <bool ONCE, class T>
-__device__ inline Vec<T> load_rows(const T* p) {
-    if constexpr (!ONCE) return load_raw(p);
-    using At = uint32_t __attribute__((ext_vector_type(4), aligned(sizeof(T))));
-    const uint32_t __attribute__((ext_vector_type(4))) w = __builtin_nontemporal_load(reinterpret_cast<const At*>(p));
-    Vec<T> v;
-    __builtin_memcpy(&v, &w, sizeof(v));
-    return v;
-}
-template <class T>
-__device__ inline void store_raw(T* p, Vec<T> v) {
-    __builtin_memcpy(p, &v, sizeof(v));
-}
-template <class T>
-__device__ inline Floats<T> floats(Vec<T> v) {
-    return __builtin_convertvector(v, Floats<T>);
-}
-template <class T>
-__device__ inline Vec<T> raw(Floats<T> f) {
-    return __builtin_convertvector(f, Vec<T>);
-}
-template <class T>
-__device__ inline Floats<T> load_vec(const T* p) {
-    return floats<T>(load_raw(p));
+    return floats<T, V>(v);
 }
 
 // A value of another lane by data-parallel primitives; every lane of the wave takes part.
