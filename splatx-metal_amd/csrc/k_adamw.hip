@@ -144,12 +144,15 @@ __device__ inline void store_param(const AdamTensor& a, int64_t i, Floats<E> p) 
     else store_few<E, ONCE>(static_cast<_Float16*>(a.param), i, a.n, p);
 }
 
-// The square root to nearest for x of 2^-100 or more, by one correction of the approximate one with the remainder of its
-// square (Markstein): 8 instructions where the library's takes 15, which the 8-bit step would wait for.
+// The square root to nearest, by one correction of the approximate one with the remainder of its square (Markstein): 12
+// instructions where the library's takes 18. Small x goes through it times 2^64: the remainder, 2^-24 of x, has to be a
+// normal number, and so has x for the hardware's reciprocal root.
 __device__ inline float root(float x) {
-    const float y = __builtin_amdgcn_rsqf(x), s = x * y;
-    const float r = __builtin_fmaf(0.5f * y, __builtin_fmaf(-s, s, x), s);
-    return x > 0.0f && x < __builtin_inff() ? r : x;  // (0, infinity and NaN are their own)
+    const bool small = x < 0x1p-96f;
+    const float z = small ? x * 0x1p64f : x;
+    const float y = __builtin_amdgcn_rsqf(z), s = z * y;
+    const float r = __builtin_fmaf(0.5f * y, __builtin_fmaf(-s, s, z), s);
+    return x > 0.0f && x < __builtin_inff() ? (small ? r * 0x1p-32f : r) : x;  // (0, infinity and NaN are their own)
 }
 
 // The moments after this gradient, the second one's root, and the parameter after its step. The quotient is off by 2 units

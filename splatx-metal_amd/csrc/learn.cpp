@@ -375,9 +375,9 @@ int32_t sxh_adamw(sxh_backend* b, const sxh_adamw_tensor* tensors, int64_t n_ten
         const double step = static_cast<double>(p->step);
         t.root_c2 = static_cast<float>(1.0 / std::sqrt(1.0 - std::pow(p->b2, step)));
         const double by = 1.0 / (1.0 - std::pow(p->b1, step));
-        constexpr size_t kCacheBytes = size_t{256} << 20;  // of the last-level cache
+        constexpr size_t kKept = size_t{128} << 20;  // half of the last-level cache
         auto flush = [&] {
-            sxk::adamw(t, eight, total > kCacheBytes, on.stream());
+            sxk::adamw(t, eight, total > kKept, on.stream());
             t.tensors = 0;
         };
         constexpr int64_t kMostChunks = int64_t{1} << 30;  // of a launch

@@ -80,6 +80,15 @@ for _packed, _struct in ((_QUEUE, Queue), (_NORM_IN, LayerNormInputs), (_NORM_OU
                          (_GRADS, LayerNormGrads), (_NORM_ROW, NormTensor), (_ADAMW_ROW, AdamWTensor), (_ADAMW, AdamWParams)):
     assert _packed.size == C.sizeof(_struct), _struct
 
+
+
+def _pack(layout, *values):
+    try:
+        return layout.pack(*values)
+    except struct.error as e:
+        raise sh.SxInvalidArgument(f"not a number of the range: {e}") from None
+
+
 _is_contiguous = torch.Tensor.is_contiguous
 _numel = torch.Tensor.numel
 _ptr = torch.Tensor.data_ptr
@@ -160,7 +169,7 @@ class TorchBackend(sh.Backend):
 
     def _like(self, t):
         """Contiguous rows like t's."""
-        return torch.empty_like(t) if t.is_contiguous() else _empty(t.shape, dtype=t.dtype, device=self.device)
+        return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
 
     # -- layer norm ------------------------------------------------------------------------------------
     def layer_norm_fwd(self, x, weight=None, bias=None, eps=1e-5, residual=None, stats=True):
@@ -180,11 +189,11 @@ class TorchBackend(sh.Backend):
         mean = rstd = None
         m = s = 0
         if stats:
-            mean = _empty(x.shape[:-1], dtype=torch.float32, device=self.device)
+            mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
             rstd = torch.empty_like(mean)
             m, s = mean.data_ptr(), rstd.data_ptr()
         self._enqueue("layer_norm_fwd",
-                      _NORM_IN.pack(x2.data_ptr(), r, w, b, rows, width, x_stride, r_stride, eps, TYPES[t], TYPES[wt]),
+                      _pack(_NORM_IN, x2.data_ptr(), r, w, b, rows, width, x_stride, r_stride, eps, TYPES[t], TYPES[wt]),
                       _NORM_OUT.pack(y.data_ptr(), h.data_ptr() if r else 0, m, s, width, width))
         return y, h, mean, rstd
 
@@ -209,13 +218,13 @@ class TorchBackend(sh.Backend):
             dx_ptr = dx.data_ptr()
         if want_dweight or want_dbias:
             if want_dweight:
-                dweight = _empty(width, dtype=wt, device=self.device)
+                dweight = h.new_empty(width, dtype=wt)
                 dweight_ptr = dweight.data_ptr()
             if want_dbias:
-                dbias = _empty(width, dtype=wt, device=self.device)
+                dbias = h.new_empty(width, dtype=wt)
                 dbias_ptr = dbias.data_ptr()
             bytes_ = self._ops["layer_norm_bwd_workspace"](rows, width)
-            work = _empty(bytes_, dtype=torch.uint8, device=self.device)
+            work = h.new_empty(bytes_, dtype=torch.uint8)
             work_ptr = work.data_ptr()
         self._enqueue("layer_norm_bwd",
                       _GRADS_IN.pack(dy.data_ptr(), h2.data_ptr(), dh_ptr, m, s, w, rows, width, dy_stride, h_stride, dh_stride,
@@ -283,9 +292,12 @@ class TorchBackend(sh.Backend):
         if len(lrs) != n or len(decays) != n:
             raise sh.SxInvalidArgument("lr and weight_decay are a number, or one for each tensor")
         norm = self._vector(grad_norm, "grad_norm", 1, _FLOAT) if grad_norm is not None else 0
-        table = b"".join(map(_ADAMW_ROW.pack, param_ptrs, master_ptrs, grad_ptrs, m, v, m_scale, v_scale, sizes, lrs, decays,
-                             map(TYPES.__getitem__, param_types), map(TYPES.__getitem__, grad_types)))
-        self._enqueue("adamw", table, n, _ADAMW.pack(step, seed, b1, b2, eps, norm, max_norm, grad_scale, 8 if eight else 32))
+        try:
+            table = b"".join(map(_ADAMW_ROW.pack, param_ptrs, master_ptrs, grad_ptrs, m, v, m_scale, v_scale, sizes, lrs, decays,
+                                 map(TYPES.__getitem__, param_types), map(TYPES.__getitem__, grad_types)))
+        except struct.error:
+            raise sh.SxInvalidArgument("lr and weight_decay must be numbers") from None
+        self._enqueue("adamw", table, n, _pack(_ADAMW, step, seed, b1, b2, eps, norm, max_norm, grad_scale, 8 if eight else 32))
 
     @staticmethod
     def _same(got, want, name):

@@ -433,6 +433,32 @@ def test_adamw8_blocks_of_nothing_and_values_not_finite(tb):
     assert not mc.any() and not rc.any() and not ms.any() and not rs.any()
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_second_moments_down_to_the_least_float(tb, bits):
+    """Elements without gradients for long: their second moments decay through the subnormal numbers to zero, and no root of
+    one is anything but small."""
+    v = torch.tensor([2.0 ** -e for e in range(60, 150)] + [0.0, 1e-38, 1.1754942e-38, 1.4e-45, 3e-42])
+    n = v.numel()
+    p, g, m = randn(n, seed=1), torch.zeros(n), torch.zeros(n)
+    if bits == 32:
+        d = [t.cuda() for t in (p, g, m, v)]
+        tb.adamw_step([d[0]], [d[1]], [d[2]], [d[3]], step=9, lr=1e-3, **{**HYPER, "eps": 1e-20})
+        new = ref.adamw(p, g, m, v, step=9, lr=1e-3, weight_decay=0.0, **{**HYPER, "eps": 1e-20})
+        within(d[3], new[2], 4 * ref.U32 * new[2] + 3e-45, "v")
+        got = d[0].cpu()
+    else:  # the gradients that give these moments, in blocks of their own size
+        g = (v.double() / 1e-3).sqrt().float()
+        _, codes, scale = coded([m])
+        d = [t.cuda() for t in (p, g, codes[0], codes[0], scale[0], scale[0])]
+        tb.adamw_step([d[0]], [d[1]], [d[2]], [d[3]], step=9, lr=1e-30, exp_avg_scale=[d[4]], exp_avg_sq_scale=[d[5]], **HYPER)
+        root = v.double().sqrt()
+        codes, _ = ref.encode(root, ref.random_bits(0, 9, 0, n) >> 16, True)
+        same_codes(d[3][v > 1e-37], codes[v > 1e-37], "exp_avg_sq")
+        assert (d[3].cpu().view(torch.uint8) < 0x7F).all()
+        got = d[0].cpu()
+    assert torch.equal(got, p)
+
+
 def test_adamw8_moments_follow_a_steady_gradient(tb):
     """200 steps of one gradient per element: the moments' averages over elements of one size go where the exact ones go,
     though a step of the second moment moves a root by a twentieth of the codes' distance: to nearest it would not move."""
@@ -625,6 +651,10 @@ def test_refusals(tb):
         f([p], [g], [m.bfloat16()], [v])
     with bad:
         f([p], [g], [m], [v], exp_avg_scale=[v[:1]])
+    with bad:
+        f([p], [g], [m], [v], seed=-1)
+    with bad:
+        f([p], [g], [m], [v], lr=None)
     with bad:
         tb.grad_norm([p.double()])
     with bad:
