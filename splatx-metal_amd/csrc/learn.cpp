@@ -23,8 +23,8 @@ void need_type(const char* what, uint8_t t, const char* name) {
 }
 
 // The device memory of a call: each range a caller names lies in an allocation of the backend's device. (A lookup is
-// 0.16 us; the buffers of a network mostly lie in one allocation of its framework's allocator, so the last one found
-// is tried first.)
+// 0.16 us; the buffers of a network mostly lie in a few allocations of its framework's allocator, so the last eight found
+// in this call are tried first.)
 class DeviceMemory {
   public:
     DeviceMemory(const char* what, int device) : what_(what), device_(device) {}
@@ -32,7 +32,8 @@ class DeviceMemory {
         if (!p) invalid(what_, std::string("null ") + name);
         const auto at = reinterpret_cast<uintptr_t>(p);
         if (at % align) invalid(what_, std::string(name) + " is not aligned to its elements");
-        if (at >= base_ && at - base_ <= size_ && bytes <= size_ - (at - base_)) return;
+        for (const Range& r : found_)
+            if (at >= r.base && at - r.base <= r.size && bytes <= r.size - (at - r.base)) return;
         hipPointerAttribute_t attr{};
         if (hipPointerGetAttributes(&attr, p) != hipSuccess || attr.type != hipMemoryTypeDevice || attr.device != device_) {
             (void)hipGetLastError();  // an unknown host pointer leaves an error behind; it is reported here
@@ -44,17 +45,22 @@ class DeviceMemory {
             (void)hipGetLastError();
             invalid(what_, std::string(name) + ": the allocation holding it is unknown");
         }
-        base_ = reinterpret_cast<uintptr_t>(base);
-        size_ = size;
-        if (at - base_ > size_ || bytes > size_ - (at - base_))
+        const Range r{reinterpret_cast<uintptr_t>(base), size};
+        found_[next_++ % kFound] = r;
+        if (at - r.base > r.size || bytes > r.size - (at - r.base))
             invalid(what_, std::string(name) + " ends outside its allocation (" + std::to_string(bytes) + " bytes needed)");
     }
 
   private:
+    struct Range {
+        uintptr_t base = 0;
+        size_t size = 0;
+    };
+    static constexpr unsigned kFound = 8;
     const char* what_;
     int device_;
-    uintptr_t base_ = 0;
-    size_t size_ = 0;
+    Range found_[kFound];
+    unsigned next_ = 0;
 };
 
 // Rows of `width` bytes, `stride` bytes apart.
