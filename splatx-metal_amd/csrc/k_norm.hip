@@ -77,6 +77,58 @@ __device__ inline void row_sums(float (&v)[N]) {
     }
 }
 
+// A vector's sum, in pairs.
+template <class F>
+__device__ inline float whole(F v) {
+    constexpr int V = sizeof(F) / sizeof(float);
+    float s[V];
+#pragma unroll
+    for (int e = 0; e < V; e++) s[e] = v[e];
+#pragma unroll
+    for (int w = V / 2; w; w /= 2)
+#pragma unroll
+        for (int e = 0; e < w; e++) s[e] += s[e + w];
+    return s[0];
+}
+
+// Its squares' sum.
+template <class F>
+__device__ inline float squares(F v) {
+    float s = 0.0f;
+#pragma unroll
+    for (int e = 0; e < static_cast<int>(sizeof(F) / sizeof(float)); e++) s = __builtin_fmaf(v[e], v[e], s);
+    return s;
+}
+
+// 1 / sqrt(x) of x > 0: the hardware's and one step of Newton's method, within a unit in the last place (the library's root
+// and quotient take 25 instructions more, a tenth of what a narrow row takes). Small x goes through it times 2^64.
+__device__ inline float inverse_root(float x) {
+    const bool small = x < 0x1p-96f;
+    const float z = small ? x * 0x1p64f : x;
+    float y = __builtin_amdgcn_rsqf(z);
+    if (z < __builtin_inff()) y = y * __builtin_fmaf(-0.5f * z * y, y, 1.5f);
+    return small ? y * 0x1p32f : y;
+}
+
+// A thread's vector between the passes over it: one alone as floats, of several each as it came, which takes half the
+// registers (of 16-bit elements) and a conversion for each pass.
+template <class T, int V, int K>
+struct Kept {
+    Vec<T, V> v;
+    __device__ void operator=(Vec<T, V> from) { v = from; }
+    __device__ Floats<V> get() { return floats_again<T, V>(v); }
+    __device__ Floats<V> minus(float mean) { return get() - mean; }
+    __device__ Floats<V> centred(float mean) { return get() - mean; }  // after minus(mean)
+};
+template <class T, int V>
+struct Kept<T, V, 1> {
+    Floats<V> v;
+    __device__ void operator=(Vec<T, V> from) { v = floats<T, V>(from); }
+    __device__ Floats<V> get() const { return v; }
+    __device__ Floats<V> minus(float mean) { return v = v - mean; }
+    __device__ Floats<V> centred(float) const { return v; }
+};
+
 template <class T, int V>
 __device__ inline Floats<V> load_weights(const void* w, int at, bool is_float, float none) {
     if (!w) return Floats<V>(none);
@@ -100,38 +152,43 @@ __global__ void __launch_bounds__(kThreadsOf<TPR>) k_norm_fwd(NormFwdArgs a, boo
     }
     const float inv_width = 1.0f / static_cast<float>(a.width);
     const int group = TPR > kWave ? 0 : threadIdx.x / TPR;
+    const bool tail = a.width % V != 0;
     for (int64_t first = blockIdx.x * int64_t{kRows * R}; first < a.rows; first += int64_t{gridDim.x} * (kRows * R)) {
-        const int64_t row0 = first + group;  // and every kRows-th after it: a load of the workgroup's covers rows side by side
-        Vec<T, V> x[R][K];
+        // the thread's rows are `group` and every kRows-th after it: a load of the workgroup's covers rows side by side. In
+        // place of rows there are not the last one is read.
+        const int left = static_cast<int>(min(a.rows - first, int64_t{kRows * R}));
+        int row[R];
+        Kept<T, V, K> x[R][K];
         float sum[R], sq[R];
+        const T* px = static_cast<const T*>(a.x) + first * a.x_stride;
 #pragma unroll
         for (int r = 0; r < R; r++) {
-            const T* px = static_cast<const T*>(a.x) + min(row0 + r * kRows, a.rows - 1) * a.x_stride;
+            row[r] = min(group + r * kRows, left - 1);
 #pragma unroll
-            for (int k = 0; k < K; k++) x[r][k] = load_raw<V>(px + p.at[k]);
+            for (int k = 0; k < K; k++) x[r][k] = load_raw<V>(px + row[r] * a.x_stride + p.at[k]);
         }
         if (a.residual) {
+            const T* pr = static_cast<const T*>(a.residual) + first * a.residual_stride;
+            T* ph = static_cast<T*>(a.h) + first * a.h_stride;
 #pragma unroll
-            for (int r = 0; r < R; r++) {
-                const int64_t row = min(row0 + r * kRows, a.rows - 1);
-                const T* pr = static_cast<const T*>(a.residual) + row * a.residual_stride;
-                T* ph = static_cast<T*>(a.h) + row * a.h_stride;
+            for (int r = 0; r < R; r++)
 #pragma unroll
                 for (int k = 0; k < K; k++) {
-                    x[r][k] = raw<T, V>(floats<T, V>(x[r][k]) + floats<T, V>(load_raw<V>(pr + p.at[k])));
-                    if (p.mine[k] && row0 + r * kRows < a.rows) store_raw<V>(ph + p.at[k], x[r][k]);
+                    const Vec<T, V> h = raw<T, V>(x[r][k].get() + floats<T, V>(load_raw<V>(pr + row[r] * a.residual_stride + p.at[k])));
+                    x[r][k] = h;
+                    if (p.mine[k] && group + r * kRows < left) store_raw<V>(ph + row[r] * a.h_stride + p.at[k], h);
                 }
-            }
         }
 #pragma unroll
         for (int r = 0; r < R; r++) {
             sum[r] = 0.0f;
 #pragma unroll
-            for (int k = 0; k < K; k++) {
-                const Floats<V> v = floats<T, V>(x[r][k]);
+            for (int k = 0; k < K - 1; k++) sum[r] += whole(x[r][k].get());
+            const Floats<V> v = x[r][K - 1].get();
+            if (tail)
 #pragma unroll
-                for (int e = 0; e < V; e++) sum[r] = k == K - 1 ? __builtin_fmaf(v[e], p.mask[e], sum[r]) : sum[r] + v[e];
-            }
+                for (int e = 0; e < V; e++) sum[r] = __builtin_fmaf(v[e], p.mask[e], sum[r]);
+            else sum[r] = __builtin_fmaf(whole(v), p.mask[V - 1], sum[r]);
         }
         row_sums<TPR>(sum);
 #pragma unroll
@@ -140,35 +197,37 @@ __global__ void __launch_bounds__(kThreadsOf<TPR>) k_norm_fwd(NormFwdArgs a, boo
             sq[r] = 0.0f;
 #pragma unroll
             for (int k = 0; k < K; k++) {
-                const Floats<V> v = floats_again<T, V>(x[r][k]);
+                const Floats<V> d = x[r][k].minus(sum[r]);
+                if (k < K - 1) {
+                    sq[r] += squares(d);
+                } else if (tail) {
 #pragma unroll
-                for (int e = 0; e < V; e++) {
-                    const float d = v[e] - sum[r];
-                    sq[r] = __builtin_fmaf(k == K - 1 ? d * p.mask[e] : d, d, sq[r]);
+                    for (int e = 0; e < V; e++) sq[r] = __builtin_fmaf(d[e] * p.mask[e], d[e], sq[r]);
+                } else {
+                    sq[r] = __builtin_fmaf(squares(d), p.mask[V - 1], sq[r]);
                 }
             }
         }
         row_sums<TPR>(sq);
+        T* py = static_cast<T*>(a.y) + first * a.y_stride;
 #pragma unroll
         for (int r = 0; r < R; r++) {
-            if (row0 + r * kRows >= a.rows) break;
-            const int64_t row = row0 + r * kRows;
-            const float rstd = 1.0f / __builtin_sqrtf(sq[r] * inv_width + a.eps), at_zero = -sum[r] * rstd;
-            T* py = static_cast<T*>(a.y) + row * a.y_stride;
+            if (group + r * kRows >= left) break;
+            const float rstd = inverse_root(__builtin_fmaf(sq[r], inv_width, a.eps));
 #pragma unroll
             for (int k = 0; k < K; k++) {
                 if constexpr (K > 1) {
                     w = load_weights<T, V>(a.weight, p.at[k], float_weights, 1.0f);
                     b = load_weights<T, V>(a.bias, p.at[k], float_weights, 0.0f);
                 }
-                Floats<V> y = floats_again<T, V>(x[r][k]);
+                Floats<V> y = x[r][k].centred(sum[r]);
 #pragma unroll
-                for (int e = 0; e < V; e++) y[e] = __builtin_fmaf(__builtin_fmaf(y[e], rstd, at_zero), w[e], b[e]);
-                if (p.mine[k]) store_raw<V>(py + p.at[k], raw<T, V>(y));
+                for (int e = 0; e < V; e++) y[e] = __builtin_fmaf(y[e] * rstd, w[e], b[e]);
+                if (p.mine[k]) store_raw<V>(py + row[r] * a.y_stride + p.at[k], raw<T, V>(y));
             }
             if (a.mean && (TPR > kWave ? threadIdx.x : threadIdx.x % TPR) == 0) {
-                a.mean[row] = sum[r];
-                a.rstd[row] = rstd;
+                a.mean[first + row[r]] = sum[r];
+                a.rstd[first + row[r]] = rstd;
             }
         }
     }
@@ -182,8 +241,12 @@ template <class T, int V, int TPR, int K, int R, bool ONCE>
 __global__ void __launch_bounds__(kThreadsOf<TPR>) k_norm_bwd(NormBwdArgs a, bool float_weights) {
     constexpr int kRows = kRowsOf<TPR>;
     const Place<V, TPR, K> p(a.width);
-    Floats<V> w, dw[K], db[K];
-    if constexpr (K == 1) w = load_weights<T, V>(a.weight, p.at[0], float_weights, 1.0f);
+    Floats<V> w, counted, dw[K], db[K];  // counted: the weights of the columns that are the thread's own, else 0
+    const auto load_weights_of = [&](int k) {
+        counted = w = load_weights<T, V>(a.weight, p.at[k], float_weights, 1.0f);
+        if (k == K - 1) counted = w * p.mask;
+    };
+    if constexpr (K == 1) load_weights_of(0);
 #pragma unroll
     for (int k = 0; k < K; k++) dw[k] = db[k] = Floats<V>(0.0f);
     const float inv_width = 1.0f / static_cast<float>(a.width);
@@ -192,33 +255,37 @@ __global__ void __launch_bounds__(kThreadsOf<TPR>) k_norm_bwd(NormBwdArgs a, boo
         Vec<T, V> dy[R][K], x[R][K], dh[R][K];
         float mean[R], rstd[R];
     };
+    // rows first + group and every kRows-th after it; in place of rows there are not the last one
     const auto load = [&](Rows& to, int64_t first) {
+        const int left = static_cast<int>(min(a.rows - first, int64_t{kRows * R}));
+        const T* pd = static_cast<const T*>(a.dy) + first * a.dy_stride;
+        const T* ph = static_cast<const T*>(a.h) + first * a.h_stride;
+        int row[R];
 #pragma unroll
         for (int r = 0; r < R; r++) {
-            const int64_t row = min(first + group + r * kRows, a.rows - 1);
-            const T* pd = static_cast<const T*>(a.dy) + row * a.dy_stride;
-            const T* ph = static_cast<const T*>(a.h) + row * a.h_stride;
-            to.mean[r] = a.mean[row];
-            to.rstd[r] = a.rstd[row];
+            row[r] = min(group + r * kRows, left - 1);
+            to.mean[r] = (a.mean + first)[row[r]];
+            to.rstd[r] = (a.rstd + first)[row[r]];
 #pragma unroll
             for (int k = 0; k < K; k++) {
-                to.dy[r][k] = load_raw<V, ONCE>(pd + p.at[k]);
-                to.x[r][k] = load_raw<V, ONCE>(ph + p.at[k]);
+                to.dy[r][k] = load_raw<V, ONCE>(pd + row[r] * a.dy_stride + p.at[k]);
+                to.x[r][k] = load_raw<V, ONCE>(ph + row[r] * a.h_stride + p.at[k]);
             }
         }
-        if (a.dh)
+        if (a.dh) {
+            const T* pdh = static_cast<const T*>(a.dh) + first * a.dh_stride;
 #pragma unroll
             for (int r = 0; r < R; r++)
 #pragma unroll
-                for (int k = 0; k < K; k++)
-                    to.dh[r][k] = load_raw<V, ONCE>(static_cast<const T*>(a.dh) + min(first + group + r * kRows, a.rows - 1) * a.dh_stride + p.at[k]);
+                for (int k = 0; k < K; k++) to.dh[r][k] = load_raw<V, ONCE>(pdh + row[r] * a.dh_stride + p.at[k]);
+        }
     };
     const int64_t stride = int64_t{gridDim.x} * (kRows * R);
     constexpr bool kAhead = K == 1;  // the next rows are on their way while these are worked on
     Rows next;
     if (kAhead && a.rows) load(next, blockIdx.x * int64_t{kRows * R});
     for (int64_t first = blockIdx.x * int64_t{kRows * R}; first < a.rows; first += stride) {
-        const int64_t row0 = first + group;  // and every kRows-th after it: a load of the workgroup's covers rows side by side
+        const int left = static_cast<int>(min(a.rows - first, int64_t{kRows * R}));
         Rows now;
         if constexpr (kAhead) {
             now = next;
@@ -226,49 +293,49 @@ __global__ void __launch_bounds__(kThreadsOf<TPR>) k_norm_bwd(NormBwdArgs a, boo
         } else {
             load(now, first);
         }
-        auto &dy = now.dy, &x = now.x;
-        const auto &mean = now.mean, &rstd = now.rstd;
+        // With c = h - mean and sums S = sum g, S' = sum g c over the row: xhat = c rstd,
+        // dx = rstd g - (rstd S + rstd^3 S' c) / width, and dweight gets dy c rstd: what a row multiplies is kept out of the
+        // elements' arithmetic.
+        Kept<T, V, K> dy[R][K], c[R][K];
         float sums[2 * R];
 #pragma unroll
         for (int r = 0; r < R; r++) {
-            if (row0 + r * kRows >= a.rows)  // read in place of a row there is not
-#pragma unroll
-                for (int k = 0; k < K; k++) dy[r][k] = Vec<T, V>(0);
             sums[2 * r] = sums[2 * r + 1] = 0.0f;
 #pragma unroll
             for (int k = 0; k < K; k++) {
-                const Floats<V> d = floats<T, V>(dy[r][k]), h = floats<T, V>(x[r][k]);
-                if constexpr (K > 1) w = load_weights<T, V>(a.weight, p.at[k], float_weights, 1.0f);
+                if (group + r * kRows >= left) now.dy[r][k] = Vec<T, V>(0);
+                dy[r][k] = now.dy[r][k];
+                c[r][k] = now.x[r][k];
+                const Floats<V> d = dy[r][k].get(), x = c[r][k].minus(now.mean[r]);
+                if constexpr (K > 1) load_weights_of(k);
 #pragma unroll
                 for (int e = 0; e < V; e++) {
-                    const float xhat = (h[e] - mean[r]) * rstd[r], g = d[e] * w[e], gm = k == K - 1 ? g * p.mask[e] : g;
-                    sums[2 * r] += gm;
-                    sums[2 * r + 1] = __builtin_fmaf(gm, xhat, sums[2 * r + 1]);
-                    dw[k][e] = __builtin_fmaf(d[e], xhat, dw[k][e]);
+                    const float dx = d[e] * x[e];
+                    sums[2 * r] = __builtin_fmaf(d[e], counted[e], sums[2 * r]);
+                    sums[2 * r + 1] = __builtin_fmaf(dx, counted[e], sums[2 * r + 1]);
+                    dw[k][e] = __builtin_fmaf(dx, now.rstd[r], dw[k][e]);
                     db[k][e] += d[e];
                 }
             }
         }
         if (!a.dx) continue;
         row_sums<TPR>(sums);
+        T* px = static_cast<T*>(a.dx) + first * a.dx_stride;
 #pragma unroll
         for (int r = 0; r < R; r++) {
-            if (row0 + r * kRows >= a.rows) break;
-            const int64_t row = row0 + r * kRows;
-            const float mg = sums[2 * r] * inv_width, mgx = sums[2 * r + 1] * inv_width;
-            T* px = static_cast<T*>(a.dx) + row * a.dx_stride;
+            const int row = group + r * kRows;
+            if (row >= left) break;
+            const float rstd = now.rstd[r], at_mean = -rstd * (sums[2 * r] * inv_width);
+            const float slope = -rstd * (rstd * (rstd * (sums[2 * r + 1] * inv_width)));
 #pragma unroll
             for (int k = 0; k < K; k++) {
-                Floats<V> d = floats_again<T, V>(dy[r][k]);
-                const Floats<V> h = floats_again<T, V>(x[r][k]);
-                if constexpr (K > 1) w = load_weights<T, V>(a.weight, p.at[k], float_weights, 1.0f);
+                Floats<V> d = dy[r][k].get();
+                const Floats<V> x = c[r][k].centred(now.mean[r]);
+                if constexpr (K > 1) load_weights_of(k);
 #pragma unroll
-                for (int e = 0; e < V; e++) {
-                    const float xhat = (h[e] - mean[r]) * rstd[r];
-                    d[e] = rstd[r] * __builtin_fmaf(-xhat, mgx, d[e] * w[e] - mg);
-                }
+                for (int e = 0; e < V; e++) d[e] = __builtin_fmaf(d[e] * w[e], rstd, __builtin_fmaf(x[e], slope, at_mean));
                 if (a.dh) d += floats<T, V>(now.dh[r][k]);
-                if (p.mine[k]) store_raw<V>(px + p.at[k], raw<T, V>(d));
+                if (p.mine[k]) store_raw<V>(px + row * a.dx_stride + p.at[k], raw<T, V>(d));
             }
         }
     }
