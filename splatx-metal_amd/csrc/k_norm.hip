@@ -641,15 +641,17 @@ void layer_norm_fwd(const NormFwdArgs& a, ElemType type, ElemType weight_type, h
 }
 
 // A workgroup's rows are as many as keep its partial sums (16 bytes a column, written and read) to a fraction of what it
-// reads, and as few as keep the memory busy: 512 threads on each of the 256 compute units, half of them where three tensors
-// are read, 1024 where a row takes over 256 (1 M x 64 with dh: 256 workgroups 90 us, 512 98, 1024 107; 1 M x 45: 512 96, 1024
-// 109; 4000 x 8000: 256 of 1024 threads 51, 512 56, 1024 67). As many on each unit: 341 workgroups of 768 threads, of which
-// a unit holds one, take as long as 512 would (10,666 x 6000: 126 us, 256 of them 85). 32 MiB of partial sums at most.
+// reads, and as few as keep the memory busy: 512 threads on each of the 256 compute units, 1024 where a row takes over 256, and
+// 256 where three tensors are read and few threads are without a vector of their own (1 M x 64 with dh: 256 workgroups 90 us,
+// 512 98, 1024 107, but 985 k x 65 180, 130 with 512; 1 M x 45 float without: 512 96, 1024 109; 4000 x 8000: 256 of 1024
+// threads 51, 512 56, 1024 67). As many on each unit: 341 workgroups of 768 threads, of which a unit holds one, take as long
+// as 512 would (10,666 x 6000: 126 us, 256 of them 85). 32 MiB of partial sums at most.
 int norm_bwd_slabs(int64_t rows, int64_t width, ElemType type, bool dh) {
     const int size = size_of(type);
     const Split sp = split_of(width, size, true);
     const int64_t per = sp.vec ? int64_t{sp.block_rows()} * sp.rows : 16;
-    const int64_t threads = sp.most > 256 && sp.vectors == 1 ? 1024 : sp.most <= kWave && dh ? 256 : 512;  // of a unit
+    const bool filled = width * size * 3 >= int64_t{sp.most} * 16 * 2;  // two thirds of the threads' bytes
+    const int64_t threads = sp.most > 256 && sp.vectors == 1 ? 1024 : sp.most <= kWave && dh && filled ? 256 : 512;  // of a unit
     const int64_t most = kUnits * std::max<int64_t>(sp.vec ? std::min(threads / sp.block(), rows * size * 3 / 128 / kUnits) : 4, 1);
     return static_cast<int>(std::max<int64_t>(std::min({(rows + per - 1) / per, most, (int64_t{32} << 20) / (8 * width)}), 1));
 }
