@@ -138,7 +138,7 @@ __device__ inline Floats<V> load_weights(const void* w, int at, bool is_float, f
 
 // R rows of each group of threads at a time. The weights of a thread's only vector stay in its registers; those of more are
 // read again for each row (they lie in the L1 cache), which leaves the registers to the rows.
-// 1 M x 48 bfloat16: 34.7 us, 5.8 TB/s; 16,383 x 2048 half with a residual: 45.4 us, 5.9 TB/s. Rows of 16-bit elements that
+// 1 M x 48 bfloat16: 33.8 us, 5.9 TB/s; 16,383 x 2048 half with a residual: 46.3 us, 5.8 TB/s. Rows of 16-bit elements that
 // begin off a multiple of four bytes take 1.1 to 1.2 times as long (1 M x 64: 52 us, 45 aligned), and rows a little wider than
 // a power of two vectors leave lanes idle, at up to 1.5 times (889 k x 72: 56 us, 666 k x 96, as many bytes, 48).
 template <class T, int V, int TPR, int K, int R>
@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(kThreadsOf<TPR>) k_norm_fwd(NormFwdArgs a, boo
 // The backward of R rows of each group of threads at a time; the columns' sums stay in registers over the rows, are added
 // over the workgroup's groups at the end and written as its part of the partial sums: one pass over dy and h for all three
 // gradients. With one vector a thread the next rows are on their way while these are worked on.
-// 1 M x 64 bfloat16 with dh: 90 us, 5.8 TB/s; 16,383 x 2048 half: 37.6 us, 5.4 TB/s; then the join, 2.8 to 4.7 us.
+// 1 M x 64 bfloat16 with dh: 89.9 us, 5.8 TB/s; 16,383 x 2048 half: 36.7 us, 5.5 TB/s; then the join, 2.7 to 4.8 us.
 template <class T, int V, int TPR, int K, int R, bool ONCE>
 __global__ void __launch_bounds__(kThreadsOf<TPR>) k_norm_bwd(NormBwdArgs a, bool float_weights) {
     constexpr int kRows = kRowsOf<TPR>;
@@ -414,7 +414,7 @@ __global__ void __launch_bounds__(kJoinBlock) k_norm_join(NormBwdArgs a, int sla
 
 // ---- rows wider than a workgroup's registers: it goes over its row several times ------------------------------------------
 // From 16,384 float elements on forward and 8,192 on backward (twice that in 16 bits). What is read again comes from the
-// caches: 3200 x 20,000 bfloat16 backward 167 us, 2.8 times what its bytes would take once.
+// caches: 3200 x 20,000 bfloat16 backward 170 us, 2.8 times what its bytes would take once.
 
 constexpr int kWideBlock = 1024;
 
