@@ -12,16 +12,16 @@ loads the library.
 from __future__ import annotations
 
 import ctypes as C
+import importlib.machinery
+import importlib.util
+import os
 import struct
 
 import torch
 
 import splatx_hip as sh
 
-TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # SXH_TYPE_*
 ADAMW_BLOCK = 256  # elements that share a scale with 8-bit moments
-_CODE_TYPES = (torch.float8_e4m3fn, torch.uint8)
-_FLOAT = (torch.float32,)
 
 
 class Queue(C.Structure):
@@ -66,35 +66,20 @@ class AdamWParams(C.Structure):
                 ("grad_norm", C.c_void_p), ("max_norm", C.c_float), ("grad_scale", C.c_float), ("state_bits", C.c_int32)]
 
 
-# The structs as bytes, which a call fills in a third of the time that it takes through ctypes: a small operator's time is
-# its call's.
-_QUEUE = struct.Struct("<Q")
-_NORM_IN = struct.Struct("<4Q4qfBB2x")
-_NORM_OUT = struct.Struct("<4Q2q")
-_GRADS_IN = struct.Struct("<6Q5qBB6x")
-_GRADS = struct.Struct("<3QqQq")
-_NORM_ROW = struct.Struct("<QqB7x")
-_ADAMW_ROW = struct.Struct("<7QqddBB6x")
-_ADAMW = struct.Struct("<qQdddQffi4x")
-for _packed, _struct in ((_QUEUE, Queue), (_NORM_IN, LayerNormInputs), (_NORM_OUT, LayerNormOutputs), (_GRADS_IN, LayerNormGradsIn),
-                         (_GRADS, LayerNormGrads), (_NORM_ROW, NormTensor), (_ADAMW_ROW, AdamWTensor), (_ADAMW, AdamWParams)):
-    assert _packed.size == C.sizeof(_struct), _struct
-
-
-
-def _pack(layout, *values):
-    try:
-        return layout.pack(*values)
-    except struct.error as e:
-        raise sh.SxInvalidArgument(f"not a number of the range: {e}") from None
-
-
-_is_contiguous = torch.Tensor.is_contiguous
-_numel = torch.Tensor.numel
-_ptr = torch.Tensor.data_ptr
-_empty = torch.empty
+_NORM_ROW = struct.Struct("<QqB7x")  # a NormTensor as bytes: a table of them is these one after another
 # (the public way to the current stream's handle makes an object of it, 2 us)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+
+
+def _extension():
+    """host/torch_ops.cpp, which is built beside the library where torch is: the calls' checks, outputs and launches."""
+    path = os.path.join(os.path.dirname(sh.LIB_PATH), "_splatx_torch.so")
+    if not os.path.exists(path):
+        raise sh.SxRuntimeError(f"the torch extension is not built: {path} (make all in splatx-metal_amd, with torch installed)")
+    loader = importlib.machinery.ExtensionFileLoader("_splatx_torch", path)
+    ops = importlib.util.module_from_spec(importlib.util.spec_from_loader("_splatx_torch", loader))
+    ops.set_errors(sh.SxInvalidArgument, sh.SxRuntimeError)
+    return ops
 
 
 def _one_hip_runtime():
@@ -117,147 +102,42 @@ class TorchBackend(sh.Backend):
     def __init__(self, device_ordinal: int = 0, lib=None):
         torch.cuda.init()
         lib = lib or sh.load_library()
+        if not os.path.samefile(lib._name, sh.LIB_PATH):
+            raise sh.SxInvalidArgument(f"the operators on tensors are those of {sh.LIB_PATH}")
         _one_hip_runtime()
         super().__init__(device_ordinal, lib)
         self.device = torch.device("cuda", device_ordinal)
-        self._index = device_ordinal
+        self._index, self._address, self._ops = device_ordinal, self.handle.value, _extension()
         p, n = C.c_void_p, C.c_int64
-        self._ops = {}
         for name, args in (("layer_norm_fwd", (p, p, p, p)), ("layer_norm_bwd", (p, p, p, p)), ("grad_norm", (p, p, n, p, p, n, p)),
                            ("adamw", (p, p, n, p, p))):
-            f = self._ops[name] = getattr(self.lib, "sxh_" + name)
+            f = getattr(self.lib, "sxh_" + name)
             f.argtypes, f.restype = args, C.c_int32
         for name, args in (("layer_norm_bwd_workspace", (n, n)), ("grad_norm_workspace", (n,))):
-            f = self._ops[name] = getattr(self.lib, "sxh_" + name)
+            f = getattr(self.lib, "sxh_" + name)
             f.argtypes, f.restype = args, n
 
-    def _enqueue(self, name, *args):
-        """The operator on torch's current stream of the device."""
-        rc = self._ops[name](self.handle, *args, _QUEUE.pack(_raw_stream(self._index)))
-        if rc != sh.SXH_OK:
-            msg = self.lib.sxh_last_error().decode(errors="replace")
-            raise (sh.SxInvalidArgument if rc == sh.SXH_ERR_INVALID_ARGUMENT else sh.SxRuntimeError)(msg)
-
-    def _rows(self, t, name, like=None):
-        """(tensor as [rows, width], its row stride)"""
-        if not isinstance(t, torch.Tensor) or t.device != self.device:
-            raise sh.SxInvalidArgument(f"{name} must be a tensor on {self.device}")
-        if like is None:
-            if t.dtype not in TYPES:
-                raise sh.SxInvalidArgument(f"{name} must be float32, bfloat16 or float16")
-        elif t.dtype != like.dtype or t.shape != like.shape:
-            raise sh.SxInvalidArgument(f"{name} must have the rows' type and shape")
-        if t.dim() != 2:
-            if t.dim() == 0:
-                raise sh.SxInvalidArgument(f"{name} has no rows")
-            try:
-                t = t.view(t.shape[:-1].numel(), t.shape[-1])
-            except RuntimeError:
-                raise sh.SxInvalidArgument(f"{name}: rows of {tuple(t.shape)} with strides {t.stride()} are not evenly spaced") from None
-        rows, width = t.shape
-        stride, inner = t.stride()
-        if inner != 1 and width > 1:
-            raise sh.SxInvalidArgument(f"{name}: the elements of a row must lie side by side")
-        return t, stride if rows > 1 else width
-
-    def _vector(self, t, name, n, types):
-        if not isinstance(t, torch.Tensor) or t.device != self.device:
-            raise sh.SxInvalidArgument(f"{name} must be a tensor on {self.device}")
-        if t.dtype not in types or t.numel() != n or not t.is_contiguous():
-            raise sh.SxInvalidArgument(f"{name} must be {n} contiguous elements of {' or '.join(map(str, types))}")
-        return t.data_ptr()
-
-    def _like(self, t):
-        """Contiguous rows like t's."""
-        return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+    def close(self):
+        self._address = 0
+        super().close()
 
     # -- layer norm ------------------------------------------------------------------------------------
     def layer_norm_fwd(self, x, weight=None, bias=None, eps=1e-5, residual=None, stats=True):
         """(y, h, mean, rstd): h = x + residual (x itself without one), y = (h - mean) rstd weight + bias over the last
         dimension; mean and rstd, one per row, are None without `stats`."""
-        x2, x_stride = self._rows(x, "x")
-        rows, width = x2.shape
-        t = x.dtype
-        wt = weight.dtype if weight is not None else bias.dtype if bias is not None else torch.float32
-        w = self._vector(weight, "weight", width, (torch.float32, t)) if weight is not None else 0
-        b = self._vector(bias, "bias", width, (wt,) if weight is not None else (torch.float32, t)) if bias is not None else 0
-        y = self._like(x)
-        h, r, r_stride = x, 0, 0
-        if residual is not None:
-            residual, r_stride = self._rows(residual, "residual", x)
-            h, r = self._like(x), residual.data_ptr()
-        mean = rstd = None
-        m = s = 0
-        if stats:
-            mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
-            rstd = torch.empty_like(mean)
-            m, s = mean.data_ptr(), rstd.data_ptr()
-        self._enqueue("layer_norm_fwd",
-                      _pack(_NORM_IN, x2.data_ptr(), r, w, b, rows, width, x_stride, r_stride, eps, TYPES[t], TYPES[wt]),
-                      _NORM_OUT.pack(y.data_ptr(), h.data_ptr() if r else 0, m, s, width, width))
-        return y, h, mean, rstd
+        return self._ops.layer_norm_fwd(self._address, self._index, _raw_stream(self._index), x, weight, bias, eps, residual, stats)
 
     def layer_norm_bwd(self, dy, h, mean, rstd, weight=None, dh=None, want_dx=True, want_dweight=True, want_dbias=True):
         """(dx, dweight, dbias) of layer_norm_fwd's h, mean and rstd; dx is the gradient of x and of the residual, with the
         gradient dh that reaches h past the norm. dweight and dbias have the weight's type (float32 without one)."""
-        h2, h_stride = self._rows(h, "h")
-        dy, dy_stride = self._rows(dy, "dy", h)
-        rows, width = h2.shape
-        wt, w, dh_ptr, dh_stride = torch.float32, 0, 0, 0
-        if weight is not None:
-            wt, w = weight.dtype, self._vector(weight, "weight", width, (torch.float32, h.dtype))
-        if dh is not None:
-            dh, dh_stride = self._rows(dh, "dh", h)
-            dh_ptr = dh.data_ptr()
-        m = self._vector(mean, "mean", rows, (torch.float32,))
-        s = self._vector(rstd, "rstd", rows, (torch.float32,))
-        dx = dweight = dbias = work = None
-        dx_ptr = dweight_ptr = dbias_ptr = work_ptr = bytes_ = 0
-        if want_dx:
-            dx = self._like(h)
-            dx_ptr = dx.data_ptr()
-        if want_dweight or want_dbias:
-            if want_dweight:
-                dweight = h.new_empty(width, dtype=wt)
-                dweight_ptr = dweight.data_ptr()
-            if want_dbias:
-                dbias = h.new_empty(width, dtype=wt)
-                dbias_ptr = dbias.data_ptr()
-            bytes_ = self._ops["layer_norm_bwd_workspace"](rows, width)
-            work = h.new_empty(bytes_, dtype=torch.uint8)
-            work_ptr = work.data_ptr()
-        self._enqueue("layer_norm_bwd",
-                      _GRADS_IN.pack(dy.data_ptr(), h2.data_ptr(), dh_ptr, m, s, w, rows, width, dy_stride, h_stride, dh_stride,
-                                     TYPES[h.dtype], TYPES[wt]),
-                      _GRADS.pack(dx_ptr, dweight_ptr, dbias_ptr, width, work_ptr, bytes_))
-        return dx, dweight, dbias
+        return self._ops.layer_norm_bwd(self._address, self._index, _raw_stream(self._index), dy, h, mean, rstd, weight, dh, want_dx,
+                                        want_dweight, want_dbias)
 
     # -- many tensors ------------------------------------------------------------------------------------
-    @staticmethod
-    def _tensors(ts, name, types):
-        """(pointers, sizes, types) of a list of contiguous tensors; that they are on the device is checked with the pointers."""
-        try:
-            ptrs, sizes = list(map(_ptr, ts)), list(map(_numel, ts))
-        except TypeError:
-            raise sh.SxInvalidArgument(f"{name} must be tensors") from None
-        dtypes = [t.dtype for t in ts]
-        for t in set(dtypes):
-            if t not in types:
-                raise sh.SxInvalidArgument(f"{name} must be {' or '.join(map(str, types))}, not {t}")
-        if not all(map(_is_contiguous, ts)):
-            raise sh.SxInvalidArgument(f"{name} must be contiguous")
-        return ptrs, sizes, dtypes
-
     def grad_norm(self, grads):
         """The 2-norm of all the tensors together, as a tensor of one float32 on the device."""
-        grads = list(grads)
-        ptrs, sizes, dtypes = self._tensors(grads, "grads", TYPES)
-        norm = _empty((), dtype=torch.float32, device=self.device)
-        bytes_ = self._ops["grad_norm_workspace"](len(grads))
-        work = _empty(bytes_, dtype=torch.uint8, device=self.device)
-        table = b"".join(map(_NORM_ROW.pack, ptrs, sizes, map(TYPES.__getitem__, dtypes)))
-        self._enqueue("grad_norm", table, len(grads), norm.data_ptr(), work.data_ptr(), bytes_)
-        return norm
+        grads = grads if isinstance(grads, (list, tuple)) else list(grads)
+        return self._ops.grad_norm(self._address, self._index, _raw_stream(self._index), grads)
 
     def adamw_step(self, params, grads, exp_avg, exp_avg_sq, *, step, lr, weight_decay=0.0, b1=0.9, b2=0.999, eps=1e-8,
                    master=None, grad_scale=1.0, grad_norm=None, max_norm=0.0, exp_avg_scale=None, exp_avg_sq_scale=None, seed=0):
@@ -265,44 +145,8 @@ class TorchBackend(sh.Backend):
         float32 copies that the step works on, with 16-bit params. With the scales, exp_avg and exp_avg_sq are float8_e4m3fn
         (or uint8) tensors: m, and the root of v, in units of their block's scale. grad_norm: `grad_norm`'s result of these
         gradients; where it is not finite the step is left out."""
-        n = len(params)
-        eight = exp_avg_scale is not None
-        if eight != (exp_avg_sq_scale is not None):
-            raise sh.SxInvalidArgument("exp_avg_scale and exp_avg_sq_scale are given together")
-        states = _CODE_TYPES if eight else _FLOAT
-        none = [0] * n
-        param_ptrs, sizes, param_types = self._tensors(params, "params", TYPES)
-        grad_ptrs, got, grad_types = self._tensors(grads, "grads", TYPES)
-        self._same(got, sizes, "grads")
-
-        def like(ts, name, types, want):
-            ptrs, got, _ = self._tensors(ts, name, types)
-            self._same(got, want, name)
-            return ptrs
-
-        master_ptrs = none if master is None else like(master, "master", _FLOAT, sizes)
-        m, v = like(exp_avg, "exp_avg", states, sizes), like(exp_avg_sq, "exp_avg_sq", states, sizes)
-        m_scale = v_scale = none
-        if eight:
-            blocks = [-(-k // ADAMW_BLOCK) for k in sizes]
-            m_scale = like(exp_avg_scale, "exp_avg_scale", _FLOAT, blocks)
-            v_scale = like(exp_avg_sq_scale, "exp_avg_sq_scale", _FLOAT, blocks)
-        lrs = lr if isinstance(lr, (list, tuple)) else [lr] * n
-        decays = weight_decay if isinstance(weight_decay, (list, tuple)) else [weight_decay] * n
-        if len(lrs) != n or len(decays) != n:
-            raise sh.SxInvalidArgument("lr and weight_decay are a number, or one for each tensor")
-        norm = self._vector(grad_norm, "grad_norm", 1, _FLOAT) if grad_norm is not None else 0
-        try:
-            table = b"".join(map(_ADAMW_ROW.pack, param_ptrs, master_ptrs, grad_ptrs, m, v, m_scale, v_scale, sizes, lrs, decays,
-                                 map(TYPES.__getitem__, param_types), map(TYPES.__getitem__, grad_types)))
-        except struct.error:
-            raise sh.SxInvalidArgument("lr and weight_decay must be numbers") from None
-        self._enqueue("adamw", table, n, _pack(_ADAMW, step, seed, b1, b2, eps, norm, max_norm, grad_scale, 8 if eight else 32))
-
-    @staticmethod
-    def _same(got, want, name):
-        if got != want:
-            raise sh.SxInvalidArgument(f"{name}: {len(got)} tensors of {got[:8]}.. elements, wanted are {len(want)} of {want[:8]}..")
+        self._ops.adamw(self._address, self._index, _raw_stream(self._index), params, grads, exp_avg, exp_avg_sq, step, lr,
+                        weight_decay, b1, b2, eps, master, grad_scale, grad_norm, max_norm, exp_avg_scale, exp_avg_sq_scale, seed)
 
 
 class _LayerNorm(torch.autograd.Function):

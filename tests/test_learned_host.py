@@ -119,3 +119,24 @@ def test_the_nearest_code_would_hold_a_second_moment_still():
         new[0] = 1.0
         codes, scale = ref.encode(new.sqrt(), half, True)
     assert float(ref.decode(codes, scale)[1]) ** 2 == pytest.approx(0.25, rel=0.01)
+
+
+def test_tensor_calls_refuse_host_memory(st, lib):
+    """The calls on tensors raise the binding's exceptions, also for arguments that are no tensors or no numbers."""
+    import splatx_hip as sh
+    import torch
+    ops = st._extension()
+    x = torch.ones(4, 8)
+    for f, args in ((ops.layer_norm_fwd, (x, None, None, 1e-5, None, True)), (ops.layer_norm_fwd, (None, None, None, 1e-5, None, True)),
+                    (ops.layer_norm_bwd, (x, x, x, x, None, None, True, True, True)), (ops.grad_norm, ([x],)), (ops.grad_norm, (x,)),
+                    (ops.grad_norm, ([x.numpy()],)), (ops.grad_norm, ()),
+                    (ops.adamw, ([x], [x], [x], [x], 1, 1e-3, 0.0, 0.9, 0.999, 1e-8, None, 1.0, None, 0.0, None, None, 0)),
+                    (ops.adamw, ([], [], [], [], 1.5, 1e-3, 0.0, 0.9, 0.999, 1e-8, None, 1.0, None, 0.0, None, None, 0)),
+                    (ops.adamw, ([], [], [], [], 1, "x", 0.0, 0.9, 0.999, 1e-8, None, 1.0, None, 0.0, None, None, 0)),
+                    (ops.adamw, ([], [], [], [x], 1, 1e-3, 0.0, 0.9, 0.999, 1e-8, None, 1.0, None, 0.0, None, None, 0)),
+                    (ops.adamw, ([], [], [], [], 1, 1e-3, 0.0, 0.9, 0.999, 1e-8, None, 1.0, None, 0.0, [], None, 0)),
+                    (ops.adamw, ([], [], [], [], 1, 1e-3, 0.0, 0.9, 0.999, 1e-8, None, 1.0, None, 0.0, None, None, 2 ** 64))):
+        with pytest.raises(sh.SxInvalidArgument):
+            f(0, 0, 0, *args)
+    with pytest.raises(sh.SxInvalidArgument, match="null backend"):
+        ops.adamw(0, 0, 0, [], [], [], [], 1, 1e-3, 0.0, 0.9, 0.999, 1e-8, None, 1.0, None, 0.0, None, None, 0)
