@@ -129,6 +129,15 @@ struct Kept<T, V, 1> {
     __device__ Floats<V> centred(float) const { return v; }
 };
 
+// How a row's vectors are read. Past: past the caches. Shifted: 16-bit elements that begin off a multiple of four bytes, which
+// a load as it is takes twice as long for.
+enum class Loads { Plain, Past, Shifted };
+template <Loads L, int V, class T>
+__device__ inline Vec<T, V> load_row(const T* p) {
+    if constexpr (L == Loads::Shifted) return load_shifted(p);
+    else return load_raw<V, L == Loads::Past>(p);
+}
+
 template <class T, int V>
 __device__ inline Floats<V> load_weights(const void* w, int at, bool is_float, float none) {
     if (!w) return Floats<V>(none);
@@ -138,10 +147,10 @@ __device__ inline Floats<V> load_weights(const void* w, int at, bool is_float, f
 
 // R rows of each group of threads at a time. The weights of a thread's only vector stay in its registers; those of more are
 // read again for each row (they lie in the L1 cache), which leaves the registers to the rows.
-// 1 M x 48 bfloat16: 33.8 us, 5.9 TB/s; 16,383 x 2048 half with a residual: 46.3 us, 5.8 TB/s. Rows of 16-bit elements that
-// begin off a multiple of four bytes take 1.1 to 1.2 times as long (1 M x 64: 52 us, 45 aligned), and rows a little wider than
-// a power of two vectors leave lanes idle, at up to 1.5 times (889 k x 72: 56 us, 666 k x 96, as many bytes, 48).
-template <class T, int V, int TPR, int K, int R>
+// 1 M x 48 bfloat16: 33.8 us, 5.9 TB/s; 16,383 x 2048 half with a residual: 46.3 us, 5.8 TB/s. Rows a little wider than a
+// power of two vectors leave lanes idle, and odd ones of 16 bits share lines with their neighbours, at up to 1.5 times
+// (242,424 x 264: 53 us, 249,027 x 257 62, 250,000 x 256, as many bytes, 46; three vectors a thread of fewer threads 58).
+template <class T, int V, int TPR, int K, int R, Loads L>
 __global__ void __launch_bounds__(kThreadsOf<TPR>) k_norm_fwd(NormFwdArgs a, bool float_weights) {
     constexpr int kRows = kRowsOf<TPR>;
     const Place<V, TPR, K> p(a.width);
@@ -165,7 +174,7 @@ __global__ void __launch_bounds__(kThreadsOf<TPR>) k_norm_fwd(NormFwdArgs a, boo
         for (int r = 0; r < R; r++) {
             row[r] = min(group + r * kRows, left - 1);
 #pragma unroll
-            for (int k = 0; k < K; k++) x[r][k] = load_raw<V>(px + row[r] * a.x_stride + p.at[k]);
+            for (int k = 0; k < K; k++) x[r][k] = load_row<L, V>(px + row[r] * a.x_stride + p.at[k]);
         }
         if (a.residual) {
             const T* pr = static_cast<const T*>(a.residual) + first * a.residual_stride;
@@ -174,7 +183,7 @@ __global__ void __launch_bounds__(kThreadsOf<TPR>) k_norm_fwd(NormFwdArgs a, boo
             for (int r = 0; r < R; r++)
 #pragma unroll
                 for (int k = 0; k < K; k++) {
-                    const Vec<T, V> h = raw<T, V>(x[r][k].get() + floats<T, V>(load_raw<V>(pr + row[r] * a.residual_stride + p.at[k])));
+                    const Vec<T, V> h = raw<T, V>(x[r][k].get() + floats<T, V>(load_row<L, V>(pr + row[r] * a.residual_stride + p.at[k])));
                     x[r][k] = h;
                     if (p.mine[k] && group + r * kRows < left) store_raw<V>(ph + row[r] * a.h_stride + p.at[k], h);
                 }
@@ -237,7 +246,7 @@ __global__ void __launch_bounds__(kThreadsOf<TPR>) k_norm_fwd(NormFwdArgs a, boo
 // over the workgroup's groups at the end and written as its part of the partial sums: one pass over dy and h for all three
 // gradients. With one vector a thread the next rows are on their way while these are worked on.
 // 1 M x 64 bfloat16 with dh: 89.9 us, 5.8 TB/s; 16,383 x 2048 half: 36.7 us, 5.5 TB/s; then the join, 2.7 to 4.8 us.
-template <class T, int V, int TPR, int K, int R, bool ONCE>
+template <class T, int V, int TPR, int K, int R, Loads L>
 __global__ void __launch_bounds__(kThreadsOf<TPR>) k_norm_bwd(NormBwdArgs a, bool float_weights) {
     constexpr int kRows = kRowsOf<TPR>;
     const Place<V, TPR, K> p(a.width);
@@ -268,8 +277,8 @@ __global__ void __launch_bounds__(kThreadsOf<TPR>) k_norm_bwd(NormBwdArgs a, boo
             to.rstd[r] = (a.rstd + first)[row[r]];
 #pragma unroll
             for (int k = 0; k < K; k++) {
-                to.dy[r][k] = load_raw<V, ONCE>(pd + row[r] * a.dy_stride + p.at[k]);
-                to.x[r][k] = load_raw<V, ONCE>(ph + row[r] * a.h_stride + p.at[k]);
+                to.dy[r][k] = load_row<L, V>(pd + row[r] * a.dy_stride + p.at[k]);
+                to.x[r][k] = load_row<L, V>(ph + row[r] * a.h_stride + p.at[k]);
             }
         }
         if (a.dh) {
@@ -277,7 +286,7 @@ __global__ void __launch_bounds__(kThreadsOf<TPR>) k_norm_bwd(NormBwdArgs a, boo
 #pragma unroll
             for (int r = 0; r < R; r++)
 #pragma unroll
-                for (int k = 0; k < K; k++) to.dh[r][k] = load_raw<V, ONCE>(pdh + row[r] * a.dh_stride + p.at[k]);
+                for (int k = 0; k < K; k++) to.dh[r][k] = load_row<L, V>(pdh + row[r] * a.dh_stride + p.at[k]);
         }
     };
     const int64_t stride = int64_t{gridDim.x} * (kRows * R);
@@ -559,26 +568,51 @@ Split split_of(int64_t width, int size, bool backward) {
     return {0, 0, kWideBlock, 0, 1};
 }
 
+// Do the rows begin on multiples of n bytes?
+bool on(int n, const void* p, int64_t stride, int size) {
+    return (reinterpret_cast<uintptr_t>(p) | static_cast<uintptr_t>(stride) * size) % n == 0;
+}
+bool on(int n, const NormFwdArgs& a, int size) { return on(n, a.x, a.x_stride, size) && on(n, a.residual, a.residual_stride, size); }
+bool on(int n, const NormBwdArgs& a, int size) {
+    return on(n, a.dy, a.dy_stride, size) && on(n, a.h, a.h_stride, size) && on(n, a.dh, a.dh_stride, size);
+}
+// The loads of 16-bit rows that begin off a multiple of four bytes, up to a wave for a row: 1.2 M x 45 bfloat16, forward 44.3 us
+// against 51.0, backward 76.3 against 82.7, with dh 82.4 against 98.4. Wider rows take as long or longer (40,000 x 1601,
+// backward: 92 us against 84), as do rows on multiples of four bytes (31,250 x 2048, forward: 55 against 49).
+template <int V, int TPR>
+constexpr bool kMayShift = V == 8 && TPR <= kWave;
+
 template <class T, int V, int TPR, int K>
 void launch(const Split& sp, const NormFwdArgs& a, bool fw, int grid, hipStream_t s) {
     constexpr int R = K == 1 ? 2 : 1;
-    hipLaunchKernelGGL((k_norm_fwd<T, V, TPR, K, R>), dim3(grid), dim3(sp.block()), 0, s, a, fw);
+    if constexpr (kMayShift<V, TPR>) {
+        if (!on(4, a, sizeof(T))) {
+            hipLaunchKernelGGL((k_norm_fwd<T, V, TPR, K, R, Loads::Shifted>), dim3(grid), dim3(sp.block()), 0, s, a, fw);
+            return;
+        }
+    }
+    hipLaunchKernelGGL((k_norm_fwd<T, V, TPR, K, R, Loads::Plain>), dim3(grid), dim3(sp.block()), 0, s, a, fw);
 }
 template <class T, int V, int TPR, int K>
 void launch(const Split& sp, const NormBwdArgs& a, bool fw, int grid, hipStream_t s) {
     constexpr int R = K == 1 && TPR <= 256 ? 2 : 1;
-    // Rows of 256 threads or more, 16-byte aligned, go past the caches where a call moves more than half of what the last
-    // one holds (256 MiB): 16,383 x 2048 36.5 us against 40.0. Within it they do not (33 against 36), nor where rows share
-    // lines with others (1 M x 45: 101 against 96), nor narrower ones, which gain nothing (65,536 x 1024: 101.6 against 98.0).
+    // Rows of 256 threads or more, 16-byte aligned, go past the caches where a call moves more than half of what the last one
+    // holds (256 MiB): 16,383 x 2048 36.5 us against 40.0, 64,000 x 1000 float 127 against 140. Within it they do not (33
+    // against 36), nor where rows share lines with others (1 M x 45: 101 against 96), nor narrower ones, which gain nothing
+    // (65,536 x 1024: 101.6 against 98.0).
     if constexpr (TPR >= 256) {
-        const auto whole = [](const void* p, int64_t stride) { return (reinterpret_cast<uintptr_t>(p) | static_cast<uintptr_t>(stride) * sizeof(T)) % 16 == 0; };
-        if (a.rows * a.width * static_cast<int64_t>(sizeof(T)) * (a.dh ? 4 : 3) > (int64_t{128} << 20) && whole(a.dy, a.dy_stride) &&
-            whole(a.h, a.h_stride) && whole(a.dh, a.dh_stride)) {
-            hipLaunchKernelGGL((k_norm_bwd<T, V, TPR, K, R, true>), dim3(grid), dim3(sp.block()), 0, s, a, fw);
+        if (a.rows * a.width * static_cast<int64_t>(sizeof(T)) * (a.dh ? 4 : 3) > (int64_t{128} << 20) && on(16, a, sizeof(T))) {
+            hipLaunchKernelGGL((k_norm_bwd<T, V, TPR, K, R, Loads::Past>), dim3(grid), dim3(sp.block()), 0, s, a, fw);
             return;
         }
     }
-    hipLaunchKernelGGL((k_norm_bwd<T, V, TPR, K, R, false>), dim3(grid), dim3(sp.block()), 0, s, a, fw);
+    if constexpr (kMayShift<V, TPR>) {
+        if (!on(4, a, sizeof(T))) {
+            hipLaunchKernelGGL((k_norm_bwd<T, V, TPR, K, R, Loads::Shifted>), dim3(grid), dim3(sp.block()), 0, s, a, fw);
+            return;
+        }
+    }
+    hipLaunchKernelGGL((k_norm_bwd<T, V, TPR, K, R, Loads::Plain>), dim3(grid), dim3(sp.block()), 0, s, a, fw);
 }
 
 template <class T, class Args>
@@ -641,25 +675,33 @@ void layer_norm_fwd(const NormFwdArgs& a, ElemType type, ElemType weight_type, h
 }
 
 // A workgroup's rows are as many as keep its partial sums (16 bytes a column, written and read) to a fraction of what it
-// reads, and as few as keep the memory busy: 512 threads on each of the 256 compute units, 1024 where a row takes over 256, and
-// 256 where three tensors are read and few threads are without a vector of their own (1 M x 64 with dh: 256 workgroups 90 us,
-// 512 98, 1024 107, but 985 k x 65 180, 130 with 512; 1 M x 45 float without: 512 96, 1024 109; 4000 x 8000: 256 of 1024
-// threads 51, 512 56, 1024 67). As many on each unit: 341 workgroups of 768 threads, of which a unit holds one, take as long
-// as 512 would (10,666 x 6000: 126 us, 256 of them 85). 32 MiB of partial sums at most.
-int norm_bwd_slabs(int64_t rows, int64_t width, ElemType type, bool dh) {
+// reads, and each of the 256 compute units has the same number of workgroups (341 of 768 threads, of which a unit holds one, take
+// as long as 512 would: 10,666 x 6000 126 us, 256 of them 85): as many as have the memory busy and no more, which counts in the
+// vectors that a unit's threads have on their way (threads without one of their own do not count, three tensors want fewer than
+// two, rows that share words and rows worked on one at a time more), up to 768 threads, all that the registers hold of 16-bit
+// elements. Measured in workgroups a unit, without dh: 1 M x 64 2: 73 us, 4 85; 249,027 x 257 2: 111, 3 90; 711,111 x 90 2: 71,
+// 3 75; 123,076 x 520 4: 98, 6 83; 62,015 x 1032 2: 100, 4 76; 31,128 x 2056 2: 78, 3 96. With dh: 1 M x 64 1: 90, 2 99;
+// 666,666 x 96 1: 103, 2 92; 126,732 x 505 1: 114, 2 98; 62,500 x 1024 2: 104, 3 91, 4 93; 31,128 x 2056 1: 120, 2 96. 32 MiB
+// of partial sums at most.
+int norm_bwd_slabs(int64_t rows, int64_t width, ElemType type, bool dh, bool even) {
     const int size = size_of(type);
     const Split sp = split_of(width, size, true);
     const int64_t per = sp.vec ? int64_t{sp.block_rows()} * sp.rows : 16;
-    const bool filled = width * size * 3 >= int64_t{sp.most} * 16 * 2;  // two thirds of the threads' bytes
-    const int64_t threads = sp.most > 256 && sp.vectors == 1 ? 1024 : sp.most <= kWave && dh && filled ? 256 : 512;  // of a unit
-    const int64_t most = kUnits * std::max<int64_t>(sp.vec ? std::min(threads / sp.block(), rows * size * 3 / 128 / kUnits) : 4, 1);
+    int64_t each = 4;  // workgroups a unit
+    if (sp.vec) {
+        const double vectors = static_cast<double>(sp.block_rows()) * static_cast<double>(width * size) / 16.0;  // of a workgroup
+        const double wanted = sp.rows == 1 ? 650.0 : (!even ? 520.0 : sp.most <= kWave ? 390.0 : 500.0) * (dh ? 0.8 : 1.0);
+        const int64_t threads = sp.rows == 1 && size == 4 ? 1024 : 768;
+        each = std::min({static_cast<int64_t>(wanted / vectors + 0.5), threads / sp.block(), rows * size * 3 / 128 / kUnits});
+    }
+    const int64_t most = kUnits * std::max<int64_t>(each, 1);
     return static_cast<int>(std::max<int64_t>(std::min({(rows + per - 1) / per, most, (int64_t{32} << 20) / (8 * width)}), 1));
 }
 
 void layer_norm_bwd(const NormBwdArgs& args, ElemType type, ElemType weight_type, hipStream_t s) {
     NormBwdArgs a = args;
     const Split sp = split_of(a.width, size_of(type), true);
-    const int slabs = norm_bwd_slabs(a.rows, a.width, type, a.dh != nullptr);
+    const int slabs = norm_bwd_slabs(a.rows, a.width, type, a.dh != nullptr, on(4, a, size_of(type)));
     const bool columns = a.dweight || a.dbias, fw = weight_type == kF32;
     if (!columns) a.partial = nullptr;
     with_type(type, [&](auto t) {

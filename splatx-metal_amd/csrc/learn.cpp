@@ -206,8 +206,7 @@ int32_t sxh_layer_norm_fwd(sxh_backend* b, const sxh_layer_norm_inputs* in, cons
 int64_t sxh_layer_norm_bwd_workspace(int64_t rows, int64_t width) {
     if (rows < 0 || width < 1 || width > (int64_t{1} << 24)) return 0;
     int slabs = 0;  // the most that any type needs
-    for (const sxk::ElemType t : {sxk::kF32, sxk::kBf16}) slabs = std::max(slabs, sxk::norm_bwd_slabs(rows, width, t, false));
-    for (const sxk::ElemType t : {sxk::kF32, sxk::kBf16}) slabs = std::max(slabs, sxk::norm_bwd_slabs(rows, width, t, true));
+    for (const sxk::ElemType t : {sxk::kF32, sxk::kBf16}) slabs = std::max(slabs, sxk::norm_bwd_slabs(rows, width, t, false, false));
     return int64_t{slabs} * 2 * width * 4;
 }
 

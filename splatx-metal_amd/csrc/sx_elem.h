@@ -32,6 +32,20 @@ __device__ inline Vec<T, V> load_raw(const T* p) {
     if constexpr (ONCE) return __builtin_nontemporal_load(reinterpret_cast<const At*>(p));
     return *reinterpret_cast<const At*>(p);
 }
+// Eight 16-bit elements that may begin off a multiple of four bytes: the words that hold them, shifted into place. Every word
+// that is read holds one of them.
+template <class T>
+__device__ inline Vec<T, 8> load_shifted(const T* p) {
+    static_assert(sizeof(T) == 2);
+    using Words = uint32_t __attribute__((ext_vector_type(4)));
+    using At = Words __attribute__((aligned(4)));
+    const uintptr_t first = reinterpret_cast<uintptr_t>(p) & ~uintptr_t{3}, last = (reinterpret_cast<uintptr_t>(p) + 15) & ~uintptr_t{3};
+    const Words w = *reinterpret_cast<const At*>(first);
+    const uint32_t end = *reinterpret_cast<const uint32_t*>(last), bits = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p) & 2) * 8;
+    const Words at = {__builtin_amdgcn_alignbit(w[1], w[0], bits), __builtin_amdgcn_alignbit(w[2], w[1], bits),
+                      __builtin_amdgcn_alignbit(w[3], w[2], bits), __builtin_amdgcn_alignbit(end, w[3], bits)};
+    return __builtin_bit_cast(Vec<T, 8>, at);
+}
 template <int V, bool ONCE = false, class T>
 __device__ inline void store_raw(T* p, Vec<T, V> v) {
     using At = Vec<T, V> __attribute__((aligned(sizeof(T))));

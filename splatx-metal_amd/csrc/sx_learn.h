@@ -28,8 +28,9 @@ struct NormBwdArgs {
     int64_t rows, dy_stride, h_stride, dh_stride, dx_stride;
     int width;
 };
-// Parts of the rows whose column sums are formed one by one, then joined.
-int norm_bwd_slabs(int64_t rows, int64_t width, ElemType type, bool dh);
+// Parts of the rows whose column sums are formed one by one, then joined: the most without dh and not `even` (every row begins
+// on a multiple of four bytes).
+int norm_bwd_slabs(int64_t rows, int64_t width, ElemType type, bool dh, bool even);
 void layer_norm_bwd(const NormBwdArgs& a, ElemType type, ElemType weight_type, hipStream_t s);
 
 // Tensors of one launch, passed by value: a launch's arguments hold at most 4 KiB.

@@ -99,6 +99,32 @@ def test_layer_norm_row_counts(tb, width, dtype, rows):
     assert all(torch.equal(a, c) for a, c in zip(got, again))
 
 
+@pytest.mark.parametrize("width", [8, 9, 15, 16, 23, 45, 64, 127, 200, 301, 505, 512, 1001])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("off", [(1, 1, 1), (1, 0, 2), (0, 3, 1), (2, 2, 1)])
+def test_layer_norm_rows_off_words(tb, width, dtype, off):
+    """16-bit rows that begin off a multiple of four bytes, each input in its own way, up to the last element of its tensor."""
+    rows = 131
+
+    def held_off(t, k):
+        flat = torch.full((k + t.numel(),), float("nan"), dtype=t.dtype, device="cuda")
+        flat[k:] = t.flatten().cuda()
+        return flat[k:].view(t.shape)
+
+    x, r = randn(rows, width, seed=1, dtype=dtype), randn(rows, width, seed=2, dtype=dtype)
+    w, b = 1 + 0.2 * randn(width, seed=4), 0.3 * randn(width, seed=5)
+    for add in (False, True):
+        y, h, mean, rstd, bound = ref.norm_fwd(x, w, b, 1e-5, r if add else None)
+        gy, gh, gm, gs = tb.layer_norm_fwd(held_off(x, off[0]), w.cuda(), b.cuda(), 1e-5, held_off(r, off[1]) if add else None)
+        assert torch.equal(gh.cpu().double(), h)
+        within(gy, y, bound, "y")
+        dy, dh = randn(rows, width, seed=6, dtype=dtype), randn(rows, width, seed=7, dtype=dtype)
+        want, bounds = ref.norm_bwd(dy, gh.cpu(), gm.cpu(), gs.cpu(), w, dh if add else None)
+        got = tb.layer_norm_bwd(held_off(dy, off[0]), held_off(gh.cpu(), off[1]), gm, gs, w.cuda(), held_off(dh, off[2]) if add else None)
+        for g, c, e, name in zip(got, want, bounds, ("dx", "dweight", "dbias")):
+            within(g, c, e, name)
+
+
 def test_layer_norm_parts(tb):
     """Without weight, bias, statistics; single gradients; shapes of one, two and four dimensions; no rows."""
     x = randn(70, 33, seed=1)
