@@ -389,7 +389,7 @@ int32_t sxh_adamw(sxh_backend* b, const sxh_adamw_tensor* tensors, int64_t n_ten
         for (int64_t i = 0; i < n_tensors; i++) {
             const sxh_adamw_tensor& x = tensors[i];
             if (!x.n) continue;
-            const int64_t chunks = (x.n + sxk::kAdamChunk - 1) / sxk::kAdamChunk;
+            const int64_t chunks = (x.n + (eight ? 0 : sxk::adam_lead(x.exp_avg)) + sxk::kAdamChunk - 1) / sxk::kAdamChunk;
             if (t.tensors == sxk::kAdamTensors || (t.tensors && t.first[t.tensors] + chunks > kMostChunks)) flush();
             sxk::AdamTensor& a = t.t[t.tensors];
             a.param = x.param; a.master = x.master; a.grad = x.grad; a.m = x.exp_avg; a.v = x.exp_avg_sq;

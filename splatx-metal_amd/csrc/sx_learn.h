@@ -74,6 +74,8 @@ struct AdamTable {
 };
 static_assert(sizeof(AdamTable) <= 4096 && sizeof(NormTable) <= 4096, "a launch's arguments hold 4 KiB");
 constexpr int kAdamChunk = 1024;  // elements of a workgroup
+// Elements of a 32-bit tensor's first chunk that lie before it: chunks begin on lines of 128 bytes of exp_avg.
+__host__ __device__ inline int adam_lead(const void* m) { return static_cast<int>(reinterpret_cast<uintptr_t>(m) / 4 % 32); }
 // The key of the rounding of the call's tensor.
 uint32_t adam_key(uint64_t seed, int64_t step, int64_t tensor);
 // `once`: the call's tensors are more than the caches hold.
