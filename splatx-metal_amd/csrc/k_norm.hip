@@ -551,16 +551,18 @@ struct Split {
 // 1 M x 48 bfloat16, forward: 8 threads 36 us, 2 of three vectors 37). Rows of over a wave take as many whole waves as they
 // need (31,128 x 2056, forward: 5 waves 56 us, 8 would leave a third of them idle). Two rows at a time where they fit the
 // registers: the loads of one alone do not cover the memory's latency (2 M x 96, forward: 133 us against 161, four rows
-// 131; 31,128 x 2056: 56 against 76). From 513 vectors on the forward takes three or four a thread (15,621 x 4100: 56 us, two
+// 131; 31,128 x 2056: 65 against 72), and three where one tensor is read by rows of over a wave (31,128 x 2056: 54, 123,076 x 520
+// 51 against 58, 62,256 x 1028 float 96 against 114, 62,500 x 1024 88 both; with a residual 99 against 101, 2048 91 against 89;
+// rows of a wave 55 against 52). From 513 vectors on the forward takes three or four a thread (15,621 x 4100: 56 us, two
 // 70, one 72), the backward, whose sums take the registers, only from 1025 on (10,666 x 6000: one 85 us, two 114, three 92).
-Split split_of(int64_t width, int size, bool backward) {
+Split split_of(int64_t width, int size, bool backward, bool residual) {
     const int full = 16 / size, vec = width >= full ? full : width >= 4 ? 4 : 1;
     const int64_t n = (width + vec - 1) / vec;
     const auto waves = [](int64_t threads) { return static_cast<int>((threads + kWave - 1) / kWave * kWave); };
     if (n <= (backward ? 1024 : 512)) {
         int t = 1;
         while (t < n) t *= 2;
-        return {vec, t, t <= kWave ? t : waves(n), 1, !backward || t <= 256 ? 2 : 1};
+        return {vec, t, t <= kWave ? t : waves(n), 1, backward ? (t <= 256 ? 2 : 1) : t > kWave && !residual ? 3 : 2};
     }
     for (int k : {3, 4})
         if (n <= 512 * k) return {vec, 512, waves((n + k - 1) / k), k, 1};
@@ -585,6 +587,12 @@ constexpr bool kMayShift = V == 8 && TPR <= kWave;
 template <class T, int V, int TPR, int K>
 void launch(const Split& sp, const NormFwdArgs& a, bool fw, int grid, hipStream_t s) {
     constexpr int R = K == 1 ? 2 : 1;
+    if constexpr (K == 1 && TPR > kWave) {
+        if (sp.rows == 3) {
+            hipLaunchKernelGGL((k_norm_fwd<T, V, TPR, K, 3, Loads::Plain>), dim3(grid), dim3(sp.block()), 0, s, a, fw);
+            return;
+        }
+    }
     if constexpr (kMayShift<V, TPR>) {
         if (!on(4, a, sizeof(T))) {
             hipLaunchKernelGGL((k_norm_fwd<T, V, TPR, K, R, Loads::Shifted>), dim3(grid), dim3(sp.block()), 0, s, a, fw);
@@ -665,7 +673,7 @@ void with_type(ElemType type, F f) {
 
 void layer_norm_fwd(const NormFwdArgs& a, ElemType type, ElemType weight_type, hipStream_t s) {
     if (a.rows == 0) return;
-    const Split sp = split_of(a.width, size_of(type), false);
+    const Split sp = split_of(a.width, size_of(type), false, a.residual != nullptr);
     const bool fw = weight_type == kF32;
     with_type(type, [&](auto t) {
         using T = decltype(t);
@@ -685,7 +693,7 @@ void layer_norm_fwd(const NormFwdArgs& a, ElemType type, ElemType weight_type, h
 // of partial sums at most.
 int norm_bwd_slabs(int64_t rows, int64_t width, ElemType type, bool dh, bool even) {
     const int size = size_of(type);
-    const Split sp = split_of(width, size, true);
+    const Split sp = split_of(width, size, true, false);
     const int64_t per = sp.vec ? int64_t{sp.block_rows()} * sp.rows : 16;
     int64_t each = 4;  // workgroups a unit
     if (sp.vec) {
@@ -700,7 +708,7 @@ int norm_bwd_slabs(int64_t rows, int64_t width, ElemType type, bool dh, bool eve
 
 void layer_norm_bwd(const NormBwdArgs& args, ElemType type, ElemType weight_type, hipStream_t s) {
     NormBwdArgs a = args;
-    const Split sp = split_of(a.width, size_of(type), true);
+    const Split sp = split_of(a.width, size_of(type), true, false);
     const int slabs = norm_bwd_slabs(a.rows, a.width, type, a.dh != nullptr, on(4, a, size_of(type)));
     const bool columns = a.dweight || a.dbias, fw = weight_type == kF32;
     if (!columns) a.partial = nullptr;
