@@ -9,6 +9,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <string>
 #include <vector>
 
@@ -383,6 +384,11 @@ PyObject* adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
             rc = sxh_adamw(c.backend, table.data(), count, &p, &c.queue);
         }
         check(rc);
+        // what autograd has saved of a parameter is no longer what it was
+        for (Py_ssize_t i = 0; i < std::min(count, params.size()); i++) {
+            const at::Tensor& t = params.at(c, i, "params");
+            if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+        }
         return none();
     });
 }

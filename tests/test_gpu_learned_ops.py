@@ -742,3 +742,15 @@ def test_adamw_class(tb, bits):
     for p, q in zip(a, b):
         assert torch.equal(p, q) and torch.isfinite(p.float()).all()
     assert not torch.equal(a[0].detach().cpu(), randn(40, 20, seed=1))
+
+
+def test_adamw_is_seen_by_autograd(tb):
+    """A step between a forward and its backward is an in-place change of what was saved."""
+    import splatx_torch
+    w = torch.nn.Parameter(randn(300, seed=1).cuda())
+    opt = splatx_torch.AdamW(tb, [w])
+    (w * w).sum().backward()
+    late = (w * w).sum()
+    opt.step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        late.backward()
