@@ -269,6 +269,11 @@ PyObject* layer_norm_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+// Item i of a list or tuple, which a number's own conversion to float may have made shorter.
+PyObject* item(PyObject* seq, Py_ssize_t i, const char* name) {
+    if (i >= PySequence_Fast_GET_SIZE(seq)) invalid(std::string(name) + " has changed during the call");
+    return PySequence_Fast_GET_ITEM(seq, i);
+}
 // The tensors of a list or tuple: contiguous, of one of the allowed types.
 struct List {
     PyObject* seq = nullptr;
@@ -280,7 +285,7 @@ struct List {
     ~List() { Py_XDECREF(seq); }
     Py_ssize_t size() const { return PySequence_Fast_GET_SIZE(seq); }
     const at::Tensor& at(const Call& c, Py_ssize_t i, const char* name, const int64_t* numel = nullptr) const {
-        const at::Tensor& t = tensor(c, PySequence_Fast_GET_ITEM(seq, i), name);
+        const at::Tensor& t = tensor(c, item(seq, i, name), name);
         if (!t.is_contiguous()) invalid(std::string(name) + " must be contiguous");
         if (numel && t.numel() != *numel)
             invalid(std::string(name) + "[" + std::to_string(i) + "]: " + std::to_string(t.numel()) + " elements, wanted are " + std::to_string(*numel));
@@ -365,8 +370,8 @@ PyObject* adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
                 t.exp_avg_sq = floats(ev, "exp_avg_sq");
             }
             if (masters) t.master = static_cast<float*>(floats(master.at(c, i, "master", &t.n), "master"));
-            t.lr = rates ? number<double>(PySequence_Fast_GET_ITEM(a[8], i), "lr") : lr;
-            t.weight_decay = decays ? number<double>(PySequence_Fast_GET_ITEM(a[9], i), "weight_decay") : decay;
+            t.lr = rates ? number<double>(item(a[8], i, "lr"), "lr") : lr;
+            t.weight_decay = decays ? number<double>(item(a[9], i, "weight_decay"), "weight_decay") : decay;
         }
         sxh_adamw_params p{};
         p.step = number<int64_t>(a[7], "step");

@@ -754,3 +754,24 @@ def test_adamw_is_seen_by_autograd(tb):
     opt.step()
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         late.backward()
+
+
+def test_lists_that_shrink_during_the_call(tb):
+    lrs, ts = [], [[randn(50, seed=4 * k + i).cuda() for i in range(2)] for k in range(4)]
+
+    class Rate:
+        def __init__(self, gone):
+            self.gone = gone
+
+        def __float__(self):
+            self.gone.clear()
+            return 1e-3
+
+    before = [t.clone() for t in ts[0]]
+    lrs += [Rate(lrs), 1e-3]
+    with pytest.raises(sh.SxInvalidArgument, match="lr has changed"):
+        tb.adamw_step(*ts, step=1, lr=lrs)
+    grads = list(ts[1])
+    with pytest.raises(sh.SxInvalidArgument, match="grads has changed"):
+        tb.adamw_step(ts[0], grads, ts[2], ts[3], step=1, lr=[Rate(grads), 1e-3])
+    assert all(torch.equal(a, b) for a, b in zip(ts[0], before))
