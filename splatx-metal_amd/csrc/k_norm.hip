@@ -549,7 +549,7 @@ struct Split {
 // A vector of 16 bytes a thread up to a workgroup: of the splits that hold a row this one was the fastest or within 3 %
 // throughout (16,383 x 2048 half, backward: a workgroup of 256 40 us, 128 threads of two vectors 44, a wave of four 57;
 // 1 M x 48 bfloat16, forward: 8 threads 36 us, 2 of three vectors 37). Rows of over a wave take as many whole waves as they
-// need (31,128 x 2056, forward: 5 waves 56 us, 8 would leave a third of them idle). Two rows at a time where they fit the
+// need (31,128 x 2056, forward: 5 waves 54 us, 8 would leave a third of them idle). Two rows at a time where they fit the
 // registers: the loads of one alone do not cover the memory's latency (2 M x 96, forward: 133 us against 161, four rows
 // 131; 31,128 x 2056: 65 against 72), and three where one tensor is read by rows of over a wave (31,128 x 2056: 54, 123,076 x 520
 // 51 against 58, 62,256 x 1028 float 96 against 114, 62,500 x 1024 88 both; with a residual 99 against 101, 2048 91 against 89;
