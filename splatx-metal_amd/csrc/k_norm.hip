@@ -465,12 +465,12 @@ __global__ void __launch_bounds__(kWideBlock) k_norm_fwd_wide(NormFwdArgs a, boo
             }
         });
         row_sums<kWideBlock>(sq);
-        const float rstd = 1.0f / __builtin_sqrtf(sq[0] / static_cast<float>(a.width) + a.eps), at_zero = -mean * rstd;
+        const float rstd = 1.0f / __builtin_sqrtf(sq[0] / static_cast<float>(a.width) + a.eps);
         each_vector<V>(a.width, [&](int at, int) {
             Floats<V> y = floats<T, V>(load_raw<V>(from + at));
             const Floats<V> w = load_weights<T, V>(a.weight, at, float_weights, 1.0f), b = load_weights<T, V>(a.bias, at, float_weights, 0.0f);
 #pragma unroll
-            for (int e = 0; e < V; e++) y[e] = __builtin_fmaf(__builtin_fmaf(y[e], rstd, at_zero), w[e], b[e]);
+            for (int e = 0; e < V; e++) y[e] = __builtin_fmaf((y[e] - mean) * rstd, w[e], b[e]);
             store_raw<V>(py + at, raw<T, V>(y));
         });
         if (a.mean && threadIdx.x == 0) {
