@@ -28,3 +28,18 @@ def test_layer_norm_long_rows_about_their_exact_mean(tb, width, dtype):
     # rstd: the squares' sum is exact too, a quotient, a root and a quotient of it half a unit each; then two products and a sum
     bound = 8 * ref.U32 * (w.double() * xhat).abs() + 2 * ref.U32 * (want.abs() + b.double().abs())
     within(y, want, bound + ref.UNIT[dtype] * want.abs() + ref.TINY[dtype], "y")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_layer_norm_rows_of_one_value_give_the_bias(tb, dtype):
+    """At every width up to 6000: a row of one value whose sums are exact in any order (whole numbers of few bits) has that
+    value as its mean, and the bias as its output, to the bit."""
+    x = torch.tensor([100.0, 1000.0, -3000.0, 117 * 512.0, 0.0]).to(dtype).cuda()
+    b = randn(6000, seed=1).cuda()
+    wrong = torch.zeros(6001, dtype=torch.int64, device="cuda")
+    for width in range(1, 6001):
+        if width % 1000 == 1:
+            print(dtype, "width", width, flush=True)
+        y, _, mean, _ = tb.layer_norm_fwd(x[:, None].expand(5, width).contiguous(), None, b[:width])
+        wrong[width] = (y != b[:width].to(dtype)).sum() + (mean != x.float()).sum()
+    assert not wrong.any(), f"{int((wrong > 0).sum())} widths, first {wrong.nonzero()[:8].flatten().tolist()}"
