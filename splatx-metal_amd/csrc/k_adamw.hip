@@ -186,11 +186,11 @@ __device__ inline AdamStep adam_one(const AdamTable& t, float decay, float rate,
 // 314 through the caches; below it takes as long or a little longer (1.2 M elements: 9.1 against 7.6).
 template <bool ONCE>
 __global__ void __launch_bounds__(kBlock) k_adamw(AdamTable t) {
-    const int k = tensor_of(t.first, t.tensors, blockIdx.x);
+    const int chunk = t.from + static_cast<int>(blockIdx.x), k = tensor_of(t.first, t.tensors, chunk);
     const AdamTensor a = t.t[k];
     float c;
     if (!grad_factor(t, &c)) return;
-    const int64_t begin = int64_t{static_cast<int>(blockIdx.x) - t.first[k]} * kAdamChunk - adam_lead(a.m), end = min(begin + kAdamChunk, a.n);
+    const int64_t begin = int64_t{chunk - t.first[k]} * kAdamChunk - adam_lead(a.m), end = min(begin + kAdamChunk, a.n);
     const float* from = a.param_type == kF32 ? static_cast<const float*>(a.param) : a.master;
     float *am = static_cast<float*>(a.m), *av = static_cast<float*>(a.v);
 #pragma unroll 1
@@ -269,12 +269,12 @@ __device__ inline uint32_t encode(const float (&u)[4], const uint32_t (&bits)[4]
 // (5.9 M). A wave's 330 vector instructions for its block would issue in 240 us of those 310: close behind the memory.
 template <bool ONCE>
 __global__ void __launch_bounds__(kBlock) k_adamw8(AdamTable t) {
-    const int k = tensor_of(t.first, t.tensors, blockIdx.x);
+    const int chunk = t.from + static_cast<int>(blockIdx.x), k = tensor_of(t.first, t.tensors, chunk);
     const AdamTensor a = t.t[k];
     float c;
     if (!grad_factor(t, &c)) return;
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int64_t block = int64_t{static_cast<int>(blockIdx.x) - t.first[k]} * (kAdamChunk / kAdamBlock) + wave;
+    const int64_t block = int64_t{chunk - t.first[k]} * (kAdamChunk / kAdamBlock) + wave;
     const int64_t i = block * kAdamBlock + lane * 4;
     if (block * kAdamBlock >= a.n) return;
     static_assert(kAdamChunk / kAdamBlock == kBlock / kWave && kAdamBlock == 4 * kWave);
@@ -356,16 +356,12 @@ uint32_t adam_key(uint64_t seed, int64_t step, int64_t tensor) {
     return k;
 }
 
-void adamw(const AdamTable& t, bool eight_bits, bool once, hipStream_t s) {
-    const dim3 grid(t.first[t.tensors]);
-    if (grid.x == 0) return;
-    if (eight_bits) {
-        if (once) hipLaunchKernelGGL(k_adamw8<true>, grid, dim3(kBlock), 0, s, t);
-        else hipLaunchKernelGGL(k_adamw8<false>, grid, dim3(kBlock), 0, s, t);
-    } else {
-        if (once) hipLaunchKernelGGL(k_adamw<true>, grid, dim3(kBlock), 0, s, t);
-        else hipLaunchKernelGGL(k_adamw<false>, grid, dim3(kBlock), 0, s, t);
-    }
+void adamw(AdamTable& t, bool eight_bits, bool once, hipStream_t s) {
+    const auto kernel = eight_bits ? (once ? k_adamw8<true> : k_adamw8<false>) : (once ? k_adamw<true> : k_adamw<false>);
+    constexpr int kMostGrid = ((int64_t{1} << 32) - 1) / kBlock;  // a launch has fewer than 2^32 threads
+    const int chunks = t.first[t.tensors];
+    for (t.from = 0; t.from < chunks; t.from += kMostGrid)
+        hipLaunchKernelGGL(kernel, dim3(std::min(chunks - t.from, kMostGrid)), dim3(kBlock), 0, s, t);
 }
 
 }  // namespace sxk

@@ -385,7 +385,7 @@ int32_t sxh_adamw(sxh_backend* b, const sxh_adamw_tensor* tensors, int64_t n_ten
             sxk::adamw(t, eight, total > kKept, on.stream());
             t.tensors = 0;
         };
-        constexpr int64_t kMostChunks = int64_t{1} << 30;  // of a launch
+        constexpr int64_t kMostChunks = int64_t{1} << 30;  // of a table (a tensor of 2^40 elements has no more, and a lead's one)
         for (int64_t i = 0; i < n_tensors; i++) {
             const sxh_adamw_tensor& x = tensors[i];
             if (!x.n) continue;

@@ -69,6 +69,7 @@ struct AdamTable {
     AdamTensor t[kAdamTensors];
     int32_t first[kAdamTensors + 1];  // tensor i has the launch's chunks [first[i], first[i + 1])
     int tensors;
+    int from;  // the launch's first chunk
     const float* grad_norm;
     float max_norm, grad_scale, b1, b2, c1, c2, root_c2, eps;  // c = 1 - b; root_c2 = 1 / sqrt(1 - b2^step)
 };
@@ -78,7 +79,7 @@ constexpr int kAdamChunk = 1024;  // elements of a workgroup
 __host__ __device__ inline int adam_lead(const void* m) { return static_cast<int>(reinterpret_cast<uintptr_t>(m) / 4 % 32); }
 // The key of the rounding of the call's tensor.
 uint32_t adam_key(uint64_t seed, int64_t step, int64_t tensor);
-// `once`: the call's tensors are more than the caches hold.
-void adamw(const AdamTable& t, bool eight_bits, bool once, hipStream_t s);
+// In as many launches as the table's chunks take. `once`: the call's tensors are more than the caches hold.
+void adamw(AdamTable& t, bool eight_bits, bool once, hipStream_t s);
 
 }  // namespace sxk

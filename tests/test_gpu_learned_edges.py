@@ -43,3 +43,32 @@ def test_layer_norm_rows_of_one_value_give_the_bias(tb, dtype):
         y, _, mean, _ = tb.layer_norm_fwd(x[:, None].expand(5, width).contiguous(), None, b[:width])
         wrong[width] = (y != b[:width].to(dtype)).sum() + (mean != x.float()).sum()
     assert not wrong.any(), f"{int((wrong > 0).sum())} widths, first {wrong.nonzero()[:8].flatten().tolist()}"
+
+
+def test_adamw_of_more_elements_than_a_launch(tb):
+    """2^34 and some elements in 8 bits, gradients in bfloat16 (137 GB): a launch takes 2^34 - 1024 of them."""
+    import math
+    torch.cuda.empty_cache()
+    border, n = 2 ** 34 - 1024, 2 ** 34 + 5003
+    if torch.cuda.mem_get_info()[0] < 150 << 30:
+        pytest.skip("needs 150 GiB of device memory")
+    p, g = torch.zeros(n, device="cuda"), torch.zeros(n, dtype=BF16, device="cuda")
+    m, r = (torch.zeros(n, dtype=torch.uint8, device="cuda") for _ in range(2))
+    ms, rs = (torch.zeros(-(-n // 256), device="cuda") for _ in range(2))
+    grads, places = randn(3000, seed=1, dtype=BF16), [(7, 507), (border - 500, border + 1000), (n - 1000, n)]
+    for at, (i, j) in zip((0, 500, 2000), places):
+        g[i:j] = grads[at:at + j - i].cuda()
+    tb.adamw_step([p], [g], [m], [r], step=1, lr=1e-2, b1=0.9, b2=0.999, eps=1e-8, exp_avg_scale=[ms], exp_avg_sq_scale=[rs], seed=1)
+    new = ref.adamw(torch.zeros(3000), grads, torch.zeros(3000), torch.zeros(3000), step=1, lr=1e-2, weight_decay=0.0, b1=0.9, b2=0.999, eps=1e-8)
+    got = torch.cat([p[i:j].cpu() for i, j in places])
+    within(got, new[0], 1e-2 * 40 * ref.U32, "param")
+    codes = torch.cat([m[i:j].cpu() for i, j in places])
+    assert ((codes & 0x7F) > 0)[grads.abs() > 0.1].all()
+    for i, j in places:
+        p[i:j] = 0
+    for i in range(0, n, 1 << 31):
+        assert not p[i:i + (1 << 31)].any(), i
+    want = math.sqrt(float(grads.double().square().sum()))
+    assert abs(float(tb.grad_norm([g])) - want) <= 2 * ref.U32 * want
+    del p, g, m, r, ms, rs
+    torch.cuda.empty_cache()
