@@ -38,24 +38,32 @@ struct Call {
     int device;
     sxh_queue queue;
 };
+// An argument whose conversion failed for what it is; any other exception of the conversion (an interrupt, an error of the device
+// whose tensor it is) is the caller's as it came.
+[[noreturn]] void not_converted(const std::string& msg) {
+    if (PyErr_ExceptionMatches(PyExc_TypeError) || PyErr_ExceptionMatches(PyExc_ValueError) || PyErr_ExceptionMatches(PyExc_OverflowError)) {
+        PyErr_Clear();
+        invalid(msg);
+    }
+    throw Raised{};
+}
+bool flag(PyObject* o) {
+    const int v = PyObject_IsTrue(o);
+    if (v < 0) throw Raised{};
+    return v != 0;
+}
 template <class T>
 T number(PyObject* o, const char* name);
 template <>
 double number<double>(PyObject* o, const char* name) {
     const double v = PyFloat_AsDouble(o);
-    if (v == -1.0 && PyErr_Occurred()) {
-        PyErr_Clear();
-        invalid(std::string(name) + " must be a number");
-    }
+    if (v == -1.0 && PyErr_Occurred()) not_converted(std::string(name) + " must be a number");
     return v;
 }
 template <>
 int64_t number<int64_t>(PyObject* o, const char* name) {
     const long long v = PyLong_AsLongLong(o);
-    if (v == -1 && PyErr_Occurred()) {
-        PyErr_Clear();
-        invalid(std::string(name) + " must be a whole number of 64 bits");
-    }
+    if (v == -1 && PyErr_Occurred()) not_converted(std::string(name) + " must be a whole number of 64 bits");
     return v;
 }
 template <>
@@ -63,10 +71,7 @@ uint64_t number<uint64_t>(PyObject* o, const char* name) {
     PyObject* whole = PyNumber_Index(o);
     const unsigned long long v = whole ? PyLong_AsUnsignedLongLong(whole) : ~0ull;
     Py_XDECREF(whole);
-    if (v == ~0ull && PyErr_Occurred()) {
-        PyErr_Clear();
-        invalid(std::string(name) + " must be a whole number of 0..2^64 - 1");
-    }
+    if (v == ~0ull && PyErr_Occurred()) not_converted(std::string(name) + " must be a whole number of 0..2^64 - 1");
     return v;
 }
 
@@ -161,6 +166,8 @@ PyObject* guarded(Py_ssize_t got, Py_ssize_t n, F&& f) {
 PyObject* layer_norm_fwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded(n, 9, [&] {
         const Call c = call_of(a);
+        const double eps = number<double>(a[6], "eps");
+        const bool add = given(a[7]), stats = flag(a[8]);
         const Rows x = rows_of(c, a[3], "x");
         sxh_layer_norm_inputs in{};
         in.x = x.p; in.rows = x.rows; in.width = x.width; in.x_stride = x.stride;
@@ -174,8 +181,7 @@ PyObject* layer_norm_fwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
             wt = bt;
         }
         in.weight_type = static_cast<uint8_t>(wt);
-        in.eps = static_cast<float>(number<double>(a[6], "eps"));
-        const bool add = given(a[7]), stats = PyObject_IsTrue(a[8]);
+        in.eps = static_cast<float>(eps);
         if (add) {
             const Rows r = rows_of(c, a[7], "residual", &x);
             in.residual = r.p;
@@ -218,6 +224,7 @@ PyObject* layer_norm_fwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* layer_norm_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded(n, 12, [&] {
         const Call c = call_of(a);
+        const bool want_dx = flag(a[9]), want_dweight = flag(a[10]), want_dbias = flag(a[11]);
         const Rows h = rows_of(c, a[4], "h"), dy = rows_of(c, a[3], "dy", &h);
         sxh_layer_norm_grads_in in{};
         in.dy = dy.p; in.h = h.p; in.dy_stride = dy.stride; in.h_stride = h.stride;
@@ -232,7 +239,6 @@ PyObject* layer_norm_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
             in.dh = dh.p;
             in.dh_stride = dh.stride;
         }
-        const bool want_dx = PyObject_IsTrue(a[9]), want_dweight = PyObject_IsTrue(a[10]), want_dbias = PyObject_IsTrue(a[11]);
         at::Tensor dx, dweight, dbias, work;
         int32_t rc;
         {

@@ -1,0 +1,52 @@
+"""The learned heads' calls on tensors where a program does what a call does not expect (no GPU use)."""
+import pytest
+import torch
+
+
+@pytest.fixture(scope="module")
+def st():
+    import splatx_torch
+    return splatx_torch
+
+
+class Raising:
+    """A number or a truth value whose conversion raises."""
+
+    def __init__(self, error):
+        self.error = error
+
+    def _raise(self):
+        raise self.error
+
+    __float__ = __bool__ = __index__ = _raise
+
+
+def adamw(ops, **k):
+    a = dict(params=[], grads=[], m=[], v=[], step=1, lr=1e-3, weight_decay=0.0, b1=0.9, b2=0.999, eps=1e-8, master=None, grad_scale=1.0,
+             grad_norm=None, max_norm=0.0, m_scale=None, v_scale=None, seed=0)
+    assert k.keys() <= a.keys()
+    return ops.adamw(0, 0, 0, *{**a, **k}.values())
+
+
+@pytest.mark.parametrize("error", [KeyboardInterrupt, ZeroDivisionError, MemoryError, RuntimeError])
+def test_exceptions_of_a_conversion_are_the_callers(st, error):
+    ops, x, bad = st._extension(), torch.ones(4, 8), Raising(error)
+    for k in ("step", "lr", "weight_decay", "b1", "b2", "eps", "grad_scale", "max_norm", "seed"):
+        with pytest.raises(error):
+            adamw(ops, **{k: bad})
+    with pytest.raises(error):
+        ops.layer_norm_fwd(0, 0, 0, x, None, None, bad, None, True)
+    with pytest.raises(error):
+        ops.layer_norm_fwd(0, 0, 0, x, None, None, 1e-5, None, bad)
+    for k in range(3):
+        with pytest.raises(error):
+            ops.layer_norm_bwd(0, 0, 0, x, x, x, x, None, None, *[bad if i == k else True for i in range(3)])
+
+
+def test_what_is_no_number_is_refused(st):
+    import splatx_hip as sh
+    ops = st._extension()
+    for bad in (Raising(TypeError), Raising(ValueError), Raising(OverflowError), "x", None, 10 ** 400):
+        for k in ("lr", "step", "seed"):
+            with pytest.raises(sh.SxInvalidArgument):
+                adamw(ops, **{k: bad})
