@@ -9,7 +9,6 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
-#include <algorithm>
 #include <string>
 #include <vector>
 
@@ -280,9 +279,19 @@ PyObject* item(PyObject* seq, Py_ssize_t i, const char* name) {
     if (i >= PySequence_Fast_GET_SIZE(seq)) invalid(std::string(name) + " has changed during the call");
     return PySequence_Fast_GET_ITEM(seq, i);
 }
-// The tensors of a list or tuple: contiguous, of one of the allowed types.
+// Item i of a list or tuple as a number; its conversion may take it out of the list.
+double number_of(PyObject* seq, Py_ssize_t i, const char* name) {
+    struct Held {
+        PyObject* o;
+        ~Held() { Py_DECREF(o); }
+    } const held{Py_NewRef(item(seq, i, name))};
+    return number<double>(held.o, name);
+}
+// The tensors of a list or tuple: contiguous, of one of the allowed types. Those that have been asked for live on with it,
+// whatever becomes of the list while other Python threads run.
 struct List {
     PyObject* seq = nullptr;
+    std::vector<at::Tensor> held;
     List(PyObject* o, const char* name) {
         if (!PyList_Check(o) && !PyTuple_Check(o)) invalid(std::string(name) + " must be a list of tensors");
         seq = Py_NewRef(o);
@@ -290,8 +299,9 @@ struct List {
     List(const List&) = delete;
     ~List() { Py_XDECREF(seq); }
     Py_ssize_t size() const { return PySequence_Fast_GET_SIZE(seq); }
-    const at::Tensor& at(const Call& c, Py_ssize_t i, const char* name, const int64_t* numel = nullptr) const {
-        const at::Tensor& t = tensor(c, item(seq, i, name), name);
+    const at::Tensor& at(const Call& c, Py_ssize_t i, const char* name, const int64_t* numel = nullptr) {
+        if (held.empty()) held.reserve(static_cast<size_t>(size()));
+        const at::Tensor& t = held.emplace_back(tensor(c, item(seq, i, name), name));
         if (!t.is_contiguous()) invalid(std::string(name) + " must be contiguous");
         if (numel && t.numel() != *numel)
             invalid(std::string(name) + "[" + std::to_string(i) + "]: " + std::to_string(t.numel()) + " elements, wanted are " + std::to_string(*numel));
@@ -312,7 +322,7 @@ uint8_t any_type(const at::Tensor& t, const char* name) {
 PyObject* grad_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded(n, 4, [&] {
         const Call c = call_of(a);
-        const List grads(a[3], "grads");
+        List grads(a[3], "grads");
         const Py_ssize_t count = grads.size();
         std::vector<sxh_norm_tensor> table(static_cast<size_t>(count));
         for (Py_ssize_t i = 0; i < count; i++) {
@@ -339,11 +349,11 @@ PyObject* grad_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded(n, 20, [&] {
         const Call c = call_of(a);
-        const List params(a[3], "params"), grads(a[4], "grads"), m(a[5], "exp_avg"), v(a[6], "exp_avg_sq");
+        List params(a[3], "params"), grads(a[4], "grads"), m(a[5], "exp_avg"), v(a[6], "exp_avg_sq");
         const bool masters = given(a[13]), eight = given(a[17]);
         if (eight != given(a[18])) invalid("exp_avg_scale and exp_avg_sq_scale are given together");
-        const List master(masters ? a[13] : a[3], "master"), m_scale(eight ? a[17] : a[3], "exp_avg_scale");
-        const List v_scale(eight ? a[18] : a[3], "exp_avg_sq_scale");
+        List master(masters ? a[13] : a[3], "master"), m_scale(eight ? a[17] : a[3], "exp_avg_scale");
+        List v_scale(eight ? a[18] : a[3], "exp_avg_sq_scale");
         const Py_ssize_t count = params.size();
         for (const List* l : {&grads, &m, &v, &master, &m_scale, &v_scale})
             if (l->size() != count) invalid("as many gradients, moments, masters and scales as params are wanted");
@@ -353,11 +363,26 @@ PyObject* adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const double lr = rates ? 0.0 : number<double>(a[8], "lr"), decay = decays ? 0.0 : number<double>(a[9], "weight_decay");
         std::vector<sxh_adamw_tensor> table(static_cast<size_t>(count));
         for (Py_ssize_t i = 0; i < count; i++) {
+            table[i].lr = rates ? number_of(a[8], i, "lr") : lr;
+            table[i].weight_decay = decays ? number_of(a[9], i, "weight_decay") : decay;
+        }
+        sxh_adamw_params p{};
+        p.step = number<int64_t>(a[7], "step");
+        p.seed = number<uint64_t>(a[19], "seed");
+        p.b1 = number<double>(a[10], "b1");
+        p.b2 = number<double>(a[11], "b2");
+        p.eps = number<double>(a[12], "eps");
+        p.grad_scale = static_cast<float>(number<double>(a[14], "grad_scale"));
+        p.max_norm = static_cast<float>(number<double>(a[16], "max_norm"));
+        p.state_bits = eight ? 8 : 32;
+        // (all the numbers first: their conversions are the caller's code, which may change the lists)
+        if (given(a[15])) p.grad_norm = static_cast<float*>(vector(c, a[15], "grad_norm", 1, nullptr, SXH_TYPE_F32));
+        for (Py_ssize_t i = 0; i < count; i++) {
             sxh_adamw_tensor& t = table[i];
-            const at::Tensor& p = params.at(c, i, "params");
-            t.n = p.numel();
-            t.param = p.data_ptr();
-            t.param_type = any_type(p, "params");
+            const at::Tensor& param = params.at(c, i, "params");
+            t.n = param.numel();
+            t.param = param.data_ptr();
+            t.param_type = any_type(param, "params");
             const at::Tensor& g = grads.at(c, i, "grads", &t.n);
             t.grad = g.data_ptr();
             t.grad_type = any_type(g, "grads");
@@ -376,19 +401,7 @@ PyObject* adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
                 t.exp_avg_sq = floats(ev, "exp_avg_sq");
             }
             if (masters) t.master = static_cast<float*>(floats(master.at(c, i, "master", &t.n), "master"));
-            t.lr = rates ? number<double>(item(a[8], i, "lr"), "lr") : lr;
-            t.weight_decay = decays ? number<double>(item(a[9], i, "weight_decay"), "weight_decay") : decay;
         }
-        sxh_adamw_params p{};
-        p.step = number<int64_t>(a[7], "step");
-        p.seed = number<uint64_t>(a[19], "seed");
-        p.b1 = number<double>(a[10], "b1");
-        p.b2 = number<double>(a[11], "b2");
-        p.eps = number<double>(a[12], "eps");
-        p.grad_scale = static_cast<float>(number<double>(a[14], "grad_scale"));
-        if (given(a[15])) p.grad_norm = static_cast<float*>(vector(c, a[15], "grad_norm", 1, nullptr, SXH_TYPE_F32));
-        p.max_norm = static_cast<float>(number<double>(a[16], "max_norm"));
-        p.state_bits = eight ? 8 : 32;
         int32_t rc;
         {
             const Unlocked unlocked;
@@ -396,10 +409,8 @@ PyObject* adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
         }
         check(rc);
         // what autograd has saved of a parameter is no longer what it was
-        for (Py_ssize_t i = 0; i < std::min(count, params.size()); i++) {
-            const at::Tensor& t = params.at(c, i, "params");
+        for (const at::Tensor& t : params.held)
             if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
-        }
         return none();
     });
 }

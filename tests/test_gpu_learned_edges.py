@@ -72,3 +72,28 @@ def test_adamw_of_more_elements_than_a_launch(tb):
     assert abs(float(tb.grad_norm([g])) - want) <= 2 * ref.U32 * want
     del p, g, m, r, ms, rs
     torch.cuda.empty_cache()
+
+
+def test_adamw_of_lists_whose_items_are_replaced(tb):
+    """A number's conversion that puts other tensors into the lists: the step is of those that are there once the numbers are
+    known, all of one kind from one list, and autograd hears of the parameter that was stepped."""
+    kinds = [[randn(5000, seed=4 * k + i).cuda() for i in range(2)] for k in range(4)]
+    kinds[3] = [t.square() for t in kinds[3]]
+    others = [[randn(5000, seed=50 + 4 * k + i).cuda() for i in range(2)] for k in range(3)] + [[t.square() for t in kinds[2]]]
+    want = [[t.clone() for t in ts] for ts in others]
+    tb.adamw_step(*want, step=1, lr=1e-3)
+    before = [[t.clone() for t in ts] for ts in kinds]
+
+    class Rate:
+        def __float__(self):
+            for ts, other in zip(lists, others):
+                ts[:] = other
+            return 1e-3
+
+    lists, versions = [list(ts) for ts in kinds], [t._version for t in kinds[0] + others[0]]
+    tb.adamw_step(*lists, step=1, lr=[1e-3, Rate()])
+    for ts, old in zip(kinds, before):
+        assert all(torch.equal(a, b) for a, b in zip(ts, old))
+    for ts, new in zip(others, want):
+        assert all(torch.equal(a, b) for a, b in zip(ts, new))
+    assert [t._version for t in kinds[0]] == versions[:2] and all(t._version > v for t, v in zip(others[0], versions[2:]))
