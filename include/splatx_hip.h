@@ -788,7 +788,8 @@ int32_t sxh_grad_norm(sxh_backend* b, const sxh_norm_tensor* tensors /* host arr
  *   g = c * grad; m = b1 m + (1 - b1) g; v = b2 v + (1 - b2) g^2
  *   param = param (1 - lr weight_decay) - lr / (1 - b1^step) * m / (sqrt(v) / sqrt(1 - b2^step) + eps).
  * With grad_norm the step is left out, no buffer changed, where n is not finite (an overflowed loss scale). The rates
- * and 1 - b^step are formed in 64 bits on the host, the rest in 32.
+ * and 1 - b^step are formed in 64 bits, the rest in 32. A tensor with `taken` has the count of its own steps there in
+ * place of `step`: the call adds this one to it where it is not left out.
  * state_bits 32: exp_avg and exp_avg_sq are float[n], the scales NULL. state_bits 8: exp_avg holds m and exp_avg_sq
  * sqrt(v) as E4M3 bytes [n] (sign, 4 exponent bits of bias 7, 3 of mantissa, 0x7f not a number), each block of 256
  * consecutive elements in units of its float scale [ceil(n / 256)], which is the block's largest finite magnitude /
@@ -810,9 +811,10 @@ typedef struct {
     int64_t n;               /* may be 0 */
     double lr, weight_decay;
     uint8_t param_type, grad_type;
+    int64_t* taken;          /* [2] device, or NULL: the steps that the tensor has taken, and the call's own word */
 } sxh_adamw_tensor;
 typedef struct {
-    int64_t step;            /* 1 for the first */
+    int64_t step;            /* 1 for the first; of tensors with `taken` for the rounding's bits alone */
     uint64_t seed;           /* of the rounding, with state_bits 8 */
     double b1, b2, eps;      /* 0 <= b < 1, eps > 0 */
     const float* grad_norm;  /* [1] device, or NULL */

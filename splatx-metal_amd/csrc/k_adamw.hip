@@ -99,14 +99,29 @@ __global__ void __launch_bounds__(kFewBlock) k_norm_of_sums(const double* __rest
     if (threadIdx.x == 0) norm[0] = static_cast<float>(__builtin_sqrt(sum));
 }
 
+// The gradients' norm without the loss scale; a step whose norm is not finite is left out.
+__device__ inline float scaled_norm(const float* grad_norm, float grad_scale) { return grad_norm ? grad_norm[0] * grad_scale : 0.0f; }
+__device__ inline bool finite(float x) { return fabsf(x) < __builtin_inff(); }
+
 // What the gradients are multiplied by; false: the step is left out.
 __device__ bool grad_factor(const AdamTable& t, float* c) {
+    const float n = scaled_norm(t.grad_norm, t.grad_scale);
     *c = t.grad_scale;
-    if (!t.grad_norm) return true;
-    const float n = t.grad_norm[0] * t.grad_scale;
-    if (!(fabsf(n) < __builtin_inff())) return false;
+    if (!finite(n)) return false;
     if (t.max_norm > 0.0f && n > t.max_norm) *c *= t.max_norm / n;
     return true;
+}
+
+// A lane for each tensor.
+__global__ void __launch_bounds__(kWave) k_count_steps(AdamCounts c) {
+    const int k = threadIdx.x;
+    if (k >= c.tensors || !finite(scaled_norm(c.grad_norm, c.grad_scale))) return;
+    const int64_t step = max(c.taken[k][0], int64_t{0}) + 1;
+    const double by = 1.0 / (1.0 - pow(c.b1, static_cast<double>(step)));
+    float* rates = reinterpret_cast<float*>(c.taken[k] + 1);
+    c.taken[k][0] = step;
+    rates[0] = static_cast<float>(c.lr[k] * by);
+    rates[1] = static_cast<float>(1.0 / sqrt(1.0 - pow(c.b2, static_cast<double>(step))));
 }
 
 // Elements i .. i + E - 1 of a tensor of n as floats, zeros before it and from n on.
@@ -167,12 +182,12 @@ __device__ inline float root(float x) {
 struct AdamStep {
     float m, v, root, p;
 };
-__device__ inline AdamStep adam_one(const AdamTable& t, float decay, float rate, float p, float g, float m, float v) {
+__device__ inline AdamStep adam_one(const AdamTable& t, float decay, float rate, float root_c2, float p, float g, float m, float v) {
     AdamStep s;
     s.m = __builtin_fmaf(t.c1, g, t.b1 * m);
     s.v = __builtin_fmaf(t.c2, g * g, t.b2 * v);
     s.root = root(s.v);
-    s.p = __builtin_fmaf(-rate, s.m * __builtin_amdgcn_rcpf(__builtin_fmaf(s.root, t.root_c2, t.eps)), p * decay);
+    s.p = __builtin_fmaf(-rate, s.m * __builtin_amdgcn_rcpf(__builtin_fmaf(s.root, root_c2, t.eps)), p * decay);
     return s;
 }
 
@@ -193,13 +208,14 @@ __global__ void __launch_bounds__(kBlock) k_adamw(AdamTable t) {
     const int64_t begin = int64_t{chunk - t.first[k]} * kAdamChunk - adam_lead(a.m), end = min(begin + kAdamChunk, a.n);
     const float* from = a.param_type == kF32 ? static_cast<const float*>(a.param) : a.master;
     float *am = static_cast<float*>(a.m), *av = static_cast<float*>(a.v);
+    const float rate = a.rates ? a.rates[0] : a.rate, root_c2 = a.rates ? a.rates[1] : t.root_c2;
 #pragma unroll 1
     for (int64_t i = begin + threadIdx.x * 2; i < end; i += kBlock * 2) {
         Floats<2> p = load_few<2, ONCE>(from, i, a.n), m = load_few<2, ONCE>(am, i, a.n), v = load_few<2, ONCE>(av, i, a.n);
         const Floats<2> g = load_grad<2, ONCE>(a, i);
 #pragma unroll
         for (int j = 0; j < 2; j++) {
-            const AdamStep s = adam_one(t, a.decay, a.rate, p[j], g[j] * c, m[j], v[j]);
+            const AdamStep s = adam_one(t, a.decay, rate, root_c2, p[j], g[j] * c, m[j], v[j]);
             p[j] = s.p;
             m[j] = s.m;
             v[j] = s.v;
@@ -253,7 +269,6 @@ __device__ inline Floats<4> decode(uint32_t w, float scale) {
     const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
     return Floats<4>{lo[0] * scale, lo[1] * scale, hi[0] * scale, hi[1] * scale};
 }
-__device__ inline bool finite(float x) { return fabsf(x) < __builtin_inff(); }
 
 // The codes of four values of at most 448 in magnitude: the hardware adds the high 20 of the random bits to what lies below
 // a code's last bit and cuts off.
@@ -279,6 +294,7 @@ __global__ void __launch_bounds__(kBlock) k_adamw8(AdamTable t) {
     if (block * kAdamBlock >= a.n) return;
     static_assert(kAdamChunk / kAdamBlock == kBlock / kWave && kAdamBlock == 4 * kWave);
     const float* from = a.param_type == kF32 ? static_cast<const float*>(a.param) : a.master;
+    const float rate = a.rates ? a.rates[0] : a.rate, root_c2 = a.rates ? a.rates[1] : t.root_c2;
     const float m_scale = a.m_scale[block], v_scale = a.v_scale[block];
     const uint32_t mc = load_codes<ONCE>(a.m, i, a.n), vc = load_codes<ONCE>(a.v, i, a.n);
     Floats<4> p = load_few<4, ONCE>(from, i, a.n);
@@ -288,7 +304,7 @@ __global__ void __launch_bounds__(kBlock) k_adamw8(AdamTable t) {
     bool good = true;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-        const AdamStep s = adam_one(t, a.decay, a.rate, p[j], g[j] * c, m[j], r[j] * r[j]);
+        const AdamStep s = adam_one(t, a.decay, rate, root_c2, p[j], g[j] * c, m[j], r[j] * r[j]);
         p[j] = s.p;
         um[j] = s.m;
         ur[j] = s.root;
@@ -355,6 +371,8 @@ uint32_t adam_key(uint64_t seed, int64_t step, int64_t tensor) {
         k = mix(k + static_cast<uint32_t>(w) * 0x9E3779B9u);
     return k;
 }
+
+void count_steps(const AdamCounts& c, hipStream_t s) { hipLaunchKernelGGL(k_count_steps, dim3(1), dim3(kWave), 0, s, c); }
 
 void adamw(AdamTable& t, bool eight_bits, bool once, hipStream_t s) {
     const auto kernel = eight_bits ? (once ? k_adamw8<true> : k_adamw8<false>) : (once ? k_adamw<true> : k_adamw<false>);

@@ -329,7 +329,7 @@ int32_t sxh_adamw(sxh_backend* b, const sxh_adamw_tensor* tensors, int64_t n_ten
         DeviceMemory mem(what, b->device);
         std::vector<Rows> written, read;
         size_t total = 0;  // bytes of all
-        written.reserve(static_cast<size_t>(n_tensors) * (eight ? 6 : 4));
+        written.reserve(static_cast<size_t>(n_tensors) * (eight ? 7 : 5));
         read.reserve(static_cast<size_t>(n_tensors) + 1);
         auto range = [&](std::vector<Rows>& to, const void* ptr, int64_t n, size_t e, const char* name) {
             const size_t bytes = static_cast<size_t>(n) * e;
@@ -355,6 +355,7 @@ int32_t sxh_adamw(sxh_backend* b, const sxh_adamw_tensor* tensors, int64_t n_ten
             range(written, t.exp_avg, t.n, state, "exp_avg");
             range(written, t.exp_avg_sq, t.n, state, "exp_avg_sq");
             range(read, t.grad, t.n, type_size(t.grad_type), "grad");
+            if (t.taken) range(written, t.taken, 2, 8, "taken");
             if (eight) {
                 const int64_t blocks = (t.n + sxk::kAdamBlock - 1) / sxk::kAdamBlock;
                 range(written, t.exp_avg_scale, blocks, 4, "exp_avg_scale");
@@ -381,9 +382,12 @@ int32_t sxh_adamw(sxh_backend* b, const sxh_adamw_tensor* tensors, int64_t n_ten
         t.root_c2 = static_cast<float>(1.0 / std::sqrt(1.0 - std::pow(p->b2, step)));
         const double by = 1.0 / (1.0 - std::pow(p->b1, step));
         constexpr size_t kKept = size_t{128} << 20;  // half of the last-level cache
+        sxk::AdamCounts counts{};  // of the table's tensors
+        counts.b1 = p->b1; counts.b2 = p->b2; counts.grad_norm = p->grad_norm; counts.grad_scale = p->grad_scale;
         auto flush = [&] {
+            if (counts.tensors) sxk::count_steps(counts, on.stream());
             sxk::adamw(t, eight, total > kKept, on.stream());
-            t.tensors = 0;
+            t.tensors = counts.tensors = 0;
         };
         constexpr int64_t kMostChunks = int64_t{1} << 30;  // of a table (a tensor of 2^40 elements has no more, and a lead's one)
         for (int64_t i = 0; i < n_tensors; i++) {
@@ -394,6 +398,11 @@ int32_t sxh_adamw(sxh_backend* b, const sxh_adamw_tensor* tensors, int64_t n_ten
             sxk::AdamTensor& a = t.t[t.tensors];
             a.param = x.param; a.master = x.master; a.grad = x.grad; a.m = x.exp_avg; a.v = x.exp_avg_sq;
             a.m_scale = x.exp_avg_scale; a.v_scale = x.exp_avg_sq_scale; a.n = x.n;
+            a.rates = x.taken ? reinterpret_cast<const float*>(x.taken + 1) : nullptr;
+            if (x.taken) {
+                counts.taken[counts.tensors] = x.taken;
+                counts.lr[counts.tensors++] = x.lr;
+            }
             a.decay = static_cast<float>(1.0 - x.lr * x.weight_decay);
             a.rate = static_cast<float>(x.lr * by);
             a.key = eight ? sxk::adam_key(p->seed, p->step, i) : 0;

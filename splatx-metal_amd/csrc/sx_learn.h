@@ -59,6 +59,7 @@ struct AdamTensor {
     const void* grad;
     void *m, *v;
     float *m_scale, *v_scale;
+    const float* rates;  // rate and root_c2 as count_steps leaves them, in place of those here; or null
     int64_t n;
     float decay;     // 1 - lr weight_decay
     float rate;      // lr / (1 - b1^step)
@@ -77,6 +78,17 @@ static_assert(sizeof(AdamTable) <= 4096 && sizeof(NormTable) <= 4096, "a launch'
 constexpr int kAdamChunk = 1024;  // elements of a workgroup
 // Elements of a 32-bit tensor's first chunk that lie before it: chunks begin on lines of 128 bytes of exp_avg.
 __host__ __device__ inline int adam_lead(const void* m) { return static_cast<int>(reinterpret_cast<uintptr_t>(m) / 4 % 32); }
+// Of the tensors that count their own steps: taken[0] goes up by one and taken[1] becomes {rate, root_c2} of that step, where the
+// step is not left out.
+struct AdamCounts {
+    int64_t* taken[kAdamTensors];
+    double lr[kAdamTensors];
+    double b1, b2;
+    const float* grad_norm;
+    float grad_scale;
+    int tensors;
+};
+void count_steps(const AdamCounts& c, hipStream_t s);
 // The key of the rounding of the call's tensor.
 uint32_t adam_key(uint64_t seed, int64_t step, int64_t tensor);
 // In as many launches as the table's chunks take. `once`: the call's tensors are more than the caches hold.

@@ -9,6 +9,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <string>
 #include <vector>
 
@@ -345,18 +346,19 @@ PyObject* grad_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // (backend, device, stream, params, grads, exp_avg, exp_avg_sq, step, lr, weight_decay, b1, b2, eps, master, grad_scale,
-//  grad_norm, max_norm, exp_avg_scale, exp_avg_sq_scale, seed) -> None
+//  grad_norm, max_norm, exp_avg_scale, exp_avg_sq_scale, seed[, taken]) -> None
 PyObject* adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
-    return guarded(n, 20, [&] {
+    return guarded(n, std::max<Py_ssize_t>(20, std::min<Py_ssize_t>(n, 21)), [&] {
         const Call c = call_of(a);
+        const bool counts = n > 20 && given(a[20]);
         List params(a[3], "params"), grads(a[4], "grads"), m(a[5], "exp_avg"), v(a[6], "exp_avg_sq");
         const bool masters = given(a[13]), eight = given(a[17]);
         if (eight != given(a[18])) invalid("exp_avg_scale and exp_avg_sq_scale are given together");
         List master(masters ? a[13] : a[3], "master"), m_scale(eight ? a[17] : a[3], "exp_avg_scale");
-        List v_scale(eight ? a[18] : a[3], "exp_avg_sq_scale");
+        List v_scale(eight ? a[18] : a[3], "exp_avg_sq_scale"), taken(counts ? a[20] : a[3], "taken");
         const Py_ssize_t count = params.size();
-        for (const List* l : {&grads, &m, &v, &master, &m_scale, &v_scale})
-            if (l->size() != count) invalid("as many gradients, moments, masters and scales as params are wanted");
+        for (const List* l : {&grads, &m, &v, &master, &m_scale, &v_scale, &taken})
+            if (l->size() != count) invalid("as many gradients, moments, masters, scales and counts as params are wanted");
         const bool rates = PyList_Check(a[8]) || PyTuple_Check(a[8]), decays = PyList_Check(a[9]) || PyTuple_Check(a[9]);
         if ((rates && PySequence_Fast_GET_SIZE(a[8]) != count) || (decays && PySequence_Fast_GET_SIZE(a[9]) != count))
             invalid("lr and weight_decay are a number, or one for each tensor");
@@ -399,6 +401,12 @@ PyObject* adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
             } else {
                 t.exp_avg = floats(em, "exp_avg");
                 t.exp_avg_sq = floats(ev, "exp_avg_sq");
+            }
+            if (counts) {
+                constexpr int64_t kWords = 2;
+                const at::Tensor& k = taken.at(c, i, "taken", &kWords);
+                if (k.scalar_type() != at::kLong) invalid("taken must be int64");
+                t.taken = static_cast<int64_t*>(k.data_ptr());
             }
             if (masters) t.master = static_cast<float*>(floats(master.at(c, i, "master", &t.n), "master"));
         }

@@ -58,7 +58,7 @@ class AdamWTensor(C.Structure):
     _fields_ = [("param", C.c_void_p), ("master", C.c_void_p), ("grad", C.c_void_p), ("exp_avg", C.c_void_p),
                 ("exp_avg_sq", C.c_void_p), ("exp_avg_scale", C.c_void_p), ("exp_avg_sq_scale", C.c_void_p),
                 ("n", C.c_int64), ("lr", C.c_double), ("weight_decay", C.c_double), ("param_type", C.c_uint8),
-                ("grad_type", C.c_uint8)]
+                ("grad_type", C.c_uint8), ("taken", C.c_void_p)]
 
 
 class AdamWParams(C.Structure):
@@ -140,13 +140,16 @@ class TorchBackend(sh.Backend):
         return self._ops.grad_norm(self._address, self._index, _raw_stream(self._index), grads)
 
     def adamw_step(self, params, grads, exp_avg, exp_avg_sq, *, step, lr, weight_decay=0.0, b1=0.9, b2=0.999, eps=1e-8,
-                   master=None, grad_scale=1.0, grad_norm=None, max_norm=0.0, exp_avg_scale=None, exp_avg_sq_scale=None, seed=0):
+                   master=None, grad_scale=1.0, grad_norm=None, max_norm=0.0, exp_avg_scale=None, exp_avg_sq_scale=None, seed=0,
+                   taken=None):
         """One AdamW step of lists of tensors, in place. `lr` and `weight_decay`: a number, or one for each tensor. `master`:
         float32 copies that the step works on, with 16-bit params. With the scales, exp_avg and exp_avg_sq are float8_e4m3fn
         (or uint8) tensors: m, and the root of v, in units of their block's scale. grad_norm: `grad_norm`'s result of these
-        gradients; where it is not finite the step is left out."""
+        gradients; where it is not finite the step is left out. `taken`: int64 tensors of two elements, each the count of its
+        tensor's own steps and a word of the call's; the bias is corrected by them in place of `step`, and a step that is not
+        left out adds one."""
         self._ops.adamw(self._address, self._index, _raw_stream(self._index), params, grads, exp_avg, exp_avg_sq, step, lr,
-                        weight_decay, b1, b2, eps, master, grad_scale, grad_norm, max_norm, exp_avg_scale, exp_avg_sq_scale, seed)
+                        weight_decay, b1, b2, eps, master, grad_scale, grad_norm, max_norm, exp_avg_scale, exp_avg_sq_scale, seed, taken)
 
 
 class _LayerNorm(torch.autograd.Function):
@@ -187,7 +190,9 @@ class AdamW:
 
     `params`: tensors, or dicts with "params" and their own "lr" or "weight_decay". A step takes the gradients from the
     parameters (one without a gradient is left as it is) and clips their norm to `max_norm` (0: does not); a step whose
-    norm is not finite is left out with `max_norm` or `skip_nonfinite`. It does not wait for the device."""
+    norm is not finite is left out with `max_norm` or `skip_nonfinite`. `steps` counts the calls; a parameter's bias is
+    corrected by the count of its own steps, those without a gradient and those left out not among them. It does not wait
+    for the device."""
 
     def __init__(self, backend: TorchBackend, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, state_bits=32,
                  max_norm=0.0, skip_nonfinite=False, seed=0):
@@ -216,6 +221,7 @@ class AdamW:
                 s[k] = torch.zeros(adamw_blocks(d.numel()), dtype=torch.float32, device=d.device)
         if d.dtype != torch.float32:
             s["master"] = d.float()
+        s["taken"] = torch.zeros(2, dtype=torch.int64, device=d.device)
         return s
 
     def moments(self, i):
@@ -243,7 +249,7 @@ class AdamW:
             if not k:
                 continue
             st = [self.state[at[j]] for j in k]
-            more = {}
+            more = dict(taken=[s["taken"] for s in st])
             if half:
                 more["master"] = [s["master"] for s in st]
             if self.state_bits == 8:
@@ -267,10 +273,12 @@ class AdamW:
     def load_state_dict(self, d):
         if d["state_bits"] != self.state_bits or len(d["state"]) != len(self.state):
             raise sh.SxInvalidArgument("the state is of another form or of other parameters")
-        for s, t in zip(self.state, d["state"]):
+        # (a state of before parameters had counts of their own: all took every step)
+        state = [{"taken": torch.tensor([d["steps"], 0]), **t} for t in d["state"]]
+        for s, t in zip(self.state, state):
             if s.keys() != t.keys() or any(s[k].shape != t[k].shape for k in s):
                 raise sh.SxInvalidArgument("the state is of other parameters")
-        for s, t in zip(self.state, d["state"]):
+        for s, t in zip(self.state, state):
             for k in s:
                 s[k].copy_(t[k])
         self.steps, self.seed = d["steps"], d["seed"]

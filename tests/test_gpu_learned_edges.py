@@ -97,3 +97,116 @@ def test_adamw_of_lists_whose_items_are_replaced(tb):
     for ts, new in zip(others, want):
         assert all(torch.equal(a, b) for a, b in zip(ts, new))
     assert [t._version for t in kinds[0]] == versions[:2] and all(t._version > v for t, v in zip(others[0], versions[2:]))
+
+
+def optimizer_params(dtype=F32):
+    return [torch.nn.Parameter(randn(n, seed=n).to(dtype).cuda()) for n in (700, 3000)]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_adamw_parameters_count_their_own_steps(tb, bits, dtype):
+    """A parameter whose first gradient comes at the sixth step takes its first step then, as it would alone; the second one
+    with no gradient between them as well."""
+    import splatx_torch
+    p = optimizer_params(dtype)
+    opt = splatx_torch.AdamW(tb, p, lr=1e-2, state_bits=bits)
+    for k in range(6):
+        p[0].grad = randn(700, seed=20 + k, dtype=dtype).cuda()
+        p[1].grad = randn(3000, seed=40, dtype=dtype).cuda() if k == 5 else None
+        opt.step()
+    q = optimizer_params(dtype)[1]
+    alone = splatx_torch.AdamW(tb, [q], lr=1e-2, state_bits=bits)
+    q.grad = randn(3000, seed=40, dtype=dtype).cuda()
+    alone.step()
+    assert torch.equal(p[1], q)  # (a first step's parameters do not depend on the moments' rounding)
+    assert [int(s["taken"][0]) for s in opt.state] == [6, 1] and opt.steps == 6
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_steps_left_out_are_not_counted(tb, bits):
+    """Overflowed steps before the first and between others: the parameters go where they would have gone without them."""
+    import splatx_torch
+    p, q = optimizer_params(), optimizer_params()
+    a = splatx_torch.AdamW(tb, p, lr=1e-2, state_bits=bits, max_norm=1e3)
+    b = splatx_torch.AdamW(tb, q, lr=1e-2, state_bits=bits, max_norm=1e3)
+    for k, bad in enumerate((True, True, False, True, False) if bits == 32 else (True, True, False)):
+        for i in (0, 1):
+            g = randn(p[i].numel(), seed=60 + 2 * k + i).cuda()
+            if bad:
+                p[i].grad = g.clone()
+                p[i].grad[5] = float("inf")
+            else:
+                p[i].grad, q[i].grad = g, g
+        a.step()
+        if not bad:
+            b.step()
+    assert all(torch.equal(x, y) for x, y in zip(p, q))
+    assert a.steps > b.steps and [int(s["taken"][0]) for s in a.state] == [b.steps] * 2
+
+
+def test_adamw_loads_states_without_counts(tb):
+    """A state saved before parameters counted their own steps: all of them took every step."""
+    import splatx_torch
+    p = optimizer_params()
+    opt = splatx_torch.AdamW(tb, p)
+    for k in range(3):
+        for x in p:
+            x.grad = randn(x.numel(), seed=70 + k).cuda()
+        opt.step()
+    d = opt.state_dict()
+    for s in d["state"]:
+        del s["taken"]
+    q = [torch.nn.Parameter(x.detach().clone()) for x in p]
+    other = splatx_torch.AdamW(tb, q)
+    other.load_state_dict(d)
+    for x, y in zip(p, q):
+        x.grad = y.grad = randn(x.numel(), seed=80).cuda()
+    opt.step(), other.step()
+    assert all(torch.equal(x, y) for x, y in zip(p, q))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("count", [1, 36, 80])
+def test_adamw_step_by_counts_on_the_device(tb, bits, count):
+    """Some tensors of a call with counts of their own, more than one launch takes; and the counts refused where they are wrong."""
+    import splatx_hip as sh
+    from test_gpu_learned_ops import HYPER, adam_bound, coded
+    taken = [torch.tensor([k % 7, 0]).cuda() for k in range(count)]
+    p, g, m = ([randn(100 + k, seed=3 * k + j) for k in range(count)] for j in range(3))
+    r = [randn(100 + k, seed=900 + k).abs() for k in range(count)]
+    if bits == 8:
+        (m, mc, ms), (r, rc, rs) = coded(m), coded(r)
+        dev = [[t.cuda() for t in ts] for ts in (p, g, mc, rc)]
+        more = dict(exp_avg_scale=[t.cuda() for t in ms], exp_avg_sq_scale=[t.cuda() for t in rs])
+    else:
+        dev, more = [[t.cuda() for t in ts] for ts in (p, g, m, [t.square() for t in r])], {}
+    tb.adamw_step(*dev, step=50, lr=[1e-3 * (k + 1) for k in range(count)], taken=taken, **more, **HYPER)
+    for k in range(count):
+        v = r[k].square()
+        new = ref.adamw(p[k], g[k], m[k], v, step=k % 7 + 1, lr=1e-3 * (k + 1), weight_decay=0.0, **HYPER)
+        within(dev[0][k], new[0], 2 * adam_bound(p[k], g[k], m[k], v, new, 1e-3 * (k + 1), k % 7 + 1)[0], "param")
+        assert int(taken[k][0]) == k % 7 + 1
+    for bad in ([t.int() for t in taken], [t[:1] for t in taken], taken[:-1], [t.cpu() for t in taken], [dev[3][0]] * count):
+        with pytest.raises(sh.SxInvalidArgument):
+            tb.adamw_step(*dev, step=50, lr=1e-3, taken=bad, **more, **HYPER)
+
+
+def test_adamw_in_a_graph_counts_its_replays(tb):
+    """Captured with counts on the device, each replay is the next step."""
+    p, m, v = (randn(2000, seed=1).cuda(), torch.zeros(2000).cuda(), torch.zeros(2000).cuda())
+    g, taken = torch.zeros(2000).cuda(), torch.zeros(2, dtype=torch.int64).cuda()
+    q = [t.clone() for t in (p, m, v, taken)]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        tb.adamw_step([p], [g], [m], [v], step=1, lr=1e-2, taken=[taken])
+    for k in range(4):
+        g.copy_(randn(2000, seed=90 + k))
+        tb.adamw_step([q[0]], [g], [q[1]], [q[2]], step=1, lr=1e-2, taken=[q[3]])
+        torch.cuda.synchronize()
+        graph.replay()
+        for a, b in zip((p, m, v), q):
+            assert torch.equal(a, b), k
+        assert int(taken[0]) == k + 1
+        (torch.randn(1000, device="cuda") ** 2).sum().item()
