@@ -288,11 +288,19 @@ double number_of(PyObject* seq, Py_ssize_t i, const char* name) {
     } const held{Py_NewRef(item(seq, i, name))};
     return number<double>(held.o, name);
 }
-// The tensors of a list or tuple: contiguous, of one of the allowed types. Those that have been asked for live on with it,
-// whatever becomes of the list while other Python threads run.
+// What a call's lists have been asked for: it lives until the call ends, whatever becomes of the lists while other Python threads
+// run. (Counted as Python's objects: as many counts of torch's own, which are atomic, take a call of fifty tensors 1 us more.)
+struct Kept {
+    std::vector<PyObject*> objects;
+    explicit Kept(Py_ssize_t most) { objects.reserve(static_cast<size_t>(most)); }
+    Kept(const Kept&) = delete;
+    ~Kept() {
+        for (PyObject* o : objects) Py_DECREF(o);
+    }
+};
+// The tensors of a list or tuple: contiguous, of one of the allowed types.
 struct List {
     PyObject* seq = nullptr;
-    std::vector<at::Tensor> held;
     List(PyObject* o, const char* name) {
         if (!PyList_Check(o) && !PyTuple_Check(o)) invalid(std::string(name) + " must be a list of tensors");
         seq = Py_NewRef(o);
@@ -300,9 +308,10 @@ struct List {
     List(const List&) = delete;
     ~List() { Py_XDECREF(seq); }
     Py_ssize_t size() const { return PySequence_Fast_GET_SIZE(seq); }
-    const at::Tensor& at(const Call& c, Py_ssize_t i, const char* name, const int64_t* numel = nullptr) {
-        if (held.empty()) held.reserve(static_cast<size_t>(size()));
-        const at::Tensor& t = held.emplace_back(tensor(c, item(seq, i, name), name));
+    const at::Tensor& at(Kept& kept, const Call& c, Py_ssize_t i, const char* name, const int64_t* numel = nullptr) const {
+        PyObject* o = item(seq, i, name);
+        const at::Tensor& t = tensor(c, o, name);
+        kept.objects.push_back(Py_NewRef(o));
         if (!t.is_contiguous()) invalid(std::string(name) + " must be contiguous");
         if (numel && t.numel() != *numel)
             invalid(std::string(name) + "[" + std::to_string(i) + "]: " + std::to_string(t.numel()) + " elements, wanted are " + std::to_string(*numel));
@@ -323,11 +332,12 @@ uint8_t any_type(const at::Tensor& t, const char* name) {
 PyObject* grad_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded(n, 4, [&] {
         const Call c = call_of(a);
-        List grads(a[3], "grads");
+        const List grads(a[3], "grads");
         const Py_ssize_t count = grads.size();
+        Kept kept(count);
         std::vector<sxh_norm_tensor> table(static_cast<size_t>(count));
         for (Py_ssize_t i = 0; i < count; i++) {
-            const at::Tensor& t = grads.at(c, i, "grads");
+            const at::Tensor& t = grads.at(kept, c, i, "grads");
             table[i] = {t.data_ptr(), t.numel(), any_type(t, "grads")};
         }
         at::Tensor norm, work;
@@ -351,12 +361,14 @@ PyObject* adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded(n, std::max<Py_ssize_t>(20, std::min<Py_ssize_t>(n, 21)), [&] {
         const Call c = call_of(a);
         const bool counts = n > 20 && given(a[20]);
-        List params(a[3], "params"), grads(a[4], "grads"), m(a[5], "exp_avg"), v(a[6], "exp_avg_sq");
+        const List params(a[3], "params"), grads(a[4], "grads"), m(a[5], "exp_avg"), v(a[6], "exp_avg_sq");
         const bool masters = given(a[13]), eight = given(a[17]);
         if (eight != given(a[18])) invalid("exp_avg_scale and exp_avg_sq_scale are given together");
-        List master(masters ? a[13] : a[3], "master"), m_scale(eight ? a[17] : a[3], "exp_avg_scale");
-        List v_scale(eight ? a[18] : a[3], "exp_avg_sq_scale"), taken(counts ? a[20] : a[3], "taken");
+        const List master(masters ? a[13] : a[3], "master"), m_scale(eight ? a[17] : a[3], "exp_avg_scale");
+        const List v_scale(eight ? a[18] : a[3], "exp_avg_sq_scale"), taken(counts ? a[20] : a[3], "taken");
         const Py_ssize_t count = params.size();
+        Kept kept(8 * count);
+        std::vector<const at::Tensor*> stepped(static_cast<size_t>(count));
         for (const List* l : {&grads, &m, &v, &master, &m_scale, &v_scale, &taken})
             if (l->size() != count) invalid("as many gradients, moments, masters, scales and counts as params are wanted");
         const bool rates = PyList_Check(a[8]) || PyTuple_Check(a[8]), decays = PyList_Check(a[9]) || PyTuple_Check(a[9]);
@@ -381,14 +393,14 @@ PyObject* adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (given(a[15])) p.grad_norm = static_cast<float*>(vector(c, a[15], "grad_norm", 1, nullptr, SXH_TYPE_F32));
         for (Py_ssize_t i = 0; i < count; i++) {
             sxh_adamw_tensor& t = table[i];
-            const at::Tensor& param = params.at(c, i, "params");
+            const at::Tensor& param = *(stepped[i] = &params.at(kept, c, i, "params"));
             t.n = param.numel();
             t.param = param.data_ptr();
             t.param_type = any_type(param, "params");
-            const at::Tensor& g = grads.at(c, i, "grads", &t.n);
+            const at::Tensor& g = grads.at(kept, c, i, "grads", &t.n);
             t.grad = g.data_ptr();
             t.grad_type = any_type(g, "grads");
-            const at::Tensor &em = m.at(c, i, "exp_avg", &t.n), &ev = v.at(c, i, "exp_avg_sq", &t.n);
+            const at::Tensor &em = m.at(kept, c, i, "exp_avg", &t.n), &ev = v.at(kept, c, i, "exp_avg_sq", &t.n);
             if (eight) {
                 for (const at::Tensor* e : {&em, &ev})
                     if (e->scalar_type() != at::kFloat8_e4m3fn && e->scalar_type() != at::kByte)
@@ -396,19 +408,19 @@ PyObject* adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
                 t.exp_avg = em.data_ptr();
                 t.exp_avg_sq = ev.data_ptr();
                 const int64_t blocks = (t.n + 255) / 256;
-                t.exp_avg_scale = static_cast<float*>(floats(m_scale.at(c, i, "exp_avg_scale", &blocks), "exp_avg_scale"));
-                t.exp_avg_sq_scale = static_cast<float*>(floats(v_scale.at(c, i, "exp_avg_sq_scale", &blocks), "exp_avg_sq_scale"));
+                t.exp_avg_scale = static_cast<float*>(floats(m_scale.at(kept, c, i, "exp_avg_scale", &blocks), "exp_avg_scale"));
+                t.exp_avg_sq_scale = static_cast<float*>(floats(v_scale.at(kept, c, i, "exp_avg_sq_scale", &blocks), "exp_avg_sq_scale"));
             } else {
                 t.exp_avg = floats(em, "exp_avg");
                 t.exp_avg_sq = floats(ev, "exp_avg_sq");
             }
             if (counts) {
                 constexpr int64_t kWords = 2;
-                const at::Tensor& k = taken.at(c, i, "taken", &kWords);
+                const at::Tensor& k = taken.at(kept, c, i, "taken", &kWords);
                 if (k.scalar_type() != at::kLong) invalid("taken must be int64");
                 t.taken = static_cast<int64_t*>(k.data_ptr());
             }
-            if (masters) t.master = static_cast<float*>(floats(master.at(c, i, "master", &t.n), "master"));
+            if (masters) t.master = static_cast<float*>(floats(master.at(kept, c, i, "master", &t.n), "master"));
         }
         int32_t rc;
         {
@@ -417,8 +429,8 @@ PyObject* adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
         }
         check(rc);
         // what autograd has saved of a parameter is no longer what it was
-        for (const at::Tensor& t : params.held)
-            if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+        for (const at::Tensor* t : stepped)
+            if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
         return none();
     });
 }
