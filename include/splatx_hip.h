@@ -821,6 +821,8 @@ typedef struct {
     float max_norm;          /* 0: no clipping */
     float grad_scale;        /* 1 / the loss scale */
     int32_t state_bits;      /* 32 or 8 */
+    int32_t adopt;           /* 0: a 16-bit param is written, not read; 1: an element of it that is not its master's rounding has
+                                been set since the last step (weights loaded), and is what this step begins from */
 } sxh_adamw_params;
 int32_t sxh_adamw(sxh_backend* b, const sxh_adamw_tensor* tensors /* host array */, int64_t n_tensors,
                   const sxh_adamw_params* params, const sxh_queue* q);

@@ -154,6 +154,24 @@ __device__ inline Floats<E> load_grad(const AdamTensor& a, int64_t i) {
     if (a.grad_type == kBf16) return load_few<E, ONCE>(static_cast<const __bf16*>(a.grad), i, a.n);
     return load_few<E, ONCE>(static_cast<const _Float16*>(a.grad), i, a.n);
 }
+// What the step begins from: of a 16-bit parameter its master, with ADOPT where the parameter is still its rounding (else it has
+// been set by someone since).
+template <int E, bool ONCE, class T>
+__device__ inline Floats<E> adopted(const AdamTensor& a, int64_t i, Floats<E> master) {
+    const Floats<E> now = load_few<E, ONCE>(static_cast<const T*>(a.param), i, a.n), was = floats<T, E>(raw<T, E>(master));
+#pragma unroll
+    for (int j = 0; j < E; j++) master[j] = now[j] == was[j] ? master[j] : now[j];
+    return master;
+}
+template <int E, bool ONCE, bool ADOPT>
+__device__ inline Floats<E> load_param(const AdamTensor& a, int64_t i) {
+    const Floats<E> p = load_few<E, ONCE>(a.param_type == kF32 ? static_cast<const float*>(a.param) : a.master, i, a.n);
+    if constexpr (ADOPT) {
+        if (a.param_type == kBf16) return adopted<E, ONCE, __bf16>(a, i, p);
+        if (a.param_type == kF16) return adopted<E, ONCE, _Float16>(a, i, p);
+    }
+    return p;
+}
 // The step's parameter, and where it is a master copy its rounded one.
 template <int E, bool ONCE>
 __device__ inline void store_param(const AdamTensor& a, int64_t i, Floats<E> p) {
@@ -199,19 +217,18 @@ __device__ inline AdamStep adam_one(const AdamTable& t, float decay, float rate,
 // gradients 219 and 185.
 // ONCE, for calls of more than 128 MiB, of which the last-level cache would hold little until the next one: 265 us against
 // 314 through the caches; below it takes as long or a little longer (1.2 M elements: 9.1 against 7.6).
-template <bool ONCE>
+template <bool ONCE, bool ADOPT>
 __global__ void __launch_bounds__(kBlock) k_adamw(AdamTable t) {
     const int chunk = t.from + static_cast<int>(blockIdx.x), k = tensor_of(t.first, t.tensors, chunk);
     const AdamTensor a = t.t[k];
     float c;
     if (!grad_factor(t, &c)) return;
     const int64_t begin = int64_t{chunk - t.first[k]} * kAdamChunk - adam_lead(a.m), end = min(begin + kAdamChunk, a.n);
-    const float* from = a.param_type == kF32 ? static_cast<const float*>(a.param) : a.master;
     float *am = static_cast<float*>(a.m), *av = static_cast<float*>(a.v);
     const float rate = a.rates ? a.rates[0] : a.rate, root_c2 = a.rates ? a.rates[1] : t.root_c2;
 #pragma unroll 1
     for (int64_t i = begin + threadIdx.x * 2; i < end; i += kBlock * 2) {
-        Floats<2> p = load_few<2, ONCE>(from, i, a.n), m = load_few<2, ONCE>(am, i, a.n), v = load_few<2, ONCE>(av, i, a.n);
+        Floats<2> p = load_param<2, ONCE, ADOPT>(a, i), m = load_few<2, ONCE>(am, i, a.n), v = load_few<2, ONCE>(av, i, a.n);
         const Floats<2> g = load_grad<2, ONCE>(a, i);
 #pragma unroll
         for (int j = 0; j < 2; j++) {
@@ -282,7 +299,7 @@ __device__ inline uint32_t encode(const float (&u)[4], const uint32_t (&bits)[4]
 // A wave per block of 256 elements, four side by side a lane: 16 bytes of parameter and of gradient and four of each moment's
 // codes, decoded and encoded by the hardware. Past the caches as above: 310 us against 338 (118 M elements), 19.5 against 19.0
 // (5.9 M). A wave's 330 vector instructions for its block would issue in 240 us of those 310: close behind the memory.
-template <bool ONCE>
+template <bool ONCE, bool ADOPT>
 __global__ void __launch_bounds__(kBlock) k_adamw8(AdamTable t) {
     const int chunk = t.from + static_cast<int>(blockIdx.x), k = tensor_of(t.first, t.tensors, chunk);
     const AdamTensor a = t.t[k];
@@ -293,11 +310,10 @@ __global__ void __launch_bounds__(kBlock) k_adamw8(AdamTable t) {
     const int64_t i = block * kAdamBlock + lane * 4;
     if (block * kAdamBlock >= a.n) return;
     static_assert(kAdamChunk / kAdamBlock == kBlock / kWave && kAdamBlock == 4 * kWave);
-    const float* from = a.param_type == kF32 ? static_cast<const float*>(a.param) : a.master;
     const float rate = a.rates ? a.rates[0] : a.rate, root_c2 = a.rates ? a.rates[1] : t.root_c2;
     const float m_scale = a.m_scale[block], v_scale = a.v_scale[block];
     const uint32_t mc = load_codes<ONCE>(a.m, i, a.n), vc = load_codes<ONCE>(a.v, i, a.n);
-    Floats<4> p = load_few<4, ONCE>(from, i, a.n);
+    Floats<4> p = load_param<4, ONCE, ADOPT>(a, i);
     const Floats<4> g = load_grad<4, ONCE>(a, i);
     const Floats<4> m = decode(mc, m_scale), r = decode(vc, v_scale);
     float um[4], ur[4], top_m = 0.0f, top_r = 0.0f;
@@ -374,8 +390,12 @@ uint32_t adam_key(uint64_t seed, int64_t step, int64_t tensor) {
 
 void count_steps(const AdamCounts& c, hipStream_t s) { hipLaunchKernelGGL(k_count_steps, dim3(1), dim3(kWave), 0, s, c); }
 
-void adamw(AdamTable& t, bool eight_bits, bool once, hipStream_t s) {
-    const auto kernel = eight_bits ? (once ? k_adamw8<true> : k_adamw8<false>) : (once ? k_adamw<true> : k_adamw<false>);
+template <bool ADOPT>
+auto adam_kernel(bool eight_bits, bool once) {
+    return eight_bits ? (once ? k_adamw8<true, ADOPT> : k_adamw8<false, ADOPT>) : (once ? k_adamw<true, ADOPT> : k_adamw<false, ADOPT>);
+}
+void adamw(AdamTable& t, bool eight_bits, bool once, bool adopt, hipStream_t s) {
+    const auto kernel = adopt ? adam_kernel<true>(eight_bits, once) : adam_kernel<false>(eight_bits, once);
     constexpr int kMostGrid = ((int64_t{1} << 32) - 1) / kBlock;  // a launch has fewer than 2^32 threads
     const int chunks = t.first[t.tensors];
     for (t.from = 0; t.from < chunks; t.from += kMostGrid)

@@ -323,6 +323,7 @@ int32_t sxh_adamw(sxh_backend* b, const sxh_adamw_tensor* tensors, int64_t n_ten
         if (!(p->eps >= 1e-30 && p->eps < 1.0)) invalid(what, "eps must be in [1e-30, 1)");
         if (!(p->max_norm >= 0.0f) || !std::isfinite(p->max_norm)) invalid(what, "max_norm must be 0 or more");
         if (!(p->grad_scale > 0.0f) || !std::isfinite(p->grad_scale)) invalid(what, "grad_scale must be positive");
+        if (p->adopt != 0 && p->adopt != 1) invalid(what, "adopt must be 0 or 1");
         if (p->max_norm > 0.0f && !p->grad_norm) invalid(what, "max_norm needs grad_norm");
         if (!b) invalid(what, "null backend");
         const bool eight = p->state_bits == 8;
@@ -386,7 +387,7 @@ int32_t sxh_adamw(sxh_backend* b, const sxh_adamw_tensor* tensors, int64_t n_ten
         counts.b1 = p->b1; counts.b2 = p->b2; counts.grad_norm = p->grad_norm; counts.grad_scale = p->grad_scale;
         auto flush = [&] {
             if (counts.tensors) sxk::count_steps(counts, on.stream());
-            sxk::adamw(t, eight, total > kKept, on.stream());
+            sxk::adamw(t, eight, total > kKept, p->adopt != 0, on.stream());
             t.tensors = counts.tensors = 0;
         };
         constexpr int64_t kMostChunks = int64_t{1} << 30;  // of a table (a tensor of 2^40 elements has no more, and a lead's one)

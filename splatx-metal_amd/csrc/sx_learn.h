@@ -91,7 +91,8 @@ struct AdamCounts {
 void count_steps(const AdamCounts& c, hipStream_t s);
 // The key of the rounding of the call's tensor.
 uint32_t adam_key(uint64_t seed, int64_t step, int64_t tensor);
-// In as many launches as the table's chunks take. `once`: the call's tensors are more than the caches hold.
-void adamw(AdamTable& t, bool eight_bits, bool once, hipStream_t s);
+// In as many launches as the table's chunks take. `once`: the call's tensors are more than the caches hold. `adopt`: parameters
+// that are not their masters' roundings take their places.
+void adamw(AdamTable& t, bool eight_bits, bool once, bool adopt, hipStream_t s);
 
 }  // namespace sxk

@@ -356,9 +356,9 @@ PyObject* grad_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // (backend, device, stream, params, grads, exp_avg, exp_avg_sq, step, lr, weight_decay, b1, b2, eps, master, grad_scale,
-//  grad_norm, max_norm, exp_avg_scale, exp_avg_sq_scale, seed[, taken]) -> None
+//  grad_norm, max_norm, exp_avg_scale, exp_avg_sq_scale, seed[, taken, adopt]) -> None
 PyObject* adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
-    return guarded(n, std::max<Py_ssize_t>(20, std::min<Py_ssize_t>(n, 21)), [&] {
+    return guarded(n, std::max<Py_ssize_t>(20, std::min<Py_ssize_t>(n, 22)), [&] {
         const Call c = call_of(a);
         const bool counts = n > 20 && given(a[20]);
         const List params(a[3], "params"), grads(a[4], "grads"), m(a[5], "exp_avg"), v(a[6], "exp_avg_sq");
@@ -389,6 +389,7 @@ PyObject* adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
         p.grad_scale = static_cast<float>(number<double>(a[14], "grad_scale"));
         p.max_norm = static_cast<float>(number<double>(a[16], "max_norm"));
         p.state_bits = eight ? 8 : 32;
+        p.adopt = n > 21 && flag(a[21]);
         // (all the numbers first: their conversions are the caller's code, which may change the lists)
         if (given(a[15])) p.grad_norm = static_cast<float*>(vector(c, a[15], "grad_norm", 1, nullptr, SXH_TYPE_F32));
         for (Py_ssize_t i = 0; i < count; i++) {

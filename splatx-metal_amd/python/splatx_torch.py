@@ -63,7 +63,8 @@ class AdamWTensor(C.Structure):
 
 class AdamWParams(C.Structure):
     _fields_ = [("step", C.c_int64), ("seed", C.c_uint64), ("b1", C.c_double), ("b2", C.c_double), ("eps", C.c_double),
-                ("grad_norm", C.c_void_p), ("max_norm", C.c_float), ("grad_scale", C.c_float), ("state_bits", C.c_int32)]
+                ("grad_norm", C.c_void_p), ("max_norm", C.c_float), ("grad_scale", C.c_float), ("state_bits", C.c_int32),
+                ("adopt", C.c_int32)]
 
 
 _NORM_ROW = struct.Struct("<QqB7x")  # a NormTensor as bytes: a table of them is these one after another
@@ -141,15 +142,17 @@ class TorchBackend(sh.Backend):
 
     def adamw_step(self, params, grads, exp_avg, exp_avg_sq, *, step, lr, weight_decay=0.0, b1=0.9, b2=0.999, eps=1e-8,
                    master=None, grad_scale=1.0, grad_norm=None, max_norm=0.0, exp_avg_scale=None, exp_avg_sq_scale=None, seed=0,
-                   taken=None):
+                   taken=None, adopt=False):
         """One AdamW step of lists of tensors, in place. `lr` and `weight_decay`: a number, or one for each tensor. `master`:
         float32 copies that the step works on, with 16-bit params. With the scales, exp_avg and exp_avg_sq are float8_e4m3fn
         (or uint8) tensors: m, and the root of v, in units of their block's scale. grad_norm: `grad_norm`'s result of these
         gradients; where it is not finite the step is left out. `taken`: int64 tensors of two elements, each the count of its
         tensor's own steps and a word of the call's; the bias is corrected by them in place of `step`, and a step that is not
-        left out adds one."""
+        left out adds one. `adopt`: an element of a 16-bit param that is not its master's rounding has been set since the last
+        step, and is what this one begins from."""
         self._ops.adamw(self._address, self._index, _raw_stream(self._index), params, grads, exp_avg, exp_avg_sq, step, lr,
-                        weight_decay, b1, b2, eps, master, grad_scale, grad_norm, max_norm, exp_avg_scale, exp_avg_sq_scale, seed, taken)
+                        weight_decay, b1, b2, eps, master, grad_scale, grad_norm, max_norm, exp_avg_scale, exp_avg_sq_scale, seed, taken,
+                        adopt)
 
 
 class _LayerNorm(torch.autograd.Function):
@@ -186,7 +189,8 @@ def layer_norm(backend: TorchBackend, x, weight=None, bias=None, eps=1e-5, resid
 
 
 class AdamW:
-    """AdamW over a model's parameters, with moments in 32 bits or in 8 and a float32 master copy of 16-bit parameters.
+    """AdamW over a model's parameters, with moments in 32 bits or in 8 and a float32 master copy of 16-bit parameters (where
+    a parameter has been set since its last step, weights loaded for one, the master follows it).
 
     `params`: tensors, or dicts with "params" and their own "lr" or "weight_decay". A step takes the gradients from the
     parameters (one without a gradient is left as it is) and clips their norm to `max_norm` (0: does not); a step whose
@@ -251,7 +255,7 @@ class AdamW:
             st = [self.state[at[j]] for j in k]
             more = dict(taken=[s["taken"] for s in st])
             if half:
-                more["master"] = [s["master"] for s in st]
+                more.update(master=[s["master"] for s in st], adopt=True)
             if self.state_bits == 8:
                 more.update(exp_avg_scale=[s["exp_avg_scale"] for s in st], exp_avg_sq_scale=[s["exp_avg_sq_scale"] for s in st],
                             seed=(self.seed * 2 + half) & (2 ** 64 - 1))

@@ -210,3 +210,43 @@ def test_adamw_in_a_graph_counts_its_replays(tb):
             assert torch.equal(a, b), k
         assert int(taken[0]) == k + 1
         (torch.randn(1000, device="cuda") ** 2).sum().item()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_adamw_weights_set_after_the_optimizer_was_made(tb, bits, dtype):
+    """16-bit parameters loaded, edited through .data or given other storage after their masters were taken: steps go on from
+    what they are, the elements that nobody set from their masters."""
+    import splatx_torch
+    sizes, lr = (700, 3001, 64), 1e-3
+    p = [torch.nn.Parameter(randn(n, seed=n).to(dtype).cuda()) for n in sizes]
+    opt = splatx_torch.AdamW(tb, p, lr=lr, weight_decay=0.0, state_bits=bits, seed=5)
+    loaded = [randn(n, seed=n + 1).to(dtype).cuda() for n in sizes]
+
+    def load():
+        with torch.no_grad():
+            p[0].copy_(loaded[0])
+        p[1].data.copy_(loaded[1])
+        p[2].data = loaded[2].clone()
+
+    load()
+    q = [torch.nn.Parameter(t.clone()) for t in loaded]
+    fresh = splatx_torch.AdamW(tb, q, lr=lr, weight_decay=0.0, state_bits=bits, seed=5)
+    for k in range(5):
+        if k == 3:  # the weights again, and some of a tensor's only
+            with torch.no_grad():
+                p[1][100:1001:3] = 0.25
+                q[1][100:1001:3] = 0.25
+            fresh.state[1]["master"][100:1001:3] = 0.25
+        for i, n in enumerate(sizes):
+            p[i].grad = q[i].grad = randn(n, seed=100 + 10 * k + i, dtype=dtype).cuda()
+        opt.step(), fresh.step()
+        for x, y, s, t in zip(p, q, opt.state, fresh.state):
+            assert torch.equal(x, y) and torch.equal(s["master"], t["master"]) and torch.equal(x, s["master"].to(dtype))
+    assert all(bool((s["master"] != x.float()).any()) for x, s in zip(p, opt.state))  # (the masters hold more than the parameters)
+    # without `adopt` the operator's parameters are its masters' roundings, whatever they were
+    s, x = opt.state[0], torch.zeros_like(p[0])
+    want = s["master"].clone()
+    kw = dict(exp_avg_scale=[s["exp_avg_scale"]], exp_avg_sq_scale=[s["exp_avg_sq_scale"]]) if bits == 8 else {}
+    tb.adamw_step([x], [torch.zeros_like(x)], [s["exp_avg"]], [s["exp_avg_sq"]], step=1, lr=0.0, master=[s["master"]], **kw)
+    assert torch.equal(s["master"], want) and torch.equal(x, want.to(dtype))
