@@ -159,7 +159,8 @@ class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, backend, x, weight, bias, eps, residual):
         y, h, mean, rstd = backend.layer_norm_fwd(x, weight, bias, eps, residual)
-        ctx.backend, ctx.has_bias, ctx.has_residual = backend, bias is not None, residual is not None
+        ctx.backend = backend
+        ctx.shapes = tuple(None if t is None else t.shape for t in (weight, bias))
         ctx.save_for_backward(h, mean, rstd, weight)
         ctx.set_materialize_grads(False)
         return (y, h) if residual is not None else y
@@ -174,6 +175,7 @@ class _LayerNorm(torch.autograd.Function):
         # (a sum's gradient is one value broadcast; a transposed layer's has its rows in other places)
         dy, dh = (t if t is None or t.dim() == 2 and t.stride(1) == 1 else t.contiguous() for t in (dy, dh))
         dx, dweight, dbias = backward_of(ctx.backend, dy, h, mean, rstd, weight, dh, need_x or need_r, need_w, need_b)
+        dweight, dbias = (g if g is None else g.view(shape) for g, shape in zip((dweight, dbias), ctx.shapes))
         return None, dx if need_x else None, dweight, dbias, None, dx if need_r else None
 
 
@@ -184,7 +186,8 @@ def backward_of(backend, dy, h, mean, rstd, weight, dh, want_dx, want_dweight, w
 
 
 def layer_norm(backend: TorchBackend, x, weight=None, bias=None, eps=1e-5, residual=None):
-    """Differentiable layer norm over the last dimension: y, or (y, x + residual) with a residual."""
+    """Differentiable layer norm over the last dimension: y, or (y, x + residual) with a residual. weight and bias have as many
+    elements as a row, in any shape, and so have their gradients."""
     return _LayerNorm.apply(backend, x, weight, bias, eps, residual)
 
 

@@ -250,3 +250,18 @@ def test_adamw_weights_set_after_the_optimizer_was_made(tb, bits, dtype):
     kw = dict(exp_avg_scale=[s["exp_avg_scale"]], exp_avg_sq_scale=[s["exp_avg_sq_scale"]]) if bits == 8 else {}
     tb.adamw_step([x], [torch.zeros_like(x)], [s["exp_avg"]], [s["exp_avg_sq"]], step=1, lr=0.0, master=[s["master"]], **kw)
     assert torch.equal(s["master"], want) and torch.equal(x, want.to(dtype))
+
+
+@pytest.mark.parametrize("wshape,bshape", [((1, 64), (64,)), ((64,), (1, 1, 64)), ((8, 8), (64, 1)), ((64,), (64,))])
+def test_layer_norm_weights_of_any_shape_get_gradients_of_it(tb, wshape, bshape):
+    import splatx_torch
+    x, w, b, dy = (randn(30, 64, seed=1), 1 + 0.2 * randn(64, seed=2), randn(64, seed=3), randn(30, 64, seed=4).cuda())
+    flat = [t.cuda().requires_grad_() for t in (x, w, b)]
+    splatx_torch.layer_norm(tb, *flat).backward(dy)
+    shaped = [t.cuda().requires_grad_() for t in (x, w.view(wshape), b.view(bshape))]
+    splatx_torch.layer_norm(tb, *shaped).backward(dy)
+    for a, c in zip(shaped, flat):
+        assert a.grad.shape == a.shape and torch.equal(a.grad.flatten(), c.grad.flatten())
+    only = shaped[1].detach().clone().requires_grad_()
+    splatx_torch.layer_norm(tb, x.cuda(), only).backward(dy)
+    assert torch.equal(only.grad.flatten(), flat[1].grad)
