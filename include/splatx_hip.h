@@ -816,7 +816,7 @@ typedef struct {
 typedef struct {
     int64_t step;            /* 1 for the first; of tensors with `taken` for the rounding's bits alone */
     uint64_t seed;           /* of the rounding, with state_bits 8 */
-    double b1, b2, eps;      /* 0 <= b < 1, eps > 0 */
+    double b1, b2, eps;      /* 0 <= b < 1, 1e-30 <= eps <= 1e30 */
     const float* grad_norm;  /* [1] device, or NULL */
     float max_norm;          /* 0: no clipping */
     float grad_scale;        /* 1 / the loss scale */

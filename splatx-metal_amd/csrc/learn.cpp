@@ -320,7 +320,8 @@ int32_t sxh_adamw(sxh_backend* b, const sxh_adamw_tensor* tensors, int64_t n_ten
         if (p->step < 1) invalid(what, "step must be 1 or more");
         if (p->state_bits != 32 && p->state_bits != 8) invalid(what, "state_bits must be 32 or 8");
         if (!(p->b1 >= 0.0 && p->b1 < 1.0 && p->b2 >= 0.0 && p->b2 < 1.0)) invalid(what, "b1 and b2 must be in [0, 1)");
-        if (!(p->eps >= 1e-30 && p->eps < 1.0)) invalid(what, "eps must be in [1e-30, 1)");
+        // (the quotient's denominator, roots of floats over roots of 2^-53 at least and eps, and its reciprocal stay normal floats)
+        if (!(p->eps >= 1e-30 && p->eps <= 1e30)) invalid(what, "eps must be in [1e-30, 1e30]");
         if (!(p->max_norm >= 0.0f) || !std::isfinite(p->max_norm)) invalid(what, "max_norm must be 0 or more");
         if (!(p->grad_scale > 0.0f) || !std::isfinite(p->grad_scale)) invalid(what, "grad_scale must be positive");
         if (p->adopt != 0 && p->adopt != 1) invalid(what, "adopt must be 0 or 1");

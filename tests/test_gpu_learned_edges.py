@@ -265,3 +265,25 @@ def test_layer_norm_weights_of_any_shape_get_gradients_of_it(tb, wshape, bshape)
     only = shaped[1].detach().clone().requires_grad_()
     splatx_torch.layer_norm(tb, x.cuda(), only).backward(dy)
     assert torch.equal(only.grad.flatten(), flat[1].grad)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("eps", [1e-30, 0.5, 1.0, 2.5, 1e30])
+def test_adamw_eps(tb, bits, eps):
+    """The whole range of eps: above 1, where it outweighs the roots, and down to 1e-30."""
+    from test_gpu_learned_ops import coded
+    hyper = dict(b1=0.9, b2=0.999, eps=eps)
+    p, g, m, r = randn(3000, seed=1), randn(3000, seed=2), 0.1 * randn(3000, seed=3), randn(3000, seed=4).abs()
+    if bits == 8:
+        (m, mc, ms), (r, rc, rs) = ([t[0] for t in coded([x])] for x in (m, r))
+        dev, more = [t.cuda() for t in (p, g, mc, rc)], dict(exp_avg_scale=[ms.cuda()], exp_avg_sq_scale=[rs.cuda()])
+    else:
+        dev, more = [t.cuda() for t in (p, g, m, r.square())], {}
+    tb.adamw_step(*([t] for t in dev), step=3, lr=1e-2 * max(eps, 1.0), **more, **hyper)
+    lr = 1e-2 * max(eps, 1.0)
+    new = ref.adamw(p, g, m, r.square(), step=3, lr=lr, weight_decay=0.0, **hyper)
+    # as in test_gpu_learned_ops.adam_bound, with this eps in the denominator
+    terms = 0.9 * m.double().abs() + 0.1 * g.double().abs()
+    below = (new[2] / (1 - 0.999 ** 3)).sqrt() + eps
+    bound = 3 * ref.U32 * p.double().abs() + lr / (1 - 0.9 ** 3) * (13 * ref.U32 * terms + 1e-38) / below
+    within(dev[0], new[0], 2 * bound, "param")

@@ -50,3 +50,13 @@ def test_what_is_no_number_is_refused(st):
         for k in ("lr", "step", "seed"):
             with pytest.raises(sh.SxInvalidArgument):
                 adamw(ops, **{k: bad})
+
+
+def test_eps_of_any_size_that_the_arithmetic_holds(st):
+    """Refused for the missing backend alone, or for eps."""
+    import splatx_hip as sh
+    ops = st._extension()
+    for eps, word in ((1e-30, "null backend"), (0.9, "null backend"), (1.0, "null backend"), (10.0, "null backend"), (1e30, "null backend"),
+                      (0.0, "eps"), (9e-31, "eps"), (1.1e30, "eps"), (float("inf"), "eps"), (float("nan"), "eps"), (-1.0, "eps")):
+        with pytest.raises(sh.SxInvalidArgument, match=word):
+            adamw(ops, eps=eps)
