@@ -283,7 +283,8 @@ class AdamW:
         # (a state of before parameters had counts of their own: all took every step)
         state = [{"taken": torch.tensor([d["steps"], 0]), **t} for t in d["state"]]
         for s, t in zip(self.state, state):
-            if s.keys() != t.keys() or any(s[k].shape != t[k].shape for k in s):
+            # (a copy would convert: codes as whole numbers are other values than the codes)
+            if s.keys() != t.keys() or any(s[k].shape != t[k].shape or s[k].dtype != t[k].dtype for k in s):
                 raise sh.SxInvalidArgument("the state is of other parameters")
         for s, t in zip(self.state, state):
             for k in s:

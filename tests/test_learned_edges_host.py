@@ -60,3 +60,21 @@ def test_eps_of_any_size_that_the_arithmetic_holds(st):
                       (0.0, "eps"), (9e-31, "eps"), (1.1e30, "eps"), (float("inf"), "eps"), (float("nan"), "eps"), (-1.0, "eps")):
         with pytest.raises(sh.SxInvalidArgument, match=word):
             adamw(ops, eps=eps)
+
+
+def test_states_of_other_types_are_refused(st):
+    """8-bit moments held as whole numbers would be taken for those numbers, not for the codes."""
+    import splatx_hip as sh
+    p = [torch.nn.Parameter(torch.randn(300)), torch.nn.Parameter(torch.randn(20, dtype=torch.bfloat16))]
+    for bits in (32, 8):
+        opt = st.AdamW(None, p, state_bits=bits)
+        good = opt.state_dict()
+        opt.load_state_dict(good)
+        for k, dtype in (("exp_avg", torch.uint8), ("exp_avg_sq", torch.float64), ("master", torch.bfloat16)):
+            bad = opt.state_dict()
+            bad["state"][1][k] = bad["state"][1][k].float().to(dtype)
+            with pytest.raises(sh.SxInvalidArgument):
+                opt.load_state_dict(bad)
+        with pytest.raises(sh.SxInvalidArgument):
+            opt.load_state_dict({**good, "state_bits": 40 - bits})
+        assert opt.steps == 0
