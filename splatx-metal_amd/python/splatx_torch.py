@@ -76,7 +76,7 @@ def _extension():
     """host/torch_ops.cpp, which is built beside the library where torch is: the calls' checks, outputs and launches."""
     path = os.path.join(os.path.dirname(sh.LIB_PATH), "_splatx_torch.so")
     if not os.path.exists(path):
-        raise sh.SxRuntimeError(f"the torch extension is not built: {path} (make all in splatx-metal_amd, with torch installed)")
+        raise sh.SxRuntimeError(f"the torch extension is not built: {path} (make all in splatx-metal_amd, with torch's and Python's headers)")
     loader = importlib.machinery.ExtensionFileLoader("_splatx_torch", path)
     ops = importlib.util.module_from_spec(importlib.util.spec_from_loader("_splatx_torch", loader))
     ops.set_errors(sh.SxInvalidArgument, sh.SxRuntimeError)

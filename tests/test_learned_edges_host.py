@@ -78,3 +78,16 @@ def test_states_of_other_types_are_refused(st):
         with pytest.raises(sh.SxInvalidArgument):
             opt.load_state_dict({**good, "state_bits": 40 - bits})
         assert opt.steps == 0
+
+
+@pytest.mark.parametrize("missing", ["TORCH=", "TORCH=/nowhere/torch", "PYTHON_INCLUDE=/nowhere", "PYTHON_INCLUDE=", "PYTHON=/nowhere/python3", None])
+def test_the_library_is_built_without_the_extension_where_it_cannot_be(missing):
+    """`make all` where torch, its headers or Python's are not there, looked over without running it."""
+    import os
+    import subprocess
+    root = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "splatx-metal_amd")
+    r = subprocess.run(["make", "-n", "-B", "all"] + ([missing] if missing else []), cwd=root, capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
+    lines = r.stdout.splitlines()
+    assert any("-o build/libsplatx_hip.so" in x for x in lines)
+    assert any("host/torch_ops.cpp" in x and "-o build/_splatx_torch.so" in x for x in "\n".join(lines).replace("\\\n", " ").splitlines()) == (missing is None)
