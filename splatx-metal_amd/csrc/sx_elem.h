@@ -8,11 +8,6 @@
 
 namespace sxd {
 
-__device__ inline float load_as_float(const void* p, int64_t i, int type) {
-    if (type == sxk::kF32) return static_cast<const float*>(p)[i];
-    if (type == sxk::kBf16) return static_cast<float>(static_cast<const __bf16*>(p)[i]);
-    return static_cast<float>(static_cast<const _Float16*>(p)[i]);
-}
 __device__ inline void store_float(void* p, int64_t i, float v, int type) {
     if (type == sxk::kF32) static_cast<float*>(p)[i] = v;
     else if (type == sxk::kBf16) static_cast<__bf16*>(p)[i] = static_cast<__bf16>(v);

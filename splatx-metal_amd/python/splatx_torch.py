@@ -24,6 +24,8 @@ import splatx_hip as sh
 ADAMW_BLOCK = 256  # elements that share a scale with 8-bit moments
 
 
+# The C structs, for programs that have device memory without torch's tensors and call the entry points through `TorchBackend.lib`
+# themselves (as the tests of the C boundary do); the methods here go through the extension.
 class Queue(C.Structure):
     _fields_ = [("stream", C.c_void_p)]
 
@@ -67,7 +69,7 @@ class AdamWParams(C.Structure):
                 ("adopt", C.c_int32)]
 
 
-_NORM_ROW = struct.Struct("<QqB7x")  # a NormTensor as bytes: a table of them is these one after another
+_NORM_ROW = struct.Struct("<QqB7x")  # a NormTensor as bytes, for a table of many
 # (the public way to the current stream's handle makes an object of it, 2 us)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
 
