@@ -287,3 +287,130 @@ def test_adamw_eps(tb, bits, eps):
     below = (new[2] / (1 - 0.999 ** 3)).sqrt() + eps
     bound = 3 * ref.U32 * p.double().abs() + lr / (1 - 0.9 ** 3) * (13 * ref.U32 * terms + 1e-38) / below
     within(dev[0], new[0], 2 * bound, "param")
+
+
+def inside(got, want, bound, what):
+    """As `within`, on the device."""
+    got = got.double()
+    bad = ~(((got - want).abs() <= bound) | (got == want))
+    assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} outside, first at {bad.nonzero()[0].tolist()}"
+
+
+def device_randn(*shape, seed, dtype):
+    return torch.randn(*shape, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda").to(dtype)
+
+
+def backward_against_64_bits(tb, rows, width, dtype, off=0):
+    """Layer norm's gradients of random rows, without and with dh; `off`: rows that begin that many elements into their tensors.
+    A column's sum chains the rows of a thread (here 44 at most), 6 additions over a wave, 4 over a workgroup's, then 16 of a
+    thread's share of at most 1024 partial sums, 16 and 2: under 96, so that a row left out or counted twice shows."""
+    print(f"rows {rows} width {width} {dtype} off {off}", flush=True)
+
+    def held(seed):
+        flat = torch.full((off + rows * width,), float("nan"), dtype=dtype, device="cuda")
+        flat[off:] = device_randn(rows * width, seed=seed, dtype=dtype)
+        return flat[off:].view(rows, width)
+
+    h, dy, dh = (held(k) for k in (1, 2, 3))
+    w = 1 + 0.2 * device_randn(width, seed=4, dtype=F32)
+    _, _, mean, rstd = tb.layer_norm_fwd(h, w)
+    for add in (None, dh):
+        want, bounds = ref.norm_bwd(dy, h, mean, rstd, w, add)
+        got = tb.layer_norm_bwd(dy, h, mean, rstd, w, add)
+        xhat = (h.double() - mean.double()[:, None]) * rstd.double()[:, None]
+        bounds = bounds[0], 100 * ref.U32 * (dy.double() * xhat).abs().sum(0) + 1e-40, 96 * ref.U32 * dy.double().abs().sum(0) + 1e-40
+        for a, b, e, name in zip(got, want, bounds, ("dx", "dweight", "dbias")):
+            inside(a, b, e, f"{name}, dh {add is not None}")
+
+
+@pytest.mark.parametrize("rows,width,dtype", [
+    (1_000_003, 1, F32), (500_001, 3, F16), (900_001, 4, F32), (500_001, 5, BF16), (600_001, 8, F16), (300_001, 9, BF16), (200_003, 16, F32),
+    (250_001, 23, BF16), (30_001, 100, F32), (50_001, 200, BF16), (20_001, 250, F32), (20_001, 301, F16), (9_001, 301, F32), (7_001, 1000, BF16),
+    (1_301, 1100, F32), (3_001, 2056, F16), (901, 2500, F32), (901, 5000, BF16), (601, 4100, F32), (601, 10_000, BF16), (601, 6200, F32),
+    (601, 13_000, F16), (20_001, 9000, F32), (9_001, 20_001, BF16)])
+def test_layer_norm_backward_of_more_rows_than_at_a_time(tb, rows, width, dtype):
+    """Each split of a row (1 to 1024 threads, one, three and four vectors a thread, a loop over the row), with rows for two to
+    fourteen turns of every workgroup: the columns' sums go on over the turns, the next rows are loaded ahead."""
+    backward_against_64_bits(tb, rows, width, dtype)
+
+
+@pytest.mark.parametrize("rows,width", [(600_001, 9), (250_001, 23), (110_001, 45), (110_001, 46), (70_001, 101), (50_001, 201), (20_001, 301), (20_001, 511)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_layer_norm_backward_of_many_rows_off_words(tb, rows, width, dtype):
+    """The same of 16-bit rows that begin off a multiple of four bytes, up to a wave for a row."""
+    backward_against_64_bits(tb, rows, width, dtype, off=1)
+
+
+@pytest.mark.parametrize("rows,width,dtype", [(22_003, 1032, BF16), (11_003, 1024, F32), (5_603, 4096, F16), (5_603, 2048, F32), (2_803, 8192, BF16),
+                                              (2_303, 5000, F32), (1_503, 8000, F32), (1_503, 15_000, F16)])
+def test_layer_norm_backward_past_the_caches(tb, rows, width, dtype):
+    """Over 128 MiB of 16-byte aligned rows, 256 threads or more a row."""
+    backward_against_64_bits(tb, rows, width, dtype)
+
+
+@pytest.mark.parametrize("rows,width,add", [(3_200_001, 520, False), (2_200_003, 520, True), (8_500_001, 260, False)])
+def test_layer_norm_forward_of_more_rows_than_a_grid(tb, rows, width, add):
+    """More rows than 2^20 workgroups take at a time: the same rows again after some millions give the same bits."""
+    head = device_randn(5_001, width, seed=1, dtype=BF16)
+    x = torch.zeros(rows, width, dtype=BF16, device="cuda")
+    x[:5_001], x[-5_001:] = head, head
+    r = x * 0.5 if add else None
+    w, b = 1 + 0.2 * device_randn(width, seed=2, dtype=F32), device_randn(width, seed=3, dtype=F32)
+    y, h, mean, rstd = tb.layer_norm_fwd(x, w, b, residual=r)
+    want = tb.layer_norm_fwd(head, w, b, residual=head * 0.5 if add else None)
+    for got, some in zip((y, h, mean, rstd), want):
+        assert torch.equal(got[:5_001], some) and torch.equal(got[-5_001:], some)
+    assert torch.equal(y[5_001:-5_001].amin(0), b.to(BF16)) and torch.equal(y[5_001:-5_001].amax(0), b.to(BF16))
+    assert not mean[5_001:-5_001].any()
+
+
+@pytest.mark.parametrize("ptype,gtype,offset", [(F32, F32, 1), (F32, BF16, 0), (BF16, BF16, 3), (F16, F32, 0)])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_past_the_caches(tb, bits, ptype, gtype, offset):
+    """Steps of over 128 MiB, tensors of odd sizes one after another in their buffers."""
+    from test_gpu_learned_ops import HYPER, adam_bound, same_codes
+    sizes = [9_000_003, 5, 70_001, 6_000_002]
+
+    def held(seed, dtype, scale=1.0, blocks=False):
+        n = [-(-k // 256) for k in sizes] if blocks else sizes
+        flat = (scale * device_randn(offset + sum(n), seed=seed, dtype=F32)).to(dtype)
+        return list(flat[offset:].split(n))
+
+    p, g = held(1, F32), held(2, gtype, 0.01)
+    master = None if ptype == F32 else p
+    param = [t.clone() for t in p] if ptype == F32 else [t.to(ptype) for t in p]
+    start = [t.clone() for t in p]
+    more = {}
+    if bits == 32:
+        m, v = held(3, F32, 0.003), [t.square() for t in held(4, F32, 0.01)]
+        m0, v0 = [t.clone() for t in m], [t.clone() for t in v]
+    else:  # (any codes are moments: m of either sign, roots without one)
+        code = lambda seed, top: [(t.abs() * 40).clamp_max(top).byte() for t in held(seed, F32)]  # noqa: E731
+        m = [c | (s < 0).byte() << 7 for c, s in zip(code(3, 126), held(5, F32))]
+        v = code(4, 126)
+        ms, vs = ([t.abs() * 1e-4 + 1e-6 for t in held(k, F32, blocks=True)] for k in (6, 7))
+        values = ref.code_values().cuda()
+        full = lambda c, s: values[c.long()] * s.double().repeat_interleave(256)[:c.numel()]  # noqa: E731
+        m0, v0 = [full(c, s) for c, s in zip(m, ms)], [full(c, s).square() for c, s in zip(v, vs)]
+        more = dict(exp_avg_scale=ms, exp_avg_sq_scale=vs, seed=77)
+    lr, step = 1e-2, 5
+    tb.adamw_step(param, g, m, v, step=step, lr=lr, weight_decay=0.02, master=master, **more, **HYPER)
+    for i, n in enumerate(sizes):
+        new = ref.adamw(start[i], g[i], m0[i], v0[i], step=step, lr=lr, weight_decay=0.02, **HYPER)
+        ep, em, ev = adam_bound(start[i], g[i], m0[i], v0[i], new, lr, step)
+        inside(param[i] if master is None else master[i], new[0], 2 * ep, f"param {i}")
+        if master is not None:
+            assert torch.equal(param[i], master[i].to(ptype))
+        if bits == 32:
+            inside(m[i], new[1], em, f"m {i}")
+            inside(v[i], new[2], ev, f"v {i}")
+            continue
+        random = ref.random_bits(77, step, i, n)
+        for at in {0, n // 512 * 256, max(n - 1, 0) // 256 * 256}:  # three places, whole blocks
+            k = slice(at, min(n, at + 25_600))
+            codes, scale = ref.encode(new[1][k].cpu(), random[k] & 0xFFFF, False)
+            same_codes(m[i][k], codes, "exp_avg")
+            within(ms[i][at // 256:at // 256 + scale.numel()], scale, 8 * ref.U32 * scale, "exp_avg_scale")
+            codes, scale = ref.encode(new[2][k].sqrt().cpu(), random[k] >> 16, True)
+            same_codes(v[i][k], codes, "exp_avg_sq")
+            within(vs[i][at // 256:at // 256 + scale.numel()], scale, 8 * ref.U32 * scale, "exp_avg_sq_scale")
