@@ -721,7 +721,7 @@ typedef struct {
  *   mean = sum(h) / width, rstd = 1 / sqrt(sum((h - mean)^2) / width + eps):
  *   y = (h - mean) * rstd * weight + bias.
  * Rows are `*_stride` elements apart (at least width; for inputs also 0: every row the same one). Rows whose
- * values are not all finite give NaN in their own y only. */
+ * values are not all finite give NaN in their own y only, and a mean and rstd that are not finite. */
 typedef struct {
     const void* x;         /* [rows, width] */
     const void* residual;  /* [rows, width] or NULL */

@@ -1,5 +1,7 @@
 """Layer norm, gradient norm and AdamW where sums are exact, rows and launches are many, or a program changes things between
 calls (the operators over their ordinary range: test_gpu_learned_ops)."""
+import math
+
 import pytest
 import torch  # before anything loads the library: its HIP runtime is the process's
 
@@ -47,7 +49,7 @@ def test_layer_norm_rows_of_one_value_give_the_bias(tb, dtype):
 
 def test_adamw_of_more_elements_than_a_launch(tb):
     """2^34 and some elements in 8 bits, gradients in bfloat16 (137 GB): a launch takes 2^34 - 1024 of them."""
-    import math
+
     torch.cuda.empty_cache()
     border, n = 2 ** 34 - 1024, 2 ** 34 + 5003
     if torch.cuda.mem_get_info()[0] < 150 << 30:
@@ -414,3 +416,17 @@ def test_adamw_past_the_caches(tb, bits, ptype, gtype, offset):
             codes, scale = ref.encode(new[2][k].sqrt().cpu(), random[k] >> 16, True)
             same_codes(v[i][k], codes, "exp_avg_sq")
             within(vs[i][at // 256:at // 256 + scale.numel()], scale, 8 * ref.U32 * scale, "exp_avg_sq_scale")
+
+
+@pytest.mark.parametrize("width", [1, 3, 45, 64, 300, 1024, 5000, 20_000])
+def test_layer_norm_statistics_of_rows_that_are_not_finite(tb, width):
+    """Neither the mean nor rstd of such a row is finite (an infinity of an element that two vectors hold may leave no number), and
+    the other rows' are theirs."""
+    x = randn(9, width, seed=1)
+    last = width - 1
+    x[1, 0], x[2, last], x[3, 0], x[4, 0], x[4, last], x[5, 0] = math.inf, -math.inf, math.nan, math.inf, -math.inf if width > 1 else math.inf, 1e30
+    want = x.double().sum(1) / width
+    mean, rstd = (t.cpu().double() for t in tb.layer_norm_fwd(x.cuda())[2:])
+    finite = torch.isfinite(want)
+    assert not torch.isfinite(mean[~finite]).any() and torch.isnan(rstd[~finite]).all()
+    assert ((mean - want).abs()[finite] <= (width / 32 + 16) * ref.U32 * x.double().abs().amax(1)[finite]).all()
