@@ -4,8 +4,8 @@
 // The tensors' pointers and sizes travel in the launch's arguments, so a call keeps nothing on the device and copies
 // nothing to it. A workgroup finds its tensor from its place among the launch's chunks.
 //
-// All are bound by memory: 59 M float gradients' norm 40 us (5.9 TB/s) and 5 for the join; the 32-bit step of 59 M elements
-// 265 us (6.2 TB/s); the 8-bit step of 118 M 310 us (6.1 TB/s). A large copy reaches 6.1, past the caches 6.4.
+// All are bound by memory: 59 M float gradients' norm 42 us (5.7 TB/s) and 5 for the join; the 32-bit step of 59 M elements
+// 263 us (6.3 TB/s); the 8-bit step of 118 M 302 us (6.3 TB/s). A large copy reaches 6.1, past the caches 6.4.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -112,7 +112,8 @@ __device__ bool grad_factor(const AdamTable& t, float* c) {
     return true;
 }
 
-// A lane for each tensor.
+// A lane for each tensor. A launch of its own, 4 us before a step's: every workgroup of the step reads the count that it changes,
+// and forming the powers there would take each wave as many instructions as its elements do.
 __global__ void __launch_bounds__(kWave) k_count_steps(AdamCounts c) {
     const int k = threadIdx.x;
     if (k >= c.tensors || !finite(scaled_norm(c.grad_norm, c.grad_scale))) return;
@@ -155,7 +156,7 @@ __device__ inline Floats<E> load_grad(const AdamTensor& a, int64_t i) {
     return load_few<E, ONCE>(static_cast<const _Float16*>(a.grad), i, a.n);
 }
 // What the step begins from: of a 16-bit parameter its master, with ADOPT where the parameter is still its rounding (else it has
-// been set by someone since).
+// been set by someone since). To read the parameter as well takes 40 M bfloat16 elements 180 -> 188 us in 32 bits, 110 -> 127 in 8.
 template <int E, bool ONCE, class T>
 __device__ inline Floats<E> adopted(const AdamTensor& a, int64_t i, Floats<E> master) {
     const Floats<E> now = load_few<E, ONCE>(static_cast<const T*>(a.param), i, a.n), was = floats<T, E>(raw<T, E>(master));
@@ -298,7 +299,7 @@ __device__ inline uint32_t encode(const float (&u)[4], const uint32_t (&bits)[4]
 
 // A wave per block of 256 elements, four side by side a lane: 16 bytes of parameter and of gradient and four of each moment's
 // codes, decoded and encoded by the hardware. Past the caches as above: 310 us against 338 (118 M elements), 19.5 against 19.0
-// (5.9 M). A wave's 330 vector instructions for its block would issue in 240 us of those 310: close behind the memory.
+// (5.9 M). A wave's 330 vector instructions for its block would issue in 240 us of the 302 there now: close behind the memory.
 template <bool ONCE, bool ADOPT>
 __global__ void __launch_bounds__(kBlock) k_adamw8(AdamTable t) {
     const int chunk = t.from + static_cast<int>(blockIdx.x), k = tensor_of(t.first, t.tensors, chunk);

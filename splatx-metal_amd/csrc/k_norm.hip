@@ -6,9 +6,12 @@
 // address, are read in whole vectors: the last one ends with the row and overlaps the one before it, and a mask keeps what
 // both hold out of the sums (both store it, the same value).
 //
-// Both directions are bound by memory: each input is read once, each output written once, at 5.4 to 5.9 TB/s where a large
+// Both directions are bound by memory: each input is read once, each output written once, at 5.3 to 5.8 TB/s where a large
 // copy reaches 6.1 (6.4 past the caches). Stores go through the caches: past them the forward takes 3 to 5 % less, and the
 // operator that reads y next more than that longer (1 M x 48: 36.4 to 35.4 us, with a reader of y 49.5 to 52.3).
+//
+// Times here are a kernel's own, from a trace. Two variants were always timed in turn; shares (a tenth longer) stand where a
+// variant was not kept to be timed again.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -157,9 +160,10 @@ __device__ inline Floats<V> load_weights(const void* w, int at, bool is_float, f
 
 // R rows of each group of threads at a time. The weights of a thread's only vector stay in its registers; those of more are
 // read again for each row (they lie in the L1 cache), which leaves the registers to the rows.
-// 1 M x 48 bfloat16: 33.8 us, 5.9 TB/s; 16,383 x 2048 half with a residual: 46.3 us, 5.8 TB/s. Rows a little wider than a
-// power of two vectors leave lanes idle, and odd ones of 16 bits share lines with their neighbours, at up to 1.5 times
-// (242,424 x 264: 53 us, 249,027 x 257 62, 250,000 x 256, as many bytes, 46; three vectors a thread of fewer threads 58).
+// 1 M x 48 bfloat16: 37.6 us, 5.3 TB/s; 16,383 x 2048 half with a residual: 50 us, 5.4 TB/s. Rows a little wider than a power
+// of two vectors leave lanes idle (242,424 x 264 bfloat16: 58 us, 250,000 x 256, as many bytes, 47; three vectors a thread of a
+// third of the threads were a tenth slower), and odd ones of 16 bits begin off words, which the loads mend (load_shifted) and
+// the stores, of 16 bytes each from wherever the row begins, do not (249,027 x 257: 67 us).
 template <class T, int V, int TPR, int K, int R, Loads L>
 __global__ void __launch_bounds__(kThreadsOf<TPR>) k_norm_fwd(NormFwdArgs a, bool float_weights) {
     constexpr int kRows = kRowsOf<TPR>;
@@ -255,7 +259,7 @@ __global__ void __launch_bounds__(kThreadsOf<TPR>) k_norm_fwd(NormFwdArgs a, boo
 // The backward of R rows of each group of threads at a time; the columns' sums stay in registers over the rows, are added
 // over the workgroup's groups at the end and written as its part of the partial sums: one pass over dy and h for all three
 // gradients. With one vector a thread the next rows are on their way while these are worked on.
-// 1 M x 64 bfloat16 with dh: 89.9 us, 5.8 TB/s; 16,383 x 2048 half: 36.7 us, 5.5 TB/s; then the join, 2.7 to 4.8 us.
+// 1 M x 64 bfloat16 with dh: 90 us, 5.8 TB/s; 16,383 x 2048 half: 36.4 us, 5.5 TB/s; then the join, 2.7 to 6.5 us.
 template <class T, int V, int TPR, int K, int R, Loads L>
 __global__ void __launch_bounds__(kThreadsOf<TPR>) k_norm_bwd(NormBwdArgs a, bool float_weights) {
     constexpr int kRows = kRowsOf<TPR>;
@@ -433,7 +437,9 @@ __global__ void __launch_bounds__(kJoinBlock) k_norm_join(NormBwdArgs a, int sla
 
 // ---- rows wider than a workgroup's registers: it goes over its row several times ------------------------------------------
 // From 16,384 float elements on forward and 8,192 on backward (twice that in 16 bits). What is read again comes from the
-// caches: 3200 x 20,000 bfloat16 backward 170 us, 2.8 times what its bytes would take once.
+// caches where it is there still. Forward, its row three times: 3200 x 20,000 float 140 us, 3200 x 40,000 bfloat16 165, 1.8 and
+// 2.1 times what their bytes would take once. Backward, dy and h twice and once more for the columns: 3200 x 20,000 bfloat16
+// 104 + 54 + 15 (the join) us, 2.9 times, 3200 x 10,000 float 90 + 49 + 8, 2.5.
 
 constexpr int kWideBlock = 1024;
 
@@ -557,14 +563,15 @@ struct Split {
     int block() const { return most <= kWave ? kBlock : threads; }
 };
 // A vector of 16 bytes a thread up to a workgroup: of the splits that hold a row this one was the fastest or within 3 %
-// throughout (16,383 x 2048 half, backward: a workgroup of 256 40 us, 128 threads of two vectors 44, a wave of four 57;
-// 1 M x 48 bfloat16, forward: 8 threads 36 us, 2 of three vectors 37). Rows of over a wave take as many whole waves as they
-// need (31,128 x 2056, forward: 5 waves 54 us, 8 would leave a third of them idle). Two rows at a time where they fit the
-// registers: the loads of one alone do not cover the memory's latency (2 M x 96, forward: 133 us against 161, four rows
-// 131; 31,128 x 2056: 65 against 72), and three where one tensor is read by rows of over a wave (31,128 x 2056: 54, 123,076 x 520
-// 51 against 58, 62,256 x 1028 float 96 against 114, 62,500 x 1024 88 both; with a residual 99 against 101, 2048 91 against 89;
-// rows of a wave 55 against 52). From 513 vectors on the forward takes three or four a thread (15,621 x 4100: 56 us, two
-// 70, one 72), the backward, whose sums take the registers, only from 1025 on (10,666 x 6000: one 85 us, two 114, three 92).
+// throughout (16,383 x 2048 half, backward: 128 threads of two vectors a tenth longer than a workgroup of 256, a wave of four
+// 1.4 times; 1 M x 48 bfloat16, forward: 2 threads of three vectors 3 % longer than 8). Rows of over a wave take as many whole
+// waves as they need (31,128 x 2056, forward: 5 waves; 8 would leave a third of them idle). Two rows at a time where they fit the
+// registers: the loads of one alone do not cover the memory's latency (bfloat16 forward, one and two: 2 M x 96 174 and 138 us,
+// 31,128 x 2056 75 and 69, 250,000 x 256 49 and 47.5), and three where one tensor is read by rows of over a wave (two and three:
+// 31,128 x 2056 69 and 58.5, 123,076 x 520 62 and 54, 62,256 x 1028 float 121 and 101, 62,500 x 1024 float 87 both; with a residual
+// 2 % either way, rows of a wave 6 % longer). From 513 vectors on the forward takes three or four a thread, one row at a time
+// (15,621 x 4100: 64 us, two or one a quarter longer), the backward, whose sums take the registers, only from 1025 on (10,666 x
+// 6000: 88 us, two a third longer, three a tenth).
 Split split_of(int64_t width, int size, bool backward, bool residual) {
     const int full = 16 / size, vec = width >= full ? full : width >= 4 ? 4 : 1;
     const int64_t n = (width + vec - 1) / vec;
@@ -588,9 +595,9 @@ bool on(int n, const NormFwdArgs& a, int size) { return on(n, a.x, a.x_stride, s
 bool on(int n, const NormBwdArgs& a, int size) {
     return on(n, a.dy, a.dy_stride, size) && on(n, a.h, a.h_stride, size) && on(n, a.dh, a.dh_stride, size);
 }
-// The loads of 16-bit rows that begin off a multiple of four bytes, up to a wave for a row: 1.2 M x 45 bfloat16, forward 44.3 us
-// against 51.0, backward 76.3 against 82.7, with dh 82.4 against 98.4. Wider rows take as long or longer (40,000 x 1601,
-// backward: 92 us against 84), as do rows on multiples of four bytes (31,250 x 2048, forward: 55 against 49).
+// The loads of 16-bit rows that begin off a multiple of four bytes, up to a wave for a row: 1.2 M x 45 bfloat16, forward 47 us
+// against 54, backward 65 against 78, with dh 86 against 99.5. Wider rows take as long or longer (40,000 x 1601, backward: a
+// tenth), as do rows on multiples of four bytes (31,250 x 2048, forward: a tenth).
 template <int V, int TPR>
 constexpr bool kMayShift = V == 8 && TPR <= kWave;
 
@@ -615,9 +622,10 @@ template <class T, int V, int TPR, int K>
 void launch(const Split& sp, const NormBwdArgs& a, bool fw, int grid, hipStream_t s) {
     constexpr int R = K == 1 && TPR <= 256 ? 2 : 1;
     // Rows of 256 threads or more, 16-byte aligned, go past the caches where a call moves more than half of what the last one
-    // holds (256 MiB): 16,383 x 2048 36.5 us against 40.0, 64,000 x 1000 float 127 against 140. Within it they do not (33
-    // against 36), nor where rows share lines with others (1 M x 45: 101 against 96), nor narrower ones, which gain nothing
-    // (65,536 x 1024: 101.6 against 98.0).
+    // holds (256 MiB): 16,383 x 2048 half 36 us against 39, 65,536 x 1024 float 141.8 against 144, 62,015 x 1032 bfloat16 76.5
+    // against 79; 64,000 x 1000 float 139.8 against 136.3, 31,128 x 2056 bfloat16 with dh 103 against 98. Within it they do not
+    // (a tenth longer), nor where rows share lines with others (5 %). Rows of 128 threads do not, and would gain: 62,500 x 1024
+    // bfloat16 70.5 us, past the caches 63.5, with dh 91.6 and 87, 65,536 x 1024 with dh 95.8 and 91.
     if constexpr (TPR >= 256) {
         if (a.rows * a.width * static_cast<int64_t>(sizeof(T)) * (a.dh ? 4 : 3) > (int64_t{128} << 20) && on(16, a, sizeof(T))) {
             hipLaunchKernelGGL((k_norm_bwd<T, V, TPR, K, R, Loads::Past>), dim3(grid), dim3(sp.block()), 0, s, a, fw);
@@ -697,10 +705,10 @@ void layer_norm_fwd(const NormFwdArgs& a, ElemType type, ElemType weight_type, h
 // as long as 512 would: 10,666 x 6000 126 us, 256 of them 85): as many as have the memory busy and no more, which counts in the
 // vectors that a unit's threads have on their way (threads without one of their own do not count, three tensors want fewer than
 // two, rows that share words and rows worked on one at a time more), up to 768 threads, all that the registers hold of 16-bit
-// elements. Measured in workgroups a unit, without dh: 1 M x 64 2: 73 us, 4 85; 249,027 x 257 2: 111, 3 90; 711,111 x 90 2: 71,
+// elements. Measured in turn, in workgroups a unit, without dh: 1 M x 64 2: 73 us, 4 85; 249,027 x 257 2: 111, 3 90; 711,111 x 90 2: 71,
 // 3 75; 123,076 x 520 4: 98, 6 83; 62,015 x 1032 2: 100, 4 76; 31,128 x 2056 2: 78, 3 96. With dh: 1 M x 64 1: 90, 2 99;
-// 666,666 x 96 1: 103, 2 92; 126,732 x 505 1: 114, 2 98; 62,500 x 1024 2: 104, 3 91, 4 93; 31,128 x 2056 1: 120, 2 96. 32 MiB
-// of partial sums at most.
+// 666,666 x 96 1: 103, 2 92; 126,732 x 505 1: 114, 2 98; 62,500 x 1024 2: 104, 3 91, 4 93; 31,128 x 2056 1: 120, 2 96. (The 390 of
+// rows of up to a wave rests on 64, 90 and 96 columns.) 32 MiB of partial sums, or one slab of 8 bytes a column where that is more.
 int norm_bwd_slabs(int64_t rows, int64_t width, ElemType type, bool dh, bool even) {
     const int size = size_of(type);
     const Split sp = split_of(width, size, true, false);

@@ -1,10 +1,10 @@
 // torch_ops.cpp — the learned heads' operators (include/splatx_hip.h) on torch tensors, for splatx_torch.py.
 //
 // A Python extension module: it checks the tensors, lets torch's allocator make the outputs and workspaces on the current
-// stream, and enqueues the operator there. A small operator takes as long as its call: layer norm of 2048 x 45 takes 6.9 us
-// (the same steps in Python with the C entries through ctypes 11.1), its gradients 10.7 (15.5), an AdamW step of the head's ten
-// tensors 7.1 (19.8), the norm of their gradients 6.0 (10.6); what is left is the launch, about 1 us an allocation and the
-// pointers' checks. It links the library; torch's own libraries are those of the process, which has imported torch.
+// stream, and enqueues the operator there. A small operator takes as long as its call: layer norm of 2000 x 45 takes 6.8 us
+// (the same steps in Python with the C entries through ctypes took 11.1), its gradients 9.5 to 10.8 (15.5), an AdamW step of the
+// head's ten tensors 7.2 (19.8), the norm of their gradients 6.0 (10.6); what is left is the launch, about 1 us an allocation and
+// the pointers' checks. It links the library; torch's own libraries are those of the process, which has imported torch.
 #include <ATen/ATen.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
