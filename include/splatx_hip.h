@@ -827,6 +827,66 @@ typedef struct {
 int32_t sxh_adamw(sxh_backend* b, const sxh_adamw_tensor* tensors /* host array */, int64_t n_tensors,
                   const sxh_adamw_params* params, const sxh_queue* q);
 
+/* A linear layer over [rows, in] features, all that follows it in the same pass:
+ *   z = x W^T + bias, y = act(z) + residual; pre = z, rounded to `type`: what the backward reads.
+ * Sums are in 32 bits and z is not rounded before act and residual; y is rounded once. act is one of
+ *   none z, relu max(z, 0), gelu z Phi(z) (the normal distribution's), silu z / (1 + e^-z), sigmoid 1 / (1 + e^-z).
+ * groups 0: one weight [out, in] and bias [out] for all rows. groups G > 0: rows come in G groups with a weight [G, out, in] and
+ * bias [G, out] of their own; group g has the rows [ends[g - 1], ends[g]), the first from row 0. `ends` lies on the device,
+ * ascends (equal ends: a group without rows) and is at most rows; of ends that are not so no row outside [0, rows) is
+ * touched, and which group has a row is not specified. Rows from the last end on belong to no group: nothing of theirs is
+ * read, and y and pre are left as they were there, or with `clear` become zero.
+ * Rows are `*_stride` elements apart (at least their width; for inputs also 0: every row the same one). */
+enum { SXH_ACT_NONE = 0, SXH_ACT_RELU = 1, SXH_ACT_GELU = 2, SXH_ACT_SILU = 3, SXH_ACT_SIGMOID = 4 };
+typedef struct {
+    const void* x;         /* [rows, in] */
+    const void* weight;    /* [out, in], with groups [groups, out, in] */
+    const void* bias;      /* [out], with groups [groups, out], or NULL: 0 */
+    const void* residual;  /* [rows, out] or NULL */
+    const int64_t* ends;   /* [groups], or NULL without groups */
+    int64_t rows, in, out; /* rows may be 0 */
+    int64_t groups;        /* 0..32768 */
+    int64_t x_stride, residual_stride;
+    uint8_t type;          /* of all of them */
+    uint8_t activation;    /* SXH_ACT_* */
+    uint8_t clear;         /* 0 or 1 */
+} sxh_linear_inputs;
+typedef struct {
+    void* y;               /* [rows, out] */
+    void* pre;             /* [rows, out], or NULL: not wanted */
+    int64_t y_stride, pre_stride;
+    void* workspace;       /* sxh_linear_fwd_workspace(...) bytes of device memory, 16-byte aligned; may be NULL if that is 0 */
+    int64_t workspace_bytes;
+} sxh_linear_outputs;
+int64_t sxh_linear_fwd_workspace(int64_t rows, int64_t in, int64_t out, int64_t groups, uint8_t type);
+int32_t sxh_linear_fwd(sxh_backend* b, const sxh_linear_inputs* in, const sxh_linear_outputs* out, const sxh_queue* q);
+
+/* Its gradients, with dz = dy act'(pre) (relu's slope is 0 where pre is not above 0):
+ *   dx = dz W, dweight = dz^T x, dbias = sum over rows of dz (of each group, over its rows; of a group without rows 0);
+ * the residual's gradient is dy. For the two products dz is rounded to `type`. */
+typedef struct {
+    const void* dy;        /* [rows, out] */
+    const void* pre;       /* [rows, out] of the forward with an activation, else NULL */
+    const void* x;         /* [rows, in]; read for dweight */
+    const void* weight;    /* as in the forward; read for dx */
+    const int64_t* ends;
+    int64_t rows, in, out, groups;
+    int64_t dy_stride, pre_stride, x_stride;
+    uint8_t type;          /* of all of them and of the gradients */
+    uint8_t activation;
+    uint8_t clear;         /* 1: dx becomes zero in rows of no group, 0: it is left as it was there */
+} sxh_linear_grads_in;
+typedef struct {
+    void* dx;              /* [rows, in], or NULL: not wanted */
+    void* dweight;         /* as weight, or NULL */
+    void* dbias;           /* as bias, or NULL */
+    int64_t dx_stride;
+    void* workspace;       /* sxh_linear_bwd_workspace(...) bytes of device memory, 16-byte aligned */
+    int64_t workspace_bytes;
+} sxh_linear_grads;
+int64_t sxh_linear_bwd_workspace(int64_t rows, int64_t in, int64_t out, int64_t groups, uint8_t type);
+int32_t sxh_linear_bwd(sxh_backend* b, const sxh_linear_grads_in* in, const sxh_linear_grads* out, const sxh_queue* q);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif

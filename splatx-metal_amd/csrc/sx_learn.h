@@ -1,4 +1,4 @@
-// sx_learn.h — kernel arguments and launchers of the learned heads' operators (k_norm.hip, k_adamw.hip).
+// sx_learn.h — kernel arguments and launchers of the learned heads' operators (k_norm.hip, k_adamw.hip, k_linear.hip).
 // Every pointer is a device pointer; launchers allocate nothing and wait for nothing.
 #pragma once
 
@@ -94,5 +94,30 @@ uint32_t adam_key(uint64_t seed, int64_t step, int64_t tensor);
 // In as many launches as the table's chunks take. `once`: the call's tensors are more than the caches hold. `adopt`: parameters
 // that are not their masters' roundings take their places.
 void adamw(AdamTable& t, bool eight_bits, bool once, bool adopt, hipStream_t s);
+
+// Linear layers of `in` to `out` features. ends: null (one weight for all rows), or [groups] on the device.
+struct LinearFwdArgs {
+    const void *x, *weight, *bias, *residual;
+    void *y, *pre;
+    const int64_t* ends;
+    int64_t rows, in, out, x_stride, residual_stride, y_stride, pre_stride;
+    int groups, act;
+    bool clear;  // rows of no group become zero
+    void* workspace;
+};
+int64_t linear_fwd_workspace(int64_t rows, int64_t in, int64_t out, int groups, bool ragged, ElemType type);
+void linear_fwd(const LinearFwdArgs& a, ElemType type, hipStream_t s);
+
+struct LinearBwdArgs {
+    const void *dy, *pre, *x, *weight;
+    void *dx, *dweight, *dbias;
+    const int64_t* ends;
+    int64_t rows, in, out, dy_stride, pre_stride, x_stride, dx_stride;
+    int groups, act;
+    bool clear;
+    void* workspace;
+};
+int64_t linear_bwd_workspace(int64_t rows, int64_t in, int64_t out, int groups, bool ragged, ElemType type);
+void linear_bwd(const LinearBwdArgs& a, ElemType type, hipStream_t s);
 
 }  // namespace sxk

@@ -436,6 +436,155 @@ PyObject* adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+// A linear layer's activation, weights and groups: weight [out, in], or with ends [groups, out, in].
+struct Layer {
+    int activation;
+    void *weight, *bias = nullptr;
+    const at::Tensor* weights;
+    const int64_t* ends = nullptr;
+    int64_t in, out, groups = 0;
+};
+Layer layer_of(const Call& c, PyObject* weight, PyObject* bias, PyObject* ends, PyObject* activation, int type) {
+    Layer l{};
+    l.activation = static_cast<int>(std::clamp<int64_t>(number<int64_t>(activation, "activation"), -1, 255));
+    if (l.activation < 0) invalid("activation must be one of SXH_ACT_*");
+    const at::Tensor& w = tensor(c, weight, "weight");
+    const int64_t lead = given(ends) ? 1 : 0;
+    if (w.dim() != 2 + lead) invalid(lead ? "weight must be [groups, out, in]" : "weight must be [out, in]");
+    if (type_of(w) != type || !w.is_contiguous()) invalid("weight must be contiguous, of the rows' type");
+    l.weights = &w;
+    l.weight = w.data_ptr();
+    l.out = w.size(lead);
+    l.in = w.size(lead + 1);
+    if (given(ends)) {
+        const at::Tensor& e = tensor(c, ends, "ends");
+        l.groups = w.size(0);
+        if (l.groups < 1) invalid("weight has no groups");
+        if (e.scalar_type() != at::kLong || e.dim() != 1 || e.size(0) != l.groups || !e.is_contiguous())
+            invalid("ends must be " + std::to_string(l.groups) + " contiguous elements of int64");
+        l.ends = static_cast<const int64_t*>(e.data_ptr());
+    }
+    if (given(bias)) {
+        const at::Tensor& b = tensor(c, bias, "bias");
+        if (type_of(b) != type || !b.is_contiguous() || b.numel() != l.out * std::max<int64_t>(l.groups, 1))
+            invalid("bias must be contiguous, of the rows' type, an element for each row of weight");
+        l.bias = b.data_ptr();
+    }
+    return l;
+}
+// Rows of another width beside x's.
+Rows rows_beside(const Call& c, PyObject* o, const char* name, const Rows& x, int64_t width) {
+    const Rows r = rows_of(c, o, name);
+    if (r.type != x.type || r.t->dim() != x.t->dim() || r.width != width || r.t->sizes().slice(0, r.t->dim() - 1) != x.t->sizes().slice(0, r.t->dim() - 1))
+        invalid(std::string(name) + " must have the rows' type and shape, " + std::to_string(width) + " wide");
+    return r;
+}
+at::Tensor rows_beside(const at::Tensor& t, int64_t width) {
+    std::vector<int64_t> sizes(t.sizes().begin(), t.sizes().end());
+    sizes.back() = width;
+    return at::empty(sizes, t.options());
+}
+
+// (backend, device, stream, x, weight, bias, ends, activation, residual, want_pre) -> (y, pre)
+PyObject* linear_fwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded(n, 10, [&] {
+        const Call c = call_of(a);
+        const bool want_pre = flag(a[9]);
+        const Rows x = rows_of(c, a[3], "x");
+        const Layer l = layer_of(c, a[4], a[5], a[6], a[7], x.type);
+        if (x.width != l.in) invalid("x must be as wide as weight's rows");
+        sxh_linear_inputs in{};
+        in.x = x.p; in.weight = l.weight; in.bias = l.bias; in.ends = l.ends;
+        in.rows = x.rows; in.in = l.in; in.out = l.out; in.groups = l.groups; in.x_stride = x.stride;
+        in.type = static_cast<uint8_t>(x.type); in.activation = static_cast<uint8_t>(l.activation); in.clear = 1;
+        if (given(a[8])) {
+            const Rows r = rows_beside(c, a[8], "residual", x, l.out);
+            in.residual = r.p;
+            in.residual_stride = r.stride;
+        }
+        at::Tensor y, pre, work;
+        int32_t rc;
+        {
+            const Unlocked unlocked;
+            sxh_linear_outputs out{};
+            y = rows_beside(*x.t, l.out);
+            out.y = y.data_ptr();
+            out.y_stride = out.pre_stride = l.out;
+            if (want_pre) {
+                pre = rows_beside(*x.t, l.out);
+                out.pre = pre.data_ptr();
+            }
+            out.workspace_bytes = sxh_linear_fwd_workspace(in.rows, in.in, in.out, in.groups, in.type);
+            if (out.workspace_bytes) {
+                work = at::empty({out.workspace_bytes}, x.t->options().dtype(at::kByte));
+                out.workspace = work.data_ptr();
+            }
+            rc = sxh_linear_fwd(c.backend, &in, &out, &c.queue);
+        }
+        check(rc);
+        PyObject* t = PyTuple_New(2);
+        if (!t) throw Raised{};
+        PyTuple_SET_ITEM(t, 0, give(y));
+        PyTuple_SET_ITEM(t, 1, give(pre));
+        return t;
+    });
+}
+
+// (backend, device, stream, dy, x, weight, ends, pre, activation, want_dx, want_dweight, want_dbias) -> (dx, dweight, dbias)
+PyObject* linear_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded(n, 12, [&] {
+        const Call c = call_of(a);
+        const bool want_dx = flag(a[9]), want_dweight = flag(a[10]), want_dbias = flag(a[11]);
+        const Rows x = rows_of(c, a[4], "x");
+        const Layer l = layer_of(c, a[5], Py_None, a[6], a[8], x.type);
+        if (x.width != l.in) invalid("x must be as wide as weight's rows");
+        const Rows dy = rows_beside(c, a[3], "dy", x, l.out);
+        sxh_linear_grads_in in{};
+        in.dy = dy.p; in.x = x.p; in.weight = l.weight; in.ends = l.ends;
+        in.rows = x.rows; in.in = l.in; in.out = l.out; in.groups = l.groups; in.dy_stride = dy.stride; in.x_stride = x.stride;
+        in.type = static_cast<uint8_t>(x.type); in.activation = static_cast<uint8_t>(l.activation); in.clear = 1;
+        if (given(a[7])) {
+            const Rows p = rows_beside(c, a[7], "pre", x, l.out);
+            in.pre = p.p;
+            in.pre_stride = p.stride;
+        }
+        if (given(a[7]) != (l.activation != SXH_ACT_NONE)) invalid("pre is given with an activation, and only then");
+        at::Tensor dx, dweight, dbias, work;
+        int32_t rc;
+        {
+            const Unlocked unlocked;
+            sxh_linear_grads out{};
+            const at::TensorOptions options = x.t->options();
+            if (want_dx) {
+                dx = rows_beside(*x.t, l.in);
+                out.dx = dx.data_ptr();
+            }
+            out.dx_stride = l.in;
+            if (want_dweight) {
+                dweight = at::empty(l.weights->sizes(), options);
+                out.dweight = dweight.data_ptr();
+            }
+            if (want_dbias) {
+                dbias = at::empty(l.weights->sizes().slice(0, l.weights->dim() - 1), options);
+                out.dbias = dbias.data_ptr();
+            }
+            out.workspace_bytes = sxh_linear_bwd_workspace(in.rows, in.in, in.out, in.groups, in.type);
+            if (out.workspace_bytes) {
+                work = at::empty({out.workspace_bytes}, options.dtype(at::kByte));
+                out.workspace = work.data_ptr();
+            }
+            rc = sxh_linear_bwd(c.backend, &in, &out, &c.queue);
+        }
+        check(rc);
+        PyObject* t = PyTuple_New(3);
+        if (!t) throw Raised{};
+        PyTuple_SET_ITEM(t, 0, give(dx));
+        PyTuple_SET_ITEM(t, 1, give(dweight));
+        PyTuple_SET_ITEM(t, 2, give(dbias));
+        return t;
+    });
+}
+
 // (exception for invalid arguments, exception for failures at run time)
 PyObject* set_errors(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded(n, 2, [&] {
@@ -450,6 +599,8 @@ PyMethodDef kMethods[] = {
     {"layer_norm_bwd", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(layer_norm_bwd)), METH_FASTCALL, nullptr},
     {"grad_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(grad_norm)), METH_FASTCALL, nullptr},
     {"adamw", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(adamw)), METH_FASTCALL, nullptr},
+    {"linear_fwd", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(linear_fwd)), METH_FASTCALL, nullptr},
+    {"linear_bwd", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(linear_bwd)), METH_FASTCALL, nullptr},
     {"set_errors", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(set_errors)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };

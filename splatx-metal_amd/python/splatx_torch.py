@@ -1,10 +1,11 @@
-"""The learned heads' operators on torch tensors: layer norm forward and backward, the gradients' norm, AdamW with
-moments in 32 or 8 bits (the device-buffer part of include/splatx_hip.h).
+"""The learned heads' operators on torch tensors: layer norm and linear layers forward and backward, linear layers of groups of
+rows with their own weights, the gradients' norm, AdamW with moments in 32 or 8 bits (the device-buffer part of
+include/splatx_hip.h).
 
 `TorchBackend` is a `splatx_hip.Backend` whose further methods take tensors of its device and enqueue on torch's current
 stream there: they return at once, like torch's own operations, and a tensor in use on another stream than the current one
 is the caller's to order, as with those. What they return or use as workspace comes from torch's allocator on that stream.
-`layer_norm` is the differentiable form, and `AdamW` keeps a model's moments and steps its parameters.
+`layer_norm`, `linear` and `grouped_linear` are the differentiable forms, and `AdamW` keeps a model's moments and steps its parameters.
 
 torch brings a HIP runtime of its own, and one process must run on one: import this module (or torch) before anything
 loads the library.
@@ -22,6 +23,7 @@ import torch
 import splatx_hip as sh
 
 ADAMW_BLOCK = 256  # elements that share a scale with 8-bit moments
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3, "sigmoid": 4}
 
 
 # The C structs, for programs that have device memory without torch's tensors and call the entry points through `TorchBackend.lib`
@@ -48,6 +50,28 @@ class LayerNormGradsIn(C.Structure):
 
 
 class LayerNormGrads(C.Structure):
+    _fields_ = [("dx", C.c_void_p), ("dweight", C.c_void_p), ("dbias", C.c_void_p), ("dx_stride", C.c_int64),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)]
+
+
+class LinearInputs(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("weight", C.c_void_p), ("bias", C.c_void_p), ("residual", C.c_void_p), ("ends", C.c_void_p),
+                ("rows", C.c_int64), ("in_", C.c_int64), ("out", C.c_int64), ("groups", C.c_int64), ("x_stride", C.c_int64),
+                ("residual_stride", C.c_int64), ("type", C.c_uint8), ("activation", C.c_uint8), ("clear", C.c_uint8)]
+
+
+class LinearOutputs(C.Structure):
+    _fields_ = [("y", C.c_void_p), ("pre", C.c_void_p), ("y_stride", C.c_int64), ("pre_stride", C.c_int64),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)]
+
+
+class LinearGradsIn(C.Structure):
+    _fields_ = [("dy", C.c_void_p), ("pre", C.c_void_p), ("x", C.c_void_p), ("weight", C.c_void_p), ("ends", C.c_void_p),
+                ("rows", C.c_int64), ("in_", C.c_int64), ("out", C.c_int64), ("groups", C.c_int64), ("dy_stride", C.c_int64),
+                ("pre_stride", C.c_int64), ("x_stride", C.c_int64), ("type", C.c_uint8), ("activation", C.c_uint8), ("clear", C.c_uint8)]
+
+
+class LinearGrads(C.Structure):
     _fields_ = [("dx", C.c_void_p), ("dweight", C.c_void_p), ("dbias", C.c_void_p), ("dx_stride", C.c_int64),
                 ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)]
 
@@ -94,6 +118,19 @@ def _one_hip_runtime():
                                 "): import splatx_torch or torch before the library is loaded")
 
 
+def _ends(ends):
+    if ends is None:
+        raise sh.SxInvalidArgument("ends must be a tensor")
+    return ends
+
+
+def _act(activation) -> int:
+    try:
+        return ACTIVATIONS[activation]
+    except (KeyError, TypeError):
+        raise sh.SxInvalidArgument(f"activation must be one of {', '.join(ACTIVATIONS)}, not {activation!r}") from None
+
+
 def adamw_blocks(n: int) -> int:
     """Scales of a tensor of n elements with 8-bit moments."""
     return -(-n // ADAMW_BLOCK)
@@ -113,10 +150,11 @@ class TorchBackend(sh.Backend):
         self._index, self._address, self._ops = device_ordinal, self.handle.value, _extension()
         p, n = C.c_void_p, C.c_int64
         for name, args in (("layer_norm_fwd", (p, p, p, p)), ("layer_norm_bwd", (p, p, p, p)), ("grad_norm", (p, p, n, p, p, n, p)),
-                           ("adamw", (p, p, n, p, p))):
+                           ("adamw", (p, p, n, p, p)), ("linear_fwd", (p, p, p, p)), ("linear_bwd", (p, p, p, p))):
             f = getattr(self.lib, "sxh_" + name)
             f.argtypes, f.restype = args, C.c_int32
-        for name, args in (("layer_norm_bwd_workspace", (n, n)), ("grad_norm_workspace", (n,))):
+        for name, args in (("layer_norm_bwd_workspace", (n, n)), ("grad_norm_workspace", (n,)),
+                           ("linear_fwd_workspace", (n, n, n, n, C.c_uint8)), ("linear_bwd_workspace", (n, n, n, n, C.c_uint8))):
             f = getattr(self.lib, "sxh_" + name)
             f.argtypes, f.restype = args, n
 
@@ -135,6 +173,30 @@ class TorchBackend(sh.Backend):
         gradient dh that reaches h past the norm. dweight and dbias have the weight's type (float32 without one)."""
         return self._ops.layer_norm_bwd(self._address, self._index, _raw_stream(self._index), dy, h, mean, rstd, weight, dh, want_dx,
                                         want_dweight, want_dbias)
+
+    # -- linear layers -----------------------------------------------------------------------------------
+    def linear_fwd(self, x, weight, bias=None, activation="none", residual=None, want_pre=False):
+        """(y, pre): z = x weight^T + bias over the last dimension, y = act(z) + residual; pre, z as the backward reads it, is
+        None without `want_pre`. weight is [out, in]; activation: one of ACTIVATIONS."""
+        return self._ops.linear_fwd(self._address, self._index, _raw_stream(self._index), x, weight, bias, None, _act(activation),
+                                    residual, want_pre)
+
+    def linear_bwd(self, dy, x, weight, pre=None, activation="none", want_dx=True, want_dweight=True, want_dbias=True):
+        """(dx, dweight, dbias) of linear_fwd; the residual's gradient is dy. `pre`: the forward's, with an activation."""
+        return self._ops.linear_bwd(self._address, self._index, _raw_stream(self._index), dy, x, weight, None, pre, _act(activation),
+                                    want_dx, want_dweight, want_dbias)
+
+    def grouped_linear_fwd(self, x, weight, ends, bias=None, activation="none", residual=None, want_pre=False):
+        """linear_fwd where the rows come in groups with a weight [groups, out, in] and bias [groups, out] of their own. ends:
+        int64 [groups] on the device, ascending: group g has the rows from ends[g - 1] (0) up to ends[g]. Rows from the last end
+        on belong to none: their y and pre are zero, and their dx in the backward."""
+        return self._ops.linear_fwd(self._address, self._index, _raw_stream(self._index), x, weight, bias, _ends(ends), _act(activation),
+                                    residual, want_pre)
+
+    def grouped_linear_bwd(self, dy, x, weight, ends, pre=None, activation="none", want_dx=True, want_dweight=True, want_dbias=True):
+        """(dx, dweight, dbias) of grouped_linear_fwd; the weights of a group without rows get zeros."""
+        return self._ops.linear_bwd(self._address, self._index, _raw_stream(self._index), dy, x, weight, _ends(ends), pre,
+                                    _act(activation), want_dx, want_dweight, want_dbias)
 
     # -- many tensors ------------------------------------------------------------------------------------
     def grad_norm(self, grads):
@@ -191,6 +253,51 @@ def layer_norm(backend: TorchBackend, x, weight=None, bias=None, eps=1e-5, resid
     """Differentiable layer norm over the last dimension: y, or (y, x + residual) with a residual. weight and bias have as many
     elements as a row, in any shape, and so have their gradients."""
     return _LayerNorm.apply(backend, x, weight, bias, eps, residual)
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, backend, x, weight, bias, ends, activation, residual):
+        want_pre = activation != "none" and any(ctx.needs_input_grad[1:4])
+        if ends is None:
+            y, pre = backend.linear_fwd(x, weight, bias, activation, residual, want_pre)
+        else:
+            y, pre = backend.grouped_linear_fwd(x, weight, ends, bias, activation, residual, want_pre)
+        ctx.backend, ctx.activation = backend, activation
+        ctx.bias_shape = None if bias is None else bias.shape
+        ctx.save_for_backward(x, weight, ends, pre)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, ends, pre = ctx.saved_tensors
+        _, need_x, need_w, need_b, _, _, need_r = ctx.needs_input_grad
+        dresidual = dy if need_r else None
+        if need_r and ends is not None:  # (a row of no group has no part of it)
+            ours = torch.arange(dy.numel() // dy.shape[-1], device=dy.device) < ends[-1]
+            dresidual = torch.where(ours.view(*dy.shape[:-1], 1), dy, torch.zeros((), dtype=dy.dtype, device=dy.device))
+        if not (need_x or need_w or need_b):
+            return None, None, None, None, None, None, dresidual
+        # (a sum's gradient is one value broadcast; a transposed layer's has its rows in other places)
+        dy = dy if dy.dim() == 2 and dy.stride(1) == 1 else dy.contiguous()
+        wanted = dict(pre=pre, activation=ctx.activation, want_dx=need_x, want_dweight=need_w, want_dbias=need_b)
+        if ends is None:
+            dx, dweight, dbias = ctx.backend.linear_bwd(dy, x, weight, **wanted)
+        else:
+            dx, dweight, dbias = ctx.backend.grouped_linear_bwd(dy, x, weight, ends, **wanted)
+        return None, dx, dweight, dbias if dbias is None else dbias.view(ctx.bias_shape), None, None, dresidual
+
+
+def linear(backend: TorchBackend, x, weight, bias=None, activation="none", residual=None):
+    """Differentiable act(x weight^T + bias) + residual over the last dimension, weight [out, in]; activation: one of ACTIVATIONS."""
+    return _Linear.apply(backend, x, weight, bias, None, activation, residual)
+
+
+def grouped_linear(backend: TorchBackend, x, weight, ends, bias=None, activation="none", residual=None):
+    """Differentiable linear layer of rows that come in groups, each with its own weight of [groups, out, in] and bias of
+    [groups, out] (TorchBackend.grouped_linear_fwd has what `ends` is)."""
+    return _Linear.apply(backend, x, weight, bias, _ends(ends), activation, residual)
 
 
 class AdamW:

@@ -1,0 +1,131 @@
+"""Linear layers and linear layers of groups of rows, forward and backward, against their definitions in 64 bits (linear_ref)."""
+import math
+
+import pytest
+import torch  # before anything loads the library: its HIP runtime is the process's
+
+import linear_ref as ref
+import splatx_hip as sh
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+TYPES = (F32, BF16, F16)
+
+
+@pytest.fixture(scope="module")
+def tb():
+    import splatx_torch
+    b = splatx_torch.TorchBackend(0)
+    yield b
+    b.close()
+
+
+def randn(*shape, seed=0, dtype=F32):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randn(*shape, generator=g, device="cuda").to(dtype)
+
+
+def whole(*shape, seed=0, dtype=F32, most=3):
+    """Whole numbers: their sums are exact, so that results have to be equal."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randint(-most, most + 1, shape, generator=g, device="cuda").to(dtype)
+
+
+def held(t, pad, off=0):
+    """t with its rows `pad` elements further apart than they are long, `off` elements into its buffer, between NaN."""
+    if not pad and not off:
+        return t
+    rows, width = t.shape
+    flat = torch.full((off + rows * (width + pad),), float("nan"), dtype=t.dtype, device="cuda")
+    v = flat[off:].view(rows, width + pad)[:, :width]
+    v.copy_(t)
+    return v
+
+
+def within(got, want, bound, what):
+    assert got.shape == want.shape, what
+    d = (got.double() - want).abs()
+    bad = ~((d <= bound) | (got == want))
+    assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} outside, first at {bad.nonzero()[0].tolist()}, worst {(d / bound)[bad].max():.3g} of the bound"
+
+
+def compare(tb, rows, n_in, n_out, dtype, act="none", bias=True, add=False, pad=0, off=0, sizes=None, seed=0):
+    print(f"rows {rows} {n_in} -> {n_out} {dtype} {act} bias {bias} add {add} pad {pad} off {off} groups {sizes if sizes is None else sizes[:8]}", flush=True)
+    lead, ends = (), None
+    if sizes is not None:
+        lead, ends = (len(sizes),), torch.cumsum(torch.tensor(sizes), 0).cuda()
+    x, w = randn(rows, n_in, seed=seed, dtype=dtype), (randn(*lead, n_out, n_in, seed=seed + 1) / math.sqrt(n_in)).to(dtype)
+    b = randn(*lead, n_out, seed=seed + 2, dtype=dtype) if bias else None
+    r = randn(rows, n_out, seed=seed + 3, dtype=dtype) if add else None
+    (y, pre), (ey, epre) = ref.fwd(x, w, b, act, r, ends)
+    held_ = lambda t: None if t is None else held(t, pad, off)  # noqa: E731
+    if sizes is None:
+        gy, gpre = tb.linear_fwd(held_(x), w, b, act, held_(r), True)
+        alone, none = tb.linear_fwd(held_(x), w, b, act, held_(r))
+    else:
+        gy, gpre = tb.grouped_linear_fwd(held_(x), w, ends, b, act, held_(r), True)
+        alone, none = tb.grouped_linear_fwd(held_(x), w, ends, b, act, held_(r))
+    assert gy.dtype == gpre.dtype == dtype and none is None and torch.equal(alone, gy)
+    within(gy, y, ey, "y")
+    within(gpre, pre, epre, "pre")
+    dy, z = randn(rows, n_out, seed=seed + 4, dtype=dtype), None if act == "none" else randn(rows, n_out, seed=seed + 5, dtype=dtype)
+    want, bounds = ref.bwd(dy, x, w, z, act, ends)
+    if sizes is None:
+        f = lambda **k: tb.linear_bwd(held_(dy), held_(x), w, held_(z), act, **k)  # noqa: E731
+    else:
+        f = lambda **k: tb.grouped_linear_bwd(held_(dy), held_(x), w, ends, held_(z), act, **k)  # noqa: E731
+    got = f()
+    for g, v, e, name in zip(got, want, bounds, ("dx", "dweight", "dbias")):
+        assert g.dtype == dtype
+        within(g, v, e, name)
+    for g, a in zip(got, f()):
+        assert torch.equal(g, a)
+    return got, f
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,n_in,n_out", [
+    (1, 1, 1), (1, 16, 64), (2, 3, 5), (31, 7, 9), (33, 8, 8), (65, 45, 64), (300, 48, 64), (257, 64, 3), (129, 64, 64), (1000, 65, 33),
+    (640, 128, 128), (513, 100, 131), (200, 129, 127), (77, 256, 300), (300, 300, 260), (9, 1024, 512), (1, 2048, 130), (40, 130, 2050),
+    (130, 1000, 1001), (1025, 512, 768)])
+def test_whole_numbers_are_exact(tb, rows, n_in, n_out, dtype):
+    """Every index counts: with whole numbers the results are the definition's, rounded once."""
+    print(rows, n_in, n_out, dtype, flush=True)
+    most = 1 if dtype == F16 and max(rows, n_in, n_out) > 900 else 3
+    x, w, b = whole(rows, n_in, seed=1, dtype=dtype, most=most), whole(n_out, n_in, seed=2, dtype=dtype, most=most), whole(n_out, seed=3, dtype=dtype)
+    r, dy = whole(rows, n_out, seed=4, dtype=dtype), whole(rows, n_out, seed=5, dtype=dtype, most=most)
+    z = x.double() @ w.double().t().contiguous() + b.double()
+    y, pre = tb.linear_fwd(x, w, b, "relu", r, True)
+    assert torch.equal(pre, z.to(dtype)) and torch.equal(y, (z.clamp_min(0) + r.double()).to(dtype))
+    dz = torch.where(pre > 0, dy, torch.zeros_like(dy)).double()
+    for act, d in (("relu", dz), ("none", dy.double())):
+        dx, dw, db = tb.linear_bwd(dy, x, w, pre if act == "relu" else None, act)
+        assert torch.equal(dx, (d @ w.double()).to(dtype))
+        assert torch.equal(dw, (d.t().contiguous() @ x.double()).to(dtype))
+        assert torch.equal(db, d.sum(0).to(dtype))
+
+
+SHAPES = [(1, 16, 64), (3, 5, 7), (64, 48, 64), (2000, 45, 64), (777, 64, 3), (1001, 64, 64), (500, 64, 128), (300, 96, 65), (70, 128, 256),
+          (515, 200, 136), (9, 2048, 520), (33, 700, 300), (1030, 520, 264), (129, 257, 383)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("act", ref.ACTS)
+@pytest.mark.parametrize("i", range(len(SHAPES)))
+def test_linear(tb, i, act, dtype):
+    k = i + ref.ACTS.index(act)
+    compare(tb, *SHAPES[i], dtype, act, bias=k % 4 != 3, add=k % 2 == 1, pad=(0, 0, 8, 3)[k % 4], off=(0, 0, 0, 1, 5)[k % 5], seed=10 * i)
+
+
+SIZES = [[5], [0], [0, 0, 7, 0], [1] * 70, [64, 64, 64], [63, 1, 65, 0, 127, 129, 300], [1000, 0, 3], [0, 2, 0, 900, 31, 0, 33, 257, 0],
+         [17, 200, 0, 1, 1, 90] * 23]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n_in,n_out,act", [(48, 64, "relu"), (64, 64, "gelu"), (45, 3, "sigmoid"), (128, 40, "none"), (96, 200, "silu"), (300, 260, "gelu")])
+@pytest.mark.parametrize("i", range(len(SIZES)))
+def test_grouped_linear(tb, i, n_in, n_out, act, dtype):
+    sizes, behind = SIZES[i], (0, 1, 70, 200)[(i + n_in) % 4]
+    k = i + n_out
+    compare(tb, sum(sizes) + behind, n_in, n_out, dtype, act, bias=k % 3 != 2, add=k % 2 == 0, pad=(0, 8, 1)[k % 3], off=k % 2, sizes=sizes, seed=i)
