@@ -17,24 +17,33 @@ namespace {
 // out[r][c] = sum over d of row(r, d) col(c, d): x W^T, dz W and dz^T x, each operand either with its sums' elements side by
 // side in memory (plain) or with its rows side by side (Across: W's columns, dz's and x's).
 
+// What follows the sums, of rows of `cols` columns.
+struct Finish {
+    void* out;
+    int64_t out_stride, cols;
+    const void* residual;
+    int64_t residual_stride;
+    void* pre;
+    int64_t pre_stride;
+    int act;
+    bool clear;  // rows behind the last group become zero
+};
+
 struct TileArgs {
     const void *row, *col;
     int64_t row_stride, col_stride;  // elements between the rows in memory
     int64_t col_group;               // elements between the groups' col operands
-    void* out;
-    int64_t out_stride, out_group;
-    int64_t rows, cols, depth;       // rows (of the products over rows), depth (of those over groups' rows): all groups'
+    Finish to;                       // (its cols are the outputs')
+    int64_t out_group;
+    int64_t rows, depth;             // rows (of the products over rows), depth (of those over groups' rows): all groups'
     Groups groups;
     int shift;                       // the parts' rows, log2
     int64_t slots;
     float* partial;                  // [slabs][rows][cols] in place of out, or null
     int64_t split;                   // depth of a slab
     int splits;
-    const void *bias, *residual;     // of out
-    void* pre;
-    int64_t bias_group, residual_stride, pre_stride;
-    int act;
-    bool clear;                      // rows behind the last group become zero
+    const void* bias;
+    int64_t bias_group;
 };
 
 // Where the 16 bytes (row r, chunk c) of a plain operand's tile lie: 128 bytes a row, the chunks of eight rows in different
@@ -130,26 +139,74 @@ __device__ inline void store_some(T* p, Floats<V> v, int n) {
         if (e < n) p[e] = static_cast<T>(v[e]);
 }
 
-// What follows the sums: four columns from c on of row r.
+// Four columns from c on of row r, bias included.
 template <class T>
-__device__ inline void finish(const TileArgs& a, int group, int64_t r, int64_t c, Floats<4> v) {
+__device__ inline void finish4(const Finish& a, int64_t r, int64_t c, Floats<4> v) {
     const int n = static_cast<int>(min(a.cols - c, int64_t{4}));
     if (n <= 0) return;
-    if (a.bias) v += load_some<T, 4>(static_cast<const T*>(a.bias) + group * a.bias_group + c, n);
     if (a.pre) store_some<T, 4>(static_cast<T*>(a.pre) + r * a.pre_stride + c, v, n);
     if (a.act)
 #pragma unroll
         for (int e = 0; e < 4; e++) v[e] = activated<T>(v[e], a.act);
     if (a.residual) v += load_some<T, 4>(static_cast<const T*>(a.residual) + r * a.residual_stride + c, n);
-    store_some<T, 4>(static_cast<T*>(a.out) + group * a.out_group + r * a.out_stride + c, v, n);
+    store_some<T, 4>(static_cast<T*>(a.out) + r * a.out_stride + c, v, n);
 }
 // The same of a row behind the last group.
 template <class T>
-__device__ inline void clear(const TileArgs& a, int64_t r, int64_t c) {
+__device__ inline void clear4(const Finish& a, int64_t r, int64_t c) {
     const int n = static_cast<int>(min(a.cols - c, int64_t{4}));
     if (n <= 0 || !a.clear) return;
     store_some<T, 4>(static_cast<T*>(a.out) + r * a.out_stride + c, Floats<4>(0.0f), n);
     if (a.pre) store_some<T, 4>(static_cast<T*>(a.pre) + r * a.pre_stride + c, Floats<4>(0.0f), n);
+}
+
+// 16-bit elements of 16 columns between the sums' layout (a lane has columns 0..3 and 8..11 of its row, its partner in the
+// wave's other half 4..7 and 12..15) and memory's (0..7 and 8..15, 16 bytes a lane): the partners swap, both ways.
+template <class T>
+__device__ inline Frag<T> swapped(Frag<T> v) {
+    using Words = uint32_t __attribute__((ext_vector_type(4)));
+    const Words w = __builtin_bit_cast(Words, v);
+    const auto a = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false), b = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
+    return __builtin_bit_cast(Frag<T>, Words{a[0], b[0], a[1], b[1]});
+}
+
+// A wave's 32 x 32 sums, bias included: row r of the lane (if it is `valid`), columns from c on. Every lane takes part.
+template <class T>
+__device__ inline void finish32(const Finish& a, int64_t r, bool valid, int64_t c, const Sums& s) {
+    constexpr int V = kPer<T>;
+    const int half = threadIdx.x % 64 / 32;
+    T* const out = static_cast<T*>(a.out) + r * a.out_stride;
+#pragma unroll
+    for (int p = 0; p < 32 / (2 * V); p++) {
+        Floats<V> v;
+#pragma unroll
+        for (int e = 0; e < V; e++) v[e] = s[p * V + e];
+        const int64_t column = c + p * 2 * V + half * V;
+        const int n = valid ? static_cast<int>(max(int64_t{0}, min(a.cols - column, int64_t{V}))) : 0;
+        const auto in_memory = [](Floats<V> f) {
+            Frag<T> t = raw<T, V>(f);
+            if constexpr (V == 8) t = swapped<T>(t);
+            return t;
+        };
+        const auto store = [&](T* row, Frag<T> t) {
+            if (n == V) store_raw<V>(row + column, t);
+            else
+#pragma unroll
+                for (int e = 0; e < V - 1; e++)
+                    if (e < n) row[column + e] = t[e];
+        };
+        Frag<T> residual(0);
+        if (a.residual && n) residual = load_within(static_cast<const T*>(a.residual) + r * a.residual_stride, column, a.cols);
+        if (a.pre) store(static_cast<T*>(a.pre) + r * a.pre_stride, in_memory(v));
+        if (a.act)
+#pragma unroll
+            for (int e = 0; e < V; e++) v[e] = activated<T>(v[e], a.act);
+        if (a.residual) {
+            if constexpr (V == 8) residual = swapped<T>(residual);
+            v += floats<T, V>(residual);
+        }
+        store(out, in_memory(v));
+    }
 }
 
 // BR x BC outputs a workgroup, WR x WC a wave. OverRows: the sums go over a group's rows (dW), else the outputs' rows are the
@@ -161,7 +218,7 @@ __global__ void __launch_bounds__(BR / WR * (BC / WC) * 64) k_tile(TileArgs a) {
     constexpr int kBuffer = (BR + BC) * 128, I = WR / 32, J = WC / 32;
     __shared__ __attribute__((aligned(128))) char lds[2 * kBuffer];
     // Which tile: workgroups go round the eight dies, and each die takes tiles side by side, eight rows of tiles at a time.
-    const int64_t across = (a.cols + BC - 1) / BC, down = OverRows ? (a.rows + BR - 1) / BR : a.slots, tiles = across * down;
+    const int64_t across = (a.to.cols + BC - 1) / BC, down = OverRows ? (a.rows + BR - 1) / BR : a.slots, tiles = across * down;
     const int64_t each = (tiles + 7) / 8, tile = blockIdx.x % 8 * each + blockIdx.x / 8;
     if (blockIdx.x / 8 >= each || tile >= tiles) return;
     const int64_t band = tile / (8 * across), height = min(down - band * 8, int64_t{8});
@@ -188,7 +245,7 @@ __global__ void __launch_bounds__(BR / WR * (BC / WC) * 64) k_tile(TileArgs a) {
     if (!OverRows && part.group >= a.groups.groups) {
         if (a.partial) return;
         for (int64_t r = r0 + threadIdx.x / 32; r < r1; r += kThreads / 32)
-            for (int c = threadIdx.x % 32 * 4; c < BC; c += 128) clear<T>(a, r, c0 + c);
+            for (int c = threadIdx.x % 32 * 4; c < BC; c += 128) clear4<T>(a.to, r, c0 + c);
         return;
     }
     Sums sums[I][J];
@@ -197,7 +254,7 @@ __global__ void __launch_bounds__(BR / WR * (BC / WC) * 64) k_tile(TileArgs a) {
 #pragma unroll
         for (int j = 0; j < J; j++) sums[i][j] = Sums(0.0f);
     Stage<T, BR, RowAcross, kThreads> row(static_cast<const T*>(a.row), a.row_stride, r0, r1);
-    Stage<T, BC, ColAcross, kThreads> col(static_cast<const T*>(a.col) + part.group * a.col_group, a.col_stride, c0, a.cols);
+    Stage<T, BC, ColAcross, kThreads> col(static_cast<const T*>(a.col) + part.group * a.col_group, a.col_stride, c0, a.to.cols);
     if (d0 < d1) {
         row.load(d0, d1);
         col.load(d0, d1);
@@ -235,55 +292,385 @@ __global__ void __launch_bounds__(BR / WR * (BC / WC) * 64) k_tile(TileArgs a) {
 #pragma unroll
     for (int i = 0; i < I; i++) {
         const int64_t r = r0 + wr + i * 32 + lane % 32;
-        if (r >= r1) continue;
 #pragma unroll
-        for (int j = 0; j < J; j++)
+        for (int j = 0; j < J; j++) {
+            const int64_t c = c0 + wc + j * 32;
+            if (c >= a.to.cols) break;
+            if (a.partial) {
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-                const int64_t c = c0 + wc + j * 32 + 8 * q + lane / 32 * 4;
-                const Floats<4> v = {sums[i][j][4 * q], sums[i][j][4 * q + 1], sums[i][j][4 * q + 2], sums[i][j][4 * q + 3]};
-                if (a.partial) {
-                    const int n = static_cast<int>(min(a.cols - c, int64_t{4}));
-                    if (n > 0) store_some<float, 4>(a.partial + (int64_t{blockIdx.y} * a.rows + r) * a.cols + c, v, n);
-                } else {
-                    finish<T>(a, part.group, r, c, v);
+                for (int q = 0; q < 4; q++) {
+                    const int64_t at = c + 8 * q + lane / 32 * 4;
+                    const int n = r < r1 ? static_cast<int>(max(int64_t{0}, min(a.to.cols - at, int64_t{4}))) : 0;
+                    const Floats<4> v = {sums[i][j][4 * q], sums[i][j][4 * q + 1], sums[i][j][4 * q + 2], sums[i][j][4 * q + 3]};
+                    store_some<float, 4>(a.partial + (int64_t{blockIdx.y} * a.rows + r) * a.to.cols + at, v, n);
                 }
+                continue;
             }
+            if (a.bias)
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const int64_t at = c + 8 * q + lane / 32 * 4;
+                    const Floats<4> v = load_some<T, 4>(static_cast<const T*>(a.bias) + part.group * a.bias_group + at,
+                                                        static_cast<int>(max(int64_t{0}, min(a.to.cols - at, int64_t{4}))));
+#pragma unroll
+                    for (int e = 0; e < 4; e++) sums[i][j][4 * q + e] += v[e];
+                }
+            Finish to = a.to;
+            to.out = static_cast<T*>(to.out) + part.group * a.out_group;
+            finish32<T>(to, r, r < r1, c, sums[i][j]);
+        }
     }
 }
 
-// The slabs of partial sums, added in order. Over rows: group blockIdx.z's slots, else all splits.
-template <class T, bool OverRows>
-__global__ void __launch_bounds__(256) k_tile_join(TileArgs a) {
-    const int64_t quads = (a.cols + 3) / 4;
-    int group = OverRows ? blockIdx.y : 0;
-    int64_t first = 0, slabs = a.splits;
-    if constexpr (OverRows) {
-        const int64_t begin = a.groups.begin(group), end = a.groups.end(group);
-        first = group + (begin >> a.shift);
-        slabs = end > begin ? ((end - begin - 1) >> a.shift) + 1 : 0;
-    }
+// The splits' slabs, added in order.
+template <class T>
+__global__ void __launch_bounds__(256) k_split_join(TileArgs a) {
+    const int64_t quads = (a.to.cols + 3) / 4;
     for (int64_t i = blockIdx.x * int64_t{256} + threadIdx.x; i < a.rows * quads; i += gridDim.x * int64_t{256}) {
         const int64_t r = i / quads, c = i % quads * 4;
-        const int n = static_cast<int>(min(a.cols - c, int64_t{4}));
-        if constexpr (!OverRows) {
-            if (a.groups.ends) {
-                int lo = 0, hi = a.groups.groups;  // the first group that ends behind the row
-                while (lo < hi) {
-                    const int mid = (lo + hi) / 2;
-                    if (a.groups.end(mid) <= r) lo = mid + 1;
-                    else hi = mid;
-                }
-                group = lo;
-                if (group >= a.groups.groups) {
-                    clear<T>(a, r, c);
-                    continue;
-                }
+        const int n = static_cast<int>(min(a.to.cols - c, int64_t{4}));
+        int group = 0;
+        if (a.groups.ends) {
+            int hi = a.groups.groups;  // the first group that ends behind the row
+            while (group < hi) {
+                const int mid = (group + hi) / 2;
+                if (a.groups.end(mid) <= r) group = mid + 1;
+                else hi = mid;
+            }
+            if (group >= a.groups.groups) {
+                clear4<T>(a.to, r, c);
+                continue;
             }
         }
         Floats<4> sum(0.0f);
-        for (int64_t s = 0; s < slabs; s++) sum += load_some<float, 4>(a.partial + ((first + s) * a.rows + r) * a.cols + c, n);
-        finish<T>(a, group, r, c, sum);
+        for (int s = 0; s < a.splits; s++) sum += load_some<float, 4>(a.partial + (s * a.rows + r) * a.to.cols + c, n);
+        if (a.bias) sum += load_some<T, 4>(static_cast<const T*>(a.bias) + group * a.bias_group + c, n);
+        finish4<T>(a.to, r, c, sum);
+    }
+}
+
+// Gradients of a group's weights from the slabs of its parts of the rows: [out * in] of dweight, then, where dbias is wanted,
+// [out] of it. A group's first slab is g + its first row / step; each has `step` rows, counted from the group's first row
+// (`from_begin`) or from the first of all. `turns` threads (a power of two) share four elements.
+struct JoinArgs {
+    const float* partial;
+    void *dweight, *dbias;
+    int64_t weights, wanted, size;  // elements of a group's dweight, of what is joined, of a slab
+    Groups groups;
+    int64_t step;
+    bool from_begin;
+    int turns;
+};
+template <class T>
+__global__ void __launch_bounds__(256) k_weights_join(JoinArgs a) {
+    __shared__ Floats<4> part[256];
+    const int each = 256 / a.turns, lane = threadIdx.x % each, turn = threadIdx.x / each, group = blockIdx.y;
+    const int64_t begin = a.groups.begin(group), end = a.groups.end(group), first = group + begin / a.step;
+    const int64_t slabs = end > begin ? (end - 1 - (a.from_begin ? begin : 0)) / a.step - (a.from_begin ? 0 : begin / a.step) + 1 : 0;
+    for (int64_t at = int64_t{blockIdx.x} * each; at * 4 < a.wanted; at += int64_t{gridDim.x} * each) {
+        const int64_t i = (at + lane) * 4;
+        const int n = static_cast<int>(max(int64_t{0}, min(a.wanted - i, int64_t{4})));
+        Floats<4> sum(0.0f);
+        if (n > 0)
+#pragma unroll 4
+            for (int64_t s = turn; s < slabs; s += a.turns) sum += load_some<float, 4>(a.partial + (first + s) * a.size + i, n);
+        if (a.turns > 1) {
+            __syncthreads();
+            part[threadIdx.x] = sum;
+            __syncthreads();
+            if (turn) continue;
+            for (int t = 1; t < a.turns; t++) sum += part[t * each + lane];
+        }
+        T* const dweight = static_cast<T*>(a.dweight) + group * a.weights;
+        if (a.dweight && i + n <= a.weights) {
+            store_some<T, 4>(dweight + i, sum, n);
+            continue;
+        }
+        for (int e = 0; e < n; e++) {
+            if (i + e >= a.weights) static_cast<T*>(a.dbias)[group * (a.wanted - a.weights) + i + e - a.weights] = static_cast<T>(sum[e]);
+            else if (a.dweight) dweight[i + e] = static_cast<T>(sum[e]);
+        }
+    }
+}
+
+// ---- narrow layers ----------------------------------------------------------------------------------------
+//
+// Where the weight fits the LDS a layer is bound by its rows' bytes: each workgroup holds the weight there, as fragments in the
+// order of the lanes, and takes its share of all rows past it, `chunk` rows side by side (a group's end among them changes the
+// weight).
+
+// The group that has the row; every lane of the wave takes part.
+__device__ inline int group_of(const Groups& g, int64_t row) {
+    int k = 0;
+    if (g.ends)
+        for (int first = 0; first < g.groups; first += 64) {
+            const int e = first + static_cast<int>(threadIdx.x % 64);
+            k += __builtin_popcountll(__ballot(e < g.groups && g.end(e) <= row));
+        }
+    return __builtin_amdgcn_readfirstlane(k);
+}
+
+struct NarrowArgs {
+    const void *x, *weight, *bias;
+    int64_t x_stride;
+    Finish to;
+    int64_t in, out, chunk;
+    Groups groups;
+};
+
+// Fragments of a row of which the last may reach past its end: load_within without a branch, for rows of a fragment at least.
+template <class T, int K>
+struct RowLoad {
+    static constexpr int V = kPer<T>;
+    int64_t in;
+    int last, down;  // where the last fragment is read, and the bytes it moves down
+    bool small;
+    __device__ explicit RowLoad(int64_t n) : in(n) {
+        const int k = (2 * (K - 1) + static_cast<int>(threadIdx.x) % 64 / 32) * V;
+        small = n < V;
+        last = small ? 0 : min(k, static_cast<int>(n) - V);
+        down = (k - last) * static_cast<int>(sizeof(T));
+    }
+    __device__ void operator()(Frag<T> (&f)[K], const T* row) const {
+        const int half = threadIdx.x % 64 / 32;
+        if (small) {
+            f[0] = load_within(row, half * V, in);
+            return;
+        }
+#pragma unroll
+        for (int k = 0; k < K - 1; k++) f[k] = load_raw<V>(row + (2 * k + half) * V);
+        f[K - 1] = load_raw<V>(row + last);
+        if (in % (2 * V)) f[K - 1] = down < 16 ? moved_down<T>(f[K - 1], down) : Frag<T>(0);
+    }
+};
+
+// K steps of 32 bytes a row. A wave takes 32 rows at a time; the next 32 are on their way meanwhile.
+template <class T, int K>
+__global__ void __launch_bounds__(512) k_narrow_fwd(NarrowArgs a) {
+    constexpr int V = kPer<T>;
+    extern __shared__ __attribute__((aligned(128))) char lds[];
+    const int tiles = static_cast<int>((a.out + 31) / 32), lane = threadIdx.x % 64, wave = threadIdx.x / 64, rows_at_once = blockDim.x / 2;
+    Frag<T>* const weights = reinterpret_cast<Frag<T>*>(lds);
+    float* const bias = reinterpret_cast<float*>(lds + tiles * K * 1024);
+    const RowLoad<T, K> load(a.in);
+    const T* const x = static_cast<const T*>(a.x);
+    const int64_t last = min(a.groups.rows, (blockIdx.x + int64_t{1}) * a.chunk);
+    for (int64_t first = blockIdx.x * a.chunk; first < last;) {
+        const int group = group_of(a.groups, first);
+        if (group >= a.groups.groups) {
+            for (int64_t r = first + threadIdx.x / 8; r < last; r += blockDim.x / 8)
+                for (int64_t c = threadIdx.x % 8 * 4; c < a.out; c += 32) clear4<T>(a.to, r, c);
+            return;
+        }
+        const int64_t stop = max(first + 1, min(last, a.groups.end(group)));  // (a row at least, whatever the ends are)
+        Frag<T> next[K];
+        int64_t base = first + wave * 32;
+        load(next, x + min(base + lane % 32, stop - 1) * a.x_stride);
+        __syncthreads();
+        const T* const w = static_cast<const T*>(a.weight) + group * a.in * a.out;
+        for (int i = threadIdx.x; i < tiles * K * 64; i += blockDim.x) {
+            const int n = i / 64 / K * 32 + i % 32;
+            weights[i] = n < a.out ? load_within(w + n * a.in, (2 * (i / 64 % K) + i % 64 / 32) * V, a.in) : Frag<T>(0);
+        }
+        for (int i = threadIdx.x; i < tiles * 32; i += blockDim.x)
+            bias[i] = a.bias && i < a.out ? static_cast<float>(static_cast<const T*>(a.bias)[group * a.out + i]) : 0.0f;
+        __syncthreads();
+        for (; base < stop; base += rows_at_once) {
+            Frag<T> now[K];
+#pragma unroll
+            for (int k = 0; k < K; k++) now[k] = next[k];
+            if (base + rows_at_once < stop) load(next, x + min(base + rows_at_once + lane % 32, stop - 1) * a.x_stride);
+            const int64_t r = base + lane % 32;
+            for (int t = 0; t < tiles; t++) {
+                Sums sums;
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const Floats<4> b = *reinterpret_cast<const Floats<4>*>(bias + t * 32 + 8 * q + lane / 32 * 4);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) sums[4 * q + e] = b[e];
+                }
+#pragma unroll
+                for (int k = 0; k < K; k++) mma(sums, weights[(t * K + k) * 64 + lane], now[k]);
+                finish32<T>(a.to, r, r < stop, t * 32, sums);
+            }
+        }
+        first = stop;
+    }
+}
+
+struct NarrowBwdArgs {
+    const void *dy, *pre, *x, *weight;  // x: null where dweight is not wanted
+    int64_t dy_stride, pre_stride, x_stride;
+    Finish to;       // dx; its out may be null
+    float* partial;  // slabs of dweight and dbias, or null
+    int64_t size;    // of a slab
+    int64_t in, out, chunk;
+    Groups groups;
+    int act;
+};
+// Bytes between the lines of a block in LDS: `tiles` times 32 elements, and what puts four lines (floats: the lanes' lines)
+// into different banks.
+template <class T>
+__host__ __device__ constexpr int line_bytes(int tiles) { return tiles * 32 * static_cast<int>(sizeof(T)) + (sizeof(T) == 2 ? 32 : 16); }
+template <class T>
+constexpr int kBlockRows = 256 / static_cast<int>(sizeof(T));
+
+// Fragments of the lane's column: the block's lines along it, step s of eight.
+template <class T>
+__device__ inline Frag<T> across_fragment(const char* block, int bytes, int column, int s) {
+    const int lane = threadIdx.x % 64, half = lane / 32;
+    if constexpr (sizeof(T) == 4) {
+        Frag<T> f;
+#pragma unroll
+        for (int i = 0; i < 4; i++) f[i] = *reinterpret_cast<const float*>(block + (s * 8 + half * 4 + i) * bytes + (column + lane % 32) * 4);
+        return f;
+    } else {
+        using Four = short __attribute__((ext_vector_type(4)));
+        using Lds = __attribute__((address_space(3))) Four*;
+        const int group = lane % 16;
+        Four part[2];
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+            part[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (Lds)(block + (s * 16 + half * 8 + j * 4 + group / 4) * bytes + (column + lane % 32 / 16 * 16 + group % 4 * 4) * 2));
+        return __builtin_bit_cast(Frag<T>, __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+}
+
+// All three gradients in one pass: a block of rows of dz and x lies in LDS, its products with the weight are dx's rows, and the
+// products of its columns with one another stay in registers over the rows of a group: `Tiles` tiles of 32 x 32 of dweight a
+// wave. The next block is on its way meanwhile, `Passes` fragments a thread of each.
+template <class T, int Waves, int Tiles, int Passes>
+__global__ void __launch_bounds__(Waves * 64) k_narrow_bwd(NarrowBwdArgs a) {
+    constexpr int V = kPer<T>, kRows = kBlockRows<T>, kThreads = Waves * 64, kSteps = static_cast<int>(sizeof(T));
+    extern __shared__ __attribute__((aligned(128))) char lds[];
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    const int nt = static_cast<int>((a.out + 31) / 32), kt = static_cast<int>((a.in + 31) / 32);
+    const int z_bytes = line_bytes<T>(nt), x_bytes = line_bytes<T>(kt);
+    char *const dz = lds, *const xs = lds + kRows * z_bytes;
+    Frag<T>* const weights = reinterpret_cast<Frag<T>*>(xs + kRows * x_bytes);
+    // where a thread's fragments lie in a block: as many threads as a power of two holds a row's go along it
+    const auto lanes_of = [](int chunks) { return chunks <= 1 ? 1 : 1 << (32 - __builtin_clz(chunks - 1)); };
+    const int z_chunks = nt * 32 / V, x_chunks = kt * 32 / V, z_lanes = lanes_of(z_chunks), x_lanes = lanes_of(x_chunks);
+    const int zc = threadIdx.x % z_lanes, zl = threadIdx.x / z_lanes, xc = threadIdx.x % x_lanes, xl = threadIdx.x / x_lanes;
+    const int z_step = kThreads / z_lanes, x_step = kThreads / x_lanes;
+    Frag<T> dy[Passes], pre[Passes], xv[Passes];
+    const auto load = [&](int64_t first, int64_t stop) {
+#pragma unroll
+        for (int p = 0; p < Passes; p++) {
+            const int l = zl + p * z_step;
+            const int64_t r = first + l;
+            dy[p] = pre[p] = Frag<T>(0);
+            if (l < kRows && r < stop && zc < z_chunks) {
+                dy[p] = load_within(static_cast<const T*>(a.dy) + r * a.dy_stride, zc * V, a.out);
+                if (a.act) pre[p] = load_within(static_cast<const T*>(a.pre) + r * a.pre_stride, zc * V, a.out);
+            }
+        }
+        if (a.x)
+#pragma unroll
+            for (int p = 0; p < Passes; p++) {
+                const int l = xl + p * x_step;
+                const int64_t r = first + l;
+                xv[p] = Frag<T>(0);
+                if (l < kRows && r < stop && xc < x_chunks) xv[p] = load_within(static_cast<const T*>(a.x) + r * a.x_stride, xc * V, a.in);
+            }
+    };
+    const int64_t last = min(a.groups.rows, (blockIdx.x + int64_t{1}) * a.chunk);
+    for (int64_t first = blockIdx.x * a.chunk; first < last;) {
+        const int group = group_of(a.groups, first);
+        if (group >= a.groups.groups) {
+            if (a.to.out)
+                for (int64_t r = first + threadIdx.x / 8; r < last; r += kThreads / 8)
+                    for (int64_t c = threadIdx.x % 8 * 4; c < a.in; c += 32) clear4<T>(a.to, r, c);
+            return;
+        }
+        const int64_t stop = max(first + 1, min(last, a.groups.end(group)));
+        load(first, stop);
+        __syncthreads();  // the group's before have been worked on
+        if (a.to.out) {
+            const T* const w = static_cast<const T*>(a.weight) + group * a.in * a.out;
+            for (int i = threadIdx.x; i < kt * nt * kSteps * 64; i += kThreads) {
+                const int k = i / 64 / (nt * kSteps) * 32 + i % 32, n = (2 * (i / 64 % (nt * kSteps)) + i % 64 / 32) * V;
+                Frag<T> f(0);
+                if (k < a.in)
+#pragma unroll
+                    for (int e = 0; e < V; e++)
+                        if (n + e < a.out) f[e] = w[(n + e) * a.in + k];
+                weights[i] = f;
+            }
+        }
+        Sums sums[Tiles];
+        Floats<V> db(0.0f);
+#pragma unroll
+        for (int t = 0; t < Tiles; t++) sums[t] = Sums(0.0f);
+        for (int64_t block = first; block < stop; block += kRows) {
+#pragma unroll
+            for (int p = 0; p < Passes; p++) {
+                const int l = zl + p * z_step;
+                if (l < kRows && zc < z_chunks) {
+                    Floats<V> d = floats<T, V>(dy[p]);
+                    if (a.act) {
+                        const Floats<V> z = floats<T, V>(pre[p]);
+#pragma unroll
+                        for (int e = 0; e < V; e++) d[e] = through<T>(d[e], z[e], a.act);
+                    }
+                    db += d;
+                    *reinterpret_cast<Frag<T>*>(dz + l * z_bytes + zc * 16) = raw<T, V>(d);
+                }
+            }
+            if (a.x)
+#pragma unroll
+                for (int p = 0; p < Passes; p++) {
+                    const int l = xl + p * x_step;
+                    if (l < kRows && xc < x_chunks) *reinterpret_cast<Frag<T>*>(xs + l * x_bytes + xc * 16) = xv[p];
+                }
+            __syncthreads();
+            if (block + kRows < stop) load(block + kRows, stop);
+            if (a.to.out)
+                for (int i = wave; i < kRows / 32 * kt; i += Waves) {
+                    const int strip = i / kt * 32, t = i % kt;
+                    const int64_t r = block + strip + lane % 32;
+                    if (block + strip >= stop) break;
+                    Sums c(0.0f);
+                    for (int s = 0; s < nt * kSteps; s++)
+                        mma(c, weights[(t * nt * kSteps + s) * 64 + lane],
+                            *reinterpret_cast<const Frag<T>*>(dz + (strip + lane % 32) * z_bytes + (2 * s + lane / 32) * 16));
+                    finish32<T>(a.to, r, r < stop, t * 32, c);
+                }
+            if (a.x)
+#pragma unroll
+                for (int i = 0; i < Tiles; i++) {
+                    const int t = wave + i * Waves;
+                    if (t < nt * kt)
+#pragma unroll
+                        for (int s = 0; s < 8; s++)
+                            mma(sums[i], across_fragment<T>(xs, x_bytes, t % kt * 32, s), across_fragment<T>(dz, z_bytes, t / kt * 32, s));
+                }
+            __syncthreads();
+        }
+        if (a.partial) {
+            float* const slab = a.partial + (int64_t{blockIdx.x} + group) * a.size;
+#pragma unroll
+            for (int i = 0; i < Tiles; i++) {
+                const int t = wave + i * Waves;
+                const int64_t n = t / kt * 32 + lane % 32;
+                if (t < nt * kt && n < a.out)
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        const int64_t k = t % kt * 32 + 8 * q + lane / 32 * 4;
+                        const Floats<4> v = {sums[i][4 * q], sums[i][4 * q + 1], sums[i][4 * q + 2], sums[i][4 * q + 3]};
+                        store_some<float, 4>(slab + n * a.in + k, v, static_cast<int>(max(int64_t{0}, min(a.in - k, int64_t{4}))));
+                    }
+            }
+            Floats<V>* const parts = reinterpret_cast<Floats<V>*>(lds);
+            parts[threadIdx.x] = db;
+            __syncthreads();
+            if (static_cast<int>(threadIdx.x) < z_lanes && zc * V < a.out) {
+                for (int l = 1; l < z_step; l++) db += parts[l * z_lanes + zc];
+                store_some<float, V>(slab + a.in * a.out + zc * V, db, static_cast<int>(min(a.out - zc * V, int64_t{V})));
+            }
+        }
+        first = stop;
     }
 }
 
@@ -420,40 +807,113 @@ void check_grid(int64_t blocks, int64_t threads) {
 
 template <class T, bool RowAcross, bool ColAcross>
 void launch_tiles(const TileArgs& a, int side, int64_t slabs, hipStream_t s) {
-    const int64_t down = RowAcross ? up(a.rows, side) : a.slots, tiles = up(down * up(a.cols, side), 8) * 8;
+    const int64_t down = RowAcross ? up(a.rows, side) : a.slots, tiles = up(down * up(a.to.cols, side), 8) * 8;
     check_grid(tiles * slabs, 256);
     const dim3 grid(static_cast<uint32_t>(tiles), static_cast<uint32_t>(slabs));
     if (side == 128) k_tile<T, 128, 128, 64, 64, RowAcross, ColAcross><<<grid, 256, 0, s>>>(a);
     else k_tile<T, 64, 64, 32, 32, RowAcross, ColAcross><<<grid, 256, 0, s>>>(a);
 }
 
-template <class T, bool OverRows>
-void join_tiles(const TileArgs& a, int groups, hipStream_t s) {
-    const int64_t blocks = std::min<int64_t>(up(a.rows * up(a.cols, 4), 256), 4096);
-    k_tile_join<T, OverRows><<<dim3(static_cast<uint32_t>(blocks), static_cast<uint32_t>(groups)), 256, 0, s>>>(a);
+// `slabs`: of a group, on average
+template <class T>
+void join_weights(JoinArgs a, int64_t slabs, hipStream_t s) {
+    a.turns = 1;
+    while (a.turns < 64 && a.turns * 4 <= slabs) a.turns *= 2;
+    const int64_t blocks = std::min<int64_t>(up(up(a.wanted, 4), 256 / a.turns), 65536);
+    k_weights_join<T><<<dim3(static_cast<uint32_t>(blocks), static_cast<uint32_t>(a.groups.groups)), 256, 0, s>>>(a);
+}
+
+// The steps of 32 bytes of a row that k_narrow_fwd is built for, or 0.
+int narrow_steps(int64_t in, int elem) {
+    for (const int k : {1, 2, 3, 4, 6, 8, 12, 16})
+        if (in * elem <= k * 32) return k;
+    return 0;
+}
+// A layer whose weight a workgroup holds: its LDS and workgroups, or none.
+struct Narrow {
+    int steps, threads, lds;
+    int64_t blocks, chunk;
+};
+Narrow plan_narrow(int64_t rows, int64_t in, int64_t out, int elem) {
+    Narrow p{};
+    const int steps = narrow_steps(in, elem);
+    const int64_t tiles = up(out, 32), kib = tiles * steps;
+    if (!steps || kib > 128 || (rows < 4096 && kib > 16)) return p;
+    p.steps = steps;
+    p.lds = static_cast<int>(kib * 1024 + tiles * 128);
+    p.threads = kib > 32 ? 512 : 256;
+    const int64_t each = std::max(1, std::min(p.threads == 512 ? 2 : 4, 160 * 1024 / p.lds));
+    p.blocks = std::max<int64_t>(1, std::min<int64_t>(256 * each, up(rows, p.threads / 2)));
+    p.chunk = up(up(rows, p.blocks), 32) * 32;
+    p.blocks = up(rows, p.chunk);
+    return p;
+}
+// A backward whose blocks of rows a workgroup holds.
+struct NarrowBwd {
+    int waves, lds;
+    int64_t blocks, chunk, size, bytes;
+};
+template <class T>
+NarrowBwd plan_narrow_bwd(int64_t rows, int64_t in, int64_t out, int groups) {
+    NarrowBwd p{};
+    const int64_t nt = up(out, 32), kt = up(in, 32);
+    if (nt * kt > 16 || nt > 8 || kt > 8) return p;
+    p.lds = kBlockRows<T> * (line_bytes<T>(static_cast<int>(nt)) + line_bytes<T>(static_cast<int>(kt))) + static_cast<int>(nt * kt * sizeof(T)) * 1024;
+    if (p.lds > 160 * 1024) return p;
+    p.waves = nt <= 2 && kt <= 2 ? 4 : 8;
+    const int64_t each = std::max(1, std::min(p.waves == 4 ? 4 : 2, 160 * 1024 / p.lds));
+    p.blocks = std::max<int64_t>(1, std::min<int64_t>(256 * each, up(rows, kBlockRows<T>)));
+    p.chunk = std::max<int64_t>(up(up(rows, p.blocks), 32) * 32, 32);
+    p.blocks = std::max<int64_t>(up(rows, p.chunk), 1);
+    p.size = in * out + out;
+    p.bytes = (p.blocks + groups) * p.size * 4;
+    return p;
+}
+
+template <class T>
+void launch_narrow(const NarrowArgs& a, const Narrow& p, hipStream_t s) {
+    const auto go = [&](auto kernel) { kernel<<<static_cast<uint32_t>(p.blocks), p.threads, p.lds, s>>>(a); };
+    switch (p.steps) {
+        case 1: return go(k_narrow_fwd<T, 1>);
+        case 2: return go(k_narrow_fwd<T, 2>);
+        case 3: return go(k_narrow_fwd<T, 3>);
+        case 4: return go(k_narrow_fwd<T, 4>);
+        case 6: return go(k_narrow_fwd<T, 6>);
+        case 8: return go(k_narrow_fwd<T, 8>);
+        case 12: return go(k_narrow_fwd<T, 12>);
+        default: return go(k_narrow_fwd<T, 16>);
+    }
 }
 
 // out = row col^T over the groups' rows (see TileArgs), with what follows.
 template <class T, bool ColAcross>
 void over_depth(TileArgs a, bool ragged, float* work, hipStream_t s) {
-    const Plan p = plan_rows(a.rows, a.cols, a.depth, a.groups.groups, ragged, sizeof(T));
+    const Plan p = plan_rows(a.rows, a.to.cols, a.depth, a.groups.groups, ragged, sizeof(T));
     a.shift = log2_up(p.side);
     a.slots = slots_of(a.rows, a.groups.groups, a.shift, ragged);
     a.split = p.split;
     a.splits = p.splits;
     a.partial = p.splits > 1 ? work : nullptr;
     launch_tiles<T, false, ColAcross>(a, p.side, p.splits, s);
-    if (a.partial) join_tiles<T, false>(a, 1, s);
+    if (a.partial) {
+        const int64_t blocks = std::min<int64_t>(up(a.rows * up(a.to.cols, 4), 256), 4096);
+        k_split_join<T><<<static_cast<uint32_t>(blocks), 256, 0, s>>>(a);
+    }
 }
 
 template <class T>
 void forward(const LinearFwdArgs& f, hipStream_t s) {
+    const Finish to{f.y, f.y_stride, f.out, f.residual, f.residual_stride, f.pre, f.pre_stride, f.act, f.clear};
+    if (const Narrow p = plan_narrow(f.rows, f.in, f.out, sizeof(T)); p.blocks) {
+        launch_narrow<T>({f.x, f.weight, f.bias, f.x_stride, to, f.in, f.out, p.chunk, {f.ends, f.groups, f.rows}}, p, s);
+        return;
+    }
     TileArgs a{};
     a.row = f.x; a.row_stride = f.x_stride; a.col = f.weight; a.col_stride = f.in; a.col_group = f.in * f.out;
-    a.out = f.y; a.out_stride = f.y_stride; a.rows = f.rows; a.cols = f.out; a.depth = f.in;
+    a.rows = f.rows; a.depth = f.in;
     a.groups = {f.ends, f.groups, f.rows};
-    a.bias = f.bias; a.bias_group = f.out; a.residual = f.residual; a.residual_stride = f.residual_stride;
-    a.pre = f.pre; a.pre_stride = f.pre_stride; a.act = f.act; a.clear = f.clear;
+    a.bias = f.bias; a.bias_group = f.out;
+    a.to = to;
     over_depth<T, false>(a, f.ends != nullptr, static_cast<float*>(f.workspace), s);
 }
 
@@ -463,6 +923,26 @@ void backward(const LinearBwdArgs& f, hipStream_t s) {
     const Slope slope = plan_slope(f.rows, f.out, f.groups, ragged, sizeof(T));
     const Groups groups{f.ends, f.groups, f.rows};
     char* work = static_cast<char*>(f.workspace);
+    if (const NarrowBwd p = plan_narrow_bwd<T>(f.rows, f.in, f.out, f.groups); p.blocks) {
+        NarrowBwdArgs a{};
+        a.dy = f.dy; a.pre = f.pre; a.x = f.dweight ? f.x : nullptr; a.weight = f.weight;
+        a.dy_stride = f.dy_stride; a.pre_stride = f.pre_stride; a.x_stride = f.x_stride;
+        a.to.out = f.dx; a.to.out_stride = f.dx_stride; a.to.cols = f.in; a.to.clear = f.clear;
+        a.in = f.in; a.out = f.out; a.chunk = p.chunk; a.size = p.size; a.groups = groups; a.act = f.act;
+        const bool sums = f.dweight || f.dbias;
+        a.partial = sums ? reinterpret_cast<float*>(work) : nullptr;
+        if (f.rows) {
+            if (p.waves == 4) k_narrow_bwd<T, 4, 1, 4><<<static_cast<uint32_t>(p.blocks), 256, p.lds, s>>>(a);
+            else k_narrow_bwd<T, 8, 2, 8><<<static_cast<uint32_t>(p.blocks), 512, p.lds, s>>>(a);
+        }
+        if (sums) {
+            JoinArgs j{};
+            j.partial = a.partial; j.dweight = f.dweight; j.dbias = f.dbias; j.weights = f.in * f.out; j.size = p.size; j.wanted = f.dbias ? p.size : j.weights;
+            j.groups = groups; j.step = p.chunk;
+            join_weights<T>(j, p.blocks / f.groups + 1, s);
+        }
+        return;
+    }
     const void* dz = f.dy;
     int64_t dz_stride = f.dy_stride;
     const bool products = f.dx || f.dweight;
@@ -486,19 +966,24 @@ void backward(const LinearBwdArgs& f, hipStream_t s) {
     if (f.dx && f.rows) {
         TileArgs a{};
         a.row = dz; a.row_stride = dz_stride; a.col = f.weight; a.col_stride = f.in; a.col_group = f.in * f.out;
-        a.out = f.dx; a.out_stride = f.dx_stride; a.rows = f.rows; a.cols = f.in; a.depth = f.out;
-        a.groups = groups; a.clear = f.clear;
+        a.to.out = f.dx; a.to.out_stride = f.dx_stride; a.to.cols = f.in; a.rows = f.rows; a.depth = f.out;
+        a.groups = groups; a.to.clear = f.clear;
         over_depth<T, true>(a, ragged, reinterpret_cast<float*>(work), s);
     }
     if (f.dweight) {
         const Over p = plan_over(f.rows, f.out, f.in, f.groups, ragged);
         TileArgs a{};
         a.row = dz; a.row_stride = dz_stride; a.col = f.x; a.col_stride = f.x_stride;
-        a.out = f.dweight; a.out_stride = f.in; a.out_group = f.in * f.out; a.rows = f.out; a.cols = f.in; a.depth = f.rows;
+        a.to.out = f.dweight; a.to.out_stride = f.in; a.to.cols = f.in; a.out_group = f.in * f.out; a.rows = f.out; a.depth = f.rows;
         a.groups = groups; a.shift = p.shift; a.slots = p.slots;
         a.partial = p.bytes ? reinterpret_cast<float*>(work) : nullptr;
         launch_tiles<T, true, true>(a, p.side, p.slots, s);
-        if (a.partial) join_tiles<T, true>(a, f.groups, s);
+        if (a.partial) {
+            JoinArgs j{};
+            j.partial = a.partial; j.dweight = f.dweight; j.weights = j.wanted = j.size = f.in * f.out;
+            j.groups = groups; j.step = int64_t{1} << p.shift; j.from_begin = true;
+            join_weights<T>(j, p.slots / f.groups, s);
+        }
     }
 }
 
@@ -512,10 +997,13 @@ void with_type(ElemType t, F&& f) {
 }  // namespace
 
 int64_t linear_fwd_workspace(int64_t rows, int64_t in, int64_t out, int groups, bool ragged, ElemType type) {
-    return plan_rows(rows, out, in, groups, ragged, type == kF32 ? 4 : 2).bytes;
+    const int elem = type == kF32 ? 4 : 2;
+    return plan_narrow(rows, in, out, elem).blocks ? 0 : plan_rows(rows, out, in, groups, ragged, elem).bytes;
 }
 int64_t linear_bwd_workspace(int64_t rows, int64_t in, int64_t out, int groups, bool ragged, ElemType type) {
     const int elem = type == kF32 ? 4 : 2;
+    const NarrowBwd narrow = elem == 4 ? plan_narrow_bwd<float>(rows, in, out, groups) : plan_narrow_bwd<__bf16>(rows, in, out, groups);
+    if (narrow.blocks) return narrow.bytes;
     const Slope slope = plan_slope(rows, out, groups, ragged, elem);
     return aligned(slope.dz_bytes) + aligned(slope.bytes) +
            std::max(plan_rows(rows, in, out, groups, ragged, elem).bytes, plan_over(rows, out, in, groups, ragged).bytes);
