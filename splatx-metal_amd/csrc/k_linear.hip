@@ -145,9 +145,7 @@ __device__ inline void finish4(const Finish& a, int64_t r, int64_t c, Floats<4> 
     const int n = static_cast<int>(min(a.cols - c, int64_t{4}));
     if (n <= 0) return;
     if (a.pre) store_some<T, 4>(static_cast<T*>(a.pre) + r * a.pre_stride + c, v, n);
-    if (a.act)
-#pragma unroll
-        for (int e = 0; e < 4; e++) v[e] = activated<T>(v[e], a.act);
+    activate<T, 4>(v, a.act);
     if (a.residual) v += load_some<T, 4>(static_cast<const T*>(a.residual) + r * a.residual_stride + c, n);
     store_some<T, 4>(static_cast<T*>(a.out) + r * a.out_stride + c, v, n);
 }
@@ -160,52 +158,106 @@ __device__ inline void clear4(const Finish& a, int64_t r, int64_t c) {
     if (a.pre) store_some<T, 4>(static_cast<T*>(a.pre) + r * a.pre_stride + c, Floats<4>(0.0f), n);
 }
 
-// 16-bit elements of 16 columns between the sums' layout (a lane has columns 0..3 and 8..11 of its row, its partner in the
-// wave's other half 4..7 and 12..15) and memory's (0..7 and 8..15, 16 bytes a lane): the partners swap, both ways.
+// A wave's outputs go through LDS of its own as floats, so that a store has whole lines of eight rows: from the sums' layout (a
+// lane has four columns of its row in each place) to memory's, 32 rows of 128 bytes of the type, of which a lane takes 16 at a
+// time through what follows the sums. (Stores of 16 bytes a row from the registers, the rows' lines in four parts: a layer of
+// 64 outputs took twice as long.)
 template <class T>
-__device__ inline Frag<T> swapped(Frag<T> v) {
-    using Words = uint32_t __attribute__((ext_vector_type(4)));
-    const Words w = __builtin_bit_cast(Words, v);
-    const auto a = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false), b = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
-    return __builtin_bit_cast(Frag<T>, Words{a[0], b[0], a[1], b[1]});
+constexpr int kUnitTiles = 4 / static_cast<int>(sizeof(T));  // tiles of 32 columns side by side
+template <class T>
+constexpr int kUnitLine = kUnitTiles<T> * 128 + 16;  // (the lines of eight rows in different banks)
+template <class T>
+constexpr int kUnitBytes = 32 * kUnitLine<T>;
+
+// What lanes of the wave have written to LDS is there for the others.
+__device__ inline void wave_sees() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// A wave's 32 x 32 sums, bias included: row r of the lane (if it is `valid`), columns from c on. Every lane takes part.
 template <class T>
-__device__ inline void finish32(const Finish& a, int64_t r, bool valid, int64_t c, const Sums& s) {
-    constexpr int V = kPer<T>;
-    const int half = threadIdx.x % 64 / 32;
-    T* const out = static_cast<T*>(a.out) + r * a.out_stride;
+__device__ inline void store_chunk(T* p, Floats<kPer<T>> f, int n) {
+    const Frag<T> v = raw<T, kPer<T>>(f);
+    if (n == kPer<T>) {
+        store_raw<kPer<T>>(p, v);
+        return;
+    }
 #pragma unroll
-    for (int p = 0; p < 32 / (2 * V); p++) {
+    for (int e = 0; e < kPer<T> - 1; e++)
+        if (e < n) p[e] = v[e];
+}
+
+// 32 rows from r on (those before `stop`) and the columns [c, c + 128 bytes), the sums' bias included. Every lane takes part.
+template <class T>
+__device__ inline void finish_unit(const Finish& a, int64_t r, int64_t stop, int64_t c, const Sums (&sums)[kUnitTiles<T>], char* lds) {
+    constexpr int V = kPer<T>;
+    const int lane = threadIdx.x % 64;
+    wave_sees();  // (what was there has been read)
+#pragma unroll
+    for (int u = 0; u < kUnitTiles<T>; u++)
+#pragma unroll
+        for (int q = 0; q < 4; q++)
+            *reinterpret_cast<Floats<4>*>(lds + lane % 32 * kUnitLine<T> + lane / 32 * 16 + u * 128 + q * 32) =
+                Floats<4>{sums[u][4 * q], sums[u][4 * q + 1], sums[u][4 * q + 2], sums[u][4 * q + 3]};
+    wave_sees();
+    const int64_t column = c + lane % 8 * V;
+    const int n = static_cast<int>(max(int64_t{0}, min(a.cols - column, int64_t{V})));
+    const int rows = static_cast<int>(min(stop - r, int64_t{32}));
+    const char* from = lds + lane / 8 * kUnitLine<T> + lane % 8 * (V * 4);
+    r += lane / 8;
+    Frag<T> residual(0);
+    const auto load_residual = [&](int row, int64_t at) {
+        if (a.residual && row < rows) residual = load_within(static_cast<const T*>(a.residual) + at * a.residual_stride, column, a.cols);
+    };
+    load_residual(lane / 8, r);
+#pragma unroll 1
+    for (int row = lane / 8; row < rows; row += 8, r += 8, from += 8 * kUnitLine<T>) {
         Floats<V> v;
 #pragma unroll
-        for (int e = 0; e < V; e++) v[e] = s[p * V + e];
-        const int64_t column = c + p * 2 * V + half * V;
-        const int n = valid ? static_cast<int>(max(int64_t{0}, min(a.cols - column, int64_t{V}))) : 0;
-        const auto in_memory = [](Floats<V> f) {
-            Frag<T> t = raw<T, V>(f);
-            if constexpr (V == 8) t = swapped<T>(t);
-            return t;
-        };
-        const auto store = [&](T* row, Frag<T> t) {
-            if (n == V) store_raw<V>(row + column, t);
-            else
-#pragma unroll
-                for (int e = 0; e < V - 1; e++)
-                    if (e < n) row[column + e] = t[e];
-        };
-        Frag<T> residual(0);
-        if (a.residual && n) residual = load_within(static_cast<const T*>(a.residual) + r * a.residual_stride, column, a.cols);
-        if (a.pre) store(static_cast<T*>(a.pre) + r * a.pre_stride, in_memory(v));
-        if (a.act)
-#pragma unroll
-            for (int e = 0; e < V; e++) v[e] = activated<T>(v[e], a.act);
-        if (a.residual) {
-            if constexpr (V == 8) residual = swapped<T>(residual);
-            v += floats<T, V>(residual);
+        for (int e = 0; e < V; e += 4) {
+            const Floats<4> f = *reinterpret_cast<const Floats<4>*>(from + e * 4);
+            v[e] = f[0]; v[e + 1] = f[1]; v[e + 2] = f[2]; v[e + 3] = f[3];
         }
-        store(out, in_memory(v));
+        if (a.pre) store_chunk(static_cast<T*>(a.pre) + r * a.pre_stride + column, v, n);
+        activate<T, V>(v, a.act);
+        if (a.residual) {
+            v += floats<T, V>(residual);
+            load_residual(row + 8, r + 8);
+        }
+        store_chunk(static_cast<T*>(a.out) + r * a.out_stride + column, v, n);
+    }
+}
+
+// The same of sums that are the outputs, through half the LDS.
+template <class T>
+constexpr int kBareLine = 128 + 16;
+template <class T>
+constexpr int kBareBytes = 32 * kBareLine<T>;
+template <class T>
+__device__ inline void store_unit(const Finish& a, int64_t r, int64_t stop, int64_t c, const Sums (&sums)[kUnitTiles<T>], char* lds) {
+    constexpr int V = kPer<T>;
+    const int lane = threadIdx.x % 64;
+    wave_sees();
+#pragma unroll
+    for (int u = 0; u < kUnitTiles<T>; u++)
+#pragma unroll
+        for (int q = 0; q < 4; q++)
+            *reinterpret_cast<Vec<T, 4>*>(lds + lane % 32 * kBareLine<T> + (u * 32 + 8 * q + lane / 32 * 4) * static_cast<int>(sizeof(T))) =
+                raw<T, 4>(Floats<4>{sums[u][4 * q], sums[u][4 * q + 1], sums[u][4 * q + 2], sums[u][4 * q + 3]});
+    wave_sees();
+    const int64_t column = c + lane % 8 * V;
+    const int n = static_cast<int>(max(int64_t{0}, min(a.cols - column, int64_t{V})));
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const Frag<T> v = *reinterpret_cast<const Frag<T>*>(lds + (lane / 8 + i * 8) * kBareLine<T> + lane % 8 * 16);
+        T* const p = static_cast<T*>(a.out) + (r + lane / 8 + i * 8) * a.out_stride + column;
+        if (r + lane / 8 + i * 8 >= stop) continue;
+        if (n == V) store_raw<V>(p, v);
+        else
+#pragma unroll
+            for (int e = 0; e < V - 1; e++)
+                if (e < n) p[e] = v[e];
     }
 }
 
@@ -289,35 +341,37 @@ __global__ void __launch_bounds__(BR / WR * (BC / WC) * 64) k_tile(TileArgs a) {
         }
         __syncthreads();
     }
+    Finish to = a.to;
+    to.out = static_cast<T*>(to.out) + part.group * a.out_group;
 #pragma unroll
     for (int i = 0; i < I; i++) {
-        const int64_t r = r0 + wr + i * 32 + lane % 32;
+        const int64_t r = r0 + wr + i * 32;
+        if (r >= r1) break;
 #pragma unroll
-        for (int j = 0; j < J; j++) {
+        for (int j = 0; j < J; j += kUnitTiles<T>) {
             const int64_t c = c0 + wc + j * 32;
             if (c >= a.to.cols) break;
-            if (a.partial) {
+            Sums unit[kUnitTiles<T>];
+#pragma unroll
+            for (int u = 0; u < kUnitTiles<T>; u++) {
+                unit[u] = sums[i][j + u];
 #pragma unroll
                 for (int q = 0; q < 4; q++) {
-                    const int64_t at = c + 8 * q + lane / 32 * 4;
-                    const int n = r < r1 ? static_cast<int>(max(int64_t{0}, min(a.to.cols - at, int64_t{4}))) : 0;
-                    const Floats<4> v = {sums[i][j][4 * q], sums[i][j][4 * q + 1], sums[i][j][4 * q + 2], sums[i][j][4 * q + 3]};
-                    store_some<float, 4>(a.partial + (int64_t{blockIdx.y} * a.rows + r) * a.to.cols + at, v, n);
+                    const int64_t at = c + u * 32 + 8 * q + lane / 32 * 4;
+                    const int n = static_cast<int>(max(int64_t{0}, min(a.to.cols - at, int64_t{4})));
+                    if (a.partial) {
+                        const Floats<4> v = {unit[u][4 * q], unit[u][4 * q + 1], unit[u][4 * q + 2], unit[u][4 * q + 3]};
+                        store_some<float, 4>(a.partial + (int64_t{blockIdx.y} * a.rows + r + lane % 32) * a.to.cols + at, v, r + lane % 32 < r1 ? n : 0);
+                    } else if (a.bias) {
+                        const Floats<4> v = load_some<T, 4>(static_cast<const T*>(a.bias) + part.group * a.bias_group + at, n);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) unit[u][4 * q + e] += v[e];
+                    }
                 }
-                continue;
             }
-            if (a.bias)
-#pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    const int64_t at = c + 8 * q + lane / 32 * 4;
-                    const Floats<4> v = load_some<T, 4>(static_cast<const T*>(a.bias) + part.group * a.bias_group + at,
-                                                        static_cast<int>(max(int64_t{0}, min(a.to.cols - at, int64_t{4}))));
-#pragma unroll
-                    for (int e = 0; e < 4; e++) sums[i][j][4 * q + e] += v[e];
-                }
-            Finish to = a.to;
-            to.out = static_cast<T*>(to.out) + part.group * a.out_group;
-            finish32<T>(to, r, r < r1, c, sums[i][j]);
+            if (a.partial) continue;
+            if constexpr (ColAcross) store_unit<T>(to, r, r1, c, unit, lds + wave * kUnitBytes<T>);
+            else finish_unit<T>(to, r, r1, c, unit, lds + wave * kUnitBytes<T>);
         }
     }
 }
@@ -449,9 +503,11 @@ template <class T, int K>
 __global__ void __launch_bounds__(512) k_narrow_fwd(NarrowArgs a) {
     constexpr int V = kPer<T>;
     extern __shared__ __attribute__((aligned(128))) char lds[];
-    const int tiles = static_cast<int>((a.out + 31) / 32), lane = threadIdx.x % 64, wave = threadIdx.x / 64, rows_at_once = blockDim.x / 2;
+    const int tiles = static_cast<int>((a.out + 32 * kUnitTiles<T> - 1) / (32 * kUnitTiles<T>)) * kUnitTiles<T>;
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, rows_at_once = blockDim.x / 2;
     Frag<T>* const weights = reinterpret_cast<Frag<T>*>(lds);
     float* const bias = reinterpret_cast<float*>(lds + tiles * K * 1024);
+    char* const mine = lds + tiles * (K * 1024 + 128) + wave * kUnitBytes<T>;
     const RowLoad<T, K> load(a.in);
     const T* const x = static_cast<const T*>(a.x);
     const int64_t last = min(a.groups.rows, (blockIdx.x + int64_t{1}) * a.chunk);
@@ -480,18 +536,20 @@ __global__ void __launch_bounds__(512) k_narrow_fwd(NarrowArgs a) {
 #pragma unroll
             for (int k = 0; k < K; k++) now[k] = next[k];
             if (base + rows_at_once < stop) load(next, x + min(base + rows_at_once + lane % 32, stop - 1) * a.x_stride);
-            const int64_t r = base + lane % 32;
-            for (int t = 0; t < tiles; t++) {
-                Sums sums;
+            for (int t = 0; t < tiles; t += kUnitTiles<T>) {
+                Sums unit[kUnitTiles<T>];
 #pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    const Floats<4> b = *reinterpret_cast<const Floats<4>*>(bias + t * 32 + 8 * q + lane / 32 * 4);
+                for (int u = 0; u < kUnitTiles<T>; u++) {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) sums[4 * q + e] = b[e];
+                    for (int q = 0; q < 4; q++) {
+                        const Floats<4> b = *reinterpret_cast<const Floats<4>*>(bias + (t + u) * 32 + 8 * q + lane / 32 * 4);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) unit[u][4 * q + e] = b[e];
+                    }
+#pragma unroll
+                    for (int k = 0; k < K; k++) mma(unit[u], weights[((t + u) * K + k) * 64 + lane], now[k]);
                 }
-#pragma unroll
-                for (int k = 0; k < K; k++) mma(sums, weights[(t * K + k) * 64 + lane], now[k]);
-                finish32<T>(a.to, r, r < stop, t * 32, sums);
+                finish_unit<T>(a.to, base, stop, t * 32, unit, mine);
             }
         }
         first = stop;
@@ -511,18 +569,19 @@ struct NarrowBwdArgs {
 // Bytes between the lines of a block in LDS: `tiles` times 32 elements, and what puts four lines (floats: the lanes' lines)
 // into different banks.
 template <class T>
-__host__ __device__ constexpr int line_bytes(int tiles) { return tiles * 32 * static_cast<int>(sizeof(T)) + (sizeof(T) == 2 ? 32 : 16); }
+constexpr int line_bytes(int tiles) { return tiles * 32 * static_cast<int>(sizeof(T)) + (sizeof(T) == 2 ? 32 : 16); }
 template <class T>
 constexpr int kBlockRows = 256 / static_cast<int>(sizeof(T));
 
-// Fragments of the lane's column: the block's lines along it, step s of eight.
-template <class T>
-__device__ inline Frag<T> across_fragment(const char* block, int bytes, int column, int s) {
+// The lane's fragment of a column of a block: the lines along it, step s of eight.
+template <class T, int Tiles>
+__device__ inline Frag<T> across_fragment(const char* block, int column, int s) {
+    constexpr int kLine = line_bytes<T>(Tiles);
     const int lane = threadIdx.x % 64, half = lane / 32;
     if constexpr (sizeof(T) == 4) {
         Frag<T> f;
 #pragma unroll
-        for (int i = 0; i < 4; i++) f[i] = *reinterpret_cast<const float*>(block + (s * 8 + half * 4 + i) * bytes + (column + lane % 32) * 4);
+        for (int i = 0; i < 4; i++) f[i] = *reinterpret_cast<const float*>(block + (s * 8 + half * 4 + i) * kLine + (column + lane % 32) * 4);
         return f;
     } else {
         using Four = short __attribute__((ext_vector_type(4)));
@@ -532,49 +591,55 @@ __device__ inline Frag<T> across_fragment(const char* block, int bytes, int colu
 #pragma unroll
         for (int j = 0; j < 2; j++)
             part[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (Lds)(block + (s * 16 + half * 8 + j * 4 + group / 4) * bytes + (column + lane % 32 / 16 * 16 + group % 4 * 4) * 2));
+                (Lds)(block + (s * 16 + half * 8 + j * 4 + group / 4) * kLine + (column + lane % 32 / 16 * 16 + group % 4 * 4) * 2));
         return __builtin_bit_cast(Frag<T>, __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7));
     }
 }
 
+// A thread's fragments of a block's rows, Tiles times 32 columns of them, on their way from memory.
+template <class T, int Tiles, int Threads>
+struct BlockPart {
+    static constexpr int V = kPer<T>, kLanes = Tiles * 32 / V, kLines = Threads / kLanes, N = kBlockRows<T> / kLines;
+    static_assert(Threads % kLanes == 0 && kBlockRows<T> % kLines == 0);
+    Frag<T> v[N];
+    static __device__ int chunk() { return threadIdx.x % kLanes; }
+    static __device__ int line(int i) { return threadIdx.x / kLanes + i * kLines; }
+    // Rows [first, stop), at most a block of them. (Of rows and chunks there are not others are read.)
+    __device__ void load(const void* from, int64_t stride, int64_t width, int64_t first, int64_t stop) {
+        const T* const base = static_cast<const T*>(from) + first * stride;
+        const int most = static_cast<int>(min(stop - 1 - first, int64_t{kBlockRows<T>}));
+        if (width % V == 0) {
+            const T* const at = base + min(int64_t{chunk()} * V, width - V);
+#pragma unroll
+            for (int i = 0; i < N; i++) v[i] = load_raw<V>(at + min(line(i), most) * stride);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; i++) v[i] = load_within(base + min(line(i), most) * stride, chunk() * V, width);
+        }
+    }
+};
+
 // All three gradients in one pass: a block of rows of dz and x lies in LDS, its products with the weight are dx's rows, and the
-// products of its columns with one another stay in registers over the rows of a group: `Tiles` tiles of 32 x 32 of dweight a
-// wave. The next block is on its way meanwhile, `Passes` fragments a thread of each.
-template <class T, int Waves, int Tiles, int Passes>
+// products of its columns with one another stay in registers over the rows of a group, tiles of 32 x 32 of dweight. The next
+// block is on its way meanwhile. Up to ZT tiles of 32 outputs and XT of 32 inputs.
+template <class T, int Waves, int ZT, int XT>
 __global__ void __launch_bounds__(Waves * 64) k_narrow_bwd(NarrowBwdArgs a) {
-    constexpr int V = kPer<T>, kRows = kBlockRows<T>, kThreads = Waves * 64, kSteps = static_cast<int>(sizeof(T));
+    constexpr int V = kPer<T>, kRows = kBlockRows<T>, kThreads = Waves * 64;
+    constexpr int kSteps = ZT * static_cast<int>(sizeof(T)), kTiles = (ZT * XT + Waves - 1) / Waves, kZ = line_bytes<T>(ZT), kX = line_bytes<T>(XT);
+    static_assert(XT % kUnitTiles<T> == 0);
     extern __shared__ __attribute__((aligned(128))) char lds[];
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
     const int nt = static_cast<int>((a.out + 31) / 32), kt = static_cast<int>((a.in + 31) / 32);
-    const int z_bytes = line_bytes<T>(nt), x_bytes = line_bytes<T>(kt);
-    char *const dz = lds, *const xs = lds + kRows * z_bytes;
-    Frag<T>* const weights = reinterpret_cast<Frag<T>*>(xs + kRows * x_bytes);
-    // where a thread's fragments lie in a block: as many threads as a power of two holds a row's go along it
-    const auto lanes_of = [](int chunks) { return chunks <= 1 ? 1 : 1 << (32 - __builtin_clz(chunks - 1)); };
-    const int z_chunks = nt * 32 / V, x_chunks = kt * 32 / V, z_lanes = lanes_of(z_chunks), x_lanes = lanes_of(x_chunks);
-    const int zc = threadIdx.x % z_lanes, zl = threadIdx.x / z_lanes, xc = threadIdx.x % x_lanes, xl = threadIdx.x / x_lanes;
-    const int z_step = kThreads / z_lanes, x_step = kThreads / x_lanes;
-    Frag<T> dy[Passes], pre[Passes], xv[Passes];
+    char *const dz = lds, *const xs = dz + kRows * kZ, *const mine = xs + kRows * kX + wave * kBareBytes<T>;
+    Frag<T>* const weights = reinterpret_cast<Frag<T>*>(xs + kRows * kX + Waves * kBareBytes<T>);
+    BlockPart<T, ZT, kThreads> dy, pre;
+    BlockPart<T, XT, kThreads> x;
     const auto load = [&](int64_t first, int64_t stop) {
-#pragma unroll
-        for (int p = 0; p < Passes; p++) {
-            const int l = zl + p * z_step;
-            const int64_t r = first + l;
-            dy[p] = pre[p] = Frag<T>(0);
-            if (l < kRows && r < stop && zc < z_chunks) {
-                dy[p] = load_within(static_cast<const T*>(a.dy) + r * a.dy_stride, zc * V, a.out);
-                if (a.act) pre[p] = load_within(static_cast<const T*>(a.pre) + r * a.pre_stride, zc * V, a.out);
-            }
-        }
-        if (a.x)
-#pragma unroll
-            for (int p = 0; p < Passes; p++) {
-                const int l = xl + p * x_step;
-                const int64_t r = first + l;
-                xv[p] = Frag<T>(0);
-                if (l < kRows && r < stop && xc < x_chunks) xv[p] = load_within(static_cast<const T*>(a.x) + r * a.x_stride, xc * V, a.in);
-            }
+        dy.load(a.dy, a.dy_stride, a.out, first, stop);
+        if (a.act) pre.load(a.pre, a.pre_stride, a.out, first, stop);
+        if (a.x) x.load(a.x, a.x_stride, a.in, first, stop);
     };
+    const int zc = dy.chunk(), xc = x.chunk();
     const int64_t last = min(a.groups.rows, (blockIdx.x + int64_t{1}) * a.chunk);
     for (int64_t first = blockIdx.x * a.chunk; first < last;) {
         const int group = group_of(a.groups, first);
@@ -589,8 +654,8 @@ __global__ void __launch_bounds__(Waves * 64) k_narrow_bwd(NarrowBwdArgs a) {
         __syncthreads();  // the group's before have been worked on
         if (a.to.out) {
             const T* const w = static_cast<const T*>(a.weight) + group * a.in * a.out;
-            for (int i = threadIdx.x; i < kt * nt * kSteps * 64; i += kThreads) {
-                const int k = i / 64 / (nt * kSteps) * 32 + i % 32, n = (2 * (i / 64 % (nt * kSteps)) + i % 64 / 32) * V;
+            for (int i = threadIdx.x; i < XT * kSteps * 64; i += kThreads) {
+                const int k = i / 64 / kSteps * 32 + i % 32, n = (2 * (i / 64 % kSteps) + i % 64 / 32) * V;
                 Frag<T> f(0);
                 if (k < a.in)
 #pragma unroll
@@ -599,74 +664,72 @@ __global__ void __launch_bounds__(Waves * 64) k_narrow_bwd(NarrowBwdArgs a) {
                 weights[i] = f;
             }
         }
-        Sums sums[Tiles];
+        Sums sums[kTiles];
         Floats<V> db(0.0f);
 #pragma unroll
-        for (int t = 0; t < Tiles; t++) sums[t] = Sums(0.0f);
+        for (int t = 0; t < kTiles; t++) sums[t] = Sums(0.0f);
         for (int64_t block = first; block < stop; block += kRows) {
+            const int rows = static_cast<int>(min(stop - block, int64_t{kRows}));
 #pragma unroll
-            for (int p = 0; p < Passes; p++) {
-                const int l = zl + p * z_step;
-                if (l < kRows && zc < z_chunks) {
-                    Floats<V> d = floats<T, V>(dy[p]);
-                    if (a.act) {
-                        const Floats<V> z = floats<T, V>(pre[p]);
-#pragma unroll
-                        for (int e = 0; e < V; e++) d[e] = through<T>(d[e], z[e], a.act);
-                    }
-                    db += d;
-                    *reinterpret_cast<Frag<T>*>(dz + l * z_bytes + zc * 16) = raw<T, V>(d);
-                }
+            for (int i = 0; i < dy.N; i++) {
+                Floats<V> d = floats<T, V>(dy.v[i]);
+                if (a.act) through<T, V>(d, floats<T, V>(pre.v[i]), a.act);
+                if (dy.line(i) >= rows || zc * V >= a.out) d = Floats<V>(0.0f);
+                db += d;
+                *reinterpret_cast<Frag<T>*>(dz + dy.line(i) * kZ + zc * 16) = raw<T, V>(d);
             }
             if (a.x)
 #pragma unroll
-                for (int p = 0; p < Passes; p++) {
-                    const int l = xl + p * x_step;
-                    if (l < kRows && xc < x_chunks) *reinterpret_cast<Frag<T>*>(xs + l * x_bytes + xc * 16) = xv[p];
-                }
+                for (int i = 0; i < x.N; i++)
+                    *reinterpret_cast<Frag<T>*>(xs + x.line(i) * kX + xc * 16) = x.line(i) < rows && xc * V < a.in ? x.v[i] : Frag<T>(0);
             __syncthreads();
             if (block + kRows < stop) load(block + kRows, stop);
             if (a.to.out)
-                for (int i = wave; i < kRows / 32 * kt; i += Waves) {
-                    const int strip = i / kt * 32, t = i % kt;
-                    const int64_t r = block + strip + lane % 32;
-                    if (block + strip >= stop) break;
-                    Sums c(0.0f);
-                    for (int s = 0; s < nt * kSteps; s++)
-                        mma(c, weights[(t * nt * kSteps + s) * 64 + lane],
-                            *reinterpret_cast<const Frag<T>*>(dz + (strip + lane % 32) * z_bytes + (2 * s + lane / 32) * 16));
-                    finish32<T>(a.to, r, r < stop, t * 32, c);
+                for (int i = wave; i < kRows / 32 * (XT / kUnitTiles<T>); i += Waves) {
+                    const int strip = i / (XT / kUnitTiles<T>) * 32, t = i % (XT / kUnitTiles<T>) * kUnitTiles<T>;
+                    if (strip >= rows) break;
+                    if (t >= kt) continue;
+                    Sums unit[kUnitTiles<T>];
+#pragma unroll
+                    for (int u = 0; u < kUnitTiles<T>; u++) unit[u] = Sums(0.0f);
+                    for (int s = 0; s < nt * static_cast<int>(sizeof(T)); s++) {
+                        const Frag<T> row = *reinterpret_cast<const Frag<T>*>(dz + (strip + lane % 32) * kZ + (2 * s + lane / 32) * 16);
+#pragma unroll
+                        for (int u = 0; u < kUnitTiles<T>; u++) mma(unit[u], weights[((t + u) * kSteps + s) * 64 + lane], row);
+                    }
+                    store_unit<T>(a.to, block + strip, stop, t * 32, unit, mine);
                 }
             if (a.x)
 #pragma unroll
-                for (int i = 0; i < Tiles; i++) {
+                for (int i = 0; i < kTiles; i++) {
                     const int t = wave + i * Waves;
-                    if (t < nt * kt)
+                    if (t / XT < nt && t % XT < kt)
 #pragma unroll
                         for (int s = 0; s < 8; s++)
-                            mma(sums[i], across_fragment<T>(xs, x_bytes, t % kt * 32, s), across_fragment<T>(dz, z_bytes, t / kt * 32, s));
+                            mma(sums[i], across_fragment<T, XT>(xs, t % XT * 32, s), across_fragment<T, ZT>(dz, t / XT * 32, s));
                 }
             __syncthreads();
         }
         if (a.partial) {
             float* const slab = a.partial + (int64_t{blockIdx.x} + group) * a.size;
 #pragma unroll
-            for (int i = 0; i < Tiles; i++) {
+            for (int i = 0; i < kTiles; i++) {
                 const int t = wave + i * Waves;
-                const int64_t n = t / kt * 32 + lane % 32;
-                if (t < nt * kt && n < a.out)
+                const int64_t n = t / XT * 32 + lane % 32;
+                if (a.x && t % XT < kt && n < a.out)
 #pragma unroll
                     for (int q = 0; q < 4; q++) {
-                        const int64_t k = t % kt * 32 + 8 * q + lane / 32 * 4;
+                        const int64_t k = t % XT * 32 + 8 * q + lane / 32 * 4;
                         const Floats<4> v = {sums[i][4 * q], sums[i][4 * q + 1], sums[i][4 * q + 2], sums[i][4 * q + 3]};
                         store_some<float, 4>(slab + n * a.in + k, v, static_cast<int>(max(int64_t{0}, min(a.in - k, int64_t{4}))));
                     }
             }
             Floats<V>* const parts = reinterpret_cast<Floats<V>*>(lds);
+            static_assert(kThreads * sizeof(Floats<V>) <= kRows * (kZ + kX));
             parts[threadIdx.x] = db;
             __syncthreads();
-            if (static_cast<int>(threadIdx.x) < z_lanes && zc * V < a.out) {
-                for (int l = 1; l < z_step; l++) db += parts[l * z_lanes + zc];
+            if (static_cast<int>(threadIdx.x) < dy.kLanes && zc * V < a.out) {
+                for (int l = 1; l < dy.kLines; l++) db += parts[l * dy.kLanes + zc];
                 store_some<float, V>(slab + a.in * a.out + zc * V, db, static_cast<int>(min(a.out - zc * V, int64_t{V})));
             }
         }
@@ -701,8 +764,7 @@ __global__ void __launch_bounds__(256) k_slope(SlopeArgs a, int lanes) {
             Floats<V> d = floats<T, V>(load_within(static_cast<const T*>(a.dy) + r * a.dy_stride, c, a.cols));
             if (a.act) {
                 const Floats<V> z = floats<T, V>(load_within(static_cast<const T*>(a.pre) + r * a.pre_stride, c, a.cols));
-#pragma unroll
-                for (int e = 0; e < V; e++) d[e] = through<T>(d[e], z[e], a.act);
+                through<T, V>(d, z, a.act);
                 if (a.dz) store_some<T, V>(static_cast<T*>(a.dz) + r * a.dz_stride + c, d, n);
             }
             sum += d;
@@ -745,14 +807,14 @@ int log2_up(int64_t n) {
 }
 int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to; }
 
-// out[rows][cols] over `depth`, rows in groups: the tile's side, and how many parts the depth is split into.
+// out[rows][cols] over `depth`, rows in groups: the tile's rows (of 128 columns), and how many parts the depth is split into.
 struct Plan {
     int side, splits;
     int64_t split, bytes;
 };
 Plan plan_rows(int64_t rows, int64_t cols, int64_t depth, int groups, bool ragged, int elem) {
     Plan p{128, 1, 0, 0};
-    const auto tiles = [&](int side) { return slots_of(rows, groups, log2_up(side), ragged) * up(cols, side); };
+    const auto tiles = [&](int side) { return slots_of(rows, groups, log2_up(side), ragged) * up(cols, 128); };
     if (tiles(128) < kManyTiles) p.side = 64;
     const int64_t step = 128 / elem, steps = up(depth, step);
     if (p.side == 64) p.splits = static_cast<int>(std::max<int64_t>(1, std::min(kManyTiles / std::max<int64_t>(tiles(64), 1), steps / 4)));
@@ -762,15 +824,15 @@ Plan plan_rows(int64_t rows, int64_t cols, int64_t depth, int groups, bool ragge
     p.bytes = p.splits > 1 ? p.splits * rows * cols * 4 : 0;
     return p;
 }
-// out[groups][out][in] over the groups' rows: the tile's side, and the parts of the rows (shift 62: each group's are one).
+// out[groups][out][in] over the groups' rows: the tile's rows, and the parts of the rows (shift 62: each group's are one).
 struct Over {
     int side, shift;
     int64_t slots, bytes;
 };
 Over plan_over(int64_t rows, int64_t out, int64_t in, int groups, bool ragged) {
     Over p{128, 62, groups, 0};
-    if (std::max(out, in) <= 64) p.side = 64;
-    const int64_t tiles = up(out, p.side) * up(in, p.side);
+    if (out <= 64) p.side = 64;
+    const int64_t tiles = up(out, p.side) * up(in, 128);
     const int64_t wanted = std::max<int64_t>(1, 2 * kManyTiles / tiles);
     const bool direct = tiles * groups >= kManyTiles && tiles >= 32;
     const int shift = std::max(8, log2_up(up(std::max<int64_t>(rows, 1), wanted)));
@@ -807,11 +869,11 @@ void check_grid(int64_t blocks, int64_t threads) {
 
 template <class T, bool RowAcross, bool ColAcross>
 void launch_tiles(const TileArgs& a, int side, int64_t slabs, hipStream_t s) {
-    const int64_t down = RowAcross ? up(a.rows, side) : a.slots, tiles = up(down * up(a.to.cols, side), 8) * 8;
+    const int64_t down = RowAcross ? up(a.rows, side) : a.slots, tiles = up(down * up(a.to.cols, 128), 8) * 8;
     check_grid(tiles * slabs, 256);
     const dim3 grid(static_cast<uint32_t>(tiles), static_cast<uint32_t>(slabs));
     if (side == 128) k_tile<T, 128, 128, 64, 64, RowAcross, ColAcross><<<grid, 256, 0, s>>>(a);
-    else k_tile<T, 64, 64, 32, 32, RowAcross, ColAcross><<<grid, 256, 0, s>>>(a);
+    else k_tile<T, 64, 128, 32, 64, RowAcross, ColAcross><<<grid, 256, 0, s>>>(a);
 }
 
 // `slabs`: of a group, on average
@@ -834,14 +896,16 @@ struct Narrow {
     int steps, threads, lds;
     int64_t blocks, chunk;
 };
-Narrow plan_narrow(int64_t rows, int64_t in, int64_t out, int elem) {
+template <class T>
+Narrow plan_narrow(int64_t rows, int64_t in, int64_t out) {
+    constexpr int elem = sizeof(T);
     Narrow p{};
     const int steps = narrow_steps(in, elem);
-    const int64_t tiles = up(out, 32), kib = tiles * steps;
-    if (!steps || kib > 128 || (rows < 4096 && kib > 16)) return p;
+    const int64_t tiles = elem == 4 ? up(out, 32) : up(out, 64) * 2, kib = tiles * steps;
+    if (!steps || kib > 112 || (rows < 4096 && kib > 16)) return p;
     p.steps = steps;
-    p.lds = static_cast<int>(kib * 1024 + tiles * 128);
     p.threads = kib > 32 ? 512 : 256;
+    p.lds = static_cast<int>(kib * 1024 + tiles * 128) + p.threads / 64 * kUnitBytes<T>;
     const int64_t each = std::max(1, std::min(p.threads == 512 ? 2 : 4, 160 * 1024 / p.lds));
     p.blocks = std::max<int64_t>(1, std::min<int64_t>(256 * each, up(rows, p.threads / 2)));
     p.chunk = up(up(rows, p.blocks), 32) * 32;
@@ -850,24 +914,35 @@ Narrow plan_narrow(int64_t rows, int64_t in, int64_t out, int elem) {
 }
 // A backward whose blocks of rows a workgroup holds.
 struct NarrowBwd {
-    int waves, lds;
+    int waves, zt, xt, lds;
     int64_t blocks, chunk, size, bytes;
 };
 template <class T>
 NarrowBwd plan_narrow_bwd(int64_t rows, int64_t in, int64_t out, int groups) {
     NarrowBwd p{};
     const int64_t nt = up(out, 32), kt = up(in, 32);
-    if (nt * kt > 16 || nt > 8 || kt > 8) return p;
-    p.lds = kBlockRows<T> * (line_bytes<T>(static_cast<int>(nt)) + line_bytes<T>(static_cast<int>(kt))) + static_cast<int>(nt * kt * sizeof(T)) * 1024;
-    if (p.lds > 160 * 1024) return p;
-    p.waves = nt <= 2 && kt <= 2 ? 4 : 8;
-    const int64_t each = std::max(1, std::min(p.waves == 4 ? 4 : 2, 160 * 1024 / p.lds));
+    if (nt <= 2 && kt <= 2) p.waves = 4, p.zt = p.xt = 2;
+    else if (nt <= 4 && kt <= 4) p.waves = 8, p.zt = p.xt = 4;
+    else if (nt <= 2 && kt <= 8) p.waves = 8, p.zt = 2, p.xt = 8;
+    else if (nt <= 8 && kt <= 2) p.waves = 8, p.zt = 8, p.xt = 2;
+    else return p;
+    p.lds = kBlockRows<T> * (line_bytes<T>(p.zt) + line_bytes<T>(p.xt)) + p.waves * kBareBytes<T> + p.zt * p.xt * static_cast<int>(sizeof(T)) * 1024;
+    if (p.lds > 160 * 1024) return {};
+    const int64_t each = std::max(1, std::min(2, 160 * 1024 / p.lds));
     p.blocks = std::max<int64_t>(1, std::min<int64_t>(256 * each, up(rows, kBlockRows<T>)));
     p.chunk = std::max<int64_t>(up(up(rows, p.blocks), 32) * 32, 32);
     p.blocks = std::max<int64_t>(up(rows, p.chunk), 1);
     p.size = in * out + out;
     p.bytes = (p.blocks + groups) * p.size * 4;
     return p;
+}
+template <class T>
+void launch_narrow_bwd(const NarrowBwdArgs& a, const NarrowBwd& p, hipStream_t s) {
+    const auto go = [&](auto kernel) { kernel<<<static_cast<uint32_t>(p.blocks), p.waves * 64, p.lds, s>>>(a); };
+    if (p.waves == 4) go(k_narrow_bwd<T, 4, 2, 2>);
+    else if (p.zt == 4) go(k_narrow_bwd<T, 8, 4, 4>);
+    else if (p.zt == 2) go(k_narrow_bwd<T, 8, 2, 8>);
+    else go(k_narrow_bwd<T, 8, 8, 2>);
 }
 
 template <class T>
@@ -904,7 +979,7 @@ void over_depth(TileArgs a, bool ragged, float* work, hipStream_t s) {
 template <class T>
 void forward(const LinearFwdArgs& f, hipStream_t s) {
     const Finish to{f.y, f.y_stride, f.out, f.residual, f.residual_stride, f.pre, f.pre_stride, f.act, f.clear};
-    if (const Narrow p = plan_narrow(f.rows, f.in, f.out, sizeof(T)); p.blocks) {
+    if (const Narrow p = plan_narrow<T>(f.rows, f.in, f.out); p.blocks) {
         launch_narrow<T>({f.x, f.weight, f.bias, f.x_stride, to, f.in, f.out, p.chunk, {f.ends, f.groups, f.rows}}, p, s);
         return;
     }
@@ -931,10 +1006,7 @@ void backward(const LinearBwdArgs& f, hipStream_t s) {
         a.in = f.in; a.out = f.out; a.chunk = p.chunk; a.size = p.size; a.groups = groups; a.act = f.act;
         const bool sums = f.dweight || f.dbias;
         a.partial = sums ? reinterpret_cast<float*>(work) : nullptr;
-        if (f.rows) {
-            if (p.waves == 4) k_narrow_bwd<T, 4, 1, 4><<<static_cast<uint32_t>(p.blocks), 256, p.lds, s>>>(a);
-            else k_narrow_bwd<T, 8, 2, 8><<<static_cast<uint32_t>(p.blocks), 512, p.lds, s>>>(a);
-        }
+        if (f.rows) launch_narrow_bwd<T>(a, p, s);
         if (sums) {
             JoinArgs j{};
             j.partial = a.partial; j.dweight = f.dweight; j.dbias = f.dbias; j.weights = f.in * f.out; j.size = p.size; j.wanted = f.dbias ? p.size : j.weights;
@@ -998,7 +1070,7 @@ void with_type(ElemType t, F&& f) {
 
 int64_t linear_fwd_workspace(int64_t rows, int64_t in, int64_t out, int groups, bool ragged, ElemType type) {
     const int elem = type == kF32 ? 4 : 2;
-    return plan_narrow(rows, in, out, elem).blocks ? 0 : plan_rows(rows, out, in, groups, ragged, elem).bytes;
+    return (elem == 4 ? plan_narrow<float>(rows, in, out) : plan_narrow<__bf16>(rows, in, out)).blocks ? 0 : plan_rows(rows, out, in, groups, ragged, elem).bytes;
 }
 int64_t linear_bwd_workspace(int64_t rows, int64_t in, int64_t out, int groups, bool ragged, ElemType type) {
     const int elem = type == kF32 ? 4 : 2;

@@ -87,36 +87,49 @@ __device__ inline float lower_tail(float z, float* density) {
     return r * t * e;
 }
 
-template <class T>
-__device__ inline float activated(float z, int act) {
+// act of each of V values.
+template <class T, int V>
+__device__ inline void activate(Floats<V>& v, int act) {
+    const auto each = [&](auto f) {
+#pragma unroll
+        for (int e = 0; e < V; e++) v[e] = f(v[e]);
+    };
     switch (act) {
-        case kRelu: return z <= 0.0f ? 0.0f : z;
-        case kGelu: {
-            float density;
-            const float q = lower_tail<T>(z, &density);
-            return z * (z > 0.0f ? 1.0f - q : q);
-        }
-        case kSilu: return z * inverse<T>(1.0f + exp_minus<T>(z));
-        case kSigmoid: return inverse<T>(1.0f + exp_minus<T>(z));
-        default: return z;
+        case kRelu: return each([](float z) { return z <= 0.0f ? 0.0f : z; });
+        case kGelu:
+            return each([](float z) {
+                float density;
+                const float q = lower_tail<T>(z, &density);
+                return z * (z > 0.0f ? 1.0f - q : q);
+            });
+        case kSilu: return each([](float z) { return z * inverse<T>(1.0f + exp_minus<T>(z)); });
+        case kSigmoid: return each([](float z) { return inverse<T>(1.0f + exp_minus<T>(z)); });
+        default: return;
     }
 }
-// dy times the activation's slope at z. (relu's is 0 wherever z is not above 0, whatever dy.)
-template <class T>
-__device__ inline float through(float dy, float z, int act) {
+// V values times the activation's slope at z. (relu's is 0 wherever z is not above 0, whatever dy.)
+template <class T, int V>
+__device__ inline void through(Floats<V>& dy, Floats<V> z, int act) {
+    const auto each = [&](auto f) {
+#pragma unroll
+        for (int e = 0; e < V; e++) dy[e] = f(dy[e], z[e]);
+    };
     switch (act) {
-        case kRelu: return z > 0.0f ? dy : 0.0f;
-        case kGelu: {
-            float density;
-            const float q = lower_tail<T>(z, &density);
-            return dy * __builtin_fmaf(z, density * 0.398942280f, z > 0.0f ? 1.0f - q : q);
-        }
-        case kSilu: {
-            const float p = inverse<T>(1.0f + exp_minus<T>(z)), q = inverse<T>(1.0f + exp_minus<T>(-z));  // p + q = 1
-            return dy * __builtin_fmaf(z * p, q, p);
-        }
-        case kSigmoid: return dy * (inverse<T>(1.0f + exp_minus<T>(z)) * inverse<T>(1.0f + exp_minus<T>(-z)));
-        default: return dy;
+        case kRelu: return each([](float d, float z) { return z > 0.0f ? d : 0.0f; });
+        case kGelu:
+            return each([](float d, float z) {
+                float density;
+                const float q = lower_tail<T>(z, &density);
+                return d * __builtin_fmaf(z, density * 0.398942280f, z > 0.0f ? 1.0f - q : q);
+            });
+        case kSilu:
+            return each([](float d, float z) {
+                const float p = inverse<T>(1.0f + exp_minus<T>(z)), q = inverse<T>(1.0f + exp_minus<T>(-z));  // p + q = 1
+                return d * __builtin_fmaf(z * p, q, p);
+            });
+        case kSigmoid:
+            return each([](float d, float z) { return d * (inverse<T>(1.0f + exp_minus<T>(z)) * inverse<T>(1.0f + exp_minus<T>(-z))); });
+        default: return;
     }
 }
 
