@@ -94,6 +94,42 @@ struct Stage {
     }
 };
 
+// The same straight from memory into LDS, of whole tiles whose lines begin on 16 bytes: a wave's load fills 1 KiB of LDS in the
+// order of the lanes, so that it is the lane's place in memory that goes by where the chunk lies.
+template <class T, int R, bool Across, int Threads>
+struct DirectStage {
+    static constexpr int V = kPer<T>, kDepth = 128 / static_cast<int>(sizeof(T)), N = R * 8 / Threads;
+    const char* base;
+    int64_t step;       // bytes to the next tile
+    uint32_t offset[N];  // of the lane's chunks
+    // As Stage's; `d` the sums' first element
+    __device__ DirectStage(const T* b, int64_t s, int64_t f, int64_t l, int64_t d) {
+        const int64_t line = s * static_cast<int64_t>(sizeof(T));
+        base = reinterpret_cast<const char*>(b) + (Across ? d * line : f * line + d * static_cast<int64_t>(sizeof(T)));
+        step = Across ? kDepth * line : 128;
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const int at = (i * Threads + static_cast<int>(threadIdx.x)) * 16;  // in the tile
+            if constexpr (Across) {
+                constexpr int kLine = R * static_cast<int>(sizeof(T));
+                const int m = at / kLine, byte = across_at<T>(m, at % kLine, kLine) - m * kLine;
+                offset[i] = static_cast<uint32_t>(m * line + min(f * static_cast<int64_t>(sizeof(T)) + byte, (l - V) * static_cast<int64_t>(sizeof(T))));
+            } else {
+                const int r = at / 128, c = (at / 16 % 8) ^ (r & 7);
+                offset[i] = static_cast<uint32_t>(min(int64_t{r}, l - 1 - f) * line + c * 16);
+            }
+        }
+    }
+    __device__ void load(char* lds) {
+        using Global = __attribute__((address_space(1))) const void*;
+        using Lds = __attribute__((address_space(3))) void*;
+#pragma unroll
+        for (int i = 0; i < N; i++)
+            __builtin_amdgcn_global_load_lds((Global)(base + offset[i]), (Lds)(lds + (i * Threads + __builtin_amdgcn_readfirstlane(threadIdx.x / 64 * 64)) * 16), 16, 0, 0);
+        base += step;
+    }
+};
+
 // The lane's fragment of rows [r, r + 32), step s of the tile's four.
 template <class T, int R, bool Across>
 __device__ inline Frag<T> fragment(const char* lds, int r, int s) {
@@ -263,12 +299,13 @@ __device__ inline void store_unit(const Finish& a, int64_t r, int64_t stop, int6
 
 // BR x BC outputs a workgroup, WR x WC a wave. OverRows: the sums go over a group's rows (dW), else the outputs' rows are the
 // groups' rows.
-template <class T, int BR, int BC, int WR, int WC, bool RowAcross, bool ColAcross>
+template <class T, int BR, int BC, int WR, int WC, bool RowAcross, bool ColAcross, bool Direct>
 __global__ void __launch_bounds__(BR / WR * (BC / WC) * 64) k_tile(TileArgs a) {
     constexpr bool OverRows = RowAcross;
     constexpr int kWaves = BR / WR * (BC / WC), kThreads = kWaves * 64, kDepth = 128 / static_cast<int>(sizeof(T));
     constexpr int kBuffer = (BR + BC) * 128, I = WR / 32, J = WC / 32;
-    __shared__ __attribute__((aligned(128))) char lds[2 * kBuffer];
+    // (two arrays, so that a load into one is seen to be no store into the other)
+    __shared__ __attribute__((aligned(128))) char lds[kBuffer], lds1[kBuffer];
     // Which tile: workgroups go round the eight dies, and each die takes tiles side by side, eight rows of tiles at a time.
     const int64_t across = (a.to.cols + BC - 1) / BC, down = OverRows ? (a.rows + BR - 1) / BR : a.slots, tiles = across * down;
     const int64_t each = (tiles + 7) / 8, tile = blockIdx.x % 8 * each + blockIdx.x / 8;
@@ -305,23 +342,7 @@ __global__ void __launch_bounds__(BR / WR * (BC / WC) * 64) k_tile(TileArgs a) {
     for (int i = 0; i < I; i++)
 #pragma unroll
         for (int j = 0; j < J; j++) sums[i][j] = Sums(0.0f);
-    Stage<T, BR, RowAcross, kThreads> row(static_cast<const T*>(a.row), a.row_stride, r0, r1);
-    Stage<T, BC, ColAcross, kThreads> col(static_cast<const T*>(a.col) + part.group * a.col_group, a.col_stride, c0, a.to.cols);
-    if (d0 < d1) {
-        row.load(d0, d1);
-        col.load(d0, d1);
-        row.store(lds);
-        col.store(lds + BR * 128);
-    }
-    __syncthreads();
-    int now = 0;
-    for (int64_t d = d0; d < d1; d += kDepth) {
-        const bool more = d + kDepth < d1;
-        if (more) {
-            row.load(d + kDepth, d1);
-            col.load(d + kDepth, d1);
-        }
-        const char* buffer = lds + now * kBuffer;
+    const auto multiply = [&](const char* buffer) {
 #pragma unroll
         for (int s = 0; s < 4; s++) {
             Frag<T> fr[I], fc[J];
@@ -334,13 +355,69 @@ __global__ void __launch_bounds__(BR / WR * (BC / WC) * 64) k_tile(TileArgs a) {
 #pragma unroll
                 for (int j = 0; j < J; j++) mma(sums[i][j], fc[j], fr[i]);
         }
-        now ^= 1;
-        if (more) {
-            row.store(lds + now * kBuffer);
-            col.store(lds + now * kBuffer + BR * 128);
+    };
+    const T *const rows_from = static_cast<const T*>(a.row), *const cols_from = static_cast<const T*>(a.col) + part.group * a.col_group;
+    Stage<T, BR, RowAcross, kThreads> row(rows_from, a.row_stride, r0, r1);
+    Stage<T, BC, ColAcross, kThreads> col(cols_from, a.col_stride, c0, a.to.cols);
+    if constexpr (Direct) {
+        DirectStage<T, BR, RowAcross, kThreads> rows(rows_from, a.row_stride, r0, r1, d0);
+        DirectStage<T, BC, ColAcross, kThreads> cols(cols_from, a.col_stride, c0, a.to.cols, d0);
+        const int64_t whole = (d1 - d0) / kDepth;
+        const auto step = [&](int64_t t, char* now, char* next) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's loads into `now` have landed; after the barrier all
+            __syncthreads();
+            if (t + 1 < whole) {
+                rows.load(next);
+                cols.load(next + BR * 128);
+            }
+            multiply(now);
+        };
+        if (whole) {
+            rows.load(lds);
+            cols.load(lds + BR * 128);
+        }
+        for (int64_t t = 0; t < whole; t += 2) {
+            step(t, lds, lds1);
+            if (t + 1 < whole) step(t + 1, lds1, lds);
+        }
+        if (d0 + whole * kDepth < d1) {
+            row.load(d0 + whole * kDepth, d1);
+            col.load(d0 + whole * kDepth, d1);
+            __syncthreads();
+            row.store(lds);
+            col.store(lds + BR * 128);
+            __syncthreads();
+            multiply(lds);
         }
         __syncthreads();
+    } else {
+        if (d0 < d1) {
+            row.load(d0, d1);
+            col.load(d0, d1);
+            row.store(lds);
+            col.store(lds + BR * 128);
+        }
+        __syncthreads();
+        char *now = lds, *next = lds1;
+        for (int64_t d = d0; d < d1; d += kDepth) {
+            const bool more = d + kDepth < d1;
+            if (more) {
+                row.load(d + kDepth, d1);
+                col.load(d + kDepth, d1);
+            }
+            multiply(now);
+            if (more) {
+                row.store(next);
+                col.store(next + BR * 128);
+            }
+            __syncthreads();
+            char* const t = now;
+            now = next;
+            next = t;
+        }
     }
+    static_assert((kWaves + 1) / 2 * kUnitBytes<T> <= kBuffer);
+    char* const mine = (wave % 2 ? lds1 : lds) + wave / 2 * kUnitBytes<T>;
     Finish to = a.to;
     to.out = static_cast<T*>(to.out) + part.group * a.out_group;
 #pragma unroll
@@ -370,8 +447,8 @@ __global__ void __launch_bounds__(BR / WR * (BC / WC) * 64) k_tile(TileArgs a) {
                 }
             }
             if (a.partial) continue;
-            if constexpr (ColAcross) store_unit<T>(to, r, r1, c, unit, lds + wave * kUnitBytes<T>);
-            else finish_unit<T>(to, r, r1, c, unit, lds + wave * kUnitBytes<T>);
+            if constexpr (ColAcross) store_unit<T>(to, r, r1, c, unit, mine);
+            else finish_unit<T>(to, r, r1, c, unit, mine);
         }
     }
 }
@@ -800,6 +877,7 @@ __global__ void __launch_bounds__(256) k_slope_join(SlopeArgs a) {
 // ---- plans ------------------------------------------------------------------------------------------------
 
 constexpr int64_t kManyTiles = 512;  // two workgroups for each unit
+int64_t columns_of(int side) { return side == 256 ? 256 : 128; }  // of a tile of so many rows
 int log2_up(int64_t n) {
     int k = 0;
     while ((int64_t{1} << k) < n) k++;
@@ -814,8 +892,9 @@ struct Plan {
 };
 Plan plan_rows(int64_t rows, int64_t cols, int64_t depth, int groups, bool ragged, int elem) {
     Plan p{128, 1, 0, 0};
-    const auto tiles = [&](int side) { return slots_of(rows, groups, log2_up(side), ragged) * up(cols, 128); };
-    if (tiles(128) < kManyTiles) p.side = 64;
+    const auto tiles = [&](int side) { return slots_of(rows, groups, log2_up(side), ragged) * up(cols, columns_of(side)); };
+    if (tiles(256) >= 200 && cols > 128) p.side = 256;
+    else if (tiles(128) < kManyTiles) p.side = 64;
     const int64_t step = 128 / elem, steps = up(depth, step);
     if (p.side == 64) p.splits = static_cast<int>(std::max<int64_t>(1, std::min(kManyTiles / std::max<int64_t>(tiles(64), 1), steps / 4)));
     const int64_t each = up(steps, p.splits);
@@ -832,8 +911,9 @@ struct Over {
 Over plan_over(int64_t rows, int64_t out, int64_t in, int groups, bool ragged) {
     Over p{128, 62, groups, 0};
     if (out <= 64) p.side = 64;
-    const int64_t tiles = up(out, p.side) * up(in, 128);
-    const int64_t wanted = std::max<int64_t>(1, 2 * kManyTiles / tiles);
+    else if (up(out, 256) * up(in, 256) * groups >= 64 && out > 128 && in > 128) p.side = 256;
+    const int64_t tiles = up(out, p.side) * up(in, columns_of(p.side));
+    const int64_t wanted = std::max<int64_t>(1, (p.side == 256 ? kManyTiles : 2 * kManyTiles) / tiles);
     const bool direct = tiles * groups >= kManyTiles && tiles >= 32;
     const int shift = std::max(8, log2_up(up(std::max<int64_t>(rows, 1), wanted)));
     if (!direct && rows > int64_t{1} << shift) {
@@ -869,11 +949,21 @@ void check_grid(int64_t blocks, int64_t threads) {
 
 template <class T, bool RowAcross, bool ColAcross>
 void launch_tiles(const TileArgs& a, int side, int64_t slabs, hipStream_t s) {
-    const int64_t down = RowAcross ? up(a.rows, side) : a.slots, tiles = up(down * up(a.to.cols, 128), 8) * 8;
-    check_grid(tiles * slabs, 256);
+    const int64_t down = RowAcross ? up(a.rows, side) : a.slots, tiles = up(down * up(a.to.cols, columns_of(side)), 8) * 8;
+    check_grid(tiles * slabs, side == 256 ? 512 : 256);
     const dim3 grid(static_cast<uint32_t>(tiles), static_cast<uint32_t>(slabs));
-    if (side == 128) k_tile<T, 128, 128, 64, 64, RowAcross, ColAcross><<<grid, 256, 0, s>>>(a);
-    else k_tile<T, 64, 128, 32, 64, RowAcross, ColAcross><<<grid, 256, 0, s>>>(a);
+    // straight into LDS: lines that begin on 16 bytes, and whose places in a tile 32 bits hold
+    const auto direct = [](const void* p, int64_t stride) {
+        return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * sizeof(T) % 16 == 0 && stride < (int64_t{1} << 30) / 256 / static_cast<int>(sizeof(T));
+    };
+    const bool whole = direct(a.row, a.row_stride) && direct(a.col, a.col_stride) && a.col_group * sizeof(T) % 16 == 0 &&
+                       (!RowAcross || a.rows % kPer<T> == 0) && (!ColAcross || a.to.cols % kPer<T> == 0);
+    if (side == 256 && whole) k_tile<T, 256, 256, 128, 64, RowAcross, ColAcross, true><<<grid, 512, 0, s>>>(a);
+    else if (side == 256) k_tile<T, 256, 256, 128, 64, RowAcross, ColAcross, false><<<grid, 512, 0, s>>>(a);
+    else if (side == 128 && whole) k_tile<T, 128, 128, 64, 64, RowAcross, ColAcross, true><<<grid, 256, 0, s>>>(a);
+    else if (side == 128) k_tile<T, 128, 128, 64, 64, RowAcross, ColAcross, false><<<grid, 256, 0, s>>>(a);
+    else if (whole) k_tile<T, 64, 128, 32, 64, RowAcross, ColAcross, true><<<grid, 256, 0, s>>>(a);
+    else k_tile<T, 64, 128, 32, 64, RowAcross, ColAcross, false><<<grid, 256, 0, s>>>(a);
 }
 
 // `slabs`: of a group, on average

@@ -129,3 +129,34 @@ def test_grouped_linear(tb, i, n_in, n_out, act, dtype):
     sizes, behind = SIZES[i], (0, 1, 70, 200)[(i + n_in) % 4]
     k = i + n_out
     compare(tb, sum(sizes) + behind, n_in, n_out, dtype, act, bias=k % 3 != 2, add=k % 2 == 0, pad=(0, 8, 1)[k % 3], off=k % 2, sizes=sizes, seed=i)
+
+
+WIDE = [(13_000, 520, 1040), (13_001, 515, 1037), (700, 2056, 2200), (1300, 2049, 2051), (70_000, 264, 264), (3000, 1024, 4104), (257, 4096, 4096)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("i", range(len(WIDE)))
+def test_wide_linear(tb, i, dtype):
+    """Tiles of every size, whole lines and others, the sums' length no multiple of a tile's."""
+    compare(tb, *WIDE[i], dtype, ref.ACTS[i % 5], add=i % 2 == 0, pad=(0, 0, 8)[i % 3], seed=i)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,n_in,n_out", [(13_000, 520, 1040), (1300, 2049, 2051), (2000, 4096, 264), (70_001, 300, 500)])
+def test_wide_whole_numbers_are_exact(tb, rows, n_in, n_out, dtype):
+    print(rows, n_in, n_out, dtype, flush=True)
+    x, w, dy = (whole(*s, seed=i, dtype=dtype, most=1) for i, s in enumerate(((rows, n_in), (n_out, n_in), (rows, n_out))))
+    b = whole(n_out, seed=3, dtype=dtype)
+    y, _ = tb.linear_fwd(x, w, b)
+    assert torch.equal(y, (x.double() @ w.double().t().contiguous() + b.double()).to(dtype))
+    dx, dw, db = tb.linear_bwd(dy, x, w)
+    assert torch.equal(dx, (dy.double() @ w.double()).to(dtype))
+    assert torch.equal(dw, (dy.double().t().contiguous() @ x.double()).to(dtype))
+    assert torch.equal(db, dy.double().sum(0).to(dtype))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n_in,n_out,sizes", [(520, 1040, [3000, 0, 4100, 1, 2000, 257, 3000]), (515, 1037, [1000, 4001]), (1024, 1408, [700, 1300, 0, 5, 2600]),
+                                              (264, 64, [90, 0, 30_000, 3])])
+def test_wide_grouped_linear(tb, n_in, n_out, sizes, dtype):
+    compare(tb, sum(sizes) + 300, n_in, n_out, dtype, "silu", sizes=sizes, seed=n_in)
