@@ -363,22 +363,61 @@ __global__ void __launch_bounds__(BR / WR * (BC / WC) * 64) k_tile(TileArgs a) {
         DirectStage<T, BR, RowAcross, kThreads> rows(rows_from, a.row_stride, r0, r1, d0);
         DirectStage<T, BC, ColAcross, kThreads> cols(cols_from, a.col_stride, c0, a.to.cols, d0);
         const int64_t whole = (d1 - d0) / kDepth;
-        const auto step = [&](int64_t t, char* now, char* next) {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's loads into `now` have landed; after the barrier all
-            __syncthreads();
-            if (t + 1 < whole) {
-                rows.load(next);
-                cols.load(next + BR * 128);
+        // The fragments of a step are read while the products of the step before it run, also over the end of a tile: when the
+        // last step's are there the tile's place in LDS is free, and the next tile's loads, as long on their way as a tile's
+        // products take, have landed.
+        Frag<T> fr[2][I], fc[2][J];
+        const auto read = [&](int to, const char* buffer, int s) {
+#pragma unroll
+            for (int i = 0; i < I; i++) fr[to][i] = fragment<T, BR, RowAcross>(buffer, wr + i * 32, s);
+#pragma unroll
+            for (int j = 0; j < J; j++) fc[to][j] = fragment<T, BC, ColAcross>(buffer + BR * 128, wc + j * 32, s);
+        };
+        const auto product = [&](int of) {
+#pragma unroll
+            for (int i = 0; i < I; i++)
+#pragma unroll
+                for (int j = 0; j < J; j++) mma(sums[i][j], fc[of][j], fr[of][i]);
+        };
+        const auto load = [&](char* to) {
+            rows.load(to);
+            cols.load(to + BR * 128);
+        };
+        constexpr int kAcrossReads = sizeof(T) == 4 ? 4 : 2, kReads = I * (RowAcross ? kAcrossReads : 1) + J * (ColAcross ? kAcrossReads : 1);
+        constexpr int kProducts = I * J * (sizeof(T) == 4 ? 4 : 1), kEach = (kReads + kProducts - 1) / kProducts;
+        const auto alternate = [&] {
+#pragma unroll
+            for (int k = 0; k < kProducts; k++) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, kEach, 0);
             }
-            multiply(now);
+        };
+        const auto step = [&](int64_t t, char* now, const char* next) {
+#pragma unroll
+            for (int s = 0; s < 3; s++) {
+                read((s + 1) % 2, now, s + 1);
+                product(s % 2);
+                alternate();
+            }
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            __syncthreads();
+            if (t + 2 < whole) load(now);
+            read(0, next, 0);  // (after the last tile of what is there, for nothing)
+            product(1);
+            alternate();
         };
         if (whole) {
-            rows.load(lds);
-            cols.load(lds + BR * 128);
-        }
-        for (int64_t t = 0; t < whole; t += 2) {
-            step(t, lds, lds1);
-            if (t + 1 < whole) step(t + 1, lds1, lds);
+            load(lds);
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            if (whole > 1) load(lds1);
+            read(0, lds, 0);
+            for (int64_t t = 0;;) {
+                step(t, lds, lds1);
+                if (++t == whole) break;
+                step(t, lds1, lds);
+                if (++t == whole) break;
+            }
         }
         if (d0 + whole * kDepth < d1) {
             row.load(d0 + whole * kDepth, d1);
