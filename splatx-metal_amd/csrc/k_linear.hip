@@ -1,1219 +1,27 @@
-// k_linear.hip — linear layers over rows, forward and backward, all rows with one weight or groups of rows with their own
-// (include/splatx_hip.h has the formulas).
+// k_linear.hip — the linear layers' launchers by type (sx_linear.h has the kernels).
 #include <hip/hip_runtime.h>
 
-#include <algorithm>
-#include <stdexcept>
-#include <string>
-
-#include "sx_mma.h"
+#include "sx_learn.h"
 
 namespace sxk {
-using namespace sxd;
 namespace {
-
-// ---- tiles ------------------------------------------------------------------------------------------------
-//
-// out[r][c] = sum over d of row(r, d) col(c, d): x W^T, dz W and dz^T x, each operand either with its sums' elements side by
-// side in memory (plain) or with its rows side by side (Across: W's columns, dz's and x's).
-
-// What follows the sums, of rows of `cols` columns.
-struct Finish {
-    void* out;
-    int64_t out_stride, cols;
-    const void* residual;
-    int64_t residual_stride;
-    void* pre;
-    int64_t pre_stride;
-    int act;
-    bool clear;  // rows behind the last group become zero
-};
-
-struct TileArgs {
-    const void *row, *col;
-    int64_t row_stride, col_stride;  // elements between the rows in memory
-    int64_t col_group;               // elements between the groups' col operands
-    Finish to;                       // (its cols are the outputs')
-    int64_t out_group;
-    int64_t rows, depth;             // rows (of the products over rows), depth (of those over groups' rows): all groups'
-    Groups groups;
-    int shift;                       // the parts' rows, log2
-    int64_t slots;
-    float* partial;                  // [slabs][rows][cols] in place of out, or null
-    int64_t split;                   // depth of a slab
-    int splits;
-    const void* bias;
-    int64_t bias_group;
-};
-
-// Where the 16 bytes (row r, chunk c) of a plain operand's tile lie: 128 bytes a row, the chunks of eight rows in different
-// places, so that lanes that read one chunk of several rows read different banks.
-__device__ inline int plain_at(int r, int c) { return r * 128 + (c ^ (r & 7)) * 16; }
-// Of an Across operand's tile: `row_bytes` a row of the sums' dimension; four rows' 32 bytes in different places.
-template <class T>
-__device__ inline int across_at(int m, int byte, int row_bytes) {
-    return m * row_bytes + (sizeof(T) == 2 ? byte ^ ((m & 3) << 5) : byte);
-}
-
-// A thread's part of an operand's tile, R rows by 128 bytes of the sums' dimension, on its way from memory to LDS.
-template <class T, int R, bool Across, int Threads>
-struct Stage {
-    static constexpr int V = kPer<T>, kDepth = 128 / static_cast<int>(sizeof(T));
-    static constexpr int kPerLine = Across ? R / V : 8;  // chunks of a line in memory
-    static constexpr int kLines = Threads / kPerLine, N = R * 8 / Threads;
-    static_assert(Threads % kPerLine == 0 && R * 8 % Threads == 0);
-    Frag<T> v[N];
-    const T* base;
-    int64_t stride, first, limit;
-    int chunk, line;
-
-    // Rows [first, limit) (clamped, of a plain operand; columns of the memory's rows else)
-    __device__ Stage(const T* b, int64_t s, int64_t f, int64_t l) : base(b), stride(s), first(f), limit(l) {
-        chunk = threadIdx.x % kPerLine;
-        line = threadIdx.x / kPerLine;
-    }
-    // Of the sums' dimension [d, d + kDepth), zeros from `end` on.
-    __device__ void load(int64_t d, int64_t end) {
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-            const int l = line + i * kLines;
-            if constexpr (Across) {
-                v[i] = d + l < end ? load_within(base + (d + l) * stride, first + chunk * V, limit) : Frag<T>(0);
-            } else {
-                v[i] = load_within(base + min(first + l, limit - 1) * stride, d + chunk * V, end);
-            }
-        }
-    }
-    __device__ void store(char* lds) const {
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-            const int l = line + i * kLines;
-            const int at = Across ? across_at<T>(l, chunk * 16, R * static_cast<int>(sizeof(T))) : plain_at(l, chunk);
-            *reinterpret_cast<Frag<T>*>(lds + at) = v[i];
-        }
-    }
-};
-
-// The same straight from memory into LDS, of whole tiles whose lines begin on 16 bytes: a wave's load fills 1 KiB of LDS in the
-// order of the lanes, so that it is the lane's place in memory that goes by where the chunk lies.
-template <class T, int R, bool Across, int Threads>
-struct DirectStage {
-    static constexpr int V = kPer<T>, kDepth = 128 / static_cast<int>(sizeof(T)), N = R * 8 / Threads;
-    const char* base;
-    int64_t step;       // bytes to the next tile
-    uint32_t offset[N];  // of the lane's chunks
-    // As Stage's; `d` the sums' first element
-    __device__ DirectStage(const T* b, int64_t s, int64_t f, int64_t l, int64_t d) {
-        const int64_t line = s * static_cast<int64_t>(sizeof(T));
-        base = reinterpret_cast<const char*>(b) + (Across ? d * line : f * line + d * static_cast<int64_t>(sizeof(T)));
-        step = Across ? kDepth * line : 128;
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-            const int at = (i * Threads + static_cast<int>(threadIdx.x)) * 16;  // in the tile
-            if constexpr (Across) {
-                constexpr int kLine = R * static_cast<int>(sizeof(T));
-                const int m = at / kLine, byte = across_at<T>(m, at % kLine, kLine) - m * kLine;
-                offset[i] = static_cast<uint32_t>(m * line + min(f * static_cast<int64_t>(sizeof(T)) + byte, (l - V) * static_cast<int64_t>(sizeof(T))));
-            } else {
-                const int r = at / 128, c = (at / 16 % 8) ^ (r & 7);
-                offset[i] = static_cast<uint32_t>(min(int64_t{r}, l - 1 - f) * line + c * 16);
-            }
-        }
-    }
-    __device__ void load(char* lds) {
-        using Global = __attribute__((address_space(1))) const void*;
-        using Lds = __attribute__((address_space(3))) void*;
-#pragma unroll
-        for (int i = 0; i < N; i++)
-            __builtin_amdgcn_global_load_lds((Global)(base + offset[i]), (Lds)(lds + (i * Threads + __builtin_amdgcn_readfirstlane(threadIdx.x / 64 * 64)) * 16), 16, 0, 0);
-        base += step;
-    }
-};
-
-// The lane's fragment of rows [r, r + 32), step s of the tile's four.
-template <class T, int R, bool Across>
-__device__ inline Frag<T> fragment(const char* lds, int r, int s) {
-    const int lane = threadIdx.x % 64, half = lane / 32;
-    if constexpr (!Across) {
-        return *reinterpret_cast<const Frag<T>*>(lds + plain_at(r + lane % 32, 2 * s + half));
-    } else if constexpr (sizeof(T) == 4) {
-        Frag<T> f;
-#pragma unroll
-        for (int i = 0; i < 4; i++) f[i] = *reinterpret_cast<const float*>(lds + across_at<T>(s * 8 + half * 4 + i, (r + lane % 32) * 4, R * 4));
-        return f;
-    } else {
-        // sixteen lanes read four lines of sixteen columns and get a column each
-        using Four = short __attribute__((ext_vector_type(4)));
-        using Lds = __attribute__((address_space(3))) Four*;
-        const int group = lane % 16, column = r + (lane % 32) / 16 * 16 + group % 4 * 4;
-        Four part[2];
-#pragma unroll
-        for (int j = 0; j < 2; j++)
-            part[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (Lds)(lds + across_at<T>(s * 16 + half * 8 + j * 4 + group / 4, column * 2, R * 2)));
-        return __builtin_bit_cast(Frag<T>, __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7));
-    }
-}
-
-template <class T, int V>
-__device__ inline Floats<V> load_some(const T* p, int n) {
-    if (n >= V) return floats<T, V>(load_raw<V>(p));
-    Floats<V> v(0.0f);
-#pragma unroll
-    for (int e = 0; e < V; e++)
-        if (e < n) v[e] = static_cast<float>(p[e]);
-    return v;
-}
-template <class T, int V>
-__device__ inline void store_some(T* p, Floats<V> v, int n) {
-    if (n >= V) {
-        store_raw<V>(p, raw<T, V>(v));
-        return;
-    }
-#pragma unroll
-    for (int e = 0; e < V; e++)
-        if (e < n) p[e] = static_cast<T>(v[e]);
-}
-
-// Four columns from c on of row r, bias included.
-template <class T>
-__device__ inline void finish4(const Finish& a, int64_t r, int64_t c, Floats<4> v) {
-    const int n = static_cast<int>(min(a.cols - c, int64_t{4}));
-    if (n <= 0) return;
-    if (a.pre) store_some<T, 4>(static_cast<T*>(a.pre) + r * a.pre_stride + c, v, n);
-    activate<T, 4>(v, a.act);
-    if (a.residual) v += load_some<T, 4>(static_cast<const T*>(a.residual) + r * a.residual_stride + c, n);
-    store_some<T, 4>(static_cast<T*>(a.out) + r * a.out_stride + c, v, n);
-}
-// The same of a row behind the last group.
-template <class T>
-__device__ inline void clear4(const Finish& a, int64_t r, int64_t c) {
-    const int n = static_cast<int>(min(a.cols - c, int64_t{4}));
-    if (n <= 0 || !a.clear) return;
-    store_some<T, 4>(static_cast<T*>(a.out) + r * a.out_stride + c, Floats<4>(0.0f), n);
-    if (a.pre) store_some<T, 4>(static_cast<T*>(a.pre) + r * a.pre_stride + c, Floats<4>(0.0f), n);
-}
-
-// A wave's outputs go through LDS of its own as floats, so that a store has whole lines of eight rows: from the sums' layout (a
-// lane has four columns of its row in each place) to memory's, 32 rows of 128 bytes of the type, of which a lane takes 16 at a
-// time through what follows the sums. (Stores of 16 bytes a row from the registers, the rows' lines in four parts: a layer of
-// 64 outputs took twice as long.)
-template <class T>
-constexpr int kUnitTiles = 4 / static_cast<int>(sizeof(T));  // tiles of 32 columns side by side
-template <class T>
-constexpr int kUnitLine = kUnitTiles<T> * 128 + 16;  // (the lines of eight rows in different banks)
-template <class T>
-constexpr int kUnitBytes = 32 * kUnitLine<T>;
-
-// What lanes of the wave have written to LDS is there for the others.
-__device__ inline void wave_sees() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
-template <class T>
-__device__ inline void store_chunk(T* p, Floats<kPer<T>> f, int n) {
-    const Frag<T> v = raw<T, kPer<T>>(f);
-    if (n == kPer<T>) {
-        store_raw<kPer<T>>(p, v);
-        return;
-    }
-#pragma unroll
-    for (int e = 0; e < kPer<T> - 1; e++)
-        if (e < n) p[e] = v[e];
-}
-
-// 32 rows from r on (those before `stop`) and the columns [c, c + 128 bytes), the sums' bias included. Every lane takes part.
-template <class T>
-__device__ inline void finish_unit(const Finish& a, int64_t r, int64_t stop, int64_t c, const Sums (&sums)[kUnitTiles<T>], char* lds) {
-    constexpr int V = kPer<T>;
-    const int lane = threadIdx.x % 64;
-    wave_sees();  // (what was there has been read)
-#pragma unroll
-    for (int u = 0; u < kUnitTiles<T>; u++)
-#pragma unroll
-        for (int q = 0; q < 4; q++)
-            *reinterpret_cast<Floats<4>*>(lds + lane % 32 * kUnitLine<T> + lane / 32 * 16 + u * 128 + q * 32) =
-                Floats<4>{sums[u][4 * q], sums[u][4 * q + 1], sums[u][4 * q + 2], sums[u][4 * q + 3]};
-    wave_sees();
-    const int64_t column = c + lane % 8 * V;
-    const int n = static_cast<int>(max(int64_t{0}, min(a.cols - column, int64_t{V})));
-    const int rows = static_cast<int>(min(stop - r, int64_t{32}));
-    const char* from = lds + lane / 8 * kUnitLine<T> + lane % 8 * (V * 4);
-    r += lane / 8;
-    Frag<T> residual(0);
-    const auto load_residual = [&](int row, int64_t at) {
-        if (a.residual && row < rows) residual = load_within(static_cast<const T*>(a.residual) + at * a.residual_stride, column, a.cols);
-    };
-    load_residual(lane / 8, r);
-#pragma unroll 1
-    for (int row = lane / 8; row < rows; row += 8, r += 8, from += 8 * kUnitLine<T>) {
-        Floats<V> v;
-#pragma unroll
-        for (int e = 0; e < V; e += 4) {
-            const Floats<4> f = *reinterpret_cast<const Floats<4>*>(from + e * 4);
-            v[e] = f[0]; v[e + 1] = f[1]; v[e + 2] = f[2]; v[e + 3] = f[3];
-        }
-        if (a.pre) store_chunk(static_cast<T*>(a.pre) + r * a.pre_stride + column, v, n);
-        activate<T, V>(v, a.act);
-        if (a.residual) {
-            v += floats<T, V>(residual);
-            load_residual(row + 8, r + 8);
-        }
-        store_chunk(static_cast<T*>(a.out) + r * a.out_stride + column, v, n);
-    }
-}
-
-// The same of sums that are the outputs, through half the LDS.
-template <class T>
-constexpr int kBareLine = 128 + 16;
-template <class T>
-constexpr int kBareBytes = 32 * kBareLine<T>;
-template <class T>
-__device__ inline void store_unit(const Finish& a, int64_t r, int64_t stop, int64_t c, const Sums (&sums)[kUnitTiles<T>], char* lds) {
-    constexpr int V = kPer<T>;
-    const int lane = threadIdx.x % 64;
-    wave_sees();
-#pragma unroll
-    for (int u = 0; u < kUnitTiles<T>; u++)
-#pragma unroll
-        for (int q = 0; q < 4; q++)
-            *reinterpret_cast<Vec<T, 4>*>(lds + lane % 32 * kBareLine<T> + (u * 32 + 8 * q + lane / 32 * 4) * static_cast<int>(sizeof(T))) =
-                raw<T, 4>(Floats<4>{sums[u][4 * q], sums[u][4 * q + 1], sums[u][4 * q + 2], sums[u][4 * q + 3]});
-    wave_sees();
-    const int64_t column = c + lane % 8 * V;
-    const int n = static_cast<int>(max(int64_t{0}, min(a.cols - column, int64_t{V})));
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const Frag<T> v = *reinterpret_cast<const Frag<T>*>(lds + (lane / 8 + i * 8) * kBareLine<T> + lane % 8 * 16);
-        T* const p = static_cast<T*>(a.out) + (r + lane / 8 + i * 8) * a.out_stride + column;
-        if (r + lane / 8 + i * 8 >= stop) continue;
-        if (n == V) store_raw<V>(p, v);
-        else
-#pragma unroll
-            for (int e = 0; e < V - 1; e++)
-                if (e < n) p[e] = v[e];
-    }
-}
-
-// BR x BC outputs a workgroup, WR x WC a wave. OverRows: the sums go over a group's rows (dW), else the outputs' rows are the
-// groups' rows.
-template <class T, int BR, int BC, int WR, int WC, bool RowAcross, bool ColAcross, bool Direct>
-__global__ void __launch_bounds__(BR / WR * (BC / WC) * 64) k_tile(TileArgs a) {
-    constexpr bool OverRows = RowAcross;
-    constexpr int kWaves = BR / WR * (BC / WC), kThreads = kWaves * 64, kDepth = 128 / static_cast<int>(sizeof(T));
-    constexpr int kBuffer = (BR + BC) * 128, I = WR / 32, J = WC / 32;
-    // (two arrays, so that a load into one is seen to be no store into the other)
-    __shared__ __attribute__((aligned(128))) char lds[kBuffer], lds1[kBuffer];
-    // Which tile: workgroups go round the eight dies, and each die takes tiles side by side, eight rows of tiles at a time.
-    const int64_t across = (a.to.cols + BC - 1) / BC, down = OverRows ? (a.rows + BR - 1) / BR : a.slots, tiles = across * down;
-    const int64_t each = (tiles + 7) / 8, tile = blockIdx.x % 8 * each + blockIdx.x / 8;
-    if (blockIdx.x / 8 >= each || tile >= tiles) return;
-    const int64_t band = tile / (8 * across), height = min(down - band * 8, int64_t{8});
-    const int64_t tr = band * 8 + (tile - band * 8 * across) % height, tc = (tile - band * 8 * across) / height;
-
-    const Part part = part_of(a.groups, OverRows ? blockIdx.y : tr, a.shift);
-    int64_t r0, r1, d0, d1;
-    const int64_t c0 = tc * BC;
-    if constexpr (OverRows) {
-        r0 = tr * BR;
-        r1 = a.rows;
-        d0 = part.begin;
-        d1 = part.end;
-        if (part.group >= a.groups.groups || (a.partial && d0 >= d1)) return;
-    } else {
-        r0 = part.begin;
-        r1 = part.end;
-        d0 = blockIdx.y * a.split;
-        d1 = min(a.depth, d0 + a.split);
-        if (r0 >= r1) return;
-    }
-    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
-    const int wr = wave / (BC / WC) * WR, wc = wave % (BC / WC) * WC;
-    if (!OverRows && part.group >= a.groups.groups) {
-        if (a.partial) return;
-        for (int64_t r = r0 + threadIdx.x / 32; r < r1; r += kThreads / 32)
-            for (int c = threadIdx.x % 32 * 4; c < BC; c += 128) clear4<T>(a.to, r, c0 + c);
-        return;
-    }
-    Sums sums[I][J];
-#pragma unroll
-    for (int i = 0; i < I; i++)
-#pragma unroll
-        for (int j = 0; j < J; j++) sums[i][j] = Sums(0.0f);
-    const auto multiply = [&](const char* buffer) {
-#pragma unroll
-        for (int s = 0; s < 4; s++) {
-            Frag<T> fr[I], fc[J];
-#pragma unroll
-            for (int i = 0; i < I; i++) fr[i] = fragment<T, BR, RowAcross>(buffer, wr + i * 32, s);
-#pragma unroll
-            for (int j = 0; j < J; j++) fc[j] = fragment<T, BC, ColAcross>(buffer + BR * 128, wc + j * 32, s);
-#pragma unroll
-            for (int i = 0; i < I; i++)
-#pragma unroll
-                for (int j = 0; j < J; j++) mma(sums[i][j], fc[j], fr[i]);
-        }
-    };
-    const T *const rows_from = static_cast<const T*>(a.row), *const cols_from = static_cast<const T*>(a.col) + part.group * a.col_group;
-    Stage<T, BR, RowAcross, kThreads> row(rows_from, a.row_stride, r0, r1);
-    Stage<T, BC, ColAcross, kThreads> col(cols_from, a.col_stride, c0, a.to.cols);
-    if constexpr (Direct) {
-        DirectStage<T, BR, RowAcross, kThreads> rows(rows_from, a.row_stride, r0, r1, d0);
-        DirectStage<T, BC, ColAcross, kThreads> cols(cols_from, a.col_stride, c0, a.to.cols, d0);
-        const int64_t whole = (d1 - d0) / kDepth;
-        // The fragments of a step are read while the products of the step before it run, also over the end of a tile: when the
-        // last step's are there the tile's place in LDS is free, and the next tile's loads, as long on their way as a tile's
-        // products take, have landed.
-        Frag<T> fr[2][I], fc[2][J];
-        const auto read = [&](int to, const char* buffer, int s) {
-#pragma unroll
-            for (int i = 0; i < I; i++) fr[to][i] = fragment<T, BR, RowAcross>(buffer, wr + i * 32, s);
-#pragma unroll
-            for (int j = 0; j < J; j++) fc[to][j] = fragment<T, BC, ColAcross>(buffer + BR * 128, wc + j * 32, s);
-        };
-        const auto product = [&](int of) {
-#pragma unroll
-            for (int i = 0; i < I; i++)
-#pragma unroll
-                for (int j = 0; j < J; j++) mma(sums[i][j], fc[of][j], fr[of][i]);
-        };
-        const auto load = [&](char* to) {
-            rows.load(to);
-            cols.load(to + BR * 128);
-        };
-        constexpr int kAcrossReads = sizeof(T) == 4 ? 4 : 2, kReads = I * (RowAcross ? kAcrossReads : 1) + J * (ColAcross ? kAcrossReads : 1);
-        constexpr int kProducts = I * J * (sizeof(T) == 4 ? 4 : 1), kEach = (kReads + kProducts - 1) / kProducts;
-        const auto alternate = [&] {
-#pragma unroll
-            for (int k = 0; k < kProducts; k++) {
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x100, kEach, 0);
-            }
-        };
-        const auto step = [&](int64_t t, char* now, const char* next) {
-#pragma unroll
-            for (int s = 0; s < 3; s++) {
-                read((s + 1) % 2, now, s + 1);
-                product(s % 2);
-                alternate();
-            }
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-            __syncthreads();
-            if (t + 2 < whole) load(now);
-            read(0, next, 0);  // (after the last tile of what is there, for nothing)
-            product(1);
-            alternate();
-        };
-        if (whole) {
-            load(lds);
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads();
-            if (whole > 1) load(lds1);
-            read(0, lds, 0);
-            for (int64_t t = 0;;) {
-                step(t, lds, lds1);
-                if (++t == whole) break;
-                step(t, lds1, lds);
-                if (++t == whole) break;
-            }
-        }
-        if (d0 + whole * kDepth < d1) {
-            row.load(d0 + whole * kDepth, d1);
-            col.load(d0 + whole * kDepth, d1);
-            __syncthreads();
-            row.store(lds);
-            col.store(lds + BR * 128);
-            __syncthreads();
-            multiply(lds);
-        }
-        __syncthreads();
-    } else {
-        if (d0 < d1) {
-            row.load(d0, d1);
-            col.load(d0, d1);
-            row.store(lds);
-            col.store(lds + BR * 128);
-        }
-        __syncthreads();
-        char *now = lds, *next = lds1;
-        for (int64_t d = d0; d < d1; d += kDepth) {
-            const bool more = d + kDepth < d1;
-            if (more) {
-                row.load(d + kDepth, d1);
-                col.load(d + kDepth, d1);
-            }
-            multiply(now);
-            if (more) {
-                row.store(next);
-                col.store(next + BR * 128);
-            }
-            __syncthreads();
-            char* const t = now;
-            now = next;
-            next = t;
-        }
-    }
-    static_assert((kWaves + 1) / 2 * kUnitBytes<T> <= kBuffer);
-    char* const mine = (wave % 2 ? lds1 : lds) + wave / 2 * kUnitBytes<T>;
-    Finish to = a.to;
-    to.out = static_cast<T*>(to.out) + part.group * a.out_group;
-#pragma unroll
-    for (int i = 0; i < I; i++) {
-        const int64_t r = r0 + wr + i * 32;
-        if (r >= r1) break;
-#pragma unroll
-        for (int j = 0; j < J; j += kUnitTiles<T>) {
-            const int64_t c = c0 + wc + j * 32;
-            if (c >= a.to.cols) break;
-            Sums unit[kUnitTiles<T>];
-#pragma unroll
-            for (int u = 0; u < kUnitTiles<T>; u++) {
-                unit[u] = sums[i][j + u];
-#pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    const int64_t at = c + u * 32 + 8 * q + lane / 32 * 4;
-                    const int n = static_cast<int>(max(int64_t{0}, min(a.to.cols - at, int64_t{4})));
-                    if (a.partial) {
-                        const Floats<4> v = {unit[u][4 * q], unit[u][4 * q + 1], unit[u][4 * q + 2], unit[u][4 * q + 3]};
-                        store_some<float, 4>(a.partial + (int64_t{blockIdx.y} * a.rows + r + lane % 32) * a.to.cols + at, v, r + lane % 32 < r1 ? n : 0);
-                    } else if (a.bias) {
-                        const Floats<4> v = load_some<T, 4>(static_cast<const T*>(a.bias) + part.group * a.bias_group + at, n);
-#pragma unroll
-                        for (int e = 0; e < 4; e++) unit[u][4 * q + e] += v[e];
-                    }
-                }
-            }
-            if (a.partial) continue;
-            if constexpr (ColAcross) store_unit<T>(to, r, r1, c, unit, mine);
-            else finish_unit<T>(to, r, r1, c, unit, mine);
-        }
-    }
-}
-
-// The splits' slabs, added in order.
-template <class T>
-__global__ void __launch_bounds__(256) k_split_join(TileArgs a) {
-    const int64_t quads = (a.to.cols + 3) / 4;
-    for (int64_t i = blockIdx.x * int64_t{256} + threadIdx.x; i < a.rows * quads; i += gridDim.x * int64_t{256}) {
-        const int64_t r = i / quads, c = i % quads * 4;
-        const int n = static_cast<int>(min(a.to.cols - c, int64_t{4}));
-        int group = 0;
-        if (a.groups.ends) {
-            int hi = a.groups.groups;  // the first group that ends behind the row
-            while (group < hi) {
-                const int mid = (group + hi) / 2;
-                if (a.groups.end(mid) <= r) group = mid + 1;
-                else hi = mid;
-            }
-            if (group >= a.groups.groups) {
-                clear4<T>(a.to, r, c);
-                continue;
-            }
-        }
-        Floats<4> sum(0.0f);
-        for (int s = 0; s < a.splits; s++) sum += load_some<float, 4>(a.partial + (s * a.rows + r) * a.to.cols + c, n);
-        if (a.bias) sum += load_some<T, 4>(static_cast<const T*>(a.bias) + group * a.bias_group + c, n);
-        finish4<T>(a.to, r, c, sum);
-    }
-}
-
-// Gradients of a group's weights from the slabs of its parts of the rows: [out * in] of dweight, then, where dbias is wanted,
-// [out] of it. A group's first slab is g + its first row / step; each has `step` rows, counted from the group's first row
-// (`from_begin`) or from the first of all. `turns` threads (a power of two) share four elements.
-struct JoinArgs {
-    const float* partial;
-    void *dweight, *dbias;
-    int64_t weights, wanted, size;  // elements of a group's dweight, of what is joined, of a slab
-    Groups groups;
-    int64_t step;
-    bool from_begin;
-    int turns;
-};
-template <class T>
-__global__ void __launch_bounds__(256) k_weights_join(JoinArgs a) {
-    __shared__ Floats<4> part[256];
-    const int each = 256 / a.turns, lane = threadIdx.x % each, turn = threadIdx.x / each, group = blockIdx.y;
-    const int64_t begin = a.groups.begin(group), end = a.groups.end(group), first = group + begin / a.step;
-    const int64_t slabs = end > begin ? (end - 1 - (a.from_begin ? begin : 0)) / a.step - (a.from_begin ? 0 : begin / a.step) + 1 : 0;
-    for (int64_t at = int64_t{blockIdx.x} * each; at * 4 < a.wanted; at += int64_t{gridDim.x} * each) {
-        const int64_t i = (at + lane) * 4;
-        const int n = static_cast<int>(max(int64_t{0}, min(a.wanted - i, int64_t{4})));
-        Floats<4> sum(0.0f);
-        if (n > 0)
-#pragma unroll 4
-            for (int64_t s = turn; s < slabs; s += a.turns) sum += load_some<float, 4>(a.partial + (first + s) * a.size + i, n);
-        if (a.turns > 1) {
-            __syncthreads();
-            part[threadIdx.x] = sum;
-            __syncthreads();
-            if (turn) continue;
-            for (int t = 1; t < a.turns; t++) sum += part[t * each + lane];
-        }
-        T* const dweight = static_cast<T*>(a.dweight) + group * a.weights;
-        if (a.dweight && i + n <= a.weights) {
-            store_some<T, 4>(dweight + i, sum, n);
-            continue;
-        }
-        for (int e = 0; e < n; e++) {
-            if (i + e >= a.weights) static_cast<T*>(a.dbias)[group * (a.wanted - a.weights) + i + e - a.weights] = static_cast<T>(sum[e]);
-            else if (a.dweight) dweight[i + e] = static_cast<T>(sum[e]);
-        }
-    }
-}
-
-// ---- narrow layers ----------------------------------------------------------------------------------------
-//
-// Where the weight fits the LDS a layer is bound by its rows' bytes: each workgroup holds the weight there, as fragments in the
-// order of the lanes, and takes its share of all rows past it, `chunk` rows side by side (a group's end among them changes the
-// weight).
-
-// The group that has the row; every lane of the wave takes part.
-__device__ inline int group_of(const Groups& g, int64_t row) {
-    int k = 0;
-    if (g.ends)
-        for (int first = 0; first < g.groups; first += 64) {
-            const int e = first + static_cast<int>(threadIdx.x % 64);
-            k += __builtin_popcountll(__ballot(e < g.groups && g.end(e) <= row));
-        }
-    return __builtin_amdgcn_readfirstlane(k);
-}
-
-struct NarrowArgs {
-    const void *x, *weight, *bias;
-    int64_t x_stride;
-    Finish to;
-    int64_t in, out, chunk;
-    Groups groups;
-};
-
-// Fragments of a row of which the last may reach past its end: load_within without a branch, for rows of a fragment at least.
-template <class T, int K>
-struct RowLoad {
-    static constexpr int V = kPer<T>;
-    int64_t in;
-    int last, down;  // where the last fragment is read, and the bytes it moves down
-    bool small;
-    __device__ explicit RowLoad(int64_t n) : in(n) {
-        const int k = (2 * (K - 1) + static_cast<int>(threadIdx.x) % 64 / 32) * V;
-        small = n < V;
-        last = small ? 0 : min(k, static_cast<int>(n) - V);
-        down = (k - last) * static_cast<int>(sizeof(T));
-    }
-    __device__ void operator()(Frag<T> (&f)[K], const T* row) const {
-        const int half = threadIdx.x % 64 / 32;
-        if (small) {
-            f[0] = load_within(row, half * V, in);
-            return;
-        }
-#pragma unroll
-        for (int k = 0; k < K - 1; k++) f[k] = load_raw<V>(row + (2 * k + half) * V);
-        f[K - 1] = load_raw<V>(row + last);
-        if (in % (2 * V)) f[K - 1] = down < 16 ? moved_down<T>(f[K - 1], down) : Frag<T>(0);
-    }
-};
-
-// K steps of 32 bytes a row. A wave takes 32 rows at a time; the next 32 are on their way meanwhile.
-template <class T, int K>
-__global__ void __launch_bounds__(512) k_narrow_fwd(NarrowArgs a) {
-    constexpr int V = kPer<T>;
-    extern __shared__ __attribute__((aligned(128))) char lds[];
-    const int tiles = static_cast<int>((a.out + 32 * kUnitTiles<T> - 1) / (32 * kUnitTiles<T>)) * kUnitTiles<T>;
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, rows_at_once = blockDim.x / 2;
-    Frag<T>* const weights = reinterpret_cast<Frag<T>*>(lds);
-    float* const bias = reinterpret_cast<float*>(lds + tiles * K * 1024);
-    char* const mine = lds + tiles * (K * 1024 + 128) + wave * kUnitBytes<T>;
-    const RowLoad<T, K> load(a.in);
-    const T* const x = static_cast<const T*>(a.x);
-    const int64_t last = min(a.groups.rows, (blockIdx.x + int64_t{1}) * a.chunk);
-    for (int64_t first = blockIdx.x * a.chunk; first < last;) {
-        const int group = group_of(a.groups, first);
-        if (group >= a.groups.groups) {
-            for (int64_t r = first + threadIdx.x / 8; r < last; r += blockDim.x / 8)
-                for (int64_t c = threadIdx.x % 8 * 4; c < a.out; c += 32) clear4<T>(a.to, r, c);
-            return;
-        }
-        const int64_t stop = max(first + 1, min(last, a.groups.end(group)));  // (a row at least, whatever the ends are)
-        Frag<T> next[K];
-        int64_t base = first + wave * 32;
-        load(next, x + min(base + lane % 32, stop - 1) * a.x_stride);
-        __syncthreads();
-        const T* const w = static_cast<const T*>(a.weight) + group * a.in * a.out;
-        for (int i = threadIdx.x; i < tiles * K * 64; i += blockDim.x) {
-            const int n = i / 64 / K * 32 + i % 32;
-            weights[i] = n < a.out ? load_within(w + n * a.in, (2 * (i / 64 % K) + i % 64 / 32) * V, a.in) : Frag<T>(0);
-        }
-        for (int i = threadIdx.x; i < tiles * 32; i += blockDim.x)
-            bias[i] = a.bias && i < a.out ? static_cast<float>(static_cast<const T*>(a.bias)[group * a.out + i]) : 0.0f;
-        __syncthreads();
-        for (; base < stop; base += rows_at_once) {
-            Frag<T> now[K];
-#pragma unroll
-            for (int k = 0; k < K; k++) now[k] = next[k];
-            if (base + rows_at_once < stop) load(next, x + min(base + rows_at_once + lane % 32, stop - 1) * a.x_stride);
-            for (int t = 0; t < tiles; t += kUnitTiles<T>) {
-                Sums unit[kUnitTiles<T>];
-#pragma unroll
-                for (int u = 0; u < kUnitTiles<T>; u++) {
-#pragma unroll
-                    for (int q = 0; q < 4; q++) {
-                        const Floats<4> b = *reinterpret_cast<const Floats<4>*>(bias + (t + u) * 32 + 8 * q + lane / 32 * 4);
-#pragma unroll
-                        for (int e = 0; e < 4; e++) unit[u][4 * q + e] = b[e];
-                    }
-#pragma unroll
-                    for (int k = 0; k < K; k++) mma(unit[u], weights[((t + u) * K + k) * 64 + lane], now[k]);
-                }
-                finish_unit<T>(a.to, base, stop, t * 32, unit, mine);
-            }
-        }
-        first = stop;
-    }
-}
-
-struct NarrowBwdArgs {
-    const void *dy, *pre, *x, *weight;  // x: null where dweight is not wanted
-    int64_t dy_stride, pre_stride, x_stride;
-    Finish to;       // dx; its out may be null
-    float* partial;  // slabs of dweight and dbias, or null
-    int64_t size;    // of a slab
-    int64_t in, out, chunk;
-    Groups groups;
-    int act;
-};
-// Bytes between the lines of a block in LDS: `tiles` times 32 elements, and what puts four lines (floats: the lanes' lines)
-// into different banks.
-template <class T>
-constexpr int line_bytes(int tiles) { return tiles * 32 * static_cast<int>(sizeof(T)) + (sizeof(T) == 2 ? 32 : 16); }
-template <class T>
-constexpr int kBlockRows = 256 / static_cast<int>(sizeof(T));
-
-// The lane's fragment of a column of a block: the lines along it, step s of eight.
-template <class T, int Tiles>
-__device__ inline Frag<T> across_fragment(const char* block, int column, int s) {
-    constexpr int kLine = line_bytes<T>(Tiles);
-    const int lane = threadIdx.x % 64, half = lane / 32;
-    if constexpr (sizeof(T) == 4) {
-        Frag<T> f;
-#pragma unroll
-        for (int i = 0; i < 4; i++) f[i] = *reinterpret_cast<const float*>(block + (s * 8 + half * 4 + i) * kLine + (column + lane % 32) * 4);
-        return f;
-    } else {
-        using Four = short __attribute__((ext_vector_type(4)));
-        using Lds = __attribute__((address_space(3))) Four*;
-        const int group = lane % 16;
-        Four part[2];
-#pragma unroll
-        for (int j = 0; j < 2; j++)
-            part[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (Lds)(block + (s * 16 + half * 8 + j * 4 + group / 4) * kLine + (column + lane % 32 / 16 * 16 + group % 4 * 4) * 2));
-        return __builtin_bit_cast(Frag<T>, __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7));
-    }
-}
-
-// A thread's fragments of a block's rows, Tiles times 32 columns of them, on their way from memory.
-template <class T, int Tiles, int Threads>
-struct BlockPart {
-    static constexpr int V = kPer<T>, kLanes = Tiles * 32 / V, kLines = Threads / kLanes, N = kBlockRows<T> / kLines;
-    static_assert(Threads % kLanes == 0 && kBlockRows<T> % kLines == 0);
-    Frag<T> v[N];
-    static __device__ int chunk() { return threadIdx.x % kLanes; }
-    static __device__ int line(int i) { return threadIdx.x / kLanes + i * kLines; }
-    // Rows [first, stop), at most a block of them. (Of rows and chunks there are not others are read.)
-    __device__ void load(const void* from, int64_t stride, int64_t width, int64_t first, int64_t stop) {
-        const T* const base = static_cast<const T*>(from) + first * stride;
-        const int most = static_cast<int>(min(stop - 1 - first, int64_t{kBlockRows<T>}));
-        if (width % V == 0) {
-            const T* const at = base + min(int64_t{chunk()} * V, width - V);
-#pragma unroll
-            for (int i = 0; i < N; i++) v[i] = load_raw<V>(at + min(line(i), most) * stride);
-        } else {
-#pragma unroll
-            for (int i = 0; i < N; i++) v[i] = load_within(base + min(line(i), most) * stride, chunk() * V, width);
-        }
-    }
-};
-
-// All three gradients in one pass: a block of rows of dz and x lies in LDS, its products with the weight are dx's rows, and the
-// products of its columns with one another stay in registers over the rows of a group, tiles of 32 x 32 of dweight. The next
-// block is on its way meanwhile. Up to ZT tiles of 32 outputs and XT of 32 inputs.
-template <class T, int Waves, int ZT, int XT>
-__global__ void __launch_bounds__(Waves * 64) k_narrow_bwd(NarrowBwdArgs a) {
-    constexpr int V = kPer<T>, kRows = kBlockRows<T>, kThreads = Waves * 64;
-    constexpr int kSteps = ZT * static_cast<int>(sizeof(T)), kTiles = (ZT * XT + Waves - 1) / Waves, kZ = line_bytes<T>(ZT), kX = line_bytes<T>(XT);
-    static_assert(XT % kUnitTiles<T> == 0);
-    extern __shared__ __attribute__((aligned(128))) char lds[];
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-    const int nt = static_cast<int>((a.out + 31) / 32), kt = static_cast<int>((a.in + 31) / 32);
-    char *const dz = lds, *const xs = dz + kRows * kZ, *const mine = xs + kRows * kX + wave * kBareBytes<T>;
-    Frag<T>* const weights = reinterpret_cast<Frag<T>*>(xs + kRows * kX + Waves * kBareBytes<T>);
-    BlockPart<T, ZT, kThreads> dy, pre;
-    BlockPart<T, XT, kThreads> x;
-    const auto load = [&](int64_t first, int64_t stop) {
-        dy.load(a.dy, a.dy_stride, a.out, first, stop);
-        if (a.act) pre.load(a.pre, a.pre_stride, a.out, first, stop);
-        if (a.x) x.load(a.x, a.x_stride, a.in, first, stop);
-    };
-    const int zc = dy.chunk(), xc = x.chunk();
-    const int64_t last = min(a.groups.rows, (blockIdx.x + int64_t{1}) * a.chunk);
-    for (int64_t first = blockIdx.x * a.chunk; first < last;) {
-        const int group = group_of(a.groups, first);
-        if (group >= a.groups.groups) {
-            if (a.to.out)
-                for (int64_t r = first + threadIdx.x / 8; r < last; r += kThreads / 8)
-                    for (int64_t c = threadIdx.x % 8 * 4; c < a.in; c += 32) clear4<T>(a.to, r, c);
-            return;
-        }
-        const int64_t stop = max(first + 1, min(last, a.groups.end(group)));
-        load(first, stop);
-        __syncthreads();  // the group's before have been worked on
-        if (a.to.out) {
-            const T* const w = static_cast<const T*>(a.weight) + group * a.in * a.out;
-            for (int i = threadIdx.x; i < XT * kSteps * 64; i += kThreads) {
-                const int k = i / 64 / kSteps * 32 + i % 32, n = (2 * (i / 64 % kSteps) + i % 64 / 32) * V;
-                Frag<T> f(0);
-                if (k < a.in)
-#pragma unroll
-                    for (int e = 0; e < V; e++)
-                        if (n + e < a.out) f[e] = w[(n + e) * a.in + k];
-                weights[i] = f;
-            }
-        }
-        Sums sums[kTiles];
-        Floats<V> db(0.0f);
-#pragma unroll
-        for (int t = 0; t < kTiles; t++) sums[t] = Sums(0.0f);
-        for (int64_t block = first; block < stop; block += kRows) {
-            const int rows = static_cast<int>(min(stop - block, int64_t{kRows}));
-#pragma unroll
-            for (int i = 0; i < dy.N; i++) {
-                Floats<V> d = floats<T, V>(dy.v[i]);
-                if (a.act) through<T, V>(d, floats<T, V>(pre.v[i]), a.act);
-                if (dy.line(i) >= rows || zc * V >= a.out) d = Floats<V>(0.0f);
-                db += d;
-                *reinterpret_cast<Frag<T>*>(dz + dy.line(i) * kZ + zc * 16) = raw<T, V>(d);
-            }
-            if (a.x)
-#pragma unroll
-                for (int i = 0; i < x.N; i++)
-                    *reinterpret_cast<Frag<T>*>(xs + x.line(i) * kX + xc * 16) = x.line(i) < rows && xc * V < a.in ? x.v[i] : Frag<T>(0);
-            __syncthreads();
-            if (block + kRows < stop) load(block + kRows, stop);
-            if (a.to.out)
-                for (int i = wave; i < kRows / 32 * (XT / kUnitTiles<T>); i += Waves) {
-                    const int strip = i / (XT / kUnitTiles<T>) * 32, t = i % (XT / kUnitTiles<T>) * kUnitTiles<T>;
-                    if (strip >= rows) break;
-                    if (t >= kt) continue;
-                    Sums unit[kUnitTiles<T>];
-#pragma unroll
-                    for (int u = 0; u < kUnitTiles<T>; u++) unit[u] = Sums(0.0f);
-                    for (int s = 0; s < nt * static_cast<int>(sizeof(T)); s++) {
-                        const Frag<T> row = *reinterpret_cast<const Frag<T>*>(dz + (strip + lane % 32) * kZ + (2 * s + lane / 32) * 16);
-#pragma unroll
-                        for (int u = 0; u < kUnitTiles<T>; u++) mma(unit[u], weights[((t + u) * kSteps + s) * 64 + lane], row);
-                    }
-                    store_unit<T>(a.to, block + strip, stop, t * 32, unit, mine);
-                }
-            if (a.x)
-#pragma unroll
-                for (int i = 0; i < kTiles; i++) {
-                    const int t = wave + i * Waves;
-                    if (t / XT < nt && t % XT < kt)
-#pragma unroll
-                        for (int s = 0; s < 8; s++)
-                            mma(sums[i], across_fragment<T, XT>(xs, t % XT * 32, s), across_fragment<T, ZT>(dz, t / XT * 32, s));
-                }
-            __syncthreads();
-        }
-        if (a.partial) {
-            float* const slab = a.partial + (int64_t{blockIdx.x} + group) * a.size;
-#pragma unroll
-            for (int i = 0; i < kTiles; i++) {
-                const int t = wave + i * Waves;
-                const int64_t n = t / XT * 32 + lane % 32;
-                if (a.x && t % XT < kt && n < a.out)
-#pragma unroll
-                    for (int q = 0; q < 4; q++) {
-                        const int64_t k = t % XT * 32 + 8 * q + lane / 32 * 4;
-                        const Floats<4> v = {sums[i][4 * q], sums[i][4 * q + 1], sums[i][4 * q + 2], sums[i][4 * q + 3]};
-                        store_some<float, 4>(slab + n * a.in + k, v, static_cast<int>(max(int64_t{0}, min(a.in - k, int64_t{4}))));
-                    }
-            }
-            Floats<V>* const parts = reinterpret_cast<Floats<V>*>(lds);
-            static_assert(kThreads * sizeof(Floats<V>) <= kRows * (kZ + kX));
-            parts[threadIdx.x] = db;
-            __syncthreads();
-            if (static_cast<int>(threadIdx.x) < dy.kLanes && zc * V < a.out) {
-                for (int l = 1; l < dy.kLines; l++) db += parts[l * dy.kLanes + zc];
-                store_some<float, V>(slab + a.in * a.out + zc * V, db, static_cast<int>(min(a.out - zc * V, int64_t{V})));
-            }
-        }
-        first = stop;
-    }
-}
-
-// ---- dz = dy act'(pre), and its columns' sums ------------------------------------------------------------
-
-struct SlopeArgs {
-    const void *dy, *pre;
-    void* dz;            // [rows][dz_stride], or null
-    float* partial;      // [slots][cols], or null
-    void* dbias;
-    int64_t dy_stride, pre_stride, dz_stride, cols;
-    Groups groups;
-    int shift, act;
-};
-
-// A part of the rows and up to 256 vectors of columns a workgroup; `lanes` threads go along a row.
-template <class T>
-__global__ void __launch_bounds__(256) k_slope(SlopeArgs a, int lanes) {
-    constexpr int V = kPer<T>;
-    __shared__ Floats<V> sums[256];
-    const Part part = part_of(a.groups, blockIdx.x, a.shift);
-    if (part.group >= a.groups.groups || part.begin >= part.end) return;
-    const int64_t c = (int64_t{blockIdx.y} * lanes + threadIdx.x % lanes) * V;
-    Floats<V> sum(0.0f);
-    if (c < a.cols) {
-        const int n = static_cast<int>(min(a.cols - c, int64_t{V}));
-        for (int64_t r = part.begin + threadIdx.x / lanes; r < part.end; r += 256 / lanes) {
-            Floats<V> d = floats<T, V>(load_within(static_cast<const T*>(a.dy) + r * a.dy_stride, c, a.cols));
-            if (a.act) {
-                const Floats<V> z = floats<T, V>(load_within(static_cast<const T*>(a.pre) + r * a.pre_stride, c, a.cols));
-                through<T, V>(d, z, a.act);
-                if (a.dz) store_some<T, V>(static_cast<T*>(a.dz) + r * a.dz_stride + c, d, n);
-            }
-            sum += d;
-        }
-    }
-    if (!a.partial) return;
-    sums[threadIdx.x] = sum;
-    __syncthreads();
-    if (static_cast<int>(threadIdx.x) >= lanes || c >= a.cols) return;
-    for (int t = threadIdx.x + lanes; t < 256; t += lanes) sum += sums[t];
-    store_some<float, V>(a.partial + int64_t{blockIdx.x} * a.cols + c, sum, static_cast<int>(min(a.cols - c, int64_t{V})));
-}
-
-// A group's partial sums, added in order: sixteen columns a workgroup, as many threads a column.
-template <class T>
-__global__ void __launch_bounds__(256) k_slope_join(SlopeArgs a) {
-    __shared__ float part[16][17];
-    const int lane = threadIdx.x % 16, turn = threadIdx.x / 16;
-    const int64_t c = int64_t{blockIdx.x} * 16 + lane;
-    const int group = blockIdx.y;
-    const int64_t begin = a.groups.begin(group), end = a.groups.end(group), first = group + (begin >> a.shift);
-    const int64_t slabs = end > begin ? ((end - begin - 1) >> a.shift) + 1 : 0;
-    float sum = 0.0f;
-    if (c < a.cols)
-        for (int64_t s = turn; s < slabs; s += 16) sum += a.partial[(first + s) * a.cols + c];
-    part[turn][lane] = sum;
-    __syncthreads();
-    if (turn || c >= a.cols) return;
-    for (int t = 1; t < 16; t++) sum += part[t][lane];
-    static_cast<T*>(a.dbias)[group * a.cols + c] = static_cast<T>(sum);
-}
-
-// ---- plans ------------------------------------------------------------------------------------------------
-
-constexpr int64_t kManyTiles = 512;  // two workgroups for each unit
-int64_t columns_of(int side) { return side == 256 ? 256 : 128; }  // of a tile of so many rows
-int log2_up(int64_t n) {
-    int k = 0;
-    while ((int64_t{1} << k) < n) k++;
-    return k;
-}
-int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to; }
-
-// out[rows][cols] over `depth`, rows in groups: the tile's rows (of 128 columns), and how many parts the depth is split into.
-struct Plan {
-    int side, splits;
-    int64_t split, bytes;
-};
-Plan plan_rows(int64_t rows, int64_t cols, int64_t depth, int groups, bool ragged, int elem) {
-    Plan p{128, 1, 0, 0};
-    const auto tiles = [&](int side) { return slots_of(rows, groups, log2_up(side), ragged) * up(cols, columns_of(side)); };
-    if (tiles(256) >= 200 && cols > 128) p.side = 256;
-    else if (tiles(128) < kManyTiles) p.side = 64;
-    const int64_t step = 128 / elem, steps = up(depth, step);
-    if (p.side == 64) p.splits = static_cast<int>(std::max<int64_t>(1, std::min(kManyTiles / std::max<int64_t>(tiles(64), 1), steps / 4)));
-    const int64_t each = up(steps, p.splits);
-    p.split = each * step;
-    p.splits = static_cast<int>(std::max<int64_t>(1, up(steps, std::max<int64_t>(each, 1))));
-    p.bytes = p.splits > 1 ? p.splits * rows * cols * 4 : 0;
-    return p;
-}
-// out[groups][out][in] over the groups' rows: the tile's rows, and the parts of the rows (shift 62: each group's are one).
-struct Over {
-    int side, shift;
-    int64_t slots, bytes;
-};
-Over plan_over(int64_t rows, int64_t out, int64_t in, int groups, bool ragged) {
-    Over p{128, 62, groups, 0};
-    if (out <= 64) p.side = 64;
-    else if (up(out, 256) * up(in, 256) * groups >= 64 && out > 128 && in > 128) p.side = 256;
-    const int64_t tiles = up(out, p.side) * up(in, columns_of(p.side));
-    const int64_t wanted = std::max<int64_t>(1, (p.side == 256 ? kManyTiles : 2 * kManyTiles) / tiles);
-    const bool direct = tiles * groups >= kManyTiles && tiles >= 32;
-    const int shift = std::max(8, log2_up(up(std::max<int64_t>(rows, 1), wanted)));
-    if (!direct && rows > int64_t{1} << shift) {
-        p.shift = shift;
-        p.slots = slots_of(rows, groups, shift, ragged);
-        p.bytes = p.slots * out * in * 4;
-    }
-    return p;
-}
-struct Slope {
-    int shift, lanes;
-    int64_t slots, columns, bytes, dz_stride, dz_bytes;
-};
-Slope plan_slope(int64_t rows, int64_t cols, int groups, bool ragged, int elem) {
-    Slope p{};
-    const int64_t vectors = up(cols, 16 / elem);
-    p.lanes = 1 << std::min(8, log2_up(vectors));
-    p.columns = up(vectors, p.lanes);
-    p.shift = std::max({log2_up(256 / p.lanes), 4, log2_up(up(std::max<int64_t>(rows, 1), std::max<int64_t>(1, 2048 / p.columns)))});
-    p.slots = slots_of(rows, groups, p.shift, ragged);
-    p.bytes = p.slots * cols * 4;
-    p.dz_stride = vectors * (16 / elem);
-    p.dz_bytes = rows * p.dz_stride * elem;
-    return p;
-}
-
-constexpr int64_t kAlign = 256;
-int64_t aligned(int64_t bytes) { return (bytes + kAlign - 1) / kAlign * kAlign; }
-
-void check_grid(int64_t blocks, int64_t threads) {
-    if (blocks * threads >= int64_t{1} << 32) throw std::runtime_error("linear: more workgroups than a launch holds");
-}
-
-template <class T, bool RowAcross, bool ColAcross>
-void launch_tiles(const TileArgs& a, int side, int64_t slabs, hipStream_t s) {
-    const int64_t down = RowAcross ? up(a.rows, side) : a.slots, tiles = up(down * up(a.to.cols, columns_of(side)), 8) * 8;
-    check_grid(tiles * slabs, side == 256 ? 512 : 256);
-    const dim3 grid(static_cast<uint32_t>(tiles), static_cast<uint32_t>(slabs));
-    // straight into LDS: lines that begin on 16 bytes, and whose places in a tile 32 bits hold
-    const auto direct = [](const void* p, int64_t stride) {
-        return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * sizeof(T) % 16 == 0 && stride < (int64_t{1} << 30) / 256 / static_cast<int>(sizeof(T));
-    };
-    const bool whole = direct(a.row, a.row_stride) && direct(a.col, a.col_stride) && a.col_group * sizeof(T) % 16 == 0 &&
-                       (!RowAcross || a.rows % kPer<T> == 0) && (!ColAcross || a.to.cols % kPer<T> == 0);
-    if (side == 256 && whole) k_tile<T, 256, 256, 128, 64, RowAcross, ColAcross, true><<<grid, 512, 0, s>>>(a);
-    else if (side == 256) k_tile<T, 256, 256, 128, 64, RowAcross, ColAcross, false><<<grid, 512, 0, s>>>(a);
-    else if (side == 128 && whole) k_tile<T, 128, 128, 64, 64, RowAcross, ColAcross, true><<<grid, 256, 0, s>>>(a);
-    else if (side == 128) k_tile<T, 128, 128, 64, 64, RowAcross, ColAcross, false><<<grid, 256, 0, s>>>(a);
-    else if (whole) k_tile<T, 64, 128, 32, 64, RowAcross, ColAcross, true><<<grid, 256, 0, s>>>(a);
-    else k_tile<T, 64, 128, 32, 64, RowAcross, ColAcross, false><<<grid, 256, 0, s>>>(a);
-}
-
-// `slabs`: of a group, on average
-template <class T>
-void join_weights(JoinArgs a, int64_t slabs, hipStream_t s) {
-    a.turns = 1;
-    while (a.turns < 64 && a.turns * 4 <= slabs) a.turns *= 2;
-    const int64_t blocks = std::min<int64_t>(up(up(a.wanted, 4), 256 / a.turns), 65536);
-    k_weights_join<T><<<dim3(static_cast<uint32_t>(blocks), static_cast<uint32_t>(a.groups.groups)), 256, 0, s>>>(a);
-}
-
-// The steps of 32 bytes of a row that k_narrow_fwd is built for, or 0.
-int narrow_steps(int64_t in, int elem) {
-    for (const int k : {1, 2, 3, 4, 6, 8, 12, 16})
-        if (in * elem <= k * 32) return k;
-    return 0;
-}
-// A layer whose weight a workgroup holds: its LDS and workgroups, or none.
-struct Narrow {
-    int steps, threads, lds;
-    int64_t blocks, chunk;
-};
-template <class T>
-Narrow plan_narrow(int64_t rows, int64_t in, int64_t out) {
-    constexpr int elem = sizeof(T);
-    Narrow p{};
-    const int steps = narrow_steps(in, elem);
-    const int64_t tiles = elem == 4 ? up(out, 32) : up(out, 64) * 2, kib = tiles * steps;
-    if (!steps || kib > 112 || (rows < 4096 && kib > 16)) return p;
-    p.steps = steps;
-    p.threads = kib > 32 ? 512 : 256;
-    p.lds = static_cast<int>(kib * 1024 + tiles * 128) + p.threads / 64 * kUnitBytes<T>;
-    const int64_t each = std::max(1, std::min(p.threads == 512 ? 2 : 4, 160 * 1024 / p.lds));
-    p.blocks = std::max<int64_t>(1, std::min<int64_t>(256 * each, up(rows, p.threads / 2)));
-    p.chunk = up(up(rows, p.blocks), 32) * 32;
-    p.blocks = up(rows, p.chunk);
-    return p;
-}
-// A backward whose blocks of rows a workgroup holds.
-struct NarrowBwd {
-    int waves, zt, xt, lds;
-    int64_t blocks, chunk, size, bytes;
-};
-template <class T>
-NarrowBwd plan_narrow_bwd(int64_t rows, int64_t in, int64_t out, int groups) {
-    NarrowBwd p{};
-    const int64_t nt = up(out, 32), kt = up(in, 32);
-    if (nt <= 2 && kt <= 2) p.waves = 4, p.zt = p.xt = 2;
-    else if (nt <= 4 && kt <= 4) p.waves = 8, p.zt = p.xt = 4;
-    else if (nt <= 2 && kt <= 8) p.waves = 8, p.zt = 2, p.xt = 8;
-    else if (nt <= 8 && kt <= 2) p.waves = 8, p.zt = 8, p.xt = 2;
-    else return p;
-    p.lds = kBlockRows<T> * (line_bytes<T>(p.zt) + line_bytes<T>(p.xt)) + p.waves * kBareBytes<T> + p.zt * p.xt * static_cast<int>(sizeof(T)) * 1024;
-    if (p.lds > 160 * 1024) return {};
-    const int64_t each = std::max(1, std::min(2, 160 * 1024 / p.lds));
-    p.blocks = std::max<int64_t>(1, std::min<int64_t>(256 * each, up(rows, kBlockRows<T>)));
-    p.chunk = std::max<int64_t>(up(up(rows, p.blocks), 32) * 32, 32);
-    p.blocks = std::max<int64_t>(up(rows, p.chunk), 1);
-    p.size = in * out + out;
-    p.bytes = (p.blocks + groups) * p.size * 4;
-    return p;
-}
-template <class T>
-void launch_narrow_bwd(const NarrowBwdArgs& a, const NarrowBwd& p, hipStream_t s) {
-    const auto go = [&](auto kernel) { kernel<<<static_cast<uint32_t>(p.blocks), p.waves * 64, p.lds, s>>>(a); };
-    if (p.waves == 4) go(k_narrow_bwd<T, 4, 2, 2>);
-    else if (p.zt == 4) go(k_narrow_bwd<T, 8, 4, 4>);
-    else if (p.zt == 2) go(k_narrow_bwd<T, 8, 2, 8>);
-    else go(k_narrow_bwd<T, 8, 8, 2>);
-}
-
-template <class T>
-void launch_narrow(const NarrowArgs& a, const Narrow& p, hipStream_t s) {
-    const auto go = [&](auto kernel) { kernel<<<static_cast<uint32_t>(p.blocks), p.threads, p.lds, s>>>(a); };
-    switch (p.steps) {
-        case 1: return go(k_narrow_fwd<T, 1>);
-        case 2: return go(k_narrow_fwd<T, 2>);
-        case 3: return go(k_narrow_fwd<T, 3>);
-        case 4: return go(k_narrow_fwd<T, 4>);
-        case 6: return go(k_narrow_fwd<T, 6>);
-        case 8: return go(k_narrow_fwd<T, 8>);
-        case 12: return go(k_narrow_fwd<T, 12>);
-        default: return go(k_narrow_fwd<T, 16>);
-    }
-}
-
-// out = row col^T over the groups' rows (see TileArgs), with what follows.
-template <class T, bool ColAcross>
-void over_depth(TileArgs a, bool ragged, float* work, hipStream_t s) {
-    const Plan p = plan_rows(a.rows, a.to.cols, a.depth, a.groups.groups, ragged, sizeof(T));
-    a.shift = log2_up(p.side);
-    a.slots = slots_of(a.rows, a.groups.groups, a.shift, ragged);
-    a.split = p.split;
-    a.splits = p.splits;
-    a.partial = p.splits > 1 ? work : nullptr;
-    launch_tiles<T, false, ColAcross>(a, p.side, p.splits, s);
-    if (a.partial) {
-        const int64_t blocks = std::min<int64_t>(up(a.rows * up(a.to.cols, 4), 256), 4096);
-        k_split_join<T><<<static_cast<uint32_t>(blocks), 256, 0, s>>>(a);
-    }
-}
-
-template <class T>
-void forward(const LinearFwdArgs& f, hipStream_t s) {
-    const Finish to{f.y, f.y_stride, f.out, f.residual, f.residual_stride, f.pre, f.pre_stride, f.act, f.clear};
-    if (const Narrow p = plan_narrow<T>(f.rows, f.in, f.out); p.blocks) {
-        launch_narrow<T>({f.x, f.weight, f.bias, f.x_stride, to, f.in, f.out, p.chunk, {f.ends, f.groups, f.rows}}, p, s);
-        return;
-    }
-    TileArgs a{};
-    a.row = f.x; a.row_stride = f.x_stride; a.col = f.weight; a.col_stride = f.in; a.col_group = f.in * f.out;
-    a.rows = f.rows; a.depth = f.in;
-    a.groups = {f.ends, f.groups, f.rows};
-    a.bias = f.bias; a.bias_group = f.out;
-    a.to = to;
-    over_depth<T, false>(a, f.ends != nullptr, static_cast<float*>(f.workspace), s);
-}
-
-template <class T>
-void backward(const LinearBwdArgs& f, hipStream_t s) {
-    const bool ragged = f.ends != nullptr;
-    const Slope slope = plan_slope(f.rows, f.out, f.groups, ragged, sizeof(T));
-    const Groups groups{f.ends, f.groups, f.rows};
-    char* work = static_cast<char*>(f.workspace);
-    if (const NarrowBwd p = plan_narrow_bwd<T>(f.rows, f.in, f.out, f.groups); p.blocks) {
-        NarrowBwdArgs a{};
-        a.dy = f.dy; a.pre = f.pre; a.x = f.dweight ? f.x : nullptr; a.weight = f.weight;
-        a.dy_stride = f.dy_stride; a.pre_stride = f.pre_stride; a.x_stride = f.x_stride;
-        a.to.out = f.dx; a.to.out_stride = f.dx_stride; a.to.cols = f.in; a.to.clear = f.clear;
-        a.in = f.in; a.out = f.out; a.chunk = p.chunk; a.size = p.size; a.groups = groups; a.act = f.act;
-        const bool sums = f.dweight || f.dbias;
-        a.partial = sums ? reinterpret_cast<float*>(work) : nullptr;
-        if (f.rows) launch_narrow_bwd<T>(a, p, s);
-        if (sums) {
-            JoinArgs j{};
-            j.partial = a.partial; j.dweight = f.dweight; j.dbias = f.dbias; j.weights = f.in * f.out; j.size = p.size; j.wanted = f.dbias ? p.size : j.weights;
-            j.groups = groups; j.step = p.chunk;
-            join_weights<T>(j, p.blocks / f.groups + 1, s);
-        }
-        return;
-    }
-    const void* dz = f.dy;
-    int64_t dz_stride = f.dy_stride;
-    const bool products = f.dx || f.dweight;
-    if (f.dbias || (f.act && products)) {
-        SlopeArgs a{};
-        a.dy = f.dy; a.pre = f.pre; a.dy_stride = f.dy_stride; a.pre_stride = f.pre_stride;
-        a.cols = f.out; a.groups = groups; a.shift = slope.shift; a.act = f.act; a.dbias = f.dbias;
-        if (f.act && products) {
-            a.dz = work;
-            dz = work;
-            dz_stride = a.dz_stride = slope.dz_stride;
-        }
-        work += aligned(slope.dz_bytes);
-        if (f.dbias) a.partial = reinterpret_cast<float*>(work);
-        work += aligned(slope.bytes);
-        check_grid(slope.slots * slope.columns, 256);
-        if (f.rows)
-            k_slope<T><<<dim3(static_cast<uint32_t>(slope.slots), static_cast<uint32_t>(slope.columns)), 256, 0, s>>>(a, slope.lanes);
-        if (f.dbias) k_slope_join<T><<<dim3(static_cast<uint32_t>(up(f.out, 16)), static_cast<uint32_t>(f.groups)), 256, 0, s>>>(a);
-    }
-    if (f.dx && f.rows) {
-        TileArgs a{};
-        a.row = dz; a.row_stride = dz_stride; a.col = f.weight; a.col_stride = f.in; a.col_group = f.in * f.out;
-        a.to.out = f.dx; a.to.out_stride = f.dx_stride; a.to.cols = f.in; a.rows = f.rows; a.depth = f.out;
-        a.groups = groups; a.to.clear = f.clear;
-        over_depth<T, true>(a, ragged, reinterpret_cast<float*>(work), s);
-    }
-    if (f.dweight) {
-        const Over p = plan_over(f.rows, f.out, f.in, f.groups, ragged);
-        TileArgs a{};
-        a.row = dz; a.row_stride = dz_stride; a.col = f.x; a.col_stride = f.x_stride;
-        a.to.out = f.dweight; a.to.out_stride = f.in; a.to.cols = f.in; a.out_group = f.in * f.out; a.rows = f.out; a.depth = f.rows;
-        a.groups = groups; a.shift = p.shift; a.slots = p.slots;
-        a.partial = p.bytes ? reinterpret_cast<float*>(work) : nullptr;
-        launch_tiles<T, true, true>(a, p.side, p.slots, s);
-        if (a.partial) {
-            JoinArgs j{};
-            j.partial = a.partial; j.dweight = f.dweight; j.weights = j.wanted = j.size = f.in * f.out;
-            j.groups = groups; j.step = int64_t{1} << p.shift; j.from_begin = true;
-            join_weights<T>(j, p.slots / f.groups, s);
-        }
-    }
-}
-
 template <class F>
-void with_type(ElemType t, F&& f) {
-    if (t == kF32) f(float{});
-    else if (t == kBf16) f(__bf16{});
-    else f(_Float16{});
+auto with_type(ElemType t, F&& f) {
+    return t == kF32 ? f(float{}) : t == kBf16 ? f(__bf16{}) : f(_Float16{});
 }
-
 }  // namespace
 
 int64_t linear_fwd_workspace(int64_t rows, int64_t in, int64_t out, int groups, bool ragged, ElemType type) {
-    const int elem = type == kF32 ? 4 : 2;
-    return (elem == 4 ? plan_narrow<float>(rows, in, out) : plan_narrow<__bf16>(rows, in, out)).blocks ? 0 : plan_rows(rows, out, in, groups, ragged, elem).bytes;
+    return with_type(type, [&](auto t) { return linear_fwd_workspace_of<decltype(t)>(rows, in, out, groups, ragged); });
 }
 int64_t linear_bwd_workspace(int64_t rows, int64_t in, int64_t out, int groups, bool ragged, ElemType type) {
-    const int elem = type == kF32 ? 4 : 2;
-    const NarrowBwd narrow = elem == 4 ? plan_narrow_bwd<float>(rows, in, out, groups) : plan_narrow_bwd<__bf16>(rows, in, out, groups);
-    if (narrow.blocks) return narrow.bytes;
-    const Slope slope = plan_slope(rows, out, groups, ragged, elem);
-    return aligned(slope.dz_bytes) + aligned(slope.bytes) +
-           std::max(plan_rows(rows, in, out, groups, ragged, elem).bytes, plan_over(rows, out, in, groups, ragged).bytes);
+    return with_type(type, [&](auto t) { return linear_bwd_workspace_of<decltype(t)>(rows, in, out, groups, ragged); });
 }
 void linear_fwd(const LinearFwdArgs& a, ElemType type, hipStream_t s) {
-    with_type(type, [&](auto t) { forward<decltype(t)>(a, s); });
+    with_type(type, [&](auto t) { linear_fwd_of<decltype(t)>(a, s); });
 }
 void linear_bwd(const LinearBwdArgs& a, ElemType type, hipStream_t s) {
-    with_type(type, [&](auto t) { backward<decltype(t)>(a, s); });
+    with_type(type, [&](auto t) { linear_bwd_of<decltype(t)>(a, s); });
 }
 
 }  // namespace sxk

@@ -119,5 +119,14 @@ struct LinearBwdArgs {
 };
 int64_t linear_bwd_workspace(int64_t rows, int64_t in, int64_t out, int groups, bool ragged, ElemType type);
 void linear_bwd(const LinearBwdArgs& a, ElemType type, hipStream_t s);
+// The same for one type of elements (float, __bf16, _Float16).
+template <class T>
+int64_t linear_fwd_workspace_of(int64_t rows, int64_t in, int64_t out, int groups, bool ragged);
+template <class T>
+int64_t linear_bwd_workspace_of(int64_t rows, int64_t in, int64_t out, int groups, bool ragged);
+template <class T>
+void linear_fwd_of(const LinearFwdArgs& a, hipStream_t s);
+template <class T>
+void linear_bwd_of(const LinearBwdArgs& a, hipStream_t s);
 
 }  // namespace sxk
