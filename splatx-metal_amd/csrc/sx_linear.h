@@ -15,6 +15,28 @@ namespace sxk {
 using namespace sxd;
 namespace {
 
+// A barrier for what lies in LDS: unlike __syncthreads it does not wait for the wave's loads and stores of memory.
+__device__ inline void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+// What has been loaded is there from here on. Loads and stores of memory are counted together, so that a wait for loads that
+// comes after stores waits for these as well: the wait comes before them.
+template <class T, int N>
+__device__ inline void arrived(Vec<T, kPer<T>> (&v)[N]) {
+    using Words = uint32_t __attribute__((ext_vector_type(4)));
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        Words w = __builtin_bit_cast(Words, v[i]);
+        asm volatile("" : "+v"(w));
+        v[i] = __builtin_bit_cast(Frag<T>, w);
+    }
+}
+
+// The wave's number in its workgroup, known to be one for all its lanes.
+__device__ inline int wave_of() { return __builtin_amdgcn_readfirstlane(threadIdx.x / 64); }
+
 // ---- tiles ------------------------------------------------------------------------------------------------
 //
 // out[r][c] = sum over d of row(r, d) col(c, d): x W^T, dz W and dz^T x, each operand either with its sums' elements side by
@@ -128,7 +150,7 @@ struct DirectStage {
         using Lds = __attribute__((address_space(3))) void*;
 #pragma unroll
         for (int i = 0; i < N; i++)
-            __builtin_amdgcn_global_load_lds((Global)(base + offset[i]), (Lds)(lds + (i * Threads + __builtin_amdgcn_readfirstlane(threadIdx.x / 64 * 64)) * 16), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((Global)(base + offset[i]), (Lds)(lds + (i * Threads + wave_of() * 64) * 16), 16, 0, 0);
         base += step;
     }
 };
@@ -227,46 +249,64 @@ __device__ inline void store_chunk(T* p, Floats<kPer<T>> f, int n) {
         if (e < n) p[e] = v[e];
 }
 
-// 32 rows from r on (those before `stop`) and the columns [c, c + 128 bytes), the sums' bias included. Every lane takes part.
+// 32 rows from r on (those before `stop`) and the columns [c, c + 128 bytes). Every lane takes part.
 template <class T>
-__device__ inline void finish_unit(const Finish& a, int64_t r, int64_t stop, int64_t c, const Sums (&sums)[kUnitTiles<T>], char* lds) {
-    constexpr int V = kPer<T>;
-    const int lane = threadIdx.x % 64;
-    wave_sees();  // (what was there has been read)
+struct Unit {
+    static constexpr int V = kPer<T>;
+    const Finish& a;
+    int64_t r, c;
+    int column, row, n, rows;
+    Frag<T> residual[4];
+
+    __device__ Unit(const Finish& f, int64_t first, int64_t stop, int64_t col) : a(f), r(first), c(col) {
+        column = threadIdx.x % 8 * V;
+        row = threadIdx.x % 64 / 8;
+        n = static_cast<int>(max(int64_t{0}, min(a.cols - c - column, int64_t{V})));
+        rows = static_cast<int>(min(stop - r, int64_t{32}));
+        if (a.residual)
 #pragma unroll
-    for (int u = 0; u < kUnitTiles<T>; u++)
-#pragma unroll
-        for (int q = 0; q < 4; q++)
-            *reinterpret_cast<Floats<4>*>(lds + lane % 32 * kUnitLine<T> + lane / 32 * 16 + u * 128 + q * 32) =
-                Floats<4>{sums[u][4 * q], sums[u][4 * q + 1], sums[u][4 * q + 2], sums[u][4 * q + 3]};
-    wave_sees();
-    const int64_t column = c + lane % 8 * V;
-    const int n = static_cast<int>(max(int64_t{0}, min(a.cols - column, int64_t{V})));
-    const int rows = static_cast<int>(min(stop - r, int64_t{32}));
-    const char* from = lds + lane / 8 * kUnitLine<T> + lane % 8 * (V * 4);
-    r += lane / 8;
-    Frag<T> residual(0);
-    const auto load_residual = [&](int row, int64_t at) {
-        if (a.residual && row < rows) residual = load_within(static_cast<const T*>(a.residual) + at * a.residual_stride, column, a.cols);
-    };
-    load_residual(lane / 8, r);
-#pragma unroll 1
-    for (int row = lane / 8; row < rows; row += 8, r += 8, from += 8 * kUnitLine<T>) {
-        Floats<V> v;
-#pragma unroll
-        for (int e = 0; e < V; e += 4) {
-            const Floats<4> f = *reinterpret_cast<const Floats<4>*>(from + e * 4);
-            v[e] = f[0]; v[e + 1] = f[1]; v[e + 2] = f[2]; v[e + 3] = f[3];
-        }
-        if (a.pre) store_chunk(static_cast<T*>(a.pre) + r * a.pre_stride + column, v, n);
-        activate<T, V>(v, a.act);
-        if (a.residual) {
-            v += floats<T, V>(residual);
-            load_residual(row + 8, r + 8);
-        }
-        store_chunk(static_cast<T*>(a.out) + r * a.out_stride + column, v, n);
+            for (int i = 0; i < 4; i++) {
+                const T* const p = static_cast<const T*>(a.residual) + (r * a.residual_stride + c) + min(row + 8 * i, rows - 1) * a.residual_stride;
+                residual[i] = a.cols - c >= 8 * V ? load_raw<V>(p + column) : load_within(p, column, a.cols - c);
+            }
     }
-}
+    // (what all lanes share is added apart from what a lane has of its own, which stays over the units)
+    template <class P>
+    __device__ P* at(P* p, int64_t stride) const { return p + (r * stride + c) + (row * stride + column); }
+
+    // The sums, bias included, through the wave's LDS.
+    __device__ void finish(const Sums (&sums)[kUnitTiles<T>], char* lds) const {
+        const int lane = threadIdx.x % 64;
+        wave_sees();  // (what was there has been read)
+#pragma unroll
+        for (int u = 0; u < kUnitTiles<T>; u++)
+#pragma unroll
+            for (int q = 0; q < 4; q++)
+                *reinterpret_cast<Floats<4>*>(lds + lane % 32 * kUnitLine<T> + lane / 32 * 16 + u * 128 + q * 32) =
+                    Floats<4>{sums[u][4 * q], sums[u][4 * q + 1], sums[u][4 * q + 2], sums[u][4 * q + 3]};
+        wave_sees();
+        T* out = at(static_cast<T*>(a.out), a.out_stride);
+        T* pre = a.pre ? at(static_cast<T*>(a.pre), a.pre_stride) : nullptr;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            Floats<V> v;
+#pragma unroll
+            for (int e = 0; e < V; e += 4) {
+                const Floats<4> f = *reinterpret_cast<const Floats<4>*>(lds + (row + 8 * i) * kUnitLine<T> + column * 4 + e * 4);
+                v[e] = f[0]; v[e + 1] = f[1]; v[e + 2] = f[2]; v[e + 3] = f[3];
+            }
+            if (a.pre) {
+                if (row + 8 * i < rows) store_chunk(pre, v, n);
+                pre += 8 * a.pre_stride;
+            }
+            activate<T, V>(v, a.act);
+            if (a.residual) v += floats<T, V>(residual[i]);
+            if (row + 8 * i < rows) store_chunk(out, v, n);
+            out += 8 * a.out_stride;
+            __builtin_amdgcn_sched_barrier(0);  // (one after another: their registers together would cost waves)
+        }
+    }
+};
 
 // The same of sums that are the outputs, through half the LDS.
 template <class T>
@@ -285,13 +325,14 @@ __device__ inline void store_unit(const Finish& a, int64_t r, int64_t stop, int6
             *reinterpret_cast<Vec<T, 4>*>(lds + lane % 32 * kBareLine<T> + (u * 32 + 8 * q + lane / 32 * 4) * static_cast<int>(sizeof(T))) =
                 raw<T, 4>(Floats<4>{sums[u][4 * q], sums[u][4 * q + 1], sums[u][4 * q + 2], sums[u][4 * q + 3]});
     wave_sees();
-    const int64_t column = c + lane % 8 * V;
-    const int n = static_cast<int>(max(int64_t{0}, min(a.cols - column, int64_t{V})));
+    const int column = lane % 8 * V, row = lane / 8;
+    const int n = static_cast<int>(max(int64_t{0}, min(a.cols - c - column, int64_t{V})));
+    const int rows = static_cast<int>(min(stop - r, int64_t{32}));
+    T* p = static_cast<T*>(a.out) + (r * a.out_stride + c) + (row * a.out_stride + column);
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const Frag<T> v = *reinterpret_cast<const Frag<T>*>(lds + (lane / 8 + i * 8) * kBareLine<T> + lane % 8 * 16);
-        T* const p = static_cast<T*>(a.out) + (r + lane / 8 + i * 8) * a.out_stride + column;
-        if (r + lane / 8 + i * 8 >= stop) continue;
+    for (int i = 0; i < 32; i += 8, p += 8 * a.out_stride) {
+        const Frag<T> v = *reinterpret_cast<const Frag<T>*>(lds + (row + i) * kBareLine<T> + lane % 8 * 16);
+        if (row + i >= rows) continue;
         if (n == V) store_raw<V>(p, v);
         else
 #pragma unroll
@@ -332,7 +373,7 @@ __global__ void __launch_bounds__(BR / WR * (BC / WC) * 64) k_tile(TileArgs a) {
         d1 = min(a.depth, d0 + a.split);
         if (r0 >= r1) return;
     }
-    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+    const int wave = wave_of(), lane = threadIdx.x % 64;
     const int wr = wave / (BC / WC) * WR, wc = wave % (BC / WC) * WC;
     if (!OverRows && part.group >= a.groups.groups) {
         if (a.partial) return;
@@ -490,7 +531,7 @@ __global__ void __launch_bounds__(BR / WR * (BC / WC) * 64) k_tile(TileArgs a) {
             }
             if (a.partial) continue;
             if constexpr (ColAcross) store_unit<T>(to, r, r1, c, unit, mine);
-            else finish_unit<T>(to, r, r1, c, unit, mine);
+            else Unit<T>(to, r, r1, c).finish(unit, mine);
         }
     }
 }
@@ -627,7 +668,7 @@ __global__ void __launch_bounds__(512) k_narrow_fwd(NarrowArgs a) {
     constexpr int V = kPer<T>;
     extern __shared__ __attribute__((aligned(128))) char lds[];
     const int tiles = static_cast<int>((a.out + 32 * kUnitTiles<T> - 1) / (32 * kUnitTiles<T>)) * kUnitTiles<T>;
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, rows_at_once = blockDim.x / 2;
+    const int lane = threadIdx.x % 64, wave = wave_of(), rows_at_once = blockDim.x / 2;
     Frag<T>* const weights = reinterpret_cast<Frag<T>*>(lds);
     float* const bias = reinterpret_cast<float*>(lds + tiles * K * 1024);
     char* const mine = lds + tiles * (K * 1024 + 128) + wave * kUnitBytes<T>;
@@ -645,7 +686,7 @@ __global__ void __launch_bounds__(512) k_narrow_fwd(NarrowArgs a) {
         Frag<T> next[K];
         int64_t base = first + wave * 32;
         load(next, x + min(base + lane % 32, stop - 1) * a.x_stride);
-        __syncthreads();
+        lds_barrier();
         const T* const w = static_cast<const T*>(a.weight) + group * a.in * a.out;
         for (int i = threadIdx.x; i < tiles * K * 64; i += blockDim.x) {
             const int n = i / 64 / K * 32 + i % 32;
@@ -653,13 +694,15 @@ __global__ void __launch_bounds__(512) k_narrow_fwd(NarrowArgs a) {
         }
         for (int i = threadIdx.x; i < tiles * 32; i += blockDim.x)
             bias[i] = a.bias && i < a.out ? static_cast<float>(static_cast<const T*>(a.bias)[group * a.out + i]) : 0.0f;
-        __syncthreads();
+        lds_barrier();
         for (; base < stop; base += rows_at_once) {
             Frag<T> now[K];
 #pragma unroll
             for (int k = 0; k < K; k++) now[k] = next[k];
-            if (base + rows_at_once < stop) load(next, x + min(base + rows_at_once + lane % 32, stop - 1) * a.x_stride);
+            const bool more = base + rows_at_once < stop;
+            if (more) load(next, x + min(base + rows_at_once + lane % 32, stop - 1) * a.x_stride);
             for (int t = 0; t < tiles; t += kUnitTiles<T>) {
+                Unit<T> to(a.to, base, stop, t * 32);
                 Sums unit[kUnitTiles<T>];
 #pragma unroll
                 for (int u = 0; u < kUnitTiles<T>; u++) {
@@ -672,7 +715,9 @@ __global__ void __launch_bounds__(512) k_narrow_fwd(NarrowArgs a) {
 #pragma unroll
                     for (int k = 0; k < K; k++) mma(unit[u], weights[((t + u) * K + k) * 64 + lane], now[k]);
                 }
-                finish_unit<T>(a.to, base, stop, t * 32, unit, mine);
+                if (t == 0) arrived<T>(next);
+                if (a.to.residual) arrived<T>(to.residual);
+                to.finish(unit, mine);
             }
         }
         first = stop;
@@ -751,7 +796,7 @@ __global__ void __launch_bounds__(Waves * 64) k_narrow_bwd(NarrowBwdArgs a) {
     constexpr int kSteps = ZT * static_cast<int>(sizeof(T)), kTiles = (ZT * XT + Waves - 1) / Waves, kZ = line_bytes<T>(ZT), kX = line_bytes<T>(XT);
     static_assert(XT % kUnitTiles<T> == 0);
     extern __shared__ __attribute__((aligned(128))) char lds[];
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    const int lane = threadIdx.x % 64, wave = wave_of();
     const int nt = static_cast<int>((a.out + 31) / 32), kt = static_cast<int>((a.in + 31) / 32);
     char *const dz = lds, *const xs = dz + kRows * kZ, *const mine = xs + kRows * kX + wave * kBareBytes<T>;
     Frag<T>* const weights = reinterpret_cast<Frag<T>*>(xs + kRows * kX + Waves * kBareBytes<T>);
@@ -774,7 +819,7 @@ __global__ void __launch_bounds__(Waves * 64) k_narrow_bwd(NarrowBwdArgs a) {
         }
         const int64_t stop = max(first + 1, min(last, a.groups.end(group)));
         load(first, stop);
-        __syncthreads();  // the group's before have been worked on
+        lds_barrier();  // the group's before have been worked on
         if (a.to.out) {
             const T* const w = static_cast<const T*>(a.weight) + group * a.in * a.out;
             for (int i = threadIdx.x; i < XT * kSteps * 64; i += kThreads) {
@@ -805,8 +850,17 @@ __global__ void __launch_bounds__(Waves * 64) k_narrow_bwd(NarrowBwdArgs a) {
 #pragma unroll
                 for (int i = 0; i < x.N; i++)
                     *reinterpret_cast<Frag<T>*>(xs + x.line(i) * kX + xc * 16) = x.line(i) < rows && xc * V < a.in ? x.v[i] : Frag<T>(0);
-            __syncthreads();
+            lds_barrier();
             if (block + kRows < stop) load(block + kRows, stop);
+            if (a.x)
+#pragma unroll
+                for (int i = 0; i < kTiles; i++) {
+                    const int t = wave + i * Waves;
+                    if (t / XT < nt && t % XT < kt)
+#pragma unroll
+                        for (int s = 0; s < 8; s++)
+                            mma(sums[i], across_fragment<T, XT>(xs, t % XT * 32, s), across_fragment<T, ZT>(dz, t / XT * 32, s));
+                }
             if (a.to.out)
                 for (int i = wave; i < kRows / 32 * (XT / kUnitTiles<T>); i += Waves) {
                     const int strip = i / (XT / kUnitTiles<T>) * 32, t = i % (XT / kUnitTiles<T>) * kUnitTiles<T>;
@@ -820,18 +874,14 @@ __global__ void __launch_bounds__(Waves * 64) k_narrow_bwd(NarrowBwdArgs a) {
 #pragma unroll
                         for (int u = 0; u < kUnitTiles<T>; u++) mma(unit[u], weights[((t + u) * kSteps + s) * 64 + lane], row);
                     }
+                    if (i == wave) {  // before the first stores
+                        arrived<T>(dy.v);
+                        if (a.act) arrived<T>(pre.v);
+                        if (a.x) arrived<T>(x.v);
+                    }
                     store_unit<T>(a.to, block + strip, stop, t * 32, unit, mine);
                 }
-            if (a.x)
-#pragma unroll
-                for (int i = 0; i < kTiles; i++) {
-                    const int t = wave + i * Waves;
-                    if (t / XT < nt && t % XT < kt)
-#pragma unroll
-                        for (int s = 0; s < 8; s++)
-                            mma(sums[i], across_fragment<T, XT>(xs, t % XT * 32, s), across_fragment<T, ZT>(dz, t / XT * 32, s));
-                }
-            __syncthreads();
+            lds_barrier();
         }
         if (a.partial) {
             float* const slab = a.partial + (int64_t{blockIdx.x} + group) * a.size;
@@ -850,7 +900,7 @@ __global__ void __launch_bounds__(Waves * 64) k_narrow_bwd(NarrowBwdArgs a) {
             Floats<V>* const parts = reinterpret_cast<Floats<V>*>(lds);
             static_assert(kThreads * sizeof(Floats<V>) <= kRows * (kZ + kX));
             parts[threadIdx.x] = db;
-            __syncthreads();
+            lds_barrier();
             if (static_cast<int>(threadIdx.x) < dy.kLanes && zc * V < a.out) {
                 for (int l = 1; l < dy.kLines; l++) db += parts[l * dy.kLanes + zc];
                 store_some<float, V>(slab + a.in * a.out + zc * V, db, static_cast<int>(min(a.out - zc * V, int64_t{V})));

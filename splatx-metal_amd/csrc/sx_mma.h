@@ -56,11 +56,11 @@ __device__ inline Frag<T> load_within(const T* row, int64_t k, int64_t n) {
 
 enum Act : int { kNone = 0, kRelu = 1, kGelu = 2, kSilu = 3, kSigmoid = 4 };
 
-// e^(-x) of the types: 16-bit outputs take the hardware's exponential and reciprocal (2^-22 and the argument's rounding).
+// e^(-x scale) of the types: 16-bit outputs take the hardware's exponential and reciprocal (2^-22 and the argument's rounding).
 template <class T>
-__device__ inline float exp_minus(float x) {
-    if constexpr (sizeof(T) == 4) return expf(-x);
-    return __builtin_amdgcn_exp2f(x * -1.44269504f);
+__device__ inline float exp_minus(float x, float scale = 1.0f) {
+    if constexpr (sizeof(T) == 4) return expf(-x * scale);
+    return __builtin_amdgcn_exp2f(x * (-1.44269504f * scale));
 }
 template <class T>
 __device__ inline float inverse(float x) {
@@ -74,7 +74,7 @@ __device__ inline float inverse(float x) {
 // keeps its relative precision.
 template <class T>
 __device__ inline float lower_tail(float z, float* density) {
-    const float a = fabsf(z), e = exp_minus<T>(0.5f * a * a);
+    const float a = fabsf(z), e = exp_minus<T>(z * z, 0.5f);
     *density = e;
     if constexpr (sizeof(T) == 4) return 0.5f * erfcf(a * 0.707106781f);
     const float t = inverse<T>(__builtin_fmaf(0.33f, a, 1.0f));
