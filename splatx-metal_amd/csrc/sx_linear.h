@@ -573,6 +573,7 @@ struct JoinArgs {
     Groups groups;
     int64_t step;
     bool from_begin;
+    int64_t slabs;  // without groups; else 0
     int turns;
 };
 template <class T>
@@ -580,7 +581,7 @@ __global__ void __launch_bounds__(256) k_weights_join(JoinArgs a) {
     __shared__ Floats<4> part[256];
     const int each = 256 / a.turns, lane = threadIdx.x % each, turn = threadIdx.x / each, group = blockIdx.y;
     const int64_t begin = a.groups.begin(group), end = a.groups.end(group), first = group + begin / a.step;
-    const int64_t slabs = end > begin ? (end - 1 - (a.from_begin ? begin : 0)) / a.step - (a.from_begin ? 0 : begin / a.step) + 1 : 0;
+    const int64_t slabs = a.slabs ? a.slabs : end > begin ? (end - 1 - (a.from_begin ? begin : 0)) / a.step - (a.from_begin ? 0 : begin / a.step) + 1 : 0;
     for (int64_t at = int64_t{blockIdx.x} * each; at * 4 < a.wanted; at += int64_t{gridDim.x} * each) {
         const int64_t i = (at + lane) * 4;
         const int n = static_cast<int>(max(int64_t{0}, min(a.wanted - i, int64_t{4})));
@@ -674,8 +675,11 @@ __global__ void __launch_bounds__(512) k_narrow_fwd(NarrowArgs a) {
     char* const mine = lds + tiles * (K * 1024 + 128) + wave * kUnitBytes<T>;
     const RowLoad<T, K> load(a.in);
     const T* const x = static_cast<const T*>(a.x);
-    const int64_t last = min(a.groups.rows, (blockIdx.x + int64_t{1}) * a.chunk);
-    for (int64_t first = blockIdx.x * a.chunk; first < last;) {
+    // without groups the workgroups' rows lie between each other's, so that all work in one place of memory at a time
+    const bool grouped = a.groups.ends;
+    const int64_t last = grouped ? min(a.groups.rows, (blockIdx.x + int64_t{1}) * a.chunk) : a.groups.rows;
+    const int64_t step = grouped ? rows_at_once : int64_t{gridDim.x} * rows_at_once;
+    for (int64_t first = blockIdx.x * (grouped ? a.chunk : rows_at_once); first < last;) {
         const int group = group_of(a.groups, first);
         if (group >= a.groups.groups) {
             for (int64_t r = first + threadIdx.x / 8; r < last; r += blockDim.x / 8)
@@ -695,12 +699,11 @@ __global__ void __launch_bounds__(512) k_narrow_fwd(NarrowArgs a) {
         for (int i = threadIdx.x; i < tiles * 32; i += blockDim.x)
             bias[i] = a.bias && i < a.out ? static_cast<float>(static_cast<const T*>(a.bias)[group * a.out + i]) : 0.0f;
         lds_barrier();
-        for (; base < stop; base += rows_at_once) {
+        for (; base < stop; base += step) {
             Frag<T> now[K];
 #pragma unroll
             for (int k = 0; k < K; k++) now[k] = next[k];
-            const bool more = base + rows_at_once < stop;
-            if (more) load(next, x + min(base + rows_at_once + lane % 32, stop - 1) * a.x_stride);
+            if (base + step < stop) load(next, x + min(base + step + lane % 32, stop - 1) * a.x_stride);
             for (int t = 0; t < tiles; t += kUnitTiles<T>) {
                 Unit<T> to(a.to, base, stop, t * 32);
                 Sums unit[kUnitTiles<T>];
@@ -808,8 +811,10 @@ __global__ void __launch_bounds__(Waves * 64) k_narrow_bwd(NarrowBwdArgs a) {
         if (a.x) x.load(a.x, a.x_stride, a.in, first, stop);
     };
     const int zc = dy.chunk(), xc = x.chunk();
-    const int64_t last = min(a.groups.rows, (blockIdx.x + int64_t{1}) * a.chunk);
-    for (int64_t first = blockIdx.x * a.chunk; first < last;) {
+    const bool grouped = a.groups.ends;
+    const int64_t last = grouped ? min(a.groups.rows, (blockIdx.x + int64_t{1}) * a.chunk) : a.groups.rows;
+    const int64_t step = grouped ? kRows : int64_t{gridDim.x} * kRows;
+    for (int64_t first = blockIdx.x * (grouped ? a.chunk : kRows); first < last;) {
         const int group = group_of(a.groups, first);
         if (group >= a.groups.groups) {
             if (a.to.out)
@@ -836,7 +841,7 @@ __global__ void __launch_bounds__(Waves * 64) k_narrow_bwd(NarrowBwdArgs a) {
         Floats<V> db(0.0f);
 #pragma unroll
         for (int t = 0; t < kTiles; t++) sums[t] = Sums(0.0f);
-        for (int64_t block = first; block < stop; block += kRows) {
+        for (int64_t block = first; block < stop; block += step) {
             const int rows = static_cast<int>(min(stop - block, int64_t{kRows}));
 #pragma unroll
             for (int i = 0; i < dy.N; i++) {
@@ -851,7 +856,7 @@ __global__ void __launch_bounds__(Waves * 64) k_narrow_bwd(NarrowBwdArgs a) {
                 for (int i = 0; i < x.N; i++)
                     *reinterpret_cast<Frag<T>*>(xs + x.line(i) * kX + xc * 16) = x.line(i) < rows && xc * V < a.in ? x.v[i] : Frag<T>(0);
             lds_barrier();
-            if (block + kRows < stop) load(block + kRows, stop);
+            if (block + step < stop) load(block + step, stop);
             if (a.x)
 #pragma unroll
                 for (int i = 0; i < kTiles; i++) {
@@ -1110,7 +1115,7 @@ struct Narrow {
     int64_t blocks, chunk;
 };
 template <class T>
-Narrow plan_narrow(int64_t rows, int64_t in, int64_t out) {
+Narrow plan_narrow(int64_t rows, int64_t in, int64_t out, bool ragged) {
     constexpr int elem = sizeof(T);
     Narrow p{};
     const int steps = narrow_steps(in, elem);
@@ -1119,7 +1124,9 @@ Narrow plan_narrow(int64_t rows, int64_t in, int64_t out) {
     p.steps = steps;
     p.threads = kib > 32 ? 512 : 256;
     p.lds = static_cast<int>(kib * 1024 + tiles * 128) + p.threads / 64 * kUnitBytes<T>;
-    const int64_t each = std::max(1, std::min(p.threads == 512 ? 2 : 4, 160 * 1024 / p.lds));
+    // with groups more workgroups than run at once: the rows worked on at a time lie closer together (1 M rows of 64 in 200 groups,
+    // 3 for each unit 90 us, 8 86)
+    const int64_t each = ragged ? 8 : std::max(1, std::min(p.threads == 512 ? 2 : 4, 160 * 1024 / p.lds));
     p.blocks = std::max<int64_t>(1, std::min<int64_t>(256 * each, up(rows, p.threads / 2)));
     p.chunk = std::max<int64_t>(up(up(rows, p.blocks), 32) * 32, 32);
     p.blocks = std::max<int64_t>(up(rows, p.chunk), 1);
@@ -1195,7 +1202,7 @@ void over_depth(TileArgs a, bool ragged, float* work, hipStream_t s) {
 template <class T>
 void forward(const LinearFwdArgs& f, hipStream_t s) {
     const Finish to{f.y, f.y_stride, f.out, f.residual, f.residual_stride, f.pre, f.pre_stride, f.act, f.clear};
-    if (const Narrow p = plan_narrow<T>(f.rows, f.in, f.out); p.blocks) {
+    if (const Narrow p = plan_narrow<T>(f.rows, f.in, f.out, f.ends != nullptr); p.blocks) {
         launch_narrow<T>({f.x, f.weight, f.bias, f.x_stride, to, f.in, f.out, p.chunk, {f.ends, f.groups, f.rows}}, p, s);
         return;
     }
@@ -1226,7 +1233,7 @@ void backward(const LinearBwdArgs& f, hipStream_t s) {
         if (sums) {
             JoinArgs j{};
             j.partial = a.partial; j.dweight = f.dweight; j.dbias = f.dbias; j.weights = f.in * f.out; j.size = p.size; j.wanted = f.dbias ? p.size : j.weights;
-            j.groups = groups; j.step = p.chunk;
+            j.groups = groups; j.step = p.chunk; j.slabs = ragged || !f.rows ? 0 : p.blocks;
             join_weights<T>(j, p.blocks / f.groups + 1, s);
         }
         return;
@@ -1282,7 +1289,7 @@ void backward(const LinearBwdArgs& f, hipStream_t s) {
 
 template <class T>
 int64_t forward_workspace(int64_t rows, int64_t in, int64_t out, int groups, bool ragged) {
-    return plan_narrow<T>(rows, in, out).blocks ? 0 : plan_rows(rows, out, in, groups, ragged, sizeof(T)).bytes;
+    return plan_narrow<T>(rows, in, out, ragged).blocks ? 0 : plan_rows(rows, out, in, groups, ragged, sizeof(T)).bytes;
 }
 template <class T>
 int64_t backward_workspace(int64_t rows, int64_t in, int64_t out, int groups, bool ragged) {
