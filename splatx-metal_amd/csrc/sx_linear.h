@@ -915,6 +915,66 @@ __global__ void __launch_bounds__(Waves * 64) k_narrow_bwd(NarrowBwdArgs a) {
     }
 }
 
+// ---- few rows ---------------------------------------------------------------------------------------------
+//
+// A layer of few rows is bound by its weight's bytes: each is read once, by a workgroup of 32 outputs whose waves share the sums'
+// length, 128 bytes of each weight's row at a time in turn, several on their way; their sums are added in LDS. (9 rows of
+// 2048 to 8192 in half precision: 10 us by tiles with the length in parts, and 5 us to join them.)
+struct FewArgs {
+    const void *x, *weight, *bias;
+    int64_t x_stride;
+    Finish to;
+    int64_t in, out;
+    Groups groups;
+};
+constexpr int kFewWaves = 8, kFewShift = 5;  // a part: 32 rows
+template <class T>
+__global__ void __launch_bounds__(kFewWaves * 64) k_few_fwd(FewArgs a) {
+    constexpr int V = kPer<T>, kLine = 128 / static_cast<int>(sizeof(T)), kAtOnce = 2, kPitch = 36;
+    __shared__ float sums[kFewWaves][32 * kPitch];
+    const Part part = part_of(a.groups, blockIdx.y, kFewShift);
+    if (part.begin >= part.end) return;
+    const int64_t c0 = int64_t{blockIdx.x} * 32;
+    const int lane = threadIdx.x % 64, half = lane / 32, wave = wave_of();
+    // (in the end a thread of the first half has four outputs)
+    const int64_t r = part.begin + threadIdx.x / 8, c = c0 + threadIdx.x % 8 * 4;
+    if (part.group >= a.groups.groups) {
+        if (threadIdx.x < 256 && r < part.end) clear4<T>(a.to, r, c);
+        return;
+    }
+    const T* const w = static_cast<const T*>(a.weight) + (part.group * a.out + min(c0 + lane % 32, a.out - 1)) * a.in;
+    const T* const x = static_cast<const T*>(a.x) + min(part.begin + lane % 32, part.end - 1) * a.x_stride;
+    Sums s(0.0f);
+    for (int64_t k = wave * kLine; k < a.in; k += kFewWaves * kAtOnce * kLine) {
+        Frag<T> fw[kAtOnce][4], fx[kAtOnce][4];
+#pragma unroll
+        for (int t = 0; t < kAtOnce; t++) {
+            const int64_t first = k + t * kFewWaves * kLine;
+            const bool whole = first + kLine <= a.in;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int64_t at = first + (2 * i + half) * V;
+                fw[t][i] = whole ? load_raw<V>(w + at) : load_within(w, at, a.in);
+                fx[t][i] = whole ? load_raw<V>(x + at) : load_within(x, at, a.in);
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < kAtOnce; t++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) mma(s, fw[t][i], fx[t][i]);
+    }
+#pragma unroll
+    for (int q = 0; q < 4; q++)
+        *reinterpret_cast<Floats<4>*>(&sums[wave][lane % 32 * kPitch + half * 4 + q * 8]) = Floats<4>{s[4 * q], s[4 * q + 1], s[4 * q + 2], s[4 * q + 3]};
+    __syncthreads();
+    if (threadIdx.x >= 256 || r >= part.end || c >= a.out) return;
+    Floats<4> v(0.0f);
+#pragma unroll
+    for (int k = 0; k < kFewWaves; k++) v += *reinterpret_cast<const Floats<4>*>(&sums[k][threadIdx.x / 8 * kPitch + threadIdx.x % 8 * 4]);
+    if (a.bias) v += load_some<T, 4>(static_cast<const T*>(a.bias) + part.group * a.out + c, static_cast<int>(min(a.out - c, int64_t{4})));
+    finish4<T>(a.to, r, c, v);
+}
+
 // ---- dz = dy act'(pre), and its columns' sums ------------------------------------------------------------
 
 struct SlopeArgs {
@@ -1168,6 +1228,9 @@ void launch_narrow_bwd(const NarrowBwdArgs& a, const NarrowBwd& p, hipStream_t s
     }
 }
 
+// Whether a forward's groups have so few rows that the weights' bytes are what it takes.
+bool few_rows(int64_t rows, int groups) { return rows <= 32 || rows / groups <= 16; }
+
 template <class T>
 void launch_narrow(const NarrowArgs& a, const Narrow& p, hipStream_t s) {
     const auto go = [&](auto kernel) { kernel<<<static_cast<uint32_t>(p.blocks), p.threads, p.lds, s>>>(a); };
@@ -1204,6 +1267,13 @@ void forward(const LinearFwdArgs& f, hipStream_t s) {
     const Finish to{f.y, f.y_stride, f.out, f.residual, f.residual_stride, f.pre, f.pre_stride, f.act, f.clear};
     if (const Narrow p = plan_narrow<T>(f.rows, f.in, f.out, f.ends != nullptr); p.blocks) {
         launch_narrow<T>({f.x, f.weight, f.bias, f.x_stride, to, f.in, f.out, p.chunk, {f.ends, f.groups, f.rows}}, p, s);
+        return;
+    }
+    if (few_rows(f.rows, f.groups)) {
+        const int64_t slots = slots_of(f.rows, f.groups, kFewShift, f.ends != nullptr), blocks = up(f.out, 32);
+        check_grid(blocks * slots, kFewWaves * 64);
+        k_few_fwd<T><<<dim3(static_cast<uint32_t>(blocks), static_cast<uint32_t>(slots)), kFewWaves * 64, 0, s>>>(
+            {f.x, f.weight, f.bias, f.x_stride, to, f.in, f.out, {f.ends, f.groups, f.rows}});
         return;
     }
     TileArgs a{};
@@ -1289,7 +1359,7 @@ void backward(const LinearBwdArgs& f, hipStream_t s) {
 
 template <class T>
 int64_t forward_workspace(int64_t rows, int64_t in, int64_t out, int groups, bool ragged) {
-    return plan_narrow<T>(rows, in, out, ragged).blocks ? 0 : plan_rows(rows, out, in, groups, ragged, sizeof(T)).bytes;
+    return plan_narrow<T>(rows, in, out, ragged).blocks || few_rows(rows, groups) ? 0 : plan_rows(rows, out, in, groups, ragged, sizeof(T)).bytes;
 }
 template <class T>
 int64_t backward_workspace(int64_t rows, int64_t in, int64_t out, int groups, bool ragged) {

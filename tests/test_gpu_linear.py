@@ -160,3 +160,13 @@ def test_wide_whole_numbers_are_exact(tb, rows, n_in, n_out, dtype):
                                               (264, 64, [90, 0, 30_000, 3])])
 def test_wide_grouped_linear(tb, n_in, n_out, sizes, dtype):
     compare(tb, sum(sizes) + 300, n_in, n_out, dtype, "silu", sizes=sizes, seed=n_in)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,n_in,n_out,sizes", [
+    (1, 2048, 8192, None), (9, 2048, 2050, None), (32, 4096, 700, None), (33, 4096, 700, None), (7, 1000, 333, None), (3, 515, 129, None), (31, 9000, 65, None),
+    (30, 201, 1486, [1] * 28), (60, 700, 515, [0, 33, 1, 0, 2, 20]), (100, 1024, 300, [65] + [0] * 40 + [1] * 10), (12, 640, 640, [0, 0]),
+    (500, 300, 300, [3] * 150 + [0] * 50)])
+def test_few_rows(tb, rows, n_in, n_out, sizes, dtype):
+    """The weights' bytes are all of it: one row to some for each weight."""
+    compare(tb, rows, n_in, n_out, dtype, "gelu", add=rows % 2 == 0, pad=rows % 3, sizes=sizes, seed=rows)
