@@ -73,7 +73,7 @@ struct TileArgs {
 
 // Where the 16 bytes (row r, chunk c) of a plain operand's tile lie: 128 bytes a row, the chunks of eight rows in different
 // places, so that lanes that read one chunk of several rows read different banks.
-__device__ inline int plain_at(int r, int c) { return r * 128 + (c ^ (r & 7)) * 16; }
+__device__ inline int plain_at(int r, int c) { return r * 128 + (c ^ (r >> 1 & 7)) * 16; }
 // Of an Across operand's tile: `row_bytes` a row of the sums' dimension; four rows' 32 bytes in different places.
 template <class T>
 __device__ inline int across_at(int m, int byte, int row_bytes) {
@@ -140,7 +140,7 @@ struct DirectStage {
                 const int m = at / kLine, byte = across_at<T>(m, at % kLine, kLine) - m * kLine;
                 offset[i] = static_cast<uint32_t>(m * line + min(f * static_cast<int64_t>(sizeof(T)) + byte, (l - V) * static_cast<int64_t>(sizeof(T))));
             } else {
-                const int r = at / 128, c = (at / 16 % 8) ^ (r & 7);
+                const int r = at / 128, c = (at / 16 % 8) ^ (r >> 1 & 7);
                 offset[i] = static_cast<uint32_t>(min(int64_t{r}, l - 1 - f) * line + c * 16);
             }
         }
@@ -930,7 +930,7 @@ struct FewArgs {
 constexpr int kFewWaves = 8, kFewShift = 5;  // a part: 32 rows
 template <class T>
 __global__ void __launch_bounds__(kFewWaves * 64) k_few_fwd(FewArgs a) {
-    constexpr int V = kPer<T>, kLine = 128 / static_cast<int>(sizeof(T)), kAtOnce = 2, kPitch = 36;
+    constexpr int V = kPer<T>, kLine = 128 / static_cast<int>(sizeof(T)), kAtOnce = 4, kPitch = 36;
     __shared__ float sums[kFewWaves][32 * kPitch];
     const Part part = part_of(a.groups, blockIdx.y, kFewShift);
     if (part.begin >= part.end) return;
