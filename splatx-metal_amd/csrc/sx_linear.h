@@ -1099,7 +1099,7 @@ Over plan_over(int64_t rows, int64_t out, int64_t in, int groups, bool ragged, i
         }
         for (int shift = 8; (int64_t{1} << shift) < rows; shift++) {
             const int64_t slots = slots_of(rows, groups, shift, ragged), bytes = slots * out * in * 4;
-            if (bytes > int64_t{256} << 20) continue;
+            if (bytes > int64_t{256} << 20 || slots > 65535) continue;
             const double parts = ragged ? static_cast<double>(rows >> shift) + 0.5 * groups : static_cast<double>(slots);
             time = tiles_take(k, tiles * parts, static_cast<double>(int64_t{1} << shift) / step, elem) + kJoinFixed +
                    2.0 * parts * static_cast<double>(out * in) * 4 / kJoinBytes / 1000;

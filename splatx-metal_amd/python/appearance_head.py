@@ -20,35 +20,59 @@ import numpy as np
 import scene
 
 
-class Block(torch.nn.Module):
-    def __init__(self, hidden, dtype):
+class CellLinear(torch.nn.Module):
+    """A linear layer of its own for each cell's rows."""
+
+    def __init__(self, cells, features, out, dtype):
         super().__init__()
+        bound = 1 / math.sqrt(features)
+        self.weight = torch.nn.Parameter(torch.empty(cells, out, features, dtype=dtype).uniform_(-bound, bound))
+        self.bias = torch.nn.Parameter(torch.empty(cells, out, dtype=dtype).uniform_(-bound, bound))
+
+
+class Block(torch.nn.Module):
+    def __init__(self, hidden, dtype, cells=0):
+        super().__init__()
+        layer = (lambda: CellLinear(cells, hidden, hidden, dtype)) if cells else (lambda: torch.nn.Linear(hidden, hidden, dtype=dtype))
         self.norm_weight = torch.nn.Parameter(torch.ones(hidden))
         self.norm_bias = torch.nn.Parameter(torch.zeros(hidden))
-        self.up = torch.nn.Linear(hidden, hidden, dtype=dtype)
-        self.down = torch.nn.Linear(hidden, hidden, dtype=dtype)
+        self.up = layer()
+        self.down = layer()
 
-    def forward(self, backend, stream, update):
+    def forward(self, backend, stream, update, fused=False, ends=None):
         """(the residual stream with the last block's update added, this block's update)"""
         if update is None:
             y = splatx_torch.layer_norm(backend, stream, self.norm_weight, self.norm_bias)
         else:
             y, stream = splatx_torch.layer_norm(backend, stream, self.norm_weight, self.norm_bias, residual=update)
+        if ends is not None:
+            y = splatx_torch.grouped_linear(backend, y, self.up.weight, ends, self.up.bias, "gelu")
+            return stream, splatx_torch.grouped_linear(backend, y, self.down.weight, ends, self.down.bias)
+        if fused:
+            y = splatx_torch.linear(backend, y, self.up.weight, self.up.bias, "gelu")
+            return stream, splatx_torch.linear(backend, y, self.down.weight, self.down.bias)
         return stream, self.down(torch.nn.functional.gelu(self.up(y)))
 
 
 class AppearanceHead(torch.nn.Module):
-    """Colour offsets [splats, 3] of the splats' features in one image."""
+    """Colour offsets [splats, 3] of the splats' features in one image. `cells`: the cell of each splat, 0 and up, of which each
+    has blocks of its own (then the layers are fused)."""
 
-    def __init__(self, backend, features, images, hidden=64, embedding=16, blocks=2, dtype=torch.bfloat16):
+    def __init__(self, backend, features, images, hidden=64, embedding=16, blocks=2, dtype=torch.bfloat16, fused=False, cells=None):
         super().__init__()
-        self.backend = backend
+        self.backend, self.fused, self.order, self.ends = backend, fused or cells is not None, None, None
+        count = 0
+        if cells is not None:
+            count = int(cells.max()) + 1
+            self.order = torch.argsort(cells, stable=True).to(backend.device)
+            self.place = torch.argsort(self.order)  # of each splat in that order
+            self.ends = torch.cumsum(torch.bincount(cells, minlength=count), 0).to(backend.device)
         self.norm_weight = torch.nn.Parameter(torch.ones(features))
         self.norm_bias = torch.nn.Parameter(torch.zeros(features))
         self.embedding = torch.nn.Parameter(0.1 * torch.randn(images, embedding, dtype=dtype))
         self.enter = torch.nn.Linear(features, hidden, dtype=dtype)
         self.mix = torch.nn.Linear(embedding, hidden, bias=False, dtype=dtype)
-        self.blocks = torch.nn.ModuleList(Block(hidden, dtype) for _ in range(blocks))
+        self.blocks = torch.nn.ModuleList(Block(hidden, dtype, count) for _ in range(blocks))
         self.last_weight = torch.nn.Parameter(torch.ones(hidden))
         self.last_bias = torch.nn.Parameter(torch.zeros(hidden))
         self.leave = torch.nn.Linear(hidden, 3, dtype=dtype)
@@ -57,12 +81,22 @@ class AppearanceHead(torch.nn.Module):
         self.to(backend.device)
 
     def forward(self, features, image):
+        if self.order is not None:
+            features = features[self.order]
         x = splatx_torch.layer_norm(self.backend, features, self.norm_weight, self.norm_bias)
-        stream, update = self.enter(x) + self.mix(self.embedding[image]), None
+        if self.fused:
+            mixed = splatx_torch.linear(self.backend, self.embedding[image].unsqueeze(0), self.mix.weight)
+            stream = splatx_torch.linear(self.backend, x, self.enter.weight, self.enter.bias, residual=mixed.expand(x.shape[0], -1))
+        else:
+            stream = self.enter(x) + self.mix(self.embedding[image])
+        update = None
         for block in self.blocks:
-            stream, update = block(self.backend, stream, update)
+            stream, update = block(self.backend, stream, update, self.fused, self.ends)
         y, _ = splatx_torch.layer_norm(self.backend, stream, self.last_weight, self.last_bias, residual=update)
-        return self.leave(y).float()
+        if not self.fused:
+            return self.leave(y).float()
+        out = splatx_torch.linear(self.backend, y, self.leave.weight, self.leave.bias).float()
+        return out if self.order is None else out[self.place]
 
 
 def optimizer(head, lr=2e-3, state_bits=32, max_norm=1.0):
@@ -118,7 +152,14 @@ def train_step(head, opt, features, view, image, target):
     return float(np.abs(difference).mean())
 
 
-def demo(n=20_000, images=6, steps=120, state_bits=8, seed=0, width=320, height=240, sh_degree=3, quiet=False):
+def cells_of(means, count):
+    """`count` cells of about as many splats each, along x."""
+    rank = np.empty(len(means), np.int64)
+    rank[np.argsort(means[:, 0], kind="stable")] = np.arange(len(means))
+    return torch.from_numpy(rank * count // len(means))
+
+
+def demo(n=20_000, images=6, steps=120, state_bits=8, seed=0, width=320, height=240, sh_degree=3, quiet=False, fused=False, cells=0):
     """A head on a synthetic scene whose images are tinted differently; the losses of the steps."""
     torch.manual_seed(seed)
     backend = splatx_torch.TorchBackend(0)
@@ -127,7 +168,7 @@ def demo(n=20_000, images=6, steps=120, state_bits=8, seed=0, width=320, height=
     views = [View(backend, sc, scene.jittered_view(rng)) for _ in range(images)]
     targets = [(v.render()[0] * rng.uniform(0.6, 1.4, 3)).astype(np.float32) for v in views]
     features = torch.from_numpy(np.concatenate([sc.params[4], sc.params[5]], 1)).to(backend.device, torch.bfloat16)
-    head = AppearanceHead(backend, features.shape[1], images)
+    head = AppearanceHead(backend, features.shape[1], images, fused=fused, cells=cells_of(sc.params[0], cells) if cells else None)
     opt = optimizer(head, state_bits=state_bits)
     losses = []
     for step in range(steps):
@@ -145,8 +186,10 @@ def main():
     p.add_argument("--images", type=int, default=6)
     p.add_argument("--steps", type=int, default=360)
     p.add_argument("--state-bits", type=int, choices=(8, 32), default=8)
+    p.add_argument("--fused", action="store_true", help="the framework's own linear layers")
+    p.add_argument("--cells", type=int, default=0, help="cut the scene into as many cells with blocks of their own")
     a = p.parse_args()
-    losses = demo(a.splats, a.images, a.steps, a.state_bits)
+    losses = demo(a.splats, a.images, a.steps, a.state_bits, fused=a.fused, cells=a.cells)
     first, last = (float(np.mean(x)) for x in (losses[:a.images], losses[-a.images:]))
     print(f"L1 over the images: {first:.5f} before, {last:.5f} after ({20 * math.log10(first / max(last, 1e-9)):.1f} dB)")
 

@@ -17,11 +17,16 @@ ACTS = ("none", "relu", "gelu", "silu", "sigmoid")
 ACT = {torch.float32: 16 * U32, torch.bfloat16: 4e-5, torch.float16: 4e-5}
 
 
+def below(z):
+    """Phi. (As 1 + erf it would lose the tail, 64 bits or not.)"""
+    return 0.5 * torch.special.erfc(-z * math.sqrt(0.5))
+
+
 def act(z, name):
     if name == "relu":
         return z.clamp_min(0)
     if name == "gelu":
-        return z * torch.special.ndtr(z)
+        return z * below(z)
     if name == "silu":
         return z * torch.sigmoid(z)
     return torch.sigmoid(z) if name == "sigmoid" else z
@@ -31,7 +36,7 @@ def slope(z, name):
     if name == "relu":
         return (z > 0).double()
     if name == "gelu":
-        return torch.special.ndtr(z) + z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+        return below(z) + z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
     p = torch.sigmoid(z)
     if name == "silu":
         return p + z * p * torch.sigmoid(-z)
