@@ -97,15 +97,25 @@ struct Stage {
         chunk = threadIdx.x % kPerLine;
         line = threadIdx.x / kPerLine;
     }
-    // Of the sums' dimension [d, d + kDepth), zeros from `end` on.
+    // Of the sums' dimension [d, d + kDepth), zeros from `end` on. (In a tile that ends inside its operand all loads go out
+    // together; a branch for each would wait for each.)
     __device__ void load(int64_t d, int64_t end) {
+        const int64_t width = Across ? limit : end;
+        const bool inside = d + kDepth <= end && (!Across || first + R <= limit);
 #pragma unroll
         for (int i = 0; i < N; i++) {
             const int l = line + i * kLines;
             if constexpr (Across) {
-                v[i] = d + l < end ? load_within(base + (d + l) * stride, first + chunk * V, limit) : Frag<T>(0);
+                const T* const p = base + min(d + l, end - 1) * stride;
+                if (inside) v[i] = load_raw<V>(p + first + chunk * V);
+                else if (width >= V) v[i] = load_clamped(p, first + chunk * V, limit);
+                else v[i] = load_within(p, first + chunk * V, limit);
+                if (!inside && d + l >= end) v[i] = Frag<T>(0);
             } else {
-                v[i] = load_within(base + min(first + l, limit - 1) * stride, d + chunk * V, end);
+                const T* const p = base + min(first + l, limit - 1) * stride;
+                if (inside) v[i] = load_raw<V>(p + d + chunk * V);
+                else if (width >= V) v[i] = load_clamped(p, d + chunk * V, end);
+                else v[i] = load_within(p, d + chunk * V, end);
             }
         }
     }
@@ -267,7 +277,7 @@ struct Unit {
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const T* const p = static_cast<const T*>(a.residual) + (r * a.residual_stride + c) + min(row + 8 * i, rows - 1) * a.residual_stride;
-                residual[i] = a.cols - c >= 8 * V ? load_raw<V>(p + column) : load_within(p, column, a.cols - c);
+                residual[i] = a.cols - c >= 8 * V ? load_raw<V>(p + column) : a.cols - c >= V ? load_clamped(p, column, a.cols - c) : load_within(p, column, a.cols - c);
             }
     }
     // (what all lanes share is added apart from what a lane has of its own, which stays over the units)
@@ -637,29 +647,30 @@ struct NarrowArgs {
     Groups groups;
 };
 
-// Fragments of a row of which the last may reach past its end: load_within without a branch, for rows of a fragment at least.
+// Fragments of a row of up to K steps. The load reads nothing outside the row; what it reads in place of elements past the
+// row's end is taken out before the products, when it has arrived.
 template <class T, int K>
 struct RowLoad {
     static constexpr int V = kPer<T>;
-    int64_t in;
-    int last, down;  // where the last fragment is read, and the bytes it moves down
-    bool small;
-    __device__ explicit RowLoad(int64_t n) : in(n) {
-        const int k = (2 * (K - 1) + static_cast<int>(threadIdx.x) % 64 / 32) * V;
-        small = n < V;
-        last = small ? 0 : min(k, static_cast<int>(n) - V);
-        down = (k - last) * static_cast<int>(sizeof(T));
-    }
+    static constexpr int kWhole = K == 6 || K == 8 ? K - 2 : K == 12 || K == 16 ? K - 4 : K - 1;  // steps that any row of so many has whole
+    int in, first;
+    bool small;  // less than a fragment
+    __device__ explicit RowLoad(int64_t n) : in(static_cast<int>(n)), first(static_cast<int>(threadIdx.x) % 64 / 32 * V), small(n < V) {}
     __device__ void operator()(Frag<T> (&f)[K], const T* row) const {
-        const int half = threadIdx.x % 64 / 32;
         if (small) {
-            f[0] = load_within(row, half * V, in);
+            f[0] = load_within(row, first, in);
             return;
         }
 #pragma unroll
-        for (int k = 0; k < K - 1; k++) f[k] = load_raw<V>(row + (2 * k + half) * V);
-        f[K - 1] = load_raw<V>(row + last);
-        if (in % (2 * V)) f[K - 1] = down < 16 ? moved_down<T>(f[K - 1], down) : Frag<T>(0);
+        for (int k = 0; k < K; k++) f[k] = load_raw<V>(row + (k < kWhole ? 2 * k * V + first : min(2 * k * V + first, in - V)));
+    }
+    __device__ void cut(Frag<T> (&f)[K]) const {
+#pragma unroll
+        for (int k = kWhole; k < K; k++)
+            if (!small && 2 * (k + 1) * V > in) {
+                const int past = (2 * k * V + first - min(2 * k * V + first, in - V)) * static_cast<int>(sizeof(T));
+                f[k] = past < 16 ? moved_down<T>(f[k], past) : Frag<T>(0);
+            }
     }
 };
 
@@ -687,22 +698,24 @@ __global__ void __launch_bounds__(512) k_narrow_fwd(NarrowArgs a) {
             return;
         }
         const int64_t stop = max(first + 1, min(last, a.groups.end(group)));  // (a row at least, whatever the ends are)
-        Frag<T> next[K];
+        Frag<T> now[K], next[K];
         int64_t base = first + wave * 32;
         load(next, x + min(base + lane % 32, stop - 1) * a.x_stride);
         lds_barrier();
         const T* const w = static_cast<const T*>(a.weight) + group * a.in * a.out;
         for (int i = threadIdx.x; i < tiles * K * 64; i += blockDim.x) {
-            const int n = i / 64 / K * 32 + i % 32;
-            weights[i] = n < a.out ? load_within(w + n * a.in, (2 * (i / 64 % K) + i % 64 / 32) * V, a.in) : Frag<T>(0);
+            const int n = i / 64 / K * 32 + i % 32, k = (2 * (i / 64 % K) + i % 64 / 32) * V;
+            const T* const p = w + min(int64_t{n}, a.out - 1) * a.in;
+            const Frag<T> f = a.in >= V ? load_clamped(p, k, a.in) : load_within(p, k, a.in);
+            weights[i] = n < a.out ? f : Frag<T>(0);
         }
         for (int i = threadIdx.x; i < tiles * 32; i += blockDim.x)
             bias[i] = a.bias && i < a.out ? static_cast<float>(static_cast<const T*>(a.bias)[group * a.out + i]) : 0.0f;
         lds_barrier();
         for (; base < stop; base += step) {
-            Frag<T> now[K];
 #pragma unroll
             for (int k = 0; k < K; k++) now[k] = next[k];
+            load.cut(now);
             if (base + step < stop) load(next, x + min(base + step + lane % 32, stop - 1) * a.x_stride);
             for (int t = 0; t < tiles; t += kUnitTiles<T>) {
                 Unit<T> to(a.to, base, stop, t * 32);
@@ -775,18 +788,26 @@ struct BlockPart {
     Frag<T> v[N];
     static __device__ int chunk() { return threadIdx.x % kLanes; }
     static __device__ int line(int i) { return threadIdx.x / kLanes + i * kLines; }
-    // Rows [first, stop), at most a block of them. (Of rows and chunks there are not others are read.)
+    // Rows [first, stop), at most a block of them. (Of rows and chunks there are not others are read, of a chunk that reaches past
+    // its row's end the last elements of the row: `get` moves them to their place.)
     __device__ void load(const void* from, int64_t stride, int64_t width, int64_t first, int64_t stop) {
         const T* const base = static_cast<const T*>(from) + first * stride;
-        const int most = static_cast<int>(min(stop - 1 - first, int64_t{kBlockRows<T>}));
-        if (width % V == 0) {
-            const T* const at = base + min(int64_t{chunk()} * V, width - V);
+        const int most = static_cast<int>(min(stop - 1 - first, int64_t{kBlockRows<T>})), n = static_cast<int>(width);
+        if (n >= V) {
+            const T* const at = base + min(chunk() * V, n - V);
 #pragma unroll
             for (int i = 0; i < N; i++) v[i] = load_raw<V>(at + min(line(i), most) * stride);
         } else {
 #pragma unroll
             for (int i = 0; i < N; i++) v[i] = load_within(base + min(line(i), most) * stride, chunk() * V, width);
         }
+    }
+    // Its i-th chunk: zeros behind the row's end and in lines from `lines` on.
+    __device__ Frag<T> get(int i, int64_t width, int lines) const {
+        const int n = static_cast<int>(width), past = n < V ? 0 : chunk() * V - min(chunk() * V, n - V);
+        Frag<T> f = v[i];
+        if (n % V) f = moved_down<T>(f, past * static_cast<int>(sizeof(T)) & 15);
+        return line(i) < lines && chunk() * V < n ? f : Frag<T>(0);
     }
 };
 
@@ -829,11 +850,12 @@ __global__ void __launch_bounds__(Waves * 64) k_narrow_bwd(NarrowBwdArgs a) {
             const T* const w = static_cast<const T*>(a.weight) + group * a.in * a.out;
             for (int i = threadIdx.x; i < XT * kSteps * 64; i += kThreads) {
                 const int k = i / 64 / kSteps * 32 + i % 32, n = (2 * (i / 64 % kSteps) + i % 64 / 32) * V;
-                Frag<T> f(0);
-                if (k < a.in)
+                Frag<T> f;
 #pragma unroll
-                    for (int e = 0; e < V; e++)
-                        if (n + e < a.out) f[e] = w[(n + e) * a.in + k];
+                for (int e = 0; e < V; e++) f[e] = w[min(int64_t{n + e}, a.out - 1) * a.in + min(int64_t{k}, a.in - 1)];
+#pragma unroll
+                for (int e = 0; e < V; e++)
+                    if (n + e >= a.out || k >= a.in) f[e] = static_cast<T>(0.0f);
                 weights[i] = f;
             }
         }
@@ -845,16 +867,15 @@ __global__ void __launch_bounds__(Waves * 64) k_narrow_bwd(NarrowBwdArgs a) {
             const int rows = static_cast<int>(min(stop - block, int64_t{kRows}));
 #pragma unroll
             for (int i = 0; i < dy.N; i++) {
-                Floats<V> d = floats<T, V>(dy.v[i]);
-                if (a.act) through<T, V>(d, floats<T, V>(pre.v[i]), a.act);
-                if (dy.line(i) >= rows || zc * V >= a.out) d = Floats<V>(0.0f);
+                Floats<V> d = floats<T, V>(dy.get(i, a.out, rows));
+                if (a.act) through<T, V>(d, floats<T, V>(pre.get(i, a.out, rows)), a.act);
                 db += d;
                 *reinterpret_cast<Frag<T>*>(dz + dy.line(i) * kZ + zc * 16) = raw<T, V>(d);
             }
             if (a.x)
 #pragma unroll
                 for (int i = 0; i < x.N; i++)
-                    *reinterpret_cast<Frag<T>*>(xs + x.line(i) * kX + xc * 16) = x.line(i) < rows && xc * V < a.in ? x.v[i] : Frag<T>(0);
+                    *reinterpret_cast<Frag<T>*>(xs + x.line(i) * kX + xc * 16) = x.get(i, a.in, rows);
             lds_barrier();
             if (block + step < stop) load(block + step, stop);
             if (a.x)
@@ -927,47 +948,60 @@ struct FewArgs {
     int64_t in, out;
     Groups groups;
 };
-constexpr int kFewWaves = 8, kFewShift = 5;  // a part: 32 rows
-template <class T>
+constexpr int kFewWaves = 8;
+// R times 32 rows a part.
+template <class T, int R>
 __global__ void __launch_bounds__(kFewWaves * 64) k_few_fwd(FewArgs a) {
-    constexpr int V = kPer<T>, kLine = 128 / static_cast<int>(sizeof(T)), kAtOnce = 4, kPitch = 36;
-    __shared__ float sums[kFewWaves][32 * kPitch];
-    const Part part = part_of(a.groups, blockIdx.y, kFewShift);
+    constexpr int V = kPer<T>, kLine = 128 / static_cast<int>(sizeof(T)), kAtOnce = R == 1 ? 4 : 2, kPitch = 36;
+    __shared__ float sums[kFewWaves][R * 32 * kPitch];
+    const Part part = part_of(a.groups, blockIdx.y, R == 1 ? 5 : 6);
     if (part.begin >= part.end) return;
     const int64_t c0 = int64_t{blockIdx.x} * 32;
     const int lane = threadIdx.x % 64, half = lane / 32, wave = wave_of();
-    // (in the end a thread of the first half has four outputs)
+    // (in the end a thread, of R 1 one of the first half, has four outputs)
     const int64_t r = part.begin + threadIdx.x / 8, c = c0 + threadIdx.x % 8 * 4;
     if (part.group >= a.groups.groups) {
-        if (threadIdx.x < 256 && r < part.end) clear4<T>(a.to, r, c);
+        if (threadIdx.x < R * 256 && r < part.end) clear4<T>(a.to, r, c);
         return;
     }
     const T* const w = static_cast<const T*>(a.weight) + (part.group * a.out + min(c0 + lane % 32, a.out - 1)) * a.in;
-    const T* const x = static_cast<const T*>(a.x) + min(part.begin + lane % 32, part.end - 1) * a.x_stride;
-    Sums s(0.0f);
+    const T* x[R];
+#pragma unroll
+    for (int b = 0; b < R; b++) x[b] = static_cast<const T*>(a.x) + min(part.begin + b * 32 + lane % 32, part.end - 1) * a.x_stride;
+    Sums s[R];
+#pragma unroll
+    for (int b = 0; b < R; b++) s[b] = Sums(0.0f);
     for (int64_t k = wave * kLine; k < a.in; k += kFewWaves * kAtOnce * kLine) {
-        Frag<T> fw[kAtOnce][4], fx[kAtOnce][4];
+        Frag<T> fw[kAtOnce][4], fx[R][kAtOnce][4];
+        const auto load_all = [&](auto load) {
 #pragma unroll
-        for (int t = 0; t < kAtOnce; t++) {
-            const int64_t first = k + t * kFewWaves * kLine;
-            const bool whole = first + kLine <= a.in;
+            for (int t = 0; t < kAtOnce; t++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int64_t at = first + (2 * i + half) * V;
-                fw[t][i] = whole ? load_raw<V>(w + at) : load_within(w, at, a.in);
-                fx[t][i] = whole ? load_raw<V>(x + at) : load_within(x, at, a.in);
-            }
-        }
+                for (int i = 0; i < 4; i++) {
+                    const int64_t at = k + t * kFewWaves * kLine + (2 * i + half) * V;
+                    fw[t][i] = load(w, at);
+#pragma unroll
+                    for (int b = 0; b < R; b++) fx[b][t][i] = load(x[b], at);
+                }
+        };
+        if (k + (kAtOnce - 1) * kFewWaves * kLine + kLine <= a.in) load_all([&](const T* p, int64_t at) { return load_raw<V>(p + at); });
+        else if (a.in >= V) load_all([&](const T* p, int64_t at) { return load_clamped(p, at, a.in); });
+        else load_all([&](const T* p, int64_t at) { return load_within(p, at, a.in); });
 #pragma unroll
         for (int t = 0; t < kAtOnce; t++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) mma(s, fw[t][i], fx[t][i]);
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int b = 0; b < R; b++) mma(s[b], fw[t][i], fx[b][t][i]);
     }
 #pragma unroll
-    for (int q = 0; q < 4; q++)
-        *reinterpret_cast<Floats<4>*>(&sums[wave][lane % 32 * kPitch + half * 4 + q * 8]) = Floats<4>{s[4 * q], s[4 * q + 1], s[4 * q + 2], s[4 * q + 3]};
+    for (int b = 0; b < R; b++)
+#pragma unroll
+        for (int q = 0; q < 4; q++)
+            *reinterpret_cast<Floats<4>*>(&sums[wave][(b * 32 + lane % 32) * kPitch + half * 4 + q * 8]) =
+                Floats<4>{s[b][4 * q], s[b][4 * q + 1], s[b][4 * q + 2], s[b][4 * q + 3]};
     __syncthreads();
-    if (threadIdx.x >= 256 || r >= part.end || c >= a.out) return;
+    if (threadIdx.x >= R * 256 || r >= part.end || c >= a.out) return;
     Floats<4> v(0.0f);
 #pragma unroll
     for (int k = 0; k < kFewWaves; k++) v += *reinterpret_cast<const Floats<4>*>(&sums[k][threadIdx.x / 8 * kPitch + threadIdx.x % 8 * 4]);
@@ -999,18 +1033,29 @@ __global__ void __launch_bounds__(256) k_slope(SlopeArgs a, int lanes) {
     Floats<V> sum(0.0f);
     if (c < a.cols) {
         const int n = static_cast<int>(min(a.cols - c, int64_t{V}));
+        // (a vector that reaches past the row's end is read so that it ends there, and moved to its place)
+        const bool small = a.cols < V;
+        const int64_t at = min(c, a.cols - V);
+        const int past = small ? 0 : static_cast<int>(c - at) * static_cast<int>(sizeof(T));
         for (int64_t first = part.begin + threadIdx.x / lanes; first < part.end; first += kAtOnce * step) {
             Frag<T> dy[kAtOnce], pre[kAtOnce];
+            const auto load = [&](Frag<T> (&v)[kAtOnce], const void* from, int64_t stride) {
 #pragma unroll
-            for (int i = 0; i < kAtOnce; i++) {
-                const int64_t r = min(first + i * step, part.end - 1);
-                dy[i] = load_within(static_cast<const T*>(a.dy) + r * a.dy_stride, c, a.cols);
-                if (a.act) pre[i] = load_within(static_cast<const T*>(a.pre) + r * a.pre_stride, c, a.cols);
-            }
+                for (int i = 0; i < kAtOnce; i++) {
+                    const T* const p = static_cast<const T*>(from) + min(first + i * step, part.end - 1) * stride;
+                    v[i] = small ? load_within(p, c, a.cols) : load_raw<V>(p + at);
+                }
+            };
+            load(dy, a.dy, a.dy_stride);
+            if (a.act) load(pre, a.pre, a.pre_stride);
 #pragma unroll
             for (int i = 0; i < kAtOnce; i++) {
                 const int64_t r = first + i * step;
                 if (r >= part.end) break;
+                if (past) {
+                    dy[i] = moved_down<T>(dy[i], past);
+                    if (a.act) pre[i] = moved_down<T>(pre[i], past);
+                }
                 Floats<V> d = floats<T, V>(dy[i]);
                 if (a.act) {
                     through<T, V>(d, floats<T, V>(pre[i]), a.act);
@@ -1038,19 +1083,19 @@ int log2_up(int64_t n) {
 int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to; }
 
 // The tiles to choose from: their rows and columns, how many run at once on 256 units, and what a step of 128 bytes of the
-// sums' length then takes, in ns of 16-bit elements (floats: as many bytes, 4.6 times). Measured on layers of 16,383 rows, 8192 to
+// sums' length then takes, in ns of 16-bit elements (floats: as many bytes, 4.6 times), and what a tile takes besides. Measured on layers of 16,383 rows, 8192 to
 // 2048: 542, 623 and 712 us by tiles of 256, 128 and 64 rows; 20,001 rows in 16 groups, 1024 to 1408, whose tiles of 256 rows
 // take three rounds for two: 121, 104 and 106.
 struct TileKind {
     int rows, cols, at_once;
-    double step;
+    double step, fixed;
 };
-constexpr TileKind kTileKinds[] = {{256, 256, 256, 1950}, {128, 128, 512, 1150}, {64, 128, 768, 1050}};
-constexpr double kTileFixed = 3000, kJoinFixed = 4000, kJoinBytes = 4;  // ns; ns; bytes a ns
+constexpr TileKind kTileKinds[] = {{256, 256, 256, 1950, 6000}, {128, 128, 512, 1150, 3000}, {64, 128, 768, 1050, 2500}};
+constexpr double kJoinFixed = 4000, kJoinBytes = 4;  // ns; bytes a ns
 // `tiles` of `steps` each; a unit's only workgroup of a kind that shares it goes faster.
 double tiles_take(const TileKind& k, double tiles, double steps, int elem) {
     const double step = k.step * (elem == 4 ? 4.6 : 1.0) * (tiles <= 256 && k.at_once > 256 ? 0.6 : 1.0);
-    return std::max(1.0, std::ceil(tiles / k.at_once)) * (kTileFixed + steps * step);
+    return std::max(1.0, std::ceil(tiles / k.at_once)) * (k.fixed + steps * step);
 }
 
 // out[rows][cols] over `depth`, rows in groups: the tile's rows, and how many parts the depth is split into.
@@ -1120,7 +1165,7 @@ Slope plan_slope(int64_t rows, int64_t cols, int groups, bool ragged, int elem) 
     const int64_t vectors = up(cols, 16 / elem);
     p.lanes = 1 << std::min(8, log2_up(vectors));
     p.columns = up(vectors, p.lanes);
-    p.shift = std::max({log2_up(256 / p.lanes) + 2, 4, log2_up(up(std::max<int64_t>(rows, 1), std::max<int64_t>(1, 1024 / p.columns)))});
+    p.shift = std::max({log2_up(256 / p.lanes) + 2, log2_up(up(std::max<int64_t>(rows, 1), std::max<int64_t>(1, 1024 / p.columns)))});
     p.slots = slots_of(rows, groups, p.shift, ragged);
     p.bytes = p.slots * cols * 4;
     p.dz_stride = vectors * (16 / elem);
@@ -1229,7 +1274,7 @@ void launch_narrow_bwd(const NarrowBwdArgs& a, const NarrowBwd& p, hipStream_t s
 }
 
 // Whether a forward's groups have so few rows that the weights' bytes are what it takes.
-bool few_rows(int64_t rows, int groups) { return rows <= 32 || rows / groups <= 16; }
+bool few_rows(int64_t rows, int groups) { return rows <= 64 || rows / groups <= 32; }
 
 template <class T>
 void launch_narrow(const NarrowArgs& a, const Narrow& p, hipStream_t s) {
@@ -1270,10 +1315,13 @@ void forward(const LinearFwdArgs& f, hipStream_t s) {
         return;
     }
     if (few_rows(f.rows, f.groups)) {
-        const int64_t slots = slots_of(f.rows, f.groups, kFewShift, f.ends != nullptr), blocks = up(f.out, 32);
+        const bool two = f.rows > 32 && f.rows / f.groups > 16;
+        const int64_t slots = slots_of(f.rows, f.groups, two ? 6 : 5, f.ends != nullptr), blocks = up(f.out, 32);
         check_grid(blocks * slots, kFewWaves * 64);
-        k_few_fwd<T><<<dim3(static_cast<uint32_t>(blocks), static_cast<uint32_t>(slots)), kFewWaves * 64, 0, s>>>(
-            {f.x, f.weight, f.bias, f.x_stride, to, f.in, f.out, {f.ends, f.groups, f.rows}});
+        const dim3 grid(static_cast<uint32_t>(blocks), static_cast<uint32_t>(slots));
+        const FewArgs a{f.x, f.weight, f.bias, f.x_stride, to, f.in, f.out, {f.ends, f.groups, f.rows}};
+        if (two) k_few_fwd<T, 2><<<grid, kFewWaves * 64, 0, s>>>(a);
+        else k_few_fwd<T, 1><<<grid, kFewWaves * 64, 0, s>>>(a);
         return;
     }
     TileArgs a{};

@@ -54,6 +54,15 @@ __device__ inline Frag<T> load_within(const T* row, int64_t k, int64_t n) {
     return v;
 }
 
+// The same without a branch, of rows of a fragment at least: what lies past the end is moved out of what ends with the row.
+template <class T>
+__device__ inline Frag<T> load_clamped(const T* row, int64_t k, int64_t n) {
+    const int64_t at = min(k, n - kPer<T>);
+    const Frag<T> v = load_raw<kPer<T>>(row + at);
+    const int64_t past = k - at;
+    return past < kPer<T> ? moved_down<T>(v, static_cast<int>(past) * static_cast<int>(sizeof(T))) : Frag<T>(0);
+}
+
 enum Act : int { kNone = 0, kRelu = 1, kGelu = 2, kSilu = 3, kSigmoid = 4 };
 
 // e^(-x scale) of the types: 16-bit outputs take the hardware's exponential and reciprocal (2^-22 and the argument's rounding).

@@ -170,3 +170,19 @@ def test_wide_grouped_linear(tb, n_in, n_out, sizes, dtype):
 def test_few_rows(tb, rows, n_in, n_out, sizes, dtype):
     """The weights' bytes are all of it: one row to some for each weight."""
     compare(tb, rows, n_in, n_out, dtype, "gelu", add=rows % 2 == 0, pad=rows % 3, sizes=sizes, seed=rows)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n_in", [5, 7, 9, 20, 40, 70, 79, 81, 100, 111, 113, 139, 145, 150, 161, 177, 193, 209, 211, 225, 230, 241, 250])
+@pytest.mark.parametrize("rows,n_out,sizes", [(130, 33, None), (4200, 40, None), (150, 70, [60, 0, 80])])
+def test_nothing_of_the_padding_is_taken(tb, rows, n_out, sizes, n_in, dtype):
+    """Rows between NaN, of widths at and about every count of steps: an element past a row's end would show."""
+    compare(tb, rows, n_in, n_out, dtype, "relu", add=True, pad=8 + n_in % 3, off=n_in % 2, sizes=sizes, seed=n_in)
+    compare(tb, rows, n_out, n_in, dtype, "relu", add=True, pad=8 + n_in % 3, off=n_in % 2, sizes=sizes, seed=n_in)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,n_in,n_out,sizes", [(377, 1500, 290, None), (372, 700, 246, None), (1850, 319, 738, None), (60, 704, 558, [20, 36]), (50, 1000, 64, None),
+                                                   (64, 515, 100, None), (100, 515, 200, [64, 0, 1, 32])])
+def test_odd_widths_and_few_rows(tb, rows, n_in, n_out, sizes, dtype):
+    compare(tb, rows, n_in, n_out, dtype, "silu", pad=8 if n_in % 2 else 0, sizes=sizes, seed=rows)
