@@ -834,8 +834,8 @@ int32_t sxh_adamw(sxh_backend* b, const sxh_adamw_tensor* tensors /* host array 
  * groups 0: one weight [out, in] and bias [out] for all rows. groups G > 0: rows come in G groups with a weight [G, out, in] and
  * bias [G, out] of their own; group g has the rows [ends[g - 1], ends[g]), the first from row 0. `ends` lies on the device,
  * ascends (equal ends: a group without rows) and is at most rows; of ends that are not so no row outside [0, rows) is
- * touched, and which group has a row is not specified. Rows from the last end on belong to no group: nothing of theirs is
- * read, and y and pre are left as they were there, or with `clear` become zero.
+ * touched, and which group has a row is not specified. Rows from the last end on belong to no group: nothing of theirs
+ * counts, and y and pre are left as they were there, or with `clear` become zero.
  * Rows are `*_stride` elements apart (at least their width; for inputs also 0: every row the same one). */
 enum { SXH_ACT_NONE = 0, SXH_ACT_RELU = 1, SXH_ACT_GELU = 2, SXH_ACT_SILU = 3, SXH_ACT_SIGMOID = 4 };
 typedef struct {
@@ -858,7 +858,7 @@ typedef struct {
     void* workspace;       /* sxh_linear_fwd_workspace(...) bytes of device memory, 16-byte aligned; may be NULL if that is 0 */
     int64_t workspace_bytes;
 } sxh_linear_outputs;
-int64_t sxh_linear_fwd_workspace(int64_t rows, int64_t in, int64_t out, int64_t groups, uint8_t type);
+int64_t sxh_linear_fwd_workspace(const sxh_linear_inputs* in /* as the call gets it */);
 int32_t sxh_linear_fwd(sxh_backend* b, const sxh_linear_inputs* in, const sxh_linear_outputs* out, const sxh_queue* q);
 
 /* Its gradients, with dz = dy act'(pre) (relu's slope is 0 where pre is not above 0):
@@ -884,7 +884,7 @@ typedef struct {
     void* workspace;       /* sxh_linear_bwd_workspace(...) bytes of device memory, 16-byte aligned */
     int64_t workspace_bytes;
 } sxh_linear_grads;
-int64_t sxh_linear_bwd_workspace(int64_t rows, int64_t in, int64_t out, int64_t groups, uint8_t type);
+int64_t sxh_linear_bwd_workspace(const sxh_linear_grads_in* in /* as the call gets it, whichever gradients are wanted */);
 int32_t sxh_linear_bwd(sxh_backend* b, const sxh_linear_grads_in* in, const sxh_linear_grads* out, const sxh_queue* q);
 
 #ifdef __cplusplus

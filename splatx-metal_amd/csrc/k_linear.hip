@@ -11,17 +11,17 @@ auto with_type(ElemType t, F&& f) {
 }
 }  // namespace
 
-int64_t linear_fwd_workspace(int64_t rows, int64_t in, int64_t out, int groups, bool ragged, ElemType type) {
-    return with_type(type, [&](auto t) { return linear_fwd_workspace_of<decltype(t)>(rows, in, out, groups, ragged); });
+int64_t linear_fwd_workspace(const LinearFwdArgs& a, ElemType type) {
+    return with_type(type, [&](auto t) { return linear_fwd_of<decltype(t)>(a, nullptr, true); });
 }
-int64_t linear_bwd_workspace(int64_t rows, int64_t in, int64_t out, int groups, bool ragged, ElemType type) {
-    return with_type(type, [&](auto t) { return linear_bwd_workspace_of<decltype(t)>(rows, in, out, groups, ragged); });
+int64_t linear_bwd_workspace(const LinearBwdArgs& a, ElemType type) {
+    return with_type(type, [&](auto t) { return linear_bwd_of<decltype(t)>(a, nullptr, true); });
 }
 void linear_fwd(const LinearFwdArgs& a, ElemType type, hipStream_t s) {
-    with_type(type, [&](auto t) { linear_fwd_of<decltype(t)>(a, s); });
+    with_type(type, [&](auto t) { return linear_fwd_of<decltype(t)>(a, s, false); });
 }
 void linear_bwd(const LinearBwdArgs& a, ElemType type, hipStream_t s) {
-    with_type(type, [&](auto t) { linear_bwd_of<decltype(t)>(a, s); });
+    with_type(type, [&](auto t) { return linear_bwd_of<decltype(t)>(a, s, false); });
 }
 
 }  // namespace sxk

@@ -3,19 +3,15 @@
 
 namespace sxk {
 template <>
-void linear_fwd_of<__bf16>(const LinearFwdArgs& a, hipStream_t s) {
-    forward<__bf16>(a, s);
+int64_t linear_fwd_of<__bf16>(const LinearFwdArgs& a, hipStream_t s, bool measure) {
+    Run run{Work(measure ? nullptr : a.workspace), s, !measure};
+    forward<__bf16>(a, run);
+    return run.work.most();
 }
 template <>
-void linear_bwd_of<__bf16>(const LinearBwdArgs& a, hipStream_t s) {
-    backward<__bf16>(a, s);
-}
-template <>
-int64_t linear_fwd_workspace_of<__bf16>(int64_t rows, int64_t in, int64_t out, int groups, bool ragged) {
-    return forward_workspace<__bf16>(rows, in, out, groups, ragged);
-}
-template <>
-int64_t linear_bwd_workspace_of<__bf16>(int64_t rows, int64_t in, int64_t out, int groups, bool ragged) {
-    return backward_workspace<__bf16>(rows, in, out, groups, ragged);
+int64_t linear_bwd_of<__bf16>(const LinearBwdArgs& a, hipStream_t s, bool measure) {
+    Run run{Work(measure ? nullptr : a.workspace), s, !measure};
+    backward<__bf16>(a, run);
+    return run.work.most();
 }
 }  // namespace sxk

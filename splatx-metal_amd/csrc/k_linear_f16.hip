@@ -3,19 +3,15 @@
 
 namespace sxk {
 template <>
-void linear_fwd_of<_Float16>(const LinearFwdArgs& a, hipStream_t s) {
-    forward<_Float16>(a, s);
+int64_t linear_fwd_of<_Float16>(const LinearFwdArgs& a, hipStream_t s, bool measure) {
+    Run run{Work(measure ? nullptr : a.workspace), s, !measure};
+    forward<_Float16>(a, run);
+    return run.work.most();
 }
 template <>
-void linear_bwd_of<_Float16>(const LinearBwdArgs& a, hipStream_t s) {
-    backward<_Float16>(a, s);
-}
-template <>
-int64_t linear_fwd_workspace_of<_Float16>(int64_t rows, int64_t in, int64_t out, int groups, bool ragged) {
-    return forward_workspace<_Float16>(rows, in, out, groups, ragged);
-}
-template <>
-int64_t linear_bwd_workspace_of<_Float16>(int64_t rows, int64_t in, int64_t out, int groups, bool ragged) {
-    return backward_workspace<_Float16>(rows, in, out, groups, ragged);
+int64_t linear_bwd_of<_Float16>(const LinearBwdArgs& a, hipStream_t s, bool measure) {
+    Run run{Work(measure ? nullptr : a.workspace), s, !measure};
+    backward<_Float16>(a, run);
+    return run.work.most();
 }
 }  // namespace sxk

@@ -27,6 +27,29 @@ void need_sizes(const char* what, int64_t rows, int64_t in, int64_t out, int64_t
     if (!ends != !groups) invalid(what, "ends is given with groups, and only then");
 }
 
+bool valid(int64_t rows, int64_t in, int64_t out, int64_t groups, uint8_t type) { return sizes_fit(rows, in, out, groups) && type <= SXH_TYPE_F16; }
+
+sxk::LinearFwdArgs arguments(const sxh_linear_inputs& in, const sxh_linear_outputs& out) {
+    sxk::LinearFwdArgs a{};
+    a.x = in.x; a.weight = in.weight; a.bias = in.bias; a.residual = in.residual;
+    a.y = out.y; a.pre = out.pre; a.ends = in.ends;
+    a.rows = in.rows; a.in = in.in; a.out = in.out;
+    a.x_stride = in.x_stride; a.residual_stride = in.residual_stride; a.y_stride = out.y_stride; a.pre_stride = out.pre_stride;
+    a.groups = in.groups ? static_cast<int>(in.groups) : 1;
+    a.act = in.activation; a.clear = in.clear != 0; a.workspace = out.workspace;
+    return a;
+}
+sxk::LinearBwdArgs arguments(const sxh_linear_grads_in& in, const sxh_linear_grads& out) {
+    sxk::LinearBwdArgs a{};
+    a.dy = in.dy; a.pre = in.pre; a.x = in.x; a.weight = in.weight; a.ends = in.ends;
+    a.dx = out.dx; a.dweight = out.dweight; a.dbias = out.dbias;
+    a.rows = in.rows; a.in = in.in; a.out = in.out;
+    a.dy_stride = in.dy_stride; a.pre_stride = in.pre_stride; a.x_stride = in.x_stride; a.dx_stride = out.dx_stride;
+    a.groups = in.groups ? static_cast<int>(in.groups) : 1;
+    a.act = in.activation; a.clear = in.clear != 0; a.workspace = out.workspace;
+    return a;
+}
+
 int64_t need_workspace(RowCheck& c, void* workspace, int64_t given, int64_t bytes, const char* function) {
     if (given < bytes) invalid(c.what, "workspace_bytes is " + std::to_string(given) + ", " + function + " " + std::to_string(bytes));
     if (bytes) {
@@ -43,9 +66,9 @@ using namespace sxh;
 
 extern "C" {
 
-int64_t sxh_linear_fwd_workspace(int64_t rows, int64_t in, int64_t out, int64_t groups, uint8_t type) {
-    if (!sizes_fit(rows, in, out, groups) || type > SXH_TYPE_F16) return 0;
-    return sxk::linear_fwd_workspace(rows, in, out, groups ? static_cast<int>(groups) : 1, groups != 0, elem(type));
+int64_t sxh_linear_fwd_workspace(const sxh_linear_inputs* in) {
+    if (!in || !valid(in->rows, in->in, in->out, in->groups, in->type)) return 0;
+    return sxk::linear_fwd_workspace(arguments(*in, sxh_linear_outputs{}), elem(in->type));
 }
 
 int32_t sxh_linear_fwd(sxh_backend* b, const sxh_linear_inputs* in, const sxh_linear_outputs* out, const sxh_queue* q) {
@@ -65,25 +88,22 @@ int32_t sxh_linear_fwd(sxh_backend* b, const sxh_linear_inputs* in, const sxh_li
         if (in->groups) c.add_flat(in->ends, in->groups, 8, "ends", false);
         c.add(out->y, out->y_stride, in->out, e, "y", true);
         if (out->pre) c.add(out->pre, out->pre_stride, in->out, e, "pre", true);
-        need_workspace(c, out->workspace, out->workspace_bytes, sxh_linear_fwd_workspace(in->rows, in->in, in->out, in->groups, in->type),
+        need_workspace(c, out->workspace, out->workspace_bytes, sxh_linear_fwd_workspace(in),
                        "sxh_linear_fwd_workspace");
         c.disjoint();
         if (in->rows == 0) return;
         Queue on(b, q, what);
-        sxk::LinearFwdArgs a{};
-        a.x = in->x; a.weight = in->weight; a.bias = in->bias; a.residual = in->residual;
-        a.y = out->y; a.pre = out->pre; a.ends = in->ends;
-        a.rows = in->rows; a.in = in->in; a.out = in->out;
-        a.x_stride = in->x_stride; a.residual_stride = in->residual_stride; a.y_stride = out->y_stride; a.pre_stride = out->pre_stride;
-        a.groups = static_cast<int>(weights); a.act = in->activation; a.clear = in->clear != 0; a.workspace = out->workspace;
-        sxk::linear_fwd(a, elem(in->type), on.stream());
+        sxk::linear_fwd(arguments(*in, *out), elem(in->type), on.stream());
         on.done();
     });
 }
 
-int64_t sxh_linear_bwd_workspace(int64_t rows, int64_t in, int64_t out, int64_t groups, uint8_t type) {
-    if (!sizes_fit(rows, in, out, groups) || type > SXH_TYPE_F16) return 0;
-    return sxk::linear_bwd_workspace(rows, in, out, groups ? static_cast<int>(groups) : 1, groups != 0, elem(type));
+int64_t sxh_linear_bwd_workspace(const sxh_linear_grads_in* in) {
+    if (!in || !valid(in->rows, in->in, in->out, in->groups, in->type)) return 0;
+    char some = 0;  // (not read or written: all gradients are wanted)
+    sxh_linear_grads out{};
+    out.dx = out.dweight = out.dbias = &some;
+    return sxk::linear_bwd_workspace(arguments(*in, out), elem(in->type));
 }
 
 int32_t sxh_linear_bwd(sxh_backend* b, const sxh_linear_grads_in* in, const sxh_linear_grads* out, const sxh_queue* q) {
@@ -106,17 +126,11 @@ int32_t sxh_linear_bwd(sxh_backend* b, const sxh_linear_grads_in* in, const sxh_
         if (out->dx) c.add(out->dx, out->dx_stride, in->in, e, "dx", true);
         if (out->dweight) c.add_flat(out->dweight, weights * in->in * in->out, e, "dweight", true);
         if (out->dbias) c.add_flat(out->dbias, weights * in->out, e, "dbias", true);
-        need_workspace(c, out->workspace, out->workspace_bytes, sxh_linear_bwd_workspace(in->rows, in->in, in->out, in->groups, in->type),
+        need_workspace(c, out->workspace, out->workspace_bytes, sxh_linear_bwd_workspace(in),
                        "sxh_linear_bwd_workspace");
         c.disjoint();
         Queue on(b, q, what);
-        sxk::LinearBwdArgs a{};
-        a.dy = in->dy; a.pre = in->pre; a.x = in->x; a.weight = in->weight; a.ends = in->ends;
-        a.dx = out->dx; a.dweight = out->dweight; a.dbias = out->dbias;
-        a.rows = in->rows; a.in = in->in; a.out = in->out;
-        a.dy_stride = in->dy_stride; a.pre_stride = in->pre_stride; a.x_stride = in->x_stride; a.dx_stride = out->dx_stride;
-        a.groups = static_cast<int>(weights); a.act = in->activation; a.clear = in->clear != 0; a.workspace = out->workspace;
-        sxk::linear_bwd(a, elem(in->type), on.stream());
+        sxk::linear_bwd(arguments(*in, *out), elem(in->type), on.stream());
         on.done();
     });
 }

@@ -105,7 +105,8 @@ struct LinearFwdArgs {
     bool clear;  // rows of no group become zero
     void* workspace;
 };
-int64_t linear_fwd_workspace(int64_t rows, int64_t in, int64_t out, int groups, bool ragged, ElemType type);
+// Bytes of a call's workspace (the arguments as they will be but for the workspace; of a backward whichever gradients it names).
+int64_t linear_fwd_workspace(const LinearFwdArgs& a, ElemType type);
 void linear_fwd(const LinearFwdArgs& a, ElemType type, hipStream_t s);
 
 struct LinearBwdArgs {
@@ -117,16 +118,12 @@ struct LinearBwdArgs {
     bool clear;
     void* workspace;
 };
-int64_t linear_bwd_workspace(int64_t rows, int64_t in, int64_t out, int groups, bool ragged, ElemType type);
+int64_t linear_bwd_workspace(const LinearBwdArgs& a, ElemType type);
 void linear_bwd(const LinearBwdArgs& a, ElemType type, hipStream_t s);
-// The same for one type of elements (float, __bf16, _Float16).
+// The same for one type of elements (float, __bf16, _Float16); `measure`: nothing runs. Both give the workspace's bytes.
 template <class T>
-int64_t linear_fwd_workspace_of(int64_t rows, int64_t in, int64_t out, int groups, bool ragged);
+int64_t linear_fwd_of(const LinearFwdArgs& a, hipStream_t s, bool measure);
 template <class T>
-int64_t linear_bwd_workspace_of(int64_t rows, int64_t in, int64_t out, int groups, bool ragged);
-template <class T>
-void linear_fwd_of(const LinearFwdArgs& a, hipStream_t s);
-template <class T>
-void linear_bwd_of(const LinearBwdArgs& a, hipStream_t s);
+int64_t linear_bwd_of(const LinearBwdArgs& a, hipStream_t s, bool measure);
 
 }  // namespace sxk

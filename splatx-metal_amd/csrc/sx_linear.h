@@ -7,6 +7,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstdint>
 #include <stdexcept>
 
 #include "sx_mma.h"
@@ -58,6 +59,7 @@ struct TileArgs {
     const void *row, *col;
     int64_t row_stride, col_stride;  // elements between the rows in memory
     int64_t col_group;               // elements between the groups' col operands
+    int64_t row_width, col_width;    // of an Across operand's rows in memory, whole fragments
     Finish to;                       // (its cols are the outputs')
     int64_t out_group;
     int64_t rows, depth;             // rows (of the products over rows), depth (of those over groups' rows): all groups'
@@ -263,17 +265,17 @@ __device__ inline void store_chunk(T* p, Floats<kPer<T>> f, int n) {
 template <class T>
 struct Unit {
     static constexpr int V = kPer<T>;
-    const Finish& a;
+    const Finish* f;
     int64_t r, c;
     int column, row, n, rows;
     Frag<T> residual[4];
 
-    __device__ Unit(const Finish& f, int64_t first, int64_t stop, int64_t col) : a(f), r(first), c(col) {
+    __device__ Unit(const Finish& a, int64_t first, int64_t stop, int64_t col) : f(&a), r(first), c(col) {
         column = threadIdx.x % 8 * V;
         row = threadIdx.x % 64 / 8;
         n = static_cast<int>(max(int64_t{0}, min(a.cols - c - column, int64_t{V})));
         rows = static_cast<int>(min(stop - r, int64_t{32}));
-        if (a.residual)
+        if (a.residual && rows > 0 && a.cols > c)
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const T* const p = static_cast<const T*>(a.residual) + (r * a.residual_stride + c) + min(row + 8 * i, rows - 1) * a.residual_stride;
@@ -286,6 +288,7 @@ struct Unit {
 
     // The sums, bias included, through the wave's LDS.
     __device__ void finish(const Sums (&sums)[kUnitTiles<T>], char* lds) const {
+        const Finish& a = *f;
         const int lane = threadIdx.x % 64;
         wave_sees();  // (what was there has been read)
 #pragma unroll
@@ -353,7 +356,7 @@ __device__ inline void store_unit(const Finish& a, int64_t r, int64_t stop, int6
 
 // BR x BC outputs a workgroup, WR x WC a wave. OverRows: the sums go over a group's rows (dW), else the outputs' rows are the
 // groups' rows.
-template <class T, int BR, int BC, int WR, int WC, bool RowAcross, bool ColAcross, bool Direct>
+template <class T, int BR, int BC, int WR, int WC, bool RowAcross, bool ColAcross>
 __global__ void __launch_bounds__(BR / WR * (BC / WC) * 64) k_tile(TileArgs a) {
     constexpr bool OverRows = RowAcross;
     constexpr int kWaves = BR / WR * (BC / WC), kThreads = kWaves * 64, kDepth = 128 / static_cast<int>(sizeof(T));
@@ -391,31 +394,20 @@ __global__ void __launch_bounds__(BR / WR * (BC / WC) * 64) k_tile(TileArgs a) {
             for (int c = threadIdx.x % 32 * 4; c < BC; c += 128) clear4<T>(a.to, r, c0 + c);
         return;
     }
+    // (the bias of the tile's columns, a thread's one, goes to LDS in the end)
+    float own_bias = 0.0f;
+    if (a.bias && threadIdx.x < BC && c0 + threadIdx.x < a.to.cols)
+        own_bias = static_cast<float>(static_cast<const T*>(a.bias)[part.group * a.bias_group + c0 + threadIdx.x]);
     Sums sums[I][J];
 #pragma unroll
     for (int i = 0; i < I; i++)
 #pragma unroll
         for (int j = 0; j < J; j++) sums[i][j] = Sums(0.0f);
-    const auto multiply = [&](const char* buffer) {
-#pragma unroll
-        for (int s = 0; s < 4; s++) {
-            Frag<T> fr[I], fc[J];
-#pragma unroll
-            for (int i = 0; i < I; i++) fr[i] = fragment<T, BR, RowAcross>(buffer, wr + i * 32, s);
-#pragma unroll
-            for (int j = 0; j < J; j++) fc[j] = fragment<T, BC, ColAcross>(buffer + BR * 128, wc + j * 32, s);
-#pragma unroll
-            for (int i = 0; i < I; i++)
-#pragma unroll
-                for (int j = 0; j < J; j++) mma(sums[i][j], fc[j], fr[i]);
-        }
-    };
     const T *const rows_from = static_cast<const T*>(a.row), *const cols_from = static_cast<const T*>(a.col) + part.group * a.col_group;
-    Stage<T, BR, RowAcross, kThreads> row(rows_from, a.row_stride, r0, r1);
-    Stage<T, BC, ColAcross, kThreads> col(cols_from, a.col_stride, c0, a.to.cols);
-    if constexpr (Direct) {
-        DirectStage<T, BR, RowAcross, kThreads> rows(rows_from, a.row_stride, r0, r1, d0);
-        DirectStage<T, BC, ColAcross, kThreads> cols(cols_from, a.col_stride, c0, a.to.cols, d0);
+    const int64_t row_end = RowAcross ? a.row_width : r1, col_end = ColAcross ? a.col_width : a.to.cols;
+    DirectStage<T, BR, RowAcross, kThreads> rows(rows_from, a.row_stride, r0, row_end, d0);
+    DirectStage<T, BC, ColAcross, kThreads> cols(cols_from, a.col_stride, c0, col_end, d0);
+    {
         const int64_t whole = (d1 - d0) / kDepth;
         // The fragments of a step are read while the products of the step before it run, also over the end of a tile: when the
         // last step's are there the tile's place in LDS is free, and the next tile's loads, as long on their way as a tile's
@@ -474,75 +466,63 @@ __global__ void __launch_bounds__(BR / WR * (BC / WC) * 64) k_tile(TileArgs a) {
             }
         }
         if (d0 + whole * kDepth < d1) {
+            Stage<T, BR, RowAcross, kThreads> row(rows_from, a.row_stride, r0, row_end);
+            Stage<T, BC, ColAcross, kThreads> col(cols_from, a.col_stride, c0, col_end);
             row.load(d0 + whole * kDepth, d1);
             col.load(d0 + whole * kDepth, d1);
             __syncthreads();
             row.store(lds);
             col.store(lds + BR * 128);
             __syncthreads();
-            multiply(lds);
+            read(0, lds, 0);
+#pragma unroll
+            for (int s = 0; s < 4; s++) {
+                if (s < 3) read((s + 1) % 2, lds, s + 1);
+                product(s % 2);
+            }
         }
         __syncthreads();
-    } else {
-        if (d0 < d1) {
-            row.load(d0, d1);
-            col.load(d0, d1);
-            row.store(lds);
-            col.store(lds + BR * 128);
-        }
-        __syncthreads();
-        char *now = lds, *next = lds1;
-        for (int64_t d = d0; d < d1; d += kDepth) {
-            const bool more = d + kDepth < d1;
-            if (more) {
-                row.load(d + kDepth, d1);
-                col.load(d + kDepth, d1);
-            }
-            multiply(now);
-            if (more) {
-                row.store(next);
-                col.store(next + BR * 128);
-            }
-            __syncthreads();
-            char* const t = now;
-            now = next;
-            next = t;
-        }
     }
-    static_assert((kWaves + 1) / 2 * kUnitBytes<T> <= kBuffer);
+    float* const bias = reinterpret_cast<float*>(lds + kBuffer - BC * 4);
+    if (a.bias) {
+        if (threadIdx.x < BC) bias[threadIdx.x] = own_bias;
+        __syncthreads();
+    }
+    static_assert((kWaves + 1) / 2 * kUnitBytes<T> + BC * 4 <= kBuffer && BC <= kThreads);
     char* const mine = (wave % 2 ? lds1 : lds) + wave / 2 * kUnitBytes<T>;
     Finish to = a.to;
     to.out = static_cast<T*>(to.out) + part.group * a.out_group;
+    // (a unit's residual is on its way while the one before it is finished)
+    constexpr int kAcross = J / kUnitTiles<T>;
+    const auto unit_of = [&](int n) { return Unit<T>(to, r0 + wr + n / kAcross * 32, r1, c0 + wc + n % kAcross * kUnitTiles<T> * 32); };
+    Unit<T> next = unit_of(0);
 #pragma unroll
-    for (int i = 0; i < I; i++) {
-        const int64_t r = r0 + wr + i * 32;
-        if (r >= r1) break;
+    for (int n = 0; n < I * kAcross; n++) {
+        const Unit<T> now = next;
+        if (n + 1 < I * kAcross) next = unit_of(n + 1);
+        if (now.rows <= 0 || now.c >= a.to.cols) continue;
+        Sums unit[kUnitTiles<T>];
 #pragma unroll
-        for (int j = 0; j < J; j += kUnitTiles<T>) {
-            const int64_t c = c0 + wc + j * 32;
-            if (c >= a.to.cols) break;
-            Sums unit[kUnitTiles<T>];
+        for (int u = 0; u < kUnitTiles<T>; u++) {
+            unit[u] = sums[n / kAcross][n % kAcross * kUnitTiles<T> + u];
 #pragma unroll
-            for (int u = 0; u < kUnitTiles<T>; u++) {
-                unit[u] = sums[i][j + u];
+            for (int q = 0; q < 4; q++) {
+                const int place = u * 32 + 8 * q + lane / 32 * 4;
+                if (a.partial) {
+                    const int64_t r = now.r + lane % 32, at = now.c + place;
+                    const Floats<4> v = {unit[u][4 * q], unit[u][4 * q + 1], unit[u][4 * q + 2], unit[u][4 * q + 3]};
+                    store_some<float, 4>(a.partial + (int64_t{blockIdx.y} * a.rows + r) * a.to.cols + at, v,
+                                         r < r1 ? static_cast<int>(max(int64_t{0}, min(a.to.cols - at, int64_t{4}))) : 0);
+                } else if (a.bias) {
+                    const Floats<4> v = *reinterpret_cast<const Floats<4>*>(bias + static_cast<int>(now.c - c0) + place);
 #pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    const int64_t at = c + u * 32 + 8 * q + lane / 32 * 4;
-                    const int n = static_cast<int>(max(int64_t{0}, min(a.to.cols - at, int64_t{4})));
-                    if (a.partial) {
-                        const Floats<4> v = {unit[u][4 * q], unit[u][4 * q + 1], unit[u][4 * q + 2], unit[u][4 * q + 3]};
-                        store_some<float, 4>(a.partial + (int64_t{blockIdx.y} * a.rows + r + lane % 32) * a.to.cols + at, v, r + lane % 32 < r1 ? n : 0);
-                    } else if (a.bias) {
-                        const Floats<4> v = load_some<T, 4>(static_cast<const T*>(a.bias) + part.group * a.bias_group + at, n);
-#pragma unroll
-                        for (int e = 0; e < 4; e++) unit[u][4 * q + e] += v[e];
-                    }
+                    for (int e = 0; e < 4; e++) unit[u][4 * q + e] += v[e];
                 }
             }
-            if (a.partial) continue;
-            if constexpr (ColAcross) store_unit<T>(to, r, r1, c, unit, mine);
-            else Unit<T>(to, r, r1, c).finish(unit, mine);
         }
+        if (a.partial) continue;
+        if constexpr (ColAcross) store_unit<T>(to, now.r, r1, now.c, unit, mine);
+        else now.finish(unit, mine);
     }
 }
 
@@ -949,30 +929,26 @@ struct FewArgs {
     Groups groups;
 };
 constexpr int kFewWaves = 8;
-// R times 32 rows a part.
-template <class T, int R>
+constexpr int kFewShift = 5;  // a part: 32 rows
+template <class T>
 __global__ void __launch_bounds__(kFewWaves * 64) k_few_fwd(FewArgs a) {
-    constexpr int V = kPer<T>, kLine = 128 / static_cast<int>(sizeof(T)), kAtOnce = R == 1 ? 4 : 2, kPitch = 36;
-    __shared__ float sums[kFewWaves][R * 32 * kPitch];
-    const Part part = part_of(a.groups, blockIdx.y, R == 1 ? 5 : 6);
+    constexpr int V = kPer<T>, kLine = 128 / static_cast<int>(sizeof(T)), kAtOnce = 4, kPitch = 36;
+    __shared__ float sums[kFewWaves][32 * kPitch];
+    const Part part = part_of(a.groups, blockIdx.y, kFewShift);
     if (part.begin >= part.end) return;
     const int64_t c0 = int64_t{blockIdx.x} * 32;
     const int lane = threadIdx.x % 64, half = lane / 32, wave = wave_of();
-    // (in the end a thread, of R 1 one of the first half, has four outputs)
+    // (in the end a thread of the first half has four outputs)
     const int64_t r = part.begin + threadIdx.x / 8, c = c0 + threadIdx.x % 8 * 4;
     if (part.group >= a.groups.groups) {
-        if (threadIdx.x < R * 256 && r < part.end) clear4<T>(a.to, r, c);
+        if (threadIdx.x < 256 && r < part.end) clear4<T>(a.to, r, c);
         return;
     }
     const T* const w = static_cast<const T*>(a.weight) + (part.group * a.out + min(c0 + lane % 32, a.out - 1)) * a.in;
-    const T* x[R];
-#pragma unroll
-    for (int b = 0; b < R; b++) x[b] = static_cast<const T*>(a.x) + min(part.begin + b * 32 + lane % 32, part.end - 1) * a.x_stride;
-    Sums s[R];
-#pragma unroll
-    for (int b = 0; b < R; b++) s[b] = Sums(0.0f);
+    const T* const x = static_cast<const T*>(a.x) + min(part.begin + lane % 32, part.end - 1) * a.x_stride;
+    Sums s(0.0f);
     for (int64_t k = wave * kLine; k < a.in; k += kFewWaves * kAtOnce * kLine) {
-        Frag<T> fw[kAtOnce][4], fx[R][kAtOnce][4];
+        Frag<T> fw[kAtOnce][4], fx[kAtOnce][4];
         const auto load_all = [&](auto load) {
 #pragma unroll
             for (int t = 0; t < kAtOnce; t++)
@@ -980,8 +956,7 @@ __global__ void __launch_bounds__(kFewWaves * 64) k_few_fwd(FewArgs a) {
                 for (int i = 0; i < 4; i++) {
                     const int64_t at = k + t * kFewWaves * kLine + (2 * i + half) * V;
                     fw[t][i] = load(w, at);
-#pragma unroll
-                    for (int b = 0; b < R; b++) fx[b][t][i] = load(x[b], at);
+                    fx[t][i] = load(x, at);
                 }
         };
         if (k + (kAtOnce - 1) * kFewWaves * kLine + kLine <= a.in) load_all([&](const T* p, int64_t at) { return load_raw<V>(p + at); });
@@ -990,18 +965,13 @@ __global__ void __launch_bounds__(kFewWaves * 64) k_few_fwd(FewArgs a) {
 #pragma unroll
         for (int t = 0; t < kAtOnce; t++)
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int b = 0; b < R; b++) mma(s[b], fw[t][i], fx[b][t][i]);
+            for (int i = 0; i < 4; i++) mma(s, fw[t][i], fx[t][i]);
     }
 #pragma unroll
-    for (int b = 0; b < R; b++)
-#pragma unroll
-        for (int q = 0; q < 4; q++)
-            *reinterpret_cast<Floats<4>*>(&sums[wave][(b * 32 + lane % 32) * kPitch + half * 4 + q * 8]) =
-                Floats<4>{s[b][4 * q], s[b][4 * q + 1], s[b][4 * q + 2], s[b][4 * q + 3]};
+    for (int q = 0; q < 4; q++)
+        *reinterpret_cast<Floats<4>*>(&sums[wave][lane % 32 * kPitch + half * 4 + q * 8]) = Floats<4>{s[4 * q], s[4 * q + 1], s[4 * q + 2], s[4 * q + 3]};
     __syncthreads();
-    if (threadIdx.x >= R * 256 || r >= part.end || c >= a.out) return;
+    if (threadIdx.x >= 256 || r >= part.end || c >= a.out) return;
     Floats<4> v(0.0f);
 #pragma unroll
     for (int k = 0; k < kFewWaves; k++) v += *reinterpret_cast<const Floats<4>*>(&sums[k][threadIdx.x / 8 * kPitch + threadIdx.x % 8 * 4]);
@@ -1057,9 +1027,9 @@ __global__ void __launch_bounds__(256) k_slope(SlopeArgs a, int lanes) {
                     if (a.act) pre[i] = moved_down<T>(pre[i], past);
                 }
                 Floats<V> d = floats<T, V>(dy[i]);
-                if (a.act) {
-                    through<T, V>(d, floats<T, V>(pre[i]), a.act);
-                    if (a.dz) store_some<T, V>(static_cast<T*>(a.dz) + r * a.dz_stride + c, d, n);
+                if (a.act) through<T, V>(d, floats<T, V>(pre[i]), a.act);
+                if (a.dz) {
+                    store_some<T, V>(static_cast<T*>(a.dz) + r * a.dz_stride + c, d, n);
                 }
                 sum += d;
             }
@@ -1173,11 +1143,59 @@ Slope plan_slope(int64_t rows, int64_t cols, int groups, bool ragged, int elem) 
     return p;
 }
 
-constexpr int64_t kAlign = 256;
-int64_t aligned(int64_t bytes) { return (bytes + kAlign - 1) / kAlign * kAlign; }
+// A call's workspace, handed out from its beginning; without memory only how much there has to be.
+class Work {
+  public:
+    explicit Work(void* base) : base_(static_cast<char*>(base)) {}
+    char* take(int64_t bytes) {
+        char* const p = base_ ? base_ + used_ : nullptr;
+        used_ += (bytes + 255) / 256 * 256;
+        most_ = std::max(most_, used_);
+        return p;
+    }
+    int64_t used() const { return used_; }
+    void back_to(int64_t used) { used_ = used; }
+    int64_t most() const { return most_; }
+
+  private:
+    char* base_;
+    int64_t used_ = 0, most_ = 0;
+};
+// Where a call is enqueued, or that it is only measured.
+struct Run {
+    Work work;
+    hipStream_t stream;
+    bool real;
+};
 
 void check_grid(int64_t blocks, int64_t threads) {
     if (blocks * threads >= int64_t{1} << 32) throw std::runtime_error("linear: more workgroups than a launch holds");
+}
+
+template <class T>
+void launch_slope(const SlopeArgs& a, const Slope& p, hipStream_t s) {
+    check_grid(p.slots * p.columns, 256);
+    k_slope<T><<<dim3(static_cast<uint32_t>(p.slots), static_cast<uint32_t>(p.columns)), 256, 0, s>>>(a, p.lanes);
+}
+
+// A product's operand as k_tile reads it: lines that begin on 16 bytes, their places in a tile in 32 bits, and across them whole
+// fragments. What lies otherwise is copied first, which takes two passes over it where loads of its own kind took the product
+// three times as long (377 rows of 5996 to 1162 bfloat16, dx 65 us for 20).
+struct Operand {
+    const void* p;
+    int64_t stride, width;
+};
+template <class T>
+Operand operand(const void* p, int64_t rows, int64_t width, int64_t stride, bool across, Run& run) {
+    const bool fits = reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * static_cast<int64_t>(sizeof(T)) % 16 == 0 &&
+                      stride < (int64_t{1} << 30) / 256 / static_cast<int>(sizeof(T)) && (!across || width % kPer<T> == 0);
+    if (fits || !rows) return {p, stride, width};
+    const Slope plan = plan_slope(rows, width, 1, false, sizeof(T));
+    SlopeArgs a{};
+    a.dy = p; a.dy_stride = stride; a.dz = run.work.take(plan.dz_bytes); a.dz_stride = plan.dz_stride;
+    a.cols = width; a.groups = {nullptr, 1, rows}; a.shift = plan.shift;
+    if (run.real) launch_slope<T>(a, plan, run.stream);
+    return {a.dz, plan.dz_stride, plan.dz_stride};
 }
 
 template <class T, bool RowAcross, bool ColAcross>
@@ -1185,18 +1203,9 @@ void launch_tiles(const TileArgs& a, int side, int64_t slabs, hipStream_t s) {
     const int64_t down = RowAcross ? up(a.rows, side) : a.slots, tiles = up(down * up(a.to.cols, side == 256 ? 256 : 128), 8) * 8;
     check_grid(tiles * slabs, side == 256 ? 512 : 256);
     const dim3 grid(static_cast<uint32_t>(tiles), static_cast<uint32_t>(slabs));
-    // straight into LDS: lines that begin on 16 bytes, and whose places in a tile 32 bits hold
-    const auto direct = [](const void* p, int64_t stride) {
-        return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * sizeof(T) % 16 == 0 && stride < (int64_t{1} << 30) / 256 / static_cast<int>(sizeof(T));
-    };
-    const bool whole = direct(a.row, a.row_stride) && direct(a.col, a.col_stride) && a.col_group * sizeof(T) % 16 == 0 &&
-                       (!RowAcross || a.rows % kPer<T> == 0) && (!ColAcross || a.to.cols % kPer<T> == 0);
-    if (side == 256 && whole) k_tile<T, 256, 256, 128, 64, RowAcross, ColAcross, true><<<grid, 512, 0, s>>>(a);
-    else if (side == 256) k_tile<T, 256, 256, 128, 64, RowAcross, ColAcross, false><<<grid, 512, 0, s>>>(a);
-    else if (side == 128 && whole) k_tile<T, 128, 128, 64, 64, RowAcross, ColAcross, true><<<grid, 256, 0, s>>>(a);
-    else if (side == 128) k_tile<T, 128, 128, 64, 64, RowAcross, ColAcross, false><<<grid, 256, 0, s>>>(a);
-    else if (whole) k_tile<T, 64, 128, 32, 64, RowAcross, ColAcross, true><<<grid, 256, 0, s>>>(a);
-    else k_tile<T, 64, 128, 32, 64, RowAcross, ColAcross, false><<<grid, 256, 0, s>>>(a);
+    if (side == 256) k_tile<T, 256, 256, 128, 64, RowAcross, ColAcross><<<grid, 512, 0, s>>>(a);
+    else if (side == 128) k_tile<T, 128, 128, 64, 64, RowAcross, ColAcross><<<grid, 256, 0, s>>>(a);
+    else k_tile<T, 64, 128, 32, 64, RowAcross, ColAcross><<<grid, 256, 0, s>>>(a);
 }
 
 // `slabs`: of a group, on average
@@ -1274,7 +1283,7 @@ void launch_narrow_bwd(const NarrowBwdArgs& a, const NarrowBwd& p, hipStream_t s
 }
 
 // Whether a forward's groups have so few rows that the weights' bytes are what it takes.
-bool few_rows(int64_t rows, int groups) { return rows <= 64 || rows / groups <= 32; }
+bool few_rows(int64_t rows, int groups) { return rows <= 32 || rows / groups <= 16; }
 
 template <class T>
 void launch_narrow(const NarrowArgs& a, const Narrow& p, hipStream_t s) {
@@ -1293,128 +1302,124 @@ void launch_narrow(const NarrowArgs& a, const Narrow& p, hipStream_t s) {
 
 // out = row col^T over the groups' rows (see TileArgs), with what follows.
 template <class T, bool ColAcross>
-void over_depth(TileArgs a, bool ragged, float* work, hipStream_t s) {
+void over_depth(TileArgs a, bool ragged, Run& run) {
     const Plan p = plan_rows(a.rows, a.to.cols, a.depth, a.groups.groups, ragged, sizeof(T));
     a.shift = log2_up(p.side);
     a.slots = slots_of(a.rows, a.groups.groups, a.shift, ragged);
     a.split = p.split;
     a.splits = p.splits;
-    a.partial = p.splits > 1 ? work : nullptr;
-    launch_tiles<T, false, ColAcross>(a, p.side, p.splits, s);
+    a.partial = p.splits > 1 ? reinterpret_cast<float*>(run.work.take(p.bytes)) : nullptr;
+    if (!run.real) return;
+    launch_tiles<T, false, ColAcross>(a, p.side, p.splits, run.stream);
     if (a.partial) {
         const int64_t blocks = std::min<int64_t>(up(a.rows * up(a.to.cols, 4), 256), 4096);
-        k_split_join<T><<<static_cast<uint32_t>(blocks), 256, 0, s>>>(a);
+        k_split_join<T><<<static_cast<uint32_t>(blocks), 256, 0, run.stream>>>(a);
     }
 }
 
 template <class T>
-void forward(const LinearFwdArgs& f, hipStream_t s) {
+void forward(const LinearFwdArgs& f, Run& run) {
     const Finish to{f.y, f.y_stride, f.out, f.residual, f.residual_stride, f.pre, f.pre_stride, f.act, f.clear};
-    if (const Narrow p = plan_narrow<T>(f.rows, f.in, f.out, f.ends != nullptr); p.blocks) {
-        launch_narrow<T>({f.x, f.weight, f.bias, f.x_stride, to, f.in, f.out, p.chunk, {f.ends, f.groups, f.rows}}, p, s);
+    const Groups groups{f.ends, f.groups, f.rows};
+    const bool ragged = f.ends != nullptr;
+    if (const Narrow p = plan_narrow<T>(f.rows, f.in, f.out, ragged); p.blocks) {
+        if (run.real) launch_narrow<T>({f.x, f.weight, f.bias, f.x_stride, to, f.in, f.out, p.chunk, groups}, p, run.stream);
         return;
     }
     if (few_rows(f.rows, f.groups)) {
-        const bool two = f.rows > 32 && f.rows / f.groups > 16;
-        const int64_t slots = slots_of(f.rows, f.groups, two ? 6 : 5, f.ends != nullptr), blocks = up(f.out, 32);
+        const int64_t slots = slots_of(f.rows, f.groups, kFewShift, ragged), blocks = up(f.out, 32);
+        if (!run.real) return;
         check_grid(blocks * slots, kFewWaves * 64);
-        const dim3 grid(static_cast<uint32_t>(blocks), static_cast<uint32_t>(slots));
-        const FewArgs a{f.x, f.weight, f.bias, f.x_stride, to, f.in, f.out, {f.ends, f.groups, f.rows}};
-        if (two) k_few_fwd<T, 2><<<grid, kFewWaves * 64, 0, s>>>(a);
-        else k_few_fwd<T, 1><<<grid, kFewWaves * 64, 0, s>>>(a);
+        k_few_fwd<T><<<dim3(static_cast<uint32_t>(blocks), static_cast<uint32_t>(slots)), kFewWaves * 64, 0, run.stream>>>(
+            {f.x, f.weight, f.bias, f.x_stride, to, f.in, f.out, groups});
         return;
     }
+    const Operand x = operand<T>(f.x, f.rows, f.in, f.x_stride, false, run);
+    const Operand w = operand<T>(f.weight, f.groups * f.out, f.in, f.in, false, run);
     TileArgs a{};
-    a.row = f.x; a.row_stride = f.x_stride; a.col = f.weight; a.col_stride = f.in; a.col_group = f.in * f.out;
-    a.rows = f.rows; a.depth = f.in;
-    a.groups = {f.ends, f.groups, f.rows};
-    a.bias = f.bias; a.bias_group = f.out;
-    a.to = to;
-    over_depth<T, false>(a, f.ends != nullptr, static_cast<float*>(f.workspace), s);
+    a.row = x.p; a.row_stride = x.stride; a.col = w.p; a.col_stride = w.stride; a.col_group = w.stride * f.out;
+    a.rows = f.rows; a.depth = f.in; a.groups = groups; a.bias = f.bias; a.bias_group = f.out; a.to = to;
+    over_depth<T, false>(a, ragged, run);
 }
 
 template <class T>
-void backward(const LinearBwdArgs& f, hipStream_t s) {
+void backward_narrow(const LinearBwdArgs& f, const NarrowBwd& p, Run& run) {
+    NarrowBwdArgs a{};
+    a.dy = f.dy; a.pre = f.pre; a.x = f.dweight ? f.x : nullptr; a.weight = f.weight;
+    a.dy_stride = f.dy_stride; a.pre_stride = f.pre_stride; a.x_stride = f.x_stride;
+    a.to.out = f.dx; a.to.out_stride = f.dx_stride; a.to.cols = f.in; a.to.clear = f.clear;
+    a.in = f.in; a.out = f.out; a.chunk = p.chunk; a.size = p.size; a.groups = {f.ends, f.groups, f.rows}; a.act = f.act;
+    const bool sums = f.dweight || f.dbias;
+    if (sums) a.partial = reinterpret_cast<float*>(run.work.take(p.bytes));
+    if (!run.real) return;
+    if (f.rows) launch_narrow_bwd<T>(a, p, run.stream);
+    if (!sums) return;
+    JoinArgs j{};
+    j.partial = a.partial; j.dweight = f.dweight; j.dbias = f.dbias; j.weights = f.in * f.out; j.size = p.size;
+    j.wanted = f.dbias ? p.size : j.weights;
+    j.groups = a.groups; j.step = p.chunk; j.slabs = f.ends || !f.rows ? 0 : p.blocks;
+    join_weights<T>(j, p.blocks / f.groups + 1, run.stream);
+}
+
+template <class T>
+void backward(const LinearBwdArgs& f, Run& run) {
     const bool ragged = f.ends != nullptr;
-    const Slope slope = plan_slope(f.rows, f.out, f.groups, ragged, sizeof(T));
     const Groups groups{f.ends, f.groups, f.rows};
-    char* work = static_cast<char*>(f.workspace);
     if (const NarrowBwd p = plan_narrow_bwd<T>(f.rows, f.in, f.out, f.groups); p.blocks) {
-        NarrowBwdArgs a{};
-        a.dy = f.dy; a.pre = f.pre; a.x = f.dweight ? f.x : nullptr; a.weight = f.weight;
-        a.dy_stride = f.dy_stride; a.pre_stride = f.pre_stride; a.x_stride = f.x_stride;
-        a.to.out = f.dx; a.to.out_stride = f.dx_stride; a.to.cols = f.in; a.to.clear = f.clear;
-        a.in = f.in; a.out = f.out; a.chunk = p.chunk; a.size = p.size; a.groups = groups; a.act = f.act;
-        const bool sums = f.dweight || f.dbias;
-        a.partial = sums ? reinterpret_cast<float*>(work) : nullptr;
-        if (f.rows) launch_narrow_bwd<T>(a, p, s);
-        if (sums) {
-            JoinArgs j{};
-            j.partial = a.partial; j.dweight = f.dweight; j.dbias = f.dbias; j.weights = f.in * f.out; j.size = p.size; j.wanted = f.dbias ? p.size : j.weights;
-            j.groups = groups; j.step = p.chunk; j.slabs = ragged || !f.rows ? 0 : p.blocks;
-            join_weights<T>(j, p.blocks / f.groups + 1, s);
-        }
+        backward_narrow<T>(f, p, run);
         return;
     }
-    const void* dz = f.dy;
-    int64_t dz_stride = f.dy_stride;
-    const bool products = f.dx || f.dweight;
-    if (f.dbias || (f.act && products)) {
+    // dz, where it is not dy itself, and its columns' sums
+    Operand dz{f.dy, f.dy_stride, f.out};
+    const bool products = f.dx || f.dweight, slopes = products && f.act;
+    if (f.dbias || slopes) {
+        const Slope slope = plan_slope(f.rows, f.out, f.groups, ragged, sizeof(T));
         SlopeArgs a{};
         a.dy = f.dy; a.pre = f.pre; a.dy_stride = f.dy_stride; a.pre_stride = f.pre_stride;
         a.cols = f.out; a.groups = groups; a.shift = slope.shift; a.act = f.act;
-        if (f.act && products) {
-            a.dz = work;
-            dz = work;
-            dz_stride = a.dz_stride = slope.dz_stride;
+        if (slopes) {
+            a.dz = run.work.take(slope.dz_bytes);
+            a.dz_stride = slope.dz_stride;
+            dz = {a.dz, slope.dz_stride, slope.dz_stride};
         }
-        work += aligned(slope.dz_bytes);
-        if (f.dbias) a.partial = reinterpret_cast<float*>(work);
-        work += aligned(slope.bytes);
-        check_grid(slope.slots * slope.columns, 256);
-        if (f.rows)
-            k_slope<T><<<dim3(static_cast<uint32_t>(slope.slots), static_cast<uint32_t>(slope.columns)), 256, 0, s>>>(a, slope.lanes);
-        if (f.dbias) {
+        if (f.dbias) a.partial = reinterpret_cast<float*>(run.work.take(slope.bytes));
+        if (run.real && f.rows) launch_slope<T>(a, slope, run.stream);
+        if (run.real && f.dbias) {
             JoinArgs j{};
             j.partial = a.partial; j.dbias = f.dbias; j.wanted = j.size = f.out;
             j.groups = groups; j.step = int64_t{1} << slope.shift; j.from_begin = true;
-            join_weights<T>(j, slope.slots / f.groups, s);
+            join_weights<T>(j, slope.slots / f.groups, run.stream);
         }
     }
+    if (!products) return;
+    if (!slopes) dz = operand<T>(f.dy, f.rows, f.out, f.dy_stride, f.dweight != nullptr, run);
+    const int64_t kept = run.work.used();
     if (f.dx && f.rows) {
+        const Operand w = operand<T>(f.weight, f.groups * f.out, f.in, f.in, true, run);
         TileArgs a{};
-        a.row = dz; a.row_stride = dz_stride; a.col = f.weight; a.col_stride = f.in; a.col_group = f.in * f.out;
-        a.to.out = f.dx; a.to.out_stride = f.dx_stride; a.to.cols = f.in; a.rows = f.rows; a.depth = f.out;
-        a.groups = groups; a.to.clear = f.clear;
-        over_depth<T, true>(a, ragged, reinterpret_cast<float*>(work), s);
+        a.row = dz.p; a.row_stride = dz.stride; a.col = w.p; a.col_stride = w.stride; a.col_group = w.stride * f.out; a.col_width = w.width;
+        a.to.out = f.dx; a.to.out_stride = f.dx_stride; a.to.cols = f.in; a.to.clear = f.clear;
+        a.rows = f.rows; a.depth = f.out; a.groups = groups;
+        over_depth<T, true>(a, ragged, run);
+        run.work.back_to(kept);
     }
     if (f.dweight) {
+        const Operand x = operand<T>(f.x, f.rows, f.in, f.x_stride, true, run);
         const Over p = plan_over(f.rows, f.out, f.in, f.groups, ragged, sizeof(T));
         TileArgs a{};
-        a.row = dz; a.row_stride = dz_stride; a.col = f.x; a.col_stride = f.x_stride;
+        a.row = dz.p; a.row_stride = dz.stride; a.row_width = dz.width; a.col = x.p; a.col_stride = x.stride; a.col_width = x.width;
         a.to.out = f.dweight; a.to.out_stride = f.in; a.to.cols = f.in; a.out_group = f.in * f.out; a.rows = f.out; a.depth = f.rows;
         a.groups = groups; a.shift = p.shift; a.slots = p.slots;
-        a.partial = p.bytes ? reinterpret_cast<float*>(work) : nullptr;
-        launch_tiles<T, true, true>(a, p.side, p.slots, s);
+        a.partial = p.bytes ? reinterpret_cast<float*>(run.work.take(p.bytes)) : nullptr;
+        if (!run.real) return;
+        launch_tiles<T, true, true>(a, p.side, p.slots, run.stream);
         if (a.partial) {
             JoinArgs j{};
             j.partial = a.partial; j.dweight = f.dweight; j.weights = j.wanted = j.size = f.in * f.out;
             j.groups = groups; j.step = int64_t{1} << p.shift; j.from_begin = true;
-            join_weights<T>(j, p.slots / f.groups, s);
+            join_weights<T>(j, p.slots / f.groups, run.stream);
         }
     }
-}
-
-template <class T>
-int64_t forward_workspace(int64_t rows, int64_t in, int64_t out, int groups, bool ragged) {
-    return plan_narrow<T>(rows, in, out, ragged).blocks || few_rows(rows, groups) ? 0 : plan_rows(rows, out, in, groups, ragged, sizeof(T)).bytes;
-}
-template <class T>
-int64_t backward_workspace(int64_t rows, int64_t in, int64_t out, int groups, bool ragged) {
-    if (const NarrowBwd narrow = plan_narrow_bwd<T>(rows, in, out, groups); narrow.blocks) return narrow.bytes;
-    const Slope slope = plan_slope(rows, out, groups, ragged, sizeof(T));
-    return aligned(slope.dz_bytes) + aligned(slope.bytes) +
-           std::max(plan_rows(rows, in, out, groups, ragged, sizeof(T)).bytes, plan_over(rows, out, in, groups, ragged, sizeof(T)).bytes);
 }
 
 }  // namespace

@@ -514,7 +514,7 @@ PyObject* linear_fwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
                 pre = rows_beside(*x.t, l.out);
                 out.pre = pre.data_ptr();
             }
-            out.workspace_bytes = sxh_linear_fwd_workspace(in.rows, in.in, in.out, in.groups, in.type);
+            out.workspace_bytes = sxh_linear_fwd_workspace(&in);
             if (out.workspace_bytes) {
                 work = at::empty({out.workspace_bytes}, x.t->options().dtype(at::kByte));
                 out.workspace = work.data_ptr();
@@ -568,7 +568,7 @@ PyObject* linear_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
                 dbias = at::empty(l.weights->sizes().slice(0, l.weights->dim() - 1), options);
                 out.dbias = dbias.data_ptr();
             }
-            out.workspace_bytes = sxh_linear_bwd_workspace(in.rows, in.in, in.out, in.groups, in.type);
+            out.workspace_bytes = sxh_linear_bwd_workspace(&in);
             if (out.workspace_bytes) {
                 work = at::empty({out.workspace_bytes}, options.dtype(at::kByte));
                 out.workspace = work.data_ptr();

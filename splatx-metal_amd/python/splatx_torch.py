@@ -154,7 +154,7 @@ class TorchBackend(sh.Backend):
             f = getattr(self.lib, "sxh_" + name)
             f.argtypes, f.restype = args, C.c_int32
         for name, args in (("layer_norm_bwd_workspace", (n, n)), ("grad_norm_workspace", (n,)),
-                           ("linear_fwd_workspace", (n, n, n, n, C.c_uint8)), ("linear_bwd_workspace", (n, n, n, n, C.c_uint8))):
+                           ("linear_fwd_workspace", (p,)), ("linear_bwd_workspace", (p,))):
             f = getattr(self.lib, "sxh_" + name)
             f.argtypes, f.restype = args, n
 

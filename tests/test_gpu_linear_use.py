@@ -287,14 +287,14 @@ def test_rows_of_no_group_are_left_as_they_were(tb, st, rows, n_in, n_out):
     dy[end:] = math.nan
     for clear in (0, 1):
         y, pre, dx = (torch.full((rows + 3, n), 7.5, device="cuda") for n in (n_out, n_out, n_in))
-        work = torch.empty(max(tb.lib.sxh_linear_fwd_workspace(rows, n_in, n_out, 2, 0), 16), dtype=torch.uint8, device="cuda")
+        a = st.LinearInputs(x.data_ptr(), w.data_ptr(), None, None, ends.data_ptr(), rows, n_in, n_out, 2, n_in, 0, 0, 2, clear)
+        work = torch.empty(max(tb.lib.sxh_linear_fwd_workspace(C.byref(a)), 16), dtype=torch.uint8, device="cuda")
         torch.cuda.synchronize()
-        rc = tb.lib.sxh_linear_fwd(tb.handle, C.byref(st.LinearInputs(x.data_ptr(), w.data_ptr(), None, None, ends.data_ptr(), rows, n_in, n_out, 2, n_in, 0, 0, 2, clear)),
-                                   C.byref(st.LinearOutputs(y.data_ptr(), pre.data_ptr(), n_out, n_out, work.data_ptr(), work.numel())), None)
+        rc = tb.lib.sxh_linear_fwd(tb.handle, C.byref(a), C.byref(st.LinearOutputs(y.data_ptr(), pre.data_ptr(), n_out, n_out, work.data_ptr(), work.numel())), None)
         assert rc == 0, tb.lib.sxh_last_error()
-        work = torch.empty(tb.lib.sxh_linear_bwd_workspace(rows, n_in, n_out, 2, 0), dtype=torch.uint8, device="cuda")
-        rc = tb.lib.sxh_linear_bwd(tb.handle, C.byref(st.LinearGradsIn(dy.data_ptr(), None, x.data_ptr(), w.data_ptr(), ends.data_ptr(), rows, n_in, n_out, 2, n_out, 0, n_in, 0, 0, clear)),
-                                   C.byref(st.LinearGrads(dx.data_ptr(), None, None, n_in, work.data_ptr(), work.numel())), None)
+        a = st.LinearGradsIn(dy.data_ptr(), None, x.data_ptr(), w.data_ptr(), ends.data_ptr(), rows, n_in, n_out, 2, n_out, 0, n_in, 0, 0, clear)
+        work = torch.empty(tb.lib.sxh_linear_bwd_workspace(C.byref(a)), dtype=torch.uint8, device="cuda")
+        rc = tb.lib.sxh_linear_bwd(tb.handle, C.byref(a), C.byref(st.LinearGrads(dx.data_ptr(), None, None, n_in, work.data_ptr(), work.numel())), None)
         assert rc == 0, tb.lib.sxh_last_error()
         left = 0.0 if clear else 7.5
         for t in (y, pre, dx):
@@ -387,7 +387,7 @@ def test_refusals(tb, st):
                  (i(w=wg, ends=ends, groups=30_000), o()), (i(stride=1 << 61), o())):
         assert call(a, c) == sh.SXH_ERR_INVALID_ARGUMENT
     g = st.LinearGradsIn(p(r), None, p(x), p(w), None, 40, 32, 24, 0, 24, 0, 32, 0, 0, 0)
-    n = tb.lib.sxh_linear_bwd_workspace(40, 32, 24, 0, 0)
+    n = tb.lib.sxh_linear_bwd_workspace(C.byref(g))
     work, dx, dw = torch.empty(n, dtype=torch.uint8, device="cuda"), torch.empty(40, 32, device="cuda"), torch.empty(24, 32, device="cuda")
     back = lambda *a: tb.lib.sxh_linear_bwd(tb.handle, C.byref(g), C.byref(st.LinearGrads(*[p(t) for t in a])), C.byref(st.Queue(None)))  # noqa: E731
     assert back(dx, dw, None, 32, work, n) == sh.SXH_OK

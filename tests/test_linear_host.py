@@ -23,7 +23,7 @@ def lib():
     lib = splatx_hip.load_library()
     for name in ("sxh_linear_fwd_workspace", "sxh_linear_bwd_workspace"):
         f = getattr(lib, name)
-        f.argtypes, f.restype = [C.c_int64] * 4 + [C.c_uint8], C.c_int64
+        f.argtypes, f.restype = [C.c_void_p], C.c_int64
     return lib
 
 
@@ -76,18 +76,34 @@ def test_refusals_without_a_device(st, lib):
         refused(bwd(bad), "pre is given")
 
 
-def test_workspaces(lib):
-    f, g = lib.sxh_linear_fwd_workspace, lib.sxh_linear_bwd_workspace
+def test_workspaces(st, lib):
+    at = 1 << 20  # never read
+
+    def f(rows, n_in, n_out, groups, t, x=at, stride=None):
+        a = st.LinearInputs(x, at, None, None, at if groups else None, rows, n_in, n_out, groups, n_in if stride is None else stride, 0, t, 0, 0)
+        return lib.sxh_linear_fwd_workspace(C.byref(a))
+
+    def g(rows, n_in, n_out, groups, t, x=at, stride=None):
+        a = st.LinearGradsIn(at, at, x, at, at if groups else None, rows, n_in, n_out, groups, n_out, n_out, n_in if stride is None else stride, t, 2, 0)
+        return lib.sxh_linear_bwd_workspace(C.byref(a))
+
     for rows in (0, 1, 13, 1000, 10 ** 6, 10 ** 9):
         for n_in, n_out in ((1, 1), (16, 64), (64, 64), (2048, 8192), (8192, 1), (1, 1 << 20)):
             for groups in (0, 1, 7, 300, 32768):
                 for t in (0, 1, 2):
-                    # a few tens of MiB for partial sums, and for the backward a copy of dy and of each group's weights' sums
-                    rows_bytes = 4 * rows * (n_out + 16)
-                    assert 0 <= f(rows, n_in, n_out, groups, t) <= 64 << 20
-                    assert 0 <= g(rows, n_in, n_out, groups, t) <= rows_bytes + (groups + 2048) * 4 * (n_in + 2) * (n_out + 2) + (256 << 20)
+                    # some tens of MiB for partial sums, and a copy of what does not lie as the products read it: of x and the
+                    # weights; for the backward also of dz
+                    rows_bytes, weights = 4 * rows * (n_in + 16), 4 * max(groups, 1) * n_out * (n_in + 16)
+                    assert 0 <= f(rows, n_in, n_out, groups, t) <= (64 << 20) + rows_bytes + weights
+                    assert 0 <= g(rows, n_in, n_out, groups, t) <= (300 << 20) + rows_bytes + 4 * rows * (n_out + 16) + 2 * weights + 2048 * 8 * n_in * min(n_out, 256)
+    # whole lines are read where they lie, others copied: rows of x, and for widths that are no multiple of 16 bytes the weights
+    assert f(100_000, 1024, 1024, 0, 1) == 0
+    assert f(100_000, 1024, 1024, 0, 1, x=at + 2) >= 100_000 * 2048 and f(100_000, 1024, 1024, 0, 1, stride=1025) >= 100_000 * 2048
+    assert f(100_000, 1023, 1024, 0, 1, stride=1024) >= 2 * 1024 * 1024 and f(100_000, 1024, 1024, 0, 1, stride=0) == 0
+    assert g(100_000, 1024, 1024, 0, 1, stride=1025) >= g(100_000, 1024, 1024, 0, 1) + 100_000 * 2048 - (300 << 20)
     for bad in ((-1, 4, 4, 0, 0), (4, 0, 4, 0, 0), (4, 4, 0, 0, 0), (4, 4, 4, -1, 0), (4, 4, 4, 32769, 0), (4, 4, 4, 0, 3), (1 << 60, 4, 4, 0, 0)):
         assert f(*bad) == g(*bad) == 0
+    assert lib.sxh_linear_fwd_workspace(None) == lib.sxh_linear_bwd_workspace(None) == 0
 
 
 def test_tensor_calls_refuse_host_memory(st):
