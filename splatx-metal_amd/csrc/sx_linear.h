@@ -492,14 +492,15 @@ __global__ void __launch_bounds__(BR / WR * (BC / WC) * 64) k_tile(TileArgs a) {
     char* const mine = (wave % 2 ? lds1 : lds) + wave / 2 * kUnitBytes<T>;
     Finish to = a.to;
     to.out = static_cast<T*>(to.out) + part.group * a.out_group;
-    // (a unit's residual is on its way while the one before it is finished)
+    // (a unit's residual is on its way while the one before it is finished, where the sums leave registers for that)
     constexpr int kAcross = J / kUnitTiles<T>;
+    constexpr bool kAhead = I * J <= 4;
     const auto unit_of = [&](int n) { return Unit<T>(to, r0 + wr + n / kAcross * 32, r1, c0 + wc + n % kAcross * kUnitTiles<T> * 32); };
     Unit<T> next = unit_of(0);
 #pragma unroll
     for (int n = 0; n < I * kAcross; n++) {
-        const Unit<T> now = next;
-        if (n + 1 < I * kAcross) next = unit_of(n + 1);
+        const Unit<T> now = kAhead || n == 0 ? next : unit_of(n);
+        if (kAhead && n + 1 < I * kAcross) next = unit_of(n + 1);
         if (now.rows <= 0 || now.c >= a.to.cols) continue;
         Sums unit[kUnitTiles<T>];
 #pragma unroll
@@ -1078,6 +1079,7 @@ Plan plan_rows(int64_t rows, int64_t cols, int64_t depth, int groups, bool ragge
     Plan best{};
     double least = INFINITY;
     for (const TileKind& k : kTileKinds) {
+        if (elem == 4 && k.rows == 256) continue;  // (floats' products are 16 times as long as their reads: 128 are enough)
         // (a group's last tile is half full)
         const double down = ragged ? static_cast<double>(rows) / k.rows + 0.5 * static_cast<double>(std::min<int64_t>(groups, rows)) : static_cast<double>(up(rows, k.rows));
         const double tiles = down * static_cast<double>(up(cols, k.cols));
@@ -1104,6 +1106,7 @@ Over plan_over(int64_t rows, int64_t out, int64_t in, int groups, bool ragged, i
     Over best{};
     double least = INFINITY;
     for (const TileKind& k : kTileKinds) {
+        if (elem == 4 && k.rows == 256) continue;
         const double tiles = static_cast<double>(up(out, k.rows) * up(in, k.cols));
         // one part each: the largest group is taken to have three times an even share
         const double even = tiles_take(k, tiles * groups, all / groups, elem);
@@ -1203,8 +1206,12 @@ void launch_tiles(const TileArgs& a, int side, int64_t slabs, hipStream_t s) {
     const int64_t down = RowAcross ? up(a.rows, side) : a.slots, tiles = up(down * up(a.to.cols, side == 256 ? 256 : 128), 8) * 8;
     check_grid(tiles * slabs, side == 256 ? 512 : 256);
     const dim3 grid(static_cast<uint32_t>(tiles), static_cast<uint32_t>(slabs));
-    if (side == 256) k_tile<T, 256, 256, 128, 64, RowAcross, ColAcross><<<grid, 512, 0, s>>>(a);
-    else if (side == 128) k_tile<T, 128, 128, 64, 64, RowAcross, ColAcross><<<grid, 256, 0, s>>>(a);
+    if constexpr (sizeof(T) == 2)
+        if (side == 256) {
+            k_tile<T, 256, 256, 128, 64, RowAcross, ColAcross><<<grid, 512, 0, s>>>(a);
+            return;
+        }
+    if (side == 128) k_tile<T, 128, 128, 64, 64, RowAcross, ColAcross><<<grid, 256, 0, s>>>(a);
     else k_tile<T, 64, 128, 32, 64, RowAcross, ColAcross><<<grid, 256, 0, s>>>(a);
 }
 
