@@ -22,6 +22,14 @@ __device__ inline void lds_barrier() {
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
+// Until of the wave's loads and stores of memory only the last N (63: any) are on their way, and none of LDS.
+template <int N>
+__device__ inline void wait_for() {
+    static_assert(N < 64);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 7 << 4);
+    asm volatile("" ::: "memory");
+}
 // What has been loaded is there from here on. Loads and stores of memory are counted together, so that a wait for loads that
 // comes after stores waits for these as well: the wait comes before them.
 template <class T, int N>
@@ -527,13 +535,29 @@ __global__ void __launch_bounds__(BR / WR * (BC / WC) * 64) k_tile(TileArgs a) {
     }
 }
 
-// The splits' slabs, added in order.
+// The splits' slabs, added in an order of their own: `turns` threads (a power of two) share four elements.
 template <class T>
-__global__ void __launch_bounds__(256) k_split_join(TileArgs a) {
-    const int64_t quads = (a.to.cols + 3) / 4;
-    for (int64_t i = blockIdx.x * int64_t{256} + threadIdx.x; i < a.rows * quads; i += gridDim.x * int64_t{256}) {
-        const int64_t r = i / quads, c = i % quads * 4;
+__global__ void __launch_bounds__(256) k_split_join(TileArgs a, int turns) {
+    __shared__ Floats<4> part[256];
+    const int each = 256 / turns, lane = threadIdx.x % each, turn = threadIdx.x / each;
+    const int64_t quads = (a.to.cols + 3) / 4, all = a.rows * quads;
+    for (int64_t first = int64_t{blockIdx.x} * each; first < all; first += int64_t{gridDim.x} * each) {
+        const int64_t i = min(first + lane, all - 1), r = i / quads, c = i % quads * 4;
         const int n = static_cast<int>(min(a.to.cols - c, int64_t{4}));
+        Floats<4> sum(0.0f);
+#pragma unroll 4
+        for (int s = turn; s < a.splits; s += turns) sum += load_some<float, 4>(a.partial + (s * a.rows + r) * a.to.cols + c, n);
+        if (turns > 1) {
+            __syncthreads();
+            part[threadIdx.x] = sum;
+            __syncthreads();
+            for (int w = turns / 2; w; w /= 2) {
+                if (turn < w) part[threadIdx.x] += part[threadIdx.x + w * each];
+                __syncthreads();
+            }
+            sum = part[lane];
+        }
+        if (turn || first + lane >= all) continue;
         int group = 0;
         if (a.groups.ends) {
             int hi = a.groups.groups;  // the first group that ends behind the row
@@ -547,8 +571,6 @@ __global__ void __launch_bounds__(256) k_split_join(TileArgs a) {
                 continue;
             }
         }
-        Floats<4> sum(0.0f);
-        for (int s = 0; s < a.splits; s++) sum += load_some<float, 4>(a.partial + (s * a.rows + r) * a.to.cols + c, n);
         if (a.bias) sum += load_some<T, 4>(static_cast<const T*>(a.bias) + group * a.bias_group + c, n);
         finish4<T>(a.to, r, c, sum);
     }
@@ -919,9 +941,11 @@ __global__ void __launch_bounds__(Waves * 64) k_narrow_bwd(NarrowBwdArgs a) {
 
 // ---- few rows ---------------------------------------------------------------------------------------------
 //
-// A layer of few rows is bound by its weight's bytes: each is read once, by a workgroup of 32 outputs whose waves share the sums'
-// length, 128 bytes of each weight's row at a time in turn, several on their way; their sums are added in LDS. (9 rows of
-// 2048 to 8192 in half precision: 10 us by tiles with the length in parts, and 5 us to join them.)
+// A layer of few rows is bound by its weight's bytes, each read once. Forward: a workgroup has 32 outputs, its waves share the
+// sums' length, 128 bytes of each weight's row at a time in turn, and add their sums in LDS at the end. What they read comes
+// through LDS of the wave's own, where lines begin on 16 bytes: a load of 16 bytes each from 32 rows takes four times as long as
+// one of whole lines, and half of them are x's, again and again. (9 rows of 2048 to 8192 in half precision: 15 us by
+// tiles, 10 by such loads.)
 struct FewArgs {
     const void *x, *weight, *bias;
     int64_t x_stride;
@@ -929,12 +953,13 @@ struct FewArgs {
     int64_t in, out;
     Groups groups;
 };
-constexpr int kFewWaves = 8;
-constexpr int kFewShift = 5;  // a part: 32 rows
-template <class T>
+constexpr int kFewWaves = 8, kFewShift = 5;  // a part: 32 rows
+template <class T, bool Lines>
 __global__ void __launch_bounds__(kFewWaves * 64) k_few_fwd(FewArgs a) {
     constexpr int V = kPer<T>, kLine = 128 / static_cast<int>(sizeof(T)), kAtOnce = 4, kPitch = 36;
-    __shared__ float sums[kFewWaves][32 * kPitch];
+    // (two arrays, so that a load into one is seen to be no store into the other)
+    __shared__ __attribute__((aligned(128))) char lds[kFewWaves * 8192], lds1[Lines ? kFewWaves * 8192 : 16];
+    static_assert(sizeof(float) * 32 * kPitch <= 8192);
     const Part part = part_of(a.groups, blockIdx.y, kFewShift);
     if (part.begin >= part.end) return;
     const int64_t c0 = int64_t{blockIdx.x} * 32;
@@ -945,10 +970,60 @@ __global__ void __launch_bounds__(kFewWaves * 64) k_few_fwd(FewArgs a) {
         if (threadIdx.x < 256 && r < part.end) clear4<T>(a.to, r, c);
         return;
     }
-    const T* const w = static_cast<const T*>(a.weight) + (part.group * a.out + min(c0 + lane % 32, a.out - 1)) * a.in;
+    const T* const weight = static_cast<const T*>(a.weight) + part.group * a.out * a.in;
+    const T* const w = weight + min(c0 + lane % 32, a.out - 1) * a.in;
     const T* const x = static_cast<const T*>(a.x) + min(part.begin + lane % 32, part.end - 1) * a.x_stride;
     Sums s(0.0f);
-    for (int64_t k = wave * kLine; k < a.in; k += kFewWaves * kAtOnce * kLine) {
+    int64_t begin = 0;
+    if constexpr (Lines) {
+        // The wave's lines: `wave` and every eighth after it. A load of the wave's fills 1 KiB: eight rows.
+        using Global = __attribute__((address_space(1))) const void*;
+        using Lds = __attribute__((address_space(3))) void*;
+        const int64_t lines = a.in / kLine, mine = (lines - wave + kFewWaves - 1) / kFewWaves;
+        begin = lines * kLine;
+        const T *from_w[4], *from_x[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int row = i * 8 + lane / 8, chunk = (plain_at(row, lane % 8) - row * 128) / 16 * V;
+            from_w[i] = weight + min(c0 + row, a.out - 1) * a.in + wave * kLine + chunk;
+            from_x[i] = static_cast<const T*>(a.x) + min(part.begin + row, part.end - 1) * a.x_stride + wave * kLine + chunk;
+        }
+        int64_t loaded = 0;
+        const auto load = [&](char* to) {  // (after the last line that again, so that as many loads are always on their way)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                __builtin_amdgcn_global_load_lds((Global)from_w[i], (Lds)(to + wave * 8192 + i * 1024), 16, 0, 0);
+                __builtin_amdgcn_global_load_lds((Global)from_x[i], (Lds)(to + wave * 8192 + 4096 + i * 1024), 16, 0, 0);
+            }
+            const int64_t next = ++loaded < mine ? kFewWaves * kLine : 0;
+#pragma unroll
+            for (int i = 0; i < 4; i++) from_w[i] += next, from_x[i] += next;
+        };
+        const auto step = [&](const char* now, char* next) {
+            wait_for<63>();  // (what was read of that place is there)
+            load(next);
+            wait_for<8>();
+            Frag<T> fw[4], fx[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                fw[i] = *reinterpret_cast<const Frag<T>*>(now + wave * 8192 + plain_at(lane % 32, 2 * i + half));
+                fx[i] = *reinterpret_cast<const Frag<T>*>(now + wave * 8192 + 4096 + plain_at(lane % 32, 2 * i + half));
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) mma(s, fw[i], fx[i]);
+        };
+        if (mine > 0) {
+            load(lds);
+            for (int64_t t = 0;;) {
+                step(lds, lds1);
+                if (++t == mine) break;
+                step(lds1, lds);
+                if (++t == mine) break;
+            }
+            wait_for<0>();
+        }
+    }
+    for (int64_t k = begin + wave * kLine; k < a.in; k += kFewWaves * kAtOnce * kLine) {
         Frag<T> fw[kAtOnce][4], fx[kAtOnce][4];
         const auto load_all = [&](auto load) {
 #pragma unroll
@@ -968,16 +1043,146 @@ __global__ void __launch_bounds__(kFewWaves * 64) k_few_fwd(FewArgs a) {
 #pragma unroll
             for (int i = 0; i < 4; i++) mma(s, fw[t][i], fx[t][i]);
     }
+    float* const sums = reinterpret_cast<float*>(lds + wave * 8192);
 #pragma unroll
     for (int q = 0; q < 4; q++)
-        *reinterpret_cast<Floats<4>*>(&sums[wave][lane % 32 * kPitch + half * 4 + q * 8]) = Floats<4>{s[4 * q], s[4 * q + 1], s[4 * q + 2], s[4 * q + 3]};
+        *reinterpret_cast<Floats<4>*>(sums + lane % 32 * kPitch + half * 4 + q * 8) = Floats<4>{s[4 * q], s[4 * q + 1], s[4 * q + 2], s[4 * q + 3]};
     __syncthreads();
     if (threadIdx.x >= 256 || r >= part.end || c >= a.out) return;
     Floats<4> v(0.0f);
 #pragma unroll
-    for (int k = 0; k < kFewWaves; k++) v += *reinterpret_cast<const Floats<4>*>(&sums[k][threadIdx.x / 8 * kPitch + threadIdx.x % 8 * 4]);
+    for (int k = 0; k < kFewWaves; k++) v += *reinterpret_cast<const Floats<4>*>(lds + k * 8192 + (threadIdx.x / 8 * kPitch + threadIdx.x % 8 * 4) * 4);
     if (a.bias) v += load_some<T, 4>(static_cast<const T*>(a.bias) + part.group * a.out + c, static_cast<int>(min(a.out - c, int64_t{4})));
     finish4<T>(a.to, r, c, v);
+}
+
+// The backward of few rows, in floats: dz of the rows lies in LDS, a thread has the columns of 16 bytes.
+struct FewBwdArgs {
+    const void *dy, *pre, *x, *weight;
+    int64_t dy_stride, pre_stride, x_stride;
+    void *dweight, *dbias;
+    float* partial;  // [slices][rows][in] of dx
+    int64_t in, out, slice;
+    Groups groups;
+    int act;
+};
+constexpr int kFewRows = 32, kFewBlock = 128;
+// dz of rows [r, r + rows) and outputs [n, n + outputs) before `end` as [outputs][pitch] floats, zeros past them
+template <class T>
+__device__ inline void few_dz(const FewBwdArgs& a, float* dz, int64_t r, int rows, int pitch, int64_t n, int outputs, int64_t end) {
+    for (int i = threadIdx.x; i < outputs * pitch; i += kFewBlock) {
+        const int m = i / outputs, o = i % outputs;  // (threads side by side: outputs side by side)
+        Floats<1> d(0.0f);
+        if (m < rows && n + o < end) {
+            d[0] = static_cast<float>(static_cast<const T*>(a.dy)[(r + m) * a.dy_stride + n + o]);
+            if (a.act) through<T, 1>(d, Floats<1>(static_cast<float>(static_cast<const T*>(a.pre)[(r + m) * a.pre_stride + n + o])), a.act);
+        }
+        dz[o * pitch + m] = d[0];
+    }
+}
+// The thread's chunks of N rows from `first` on, of those before `end`, on their way together.
+template <class T, int N>
+__device__ inline void few_chunks(Frag<T> (&v)[N], const T* base, int64_t stride, int64_t first, int64_t end, int64_t c, int64_t n) {
+    constexpr int V = kPer<T>;
+    if (n < V) {
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] = load_within(base + min(first + i, end - 1) * stride, c, n);
+        return;
+    }
+    const int64_t at = min(c, n - V);
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = load_raw<V>(base + min(first + i, end - 1) * stride + at);
+    if (n % V)
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] = moved_down<T>(v[i], static_cast<int>(c - at) * static_cast<int>(sizeof(T)) & 15);
+}
+
+// dx = dz W of a slice of the outputs, sixteen rows at a time: the weight's rows pass by once for each sixteen.
+template <class T>
+__global__ void __launch_bounds__(kFewBlock) k_few_dx(FewBwdArgs a) {
+    constexpr int V = kPer<T>, kAtOnce = 16, kOutputs = 32, kBatch = 16;
+    __shared__ __attribute__((aligned(16))) float dz[kOutputs * kAtOnce];
+    const Part part = part_of(a.groups, blockIdx.z, kFewShift);
+    if (part.group >= a.groups.groups || part.begin >= part.end) return;
+    const int64_t c = (int64_t{blockIdx.x} * kFewBlock + threadIdx.x) * V;
+    const int64_t n0 = blockIdx.y * a.slice, n1 = min(a.out, n0 + a.slice);
+    const T* const w = static_cast<const T*>(a.weight) + part.group * a.in * a.out;
+    for (int64_t r = part.begin; r < part.end; r += kAtOnce) {
+        const int rows = static_cast<int>(min(part.end - r, int64_t{kAtOnce}));
+        Floats<V> sum[kAtOnce];
+#pragma unroll
+        for (int m = 0; m < kAtOnce; m++) sum[m] = Floats<V>(0.0f);
+        for (int64_t n = n0; n < n1; n += kOutputs) {
+            __syncthreads();
+            few_dz<T>(a, dz, r, rows, kAtOnce, n, kOutputs, n1);
+            __syncthreads();
+            const int here = static_cast<int>(min(n1 - n, int64_t{kOutputs}));
+            if (c < a.in)
+                for (int o = 0; o < here; o += kBatch) {
+                    Frag<T> v[kBatch];
+                    few_chunks<T, kBatch>(v, w, a.in, n + o, n1, c, a.in);
+#pragma unroll
+                    for (int b = 0; b < kBatch; b++) {  // (dz is zero past the slice's end)
+                        const Floats<V> f = floats<T, V>(v[b]);
+#pragma unroll
+                        for (int q = 0; q < kAtOnce; q += 4) {
+                            if (q >= rows) break;
+                            const Floats<4> d = *reinterpret_cast<const Floats<4>*>(dz + (o + b) * kAtOnce + q);
+#pragma unroll
+                            for (int m = 0; m < 4; m++)
+#pragma unroll
+                                for (int e = 0; e < V; e++) sum[q + m][e] = __builtin_fmaf(d[m], f[e], sum[q + m][e]);
+                        }
+                    }
+                }
+        }
+        if (c >= a.in) continue;
+#pragma unroll
+        for (int m = 0; m < kAtOnce; m++)
+            if (m < rows)
+                store_some<float, V>(a.partial + (blockIdx.y * a.groups.rows + r + m) * a.in + c, sum[m], static_cast<int>(min(a.in - c, int64_t{V})));
+    }
+}
+
+// dweight = dz^T x and dbias of eight outputs.
+template <class T>
+__global__ void __launch_bounds__(kFewBlock) k_few_dw(FewBwdArgs a) {
+    constexpr int V = kPer<T>, kOutputs = 8, kBatch = 8;
+    __shared__ __attribute__((aligned(16))) float dz[kOutputs * kFewRows];
+    const int group = blockIdx.z;
+    const int64_t begin = a.groups.begin(group);
+    const int rows = static_cast<int>(max(int64_t{0}, min(a.groups.end(group) - begin, int64_t{kFewRows})));
+    const int64_t n = int64_t{blockIdx.y} * kOutputs, c = (int64_t{blockIdx.x} * kFewBlock + threadIdx.x) * V;
+    few_dz<T>(a, dz, begin, rows, kFewRows, n, kOutputs, a.out);
+    __syncthreads();
+    if (a.dbias && blockIdx.x == 0 && threadIdx.x < kOutputs && n + threadIdx.x < a.out) {
+        float sum = 0.0f;
+        for (int m = 0; m < rows; m++) sum += dz[threadIdx.x * kFewRows + m];
+        static_cast<T*>(a.dbias)[group * a.out + n + threadIdx.x] = static_cast<T>(sum);
+    }
+    if (!a.dweight || c >= a.in) return;
+    Floats<V> sum[kOutputs];
+#pragma unroll
+    for (int o = 0; o < kOutputs; o++) sum[o] = Floats<V>(0.0f);
+    for (int m = 0; m < rows; m += kBatch) {
+        Frag<T> v[kBatch];
+        few_chunks<T, kBatch>(v, static_cast<const T*>(a.x), a.x_stride, begin + m, begin + rows, c, a.in);
+#pragma unroll
+        for (int b = 0; b < kBatch; b++) {
+            if (m + b >= rows) break;
+            const Floats<V> f = floats<T, V>(v[b]);
+#pragma unroll
+            for (int o = 0; o < kOutputs; o++) {
+                const float d = dz[o * kFewRows + m + b];
+#pragma unroll
+                for (int e = 0; e < V; e++) sum[o][e] = __builtin_fmaf(d, f[e], sum[o][e]);
+            }
+        }
+    }
+#pragma unroll
+    for (int o = 0; o < kOutputs; o++)
+        if (n + o < a.out)
+            store_some<T, V>(static_cast<T*>(a.dweight) + (group * a.out + n + o) * a.in + c, sum[o], static_cast<int>(min(a.in - c, int64_t{V})));
 }
 
 // ---- dz = dy act'(pre), and its columns' sums ------------------------------------------------------------
@@ -1307,6 +1512,14 @@ void launch_narrow(const NarrowArgs& a, const Narrow& p, hipStream_t s) {
     }
 }
 
+template <class T>
+void join_splits(const TileArgs& a, hipStream_t s) {
+    int turns = 1;
+    while (turns < 32 && turns * 4 <= a.splits) turns *= 2;
+    const int64_t blocks = std::min<int64_t>(up(a.rows * up(a.to.cols, 4), 256 / turns), 4096);
+    k_split_join<T><<<static_cast<uint32_t>(blocks), 256, 0, s>>>(a, turns);
+}
+
 // out = row col^T over the groups' rows (see TileArgs), with what follows.
 template <class T, bool ColAcross>
 void over_depth(TileArgs a, bool ragged, Run& run) {
@@ -1318,10 +1531,7 @@ void over_depth(TileArgs a, bool ragged, Run& run) {
     a.partial = p.splits > 1 ? reinterpret_cast<float*>(run.work.take(p.bytes)) : nullptr;
     if (!run.real) return;
     launch_tiles<T, false, ColAcross>(a, p.side, p.splits, run.stream);
-    if (a.partial) {
-        const int64_t blocks = std::min<int64_t>(up(a.rows * up(a.to.cols, 4), 256), 4096);
-        k_split_join<T><<<static_cast<uint32_t>(blocks), 256, 0, run.stream>>>(a);
-    }
+    if (a.partial) join_splits<T>(a, run.stream);
 }
 
 template <class T>
@@ -1337,8 +1547,11 @@ void forward(const LinearFwdArgs& f, Run& run) {
         const int64_t slots = slots_of(f.rows, f.groups, kFewShift, ragged), blocks = up(f.out, 32);
         if (!run.real) return;
         check_grid(blocks * slots, kFewWaves * 64);
-        k_few_fwd<T><<<dim3(static_cast<uint32_t>(blocks), static_cast<uint32_t>(slots)), kFewWaves * 64, 0, run.stream>>>(
-            {f.x, f.weight, f.bias, f.x_stride, to, f.in, f.out, groups});
+        const dim3 grid(static_cast<uint32_t>(blocks), static_cast<uint32_t>(slots));
+        const FewArgs a{f.x, f.weight, f.bias, f.x_stride, to, f.in, f.out, groups};
+        const auto lines = [](const void* p, int64_t stride) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * sizeof(T) % 16 == 0; };
+        if (lines(f.x, f.x_stride) && lines(f.weight, f.in)) k_few_fwd<T, true><<<grid, kFewWaves * 64, 0, run.stream>>>(a);
+        else k_few_fwd<T, false><<<grid, kFewWaves * 64, 0, run.stream>>>(a);
         return;
     }
     const Operand x = operand<T>(f.x, f.rows, f.in, f.x_stride, false, run);
@@ -1369,11 +1582,42 @@ void backward_narrow(const LinearBwdArgs& f, const NarrowBwd& p, Run& run) {
 }
 
 template <class T>
+void backward_few(const LinearBwdArgs& f, Run& run) {
+    FewBwdArgs a{};
+    a.dy = f.dy; a.pre = f.pre; a.x = f.x; a.weight = f.weight; a.dy_stride = f.dy_stride; a.pre_stride = f.pre_stride; a.x_stride = f.x_stride;
+    a.dweight = f.dweight; a.dbias = f.dbias; a.in = f.in; a.out = f.out; a.groups = {f.ends, f.groups, f.rows}; a.act = f.act;
+    const int64_t across = up(f.in, kFewBlock * kPer<T>);
+    if (f.dx && f.rows) {
+        // (slices of 32 outputs, of 16 where those were too few workgroups)
+        a.slice = across * up(f.out, 32) * std::min<int64_t>(f.groups, f.rows) < 512 ? 16 : up(up(f.out, 256), 32) * 32;
+        const int64_t slices = up(f.out, a.slice), slots = slots_of(f.rows, f.groups, kFewShift, f.ends != nullptr);
+        a.partial = reinterpret_cast<float*>(run.work.take(slices * f.rows * f.in * 4));
+        TileArgs t{};  // (what joins the slices)
+        t.to.out = f.dx; t.to.out_stride = f.dx_stride; t.to.cols = f.in; t.to.clear = f.clear;
+        t.rows = f.rows; t.groups = a.groups; t.partial = a.partial; t.splits = static_cast<int>(slices);
+        if (run.real) {
+            check_grid(across * slices * slots, kFewBlock);
+            k_few_dx<T><<<dim3(static_cast<uint32_t>(across), static_cast<uint32_t>(slices), static_cast<uint32_t>(slots)), kFewBlock, 0, run.stream>>>(a);
+            join_splits<T>(t, run.stream);
+        }
+    }
+    if ((f.dweight || f.dbias) && run.real) {
+        const int64_t down = up(f.out, 8), wide = f.dweight ? across : 1;
+        check_grid(wide * down * f.groups, kFewBlock);
+        k_few_dw<T><<<dim3(static_cast<uint32_t>(wide), static_cast<uint32_t>(down), static_cast<uint32_t>(f.groups)), kFewBlock, 0, run.stream>>>(a);
+    }
+}
+
+template <class T>
 void backward(const LinearBwdArgs& f, Run& run) {
     const bool ragged = f.ends != nullptr;
     const Groups groups{f.ends, f.groups, f.rows};
     if (const NarrowBwd p = plan_narrow_bwd<T>(f.rows, f.in, f.out, f.groups); p.blocks) {
         backward_narrow<T>(f, p, run);
+        return;
+    }
+    if (f.rows <= kFewRows && f.out <= 8 * 65535) {
+        backward_few<T>(f, run);
         return;
     }
     // dz, where it is not dy itself, and its columns' sums

@@ -186,3 +186,11 @@ def test_nothing_of_the_padding_is_taken(tb, rows, n_out, sizes, n_in, dtype):
                                                    (64, 515, 100, None), (100, 515, 200, [64, 0, 1, 32])])
 def test_odd_widths_and_few_rows(tb, rows, n_in, n_out, sizes, dtype):
     compare(tb, rows, n_in, n_out, dtype, "silu", pad=8 if n_in % 2 else 0, sizes=sizes, seed=rows)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,n_in,n_out,sizes", [(1, 7544, 1384, None), (3, 1856, 992, None), (36, 5692, 796, None), (64, 300, 9000, None), (65, 300, 1000, None), (17, 5, 700, None),
+                                                   (6, 1984, 1536, [2, 1, 3]), (64, 600, 333, [0] * 20 + [40] + [1] * 20), (50, 1000, 77, [16, 17, 0, 1]), (2, 130, 20_000, [0, 1])])
+def test_few_rows_backward(tb, rows, n_in, n_out, sizes, dtype):
+    for act in ("none", "gelu"):
+        compare(tb, rows, n_in, n_out, dtype, act, pad=rows % 3, off=rows % 2, sizes=sizes, seed=rows)
