@@ -81,13 +81,14 @@ struct TileArgs {
     int64_t bias_group;
 };
 
-// Where the 16 bytes (row r, chunk c) of a plain operand's tile lie: 128 bytes a row, the chunks of eight rows in different
-// places, so that lanes that read one chunk of several rows read different banks.
+// Where the 16 bytes (row r, chunk c) of a plain operand's tile lie: 128 bytes a row, one chunk of sixteen rows in sixteen places of
+// 256 bytes, so that lanes that read one chunk of several rows read different banks.
 __device__ inline int plain_at(int r, int c) { return r * 128 + (c ^ (r >> 1 & 7)) * 16; }
-// Of an Across operand's tile: `row_bytes` a row of the sums' dimension; four rows' 32 bytes in different places.
+// Of an Across operand's tile: `row_bytes` (128 or a multiple of 256) a row of the sums' dimension; the 64 bytes that thirty-two
+// lanes read of each of four rows in different places of 256 bytes.
 template <class T>
 __device__ inline int across_at(int m, int byte, int row_bytes) {
-    return m * row_bytes + (sizeof(T) == 2 ? byte ^ ((m & 3) << 5) : byte);
+    return m * row_bytes + (sizeof(T) == 4 ? byte : row_bytes == 128 ? byte ^ ((m >> 1 & 1) << 6) : byte ^ ((m & 3) << 6));
 }
 
 // A thread's part of an operand's tile, R rows by 128 bytes of the sums' dimension, on its way from memory to LDS.
@@ -945,7 +946,7 @@ __global__ void __launch_bounds__(Waves * 64) k_narrow_bwd(NarrowBwdArgs a) {
 // sums' length, 128 bytes of each weight's row at a time in turn, and add their sums in LDS at the end. What they read comes
 // through LDS of the wave's own, where lines begin on 16 bytes: a load of 16 bytes each from 32 rows takes four times as long as
 // one of whole lines, and half of them are x's, again and again. (9 rows of 2048 to 8192 in half precision: 15 us by
-// tiles, 10 by such loads.)
+// tiles, 10.5 by such loads, 9 so: 3.7 TB/s.)
 struct FewArgs {
     const void *x, *weight, *bias;
     int64_t x_stride;
@@ -1388,7 +1389,7 @@ void launch_slope(const SlopeArgs& a, const Slope& p, hipStream_t s) {
 
 // A product's operand as k_tile reads it: lines that begin on 16 bytes, their places in a tile in 32 bits, and across them whole
 // fragments. What lies otherwise is copied first, which takes two passes over it where loads of its own kind took the product
-// three times as long (377 rows of 5996 to 1162 bfloat16, dx 65 us for 20).
+// three times as long (377 rows of 5996 to 1162 bfloat16, the gradients 98 us, with the copies 66).
 struct Operand {
     const void* p;
     int64_t stride, width;
@@ -1494,8 +1495,15 @@ void launch_narrow_bwd(const NarrowBwdArgs& a, const NarrowBwd& p, hipStream_t s
     }
 }
 
-// Whether a forward's groups have so few rows that the weights' bytes are what it takes.
-bool few_rows(int64_t rows, int groups) { return rows <= 32 || rows / groups <= 16; }
+// Whether a forward's groups have so few rows that the weights' bytes are what it takes (and its workgroups fit a launch).
+bool few_rows(int64_t rows, int64_t out, int groups) {
+    return (rows <= 32 || rows / groups <= 16) && up(out, 32) * (groups + 1 + (rows >> kFewShift)) < int64_t{1} << 22;
+}
+// Whether a backward's rows are.
+template <class T>
+bool few_rows_backward(int64_t rows, int64_t in, int64_t out, int groups) {
+    return rows <= kFewRows && out <= 8 * 65535 && up(in, kFewBlock * kPer<T>) * up(out, 8) * groups < int64_t{1} << 24;
+}
 
 template <class T>
 void launch_narrow(const NarrowArgs& a, const Narrow& p, hipStream_t s) {
@@ -1543,7 +1551,7 @@ void forward(const LinearFwdArgs& f, Run& run) {
         if (run.real) launch_narrow<T>({f.x, f.weight, f.bias, f.x_stride, to, f.in, f.out, p.chunk, groups}, p, run.stream);
         return;
     }
-    if (few_rows(f.rows, f.groups)) {
+    if (few_rows(f.rows, f.out, f.groups)) {
         const int64_t slots = slots_of(f.rows, f.groups, kFewShift, ragged), blocks = up(f.out, 32);
         if (!run.real) return;
         check_grid(blocks * slots, kFewWaves * 64);
@@ -1616,7 +1624,7 @@ void backward(const LinearBwdArgs& f, Run& run) {
         backward_narrow<T>(f, p, run);
         return;
     }
-    if (f.rows <= kFewRows && f.out <= 8 * 65535) {
+    if (few_rows_backward<T>(f.rows, f.in, f.out, f.groups)) {
         backward_few<T>(f, run);
         return;
     }
