@@ -9,6 +9,7 @@
 #include <cmath>
 #include <cstdint>
 #include <stdexcept>
+#include <type_traits>
 
 #include "sx_mma.h"
 
@@ -364,7 +365,10 @@ __device__ inline void store_unit(const Finish& a, int64_t r, int64_t stop, int6
 }
 
 // BR x BC outputs a workgroup, WR x WC a wave. OverRows: the sums go over a group's rows (dW), else the outputs' rows are the
-// groups' rows.
+// groups' rows. Bound by the matrix cores, and of long sums by the power they take (1.6 GHz, 64 % of the cycles a product on its
+// way): 16,383 rows, 8192 to 2048 half with a residual 505 us, 1.09 PFLOP/s (the library's bare product 457); of 2048 to 4096 dx
+// 294 us and dweight 284 (the library 272 and 330); 20,001 rows in 16 groups, 1024 to 1408, bfloat16 90 us. Floats of 4096 cubed
+// 998 us, 138 TFLOP/s (the library 910).
 template <class T, int BR, int BC, int WR, int WC, bool RowAcross, bool ColAcross>
 __global__ void __launch_bounds__(BR / WR * (BC / WC) * 64) k_tile(TileArgs a) {
     constexpr bool OverRows = RowAcross;
@@ -372,9 +376,11 @@ __global__ void __launch_bounds__(BR / WR * (BC / WC) * 64) k_tile(TileArgs a) {
     constexpr int kBuffer = (BR + BC) * 128, I = WR / 32, J = WC / 32;
     // (two arrays, so that a load into one is seen to be no store into the other)
     __shared__ __attribute__((aligned(128))) char lds[kBuffer], lds1[kBuffer];
-    // Which tile: workgroups go round the eight dies, and each die takes tiles side by side, eight rows of tiles at a time.
+    // Which tile: workgroups go round the eight dies, and each die takes tiles side by side, eight rows of tiles at a time. A slab
+    // begins with a die of its own: where it has fewer than eight tiles the others would have no work. (Floats, 919,424 rows of 32
+    // in 4 groups, gradients of 144 outputs: 1,900 us without, 1,527 so.)
     const int64_t across = (a.to.cols + BC - 1) / BC, down = OverRows ? (a.rows + BR - 1) / BR : a.slots, tiles = across * down;
-    const int64_t each = (tiles + 7) / 8, tile = blockIdx.x % 8 * each + blockIdx.x / 8;
+    const int64_t each = (tiles + 7) / 8, tile = (blockIdx.x + blockIdx.y) % 8 * each + blockIdx.x / 8;
     if (blockIdx.x / 8 >= each || tile >= tiles) return;
     const int64_t band = tile / (8 * across), height = min(down - band * 8, int64_t{8});
     const int64_t tr = band * 8 + (tile - band * 8 * across) % height, tc = (tile - band * 8 * across) / height;
@@ -416,8 +422,8 @@ __global__ void __launch_bounds__(BR / WR * (BC / WC) * 64) k_tile(TileArgs a) {
     const int64_t row_end = RowAcross ? a.row_width : r1, col_end = ColAcross ? a.col_width : a.to.cols;
     DirectStage<T, BR, RowAcross, kThreads> rows(rows_from, a.row_stride, r0, row_end, d0);
     DirectStage<T, BC, ColAcross, kThreads> cols(cols_from, a.col_stride, c0, col_end, d0);
+    const int64_t whole = (d1 - d0) / kDepth;
     {
-        const int64_t whole = (d1 - d0) / kDepth;
         // The fragments of a step are read while the products of the step before it run, also over the end of a tile: when the
         // last step's are there the tile's place in LDS is free, and the next tile's loads, as long on their way as a tile's
         // products take, have landed.
@@ -678,7 +684,8 @@ struct RowLoad {
     }
 };
 
-// K steps of 32 bytes a row. A wave takes 32 rows at a time; the next 32 are on their way meanwhile.
+// K steps of 32 bytes a row. A wave takes 32 rows at a time; the next 32 are on their way meanwhile. Bound by the rows' bytes:
+// 1 M rows, 48 to 64 bfloat16 39 us (5.7 TB/s); 64 to 64 with gelu and pre 78 (4.9); in 200 groups 86 (4.5).
 template <class T, int K>
 __global__ void __launch_bounds__(512) k_narrow_fwd(NarrowArgs a) {
     constexpr int V = kPer<T>;
@@ -815,13 +822,32 @@ struct BlockPart {
     }
 };
 
+// d as two terms of the type: the first is rounded from a little less than d, so that the second has d's sign and is not zero
+// where d is not (a product with an infinite x or weight then stays infinite in their sum; of half below 2^-14 the second term may
+// vanish). Of what is not finite both are that.
+template <class T>
+__device__ inline void two_terms(Floats<8> d, char* first, char* second) {
+    constexpr float kLess = std::is_same_v<T, _Float16> ? 1.0f - 1.0f / 512 : 1.0f - 1.0f / 64;
+    const Frag<T> high = raw<T, 8>(d * kLess);
+    const Floats<8> h = floats<T, 8>(high);
+    Floats<8> low = d - h;
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+        if (!(__builtin_fabsf(h[e]) < INFINITY)) low[e] = h[e];
+    *reinterpret_cast<Frag<T>*>(first) = high;
+    *reinterpret_cast<Frag<T>*>(second) = raw<T, 8>(low);
+}
+
 // All three gradients in one pass: a block of rows of dz and x lies in LDS, its products with the weight are dx's rows, and the
 // products of its columns with one another stay in registers over the rows of a group, tiles of 32 x 32 of dweight. The next
-// block is on its way meanwhile. Up to ZT tiles of 32 outputs and XT of 32 inputs.
-template <class T, int Waves, int ZT, int XT>
+// block is on its way meanwhile. Up to ZT tiles of 32 outputs (Fine, of dz in two terms: half as many) and XT of 32 inputs. Bound
+// by the rows' bytes, as far as two workgroups a unit, which is what LDS and registers hold, keep on their way: 1 M rows, 64 to 64
+// bfloat16 with gelu 119 us (4.3 TB/s), 300,000 of floats, 48 to 64, in groups 109 (floats' products take 26 of them).
+template <class T, int Waves, int ZT, int XT, bool Fine>
 __global__ void __launch_bounds__(Waves * 64) k_narrow_bwd(NarrowBwdArgs a) {
     constexpr int V = kPer<T>, kRows = kBlockRows<T>, kThreads = Waves * 64;
     constexpr int kSteps = ZT * static_cast<int>(sizeof(T)), kTiles = (ZT * XT + Waves - 1) / Waves, kZ = line_bytes<T>(ZT), kX = line_bytes<T>(XT);
+    constexpr int kLow = ZT * 32 / 2 * static_cast<int>(sizeof(T));  // from a first term to its second
     static_assert(XT % kUnitTiles<T> == 0);
     extern __shared__ __attribute__((aligned(128))) char lds[];
     const int lane = threadIdx.x % 64, wave = wave_of();
@@ -874,7 +900,12 @@ __global__ void __launch_bounds__(Waves * 64) k_narrow_bwd(NarrowBwdArgs a) {
                 Floats<V> d = floats<T, V>(dy.get(i, a.out, rows));
                 if (a.act) through<T, V>(d, floats<T, V>(pre.get(i, a.out, rows)), a.act);
                 db += d;
-                *reinterpret_cast<Frag<T>*>(dz + dy.line(i) * kZ + zc * 16) = raw<T, V>(d);
+                char* const at = dz + dy.line(i) * kZ + zc * 16;
+                if constexpr (Fine) {
+                    if (zc < dy.kLanes / 2) two_terms<T>(d, at, at + kLow);
+                } else {
+                    *reinterpret_cast<Frag<T>*>(at) = raw<T, V>(d);
+                }
             }
             if (a.x)
 #pragma unroll
@@ -888,8 +919,11 @@ __global__ void __launch_bounds__(Waves * 64) k_narrow_bwd(NarrowBwdArgs a) {
                     const int t = wave + i * Waves;
                     if (t / XT < nt && t % XT < kt)
 #pragma unroll
-                        for (int s = 0; s < 8; s++)
-                            mma(sums[i], across_fragment<T, XT>(xs, t % XT * 32, s), across_fragment<T, ZT>(dz, t / XT * 32, s));
+                        for (int s = 0; s < 8; s++) {
+                            const Frag<T> col = across_fragment<T, XT>(xs, t % XT * 32, s);
+                            mma(sums[i], col, across_fragment<T, ZT>(dz, t / XT * 32, s));
+                            if constexpr (Fine) mma(sums[i], col, across_fragment<T, ZT>(dz + kLow, t / XT * 32, s));
+                        }
                 }
             if (a.to.out)
                 for (int i = wave; i < kRows / 32 * (XT / kUnitTiles<T>); i += Waves) {
@@ -900,9 +934,15 @@ __global__ void __launch_bounds__(Waves * 64) k_narrow_bwd(NarrowBwdArgs a) {
 #pragma unroll
                     for (int u = 0; u < kUnitTiles<T>; u++) unit[u] = Sums(0.0f);
                     for (int s = 0; s < nt * static_cast<int>(sizeof(T)); s++) {
-                        const Frag<T> row = *reinterpret_cast<const Frag<T>*>(dz + (strip + lane % 32) * kZ + (2 * s + lane / 32) * 16);
+                        const char* const at = dz + (strip + lane % 32) * kZ + (2 * s + lane / 32) * 16;
+                        const Frag<T> row = *reinterpret_cast<const Frag<T>*>(at);
 #pragma unroll
                         for (int u = 0; u < kUnitTiles<T>; u++) mma(unit[u], weights[((t + u) * kSteps + s) * 64 + lane], row);
+                        if constexpr (Fine) {
+                            const Frag<T> low = *reinterpret_cast<const Frag<T>*>(at + kLow);
+#pragma unroll
+                            for (int u = 0; u < kUnitTiles<T>; u++) mma(unit[u], weights[((t + u) * kSteps + s) * 64 + lane], low);
+                        }
                     }
                     if (i == wave) {  // before the first stores
                         arrived<T>(dy.v);
@@ -1098,7 +1138,9 @@ __device__ inline void few_chunks(Frag<T> (&v)[N], const T* base, int64_t stride
         for (int i = 0; i < N; i++) v[i] = moved_down<T>(v[i], static_cast<int>(c - at) * static_cast<int>(sizeof(T)) & 15);
 }
 
-// dx = dz W of a slice of the outputs, sixteen rows at a time: the weight's rows pass by once for each sixteen.
+// dx = dz W of a slice of the outputs, sixteen rows at a time: the weight's rows pass by once for each sixteen. With floats' own
+// products: dz stays unrounded, and the weight's bytes are what it takes (the gradients of 6 rows in 3 groups, 1984 to 5536 float,
+// by tiles 134 us, so 58; of 3 rows, 1856 to 992, 29 and 15).
 template <class T>
 __global__ void __launch_bounds__(kFewBlock) k_few_dx(FewBwdArgs a) {
     constexpr int V = kPer<T>, kAtOnce = 16, kOutputs = 32, kBatch = 16;
@@ -1197,8 +1239,9 @@ struct SlopeArgs {
     int shift, act;
 };
 
-// A part of the rows and up to 256 vectors of columns a workgroup; `lanes` threads go along a row, four rows at a time (their
-// loads on their way together).
+// A part of the rows and up to 256 vectors of columns a workgroup; `lanes` threads go along a row, as many as it has vectors (by
+// the next power of two: 800,000 rows, 64 to 300 bfloat16, gradients 878 us for 826), four rows at a time (their loads on their
+// way together). Bound by its bytes: those 403 MB in 87 us, 4.6 TB/s.
 template <class T>
 __global__ void __launch_bounds__(256) k_slope(SlopeArgs a, int lanes) {
     constexpr int V = kPer<T>, kAtOnce = 4;
@@ -1208,7 +1251,7 @@ __global__ void __launch_bounds__(256) k_slope(SlopeArgs a, int lanes) {
     const int64_t c = (int64_t{blockIdx.y} * lanes + threadIdx.x % lanes) * V;
     const int step = 256 / lanes;
     Floats<V> sum(0.0f);
-    if (c < a.cols) {
+    if (c < a.cols && static_cast<int>(threadIdx.x) < step * lanes) {
         const int n = static_cast<int>(min(a.cols - c, int64_t{V}));
         // (a vector that reaches past the row's end is read so that it ends there, and moved to its place)
         const bool small = a.cols < V;
@@ -1246,7 +1289,7 @@ __global__ void __launch_bounds__(256) k_slope(SlopeArgs a, int lanes) {
     sums[threadIdx.x] = sum;
     __syncthreads();
     if (static_cast<int>(threadIdx.x) >= lanes || c >= a.cols) return;
-    for (int t = threadIdx.x + lanes; t < 256; t += lanes) sum += sums[t];
+    for (int t = threadIdx.x + lanes; t < step * lanes; t += lanes) sum += sums[t];
     store_some<float, V>(a.partial + int64_t{blockIdx.x} * a.cols + c, sum, static_cast<int>(min(a.cols - c, int64_t{V})));
 }
 
@@ -1342,7 +1385,7 @@ struct Slope {
 Slope plan_slope(int64_t rows, int64_t cols, int groups, bool ragged, int elem) {
     Slope p{};
     const int64_t vectors = up(cols, 16 / elem);
-    p.lanes = 1 << std::min(8, log2_up(vectors));
+    p.lanes = static_cast<int>(std::min<int64_t>(vectors, 256));
     p.columns = up(vectors, p.lanes);
     p.shift = std::max({log2_up(256 / p.lanes) + 2, log2_up(up(std::max<int64_t>(rows, 1), std::max<int64_t>(1, 1024 / p.columns)))});
     p.slots = slots_of(rows, groups, p.shift, ragged);
@@ -1462,15 +1505,27 @@ Narrow plan_narrow(int64_t rows, int64_t in, int64_t out, bool ragged) {
 // A backward whose blocks of rows a workgroup holds.
 struct NarrowBwd {
     int waves, zt, xt, lds;
+    bool fine;
     int64_t blocks, chunk, size, bytes;
 };
 template <class T>
-NarrowBwd plan_narrow_bwd(int64_t rows, int64_t in, int64_t out, int groups) {
+NarrowBwd plan_narrow_bwd(int64_t rows, int64_t in, int64_t out, int groups, int act) {
     NarrowBwd p{};
-    const int64_t nt = up(out, 32), kt = up(in, 32);
+    const int64_t kt = up(in, 32);
+    // dz is rounded to the type for its products, by which dx and dweight lose about what their own rounding takes. Where one of
+    // them has few elements chance may make that more, and the products are little next to the bytes: there dz is two terms
+    // (600,000 rows, 20 to 30, bfloat16: 76 us in one, 84 in two; 11 rows of 26 to 62: dx's error in one 1.5 times its own rounding's).
+    // (dy itself, and what relu leaves of it, has no more digits than the type.)
+    const bool wanted = sizeof(T) == 2 && act != kNone && act != kRelu && std::min(in * out, rows * in) < 1024;
+    p.fine = wanted && (out <= 32 || (out <= 64 && kt <= 4) || (out <= 128 && kt <= 2));
+    if (wanted && !p.fine && rows <= kFewRows) return p;  // (the few rows' kernels keep floats)
+    const int64_t nt = up(out, 32) * (p.fine ? 2 : 1);
     if (nt <= 2 && kt <= 2) p.waves = 4, p.zt = p.xt = 2;
-    else if (sizeof(T) == 4) return p;  // (blocks of 64 rows of more floats do not fit)
-    else if (nt <= 4 && kt <= 4) p.waves = 8, p.zt = p.xt = 4;
+    else if (sizeof(T) == 4) {  // (blocks of 64 rows of more floats do not fit; 919,424 rows, 32 to 80, by tiles 2,400 us, so 500)
+        if (nt <= 4 && kt <= 2) p.waves = 8, p.zt = 4, p.xt = 2;
+        else if (nt <= 2 && kt <= 4) p.waves = 8, p.zt = 2, p.xt = 4;
+        else return p;
+    } else if (nt <= 4 && kt <= 4) p.waves = 8, p.zt = p.xt = 4;
     else if (nt <= 2 && kt <= 8) p.waves = 8, p.zt = 2, p.xt = 8;
     else if (nt <= 8 && kt <= 2) p.waves = 8, p.zt = 8, p.xt = 2;
     else return p;
@@ -1487,11 +1542,19 @@ NarrowBwd plan_narrow_bwd(int64_t rows, int64_t in, int64_t out, int groups) {
 template <class T>
 void launch_narrow_bwd(const NarrowBwdArgs& a, const NarrowBwd& p, hipStream_t s) {
     const auto go = [&](auto kernel) { kernel<<<static_cast<uint32_t>(p.blocks), p.waves * 64, p.lds, s>>>(a); };
-    if (p.waves == 4) return go(k_narrow_bwd<T, 4, 2, 2>);
-    if constexpr (sizeof(T) == 2) {
-        if (p.zt == 4) go(k_narrow_bwd<T, 8, 4, 4>);
-        else if (p.zt == 2) go(k_narrow_bwd<T, 8, 2, 8>);
-        else go(k_narrow_bwd<T, 8, 8, 2>);
+    if constexpr (sizeof(T) == 4) {
+        if (p.waves == 4) go(k_narrow_bwd<T, 4, 2, 2, false>);
+        else if (p.zt == 4) go(k_narrow_bwd<T, 8, 4, 2, false>);
+        else go(k_narrow_bwd<T, 8, 2, 4, false>);
+    } else {
+        const auto by_terms = [&](auto fine) {
+            if (p.waves == 4) go(k_narrow_bwd<T, 4, 2, 2, fine.value>);
+            else if (p.zt == 4) go(k_narrow_bwd<T, 8, 4, 4, fine.value>);
+            else if (p.zt == 2) go(k_narrow_bwd<T, 8, 2, 8, fine.value>);
+            else go(k_narrow_bwd<T, 8, 8, 2, fine.value>);
+        };
+        if (p.fine) by_terms(std::true_type{});
+        else by_terms(std::false_type{});
     }
 }
 
@@ -1620,7 +1683,7 @@ template <class T>
 void backward(const LinearBwdArgs& f, Run& run) {
     const bool ragged = f.ends != nullptr;
     const Groups groups{f.ends, f.groups, f.rows};
-    if (const NarrowBwd p = plan_narrow_bwd<T>(f.rows, f.in, f.out, f.groups); p.blocks) {
+    if (const NarrowBwd p = plan_narrow_bwd<T>(f.rows, f.in, f.out, f.groups, f.act); p.blocks) {
         backward_narrow<T>(f, p, run);
         return;
     }

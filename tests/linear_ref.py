@@ -6,7 +6,7 @@ off by u. A sum of n terms in any order is within n u sum|terms|; twice that is 
 products without saying how. An activation's own error is ACT relative to the largest of it and its argument: for floats what
 the library's exponential, error function and quotient add up to (16 u), for 16-bit outputs that of Phi(-|z|), 2.5e-5 relative
 with at most half of |z| before it, and of the hardware's exponential and reciprocal, 2^-22 each and the argument's rounding.
-A slope has the same. dz is rounded to the type before the products: UNIT |dz|."""
+A slope has the same. dz may be rounded to the type before the products: UNIT |dz|."""
 import math
 
 import torch
@@ -14,6 +14,7 @@ import torch
 from learned_ref import TINY, U32, UNIT
 
 ACTS = ("none", "relu", "gelu", "silu", "sigmoid")
+DZ_UNIT = dict(UNIT)  # (of dz before the products, relative)
 ACT = {torch.float32: 16 * U32, torch.bfloat16: 4e-5, torch.float16: 4e-5}
 
 
@@ -86,7 +87,7 @@ def bwd(dy, x, w, pre=None, name="none", ends=None):
                 off = d.abs() * ACT[t] * (1 + z.abs().clamp_max(8))
             d = d * slope(z, name)
         size, m = d.abs() + off, d.shape[0]
-        rounded = off + UNIT[t] * size + TINY[t]
+        rounded = off + DZ_UNIT[t] * size + TINY[t]
         final = lambda v, e: torch.stack([v, e + UNIT[t] * (v.abs() + e) + TINY[t]])  # noqa: E731
         dx[:, r] = final(d @ wd, rounded @ wd.abs() + 2 * (n + 2) * U32 * (size @ wd.abs()))
         dw[(slice(None), *i)] = final(d.t().contiguous() @ xd, rounded.t().contiguous() @ xd.abs() + 2 * (m + 2) * U32 * (size.t().contiguous() @ xd.abs()))

@@ -194,3 +194,33 @@ def test_odd_widths_and_few_rows(tb, rows, n_in, n_out, sizes, dtype):
 def test_few_rows_backward(tb, rows, n_in, n_out, sizes, dtype):
     for act in ("none", "gelu"):
         compare(tb, rows, n_in, n_out, dtype, act, pad=rows % 3, off=rows % 2, sizes=sizes, seed=rows)
+
+
+@pytest.mark.parametrize("rows,n_in,n_out,sizes", [(70, 64, 65, None), (3000, 33, 128, None), (5001, 32, 80, [2000, 0, 3, 2998]), (65, 65, 64, None), (3000, 128, 33, None),
+                                                   (4099, 97, 20, [64, 65, 1, 3960]), (200, 64, 129, None), (9000, 32, 144, None), (9000, 16, 300, [4000, 5000])])
+def test_middle_layers_of_floats(tb, rows, n_in, n_out, sizes):
+    for act in ("none", "silu"):
+        compare(tb, rows, n_in, n_out, F32, act, pad=rows % 3, off=rows % 2, sizes=sizes, seed=rows)
+
+
+# Where dx or dweight has under 1024 elements dz's rounding is kept out of them: what is left of it is a second term's own, half a step of
+# at most 2^-5 (bfloat16; half 2^-8) of dz, far under an eighth of dz's.
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,n_in,n_out,sizes", [(11, 26, 62, None), (33, 7, 9, None), (33, 20, 128, None), (40, 3, 64, [20, 0, 20]), (2000, 1, 1, None), (5000, 5, 100, None),
+                                                   (3000, 31, 33, [1000, 0, 1, 1999]), (20, 40, 200, None), (3, 200, 60, None), (700, 250, 4, None)])
+def test_few_elements_keep_more_of_dz(tb, rows, n_in, n_out, sizes, dtype, monkeypatch):
+    monkeypatch.setitem(ref.DZ_UNIT, dtype, ref.UNIT[dtype] / 8)
+    for act in ("gelu", "silu", "sigmoid", "relu", "none"):
+        compare(tb, rows, n_in, n_out, dtype, act, pad=rows % 3, off=rows % 2, sizes=sizes, seed=rows)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_infinite_values_among_few_elements(tb, dtype):
+    dy, x, w, pre = (randn(40, 8, seed=i, dtype=dtype) for i in range(4))
+    w = w[:8].clone()
+    x[3, 2], x[9, 5], w[4, 6], dy[7, 1] = math.inf, math.nan, -math.inf, math.inf
+    got = tb.linear_bwd(dy, x, w, pre, "silu")
+    want, _ = ref.bwd(dy, x, w, pre, "silu", None)
+    for g, v in zip(got, want):
+        assert torch.equal(g.isnan(), v[0].isnan() if v.dim() > g.dim() else v.isnan())
+        assert torch.equal(g.isposinf(), v.isposinf()) and torch.equal(g.isneginf(), v.isneginf())
