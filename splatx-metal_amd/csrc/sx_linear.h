@@ -993,6 +993,8 @@ struct FewArgs {
     Finish to;
     int64_t in, out;
     Groups groups;
+    float* partial;  // [slices][rows][out] in place of y, or null
+    int64_t rows, slice;  // of the sums' length, whole lines of every wave
 };
 constexpr int kFewWaves = 8, kFewShift = 5;  // a part: 32 rows
 template <class T, bool Lines>
@@ -1008,26 +1010,29 @@ __global__ void __launch_bounds__(kFewWaves * 64) k_few_fwd(FewArgs a) {
     // (in the end a thread of the first half has four outputs)
     const int64_t r = part.begin + threadIdx.x / 8, c = c0 + threadIdx.x % 8 * 4;
     if (part.group >= a.groups.groups) {
+        if (a.partial) return;
         if (threadIdx.x < 256 && r < part.end) clear4<T>(a.to, r, c);
         return;
     }
-    const T* const weight = static_cast<const T*>(a.weight) + part.group * a.out * a.in;
+    const int64_t first = blockIdx.z * a.slice, length = min(a.slice, a.in - first);
+    const T* const weight = static_cast<const T*>(a.weight) + part.group * a.out * a.in + first;
+    const T* const xs = static_cast<const T*>(a.x) + first;
     const T* const w = weight + min(c0 + lane % 32, a.out - 1) * a.in;
-    const T* const x = static_cast<const T*>(a.x) + min(part.begin + lane % 32, part.end - 1) * a.x_stride;
+    const T* const x = xs + min(part.begin + lane % 32, part.end - 1) * a.x_stride;
     Sums s(0.0f);
     int64_t begin = 0;
     if constexpr (Lines) {
         // The wave's lines: `wave` and every eighth after it. A load of the wave's fills 1 KiB: eight rows.
         using Global = __attribute__((address_space(1))) const void*;
         using Lds = __attribute__((address_space(3))) void*;
-        const int64_t lines = a.in / kLine, mine = (lines - wave + kFewWaves - 1) / kFewWaves;
+        const int64_t lines = length / kLine, mine = (lines - wave + kFewWaves - 1) / kFewWaves;
         begin = lines * kLine;
         const T *from_w[4], *from_x[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int row = i * 8 + lane / 8, chunk = (plain_at(row, lane % 8) - row * 128) / 16 * V;
             from_w[i] = weight + min(c0 + row, a.out - 1) * a.in + wave * kLine + chunk;
-            from_x[i] = static_cast<const T*>(a.x) + min(part.begin + row, part.end - 1) * a.x_stride + wave * kLine + chunk;
+            from_x[i] = xs + min(part.begin + row, part.end - 1) * a.x_stride + wave * kLine + chunk;
         }
         int64_t loaded = 0;
         const auto load = [&](char* to) {  // (after the last line that again, so that as many loads are always on their way)
@@ -1064,7 +1069,7 @@ __global__ void __launch_bounds__(kFewWaves * 64) k_few_fwd(FewArgs a) {
             wait_for<0>();
         }
     }
-    for (int64_t k = begin + wave * kLine; k < a.in; k += kFewWaves * kAtOnce * kLine) {
+    for (int64_t k = begin + wave * kLine; k < length; k += kFewWaves * kAtOnce * kLine) {
         Frag<T> fw[kAtOnce][4], fx[kAtOnce][4];
         const auto load_all = [&](auto load) {
 #pragma unroll
@@ -1076,9 +1081,9 @@ __global__ void __launch_bounds__(kFewWaves * 64) k_few_fwd(FewArgs a) {
                     fx[t][i] = load(x, at);
                 }
         };
-        if (k + (kAtOnce - 1) * kFewWaves * kLine + kLine <= a.in) load_all([&](const T* p, int64_t at) { return load_raw<V>(p + at); });
-        else if (a.in >= V) load_all([&](const T* p, int64_t at) { return load_clamped(p, at, a.in); });
-        else load_all([&](const T* p, int64_t at) { return load_within(p, at, a.in); });
+        if (k + (kAtOnce - 1) * kFewWaves * kLine + kLine <= length) load_all([&](const T* p, int64_t at) { return load_raw<V>(p + at); });
+        else if (length >= V) load_all([&](const T* p, int64_t at) { return load_clamped(p, at, length); });
+        else load_all([&](const T* p, int64_t at) { return load_within(p, at, length); });
 #pragma unroll
         for (int t = 0; t < kAtOnce; t++)
 #pragma unroll
@@ -1093,6 +1098,10 @@ __global__ void __launch_bounds__(kFewWaves * 64) k_few_fwd(FewArgs a) {
     Floats<4> v(0.0f);
 #pragma unroll
     for (int k = 0; k < kFewWaves; k++) v += *reinterpret_cast<const Floats<4>*>(lds + k * 8192 + (threadIdx.x / 8 * kPitch + threadIdx.x % 8 * 4) * 4);
+    if (a.partial) {
+        store_some<float, 4>(a.partial + (blockIdx.z * a.rows + r) * a.out + c, v, static_cast<int>(min(a.out - c, int64_t{4})));
+        return;
+    }
     if (a.bias) v += load_some<T, 4>(static_cast<const T*>(a.bias) + part.group * a.out + c, static_cast<int>(min(a.out - c, int64_t{4})));
     finish4<T>(a.to, r, c, v);
 }
@@ -1616,13 +1625,24 @@ void forward(const LinearFwdArgs& f, Run& run) {
     }
     if (few_rows(f.rows, f.out, f.groups)) {
         const int64_t slots = slots_of(f.rows, f.groups, kFewShift, ragged), blocks = up(f.out, 32);
-        if (!run.real) return;
-        check_grid(blocks * slots, kFewWaves * 64);
-        const dim3 grid(static_cast<uint32_t>(blocks), static_cast<uint32_t>(slots));
-        const FewArgs a{f.x, f.weight, f.bias, f.x_stride, to, f.in, f.out, groups};
-        const auto lines = [](const void* p, int64_t stride) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * sizeof(T) % 16 == 0; };
-        if (lines(f.x, f.x_stride) && lines(f.weight, f.in)) k_few_fwd<T, true><<<grid, kFewWaves * 64, 0, run.stream>>>(a);
+        const auto whole_lines = [](const void* p, int64_t stride) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * sizeof(T) % 16 == 0; };
+        const bool whole = whole_lines(f.x, f.x_stride) && whole_lines(f.weight, f.in);
+        // Where that leaves units without work and a wave has eight lines and more (sixteen, of those that go through LDS), slices of the
+        // sums' length, of two lines a wave at least, are workgroups of their own. (24 rows of 4281 to 1967 half 41 us whole, 22 in
+        // slices; 8 rows of 4096 to 1024 bfloat16, eight lines through LDS, 7.9 and 9.5.)
+        constexpr int64_t line = kFewWaves * 128 / static_cast<int>(sizeof(T));
+        const int64_t lines = up(f.in, line), most = lines < (whole ? 16 : 8) ? 1 : std::min(lines / 2, 256 / (blocks * slots));
+        const int64_t slice = up(lines, std::max<int64_t>(most, 1)) * line, slices = up(f.in, slice);
+        TileArgs t{};  // (what joins the slices)
+        t.to = to; t.rows = f.rows; t.groups = groups; t.bias = f.bias; t.bias_group = f.out; t.splits = static_cast<int>(slices);
+        if (slices > 1) t.partial = reinterpret_cast<float*>(run.work.take(slices * f.rows * f.out * 4));
+        if (!run.real || !f.rows) return;
+        check_grid(blocks * slots * slices, kFewWaves * 64);
+        const dim3 grid(static_cast<uint32_t>(blocks), static_cast<uint32_t>(slots), static_cast<uint32_t>(slices));
+        const FewArgs a{f.x, f.weight, f.bias, f.x_stride, to, f.in, f.out, groups, t.partial, f.rows, slice};
+        if (whole) k_few_fwd<T, true><<<grid, kFewWaves * 64, 0, run.stream>>>(a);
         else k_few_fwd<T, false><<<grid, kFewWaves * 64, 0, run.stream>>>(a);
+        if (slices > 1) join_splits<T>(t, run.stream);
         return;
     }
     const Operand x = operand<T>(f.x, f.rows, f.in, f.x_stride, false, run);

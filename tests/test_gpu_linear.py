@@ -224,3 +224,11 @@ def test_infinite_values_among_few_elements(tb, dtype):
     for g, v in zip(got, want):
         assert torch.equal(g.isnan(), v[0].isnan() if v.dim() > g.dim() else v.isnan())
         assert torch.equal(g.isposinf(), v.isposinf()) and torch.equal(g.isneginf(), v.isneginf())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,n_in,n_out,sizes", [(24, 4281, 200, None), (31, 2274, 90, None), (2, 8000, 33, None), (1, 4097, 1, None), (3, 2049, 7, [1, 0, 1]), (32, 9001, 64, [30]),
+                                                   (16, 16_385, 20, [5, 6])])
+def test_few_rows_of_long_sums(tb, rows, n_in, n_out, sizes, dtype):
+    for pad in (0, 8):
+        compare(tb, rows, n_in, n_out, dtype, "silu", add=True, pad=pad, sizes=sizes, seed=rows)
