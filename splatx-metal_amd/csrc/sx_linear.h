@@ -1631,7 +1631,7 @@ void forward(const LinearFwdArgs& f, Run& run) {
         // sums' length, of two lines a wave at least, are workgroups of their own. (24 rows of 4281 to 1967 half 41 us whole, 22 in
         // slices; 8 rows of 4096 to 1024 bfloat16, eight lines through LDS, 7.9 and 9.5.)
         constexpr int64_t line = kFewWaves * 128 / static_cast<int>(sizeof(T));
-        const int64_t lines = up(f.in, line), most = lines < (whole ? 16 : 8) ? 1 : std::min(lines / 2, 256 / (blocks * slots));
+        const int64_t lines = up(f.in, line), most = lines < (whole ? 16 : 8) ? 1 : std::min(lines / 2, 256 / std::max<int64_t>(blocks * slots, 1));
         const int64_t slice = up(lines, std::max<int64_t>(most, 1)) * line, slices = up(f.in, slice);
         TileArgs t{};  // (what joins the slices)
         t.to = to; t.rows = f.rows; t.groups = groups; t.bias = f.bias; t.bias_group = f.out; t.splits = static_cast<int>(slices);
