@@ -14,7 +14,7 @@ import torch
 from learned_ref import TINY, U32, UNIT
 
 ACTS = ("none", "relu", "gelu", "silu", "sigmoid")
-DZ_UNIT = dict(UNIT)  # (of dz before the products, relative)
+DZ_UNIT = {}  # of dz before the products, where it is not UNIT
 ACT = {torch.float32: 16 * U32, torch.bfloat16: 4e-5, torch.float16: 4e-5}
 
 
@@ -87,7 +87,7 @@ def bwd(dy, x, w, pre=None, name="none", ends=None):
                 off = d.abs() * ACT[t] * (1 + z.abs().clamp_max(8))
             d = d * slope(z, name)
         size, m = d.abs() + off, d.shape[0]
-        rounded = off + DZ_UNIT[t] * size + TINY[t]
+        rounded = off + DZ_UNIT.get(t, UNIT[t]) * size + TINY[t]
         final = lambda v, e: torch.stack([v, e + UNIT[t] * (v.abs() + e) + TINY[t]])  # noqa: E731
         dx[:, r] = final(d @ wd, rounded @ wd.abs() + 2 * (n + 2) * U32 * (size @ wd.abs()))
         dw[(slice(None), *i)] = final(d.t().contiguous() @ xd, rounded.t().contiguous() @ xd.abs() + 2 * (m + 2) * U32 * (size.t().contiguous() @ xd.abs()))
