@@ -232,3 +232,10 @@ def test_infinite_values_among_few_elements(tb, dtype):
 def test_few_rows_of_long_sums(tb, rows, n_in, n_out, sizes, dtype):
     for pad in (0, 8):
         compare(tb, rows, n_in, n_out, dtype, "silu", add=True, pad=pad, sizes=sizes, seed=rows)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n_in,n_out", [(40, 200), (7, 9), (9001, 64), (64, 128)])
+@pytest.mark.parametrize("sizes", [None, [0, 0, 0]])
+def test_no_rows(tb, sizes, n_in, n_out, dtype):
+    compare(tb, 0, n_in, n_out, dtype, "gelu", sizes=sizes)
