@@ -6,11 +6,11 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
-#include <cmath>
 #include <cstdint>
 #include <stdexcept>
 #include <type_traits>
 
+#include "sx_linear_plan.h"
 #include "sx_mma.h"
 
 namespace sxk {
@@ -246,11 +246,11 @@ __device__ inline void clear4(const Finish& a, int64_t r, int64_t c) {
 // time through what follows the sums. (Stores of 16 bytes a row from the registers, the rows' lines in four parts: a layer of
 // 64 outputs took twice as long.)
 template <class T>
-constexpr int kUnitTiles = 4 / static_cast<int>(sizeof(T));  // tiles of 32 columns side by side
+constexpr int kUnitTiles = unit_tiles(sizeof(T));
 template <class T>
-constexpr int kUnitLine = kUnitTiles<T> * 128 + 16;  // (the lines of eight rows in different banks)
+constexpr int kUnitLine = unit_line(sizeof(T));
 template <class T>
-constexpr int kUnitBytes = 32 * kUnitLine<T>;
+constexpr int kUnitBytes = unit_bytes(sizeof(T));
 
 // What lanes of the wave have written to LDS is there for the others.
 __device__ inline void wave_sees() {
@@ -333,10 +333,6 @@ struct Unit {
 
 // The same of sums that are the outputs, through half the LDS.
 template <class T>
-constexpr int kBareLine = 128 + 16;
-template <class T>
-constexpr int kBareBytes = 32 * kBareLine<T>;
-template <class T>
 __device__ inline void store_unit(const Finish& a, int64_t r, int64_t stop, int64_t c, const Sums (&sums)[kUnitTiles<T>], char* lds) {
     constexpr int V = kPer<T>;
     const int lane = threadIdx.x % 64;
@@ -345,7 +341,7 @@ __device__ inline void store_unit(const Finish& a, int64_t r, int64_t stop, int6
     for (int u = 0; u < kUnitTiles<T>; u++)
 #pragma unroll
         for (int q = 0; q < 4; q++)
-            *reinterpret_cast<Vec<T, 4>*>(lds + lane % 32 * kBareLine<T> + (u * 32 + 8 * q + lane / 32 * 4) * static_cast<int>(sizeof(T))) =
+            *reinterpret_cast<Vec<T, 4>*>(lds + lane % 32 * kBareLine + (u * 32 + 8 * q + lane / 32 * 4) * static_cast<int>(sizeof(T))) =
                 raw<T, 4>(Floats<4>{sums[u][4 * q], sums[u][4 * q + 1], sums[u][4 * q + 2], sums[u][4 * q + 3]});
     wave_sees();
     const int column = lane % 8 * V, row = lane / 8;
@@ -354,7 +350,7 @@ __device__ inline void store_unit(const Finish& a, int64_t r, int64_t stop, int6
     T* p = static_cast<T*>(a.out) + (r * a.out_stride + c) + (row * a.out_stride + column);
 #pragma unroll
     for (int i = 0; i < 32; i += 8, p += 8 * a.out_stride) {
-        const Frag<T> v = *reinterpret_cast<const Frag<T>*>(lds + (row + i) * kBareLine<T> + lane % 8 * 16);
+        const Frag<T> v = *reinterpret_cast<const Frag<T>*>(lds + (row + i) * kBareLine + lane % 8 * 16);
         if (row + i >= rows) continue;
         if (n == V) store_raw<V>(p, v);
         else
@@ -761,17 +757,13 @@ struct NarrowBwdArgs {
     Groups groups;
     int act;
 };
-// Bytes between the lines of a block in LDS: `tiles` times 32 elements, and what puts four lines (floats: the lanes' lines)
-// into different banks.
 template <class T>
-constexpr int line_bytes(int tiles) { return tiles * 32 * static_cast<int>(sizeof(T)) + (sizeof(T) == 2 ? 32 : 16); }
-template <class T>
-constexpr int kBlockRows = 256 / static_cast<int>(sizeof(T));
+constexpr int kBlockRows = block_rows(sizeof(T));
 
 // The lane's fragment of a column of a block: the lines along it, step s of eight.
 template <class T, int Tiles>
 __device__ inline Frag<T> across_fragment(const char* block, int column, int s) {
-    constexpr int kLine = line_bytes<T>(Tiles);
+    constexpr int kLine = line_bytes(Tiles, sizeof(T));
     const int lane = threadIdx.x % 64, half = lane / 32;
     if constexpr (sizeof(T) == 4) {
         Frag<T> f;
@@ -846,14 +838,14 @@ __device__ inline void two_terms(Floats<8> d, char* first, char* second) {
 template <class T, int Waves, int ZT, int XT, bool Fine>
 __global__ void __launch_bounds__(Waves * 64) k_narrow_bwd(NarrowBwdArgs a) {
     constexpr int V = kPer<T>, kRows = kBlockRows<T>, kThreads = Waves * 64;
-    constexpr int kSteps = ZT * static_cast<int>(sizeof(T)), kTiles = (ZT * XT + Waves - 1) / Waves, kZ = line_bytes<T>(ZT), kX = line_bytes<T>(XT);
+    constexpr int kSteps = ZT * static_cast<int>(sizeof(T)), kTiles = (ZT * XT + Waves - 1) / Waves, kZ = line_bytes(ZT, sizeof(T)), kX = line_bytes(XT, sizeof(T));
     constexpr int kLow = ZT * 32 / 2 * static_cast<int>(sizeof(T));  // from a first term to its second
     static_assert(XT % kUnitTiles<T> == 0);
     extern __shared__ __attribute__((aligned(128))) char lds[];
     const int lane = threadIdx.x % 64, wave = wave_of();
     const int nt = static_cast<int>((a.out + 31) / 32), kt = static_cast<int>((a.in + 31) / 32);
-    char *const dz = lds, *const xs = dz + kRows * kZ, *const mine = xs + kRows * kX + wave * kBareBytes<T>;
-    Frag<T>* const weights = reinterpret_cast<Frag<T>*>(xs + kRows * kX + Waves * kBareBytes<T>);
+    char *const dz = lds, *const xs = dz + kRows * kZ, *const mine = xs + kRows * kX + wave * kBareBytes;
+    Frag<T>* const weights = reinterpret_cast<Frag<T>*>(xs + kRows * kX + Waves * kBareBytes);
     BlockPart<T, ZT, kThreads> dy, pre;
     BlockPart<T, XT, kThreads> x;
     const auto load = [&](int64_t first, int64_t stop) {
@@ -996,7 +988,6 @@ struct FewArgs {
     float* partial;  // [slices][rows][out] in place of y, or null
     int64_t rows, slice;  // of the sums' length, whole lines of every wave
 };
-constexpr int kFewWaves = 8, kFewShift = 5;  // a part: 32 rows
 template <class T, bool Lines>
 __global__ void __launch_bounds__(kFewWaves * 64) k_few_fwd(FewArgs a) {
     constexpr int V = kPer<T>, kLine = 128 / static_cast<int>(sizeof(T)), kAtOnce = 4, kPitch = 36;
@@ -1116,7 +1107,6 @@ struct FewBwdArgs {
     Groups groups;
     int act;
 };
-constexpr int kFewRows = 32, kFewBlock = 128;
 // dz of rows [r, r + rows) and outputs [n, n + outputs) before `end` as [outputs][pitch] floats, zeros past them
 template <class T>
 __device__ inline void few_dz(const FewBwdArgs& a, float* dz, int64_t r, int rows, int pitch, int64_t n, int outputs, int64_t end) {
@@ -1302,107 +1292,7 @@ __global__ void __launch_bounds__(256) k_slope(SlopeArgs a, int lanes) {
     store_some<float, V>(a.partial + int64_t{blockIdx.x} * a.cols + c, sum, static_cast<int>(min(a.cols - c, int64_t{V})));
 }
 
-// ---- plans ------------------------------------------------------------------------------------------------
-
-int log2_up(int64_t n) {
-    int k = 0;
-    while ((int64_t{1} << k) < n) k++;
-    return k;
-}
-int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to; }
-
-// The tiles to choose from: their rows and columns, how many run at once on 256 units, and what a step of 128 bytes of the
-// sums' length then takes, in ns of 16-bit elements (floats: as many bytes, 4.6 times), and what a tile takes besides. Measured on layers of 16,383 rows, 8192 to
-// 2048: 542, 623 and 712 us by tiles of 256, 128 and 64 rows; 20,001 rows in 16 groups, 1024 to 1408, whose tiles of 256 rows
-// take three rounds for two: 121, 104 and 106.
-struct TileKind {
-    int rows, cols, at_once;
-    double step, fixed;
-};
-constexpr TileKind kTileKinds[] = {{256, 256, 256, 1950, 6000}, {128, 128, 512, 1150, 3000}, {64, 128, 768, 1050, 2500}};
-constexpr double kJoinFixed = 4000, kJoinBytes = 4;  // ns; bytes a ns
-// `tiles` of `steps` each; a unit's only workgroup of a kind that shares it goes faster.
-double tiles_take(const TileKind& k, double tiles, double steps, int elem) {
-    const double step = k.step * (elem == 4 ? 4.6 : 1.0) * (tiles <= 256 && k.at_once > 256 ? 0.6 : 1.0);
-    return std::max(1.0, std::ceil(tiles / k.at_once)) * (k.fixed + steps * step);
-}
-
-// out[rows][cols] over `depth`, rows in groups: the tile's rows, and how many parts the depth is split into.
-struct Plan {
-    int side, splits;
-    int64_t split, bytes;
-};
-Plan plan_rows(int64_t rows, int64_t cols, int64_t depth, int groups, bool ragged, int elem) {
-    const int64_t step = 128 / elem, steps = up(depth, step);
-    Plan best{};
-    double least = INFINITY;
-    for (const TileKind& k : kTileKinds) {
-        if (elem == 4 && k.rows == 256) continue;  // (floats' products are 16 times as long as their reads: 128 are enough)
-        // (a group's last tile is half full)
-        const double down = ragged ? static_cast<double>(rows) / k.rows + 0.5 * static_cast<double>(std::min<int64_t>(groups, rows)) : static_cast<double>(up(rows, k.rows));
-        const double tiles = down * static_cast<double>(up(cols, k.cols));
-        for (int64_t splits = 1; splits <= 64 && (splits == 1 || steps / splits >= 2); splits *= 2) {
-            const int64_t each = up(steps, splits), parts = up(steps, each), bytes = parts > 1 ? parts * rows * cols * 4 : 0;
-            if (bytes > int64_t{64} << 20) break;
-            const double time = tiles_take(k, tiles * static_cast<double>(parts), static_cast<double>(each), elem) +
-                                (parts > 1 ? kJoinFixed + 2.0 * static_cast<double>(bytes) / kJoinBytes / 1000 : 0.0);
-            if (time < least) {
-                least = time;
-                best = {k.rows, static_cast<int>(parts), each * step, bytes};
-            }
-        }
-    }
-    return best;
-}
-// out[groups][out][in] over the groups' rows: the tile's rows, and the parts of the rows (shift 62: each group's are one).
-struct Over {
-    int side, shift;
-    int64_t slots, bytes;
-};
-Over plan_over(int64_t rows, int64_t out, int64_t in, int groups, bool ragged, int elem) {
-    const double step = 128.0 / elem, all = static_cast<double>(rows) / step;
-    Over best{};
-    double least = INFINITY;
-    for (const TileKind& k : kTileKinds) {
-        if (elem == 4 && k.rows == 256) continue;
-        const double tiles = static_cast<double>(up(out, k.rows) * up(in, k.cols));
-        // one part each: the largest group is taken to have three times an even share
-        const double even = tiles_take(k, tiles * groups, all / groups, elem);
-        double time = std::max(even, groups > 1 ? tiles_take(k, 1, std::min(all, 3 * all / groups), elem) : 0.0);
-        if (time < least) {
-            least = time;
-            best = {k.rows, 62, groups, 0};
-        }
-        for (int shift = 8; (int64_t{1} << shift) < rows; shift++) {
-            const int64_t slots = slots_of(rows, groups, shift, ragged), bytes = slots * out * in * 4;
-            if (bytes > int64_t{256} << 20 || slots > 65535) continue;
-            const double parts = ragged ? static_cast<double>(rows >> shift) + 0.5 * groups : static_cast<double>(slots);
-            time = tiles_take(k, tiles * parts, static_cast<double>(int64_t{1} << shift) / step, elem) + kJoinFixed +
-                   2.0 * parts * static_cast<double>(out * in) * 4 / kJoinBytes / 1000;
-            if (time < least) {
-                least = time;
-                best = {k.rows, shift, slots, bytes};
-            }
-        }
-    }
-    return best;
-}
-struct Slope {
-    int shift, lanes;
-    int64_t slots, columns, bytes, dz_stride, dz_bytes;
-};
-Slope plan_slope(int64_t rows, int64_t cols, int groups, bool ragged, int elem) {
-    Slope p{};
-    const int64_t vectors = up(cols, 16 / elem);
-    p.lanes = static_cast<int>(std::min<int64_t>(vectors, 256));
-    p.columns = up(vectors, p.lanes);
-    p.shift = std::max({log2_up(256 / p.lanes) + 2, log2_up(up(std::max<int64_t>(rows, 1), std::max<int64_t>(1, 1024 / p.columns)))});
-    p.slots = slots_of(rows, groups, p.shift, ragged);
-    p.bytes = p.slots * cols * 4;
-    p.dz_stride = vectors * (16 / elem);
-    p.dz_bytes = rows * p.dz_stride * elem;
-    return p;
-}
+// ---- launches ---------------------------------------------------------------------------------------------
 
 // A call's workspace, handed out from its beginning; without memory only how much there has to be.
 class Work {
@@ -1482,72 +1372,6 @@ void join_weights(JoinArgs a, int64_t slabs, hipStream_t s) {
     k_weights_join<T><<<dim3(static_cast<uint32_t>(blocks), static_cast<uint32_t>(a.groups.groups)), 256, 0, s>>>(a);
 }
 
-// The steps of 32 bytes of a row that k_narrow_fwd is built for, or 0.
-int narrow_steps(int64_t in, int elem) {
-    for (const int k : {1, 2, 3, 4, 6, 8, 12, 16})
-        if (in * elem <= k * 32) return k;
-    return 0;
-}
-// A layer whose weight a workgroup holds: its LDS and workgroups, or none.
-struct Narrow {
-    int steps, threads, lds;
-    int64_t blocks, chunk;
-};
-template <class T>
-Narrow plan_narrow(int64_t rows, int64_t in, int64_t out, bool ragged) {
-    constexpr int elem = sizeof(T);
-    Narrow p{};
-    const int steps = narrow_steps(in, elem);
-    const int64_t tiles = elem == 4 ? up(out, 32) : up(out, 64) * 2, kib = tiles * steps;
-    if (!steps || kib > 112 || (rows < 4096 && kib > 16)) return p;
-    p.steps = steps;
-    p.threads = kib > 32 ? 512 : 256;
-    p.lds = static_cast<int>(kib * 1024 + tiles * 128) + p.threads / 64 * kUnitBytes<T>;
-    // with groups more workgroups than run at once: the rows worked on at a time lie closer together (1 M rows of 64 in 200 groups,
-    // 3 for each unit 90 us, 8 86)
-    const int64_t each = ragged ? 8 : std::max(1, std::min(p.threads == 512 ? 2 : 4, 160 * 1024 / p.lds));
-    p.blocks = std::max<int64_t>(1, std::min<int64_t>(256 * each, up(rows, p.threads / 2)));
-    p.chunk = std::max<int64_t>(up(up(rows, p.blocks), 32) * 32, 32);
-    p.blocks = std::max<int64_t>(up(rows, p.chunk), 1);
-    return p;
-}
-// A backward whose blocks of rows a workgroup holds.
-struct NarrowBwd {
-    int waves, zt, xt, lds;
-    bool fine;
-    int64_t blocks, chunk, size, bytes;
-};
-template <class T>
-NarrowBwd plan_narrow_bwd(int64_t rows, int64_t in, int64_t out, int groups, int act) {
-    NarrowBwd p{};
-    const int64_t kt = up(in, 32);
-    // dz is rounded to the type for its products, by which dx and dweight lose about what their own rounding takes. Where one of
-    // them has few elements chance may make that more, and the products are little next to the bytes: there dz is two terms
-    // (600,000 rows, 20 to 30, bfloat16: 76 us in one, 84 in two; 11 rows of 26 to 62: dx's error in one 1.5 times its own rounding's).
-    // (dy itself, and what relu leaves of it, has no more digits than the type.)
-    const bool wanted = sizeof(T) == 2 && act != kNone && act != kRelu && std::min(in * out, rows * in) < 1024;
-    p.fine = wanted && (out <= 32 || (out <= 64 && kt <= 4) || (out <= 128 && kt <= 2));
-    if (wanted && !p.fine && rows <= kFewRows) return p;  // (the few rows' kernels keep floats)
-    const int64_t nt = up(out, 32) * (p.fine ? 2 : 1);
-    if (nt <= 2 && kt <= 2) p.waves = 4, p.zt = p.xt = 2;
-    else if (sizeof(T) == 4) {  // (blocks of 64 rows of more floats do not fit; 919,424 rows, 32 to 80, by tiles 2,400 us, so 500)
-        if (nt <= 4 && kt <= 2) p.waves = 8, p.zt = 4, p.xt = 2;
-        else if (nt <= 2 && kt <= 4) p.waves = 8, p.zt = 2, p.xt = 4;
-        else return p;
-    } else if (nt <= 4 && kt <= 4) p.waves = 8, p.zt = p.xt = 4;
-    else if (nt <= 2 && kt <= 8) p.waves = 8, p.zt = 2, p.xt = 8;
-    else if (nt <= 8 && kt <= 2) p.waves = 8, p.zt = 8, p.xt = 2;
-    else return p;
-    p.lds = kBlockRows<T> * (line_bytes<T>(p.zt) + line_bytes<T>(p.xt)) + p.waves * kBareBytes<T> + p.zt * p.xt * static_cast<int>(sizeof(T)) * 1024;
-    static_assert(sizeof(T) == 4 || kBlockRows<T> * (line_bytes<T>(2) + line_bytes<T>(8)) + 8 * kBareBytes<T> + 16 * 2048 <= 160 * 1024);
-    const int64_t each = std::max(1, std::min(2, 160 * 1024 / p.lds));
-    p.blocks = std::max<int64_t>(1, std::min<int64_t>(256 * each, up(rows, kBlockRows<T>)));
-    p.chunk = std::max<int64_t>(up(up(rows, p.blocks), 32) * 32, 32);
-    p.blocks = std::max<int64_t>(up(rows, p.chunk), 1);
-    p.size = in * out + out;
-    p.bytes = (p.blocks + groups) * p.size * 4;
-    return p;
-}
 template <class T>
 void launch_narrow_bwd(const NarrowBwdArgs& a, const NarrowBwd& p, hipStream_t s) {
     const auto go = [&](auto kernel) { kernel<<<static_cast<uint32_t>(p.blocks), p.waves * 64, p.lds, s>>>(a); };
@@ -1565,16 +1389,6 @@ void launch_narrow_bwd(const NarrowBwdArgs& a, const NarrowBwd& p, hipStream_t s
         if (p.fine) by_terms(std::true_type{});
         else by_terms(std::false_type{});
     }
-}
-
-// Whether a forward's groups have so few rows that the weights' bytes are what it takes (and its workgroups fit a launch).
-bool few_rows(int64_t rows, int64_t out, int groups) {
-    return (rows <= 32 || rows / groups <= 16) && up(out, 32) * (groups + 1 + (rows >> kFewShift)) < int64_t{1} << 22;
-}
-// Whether a backward's rows are.
-template <class T>
-bool few_rows_backward(int64_t rows, int64_t in, int64_t out, int groups) {
-    return rows <= kFewRows && out <= 8 * 65535 && up(in, kFewBlock * kPer<T>) * up(out, 8) * groups < int64_t{1} << 24;
 }
 
 template <class T>
@@ -1619,7 +1433,7 @@ void forward(const LinearFwdArgs& f, Run& run) {
     const Finish to{f.y, f.y_stride, f.out, f.residual, f.residual_stride, f.pre, f.pre_stride, f.act, f.clear};
     const Groups groups{f.ends, f.groups, f.rows};
     const bool ragged = f.ends != nullptr;
-    if (const Narrow p = plan_narrow<T>(f.rows, f.in, f.out, ragged); p.blocks) {
+    if (const Narrow p = plan_narrow(f.rows, f.in, f.out, ragged, sizeof(T)); p.blocks) {
         if (run.real) launch_narrow<T>({f.x, f.weight, f.bias, f.x_stride, to, f.in, f.out, p.chunk, groups}, p, run.stream);
         return;
     }
@@ -1703,11 +1517,11 @@ template <class T>
 void backward(const LinearBwdArgs& f, Run& run) {
     const bool ragged = f.ends != nullptr;
     const Groups groups{f.ends, f.groups, f.rows};
-    if (const NarrowBwd p = plan_narrow_bwd<T>(f.rows, f.in, f.out, f.groups, f.act); p.blocks) {
+    if (const NarrowBwd p = plan_narrow_bwd(f.rows, f.in, f.out, f.groups, f.act != kNone && f.act != kRelu, sizeof(T)); p.blocks) {
         backward_narrow<T>(f, p, run);
         return;
     }
-    if (few_rows_backward<T>(f.rows, f.in, f.out, f.groups)) {
+    if (few_rows_backward(f.rows, f.in, f.out, f.groups, sizeof(T))) {
         backward_few<T>(f, run);
         return;
     }

@@ -1,0 +1,215 @@
+// sx_linear_plan.h — how the linear layers' calls are divided (sx_linear.h has the kernels): which kernels take one, their tiles,
+// parts, workgroups, LDS and workspace, from sizes and types alone. Plain C++, so that any compiler checks it over all sizes.
+// `elem` is the elements' bytes, 4 or 2.
+#pragma once
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+
+namespace sxk {
+namespace {
+
+int log2_up(int64_t n) {
+    int k = 0;
+    while ((int64_t{1} << k) < n) k++;
+    return k;
+}
+int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to; }
+// Slots of a division of all groups' rows into parts of 2^shift (Groups and part_of in sx_mma.h).
+int64_t slots_of(int64_t rows, int groups, int shift, bool ragged) {
+    return ragged ? groups + 1 + (rows >> shift) : ((rows + (int64_t{1} << shift) - 1) >> shift);
+}
+
+// Few rows: a forward's workgroups have kFewWaves waves for a part of 2^kFewShift rows, a backward up to kFewRows rows and kFewBlock
+// threads a workgroup.
+constexpr int kFewWaves = 8, kFewShift = 5, kFewRows = 32, kFewBlock = 128;
+
+// ---- LDS ----------------------------------------------------------------------------------------------------
+
+// A wave's outputs on their way to whole lines (Unit in sx_linear.h): `unit_tiles` tiles of 32 columns side by side, as floats, 32
+// lines (of eight rows in different banks), and of sums that are the outputs in the type.
+constexpr int unit_tiles(int elem) { return 4 / elem; }
+constexpr int unit_line(int elem) { return unit_tiles(elem) * 128 + 16; }
+constexpr int unit_bytes(int elem) { return 32 * unit_line(elem); }
+constexpr int kBareLine = 128 + 16;
+constexpr int kBareBytes = 32 * kBareLine;
+// A narrow backward's block of rows, and the bytes between its lines: `tiles` times 32 elements, and what puts four lines (floats:
+// the lanes' lines) into different banks.
+constexpr int block_rows(int elem) { return 256 / elem; }
+constexpr int line_bytes(int tiles, int elem) { return tiles * 32 * elem + (elem == 2 ? 32 : 16); }
+
+// ---- tiles --------------------------------------------------------------------------------------------------
+
+// The tiles to choose from: their rows and columns, how many run at once on 256 units, and what a step of 128 bytes of the
+// sums' length then takes, in ns of 16-bit elements (floats: as many bytes, 4.6 times), and what a tile takes besides. Measured on layers of 16,383 rows, 8192 to
+// 2048: 542, 623 and 712 us by tiles of 256, 128 and 64 rows; 20,001 rows in 16 groups, 1024 to 1408, whose tiles of 256 rows
+// take three rounds for two: 121, 104 and 106.
+struct TileKind {
+    int rows, cols, at_once;
+    double step, fixed;
+};
+constexpr TileKind kTileKinds[] = {{256, 256, 256, 1950, 6000}, {128, 128, 512, 1150, 3000}, {64, 128, 768, 1050, 2500}};
+constexpr double kJoinFixed = 4000, kJoinBytes = 4;  // ns; bytes a ns
+// `tiles` of `steps` each; a unit's only workgroup of a kind that shares it goes faster.
+double tiles_take(const TileKind& k, double tiles, double steps, int elem) {
+    const double step = k.step * (elem == 4 ? 4.6 : 1.0) * (tiles <= 256 && k.at_once > 256 ? 0.6 : 1.0);
+    return std::max(1.0, std::ceil(tiles / k.at_once)) * (k.fixed + steps * step);
+}
+
+// out[rows][cols] over `depth`, rows in groups: the tile's rows, and how many parts the depth is split into.
+struct Plan {
+    int side, splits;
+    int64_t split, bytes;
+};
+Plan plan_rows(int64_t rows, int64_t cols, int64_t depth, int groups, bool ragged, int elem) {
+    const int64_t step = 128 / elem, steps = up(depth, step);
+    Plan best{};
+    double least = INFINITY;
+    for (const TileKind& k : kTileKinds) {
+        if (elem == 4 && k.rows == 256) continue;  // (floats' products are 16 times as long as their reads: 128 are enough)
+        // (a group's last tile is half full)
+        const double down = ragged ? static_cast<double>(rows) / k.rows + 0.5 * static_cast<double>(std::min<int64_t>(groups, rows)) : static_cast<double>(up(rows, k.rows));
+        const double tiles = down * static_cast<double>(up(cols, k.cols));
+        for (int64_t splits = 1; splits <= 64 && (splits == 1 || steps / splits >= 2); splits *= 2) {
+            const int64_t each = up(steps, splits), parts = up(steps, each), bytes = parts > 1 ? parts * rows * cols * 4 : 0;
+            if (bytes > int64_t{64} << 20) break;
+            const double time = tiles_take(k, tiles * static_cast<double>(parts), static_cast<double>(each), elem) +
+                                (parts > 1 ? kJoinFixed + 2.0 * static_cast<double>(bytes) / kJoinBytes / 1000 : 0.0);
+            if (time < least) {
+                least = time;
+                best = {k.rows, static_cast<int>(parts), each * step, bytes};
+            }
+        }
+    }
+    return best;
+}
+// out[groups][out][in] over the groups' rows: the tile's rows, and the parts of the rows (shift 62: each group's are one).
+struct Over {
+    int side, shift;
+    int64_t slots, bytes;
+};
+Over plan_over(int64_t rows, int64_t out, int64_t in, int groups, bool ragged, int elem) {
+    const double step = 128.0 / elem, all = static_cast<double>(rows) / step;
+    Over best{};
+    double least = INFINITY;
+    for (const TileKind& k : kTileKinds) {
+        if (elem == 4 && k.rows == 256) continue;
+        const double tiles = static_cast<double>(up(out, k.rows) * up(in, k.cols));
+        // one part each: the largest group is taken to have three times an even share
+        const double even = tiles_take(k, tiles * groups, all / groups, elem);
+        double time = std::max(even, groups > 1 ? tiles_take(k, 1, std::min(all, 3 * all / groups), elem) : 0.0);
+        if (time < least) {
+            least = time;
+            best = {k.rows, 62, groups, 0};
+        }
+        for (int shift = 8; (int64_t{1} << shift) < rows; shift++) {
+            const int64_t slots = slots_of(rows, groups, shift, ragged), bytes = slots * out * in * 4;
+            if (bytes > int64_t{256} << 20 || slots > 65535) continue;
+            const double parts = ragged ? static_cast<double>(rows >> shift) + 0.5 * groups : static_cast<double>(slots);
+            time = tiles_take(k, tiles * parts, static_cast<double>(int64_t{1} << shift) / step, elem) + kJoinFixed +
+                   2.0 * parts * static_cast<double>(out * in) * 4 / kJoinBytes / 1000;
+            if (time < least) {
+                least = time;
+                best = {k.rows, shift, slots, bytes};
+            }
+        }
+    }
+    return best;
+}
+struct Slope {
+    int shift, lanes;
+    int64_t slots, columns, bytes, dz_stride, dz_bytes;
+};
+Slope plan_slope(int64_t rows, int64_t cols, int groups, bool ragged, int elem) {
+    Slope p{};
+    const int64_t vectors = up(cols, 16 / elem);
+    p.lanes = static_cast<int>(std::min<int64_t>(vectors, 256));
+    p.columns = up(vectors, p.lanes);
+    p.shift = std::max({log2_up(256 / p.lanes) + 2, log2_up(up(std::max<int64_t>(rows, 1), std::max<int64_t>(1, 1024 / p.columns)))});
+    p.slots = slots_of(rows, groups, p.shift, ragged);
+    p.bytes = p.slots * cols * 4;
+    p.dz_stride = vectors * (16 / elem);
+    p.dz_bytes = rows * p.dz_stride * elem;
+    return p;
+}
+
+// ---- narrow layers ------------------------------------------------------------------------------------------
+
+// The steps of 32 bytes of a row that k_narrow_fwd is built for, or 0.
+int narrow_steps(int64_t in, int elem) {
+    for (const int k : {1, 2, 3, 4, 6, 8, 12, 16})
+        if (in * elem <= k * 32) return k;
+    return 0;
+}
+// A layer whose weight a workgroup holds: its LDS and workgroups, or none.
+struct Narrow {
+    int steps, threads, lds;
+    int64_t blocks, chunk;
+};
+Narrow plan_narrow(int64_t rows, int64_t in, int64_t out, bool ragged, int elem) {
+    Narrow p{};
+    const int steps = narrow_steps(in, elem);
+    const int64_t tiles = elem == 4 ? up(out, 32) : up(out, 64) * 2, kib = tiles * steps;
+    if (!steps || kib > 112 || (rows < 4096 && kib > 16)) return p;
+    p.steps = steps;
+    p.threads = kib > 32 ? 512 : 256;
+    p.lds = static_cast<int>(kib * 1024 + tiles * 128) + p.threads / 64 * unit_bytes(elem);
+    // with groups more workgroups than run at once: the rows worked on at a time lie closer together (1 M rows of 64 in 200 groups,
+    // 3 for each unit 90 us, 8 86)
+    const int64_t each = ragged ? 8 : std::max(1, std::min(p.threads == 512 ? 2 : 4, 160 * 1024 / p.lds));
+    p.blocks = std::max<int64_t>(1, std::min<int64_t>(256 * each, up(rows, p.threads / 2)));
+    p.chunk = std::max<int64_t>(up(up(rows, p.blocks), 32) * 32, 32);
+    p.blocks = std::max<int64_t>(up(rows, p.chunk), 1);
+    return p;
+}
+// A backward whose blocks of rows a workgroup holds.
+struct NarrowBwd {
+    int waves, zt, xt, lds;
+    bool fine;
+    int64_t blocks, chunk, size, bytes;
+};
+NarrowBwd plan_narrow_bwd(int64_t rows, int64_t in, int64_t out, int groups, bool curved, int elem) {
+    NarrowBwd p{};
+    const int64_t kt = up(in, 32);
+    // dz is rounded to the type for its products, by which dx and dweight lose about what their own rounding takes. Where one of
+    // them has few elements chance may make that more, and the products are little next to the bytes: there dz is two terms
+    // (600,000 rows, 20 to 30, bfloat16: 76 us in one, 84 in two; 11 rows of 26 to 62: dx's error in one 1.5 times its own rounding's).
+    // (dy itself, and what relu leaves of it, has no more digits than the type.)
+    const bool wanted = elem == 2 && curved && std::min(in * out, rows * in) < 1024;
+    p.fine = wanted && (out <= 32 || (out <= 64 && kt <= 4) || (out <= 128 && kt <= 2));
+    if (wanted && !p.fine && rows <= kFewRows) return p;  // (the few rows' kernels keep floats)
+    const int64_t nt = up(out, 32) * (p.fine ? 2 : 1);
+    if (nt <= 2 && kt <= 2) p.waves = 4, p.zt = p.xt = 2;
+    else if (elem == 4) {  // (blocks of 64 rows of more floats do not fit; 919,424 rows, 32 to 80, by tiles 2,400 us, so 500)
+        if (nt <= 4 && kt <= 2) p.waves = 8, p.zt = 4, p.xt = 2;
+        else if (nt <= 2 && kt <= 4) p.waves = 8, p.zt = 2, p.xt = 4;
+        else return p;
+    } else if (nt <= 4 && kt <= 4) p.waves = 8, p.zt = p.xt = 4;
+    else if (nt <= 2 && kt <= 8) p.waves = 8, p.zt = 2, p.xt = 8;
+    else if (nt <= 8 && kt <= 2) p.waves = 8, p.zt = 8, p.xt = 2;
+    else return p;
+    p.lds = block_rows(elem) * (line_bytes(p.zt, elem) + line_bytes(p.xt, elem)) + p.waves * kBareBytes + p.zt * p.xt * elem * 1024;
+    static_assert(block_rows(2) * (line_bytes(2, 2) + line_bytes(8, 2)) + 8 * kBareBytes + 16 * 2048 <= 160 * 1024);
+    const int64_t each = std::max(1, std::min(2, 160 * 1024 / p.lds));
+    p.blocks = std::max<int64_t>(1, std::min<int64_t>(256 * each, up(rows, block_rows(elem))));
+    p.chunk = std::max<int64_t>(up(up(rows, p.blocks), 32) * 32, 32);
+    p.blocks = std::max<int64_t>(up(rows, p.chunk), 1);
+    p.size = in * out + out;
+    p.bytes = (p.blocks + groups) * p.size * 4;
+    return p;
+}
+
+// ---- few rows -----------------------------------------------------------------------------------------------
+
+// Whether a forward's groups have so few rows that the weights' bytes are what it takes (and its workgroups fit a launch).
+bool few_rows(int64_t rows, int64_t out, int groups) {
+    return (rows <= 32 || rows / groups <= 16) && up(out, 32) * (groups + 1 + (rows >> kFewShift)) < int64_t{1} << 22;
+}
+// Whether a backward's rows are.
+bool few_rows_backward(int64_t rows, int64_t in, int64_t out, int groups, int elem) {
+    return rows <= kFewRows && out <= 8 * 65535 && up(in, kFewBlock * 16 / elem) * up(out, 8) * groups < int64_t{1} << 24;
+}
+
+}  // namespace
+}  // namespace sxk

@@ -173,9 +173,5 @@ __device__ inline Part part_of(const Groups& g, int64_t slot, int shift) {
     const int64_t begin = start + (part << shift);
     return {k, min(begin, end), min(end, begin + (int64_t{1} << shift))};
 }
-// (of a division of all groups)
-__host__ __device__ inline int64_t slots_of(int64_t rows, int groups, int shift, bool ragged) {
-    return ragged ? groups + 1 + (rows >> shift) : ((rows + (int64_t{1} << shift) - 1) >> shift);
-}
 
 }  // namespace sxd
