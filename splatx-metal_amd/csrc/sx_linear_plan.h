@@ -27,6 +27,8 @@ constexpr int kFewWaves = 8, kFewShift = 5, kFewRows = 32, kFewBlock = 128;
 
 // ---- LDS ----------------------------------------------------------------------------------------------------
 
+constexpr int kLds = 160 * 1024;  // a workgroup's most
+
 // A wave's outputs on their way to whole lines (Unit in sx_linear.h): `unit_tiles` tiles of 32 columns side by side, as floats, 32
 // lines (of eight rows in different banks), and of sums that are the outputs in the type.
 constexpr int unit_tiles(int elem) { return 4 / elem; }
@@ -152,12 +154,18 @@ Narrow plan_narrow(int64_t rows, int64_t in, int64_t out, bool ragged, int elem)
     const int steps = narrow_steps(in, elem);
     const int64_t tiles = elem == 4 ? up(out, 32) : up(out, 64) * 2, kib = tiles * steps;
     if (!steps || kib > 112 || (rows < 4096 && kib > 16)) return p;
+    const int held = static_cast<int>(kib * 1024 + tiles * 128), eight = held + 8 * unit_bytes(elem);
+    // Where eight waves' outputs have no room beside the weight four waves' have. Four waves alone on a unit hide less, and each
+    // workgroup fetches the weight: they pay for short rows, many of them, of one group; else tiles take the layer. (bfloat16 and half,
+    // us of four waves and by tiles: 1 M rows 64 to 768 462 and 630, 300,000 rows 96 to 512 136 and 194, 40,000 rows 38 and 33;
+    // 100,000 rows 128 to 384 56 and 44; 4096 rows 64 to 768 26 and 8; 300,000 rows in 16 groups 64 to 768 396 and 217.)
+    if (eight > kLds && (steps > 6 || ragged || rows < 65536)) return p;
     p.steps = steps;
-    p.threads = kib > 32 ? 512 : 256;
-    p.lds = static_cast<int>(kib * 1024 + tiles * 128) + p.threads / 64 * unit_bytes(elem);
+    p.threads = kib > 32 && eight <= kLds ? 512 : 256;
+    p.lds = held + p.threads / 64 * unit_bytes(elem);
     // with groups more workgroups than run at once: the rows worked on at a time lie closer together (1 M rows of 64 in 200 groups,
     // 3 for each unit 90 us, 8 86)
-    const int64_t each = ragged ? 8 : std::max(1, std::min(p.threads == 512 ? 2 : 4, 160 * 1024 / p.lds));
+    const int64_t each = ragged ? 8 : std::min(p.threads == 512 ? 2 : 4, kLds / p.lds);
     p.blocks = std::max<int64_t>(1, std::min<int64_t>(256 * each, up(rows, p.threads / 2)));
     p.chunk = std::max<int64_t>(up(up(rows, p.blocks), 32) * 32, 32);
     p.blocks = std::max<int64_t>(up(rows, p.chunk), 1);
@@ -190,8 +198,8 @@ NarrowBwd plan_narrow_bwd(int64_t rows, int64_t in, int64_t out, int groups, boo
     else if (nt <= 8 && kt <= 2) p.waves = 8, p.zt = 8, p.xt = 2;
     else return p;
     p.lds = block_rows(elem) * (line_bytes(p.zt, elem) + line_bytes(p.xt, elem)) + p.waves * kBareBytes + p.zt * p.xt * elem * 1024;
-    static_assert(block_rows(2) * (line_bytes(2, 2) + line_bytes(8, 2)) + 8 * kBareBytes + 16 * 2048 <= 160 * 1024);
-    const int64_t each = std::max(1, std::min(2, 160 * 1024 / p.lds));
+    static_assert(block_rows(2) * (line_bytes(2, 2) + line_bytes(8, 2)) + 8 * kBareBytes + 16 * 2048 <= kLds);
+    const int64_t each = std::min(2, kLds / p.lds);
     p.blocks = std::max<int64_t>(1, std::min<int64_t>(256 * each, up(rows, block_rows(elem))));
     p.chunk = std::max<int64_t>(up(up(rows, p.blocks), 32) * 32, 32);
     p.blocks = std::max<int64_t>(up(rows, p.chunk), 1);

@@ -1,0 +1,55 @@
+// Every plan of the linear layers over their sizes, against what a workgroup and a launch can hold: the plans that do not fit, one a
+// line, and how many were looked at.
+#include <cstdio>
+
+#include "sx_linear_plan.h"
+
+using namespace sxk;
+
+namespace {
+
+constexpr int kMostLds = 163840;  // of a workgroup, bytes
+long looked = 0;
+
+void narrow() {
+    for (const int elem : {2, 4})
+        for (int in = 1; in <= 520 / elem; in++)
+            for (int out = 1; out <= 3700; out++)
+                for (const long rows : {1L, 1000L, 4095L, 4096L, 100'000L, 40'000'000L})
+                    for (const bool ragged : {false, true}) {
+                        const Narrow p = plan_narrow(rows, in, out, ragged, elem);
+                        if (!p.blocks) continue;
+                        looked++;
+                        // the weight's fragments, the bias, each wave's outputs
+                        const long tiles = elem == 4 ? up(out, 32) : up(out, 64) * 2;
+                        const long lds = tiles * p.steps * 1024 + tiles * 128 + p.threads / 64 * unit_bytes(elem);
+                        if (p.lds != lds || lds > kMostLds || p.steps * 32 < in * elem || p.blocks > 65535 || p.chunk < 32 || p.chunk % 32 ||
+                            (ragged ? p.blocks * p.chunk < rows : (p.blocks - 1) * (p.threads / 2) >= rows))
+                            std::printf("forward %ld rows, %d to %d, elem %d, ragged %d: lds %d threads %d\n", rows, in, out, elem, ragged, p.lds, p.threads);
+                    }
+}
+
+void narrow_backward() {
+    for (const int elem : {2, 4})
+        for (int in = 1; in <= 300; in++)
+            for (int out = 1; out <= 300; out++)
+                for (const long rows : {0L, 1L, 32L, 33L, 4096L, 40'000'000L})
+                    for (const int groups : {1, 7, 32768})
+                        for (const bool curved : {false, true}) {
+                            const NarrowBwd p = plan_narrow_bwd(rows, in, out, groups, curved, elem);
+                            if (!p.blocks) continue;
+                            looked++;
+                            const int terms = p.fine ? 2 : 1;
+                            if (p.lds > kMostLds || up(out, 32) * terms > p.zt || up(in, 32) > p.xt || p.blocks > 65535 || p.blocks * p.chunk < rows ||
+                                (rows && (p.blocks - 1) * block_rows(elem) >= rows) || p.bytes != (p.blocks + groups) * (1L * in * out + out) * 4)
+                                std::printf("backward %ld rows, %d to %d, elem %d, groups %d: lds %d\n", rows, in, out, elem, groups, p.lds);
+                        }
+}
+
+}  // namespace
+
+int main() {
+    narrow();
+    narrow_backward();
+    std::printf("looked at %ld\n", looked);
+}
