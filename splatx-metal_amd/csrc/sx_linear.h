@@ -142,28 +142,34 @@ struct Stage {
 };
 
 // The same straight from memory into LDS, of whole tiles whose lines begin on 16 bytes: a wave's load fills 1 KiB of LDS in the
-// order of the lanes, so that it is the lane's place in memory that goes by where the chunk lies.
+// order of the lanes, so that it is the lane's place in memory that goes by where the chunk lies. A plain operand's eight lines
+// of a load have a beginning of their own: those of the whole tile may be further apart than 32 bits reach.
 template <class T, int R, bool Across, int Threads>
 struct DirectStage {
-    static constexpr int V = kPer<T>, kDepth = 128 / static_cast<int>(sizeof(T)), N = R * 8 / Threads;
-    const char* base;
-    int64_t step;       // bytes to the next tile
+    static constexpr int V = kPer<T>, kDepth = kTileDepthBytes / static_cast<int>(sizeof(T)), N = R * 8 / Threads;
+    static_assert(kTileDepthBytes * kLoadLines == 64 * 16);
+    const char* base[Across ? 1 : N];
+    int64_t step;        // bytes to the next tile
     uint32_t offset[N];  // of the lane's chunks
     // As Stage's; `d` the sums' first element
     __device__ DirectStage(const T* b, int64_t s, int64_t f, int64_t l, int64_t d) {
         const int64_t line = s * static_cast<int64_t>(sizeof(T));
-        base = reinterpret_cast<const char*>(b) + (Across ? d * line : f * line + d * static_cast<int64_t>(sizeof(T)));
-        step = Across ? kDepth * line : 128;
+        const char* const from = reinterpret_cast<const char*>(b);
+        step = Across ? kDepth * line : kTileDepthBytes;
+        if constexpr (Across) base[0] = from + d * line;
 #pragma unroll
         for (int i = 0; i < N; i++) {
-            const int at = (i * Threads + static_cast<int>(threadIdx.x)) * 16;  // in the tile
             if constexpr (Across) {
                 constexpr int kLine = R * static_cast<int>(sizeof(T));
+                const int at = (i * Threads + static_cast<int>(threadIdx.x)) * 16;  // in the tile
                 const int m = at / kLine, byte = across_at<T>(m, at % kLine, kLine) - m * kLine;
-                offset[i] = static_cast<uint32_t>(m * line + min(f * static_cast<int64_t>(sizeof(T)) + byte, (l - V) * static_cast<int64_t>(sizeof(T))));
+                offset[i] = static_cast<uint32_t>(
+                    across_offset(m, line, min(f * static_cast<int64_t>(sizeof(T)) + byte, (l - V) * static_cast<int64_t>(sizeof(T)))));
             } else {
-                const int r = at / 128, c = (at / 16 % 8) ^ (r >> 1 & 7);
-                offset[i] = static_cast<uint32_t>(min(int64_t{r}, l - 1 - f) * line + c * 16);
+                const int first = i * Threads / 8 + wave_of() * kLoadLines, r = first + static_cast<int>(threadIdx.x) % 64 / 8;
+                const int64_t last = l - 1 - f, start = min(int64_t{first}, last);
+                base[i] = from + (f + start) * line + d * static_cast<int64_t>(sizeof(T));
+                offset[i] = static_cast<uint32_t>(plain_offset(min(int64_t{r}, last) - start, line, static_cast<int>(threadIdx.x) % 8 ^ (r >> 1 & 7)));
             }
         }
     }
@@ -171,9 +177,12 @@ struct DirectStage {
         using Global = __attribute__((address_space(1))) const void*;
         using Lds = __attribute__((address_space(3))) void*;
 #pragma unroll
-        for (int i = 0; i < N; i++)
-            __builtin_amdgcn_global_load_lds((Global)(base + offset[i]), (Lds)(lds + (i * Threads + wave_of() * 64) * 16), 16, 0, 0);
-        base += step;
+        for (int i = 0; i < N; i++) {
+            const char* const p = base[Across ? 0 : i];
+            __builtin_amdgcn_global_load_lds((Global)(p + offset[i]), (Lds)(lds + (i * Threads + wave_of() * 64) * 16), 16, 0, 0);
+            if constexpr (!Across) base[i] += step;
+        }
+        if constexpr (Across) base[0] += step;
     }
 };
 
@@ -1339,7 +1348,7 @@ struct Operand {
 template <class T>
 Operand operand(const void* p, int64_t rows, int64_t width, int64_t stride, bool across, Run& run) {
     const bool fits = reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * static_cast<int64_t>(sizeof(T)) % 16 == 0 &&
-                      stride < (int64_t{1} << 30) / 256 / static_cast<int>(sizeof(T)) && (!across || width % kPer<T> == 0);
+                      stride <= kMostLine / static_cast<int>(sizeof(T)) && (!across || width % kPer<T> == 0);
     if (fits || !rows) return {p, stride, width};
     const Slope plan = plan_slope(rows, width, 1, false, sizeof(T));
     SlopeArgs a{};

@@ -59,6 +59,16 @@ double tiles_take(const TileKind& k, double tiles, double steps, int elem) {
     return std::max(1.0, std::ceil(tiles / k.at_once)) * (k.fixed + steps * step);
 }
 
+// A tile's lines in memory, those of an operand's rows, may be so many bytes apart: then what a lane adds to its load's beginning,
+// which is 32 bits, is `plain_offset` or `across_offset`. (A row of the most elements, 2^24 floats.)
+constexpr int64_t kMostLine = int64_t{1} << 26;
+constexpr int kTileDepthBytes = 128;
+// Plain: a load of a wave's takes 128 bytes of each of eight lines, from a beginning of its own. Across: whole rows of a tile's
+// depth, from the tile's beginning.
+constexpr int kLoadLines = 8;
+constexpr int64_t plain_offset(int64_t lines, int64_t line, int chunk) { return lines * line + chunk * 16; }
+constexpr int64_t across_offset(int64_t lines, int64_t line, int64_t byte) { return lines * line + byte; }
+
 // out[rows][cols] over `depth`, rows in groups: the tile's rows, and how many parts the depth is split into.
 struct Plan {
     int side, splits;

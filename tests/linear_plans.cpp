@@ -46,9 +46,25 @@ void narrow_backward() {
                         }
 }
 
+// What a tile's loads add to their beginnings in 32 bits, of rows of any width that a layer may have.
+void offsets() {
+    for (const int elem : {2, 4})
+        for (int width = 0; width <= 24; width++)
+            for (const int less : {0, 1}) {
+                const long in = (1L << width) - less, line = up(in, 16 / elem) * 16;
+                if (in < 1) continue;
+                const int depth = kTileDepthBytes / elem;
+                looked++;
+                if (line > kMostLine) std::printf("rows of %ld, elem %d: lines of %ld bytes, over %ld\n", in, elem, line, kMostLine);
+                if (plain_offset(kLoadLines - 1, kMostLine, 7) >> 32 || across_offset(depth - 1, kMostLine, kMostLine - 16) >> 32)
+                    std::printf("elem %d: offsets past 32 bits\n", elem);
+            }
+}
+
 }  // namespace
 
 int main() {
+    offsets();
     narrow();
     narrow_backward();
     std::printf("looked at %ld\n", looked);

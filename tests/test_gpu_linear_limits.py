@@ -1,4 +1,4 @@
-"""Linear layers at the limits of their plans: weights that fill a workgroup's LDS."""
+"""Linear layers at the limits of their plans: weights that fill a workgroup's LDS, rows of the most elements."""
 import pytest
 import torch  # before anything loads the library: its HIP runtime is the process's
 
@@ -14,3 +14,39 @@ pytestmark = pytest.mark.gpu
     (BF16, 128, 320), (F16, 40, 900), (BF16, 16, 3584), (F16, 13, 3500), (BF16, 200, 130), (F32, 8, 3584), (F32, 5, 3530), (F32, 8, 3520), (F32, 64, 384)])
 def test_weights_that_fill_the_lds(tb, dtype, n_in, n_out, rows, sizes):  # noqa: F811
     compare(tb, rows, n_in, n_out, dtype, "silu", add=True, pad=n_in % 3, sizes=sizes, seed=n_in)
+
+
+# Rows of as many elements as a layer may have: a tile's lines lie 2^25 bytes (16 bits) and 2^26 (floats) apart, 256 and 128 of them
+# (64 floats' already 2^32 bytes).
+@pytest.mark.parametrize("dtype,rows,n_in,n_out", [(F32, 33, 1 << 24, 100), (BF16, 40, 1 << 24, 200), (F16, 260, (1 << 23) + 8, 40), (F32, 100, 5, 1 << 24),
+                                                   (BF16, 264, 3, (1 << 24) - 8)])
+def test_rows_of_the_most_elements(tb, dtype, rows, n_in, n_out):  # noqa: F811
+    """Whole numbers, -1 to 1: every partial sum is exact. Compared a range of the long dimension at a time."""
+    print(dtype, rows, n_in, n_out, flush=True)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    part = 1 << 20
+
+    def ones(n, m):
+        t = torch.empty(n, m, dtype=dtype, device="cuda")
+        for c in range(0, m, part):
+            t[:, c:c + part] = torch.randint(-1, 2, (n, min(part, m - c)), generator=g, device="cuda", dtype=torch.int8)
+        return t
+
+    x, w, dy = ones(rows, n_in), (ones(n_out, n_in) if n_out < n_in else ones(n_in, n_out).t().contiguous()), ones(rows, n_out)
+    y, _ = tb.linear_fwd(x, w)
+    dx, dw, db = tb.linear_bwd(dy, x, w)
+    wide = range(0, max(n_in, n_out), part)
+    if n_in > n_out:
+        z = sum(x[:, c:c + part].double() @ w[:, c:c + part].double().t().contiguous() for c in wide)
+        assert torch.equal(y, z.to(dtype))
+        for c in wide:
+            assert torch.equal(dx[:, c:c + part], (dy.double() @ w[:, c:c + part].double()).to(dtype))
+            assert torch.equal(dw[:, c:c + part], (dy.double().t().contiguous() @ x[:, c:c + part].double()).to(dtype))
+        assert torch.equal(db, dy.double().sum(0).to(dtype))
+        return
+    d = sum(dy[:, c:c + part].double() @ w[c:c + part].double() for c in wide)
+    assert torch.equal(dx, d.to(dtype))
+    for c in wide:
+        assert torch.equal(y[:, c:c + part], (x.double() @ w[c:c + part].double().t().contiguous()).to(dtype))
+        assert torch.equal(dw[c:c + part], (dy[:, c:c + part].double().t().contiguous() @ x.double()).to(dtype))
+        assert torch.equal(db[c:c + part], dy[:, c:c + part].double().sum(0).to(dtype))
