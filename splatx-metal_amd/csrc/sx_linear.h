@@ -1173,7 +1173,8 @@ __global__ void __launch_bounds__(kFewBlock) k_few_dx(FewBwdArgs a) {
                     Frag<T> v[kBatch];
                     few_chunks<T, kBatch>(v, w, a.in, n + o, n1, c, a.in);
 #pragma unroll
-                    for (int b = 0; b < kBatch; b++) {  // (dz is zero past the slice's end)
+                    for (int b = 0; b < kBatch; b++) {
+                        if (o + b >= here) break;  // (past the slice's end lies its last row again, and an infinity times 0 is none)
                         const Floats<V> f = floats<T, V>(v[b]);
 #pragma unroll
                         for (int q = 0; q < kAtOnce; q += 4) {
