@@ -985,9 +985,10 @@ __global__ void __launch_bounds__(Waves * 64) k_narrow_bwd(NarrowBwdArgs a) {
 //
 // A layer of few rows is bound by its weight's bytes, each read once. Forward: a workgroup has 32 outputs, its waves share the
 // sums' length, 128 bytes of each weight's row at a time in turn, and add their sums in LDS at the end. What they read comes
-// through LDS of the wave's own, where lines begin on 16 bytes: a load of 16 bytes each from 32 rows takes four times as long as
-// one of whole lines, and half of them are x's, again and again. (9 rows of 2048 to 8192 in half precision: 15 us by
-// tiles, 10.5 by such loads, 9 so: 3.7 TB/s.)
+// through LDS of the wave's own, straight there where all lines begin on 16 bytes, else through registers: a load of 16 bytes each
+// from 32 rows takes four times as long as one of whole lines, and half of them are x's, again and again. (9 rows to 8192 in half
+// precision, us: of 2048 15 by tiles, 10.5 by such loads, 8.9 so, 3.7 TB/s; of 2049 19.5 by such loads, 9.6 so. 2 rows of 7187 to
+// 2267 in floats 35 and 20.4, the library's product 28.)
 struct FewArgs {
     const void *x, *weight, *bias;
     int64_t x_stride;
@@ -999,7 +1000,7 @@ struct FewArgs {
 };
 template <class T, bool Lines>
 __global__ void __launch_bounds__(kFewWaves * 64) k_few_fwd(FewArgs a) {
-    constexpr int V = kPer<T>, kLine = 128 / static_cast<int>(sizeof(T)), kAtOnce = 4, kPitch = 36;
+    constexpr int V = kPer<T>, kLine = 128 / static_cast<int>(sizeof(T)), kPitch = 36;
     // (two arrays, so that a load into one is seen to be no store into the other)
     __shared__ __attribute__((aligned(128))) char lds[kFewWaves * 8192], lds1[Lines ? kFewWaves * 8192 : 16];
     static_assert(sizeof(float) * 32 * kPitch <= 8192);
@@ -1020,43 +1021,48 @@ __global__ void __launch_bounds__(kFewWaves * 64) k_few_fwd(FewArgs a) {
     const T* const w = weight + min(c0 + lane % 32, a.out - 1) * a.in;
     const T* const x = xs + min(part.begin + lane % 32, part.end - 1) * a.x_stride;
     Sums s(0.0f);
-    int64_t begin = 0;
-    if constexpr (Lines) {
-        // The wave's lines: `wave` and every eighth after it. A load of the wave's fills 1 KiB: eight rows.
-        using Global = __attribute__((address_space(1))) const void*;
-        using Lds = __attribute__((address_space(3))) void*;
-        const int64_t lines = length / kLine, mine = (lines - wave + kFewWaves - 1) / kFewWaves;
-        begin = lines * kLine;
-        const T *from_w[4], *from_x[4];
+    // The wave's lines: `wave` and every eighth after it. A load of the wave's takes eight rows', as they lie in a tile (plain_at).
+    const int64_t lines = length / kLine, mine = (lines - wave + kFewWaves - 1) / kFewWaves;
+    const T *from_w[4], *from_x[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int row = i * 8 + lane / 8, chunk = (plain_at(row, lane % 8) - row * 128) / 16 * V;
+        from_w[i] = weight + min(c0 + row, a.out - 1) * a.in + wave * kLine + chunk;
+        from_x[i] = xs + min(part.begin + row, part.end - 1) * a.x_stride + wave * kLine + chunk;
+    }
+    const auto product = [&](const char* now) {
+        Frag<T> fw[4], fx[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const int row = i * 8 + lane / 8, chunk = (plain_at(row, lane % 8) - row * 128) / 16 * V;
-            from_w[i] = weight + min(c0 + row, a.out - 1) * a.in + wave * kLine + chunk;
-            from_x[i] = xs + min(part.begin + row, part.end - 1) * a.x_stride + wave * kLine + chunk;
+            fw[i] = *reinterpret_cast<const Frag<T>*>(now + wave * 8192 + plain_at(lane % 32, 2 * i + half));
+            fx[i] = *reinterpret_cast<const Frag<T>*>(now + wave * 8192 + 4096 + plain_at(lane % 32, 2 * i + half));
         }
-        int64_t loaded = 0;
-        const auto load = [&](char* to) {  // (after the last line that again, so that as many loads are always on their way)
+#pragma unroll
+        for (int i = 0; i < 4; i++) mma(s, fw[i], fx[i]);
+    };
+    int64_t loaded = 0;
+    // (after the last line that again, so that as many loads are always on their way)
+    const auto onwards = [&] {
+        const int64_t next = ++loaded < mine ? kFewWaves * kLine : 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) from_w[i] += next, from_x[i] += next;
+    };
+    if constexpr (Lines) {
+        using Global = __attribute__((address_space(1))) const void*;
+        using Lds = __attribute__((address_space(3))) void*;
+        const auto load = [&](char* to) {
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 __builtin_amdgcn_global_load_lds((Global)from_w[i], (Lds)(to + wave * 8192 + i * 1024), 16, 0, 0);
                 __builtin_amdgcn_global_load_lds((Global)from_x[i], (Lds)(to + wave * 8192 + 4096 + i * 1024), 16, 0, 0);
             }
-            const int64_t next = ++loaded < mine ? kFewWaves * kLine : 0;
-#pragma unroll
-            for (int i = 0; i < 4; i++) from_w[i] += next, from_x[i] += next;
+            onwards();
         };
         const auto step = [&](const char* now, char* next) {
             wait_for<63>();  // (what was read of that place is there)
             load(next);
             wait_for<8>();
-            Frag<T> fw[4], fx[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                fw[i] = *reinterpret_cast<const Frag<T>*>(now + wave * 8192 + plain_at(lane % 32, 2 * i + half));
-                fx[i] = *reinterpret_cast<const Frag<T>*>(now + wave * 8192 + 4096 + plain_at(lane % 32, 2 * i + half));
-            }
-#pragma unroll
-            for (int i = 0; i < 4; i++) mma(s, fw[i], fx[i]);
+            product(now);
         };
         if (mine > 0) {
             load(lds);
@@ -1068,26 +1074,57 @@ __global__ void __launch_bounds__(kFewWaves * 64) k_few_fwd(FewArgs a) {
             }
             wait_for<0>();
         }
-    }
-    for (int64_t k = begin + wave * kLine; k < length; k += kFewWaves * kAtOnce * kLine) {
-        Frag<T> fw[kAtOnce][4], fx[kAtOnce][4];
-        const auto load_all = [&](auto load) {
+    } else if (mine > 0) {
+        // Of rows that begin anywhere the lines go through registers, two of them on their way; of x only the rows there are, eight at
+        // a time. (What LDS holds in place of others goes into sums that nothing takes.)
+        const auto pass = [&](auto eights) {
+            constexpr int X = eights.value;
+            struct Line {
+                Frag<T> w[4], x[X];
+            } first, second;
+            const auto load = [&](Line& v) {
 #pragma unroll
-            for (int t = 0; t < kAtOnce; t++)
+                for (int i = 0; i < 4; i++) v.w[i] = load_raw<V>(from_w[i]);
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int64_t at = k + t * kFewWaves * kLine + (2 * i + half) * V;
-                    fw[t][i] = load(w, at);
-                    fx[t][i] = load(x, at);
-                }
+                for (int i = 0; i < X; i++) v.x[i] = load_raw<V>(from_x[i]);
+                onwards();
+            };
+            const auto step = [&](Line& v) {
+                char* const to = lds + wave * 8192 + lane * 16;
+                wave_sees();  // (what was there has been read)
+#pragma unroll
+                for (int i = 0; i < 4; i++) *reinterpret_cast<Frag<T>*>(to + i * 1024) = v.w[i];
+#pragma unroll
+                for (int i = 0; i < X; i++) *reinterpret_cast<Frag<T>*>(to + 4096 + i * 1024) = v.x[i];
+                load(v);
+                wave_sees();
+                product(lds);
+            };
+            load(first);
+            load(second);
+            for (int64_t t = 0;;) {
+                step(first);
+                if (++t == mine) break;
+                step(second);
+                if (++t == mine) break;
+            }
         };
-        if (k + (kAtOnce - 1) * kFewWaves * kLine + kLine <= length) load_all([&](const T* p, int64_t at) { return load_raw<V>(p + at); });
-        else if (length >= V) load_all([&](const T* p, int64_t at) { return load_clamped(p, at, length); });
-        else load_all([&](const T* p, int64_t at) { return load_within(p, at, length); });
+        const int64_t rows = part.end - part.begin;
+        if (rows <= 8) pass(std::integral_constant<int, 1>{});
+        else if (rows <= 16) pass(std::integral_constant<int, 2>{});
+        else pass(std::integral_constant<int, 4>{});
+    }
+    // what is left of the length, less than a line
+    if (const int64_t k = lines * kLine; wave == 0 && k < length) {
+        Frag<T> fw[4], fx[4];
 #pragma unroll
-        for (int t = 0; t < kAtOnce; t++)
+        for (int i = 0; i < 4; i++) {
+            const int64_t at = k + (2 * i + half) * V;
+            fw[i] = length >= V ? load_clamped(w, at, length) : load_within(w, at, length);
+            fx[i] = length >= V ? load_clamped(x, at, length) : load_within(x, at, length);
+        }
 #pragma unroll
-            for (int i = 0; i < 4; i++) mma(s, fw[t][i], fx[t][i]);
+        for (int i = 0; i < 4; i++) mma(s, fw[i], fx[i]);
     }
     float* const sums = reinterpret_cast<float*>(lds + wave * 8192);
 #pragma unroll
@@ -1451,9 +1488,9 @@ void forward(const LinearFwdArgs& f, Run& run) {
         const int64_t slots = slots_of(f.rows, f.groups, kFewShift, ragged), blocks = up(f.out, 32);
         const auto whole_lines = [](const void* p, int64_t stride) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * sizeof(T) % 16 == 0; };
         const bool whole = whole_lines(f.x, f.x_stride) && whole_lines(f.weight, f.in);
-        // Where that leaves units without work and a wave has eight lines and more (sixteen, of those that go through LDS), slices of the
-        // sums' length, of two lines a wave at least, are workgroups of their own. (24 rows of 4281 to 1967 half 41 us whole, 22 in
-        // slices; 8 rows of 4096 to 1024 bfloat16, eight lines through LDS, 7.9 and 9.5.)
+        // Where that leaves units without work and a wave has eight lines and more (sixteen, of those that go straight into LDS), slices
+        // of the sums' length, of two lines a wave at least, are workgroups of their own. (31 rows of 2274 to 906 float, nine lines, 15.5 us
+        // whole, 12.5 in slices; 8 rows of 4096 to 1024 bfloat16, eight lines straight into LDS, 7.9 and 9.5.)
         constexpr int64_t line = kFewWaves * 128 / static_cast<int>(sizeof(T));
         const int64_t lines = up(f.in, line), most = lines < (whole ? 16 : 8) ? 1 : std::min(lines / 2, 256 / std::max<int64_t>(blocks * slots, 1));
         const int64_t slice = up(lines, std::max<int64_t>(most, 1)) * line, slices = up(f.in, slice);

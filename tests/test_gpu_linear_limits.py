@@ -50,3 +50,11 @@ def test_rows_of_the_most_elements(tb, dtype, rows, n_in, n_out):  # noqa: F811
         assert torch.equal(y[:, c:c + part], (x.double() @ w[c:c + part].double().t().contiguous()).to(dtype))
         assert torch.equal(dw[c:c + part], (dy[:, c:c + part].double().t().contiguous() @ x.double()).to(dtype))
         assert torch.equal(db[c:c + part], dy[:, c:c + part].double().sum(0).to(dtype))
+
+
+# The lines of a sum are shared by eight waves, x's rows are taken eight at a time, and rows begin anywhere, between NaN.
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n_in", [31, 63, 64, 65, 255, 257, 511, 512, 513, 1025, 2111, 4099, 8321])
+def test_few_rows_off_their_lines(tb, n_in, dtype):  # noqa: F811
+    for rows, sizes in ((1, None), (8, None), (9, None), (16, None), (17, None), (32, None), (41, [8, 0, 33]), (20, [17])):
+        compare(tb, rows, n_in, 77, dtype, "gelu", add=True, pad=1 + rows % 2, off=rows % 3, sizes=sizes, seed=rows)
