@@ -44,19 +44,27 @@ constexpr int line_bytes(int tiles, int elem) { return tiles * 32 * elem + (elem
 // ---- tiles --------------------------------------------------------------------------------------------------
 
 // The tiles to choose from: their rows and columns, how many run at once on 256 units, and what a step of 128 bytes of the
-// sums' length then takes, in ns of 16-bit elements (floats: as many bytes, 4.6 times), and what a tile takes besides. Measured on layers of 16,383 rows, 8192 to
+// sums' length then takes, in ns of 16-bit elements, and what a tile takes besides. Measured on layers of 16,383 rows, 8192 to
 // 2048: 542, 623 and 712 us by tiles of 256, 128 and 64 rows; 20,001 rows in 16 groups, 1024 to 1408, whose tiles of 256 rows
 // take three rounds for two: 121, 104 and 106.
 struct TileKind {
     int rows, cols, at_once;
-    double step, fixed;
+    double step, fixed, float_step, float_fixed;
 };
-constexpr TileKind kTileKinds[] = {{256, 256, 256, 1950, 6000}, {128, 128, 512, 1150, 3000}, {64, 128, 768, 1050, 2500}};
+constexpr TileKind kTileKinds[] = {{256, 256, 256, 1950, 6000, 0, 0}, {128, 128, 512, 1150, 3000, 1860, 9000}, {64, 128, 768, 1050, 2500, 950, 5500}};
 constexpr double kJoinFixed = 4000, kJoinBytes = 4;  // ns; bytes a ns
-// `tiles` of `steps` each; a unit's only workgroup of a kind that shares it goes faster.
+// `tiles` of `steps` each; a unit's only workgroup of a kind that shares it goes faster. Floats' sums over rows, whose operands both
+// come from memory as long as they last, as 16-bit elements of 4.6 times the step: what runs side by side hides loads (300,000 rows of
+// 64 to 144, gradients 465 us; 650 by the figures below, which choose parts that fill each unit once).
 double tiles_take(const TileKind& k, double tiles, double steps, int elem) {
     const double step = k.step * (elem == 4 ? 4.6 : 1.0) * (tiles <= 256 && k.at_once > 256 ? 0.6 : 1.0);
     return std::max(1.0, std::ceil(tiles / k.at_once)) * (k.fixed + steps * step);
+}
+// The same of floats' sums over features. Their products fill a unit by one workgroup, and a second one waits for them (one of 128 rows
+// leaves a twelfth): 429 rows of 5312 to 1072 in slices of the sums, us: 36 tiles of 128 rows 330, 216 67, 288, more than units, 93,
+// 504 69 to 84; 63 tiles of 64 rows 168, 252 52, 504 54. 4096 cubed 980 and 1017.
+double float_tiles_take(const TileKind& k, double tiles, double steps) {
+    return std::max(1.0, std::ceil(tiles / 256)) * (k.float_fixed + steps * k.float_step * (k.rows == 128 && tiles <= 256 ? 1.08 : 1.0));
 }
 
 // A tile's lines in memory, those of an operand's rows, may be so many bytes apart: then what a lane adds to its load's beginning,
@@ -86,7 +94,8 @@ Plan plan_rows(int64_t rows, int64_t cols, int64_t depth, int groups, bool ragge
         for (int64_t splits = 1; splits <= 64 && (splits == 1 || steps / splits >= 2); splits *= 2) {
             const int64_t each = up(steps, splits), parts = up(steps, each), bytes = parts > 1 ? parts * rows * cols * 4 : 0;
             if (bytes > int64_t{64} << 20) break;
-            const double time = tiles_take(k, tiles * static_cast<double>(parts), static_cast<double>(each), elem) +
+            const double all = tiles * static_cast<double>(parts), length = static_cast<double>(each);
+            const double time = (elem == 4 ? float_tiles_take(k, all, length) : tiles_take(k, all, length, elem)) +
                                 (parts > 1 ? kJoinFixed + 2.0 * static_cast<double>(bytes) / kJoinBytes / 1000 : 0.0);
             if (time < least) {
                 least = time;
