@@ -49,9 +49,9 @@ constexpr int line_bytes(int tiles, int elem) { return tiles * 32 * elem + (elem
 // take three rounds for two: 121, 104 and 106.
 struct TileKind {
     int rows, cols, at_once;
-    double step, fixed, float_step, float_fixed;
+    double step, fixed, float_step;
 };
-constexpr TileKind kTileKinds[] = {{256, 256, 256, 1950, 6000, 0, 0}, {128, 128, 512, 1150, 3000, 1860, 9000}, {64, 128, 768, 1050, 2500, 950, 5500}};
+constexpr TileKind kTileKinds[] = {{256, 256, 256, 1950, 6000, 0}, {128, 128, 512, 1150, 3000, 1860}, {64, 128, 768, 1050, 2500, 950}};
 constexpr double kJoinFixed = 4000, kJoinBytes = 4;  // ns; bytes a ns
 // `tiles` of `steps` each; a unit's only workgroup of a kind that shares it goes faster. Floats' sums over rows, whose operands both
 // come from memory as long as they last, as 16-bit elements of 4.6 times the step: what runs side by side hides loads (300,000 rows of
@@ -60,11 +60,15 @@ double tiles_take(const TileKind& k, double tiles, double steps, int elem) {
     const double step = k.step * (elem == 4 ? 4.6 : 1.0) * (tiles <= 256 && k.at_once > 256 ? 0.6 : 1.0);
     return std::max(1.0, std::ceil(tiles / k.at_once)) * (k.fixed + steps * step);
 }
-// The same of floats' sums over features. Their products fill a unit by one workgroup, and a second one waits for them (one of 128 rows
-// leaves a twelfth): 429 rows of 5312 to 1072 in slices of the sums, us: 36 tiles of 128 rows 330, 216 67, 288, more than units, 93,
-// 504 69 to 84; 63 tiles of 64 rows 168, 252 52, 504 54. 4096 cubed 980 and 1017.
-double float_tiles_take(const TileKind& k, double tiles, double steps) {
-    return std::max(1.0, std::ceil(tiles / 256)) * (k.float_fixed + steps * k.float_step * (k.rows == 128 && tiles <= 256 ? 1.08 : 1.0));
+// The same of floats' sums over features, in `parts` whose sums are `bytes`. Their products fill a unit by one workgroup, and what shares
+// it waits for them (one of 128 rows leaves a twelfth); loads and stores at the ends hide behind the others' products but for those
+// that run at once. 429 rows of 5312 to 1072, us: 36 tiles of 128 rows whole 330, in 6 parts (216) 67, in 8 (288, more than units) 93;
+// 63 tiles of 64 rows whole 168, in 4 parts (252) 52, in 8 54, in 12 (756, 22 MB of sums) 57, in 16 (more than run at once) 75.
+// 4096 cubed 980 and 1017.
+double float_tiles_take(const TileKind& k, double tiles, double steps, int64_t parts, int64_t bytes) {
+    return 9000 + (std::ceil(std::max(1.0, tiles / k.at_once)) - 1) * 8000 +
+           std::max(1.0, std::ceil(tiles / 256)) * steps * k.float_step * (k.rows == 128 && tiles <= 256 ? 1.08 : 1.0) +
+           (parts > 1 ? 2000 + static_cast<double>(bytes) * 1e-4 : 0.0);
 }
 
 // A tile's lines in memory, those of an operand's rows, may be so many bytes apart: then what a lane adds to its load's beginning,
@@ -91,12 +95,12 @@ Plan plan_rows(int64_t rows, int64_t cols, int64_t depth, int groups, bool ragge
         // (a group's last tile is half full)
         const double down = ragged ? static_cast<double>(rows) / k.rows + 0.5 * static_cast<double>(std::min<int64_t>(groups, rows)) : static_cast<double>(up(rows, k.rows));
         const double tiles = down * static_cast<double>(up(cols, k.cols));
-        for (int64_t splits = 1; splits <= 64 && (splits == 1 || steps / splits >= 2); splits *= 2) {
+        for (int64_t splits = 1; splits <= 64 && (splits == 1 || steps / splits >= 2); splits += elem == 2 ? splits : splits < 16 ? 1 : 4) {
             const int64_t each = up(steps, splits), parts = up(steps, each), bytes = parts > 1 ? parts * rows * cols * 4 : 0;
             if (bytes > int64_t{64} << 20) break;
             const double all = tiles * static_cast<double>(parts), length = static_cast<double>(each);
-            const double time = (elem == 4 ? float_tiles_take(k, all, length) : tiles_take(k, all, length, elem)) +
-                                (parts > 1 ? kJoinFixed + 2.0 * static_cast<double>(bytes) / kJoinBytes / 1000 : 0.0);
+            const double time = elem == 4 ? float_tiles_take(k, all, length, parts, bytes)
+                                          : tiles_take(k, all, length, elem) + (parts > 1 ? kJoinFixed + 2.0 * static_cast<double>(bytes) / kJoinBytes / 1000 : 0.0);
             if (time < least) {
                 least = time;
                 best = {k.rows, static_cast<int>(parts), each * step, bytes};
