@@ -374,7 +374,8 @@ __device__ inline void store_unit(const Finish& a, int64_t r, int64_t stop, int6
 // way): 16,383 rows, 8192 to 2048 half with a residual 505 us, 1.09 PFLOP/s (the library's bare product 457); of 2048 to 4096 dx
 // 294 us and dweight 284 (the library 272 and 330); 20,001 rows in 16 groups, 1024 to 1408, bfloat16 90 us. Floats of 4096 cubed
 // 998 us, 138 TFLOP/s (the library 910).
-template <class T, int BR, int BC, int WR, int WC, bool RowAcross, bool ColAcross>
+// Staged: the operands lie anywhere and go through registers.
+template <class T, int BR, int BC, int WR, int WC, bool RowAcross, bool ColAcross, bool Staged>
 __global__ void __launch_bounds__(BR / WR * (BC / WC) * 64) k_tile(TileArgs a) {
     constexpr bool OverRows = RowAcross;
     constexpr int kWaves = BR / WR * (BC / WC), kThreads = kWaves * 64, kDepth = 128 / static_cast<int>(sizeof(T));
@@ -425,9 +426,6 @@ __global__ void __launch_bounds__(BR / WR * (BC / WC) * 64) k_tile(TileArgs a) {
         for (int j = 0; j < J; j++) sums[i][j] = Sums(0.0f);
     const T *const rows_from = static_cast<const T*>(a.row), *const cols_from = static_cast<const T*>(a.col) + part.group * a.col_group;
     const int64_t row_end = RowAcross ? a.row_width : r1, col_end = ColAcross ? a.col_width : a.to.cols;
-    DirectStage<T, BR, RowAcross, kThreads> rows(rows_from, a.row_stride, r0, row_end, d0);
-    DirectStage<T, BC, ColAcross, kThreads> cols(cols_from, a.col_stride, c0, col_end, d0);
-    const int64_t whole = (d1 - d0) / kDepth;
     {
         // The fragments of a step are read while the products of the step before it run, also over the end of a tile: when the
         // last step's are there the tile's place in LDS is free, and the next tile's loads, as long on their way as a tile's
@@ -445,60 +443,93 @@ __global__ void __launch_bounds__(BR / WR * (BC / WC) * 64) k_tile(TileArgs a) {
 #pragma unroll
                 for (int j = 0; j < J; j++) mma(sums[i][j], fc[of][j], fr[of][i]);
         };
-        const auto load = [&](char* to) {
-            rows.load(to);
-            cols.load(to + BR * 128);
-        };
-        constexpr int kAcrossReads = sizeof(T) == 4 ? 4 : 2, kReads = I * (RowAcross ? kAcrossReads : 1) + J * (ColAcross ? kAcrossReads : 1);
-        constexpr int kProducts = I * J * (sizeof(T) == 4 ? 4 : 1), kEach = (kReads + kProducts - 1) / kProducts;
-        const auto alternate = [&] {
+        if constexpr (Staged) {
+            // A tile's chunks are on their way while the products of the tile before it run; one barrier a tile, for the place that is
+            // written was read before the last one.
+            Stage<T, BR, RowAcross, kThreads> rows(rows_from, a.row_stride, r0, row_end);
+            Stage<T, BC, ColAcross, kThreads> cols(cols_from, a.col_stride, c0, col_end);
+            const auto load = [&](int64_t d) {
+                rows.load(d, d1);
+                cols.load(d, d1);
+            };
+            const auto step = [&](int64_t d, char* now) {
+                rows.store(now);
+                cols.store(now + BR * 128);
+                lds_barrier();
+                if (d + kDepth < d1) load(d + kDepth);
+                read(0, now, 0);
 #pragma unroll
-            for (int k = 0; k < kProducts; k++) {
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x100, kEach, 0);
+                for (int s = 0; s < 4; s++) {
+                    if (s < 3) read((s + 1) % 2, now, s + 1);
+                    product(s % 2);
+                }
+            };
+            if (d0 < d1) load(d0);
+            for (int64_t d = d0; d < d1;) {
+                step(d, lds);
+                if ((d += kDepth) >= d1) break;
+                step(d, lds1);
+                d += kDepth;
             }
-        };
-        const auto step = [&](int64_t t, char* now, const char* next) {
+        } else {
+            DirectStage<T, BR, RowAcross, kThreads> rows(rows_from, a.row_stride, r0, row_end, d0);
+            DirectStage<T, BC, ColAcross, kThreads> cols(cols_from, a.col_stride, c0, col_end, d0);
+            const int64_t whole = (d1 - d0) / kDepth;
+            const auto load = [&](char* to) {
+                rows.load(to);
+                cols.load(to + BR * 128);
+            };
+            constexpr int kAcrossReads = sizeof(T) == 4 ? 4 : 2, kReads = I * (RowAcross ? kAcrossReads : 1) + J * (ColAcross ? kAcrossReads : 1);
+            constexpr int kProducts = I * J * (sizeof(T) == 4 ? 4 : 1), kEach = (kReads + kProducts - 1) / kProducts;
+            const auto alternate = [&] {
 #pragma unroll
-            for (int s = 0; s < 3; s++) {
-                read((s + 1) % 2, now, s + 1);
-                product(s % 2);
+                for (int k = 0; k < kProducts; k++) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x100, kEach, 0);
+                }
+            };
+            const auto step = [&](int64_t t, char* now, const char* next) {
+#pragma unroll
+                for (int s = 0; s < 3; s++) {
+                    read((s + 1) % 2, now, s + 1);
+                    product(s % 2);
+                    alternate();
+                }
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                __syncthreads();
+                if (t + 2 < whole) load(now);
+                read(0, next, 0);  // (after the last tile of what is there, for nothing)
+                product(1);
                 alternate();
+            };
+            if (whole) {
+                load(lds);
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                __syncthreads();
+                if (whole > 1) load(lds1);
+                read(0, lds, 0);
+                for (int64_t t = 0;;) {
+                    step(t, lds, lds1);
+                    if (++t == whole) break;
+                    step(t, lds1, lds);
+                    if (++t == whole) break;
+                }
             }
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-            __syncthreads();
-            if (t + 2 < whole) load(now);
-            read(0, next, 0);  // (after the last tile of what is there, for nothing)
-            product(1);
-            alternate();
-        };
-        if (whole) {
-            load(lds);
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads();
-            if (whole > 1) load(lds1);
-            read(0, lds, 0);
-            for (int64_t t = 0;;) {
-                step(t, lds, lds1);
-                if (++t == whole) break;
-                step(t, lds1, lds);
-                if (++t == whole) break;
-            }
-        }
-        if (d0 + whole * kDepth < d1) {
-            Stage<T, BR, RowAcross, kThreads> row(rows_from, a.row_stride, r0, row_end);
-            Stage<T, BC, ColAcross, kThreads> col(cols_from, a.col_stride, c0, col_end);
-            row.load(d0 + whole * kDepth, d1);
-            col.load(d0 + whole * kDepth, d1);
-            __syncthreads();
-            row.store(lds);
-            col.store(lds + BR * 128);
-            __syncthreads();
-            read(0, lds, 0);
+            if (d0 + whole * kDepth < d1) {
+                Stage<T, BR, RowAcross, kThreads> row(rows_from, a.row_stride, r0, row_end);
+                Stage<T, BC, ColAcross, kThreads> col(cols_from, a.col_stride, c0, col_end);
+                row.load(d0 + whole * kDepth, d1);
+                col.load(d0 + whole * kDepth, d1);
+                __syncthreads();
+                row.store(lds);
+                col.store(lds + BR * 128);
+                __syncthreads();
+                read(0, lds, 0);
 #pragma unroll
-            for (int s = 0; s < 4; s++) {
-                if (s < 3) read((s + 1) % 2, lds, s + 1);
-                product(s % 2);
+                for (int s = 0; s < 4; s++) {
+                    if (s < 3) read((s + 1) % 2, lds, s + 1);
+                    product(s % 2);
+                }
             }
         }
         __syncthreads();
@@ -1377,17 +1408,20 @@ void launch_slope(const SlopeArgs& a, const Slope& p, hipStream_t s) {
 }
 
 // A product's operand as k_tile reads it: lines that begin on 16 bytes, their places in a tile in 32 bits, and across them whole
-// fragments. What lies otherwise is copied first, which takes two passes over it where loads of its own kind took the product
-// three times as long (377 rows of 5996 to 1162 bfloat16, the gradients 98 us, with the copies 66).
+// fragments. What lies otherwise is copied first, which takes two passes over it where loads of its own kind took the product three
+// times as long (377 rows of 5996 to 1162 bfloat16, the gradients 98 us, with the copies 66; but see staged_pays).
 struct Operand {
     const void* p;
     int64_t stride, width;
 };
 template <class T>
+bool lies_for_tiles(const void* p, int64_t width, int64_t stride, bool across) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * static_cast<int64_t>(sizeof(T)) % 16 == 0 &&
+           stride <= kMostLine / static_cast<int>(sizeof(T)) && (!across || width % kPer<T> == 0);
+}
+template <class T>
 Operand operand(const void* p, int64_t rows, int64_t width, int64_t stride, bool across, Run& run) {
-    const bool fits = reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * static_cast<int64_t>(sizeof(T)) % 16 == 0 &&
-                      stride <= kMostLine / static_cast<int>(sizeof(T)) && (!across || width % kPer<T> == 0);
-    if (fits || !rows) return {p, stride, width};
+    if (lies_for_tiles<T>(p, width, stride, across) || !rows) return {p, stride, width};
     const Slope plan = plan_slope(rows, width, 1, false, sizeof(T));
     SlopeArgs a{};
     a.dy = p; a.dy_stride = stride; a.dz = run.work.take(plan.dz_bytes); a.dz_stride = plan.dz_stride;
@@ -1397,17 +1431,24 @@ Operand operand(const void* p, int64_t rows, int64_t width, int64_t stride, bool
 }
 
 template <class T, bool RowAcross, bool ColAcross>
-void launch_tiles(const TileArgs& a, int side, int64_t slabs, hipStream_t s) {
+void launch_tiles(const TileArgs& a, int side, int64_t slabs, bool staged, hipStream_t s) {
     const int64_t down = RowAcross ? up(a.rows, side) : a.slots, tiles = up(down * up(a.to.cols, side == 256 ? 256 : 128), 8) * 8;
     check_grid(tiles * slabs, side == 256 ? 512 : 256);
     const dim3 grid(static_cast<uint32_t>(tiles), static_cast<uint32_t>(slabs));
-    if constexpr (sizeof(T) == 2)
+    if constexpr (sizeof(T) == 2) {
         if (side == 256) {
-            k_tile<T, 256, 256, 128, 64, RowAcross, ColAcross><<<grid, 512, 0, s>>>(a);
+            k_tile<T, 256, 256, 128, 64, RowAcross, ColAcross, false><<<grid, 512, 0, s>>>(a);
             return;
         }
-    if (side == 128) k_tile<T, 128, 128, 64, 64, RowAcross, ColAcross><<<grid, 256, 0, s>>>(a);
-    else k_tile<T, 64, 128, 32, 64, RowAcross, ColAcross><<<grid, 256, 0, s>>>(a);
+    } else if constexpr (!RowAcross && !ColAcross) {
+        if (staged) {
+            if (side == 128) k_tile<T, 128, 128, 64, 64, false, false, true><<<grid, 256, 0, s>>>(a);
+            else k_tile<T, 64, 128, 32, 64, false, false, true><<<grid, 256, 0, s>>>(a);
+            return;
+        }
+    }
+    if (side == 128) k_tile<T, 128, 128, 64, 64, RowAcross, ColAcross, false><<<grid, 256, 0, s>>>(a);
+    else k_tile<T, 64, 128, 32, 64, RowAcross, ColAcross, false><<<grid, 256, 0, s>>>(a);
 }
 
 // `slabs`: of a group, on average
@@ -1463,7 +1504,7 @@ void join_splits(const TileArgs& a, hipStream_t s) {
 
 // out = row col^T over the groups' rows (see TileArgs), with what follows.
 template <class T, bool ColAcross>
-void over_depth(TileArgs a, bool ragged, Run& run) {
+void over_depth(TileArgs a, bool ragged, bool staged, Run& run) {
     const Plan p = plan_rows(a.rows, a.to.cols, a.depth, a.groups.groups, ragged, sizeof(T));
     a.shift = log2_up(p.side);
     a.slots = slots_of(a.rows, a.groups.groups, a.shift, ragged);
@@ -1471,7 +1512,7 @@ void over_depth(TileArgs a, bool ragged, Run& run) {
     a.splits = p.splits;
     a.partial = p.splits > 1 ? reinterpret_cast<float*>(run.work.take(p.bytes)) : nullptr;
     if (!run.real) return;
-    launch_tiles<T, false, ColAcross>(a, p.side, p.splits, run.stream);
+    launch_tiles<T, false, ColAcross>(a, p.side, p.splits, staged, run.stream);
     if (a.partial) join_splits<T>(a, run.stream);
 }
 
@@ -1484,10 +1525,10 @@ void forward(const LinearFwdArgs& f, Run& run) {
         if (run.real) launch_narrow<T>({f.x, f.weight, f.bias, f.x_stride, to, f.in, f.out, p.chunk, groups}, p, run.stream);
         return;
     }
-    if (few_rows(f.rows, f.out, f.groups)) {
+    const auto whole_lines = [](const void* p, int64_t stride) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * sizeof(T) % 16 == 0; };
+    const bool whole = whole_lines(f.x, f.x_stride) && whole_lines(f.weight, f.in);
+    if (few_rows(f.rows, f.out, f.groups, sizeof(T), whole)) {
         const int64_t slots = slots_of(f.rows, f.groups, kFewShift, ragged), blocks = up(f.out, 32);
-        const auto whole_lines = [](const void* p, int64_t stride) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * sizeof(T) % 16 == 0; };
-        const bool whole = whole_lines(f.x, f.x_stride) && whole_lines(f.weight, f.in);
         // Where that leaves units without work and a wave has eight lines and more (sixteen, of those that go straight into LDS), slices
         // of the sums' length, of two lines a wave at least, are workgroups of their own. (31 rows of 2274 to 906 float, nine lines, 15.5 us
         // whole, 12.5 in slices; 8 rows of 4096 to 1024 bfloat16, eight lines straight into LDS, 7.9 and 9.5.)
@@ -1506,12 +1547,14 @@ void forward(const LinearFwdArgs& f, Run& run) {
         if (slices > 1) join_splits<T>(t, run.stream);
         return;
     }
-    const Operand x = operand<T>(f.x, f.rows, f.in, f.x_stride, false, run);
-    const Operand w = operand<T>(f.weight, f.groups * f.out, f.in, f.in, false, run);
+    const bool x_lies = lies_for_tiles<T>(f.x, f.in, f.x_stride, false), w_lies = lies_for_tiles<T>(f.weight, f.in, f.in, false);
+    const bool staged = sizeof(T) == 4 && staged_pays(f.rows, f.in, f.out, f.groups, !x_lies, !w_lies);
+    const Operand x = staged ? Operand{f.x, f.x_stride, f.in} : operand<T>(f.x, f.rows, f.in, f.x_stride, false, run);
+    const Operand w = staged ? Operand{f.weight, f.in, f.in} : operand<T>(f.weight, f.groups * f.out, f.in, f.in, false, run);
     TileArgs a{};
     a.row = x.p; a.row_stride = x.stride; a.col = w.p; a.col_stride = w.stride; a.col_group = w.stride * f.out;
     a.rows = f.rows; a.depth = f.in; a.groups = groups; a.bias = f.bias; a.bias_group = f.out; a.to = to;
-    over_depth<T, false>(a, ragged, run);
+    over_depth<T, false>(a, ragged, staged, run);
 }
 
 template <class T>
@@ -1603,7 +1646,7 @@ void backward(const LinearBwdArgs& f, Run& run) {
         a.row = dz.p; a.row_stride = dz.stride; a.col = w.p; a.col_stride = w.stride; a.col_group = w.stride * f.out; a.col_width = w.width;
         a.to.out = f.dx; a.to.out_stride = f.dx_stride; a.to.cols = f.in; a.to.clear = f.clear;
         a.rows = f.rows; a.depth = f.out; a.groups = groups;
-        over_depth<T, true>(a, ragged, run);
+        over_depth<T, true>(a, ragged, false, run);
         run.work.back_to(kept);
     }
     if (f.dweight) {
@@ -1615,7 +1658,7 @@ void backward(const LinearBwdArgs& f, Run& run) {
         a.groups = groups; a.shift = p.shift; a.slots = p.slots;
         a.partial = p.bytes ? reinterpret_cast<float*>(run.work.take(p.bytes)) : nullptr;
         if (!run.real) return;
-        launch_tiles<T, true, true>(a, p.side, p.slots, run.stream);
+        launch_tiles<T, true, true>(a, p.side, p.slots, false, run.stream);
         if (a.partial) {
             JoinArgs j{};
             j.partial = a.partial; j.dweight = f.dweight; j.weights = j.wanted = j.size = f.in * f.out;

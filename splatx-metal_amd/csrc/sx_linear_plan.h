@@ -109,6 +109,15 @@ Plan plan_rows(int64_t rows, int64_t cols, int64_t depth, int groups, bool ragge
     }
     return best;
 }
+// Whether a forward of floats reads operands that do not lie for its tiles through registers rather than copy them first: the copies
+// take two passes over them and a launch each, the registers a fifth of what the products take. (us so and with copies: 81 rows of
+// 1835 to 7894 53 and 69, 44 of 6309 to 2451 45 and 66, 16,384 of 513 to 512 93 and 100; 4097 cubed 1294 and 1220. A backward's tiles,
+// which read across the rows, took half as long again.)
+bool staged_pays(int64_t rows, int64_t in, int64_t out, int groups, bool copy_x, bool copy_w) {
+    const double passes = 2.0 * 4 * static_cast<double>(in) * (copy_x * static_cast<double>(rows) + copy_w * static_cast<double>(groups) * static_cast<double>(out));
+    const double copies = passes / 4500 + 4000 * (copy_x + copy_w), products = 2.0 * static_cast<double>(rows) * static_cast<double>(in) * static_cast<double>(out) / 140'000;
+    return copies > 0.2 * products;
+}
 // out[groups][out][in] over the groups' rows: the tile's rows, and the parts of the rows (shift 62: each group's are one).
 struct Over {
     int side, shift;
@@ -233,9 +242,12 @@ NarrowBwd plan_narrow_bwd(int64_t rows, int64_t in, int64_t out, int groups, boo
 
 // ---- few rows -----------------------------------------------------------------------------------------------
 
-// Whether a forward's groups have so few rows that the weights' bytes are what it takes (and its workgroups fit a launch).
-bool few_rows(int64_t rows, int64_t out, int groups) {
-    return (rows <= 32 || rows / groups <= 16) && up(out, 32) * (groups + 1 + (rows >> kFewShift)) < int64_t{1} << 22;
+// Whether a forward's groups have so few rows that the weights' bytes are what it takes (and its workgroups fit a launch). Of floats,
+// whose tiles are slower next to their bytes, more, and more again where their lines would have to be copied (us here and by tiles:
+// 64 rows of 4096 to 4096 25.5 and 27.0, of 4097 25.7 and 34.2; 96 of 4096 45.4 and 41.7, of 4097 46.6 and 55.9; 81 of 1835 to 7894
+// 46.0 and 53.4).
+bool few_rows(int64_t rows, int64_t out, int groups, int elem, bool whole_lines) {
+    return (rows <= (elem == 2 ? 32 : whole_lines ? 64 : 128) || rows / groups <= 16) && up(out, 32) * (groups + 1 + (rows >> kFewShift)) < int64_t{1} << 22;
 }
 // Whether a backward's rows are.
 bool few_rows_backward(int64_t rows, int64_t in, int64_t out, int groups, int elem) {

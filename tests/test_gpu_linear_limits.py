@@ -58,3 +58,11 @@ def test_rows_of_the_most_elements(tb, dtype, rows, n_in, n_out):  # noqa: F811
 def test_few_rows_off_their_lines(tb, n_in, dtype):  # noqa: F811
     for rows, sizes in ((1, None), (8, None), (9, None), (16, None), (17, None), (32, None), (41, [8, 0, 33]), (20, [17])):
         compare(tb, rows, n_in, 77, dtype, "gelu", add=True, pad=1 + rows % 2, off=rows % 3, sizes=sizes, seed=rows)
+
+
+# Floats between few rows and many, in lines off 16 bytes and on them: 33 to 128 rows by the few rows' kernel, more by tiles through registers.
+@pytest.mark.parametrize("n_in,n_out", [(31, 600), (33, 1000), (64, 300), (127, 700), (257, 513), (1025, 200), (2047, 129)])
+@pytest.mark.parametrize("rows,sizes", [(33, None), (64, None), (65, None), (128, None), (129, None), (515, None), (600, [100, 0, 65, 400]), (100, [64, 36])])
+def test_floats_off_their_lines(tb, rows, sizes, n_in, n_out):  # noqa: F811
+    for pad, off in ((0, 0), (1, 1), (4, 0), (3, 2)):
+        compare(tb, rows, n_in, n_out, F32, "silu", add=True, pad=pad, off=off, sizes=sizes, seed=rows)

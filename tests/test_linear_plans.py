@@ -35,5 +35,5 @@ def test_the_widest_rows_are_not_copied(t, size):
     wide, rows, n = 1 << 24, 200, 128
     assert f(C.byref(st.LinearInputs(at, at, None, None, None, rows, wide, n, 0, wide, 0, t, 0, 0))) <= 64 << 20
     assert g(C.byref(st.LinearGradsIn(at, None, at, at, None, rows, wide, n, 0, n, 0, wide, t, 0, 0))) <= 64 << 20
-    # rows further apart than that are
-    assert f(C.byref(st.LinearInputs(at, at, None, None, None, rows, 1024, n, 0, 1 << 25, 0, t, 0, 0))) >= rows * 1024 * size
+    # rows of 16 bits further apart than that are (floats are read where they lie)
+    assert t == 0 or f(C.byref(st.LinearInputs(at, at, None, None, None, rows, 1024, n, 0, 1 << 25, 0, t, 0, 0))) >= rows * 1024 * size
