@@ -787,6 +787,99 @@ __global__ void __launch_bounds__(512) k_narrow_fwd(NarrowArgs a) {
     }
 }
 
+// Longer rows of floats, up to Tiles times 32 outputs: a row's fragments do not fit a lane's registers, and 16 bytes of each of 32 rows
+// a load would have the rows read in pieces. A wave takes 32 rows as whole lines, 128 bytes of each at a time, through registers
+// (two of them on their way) and LDS of its own, which its outputs take afterwards. Bound by the rows' bytes, as far as sixteen waves
+// a unit keep on their way: 1,129,273 rows of 192 to 32 234 us (4.3 TB/s).
+template <class T, int Tiles>
+__global__ void __launch_bounds__(512) k_long_fwd(NarrowArgs a, int lines) {
+    static_assert(kUnitTiles<T> == 1 && kUnitBytes<T> >= 4096);
+    constexpr int V = kPer<T>, kLine = 128 / static_cast<int>(sizeof(T));
+    extern __shared__ __attribute__((aligned(128))) char lds[];
+    const int lane = threadIdx.x % 64, half = lane / 32, wave = wave_of(), rows_at_once = blockDim.x / 2, steps = lines * 4;
+    Frag<T>* const weights = reinterpret_cast<Frag<T>*>(lds);
+    float* const bias = reinterpret_cast<float*>(lds + Tiles * steps * 1024);
+    char* const mine = lds + Tiles * (steps * 1024 + 128) + wave * kUnitBytes<T>;
+    const T* const x = static_cast<const T*>(a.x);
+    const bool grouped = a.groups.ends;
+    const int64_t last = grouped ? min(a.groups.rows, (blockIdx.x + int64_t{1}) * a.chunk) : a.groups.rows;
+    const int64_t stride = grouped ? rows_at_once : int64_t{gridDim.x} * rows_at_once;
+    int chunk[4];  // the lane's, of a line of row i * 8 + lane / 8
+#pragma unroll
+    for (int i = 0; i < 4; i++) chunk[i] = (plain_at(i * 8 + lane / 8, lane % 8) - (i * 8 + lane / 8) * 128) / 16 * V;
+    for (int64_t first = blockIdx.x * (grouped ? a.chunk : rows_at_once); first < last;) {
+        const int group = group_of(a.groups, first);
+        if (group >= a.groups.groups) {
+            for (int64_t r = first + threadIdx.x / 8; r < last; r += blockDim.x / 8)
+                for (int64_t c = threadIdx.x % 8 * 4; c < a.out; c += 32) clear4<T>(a.to, r, c);
+            return;
+        }
+        const int64_t stop = max(first + 1, min(last, a.groups.end(group)));  // (a row at least, whatever the ends are)
+        const T* const w = static_cast<const T*>(a.weight) + group * a.in * a.out;
+        struct Line {
+            Frag<T> v[4];
+        } even, odd;
+        // what is loaded next, and what is worked on
+        int64_t ahead = first + wave * 32, base = ahead;
+        int line_ahead = 0, line = 0;
+        const auto load = [&](Line& to) {
+            if (ahead >= stop) return;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const T* const row = x + min(ahead + i * 8 + lane / 8, stop - 1) * a.x_stride;
+                const int at = line_ahead * kLine + chunk[i];
+                to.v[i] = line_ahead + 1 < lines ? load_raw<V>(row + at) : load_clamped(row, at, a.in);
+            }
+            if (++line_ahead == lines) line_ahead = 0, ahead += stride;
+        };
+        load(even);
+        load(odd);
+        lds_barrier();  // the group's before have been worked on
+        for (int i = threadIdx.x; i < Tiles * steps * 64; i += blockDim.x) {
+            const int n = i / 64 / steps * 32 + i % 32, k = (2 * (i / 64 % steps) + i % 64 / 32) * V;
+            const Frag<T> f = load_clamped(w + min(int64_t{n}, a.out - 1) * a.in, k, a.in);
+            weights[i] = n < a.out ? f : Frag<T>(0);
+        }
+        for (int i = threadIdx.x; i < Tiles * 32; i += blockDim.x)
+            bias[i] = a.bias && i < a.out ? static_cast<float>(static_cast<const T*>(a.bias)[group * a.out + i]) : 0.0f;
+        lds_barrier();
+        Sums sums[Tiles];
+        const auto step = [&](Line& v) {
+            if (line == 0)
+#pragma unroll
+                for (int t = 0; t < Tiles; t++)
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        const Floats<4> b = *reinterpret_cast<const Floats<4>*>(bias + t * 32 + 8 * q + half * 4);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) sums[t][4 * q + e] = b[e];
+                    }
+            wave_sees();  // (what was there has been read)
+#pragma unroll
+            for (int i = 0; i < 4; i++) *reinterpret_cast<Frag<T>*>(mine + i * 1024 + lane * 16) = v.v[i];
+            load(v);
+            wave_sees();
+#pragma unroll
+            for (int s = 0; s < 4; s++) {
+                const Frag<T> row = *reinterpret_cast<const Frag<T>*>(mine + plain_at(lane % 32, 2 * s + half));
+#pragma unroll
+                for (int t = 0; t < Tiles; t++) mma(sums[t], weights[(t * steps + line * 4 + s) * 64 + lane], row);
+            }
+            if (++line < lines) return;
+#pragma unroll
+            for (int t = 0; t < Tiles; t++) Unit<T>(a.to, base, stop, t * 32).finish({sums[t]}, mine);
+            line = 0;
+            base += stride;
+        };
+        while (base < stop) {
+            step(even);
+            if (base >= stop) break;
+            step(odd);
+        }
+        first = stop;
+    }
+}
+
 struct NarrowBwdArgs {
     const void *dy, *pre, *x, *weight;  // x: null where dweight is not wanted
     int64_t dy_stride, pre_stride, x_stride;
@@ -1525,6 +1618,13 @@ void forward(const LinearFwdArgs& f, Run& run) {
         if (run.real) launch_narrow<T>({f.x, f.weight, f.bias, f.x_stride, to, f.in, f.out, p.chunk, groups}, p, run.stream);
         return;
     }
+    if constexpr (sizeof(T) == 4)
+        if (const Long p = plan_long(f.rows, f.in, f.out, f.groups, ragged); p.blocks) {
+            const NarrowArgs a{f.x, f.weight, f.bias, f.x_stride, to, f.in, f.out, p.chunk, groups};
+            const auto go = [&](auto kernel) { kernel<<<static_cast<uint32_t>(p.blocks), 512, p.lds, run.stream>>>(a, p.lines); };
+            if (run.real) p.tiles == 1 ? go(k_long_fwd<T, 1>) : go(k_long_fwd<T, 2>);
+            return;
+        }
     const auto whole_lines = [](const void* p, int64_t stride) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * sizeof(T) % 16 == 0; };
     const bool whole = whole_lines(f.x, f.x_stride) && whole_lines(f.weight, f.in);
     if (few_rows(f.rows, f.out, f.groups, sizeof(T), whole)) {

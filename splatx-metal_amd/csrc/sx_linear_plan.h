@@ -203,6 +203,26 @@ Narrow plan_narrow(int64_t rows, int64_t in, int64_t out, bool ragged, int elem)
     p.blocks = std::max<int64_t>(up(rows, p.chunk), 1);
     return p;
 }
+// A layer of floats with longer rows than those (`lines` of 128 bytes, the last may end early) and up to two tiles of 32 outputs, whose
+// weight a workgroup of eight waves holds: or none. Each workgroup fetches the weight, and again for each group: it pays for many
+// rows, a thousand of each group. (us so and by tiles: 158,303 rows of 178 to 2 43 and 138, 1 M of 192 to 64 301 and 570, 32,768 24.8
+// and 24.8, 16,384 24 and 13; 300,000 in 200 groups of 200 to 32 119 and 192, 100,000 of 300 to 64 155 and 112.)
+struct Long {
+    int lines, tiles, lds;
+    int64_t blocks, chunk;
+};
+Long plan_long(int64_t rows, int64_t in, int64_t out, int groups, bool ragged) {
+    Long p{};
+    const int64_t lines = up(in, 32), tiles = up(out, 32), lds = tiles * (lines * 4096 + 128) + 8 * unit_bytes(4);
+    if (narrow_steps(in, 4) || tiles > 2 || lds > kLds || rows < 32768 || rows / groups < 1024) return p;
+    p.lines = static_cast<int>(lines);
+    p.tiles = static_cast<int>(tiles);
+    p.lds = static_cast<int>(lds);
+    p.blocks = std::min<int64_t>(256 * (ragged ? 8 : std::min(2, kLds / p.lds)), up(rows, 256));
+    p.chunk = up(up(rows, p.blocks), 32) * 32;
+    p.blocks = up(rows, p.chunk);
+    return p;
+}
 // A backward whose blocks of rows a workgroup holds.
 struct NarrowBwd {
     int waves, zt, xt, lds;

@@ -29,6 +29,22 @@ void narrow() {
                     }
 }
 
+void long_rows() {
+    for (int in = 1; in <= 1200; in++)
+        for (int out = 1; out <= 100; out++)
+            for (const long rows : {1L, 4095L, 32767L, 32768L, 100'001L, 40'000'000L})
+                for (const bool ragged : {false, true}) {
+                    const Long p = plan_long(rows, in, out, ragged ? 3 : 1, ragged);
+                    if (!p.blocks) continue;
+                    looked++;
+                    // the weight's fragments, the bias, eight waves' lines and outputs
+                    const long lds = p.tiles * (p.lines * 4096L + 128) + 8 * unit_bytes(4);
+                    if (p.lds != lds || lds > kMostLds || p.lines * 32 < in || (p.lines - 1) * 32 >= in || p.tiles * 32 < out || p.tiles > 2 || in < 4 ||
+                        p.blocks > 65535 || p.chunk < 32 || p.chunk % 32 || (ragged ? p.blocks * p.chunk < rows : (p.blocks - 1) * 256 >= rows))
+                        std::printf("long %ld rows, %d to %d, ragged %d: lds %d\n", rows, in, out, ragged, p.lds);
+                }
+}
+
 void narrow_backward() {
     for (const int elem : {2, 4})
         for (int in = 1; in <= 300; in++)
@@ -66,6 +82,7 @@ void offsets() {
 int main() {
     offsets();
     narrow();
+    long_rows();
     narrow_backward();
     std::printf("looked at %ld\n", looked);
 }

@@ -66,3 +66,47 @@ def test_few_rows_off_their_lines(tb, n_in, dtype):  # noqa: F811
 def test_floats_off_their_lines(tb, rows, sizes, n_in, n_out):  # noqa: F811
     for pad, off in ((0, 0), (1, 1), (4, 0), (3, 2)):
         compare(tb, rows, n_in, n_out, F32, "silu", add=True, pad=pad, off=off, sizes=sizes, seed=rows)
+
+
+# Floats: rows of several lines, the last of any length, and one or two tiles of outputs.
+@pytest.mark.parametrize("n_in,n_out", [(129, 1), (130, 33), (131, 64), (160, 32), (178, 2), (193, 31), (257, 5), (283, 4), (300, 64), (512, 32), (601, 17), (990, 3),
+                                        (496, 64), (497, 64)])
+@pytest.mark.parametrize("rows,sizes", [(32_768, None), (32_801, None), (70_001, None), (40_000, [1000, 0, 3, 30_100, 1, 33, 300]), (33_000, [31, 32, 33, 0, 0, 1, 1, 32_000])])
+def test_long_rows_of_floats(tb, rows, sizes, n_in, n_out):  # noqa: F811
+    compare(tb, rows, n_in, n_out, F32, "gelu", bias=n_in % 2 == 0, add=n_out % 2 == 0, pad=n_out % 3, off=n_in % 2, sizes=sizes, seed=n_in)
+
+
+@pytest.mark.parametrize("dtype,rows,n_in,n_out,sizes", [(F32, 33_000, 201, 5, None), (F32, 35_000, 161, 40, [20_000, 0, 14_000]), (BF16, 70_000, 64, 768, None),
+                                                         (F16, 9, 2049, 300, None), (F32, 100, 515, 333, None), (F32, 300, 1001, 333, None)])
+def test_captured_and_on_two_streams(tb, dtype, rows, n_in, n_out, sizes):  # noqa: F811
+    """A graph of both passes, replayed with new inputs in place between other work, and the same on two streams at once."""
+    lead, ends = ((len(sizes),), torch.cumsum(torch.tensor(sizes), 0).cuda()) if sizes else ((), None)
+    x, dy, w, b = randn(rows, n_in, seed=1, dtype=dtype), randn(rows, n_out, seed=2, dtype=dtype), randn(*lead, n_out, n_in, seed=3, dtype=dtype), randn(*lead, n_out, seed=4, dtype=dtype)
+
+    def work():
+        if ends is None:
+            y, pre = tb.linear_fwd(x, w, b, "gelu", dy, True)
+            return (y, pre, *tb.linear_bwd(dy, x, w, pre, "gelu"))
+        y, pre = tb.grouped_linear_fwd(x, w, ends, b, "gelu", dy, True)
+        return (y, pre, *tb.grouped_linear_bwd(dy, x, w, ends, pre, "gelu"))
+
+    want = work()
+    streams, outs = [torch.cuda.Stream() for _ in range(2)], []
+    torch.cuda.synchronize()
+    for s in streams * 3:
+        with torch.cuda.stream(s):
+            outs.append(work())
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, e) for o in outs for a, e in zip(o, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = work()
+    for k in range(3):
+        x.copy_(randn(rows, n_in, seed=30 + k, dtype=dtype))
+        if sizes:
+            ends[:2] += k  # (the second group has no rows: they go on ascending)
+        want = [t.clone() for t in work()]
+        torch.cuda.synchronize()
+        graph.replay()
+        assert all(torch.equal(a, e) for a, e in zip(out, want)), k
+        (torch.randn(1000, device="cuda") ** 2).sum().item()

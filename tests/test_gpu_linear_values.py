@@ -20,7 +20,8 @@ def alike(got, want, what):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows,n_in,n_out,sizes", [
     (3, 700, 333, None), (20, 1856, 37, None), (32, 300, 1000, None), (5, 1000, 17, None), (4, 9001, 301, None), (7, 515, 259, [2, 0, 4]), (60, 704, 323, [20, 36]),
-    (40, 8, 8, None), (5000, 64, 64, None), (5000, 45, 33, [2000, 0, 2500]), (300, 520, 300, None), (700, 515, 333, [300, 0, 400]), (9000, 33, 130, None)])
+    (40, 8, 8, None), (5000, 64, 64, None), (5000, 45, 33, [2000, 0, 2500]), (300, 520, 300, None), (700, 515, 333, [300, 0, 400]), (9000, 33, 130, None), (33_000, 201, 5, None), (35_000, 161, 40, [20_000, 0, 14_000]),
+    (70_000, 40, 1200, None), (100, 515, 333, None)])
 def test_infinities_are_the_definitions(tb, rows, n_in, n_out, sizes, dtype):  # noqa: F811
     print(rows, n_in, n_out, sizes, dtype, flush=True)
     lead, ends = ((len(sizes),), torch.cumsum(torch.tensor(sizes), 0).cuda()) if sizes else ((), None)
