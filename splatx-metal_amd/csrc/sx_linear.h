@@ -948,12 +948,18 @@ struct BlockPart {
 };
 
 // d as two terms of the type: the first is rounded from a little less than d, so that the second has d's sign and is not zero
-// where d is not (a product with an infinite x or weight then stays infinite in their sum; of half below 2^-14 the second term may
-// vanish). Of what is not finite both are that.
+// where d is not (a product with an infinite x or weight then stays infinite in their sum). Of half below 2^-14, where all values are
+// 2^-24 apart, from half of d; only within 1.5 of those steps of 0 a term may vanish. Of what is not finite both are that.
 template <class T>
 __device__ inline void two_terms(Floats<8> d, char* first, char* second) {
-    constexpr float kLess = std::is_same_v<T, _Float16> ? 1.0f - 1.0f / 512 : 1.0f - 1.0f / 64;
-    const Frag<T> high = raw<T, 8>(d * kLess);
+    constexpr bool kHalf = std::is_same_v<T, _Float16>;
+    constexpr float kLess = kHalf ? 1.0f - 1.0f / 512 : 1.0f - 1.0f / 64;
+    Floats<8> less = d * kLess;
+    if constexpr (kHalf)
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            if (__builtin_fabsf(d[e]) < 0x1p-14f) less[e] = d[e] * 0.5f;
+    const Frag<T> high = raw<T, 8>(less);
     const Floats<8> h = floats<T, 8>(high);
     Floats<8> low = d - h;
 #pragma unroll
