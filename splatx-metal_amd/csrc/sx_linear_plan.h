@@ -232,9 +232,11 @@ struct NarrowBwd {
 NarrowBwd plan_narrow_bwd(int64_t rows, int64_t in, int64_t out, int groups, bool curved, int elem) {
     NarrowBwd p{};
     const int64_t kt = up(in, 32);
-    // dz is rounded to the type for its products, by which dx and dweight lose about what their own rounding takes. Where one of
-    // them has few elements chance may make that more, and the products are little next to the bytes: there dz is two terms
-    // (600,000 rows, 20 to 30, bfloat16: 76 us in one, 84 in two; 11 rows of 26 to 62: dx's error in one 1.5 times its own rounding's).
+    // dz is rounded to the type for its products, by which dx and dweight lose about what their own rounding takes, element for
+    // element: of all together 1.4 times the error of floats' products. Of a gradient of few elements that sum of errors varies, and
+    // may be more of the whole (11 rows of 26 to 62: dx's 1.5 times its own rounding's): under 1024 elements dz is two terms, where the
+    // kernel holds those. (600,000 rows, 20 to 30, bfloat16: 76 us in one, 84 in two; 1 M of 64 to 64 125 and 224, for two terms
+    // leave a unit one workgroup. Wider layers with such a gradient and more than 32 rows, 100 rows of 3 to 300, take one term.)
     // (dy itself, and what relu leaves of it, has no more digits than the type.)
     const bool wanted = elem == 2 && curved && std::min(in * out, rows * in) < 1024;
     p.fine = wanted && (out <= 32 || (out <= 64 && kt <= 4) || (out <= 128 && kt <= 2));
