@@ -110,3 +110,27 @@ def test_captured_and_on_two_streams(tb, dtype, rows, n_in, n_out, sizes):  # no
         graph.replay()
         assert all(torch.equal(a, e) for a, e in zip(out, want)), k
         (torch.randn(1000, device="cuda") ** 2).sum().item()
+
+
+@pytest.mark.parametrize("dtype,rows,n_in,n_out,groups", [(F32, 40_000, 16, 16, 32768), (BF16, 50_000, 40, 24, 32768), (F16, 20_000, 200, 33, 32768), (F32, 9_000, 70, 33, 4000),
+                                                          (BF16, 100, 8, 8, 32768), (F32, 60_000, 130, 20, 1000)])
+def test_the_most_groups(tb, dtype, rows, n_in, n_out, groups):  # noqa: F811
+    """Whole numbers: every row of every group counts. Rows behind the last group are zero."""
+    print(dtype, rows, n_in, n_out, groups, flush=True)
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    ends = torch.randint(0, rows - 10, (groups,), generator=g, device="cuda").sort()[0]
+    of = torch.searchsorted(ends, torch.arange(rows, device="cuda"), right=True)  # the first group that ends behind the row
+    ours = of < groups
+    of = of[ours]
+    x, w, dy, b = whole(rows, n_in, seed=1, dtype=dtype, most=1), whole(groups, n_out, n_in, seed=2, dtype=dtype, most=1), whole(rows, n_out, seed=3, dtype=dtype), whole(groups, n_out, seed=4, dtype=dtype)
+    y, _ = tb.grouped_linear_fwd(x, w, ends, b)
+    z = torch.cat([(x[i].double()[:, None] * w[o].double()).sum(-1) + b[o].double() for i, o in zip(torch.arange(rows, device="cuda")[ours].split(5000), of.split(5000))])
+    assert torch.equal(y[ours], z.to(dtype)) and not y[~ours].any()
+    dx, dw, db = tb.grouped_linear_bwd(dy, x, w, ends)
+    d = torch.cat([(dy[i].double()[:, :, None] * w[o].double()).sum(1) for i, o in zip(torch.arange(rows, device="cuda")[ours].split(5000), of.split(5000))])
+    assert torch.equal(dx[ours], d.to(dtype)) and not dx[~ours].any()
+    want = torch.zeros(groups, n_out, n_in, device="cuda")
+    for i, o in zip(torch.arange(rows, device="cuda")[ours].split(5000), of.split(5000)):
+        want.index_add_(0, o, dy[i].float()[:, :, None] * x[i].float()[:, None])
+    assert torch.equal(dw, want.to(dtype))
+    assert torch.equal(db, torch.zeros(groups, n_out, device="cuda").index_add_(0, of, dy[ours].float()).to(dtype))
