@@ -1627,7 +1627,7 @@ void forward(const LinearFwdArgs& f, Run& run) {
     if constexpr (sizeof(T) == 4)
         if (const Long p = plan_long(f.rows, f.in, f.out, f.groups, ragged); p.blocks) {
             const NarrowArgs a{f.x, f.weight, f.bias, f.x_stride, to, f.in, f.out, p.chunk, groups};
-            const auto go = [&](auto kernel) { kernel<<<static_cast<uint32_t>(p.blocks), 512, p.lds, run.stream>>>(a, p.lines); };
+            const auto go = [&](auto kernel) { kernel<<<static_cast<uint32_t>(p.blocks), p.threads, p.lds, run.stream>>>(a, p.lines); };
             if (run.real) p.tiles == 1 ? go(k_long_fwd<T, 1>) : go(k_long_fwd<T, 2>);
             return;
         }

@@ -204,21 +204,25 @@ Narrow plan_narrow(int64_t rows, int64_t in, int64_t out, bool ragged, int elem)
     return p;
 }
 // A layer of floats with longer rows than those (`lines` of 128 bytes, the last may end early) and up to two tiles of 32 outputs, whose
-// weight a workgroup of eight waves holds: or none. Each workgroup fetches the weight, and again for each group: it pays for many
-// rows, a thousand of each group. (us so and by tiles: 158,303 rows of 178 to 2 43 and 138, 1 M of 192 to 64 301 and 570, 32,768 24.8
+// weight a workgroup holds: or none. Each workgroup fetches the weight, and again for each group: it pays for many
+// rows, a thousand of each group. (us so and by tiles: 158,303 rows of 178 to 2 43 and 138, 1 M of 192 to 64 301 and 570, 32,768 23
 // and 24.8, 16,384 24 and 13; 300,000 in 200 groups of 200 to 32 119 and 192, 100,000 of 300 to 64 155 and 112.)
 struct Long {
-    int lines, tiles, lds;
+    int lines, tiles, threads, lds;
     int64_t blocks, chunk;
 };
 Long plan_long(int64_t rows, int64_t in, int64_t out, int groups, bool ragged) {
     Long p{};
-    const int64_t lines = up(in, 32), tiles = up(out, 32), lds = tiles * (lines * 4096 + 128) + 8 * unit_bytes(4);
+    const int64_t lines = up(in, 32), tiles = up(out, 32), weight = tiles * (lines * 4096 + 128);
+    // (four waves where eight would leave units a workgroup or two of all, and two of four fit: 66,580 rows of 288 to 16 36 us and 45; one
+    // of four of 49,152 rows of 900 to 32 78 and 57)
+    p.threads = rows < 256 * 512 && 2 * (weight + 4 * unit_bytes(4)) <= kLds ? 256 : 512;
+    const int64_t lds = weight + p.threads / 64 * unit_bytes(4);
     if (narrow_steps(in, 4) || tiles > 2 || lds > kLds || rows < 32768 || rows / groups < 1024) return p;
     p.lines = static_cast<int>(lines);
     p.tiles = static_cast<int>(tiles);
     p.lds = static_cast<int>(lds);
-    p.blocks = std::min<int64_t>(256 * (ragged ? 8 : std::min(2, kLds / p.lds)), up(rows, 256));
+    p.blocks = std::min<int64_t>(256 * (ragged ? 8 : std::min(p.threads == 512 ? 2 : 4, kLds / p.lds)), up(rows, p.threads / 2));
     p.chunk = up(up(rows, p.blocks), 32) * 32;
     p.blocks = up(rows, p.chunk);
     return p;

@@ -37,10 +37,10 @@ void long_rows() {
                     const Long p = plan_long(rows, in, out, ragged ? 3 : 1, ragged);
                     if (!p.blocks) continue;
                     looked++;
-                    // the weight's fragments, the bias, eight waves' lines and outputs
-                    const long lds = p.tiles * (p.lines * 4096L + 128) + 8 * unit_bytes(4);
+                    // the weight's fragments, the bias, each wave's lines and outputs
+                    const long lds = p.tiles * (p.lines * 4096L + 128) + p.threads / 64 * unit_bytes(4);
                     if (p.lds != lds || lds > kMostLds || p.lines * 32 < in || (p.lines - 1) * 32 >= in || p.tiles * 32 < out || p.tiles > 2 || in < 4 ||
-                        p.blocks > 65535 || p.chunk < 32 || p.chunk % 32 || (ragged ? p.blocks * p.chunk < rows : (p.blocks - 1) * 256 >= rows))
+                        p.blocks > 65535 || p.chunk < 32 || p.chunk % 32 || (ragged ? p.blocks * p.chunk < rows : (p.blocks - 1) * (p.threads / 2) >= rows))
                         std::printf("long %ld rows, %d to %d, ragged %d: lds %d\n", rows, in, out, ragged, p.lds);
                 }
 }
