@@ -372,8 +372,8 @@ __device__ inline void store_unit(const Finish& a, int64_t r, int64_t stop, int6
 // BR x BC outputs a workgroup, WR x WC a wave. OverRows: the sums go over a group's rows (dW), else the outputs' rows are the
 // groups' rows. Bound by the matrix cores, and of long sums by the power they take (1.6 GHz, 64 % of the cycles a product on its
 // way): 16,383 rows, 8192 to 2048 half with a residual 505 us, 1.09 PFLOP/s (the library's bare product 457); of 2048 to 4096 dx
-// 294 us and dweight 284 (the library 272 and 330); 20,001 rows in 16 groups, 1024 to 1408, bfloat16 90 us. Floats of 4096 cubed
-// 998 us, 138 TFLOP/s (the library 910).
+// 290 us and dweight 291 (the library 272 and 330); 20,001 rows in 16 groups, 1024 to 1408, bfloat16 90 us. Floats of 4096 cubed
+// 978 us, 140 TFLOP/s (the library 910).
 // Staged: the operands lie anywhere and go through registers.
 template <class T, int BR, int BC, int WR, int WC, bool RowAcross, bool ColAcross, bool Staged>
 __global__ void __launch_bounds__(BR / WR * (BC / WC) * 64) k_tile(TileArgs a) {
